@@ -940,11 +940,11 @@ static int host_chunk_plan(int64_t T, int64_t chunk, int64_t* sizes, int max_n) 
   if (T <= 0) return 0;
   const int64_t c = chunk < 1 ? 1 : chunk;
   auto put = [&](int64_t v) { if (n < max_n) sizes[n] = v; ++n; };
-  if (T <= 2 * c) {
+  const int64_t edge = c / 2 > 128 ? c / 2 : 128;
+  if (T <= 2 * c || T < 2 * edge) {                // the second: small chunks, whose two edges would be more than there is
     for (int64_t t0 = 0; t0 < T; t0 += c) put(T - t0 < c ? T - t0 : c);
     return n;
   }
-  const int64_t edge = c / 2 > 128 ? c / 2 : 128;
   int64_t rest = T - 2 * edge;
   const int64_t mid = c + c / 2;
   const int64_t n_mid = (rest + mid - 1) / mid > 1 ? (rest + mid - 1) / mid : 1;
