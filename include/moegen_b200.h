@@ -48,6 +48,9 @@ extern "C" {
 /* expert weight formats */
 #define MG_WEIGHT_BF16          0
 #define MG_WEIGHT_FP8_BLOCK128  1  /* e4m3 + fp32 scale per 128x128 block (Wrapper.py:109-138) */
+#define MG_WEIGHT_INT8_CHANNEL  2  /* int8 + fp32 scale per output channel; the rows they multiply are quantised to int8 with a
+                                      scale per token (mg_quantize_rows_int8).  Single GPU (ep_size 1).  No counterpart in the
+                                      reference */
 
 /* error codes (negative: host-side argument/state errors) */
 #define MG_OK                 0
@@ -65,7 +68,7 @@ extern "C" {
 #define MG_DEV_CAPACITY       2  /* expert-parallel receive buffer too small; detail = rank */
 #define MG_DEV_BOUNDS         3  /* checked build (-DMG_BOUNDS_CHECK) only: a row index read from a table lay outside
                                     its buffer; the access was skipped; detail = 103 scatter, 104 combine,
-                                    105 duplicate fill, 106 pushed return */
+                                    105 duplicate fill, 106 pushed return, 107 gradient of the combine */
 
 /* stages of mg_moe_forward, in launch order (mg_stage_times) */
 #define MG_STAGE_GATE_LOGITS   0
@@ -152,7 +155,8 @@ int mg_padded_rows(mg_handle h, int64_t n_rows, int64_t* padded);
  * or -1 for the shared expert ([I_s,H],[I_s,H],[H,I_s]).  For
  * MG_WEIGHT_FP8_BLOCK128 the matrices are e4m3 bytes and d_*_scale are the fp32
  * [ceil(rows/128), ceil(cols/128)] weight_scale_inv tensors; for MG_WEIGHT_BF16
- * the scale pointers are ignored.  The shared expert is always bf16.
+ * the scale pointers are ignored.  For MG_WEIGHT_INT8_CHANNEL the matrices, the shared expert's too, are int8 and
+ * d_*_scale the fp32 scales of their rows ([I], [I] and [H]).  In the other formats the shared expert is bf16.
  * Replaces HtoD copy into a slot + Expert_Wrapper's per-call parameter binding
  * (moe_gen/models/Wrapper.py:470-491). */
 int mg_pack_expert(mg_handle h, int32_t local_expert,
@@ -278,7 +282,8 @@ int mg_shared_ffn(mg_handle h, const void* d_x, int64_t n_tokens, const void* d_
                   void* d_hs_buf, void* d_shared_out, void* stream);
 
 /* y[t] = sum_j topk_w[t,j] * out_rows[dst_row[t*k+j]]  (+ shared_out[t] when
- * d_shared_out != NULL), arithmetic per combine_mode.  Picks with dst_row < 0
+ * d_shared_out != NULL), arithmetic per combine_mode; the sum is rounded to bf16 before shared_out is added, except in
+ * MG_WEIGHT_INT8_CHANNEL layers.  Picks with dst_row < 0
  * contribute nothing.  Replaces new_x[idxs] = outs and the weighted sum
  * (modeling_deepseek_v3.py:702-711) and y + shared (…:624-625). */
 int mg_combine(mg_handle h, const void* d_out_rows, const int32_t* d_dst_row,
@@ -321,6 +326,73 @@ int mg_moe_forward_host(mg_handle h, const void* x_host, int64_t n_tokens, const
 int mg_moe_forward_from_logits(mg_handle h, const void* d_x, int64_t n_tokens, const float* d_logits,
                                const float* d_bias, const void* d_packed, void* d_workspace,
                                size_t workspace_bytes, void* d_y, void* stream);
+
+/* ---- 8-bit integers ------------------------------------------------------------ */
+/* No counterpart in the reference, whose 8-bit checkpoints are FP8 and multiplied in bf16
+ * (moe_gen/models/Wrapper.py:109-138).  A row x of bf16 is held as bytes q in [-127, 127] and one fp32 scale:
+ *   m = max(max|x|, 2^-100), scale = m / 127, q = x * (127 / m) rounded to the nearest integer, ties to even
+ * (both quotients in fp32, the product exact).  A row with an infinity or a NaN in it has scale NaN and bytes 0, so that
+ * what is made of it is NaN.  Weights w are int8 with one fp32 scale per row (output channel).  A product is
+ *   y[t, n] = bf16(float(sum_k q[t, k] w[n, k]) * scale[t] * w_scale[n]),
+ * its sum exact in 32 bits, so cols <= 131071.  Results do not depend on the batch a row is in.
+ *
+ * mg_quantize_rows_int8: rows of any length; ldx in elements, ldq in bytes.  Rows whose addresses and lengths are multiples
+ *   of 8 elements are read in 16-byte vectors.
+ * mg_int8_matmul: x_q [n_rows, cols] and w_q [n_out, cols] with rows on 16-byte boundaries (ldx, ldw bytes apart), d_out
+ *   [n_rows, n_out] bf16 with rows ldo elements apart, ldo a multiple of 8; any sizes otherwise.
+ * mg_int8_linear: both in one call, for bf16 rows; d_ws is scratch of mg_int8_linear_ws_bytes bytes on a 16-byte boundary.
+ * The handle may be any layer's: it gives the device, its status word and its cache of tensor maps. */
+int mg_quantize_rows_int8(mg_handle h, const void* d_x, int64_t n_rows, int64_t cols, int64_t ldx, void* d_q, int64_t ldq,
+                          float* d_scale, void* stream);
+int mg_int8_matmul(mg_handle h, const void* d_xq, int64_t ldx, const float* d_x_scale, int64_t n_rows, const void* d_wq,
+                   int64_t ldw, const float* d_w_scale, int64_t n_out, int64_t cols, void* d_out, int64_t ldo, void* stream);
+int mg_int8_linear_ws_bytes(int64_t n_rows, int64_t cols, size_t* bytes);
+int mg_int8_linear(mg_handle h, const void* d_x, int64_t ldx, int64_t n_rows, const void* d_wq, int64_t ldw,
+                   const float* d_w_scale, int64_t n_out, int64_t cols, void* d_ws, size_t ws_bytes, void* d_out, int64_t ldo,
+                   void* stream);
+
+/* The stages of an MG_WEIGHT_INT8_CHANNEL layer; mg_moe_forward and its host, block and from-logits forms run them.
+ *   mg_permute_rows_int8   mg_permute_rows for quantised rows [T,H] (contiguous) and their scales [T]
+ *   mg_expert_ffn_int8     mg_expert_ffn on such expert-sorted rows: h_buf[r] = silu(g) * u in bf16, quantised into
+ *                          h_q [rows, I] and h_scale [rows] for the rows that d_dst_row [T, k] names, out_rows = the down
+ *                          product in bf16
+ *   mg_shared_ffn_int8     mg_shared_ffn on the quantised tokens; hs_buf [T, I_s] bf16, hs_q [T, I_s] and hs_scale [T] scratch
+ * mg_expert_ffn and mg_shared_ffn refuse such a layer. */
+int mg_permute_rows_int8(mg_handle h, const void* d_xq, const float* d_x_scale, const int32_t* d_dst_row, int64_t n_tokens,
+                         void* d_perm_q, float* d_perm_scale, void* stream);
+int mg_expert_ffn_int8(mg_handle h, const void* d_perm_q, const float* d_perm_scale, const int32_t* d_pad_offsets,
+                       const int32_t* d_counts, int64_t n_rows_padded, const int32_t* d_dst_row, int64_t n_tokens,
+                       const void* d_packed, void* d_h_buf, void* d_h_q, float* d_h_scale, void* d_out_rows, void* stream);
+int mg_shared_ffn_int8(mg_handle h, const void* d_xq, const float* d_x_scale, int64_t n_tokens, const void* d_packed,
+                       void* d_hs_buf, void* d_hs_q, float* d_hs_scale, void* d_out, void* stream);
+
+/* ---- gradients around the experts ------------------------------------------------ */
+/* For what is trained around experts that stay as they are (a router calibrated behind their quantisation, adapters on the
+ * sorted rows).  No counterpart in the reference, which has no training path.  dst_row, counts and pad_offsets are those of
+ * mg_permute_plan over n_plan_experts experts, with the experts a token names distinct, as every routing here gives them; entries
+ * of dst_row that are negative, or not below n_rows_padded where that is given, are left out.
+ *
+ * mg_permute_rows_padded: mg_permute_rows with zeros in the rows of perm_x [n_rows_padded, H] that hold no pick: behind an
+ *   expert's rows and behind the last segment.
+ * mg_permute_rows_grad: grad_x[t] = sum_j grad_rows[dst_row[t, j]], summed in fp32 in the order of the slots, rounded once.
+ * mg_combine_grad: the gradients of mg_combine's sum, for grad_y [T, H] bf16 and the weights topk_w [T, k] (rounded to bf16
+ *   first in the bf16 combine modes; the modes' other roundings count as the identity):
+ *     grad_rows[dst_row[t, j]] = bf16(w[t, j] * grad_y[t]),  grad_w[t, j] = sum_h grad_y[t, h] * out_rows[dst_row[t, j], h]
+ *   in fp32, always in the same order for the same T.  Either output may be NULL; d_out_rows is read for grad_w alone.  With
+ *   counts and pad_offsets (else NULL and left as they were) rows of grad_rows that hold no pick are written as zeros.  grad_w
+ *   of a pick that is left out is 0.  The gradient of mg_combine's shared_out is grad_y itself.
+ * mg_route_topk_grad: the gradient of mg_route_topk's weights with respect to the logits, the picks being constants:
+ *   grad_logits[T, E], zero (sigmoid) or the softmax's share for experts not picked.  topk_idx and topk_w are that call's; a
+ *   pick whose weight is 0 competed from a group that was not kept, and passes nothing on. */
+int mg_permute_rows_padded(mg_handle h, const void* d_x, const int32_t* d_dst_row, int64_t n_tokens, const int32_t* d_counts,
+                           const int32_t* d_pad_offsets, int32_t n_plan_experts, int64_t n_rows_padded, void* d_perm_x, void* stream);
+int mg_permute_rows_grad(mg_handle h, const void* d_grad_rows, const int32_t* d_dst_row, int64_t n_tokens, void* d_grad_x,
+                         void* stream);
+int mg_combine_grad(mg_handle h, const void* d_grad_y, const void* d_out_rows, const int32_t* d_dst_row, const float* d_topk_w,
+                    int64_t n_tokens, const int32_t* d_counts, const int32_t* d_pad_offsets, int32_t n_plan_experts,
+                    int64_t n_rows_padded, void* d_grad_rows, float* d_grad_w, void* stream);
+int mg_route_topk_grad(mg_handle h, const float* d_logits, const int32_t* d_topk_idx, const float* d_topk_w, const float* d_grad_w,
+                       int64_t n_tokens, float* d_grad_logits, void* stream);
 
 /* ---- expert parallelism (ep_size > 1): one process per GPU ------------------- */
 /* The reference's expert-parallel branch (modeling_deepseek_v3.py:636-672,692-700) exchanges

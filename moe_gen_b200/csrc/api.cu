@@ -49,7 +49,8 @@ static int64_t padded_rows(const Handle* h, int64_t rows) {
 
 // workspace carving ---------------------------------------------------------------------
 enum { WS_LOGITS, WS_IDX, WS_W, WS_COUNTS, WS_OFFSETS, WS_PAD, WS_DST, WS_PERM, WS_H, WS_OUT, WS_PLAN,
-       WS_HS, WS_SHARED, WS_DEQ, WS_FIX, WS_JOBS, WS_N };
+       WS_HS, WS_SHARED, WS_DEQ, WS_FIX, WS_JOBS,
+       WS_XQ, WS_XS, WS_PERM_S, WS_HQ, WS_H_S, WS_SHQ, WS_SH_S, WS_N };       // int8 layers: quantised rows and their scales
 struct WsLayout { size_t off[WS_N]; size_t total; };
 
 static size_t dequant_ws(const Handle* h) {
@@ -124,7 +125,8 @@ static WsLayout ws_layout(const Handle* h, int64_t T, int64_t R) {
   take(WS_OFFSETS, static_cast<size_t>(d.n_experts + 1) * 4);
   take(WS_PAD, static_cast<size_t>(d.n_experts + 1) * 4);
   take(WS_DST, static_cast<size_t>(T) * d.top_k * 4);
-  take(WS_PERM, Rp * d.hidden * 2);
+  const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
+  take(WS_PERM, Rp * d.hidden * (i8 ? 1 : 2));
   take(WS_H, Rp * d.inter * 2);
   take(WS_OUT, Rp * d.hidden * 2);
   take(WS_PLAN, plan_ws_bytes(h, T));
@@ -132,6 +134,14 @@ static WsLayout ws_layout(const Handle* h, int64_t T, int64_t R) {
   take(WS_SHARED, d.inter_shared ? static_cast<size_t>(T) * d.hidden * 2 : 0);
   take(WS_FIX, route_fix_bytes(T));
   take(WS_JOBS, kJobCounters * sizeof(int32_t));
+  const size_t t8 = i8 ? static_cast<size_t>(T) : 0, r8 = i8 ? Rp : 0;
+  take(WS_XQ, t8 * d.hidden);
+  take(WS_XS, t8 * 4);
+  take(WS_PERM_S, r8 * 4);
+  take(WS_HQ, r8 * d.inter);
+  take(WS_H_S, r8 * 4);
+  take(WS_SHQ, t8 * d.inter_shared);
+  take(WS_SH_S, t8 * 4);
   L.total = off;
   return L;
 }
@@ -160,8 +170,14 @@ int mg_create(const mg_layer_desc* desc, mg_handle* out) {
              "top_k=%d must be in [1,min(%d,n_experts)]", d.top_k, kMaxTopK);
   MG_REQUIRE(d.gating >= 0 && d.gating <= 3, MG_ERR_CONFIG, "unknown gating mode %d", d.gating);
   MG_REQUIRE(d.combine_mode >= 0 && d.combine_mode <= 2, MG_ERR_CONFIG, "unknown combine mode %d", d.combine_mode);
-  MG_REQUIRE(d.weight_format == MG_WEIGHT_BF16 || d.weight_format == MG_WEIGHT_FP8_BLOCK128, MG_ERR_CONFIG,
-             "unknown weight format %d", d.weight_format);
+  MG_REQUIRE(d.weight_format == MG_WEIGHT_BF16 || d.weight_format == MG_WEIGHT_FP8_BLOCK128 ||
+             d.weight_format == MG_WEIGHT_INT8_CHANNEL, MG_ERR_CONFIG, "unknown weight format %d", d.weight_format);
+  if (d.weight_format == MG_WEIGHT_INT8_CHANNEL) {
+    MG_REQUIRE(d.ep_size == 1, MG_ERR_CONFIG, "int8 layers are single-GPU (ep_size=%d)", d.ep_size);
+    MG_REQUIRE(d.hidden <= kInt8MaxK && d.inter <= kInt8MaxK && d.inter_shared <= kInt8MaxK, MG_ERR_LIMIT,
+               "int8 layer: hidden=%d, inter=%d and inter_shared=%d must be <= %d (sums in 32 bits)", d.hidden, d.inter,
+               d.inter_shared, kInt8MaxK);
+  }
   if (d.gating == MG_GATE_SOFTMAX_GROUP_MAX || d.gating == MG_GATE_SIGMOID_NOAUX_TC) {
     MG_REQUIRE(d.n_group >= 1 && d.n_group <= 32 && d.n_experts % d.n_group == 0, MG_ERR_CONFIG,
                "n_group=%d must divide n_experts and be <= 32", d.n_group);
@@ -564,6 +580,7 @@ static int expert_ffn(Handle* h, const void* perm_x, const int32_t* pad, const i
     if (rc0 != MG_OK) return rc0;
   }
   const mg_layer_desc& d = h->d;
+  MG_REQUIRE(d.weight_format != MG_WEIGHT_INT8_CHANNEL, MG_ERR_CONFIG, "int8 layer: its experts take quantised rows (mg_expert_ffn_int8)");
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
   const bool fp8 = d.weight_format == MG_WEIGHT_FP8_BLOCK128;
@@ -735,6 +752,7 @@ static int shared_ffn(Handle* h, const void* x, int64_t T, const void* packed, v
                       bool timed = false) {
   const mg_layer_desc& d = h->d;
   MG_REQUIRE(d.inter_shared > 0, MG_ERR_CONFIG, "layer has no shared expert");
+  MG_REQUIRE(d.weight_format != MG_WEIGHT_INT8_CHANNEL, MG_ERR_CONFIG, "int8 layer: its shared expert takes quantised rows (mg_shared_ffn_int8)");
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
   GemmProblem p{};
@@ -746,6 +764,228 @@ static int shared_ffn(Handle* h, const void* x, int64_t T, const void* packed, v
   p.a = hs; p.b = base + L.sh2; p.n_per_group = d.hidden; p.K = d.inter_shared; p.out = out; p.ldo = d.hidden;
   p.epilogue = EPI_PLAIN_BF16;
   return launch_grouped_gemm(h, p, st);
+}
+
+// The experts of an int8 layer over expert-sorted quantised rows.  dst_row lists the live rows: the rows between the products
+// are quantised for them alone.
+static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, const int32_t* pad, const int32_t* counts,
+                           int64_t rows_padded, const int32_t* dst_row, int64_t T, const void* packed, void* h_buf, void* h_q,
+                           float* h_s, void* out_rows, cudaStream_t st, int* launches, bool timed, int32_t* job_counters,
+                           bool chain_down) {
+  const mg_layer_desc& d = h->d;
+  const PackedLayout L = packed_layout(h);
+  const uint8_t* base = static_cast<const uint8_t*>(packed);
+  GemmProblem p{};
+  p.a_rows = rows_padded; p.b_i8 = true; p.n_groups = h->e_local; p.pad_offsets = pad; p.counts = counts;
+  if (timed) mark(h, MG_STAGE_DEQUANT, st);
+  p.a = perm_q; p.lda = d.hidden; p.a_scales = perm_s; p.b = base + L.w13; p.ldb = d.hidden;
+  p.scales = reinterpret_cast<const float*>(base + L.s13); p.n_per_group = 2 * d.inter; p.K = d.hidden;
+  p.out = h_buf; p.ldo = d.inter; p.epilogue = EPI_SWIGLU_BF16; p.next_job = job_counters;
+  int rc = launch_grouped_gemm(h, p, st);
+  if (rc != MG_OK) return rc;
+  if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
+  rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, dst_row, h_q, d.inter, h_s, st);
+  if (rc != MG_OK) return rc;
+  if (!chain_down) h->chain = false;
+  p.a = h_q; p.lda = d.inter; p.a_scales = h_s; p.b = base + L.w2; p.ldb = d.inter;
+  p.scales = reinterpret_cast<const float*>(base + L.s2); p.n_per_group = d.hidden; p.K = d.inter;
+  p.out = out_rows; p.ldo = d.hidden; p.epilogue = EPI_PLAIN_BF16;
+  p.next_job = job_counters != nullptr ? job_counters + 1 : nullptr;
+  rc = launch_grouped_gemm(h, p, st);
+  if (rc != MG_OK) return rc;
+  if (timed) mark(h, MG_STAGE_EXPERT_GEMM2, st);
+  if (launches) *launches += 3;
+  return MG_OK;
+}
+
+static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T, const void* packed, void* hs, void* hs_q,
+                           float* hs_s, void* out, cudaStream_t st, bool timed = false) {
+  const mg_layer_desc& d = h->d;
+  const PackedLayout L = packed_layout(h);
+  const uint8_t* base = static_cast<const uint8_t*>(packed);
+  int rc = launch_int8_matmul(h, xq, d.hidden, xs, T, base + L.sh13, d.hidden, reinterpret_cast<const float*>(base + L.shs13),
+                              2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st);
+  if (rc != MG_OK) return rc;
+  if (timed) mark(h, MG_STAGE_SHARED_GEMM1, st);
+  rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, nullptr, hs_q, d.inter_shared, hs_s, st);
+  if (rc != MG_OK) return rc;
+  return launch_int8_matmul(h, hs_q, d.inter_shared, hs_s, T, base + L.sh2, d.inter_shared,
+                            reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st);
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int mg_quantize_rows_int8(mg_handle hh, const void* d_x, int64_t n_rows, int64_t cols, int64_t ldx, void* d_q, int64_t ldq,
+                          float* d_scale, void* stream) {
+  MG_TRACE("mg_quantize_rows_int8", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(n_rows >= 0 && cols >= 1 && ldx >= cols && ldq >= cols, MG_ERR_SHAPE, "mg_quantize_rows_int8: %lld rows of %lld, strides %lld and %lld",
+             static_cast<long long>(n_rows), static_cast<long long>(cols), static_cast<long long>(ldx), static_cast<long long>(ldq));
+  MG_REQUIRE(cols <= kInt8MaxK, MG_ERR_LIMIT, "mg_quantize_rows_int8: rows of %lld, at most %d", static_cast<long long>(cols), kInt8MaxK);
+  if (n_rows == 0) return MG_OK;
+  MG_REQUIRE(d_x && d_q && d_scale, MG_ERR_NULL, "mg_quantize_rows_int8: null pointer");
+  return launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_q, ldq, d_scale, static_cast<cudaStream_t>(stream));
+}
+
+static int check_int8_product(int64_t n_rows, int64_t n_out, int64_t cols, const void* d_w, int64_t ldw, const float* d_ws,
+                              const void* d_out, int64_t ldo) {
+  MG_REQUIRE(n_rows >= 0 && n_out >= 1 && cols >= 1, MG_ERR_SHAPE, "int8 product: %lld rows, %lld outputs, %lld inputs",
+             static_cast<long long>(n_rows), static_cast<long long>(n_out), static_cast<long long>(cols));
+  MG_REQUIRE(cols <= kInt8MaxK, MG_ERR_LIMIT, "int8 product: %lld inputs, sums in 32 bits hold %d", static_cast<long long>(cols), kInt8MaxK);
+  MG_REQUIRE(n_rows < (1ll << 31) - 512 && n_out < (1ll << 31) - 512 && n_out * ((n_rows + 31) / 32) < (1ll << 38), MG_ERR_LIMIT,
+             "int8 product: %lld rows by %lld outputs", static_cast<long long>(n_rows), static_cast<long long>(n_out));
+  MG_REQUIRE(ldw >= cols && ldw % 16 == 0 && ldo >= n_out && ldo % 8 == 0, MG_ERR_SHAPE,
+             "int8 product: weight rows of %lld bytes (a multiple of 16 needed), output rows of %lld elements (a multiple of 8 needed)",
+             static_cast<long long>(ldw), static_cast<long long>(ldo));
+  if (n_rows == 0) return MG_OK;
+  MG_REQUIRE(d_w && d_ws && d_out, MG_ERR_NULL, "int8 product: null pointer");
+  MG_REQUIRE(aligned16(d_w) && aligned16(d_out), MG_ERR_SHAPE, "int8 product: weights and output must begin on a 16-byte boundary");
+  return MG_OK;
+}
+
+int mg_int8_matmul(mg_handle hh, const void* d_xq, int64_t ldx, const float* d_x_scale, int64_t n_rows, const void* d_wq, int64_t ldw,
+                   const float* d_w_scale, int64_t n_out, int64_t cols, void* d_out, int64_t ldo, void* stream) {
+  MG_TRACE("mg_int8_matmul", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_int8_product(n_rows, n_out, cols, d_wq, ldw, d_w_scale, d_out, ldo);
+  if (rc != MG_OK || n_rows == 0) return rc;
+  MG_REQUIRE(d_xq && d_x_scale, MG_ERR_NULL, "mg_int8_matmul: null pointer");
+  MG_REQUIRE(ldx >= cols && ldx % 16 == 0 && aligned16(d_xq), MG_ERR_SHAPE, "mg_int8_matmul: rows of x (%lld bytes) must begin on 16-byte boundaries",
+             static_cast<long long>(ldx));
+  return launch_int8_matmul(h, d_xq, ldx, d_x_scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16,
+                            static_cast<cudaStream_t>(stream));
+}
+
+// scratch of mg_int8_linear: quantised rows on 128-byte strides, then their scales
+static size_t int8_linear_rows_bytes(int64_t n_rows, int64_t cols) {
+  return static_cast<size_t>(round_up(n_rows * round_up(cols, 128), 256));
+}
+int mg_int8_linear_ws_bytes(int64_t n_rows, int64_t cols, size_t* bytes) {
+  MG_REQUIRE(bytes, MG_ERR_NULL, "null argument");
+  MG_REQUIRE(n_rows >= 0 && cols >= 1, MG_ERR_SHAPE, "mg_int8_linear_ws_bytes: bad size");
+  MG_REQUIRE(cols <= kInt8MaxK && n_rows < (1ll << 31), MG_ERR_LIMIT, "mg_int8_linear_ws_bytes: %lld rows of %lld",
+             static_cast<long long>(n_rows), static_cast<long long>(cols));
+  *bytes = int8_linear_rows_bytes(n_rows, cols) + static_cast<size_t>(round_up(4 * n_rows, 256));
+  return MG_OK;
+}
+
+int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, const void* d_wq, int64_t ldw, const float* d_w_scale,
+                   int64_t n_out, int64_t cols, void* d_ws, size_t ws_bytes, void* d_out, int64_t ldo, void* stream) {
+  MG_TRACE("mg_int8_linear", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_int8_product(n_rows, n_out, cols, d_wq, ldw, d_w_scale, d_out, ldo);
+  if (rc != MG_OK || n_rows == 0) return rc;
+  MG_REQUIRE(ldx >= cols, MG_ERR_SHAPE, "mg_int8_linear: rows of x are %lld elements apart", static_cast<long long>(ldx));
+  size_t need = 0;
+  rc = mg_int8_linear_ws_bytes(n_rows, cols, &need);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(d_x && d_ws, MG_ERR_NULL, "mg_int8_linear: null pointer");
+  MG_REQUIRE(ws_bytes >= need && aligned16(d_ws), MG_ERR_WORKSPACE, "mg_int8_linear: scratch of %zu bytes < %zu needed, or not on a 16-byte boundary",
+             ws_bytes, need);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t ldq = round_up(cols, 128);
+  float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
+  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_ws, ldq, scale, st);
+  if (rc != MG_OK) return rc;
+  h->chain = true;
+  rc = launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
+  h->chain = false;
+  return rc;
+}
+
+int mg_permute_rows_int8(mg_handle hh, const void* d_q, const float* d_scale, const int32_t* d_dst, int64_t T, void* d_perm_q,
+                         float* d_perm_scale, void* stream) {
+  MG_TRACE("mg_permute_rows_int8", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
+  MG_REQUIRE(d_q && d_scale && d_dst && d_perm_q && d_perm_scale, MG_ERR_NULL, "mg_permute_rows_int8: null pointer");
+  return launch_permute_rows(h, d_q, d_dst, T, d_perm_q, static_cast<cudaStream_t>(stream), d_scale, d_perm_scale);
+}
+
+int mg_expert_ffn_int8(mg_handle hh, const void* d_perm_q, const float* d_perm_scale, const int32_t* d_pad, const int32_t* d_counts,
+                       int64_t n_rows_padded, const int32_t* d_dst, int64_t T, const void* d_packed, void* d_h_buf, void* d_h_q,
+                       float* d_h_scale, void* d_out_rows, void* stream) {
+  MG_TRACE("mg_expert_ffn_int8", n_rows_padded);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(h->d.weight_format == MG_WEIGHT_INT8_CHANNEL, MG_ERR_CONFIG, "mg_expert_ffn_int8: the layer's experts are not int8");
+  MG_REQUIRE(T >= 0 && n_rows_padded >= 0 && n_rows_padded % kTileM == 0, MG_ERR_SHAPE,
+             "n_rows_padded=%lld must be a multiple of %d", static_cast<long long>(n_rows_padded), kTileM);
+  if (T == 0 || n_rows_padded == 0) return MG_OK;
+  MG_REQUIRE(d_perm_q && d_perm_scale && d_pad && d_counts && d_dst && d_packed && d_h_buf && d_h_q && d_h_scale && d_out_rows,
+             MG_ERR_NULL, "mg_expert_ffn_int8: null pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc = zero_job_counters(h, st);
+  if (rc != MG_OK) return rc;
+  return expert_ffn_int8(h, d_perm_q, d_perm_scale, d_pad, d_counts, n_rows_padded, d_dst, T, d_packed, d_h_buf, d_h_q, d_h_scale,
+                         d_out_rows, st, nullptr, false, h->job_counters, true);
+}
+
+int mg_shared_ffn_int8(mg_handle hh, const void* d_xq, const float* d_x_scale, int64_t T, const void* d_packed, void* d_hs,
+                       void* d_hs_q, float* d_hs_scale, void* d_out, void* stream) {
+  MG_TRACE("mg_shared_ffn_int8", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(h->d.weight_format == MG_WEIGHT_INT8_CHANNEL && h->d.inter_shared > 0, MG_ERR_CONFIG,
+             "mg_shared_ffn_int8: the layer has no int8 shared expert");
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
+  MG_REQUIRE(d_xq && d_x_scale && d_packed && d_hs && d_hs_q && d_hs_scale && d_out, MG_ERR_NULL, "mg_shared_ffn_int8: null pointer");
+  return shared_ffn_int8(h, d_xq, d_x_scale, T, d_packed, d_hs, d_hs_q, d_hs_scale, d_out, static_cast<cudaStream_t>(stream));
+}
+
+// ---- gradients around the experts -------------------------------------------------------------------
+int mg_permute_rows_padded(mg_handle hh, const void* d_x, const int32_t* d_dst, int64_t T, const int32_t* d_counts,
+                           const int32_t* d_pad, int32_t n_plan, int64_t n_rows, void* d_perm, void* stream) {
+  MG_TRACE("mg_permute_rows_padded", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0 && n_rows >= 0 && n_plan >= 1 && n_plan <= h->d.n_experts, MG_ERR_SHAPE,
+             "mg_permute_rows_padded: %lld tokens, %lld rows, %d experts", static_cast<long long>(T), static_cast<long long>(n_rows), n_plan);
+  if (n_rows == 0) return MG_OK;
+  MG_REQUIRE((T == 0 || (d_x && d_dst)) && d_counts && d_pad && d_perm, MG_ERR_NULL, "mg_permute_rows_padded: null pointer");
+  return launch_permute_rows_padded(h, d_x, d_dst, T, d_counts, d_pad, n_plan, n_rows, d_perm, static_cast<cudaStream_t>(stream));
+}
+
+int mg_permute_rows_grad(mg_handle hh, const void* d_grad_rows, const int32_t* d_dst, int64_t T, void* d_grad_x, void* stream) {
+  MG_TRACE("mg_permute_rows_grad", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
+  MG_REQUIRE(d_grad_rows && d_dst && d_grad_x, MG_ERR_NULL, "mg_permute_rows_grad: null pointer");
+  return launch_permute_rows_grad(h, d_grad_rows, d_dst, T, d_grad_x, static_cast<cudaStream_t>(stream));
+}
+
+int mg_combine_grad(mg_handle hh, const void* d_grad_y, const void* d_out_rows, const int32_t* d_dst, const float* d_w, int64_t T,
+                    const int32_t* d_counts, const int32_t* d_pad, int32_t n_plan, int64_t n_rows, void* d_grad_rows, float* d_grad_w,
+                    void* stream) {
+  MG_TRACE("mg_combine_grad", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0 && n_rows >= 0 && (d_counts == nullptr || (n_plan >= 1 && n_plan <= h->d.n_experts)), MG_ERR_SHAPE,
+             "mg_combine_grad: %lld tokens, %lld rows, %d experts", static_cast<long long>(T), static_cast<long long>(n_rows), n_plan);
+  MG_REQUIRE((d_counts == nullptr) == (d_pad == nullptr), MG_ERR_NULL, "mg_combine_grad: counts and pad_offsets come together");
+  MG_REQUIRE(T == 0 || (d_grad_y && d_dst && d_w && (d_out_rows || d_grad_w == nullptr)), MG_ERR_NULL, "mg_combine_grad: null pointer");
+  return launch_combine_grad(h, d_grad_y, d_out_rows, d_dst, d_w, T, d_counts, d_pad, n_plan, n_rows, d_grad_rows, d_grad_w,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int mg_route_topk_grad(mg_handle hh, const float* d_logits, const int32_t* d_idx, const float* d_w, const float* d_grad_w, int64_t T,
+                       float* d_grad_logits, void* stream) {
+  MG_TRACE("mg_route_topk_grad", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
+  MG_REQUIRE(d_logits && d_idx && d_w && d_grad_w && d_grad_logits, MG_ERR_NULL, "mg_route_topk_grad: null pointer");
+  MG_REQUIRE(aligned16(d_logits) && aligned16(d_grad_logits), MG_ERR_SHAPE, "mg_route_topk_grad: logits must begin on a 16-byte boundary");
+  return launch_route_topk_grad(h, d_logits, d_idx, d_w, d_grad_w, T, d_grad_logits, static_cast<cudaStream_t>(stream));
 }
 
 int mg_shared_ffn(mg_handle hh, const void* d_x, int64_t T, const void* d_packed, void* d_hs, void* d_out,
@@ -836,6 +1076,18 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     rc = start_dequant(h, d_packed, deq, st, &launches);
     if (rc != MG_OK) return rc;
   }
+  // int8 experts: the tokens are quantised once, for the scatter and for the shared expert.  Ahead of the chain: the kernel
+  // behind it is launched by an ordinary dependence, so that the scatter may read the quantised rows as older memory.
+  const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
+  uint8_t* xq = ws + L.off[WS_XQ];
+  float* xs = reinterpret_cast<float*>(ws + L.off[WS_XS]);
+  float* perm_s = i8 ? reinterpret_cast<float*>(ws + L.off[WS_PERM_S]) : nullptr;
+  if (i8) {
+    rc = launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, nullptr, xq, d.hidden, xs, st);
+    if (rc != MG_OK) return rc;
+    launches += 1;
+  }
+  const void* rows_in = i8 ? xq : d_x;
   if (d_logits_in != nullptr) {
     logits = const_cast<float*>(d_logits_in);      // only read from here on
   } else {
@@ -854,6 +1106,10 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   // time of their own.
   const bool shared_early = d.inter_shared && (h->opt_shared_early == 1 ||
                                                (h->opt_shared_early == 2 && T <= (h->stage_timing ? 4096 : 16384)));
+  auto run_shared = [&](cudaStream_t on, bool timed) {
+    return i8 ? shared_ffn_int8(h, xq, xs, T, d_packed, hs, ws + L.off[WS_SHQ], reinterpret_cast<float*>(ws + L.off[WS_SH_S]), sh, on, timed)
+              : shared_ffn(h, d_x, T, d_packed, hs, sh, on, timed);
+  };
   if (shared_early) {
     if (!h->side2) {
       MG_CUDA(cudaStreamCreateWithFlags(&h->side2, cudaStreamNonBlocking));
@@ -864,11 +1120,11 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     MG_CUDA(cudaStreamWaitEvent(h->side2, h->ev_shared_in, 0));
     const bool keep = h->chain;
     h->chain = false;
-    rc = shared_ffn(h, d_x, T, d_packed, hs, sh, h->side2, false);
+    rc = run_shared(h->side2, false);
     h->chain = keep;
     if (rc != MG_OK) return rc;
     MG_CUDA(cudaEventRecord(h->ev_shared_out, h->side2));
-    launches += 2;
+    launches += i8 ? 3 : 2;
   }
   if (d_logits_in == nullptr && route_fixup_applies(h)) {
     // logits from the tensor-core product: tokens whose pick its rounding could have changed are re-routed
@@ -884,27 +1140,30 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   mark(h, MG_STAGE_ROUTE_TOPK, st);
   int32_t* jobs = reinterpret_cast<int32_t*>(ws + L.off[WS_JOBS]);
   if (plan_copies(h, T) && !h->stage_timing) {      // while stage times are recorded each has its own
-    rc = launch_plan_and_rows(h, idx, T, counts, offsets, pad, dst, jobs, d_x, perm, st);
+    rc = launch_plan_and_rows(h, idx, T, counts, offsets, pad, dst, jobs, rows_in, perm, i8 ? xs : nullptr, perm_s, st);
   } else {
     rc = launch_permute_plan(h, idx, T, 0, d.n_experts, counts, offsets, pad, dst, plan, st, &launches, jobs);
     if (rc != MG_OK) return rc;
     mark(h, MG_STAGE_PERMUTE_PLAN, st);
-    rc = launch_permute_rows(h, d_x, dst, T, perm, st);
+    rc = launch_permute_rows(h, rows_in, dst, T, perm, st, i8 ? xs : nullptr, perm_s);
   }
   if (rc != MG_OK) return rc;
   mark(h, MG_STAGE_PERMUTE_ROWS, st);
   launches += 1;
-  rc = expert_ffn(h, perm, pad, counts, padded_rows(h, T * d.top_k), d_packed, hbuf, orow, deq, st, &launches, true,
-                  nullptr, reinterpret_cast<int32_t*>(ws + L.off[WS_JOBS]), !(shared_early && T <= kUnchainedDownTokens));
+  const bool chain_down = !(shared_early && T <= kUnchainedDownTokens);
+  rc = i8 ? expert_ffn_int8(h, perm, perm_s, pad, counts, padded_rows(h, T * d.top_k), dst, T, d_packed, hbuf, ws + L.off[WS_HQ],
+                            reinterpret_cast<float*>(ws + L.off[WS_H_S]), orow, st, &launches, true, jobs, chain_down)
+          : expert_ffn(h, perm, pad, counts, padded_rows(h, T * d.top_k), d_packed, hbuf, orow, deq, st, &launches, true,
+                       nullptr, jobs, chain_down);
   if (rc != MG_OK) return rc;
   if (shared_early) {
     MG_CUDA(cudaStreamWaitEvent(st, h->ev_shared_out, 0));
     h->chain = false;
     mark(h, MG_STAGE_SHARED_GEMM1, st);
   } else if (d.inter_shared) {
-    rc = shared_ffn(h, d_x, T, d_packed, hs, sh, st, true);
+    rc = run_shared(st, true);
     if (rc != MG_OK) return rc;
-    launches += 2;
+    launches += i8 ? 3 : 2;
   } else {
     mark(h, MG_STAGE_SHARED_GEMM1, st);
   }

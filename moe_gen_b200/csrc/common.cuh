@@ -17,6 +17,7 @@ constexpr int kMaxPeers = 8;         // ranks of one NVSwitch domain
 constexpr int kPeerShift = 24;       // expert-parallel destinations: rank << 24 | row
 constexpr int kPeerRowMask = (1 << kPeerShift) - 1;
 constexpr int kSkipRow = -(1 << 30); // stays negative after the in-segment rank is added
+constexpr int kInt8MaxK = 131071;    // 2^31 / 2^14: sums of products of bytes stay within 32 bits
 constexpr int kDequantChunks = 8;    // expert chunks of the overlapped FP8 de-quantisation
 constexpr int kJobCounters = MG_JOB_COUNTERS;      // one per expert GEMM launch of a forward
 static_assert(kJobCounters >= 2 * kDequantChunks, "every part of the experts has a counter for either product");
@@ -42,7 +43,7 @@ struct TensorMapCache {
   static constexpr int kEntries = 96;
   struct Entry {
     const void* base;
-    uint64_t rows, cols;
+    uint64_t rows, cols, ld;
     uint32_t box_rows, kind;
     CUtensorMap map;
   };
@@ -54,7 +55,7 @@ struct TensorMapCache {
 // fetches all steps of a stage: with a copy per step and per 64 or 16 tokens the kernel's token role was late at 32 to 128
 // tokens per expert (V3, 4096 skewed tokens 4.89 against 4.77 ms).
 struct WlMaps {
-  CUtensorMap w;                // FP8: weights [blocks of 128 rows][128][K]; bf16: [8][blocks][16][K]
+  CUtensorMap w;                // FP8: weights [blocks of 128 rows][128][K]; bf16, int8 gate/up: [8][blocks][16][K]; int8: [rows][K]
   CUtensorMap t[8];             // 16 .. 128 tokens
   CUtensorMap t8;               // 8 tokens: jobs of up to 32 leave out groups of eight without a live one
   CUtensorMap t2[5];            // 16 .. 80 tokens, one step: the parts of a job of more than 256
@@ -64,12 +65,12 @@ struct WlMapCache {
   static constexpr int kEntries = 24;      // a forward launches 2, with weights de-quantised first 16
   struct Key {
     const void *a, *b, *out;
-    int64_t a_rows, w_rows, ldo;
-    int K;
-    bool fp8, swiglu;
+    int64_t a_rows, w_rows, ldo, lda, ldb;
+    int K, type;
+    bool swiglu;
     bool operator==(const Key& o) const {
-      return a == o.a && b == o.b && out == o.out && a_rows == o.a_rows && w_rows == o.w_rows && ldo == o.ldo && K == o.K &&
-             fp8 == o.fp8 && swiglu == o.swiglu;
+      return a == o.a && b == o.b && out == o.out && a_rows == o.a_rows && w_rows == o.w_rows && ldo == o.ldo &&
+             lda == o.lda && ldb == o.ldb && K == o.K && type == o.type && swiglu == o.swiglu;
     }
   };
   struct Entry { Key key; WlMaps maps; };
@@ -167,6 +168,7 @@ static inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * 
 // packed weight buffer offsets (bytes) ------------------------------------------------
 struct PackedLayout {
   size_t w13, w2, s13, s2, sh13, sh2, total;
+  size_t shs13, shs2;     // int8: the shared expert's scales
   size_t w_elem;          // bytes per routed weight element
 };
 PackedLayout packed_layout(const Handle* h);
@@ -185,12 +187,22 @@ int launch_permute_plan(const Handle* h, const int32_t* idx, int64_t T, int expe
                         void* ws, cudaStream_t st, int* launches, int32_t* job_counters = nullptr);
 bool plan_copies(const Handle* h, int64_t T);      // the forward's plan and scatter are one launch, launch_plan_and_rows
 int launch_plan_and_rows(const Handle* h, const int32_t* idx, int64_t T, int32_t* counts, int32_t* offsets, int32_t* pad_offsets,
-                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, cudaStream_t st);
+                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, const float* x_scale,
+                         float* perm_scale, cudaStream_t st);
 int launch_permute_plan_static(const Handle* h, const int32_t* idx, int64_t T, int expert_lo, int n_exp,
                                int32_t* counts, int32_t* offsets, int32_t* pad_offsets, int32_t* dst_row,
                                cudaStream_t st);
+// x_scale != nullptr: int8 rows and their scales, else bf16 rows
 int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, int64_t T,
-                        void* perm_x, cudaStream_t st);
+                        void* perm_x, cudaStream_t st, const float* x_scale = nullptr, float* perm_scale = nullptr);
+int launch_permute_rows_padded(const Handle* h, const void* x, const int32_t* dst_row, int64_t T, const int32_t* counts,
+                               const int32_t* pad, int n, int64_t n_rows, void* rows, cudaStream_t st);
+int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st);
+int launch_combine_grad(const Handle* h, const void* gy, const void* out_rows, const int32_t* dst_row, const float* w, int64_t T,
+                        const int32_t* counts, const int32_t* pad, int n, int64_t n_rows, void* grad_rows, float* grad_w,
+                        cudaStream_t st);
+int launch_route_topk_grad(const Handle* h, const float* logits, const int32_t* idx, const float* w, const float* grad_w, int64_t T,
+                           float* grad_logits, cudaStream_t st);
 int launch_combine(const Handle* h, const void* out_rows, const int32_t* dst_row,
                    const int32_t* idx, const float* w, const void* shared, const void* residual, int64_t T,
                    void* y, cudaStream_t st);
@@ -245,6 +257,12 @@ int launch_ep_place(const Handle* h, const int32_t* idx, int64_t T, const int32_
                     int cap_rows, void* ws, int32_t* recv_counts, int32_t* recv_pad, int32_t* dst,
                     cudaStream_t st);
 
+// 8-bit integers (int8.cu) ---------------------------------------------------------------
+int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, const int32_t* list, void* q,
+                         int64_t ldq, float* scale, cudaStream_t st);
+int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
+                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st);
+
 // weights (pack.cu) --------------------------------------------------------------------
 int launch_pack_expert(const Handle* h, int local_expert, const void* g, const void* u,
                        const void* dn, const float* gs, const float* us, const float* ds,
@@ -265,6 +283,9 @@ struct GemmProblem {
   const void* b;          // [n_groups * n_per_group, K] row-major ("N x K, K-major"), bf16 or FP8 e4m3
   bool b_fp8;             // B holds e4m3 bytes; `scales` holds fp32 [rows/128][K/128]
   const float* scales;
+  bool b_i8;              // A and B hold int8: a_scales [a_rows], `scales` [rows of B]; weight-lane GEMM, grouped or dense
+  const float* a_scales;
+  int64_t lda, ldb;       // int8: bytes between the rows of A and of B
   int n_groups;
   int n_per_group;        // rows of B per group (2I for SwiGLU, H for down, E for the gate)
   int K;

@@ -9,7 +9,9 @@
 //   W2  [E_l][H][I]   down_proj as stored by nn.Linear.
 //   S13 [E_l][2I/128][H/128], S2 [E_l][H/128][I/128]  fp32 scales (FP8 layers only), in the
 //                     same block order as the rows they scale.
-//   SH13 [2I_s][H], SH2 [H][I_s]   shared expert, always bf16, same interleave.
+//   SH13 [2I_s][H], SH2 [H][I_s]   shared expert, same interleave; bf16, or int8 in int8 layers
+//   int8 layers: S13 [E_l][2I], S2 [E_l][H] and, of the shared expert, SHS13 [2I_s], SHS2 [H]: fp32 scales of the rows, in
+//                     their order.
 // nn.Linear weights are [out, in] row-major = "N x K, K-major", which is the B operand
 // layout of the GEMM, so packing is a copy.
 #include <cuda_fp8.h>
@@ -22,7 +24,9 @@ PackedLayout packed_layout(const Handle* h) {
   const mg_layer_desc& d = h->d;
   PackedLayout L;
   const size_t E = h->e_local, I = d.inter, H = d.hidden, Is = d.inter_shared;
-  L.w_elem = d.weight_format == MG_WEIGHT_FP8_BLOCK128 ? 1 : 2;
+  const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
+  const size_t sh_elem = i8 ? 1 : 2;
+  L.w_elem = d.weight_format == MG_WEIGHT_BF16 ? 2 : 1;
   size_t off = 0;
   auto take = [&](size_t bytes) { size_t o = off; off += (bytes + 255) / 256 * 256; return o; };
   L.w13 = take(E * 2 * I * H * L.w_elem);
@@ -30,11 +34,16 @@ PackedLayout packed_layout(const Handle* h) {
   if (d.weight_format == MG_WEIGHT_FP8_BLOCK128) {
     L.s13 = take(E * (2 * I / 128) * (H / 128) * 4);
     L.s2 = take(E * (H / 128) * (I / 128) * 4);
+  } else if (i8) {
+    L.s13 = take(E * 2 * I * 4);
+    L.s2 = take(E * H * 4);
   } else {
     L.s13 = L.s2 = off;
   }
-  L.sh13 = take(2 * Is * H * 2);
-  L.sh2 = take(H * Is * 2);
+  L.sh13 = take(2 * Is * H * sh_elem);
+  L.sh2 = take(H * Is * sh_elem);
+  L.shs13 = i8 ? take(2 * Is * 4) : off;
+  L.shs2 = i8 && Is ? take(H * 4) : off;
   L.total = off;
   return L;
 }
@@ -71,6 +80,17 @@ __global__ void interleave_scales_kernel(const float* __restrict__ gs, const flo
   }
 }
 
+// scales of gate and up rows ([n] each) -> in the order of the interleaved rows
+__global__ void interleave_row_scales_kernel(const float* __restrict__ gs, const float* __restrict__ us, int n,
+                                             float* __restrict__ dst) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) {
+    const int at = i / 128 * 256 + i % 128;
+    dst[at] = gs[i];
+    dst[at + 128] = us[i];
+  }
+}
+
 int launch_pack_expert(const Handle* h, int local_expert, const void* g, const void* u, const void* dn,
                        const float* gs, const float* us, const float* ds, void* packed, cudaStream_t st) {
   const mg_layer_desc& d = h->d;
@@ -80,18 +100,29 @@ int launch_pack_expert(const Handle* h, int local_expert, const void* g, const v
   if (local_expert < 0) {
     const size_t Is = d.inter_shared;
     MG_REQUIRE(Is > 0, MG_ERR_CONFIG, "layer has no shared expert");
-    const int vpr = static_cast<int>(H * 2 / 16);
+    const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
+    const size_t elem = i8 ? 1 : 2;
+    MG_REQUIRE(!i8 || (gs && us && ds), MG_ERR_NULL, "int8 layer needs the three scale tensors of the shared expert");
+    const int vpr = static_cast<int>(H * elem / 16);
     interleave_rows_kernel<<<static_cast<unsigned>(Is), 256, 0, st>>>(
         static_cast<const uint4*>(g), static_cast<const uint4*>(u), static_cast<int>(Is), vpr,
         reinterpret_cast<uint4*>(base + L.sh13));
     MG_CUDA(cudaGetLastError());
-    copy_vec_kernel<<<1024, 256, 0, st>>>(static_cast<const uint4*>(dn), static_cast<int64_t>(H * Is * 2 / 16),
+    copy_vec_kernel<<<1024, 256, 0, st>>>(static_cast<const uint4*>(dn), static_cast<int64_t>(H * Is * elem / 16),
                                           reinterpret_cast<uint4*>(base + L.sh2));
     MG_CUDA(cudaGetLastError());
+    if (i8) {
+      interleave_row_scales_kernel<<<static_cast<unsigned>((Is + 255) / 256), 256, 0, st>>>(
+          gs, us, static_cast<int>(Is), reinterpret_cast<float*>(base + L.shs13));
+      MG_CUDA(cudaGetLastError());
+      MG_CUDA(cudaMemcpyAsync(base + L.shs2, ds, sizeof(float) * H, cudaMemcpyDeviceToDevice, st));
+    }
     return MG_OK;
   }
   MG_REQUIRE(local_expert < h->e_local, MG_ERR_SHAPE, "local_expert %d out of range [0,%d)", local_expert,
              h->e_local);
+  MG_REQUIRE(d.weight_format == MG_WEIGHT_BF16 || (gs && us && ds), MG_ERR_NULL, "%s layer needs the three scale tensors",
+             d.weight_format == MG_WEIGHT_INT8_CHANNEL ? "int8" : "FP8");
   const size_t I = d.inter, w = L.w_elem;
   const int vpr = static_cast<int>(H * w / 16);
   interleave_rows_kernel<<<static_cast<unsigned>(I), 256, 0, st>>>(
@@ -102,13 +133,19 @@ int launch_pack_expert(const Handle* h, int local_expert, const void* g, const v
                                         reinterpret_cast<uint4*>(base + L.w2 + static_cast<size_t>(local_expert) * H * I * w));
   MG_CUDA(cudaGetLastError());
   if (d.weight_format == MG_WEIGHT_FP8_BLOCK128) {
-    MG_REQUIRE(gs && us && ds, MG_ERR_NULL, "FP8 layer needs the three scale tensors");
     const int br = static_cast<int>(I / 128), bc = static_cast<int>(H / 128);
     float* s13 = reinterpret_cast<float*>(base + L.s13) + static_cast<size_t>(local_expert) * 2 * br * bc;
     interleave_scales_kernel<<<(br * bc + 255) / 256, 256, 0, st>>>(gs, us, br, bc, s13);
     MG_CUDA(cudaGetLastError());
     float* s2 = reinterpret_cast<float*>(base + L.s2) + static_cast<size_t>(local_expert) * bc * br;
     MG_CUDA(cudaMemcpyAsync(s2, ds, sizeof(float) * bc * br, cudaMemcpyDeviceToDevice, st));
+  }
+  if (d.weight_format == MG_WEIGHT_INT8_CHANNEL) {
+    interleave_row_scales_kernel<<<static_cast<unsigned>((I + 255) / 256), 256, 0, st>>>(
+        gs, us, static_cast<int>(I), reinterpret_cast<float*>(base + L.s13) + static_cast<size_t>(local_expert) * 2 * I);
+    MG_CUDA(cudaGetLastError());
+    float* s2 = reinterpret_cast<float*>(base + L.s2) + static_cast<size_t>(local_expert) * H;
+    MG_CUDA(cudaMemcpyAsync(s2, ds, sizeof(float) * H, cudaMemcpyDeviceToDevice, st));
   }
   return MG_OK;
 }

@@ -929,6 +929,14 @@ __global__ void __launch_bounds__(kPlanTokens) plan_place_kernel(const int32_t* 
   }
 }
 
+constexpr int kGapRows = 8;          // consecutive rows a warp looks at before the next warp's
+// blocks of so many warps that write zeros into the gaps of n_rows rows
+static unsigned gap_zero_blocks(const Handle* h, int64_t n_rows, int warps) {
+  const int64_t runs = (n_rows + kGapRows - 1) / kGapRows, want = (runs + warps - 1) / warps;
+  const int64_t most = static_cast<int64_t>(h->sm_count) * 16 / warps * 2;
+  return n_rows <= 0 ? 0u : static_cast<unsigned>(want < most ? want : most);
+}
+
 // vectors [v_begin, v_end) of a row, read once, to the k places row_of(pick, entry of the pick) names (nullptr: none); lane j
 // holds pick j's entry
 template <typename RowOf>
@@ -971,6 +979,8 @@ struct PlanCopy {
   const uint4* x;
   uint4* rows;
   int vec_per_row, slices, v_chunk;
+  const float* scale;           // int8 rows: of every token, nullptr else
+  float* row_scale;
 };
 template <bool COPY>
 __global__ void __launch_bounds__(1024) plan_small_kernel(const int32_t* idx, int T, int k, int lo, int n,
@@ -1044,6 +1054,7 @@ __global__ void __launch_bounds__(1024) plan_small_kernel(const int32_t* idx, in
     const int e = lane < k ? idx[t * k + lane] - lo : -1, at = (t >> 5) * n + e;
     int32_t dst = e >= 0 && e < n ? wbase[at] + __popc(bm[at] & ((1u << (t & 31)) - 1u)) : -1;
     if (dst >= 0 && !MG_GUARD(dst < guard.rows_bound, guard, 103)) dst = -1;
+    if (copy.scale != nullptr && v == 0 && dst >= 0) copy.row_scale[dst] = copy.scale[t];
     copy_row(copy.x + static_cast<int64_t>(t) * copy.vec_per_row, dst, k, v, min(copy.vec_per_row, v + copy.v_chunk), lane,
              [&](int, int32_t d) { return d < 0 ? nullptr : copy.rows + static_cast<int64_t>(d) * copy.vec_per_row; });
   }
@@ -1052,8 +1063,8 @@ __global__ void __launch_bounds__(1024) plan_small_kernel(const int32_t* idx, in
 // slices a token's row is cut into by the scatter while there are fewer than 16 warps per SM: 128 vectors or a multiple, the last
 // one what is left
 struct RowSlices { int n, v_chunk; };
-static RowSlices row_slices(const Handle* h, int64_t T) {
-  const int vpr = h->d.hidden / 8, steps = (vpr + 127) / 128;
+static RowSlices row_slices(const Handle* h, int64_t T, int vpr) {
+  const int steps = (vpr + 127) / 128;
   int64_t want = (static_cast<int64_t>(h->sm_count) * 16 + T - 1) / T;
   if (want > steps) want = steps;
   const int v_chunk = static_cast<int>((steps + want - 1) / want) * 128;
@@ -1066,7 +1077,7 @@ static_assert(plan_small_smem(kPlanCopyTokens, kMaxExperts) <= 48 * 1024, "the c
 // x == nullptr: the plan alone
 static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo, int n, int32_t* counts,
                              int32_t* offsets, int32_t* pad_offsets, int32_t* dst_row, int32_t* job_counters,
-                             const void* x, void* perm_x, cudaStream_t st) {
+                             const void* x, void* perm_x, const float* x_scale, float* perm_scale, cudaStream_t st) {
   const size_t smem = plan_small_smem(T, n);
   static bool done[64];
   if (smem > 48 * 1024 && !(h->device >= 0 && h->device < 64 && done[h->device])) {
@@ -1082,11 +1093,12 @@ static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo,
     return MG_OK;
   }
   if (threads < 256) threads = 256;
-  const RowSlices rs = row_slices(h, T);
+  const int vpr = h->d.hidden / (x_scale != nullptr ? 16 : 8);
+  const RowSlices rs = row_slices(h, T, vpr);
   const int warps = threads / 32;
   MG_CUDA(launch_chained(h, plan_small_kernel<true>, (T * rs.n + warps - 1) / warps, threads, smem, st, idx, T, h->d.top_k, lo, n,
                          counts, offsets, pad_offsets, dst_row, job_counters,
-                         PlanCopy{static_cast<const uint4*>(x), static_cast<uint4*>(perm_x), h->d.hidden / 8, rs.n, rs.v_chunk},
+                         PlanCopy{static_cast<const uint4*>(x), static_cast<uint4*>(perm_x), vpr, rs.n, rs.v_chunk, x_scale, perm_scale},
                          guard));
   return MG_OK;
 }
@@ -1097,9 +1109,10 @@ static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo,
 // and 467.7; V2-236B 8 tokens 359 and 357, 128 1170 and 1171, 512 1230 and 1239; V3 1 token 149.7 and 146.5, 256 2562 and 2570.
 bool plan_copies(const Handle* h, int64_t T) { return T > 0 && T <= kPlanCopyTokens && T * h->d.hidden >= 4096; }
 int launch_plan_and_rows(const Handle* h, const int32_t* idx, int64_t T, int32_t* counts, int32_t* offsets, int32_t* pad_offsets,
-                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, cudaStream_t st) {
+                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, const float* x_scale,
+                         float* perm_scale, cudaStream_t st) {
   return launch_plan_small(h, idx, static_cast<int>(T), 0, h->d.n_experts, counts, offsets, pad_offsets, dst_row, job_counters, x,
-                           perm_x, st);
+                           perm_x, x_scale, perm_scale, st);
 }
 
 size_t plan_ws_bytes(const Handle* h, int64_t T) {
@@ -1116,7 +1129,7 @@ int launch_permute_plan(const Handle* h, const int32_t* idx, int64_t T, int expe
   if (T > 0 && T <= kPlanSmallTokens) {
     if (launches) *launches += 1;
     return launch_plan_small(h, idx, static_cast<int>(T), expert_lo, n_exp, counts, offsets, pad_offsets, dst_row,
-                             job_counters, nullptr, nullptr, st);
+                             job_counters, nullptr, nullptr, nullptr, nullptr, st);
   }
   int nblk = static_cast<int>((T + kPlanTokens - 1) / kPlanTokens);
   int32_t* bc = static_cast<int32_t*>(ws);
@@ -1200,7 +1213,7 @@ template <bool PEER, bool DEDUP, bool BACK>
 __global__ void __launch_bounds__(256) permute_rows_kernel(const uint4* __restrict__ x, const int32_t* dst_row,
                                                            int64_t T, int k, int vec_per_row, int slices, int v_chunk,
                                                            PeerPtrs bufs, PeerPtrs dups, PeerPtrs backs, int my_rank,
-                                                           Guard guard) {
+                                                           const float* scale, float* row_scale, Guard guard) {
   chain_wait();
   chain_go();
   const int lane = threadIdx.x & 31;
@@ -1213,6 +1226,7 @@ __global__ void __launch_bounds__(256) permute_rows_kernel(const uint4* __restri
   if (my_dst >= 0 && !MG_GUARD((PEER ? (my_dst & kPeerRowMask) : my_dst) < guard.rows_bound &&
                                (!PEER || (my_dst >> kPeerShift) < guard.n_peers), guard, 103))
     my_dst = -1;
+  if (!PEER && scale != nullptr && v_begin == 0 && my_dst >= 0) row_scale[my_dst] = scale[t];      // int8 rows
   if (BACK && my_dst >= 0)
     static_cast<int32_t*>(backs.p[my_dst >> kPeerShift])[my_dst & kPeerRowMask] =
         (my_rank << kPeerShift) | static_cast<int32_t>(t * k + lane);
@@ -1266,15 +1280,190 @@ __global__ void __launch_bounds__(256) fill_duplicate_rows_kernel(uint4* __restr
 }
 
 int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, int64_t T,
-                        void* perm_x, cudaStream_t st) {
+                        void* perm_x, cudaStream_t st, const float* x_scale, float* perm_scale) {
   if (T == 0) return MG_OK;
-  const int warps = 8;
-  const RowSlices rs = row_slices(h, T);
+  const int warps = 8, vpr = h->d.hidden / (x_scale != nullptr ? 16 : 8);
+  const RowSlices rs = row_slices(h, T, vpr);
   dim3 grid(static_cast<unsigned>((T * rs.n + warps - 1) / warps)), block(warps * 32);
   PeerPtrs bufs{};
   bufs.p[0] = perm_x;
   MG_CUDA(launch_chained(h, permute_rows_kernel<false, false, false>, grid, block, 0, st, static_cast<const uint4*>(x), dst_row,
-                         T, h->d.top_k, h->d.hidden / 8, rs.n, rs.v_chunk, bufs, bufs, bufs, 0, Guard{h->d_status, h->guard_rows, 1}));
+                         T, h->d.top_k, vpr, rs.n, rs.v_chunk, bufs, bufs, bufs, 0, x_scale, perm_scale,
+                         Guard{h->d_status, h->guard_rows, 1}));
+  return MG_OK;
+}
+
+// The scatter with zeros in the rows that hold no pick: blocks behind those of the scatter write them.  A row is a gap if it
+// lies behind the rows of its expert's segment or behind the last segment; a lane looks one row up, the warp writes.
+__device__ __forceinline__ void zero_gap_rows(uint4* rows, int64_t n_rows, int vec_per_row, const int32_t* counts, const int32_t* pad,
+                                              int n, int64_t warp, int64_t n_warps, int32_t* s_pad) {
+  for (int i = threadIdx.x; i <= n; i += blockDim.x) s_pad[i] = pad[i];
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r0 = warp * kGapRows; r0 < n_rows; r0 += n_warps * kGapRows) {
+    const int64_t r = r0 + lane;
+    bool gap = lane < kGapRows && r < n_rows;
+    if (gap && r < s_pad[n]) {
+      int lo = 0, hi = n;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_pad[mid] <= r) lo = mid; else hi = mid;
+      }
+      gap = r - s_pad[lo] >= counts[lo];
+    }
+    uint32_t todo = __ballot_sync(0xFFFFFFFFu, gap);
+    while (todo != 0u) {
+      uint4* row = rows + (r0 + __ffs(todo) - 1) * vec_per_row;
+      todo &= todo - 1;
+      for (int v = lane; v < vec_per_row; v += 32) row[v] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+}
+__global__ void __launch_bounds__(256) permute_rows_padded_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ dst_row,
+                                                                  int64_t T, int k, int vec_per_row, int slices, int v_chunk,
+                                                                  unsigned copy_blocks, const int32_t* __restrict__ counts,
+                                                                  const int32_t* __restrict__ pad, int n, int64_t n_rows,
+                                                                  uint4* __restrict__ rows, Guard guard) {
+  __shared__ int32_t s_pad[kMaxExperts + 1];
+  const int lane = threadIdx.x & 31;
+  if (blockIdx.x >= copy_blocks) {
+    zero_gap_rows(rows, n_rows, vec_per_row, counts, pad, n, static_cast<int64_t>(blockIdx.x - copy_blocks) * 8 + (threadIdx.x >> 5),
+                  static_cast<int64_t>(gridDim.x - copy_blocks) * 8, s_pad);
+    return;
+  }
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t t = item / slices;
+  const int v_begin = static_cast<int>(item - t * slices) * v_chunk;
+  if (t >= T) return;
+  int32_t my_dst = lane < k ? dst_row[t * k + lane] : -1;
+  if (my_dst >= n_rows || (my_dst >= 0 && !MG_GUARD(my_dst < guard.rows_bound, guard, 103))) my_dst = -1;
+  copy_row(x + t * vec_per_row, my_dst, k, v_begin, min(vec_per_row, v_begin + v_chunk), lane,
+           [&](int, int32_t d) { return d < 0 ? nullptr : rows + static_cast<int64_t>(d) * vec_per_row; });
+}
+
+int launch_permute_rows_padded(const Handle* h, const void* x, const int32_t* dst_row, int64_t T, const int32_t* counts,
+                               const int32_t* pad, int n, int64_t n_rows, void* rows, cudaStream_t st) {
+  const int vpr = h->d.hidden / 8;
+  const RowSlices rs = row_slices(h, T > 0 ? T : 1, vpr);
+  const unsigned copy_blocks = static_cast<unsigned>((T * rs.n + 7) / 8), gap_blocks = gap_zero_blocks(h, n_rows, 8);
+  if (copy_blocks + gap_blocks == 0) return MG_OK;
+  permute_rows_padded_kernel<<<copy_blocks + gap_blocks, 256, 0, st>>>(
+      static_cast<const uint4*>(x), dst_row, T, h->d.top_k, vpr, rs.n, rs.v_chunk, copy_blocks, counts, pad, n, n_rows,
+      static_cast<uint4*>(rows), Guard{h->d_status, h->guard_rows, 1});
+  MG_CUDA(cudaGetLastError());
+  return MG_OK;
+}
+
+// Gradient of the return: gr[dst[t,j]] = w[t,j] gy[t], gw[t,j] = <gy[t], r[dst[t,j]]> (fp32 sums of exact products, always in the
+// same order).  A block per token; every row is read once and written once, gy once per token.  Two picks of one row (a token
+// that names an expert twice) add their weights, and the first of them writes.
+template <bool ROWS, bool WEIGHTS>
+__global__ void __launch_bounds__(1024) combine_grad_kernel(const uint4* __restrict__ gy, const uint4* __restrict__ out_rows,
+                                                            const int32_t* __restrict__ dst_row, const float* __restrict__ topk_w,
+                                                            int64_t T, int k, int vec_per_row, bool round_w, int64_t n_rows,
+                                                            const int32_t* __restrict__ counts, const int32_t* __restrict__ pad, int n,
+                                                            uint4* __restrict__ grad_rows, float* __restrict__ grad_w, Guard guard) {
+  __shared__ int32_t s_pad[kMaxExperts + 1];
+  __shared__ float s_part[32][kMaxTopK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t t = blockIdx.x;
+  if (t >= T) {
+    zero_gap_rows(grad_rows, n_rows, vec_per_row, counts, pad, n, (t - T) * warps + warp, (gridDim.x - T) * warps, s_pad);
+    return;
+  }
+  int32_t my_dst = -1;
+  float my_w = 0.f;
+  if (lane < k) {
+    my_dst = dst_row[t * k + lane];
+    if (my_dst >= n_rows || (my_dst >= 0 && !MG_GUARD(my_dst < guard.rows_bound, guard, 107))) my_dst = -1;
+    my_w = topk_w[t * k + lane];
+    if (round_w) my_w = round_bf16(my_w);
+  }
+  int32_t write = my_dst;
+  if (ROWS) {
+    const float w0 = my_w;
+    for (int j = 0; j < k; ++j) {
+      const int32_t d = __shfl_sync(0xFFFFFFFFu, my_dst, j);
+      const float w = __shfl_sync(0xFFFFFFFFu, w0, j);
+      if (lane < k && j != lane && d == my_dst) {
+        if (j < lane) write = -1; else my_w = __fadd_rn(my_w, w);
+      }
+    }
+  }
+  float dot[kMaxTopK];
+#pragma unroll
+  for (int j = 0; j < kMaxTopK; ++j) dot[j] = 0.f;
+  for (int v = threadIdx.x; v < vec_per_row; v += blockDim.x) {       // whole warps: a row is a multiple of 32 vectors
+    float g[8];
+    unpack8(__ldg(gy + t * vec_per_row + v), g);
+#pragma unroll
+    for (int j0 = 0; j0 < kMaxTopK; j0 += 4) {
+      if (j0 >= k) break;
+      uint4 val[4];
+      if (WEIGHTS) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int32_t d = __shfl_sync(0xFFFFFFFFu, my_dst, j0 + u);
+          val[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (d >= 0) val[u] = __ldg(out_rows + static_cast<int64_t>(d) * vec_per_row + v);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (WEIGHTS) {
+          float r[8];
+          unpack8(val[u], r);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dot[j0 + u] = fmaf(g[i], r[i], dot[j0 + u]);
+        }
+        if (ROWS) {
+          const int32_t d = __shfl_sync(0xFFFFFFFFu, write, j0 + u);
+          const float w = __shfl_sync(0xFFFFFFFFu, my_w, j0 + u);
+          if (d >= 0) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __fmul_rn(g[i], w);
+            grad_rows[static_cast<int64_t>(d) * vec_per_row + v] = pack8(o);
+          }
+        }
+      }
+    }
+  }
+  if (!WEIGHTS) return;
+#pragma unroll
+  for (int j = 0; j < kMaxTopK; ++j) {
+    if (j >= k) break;
+    const float sum = warp_sum_f(dot[j]);
+    if (lane == 0) s_part[warp][j] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x < k) {
+    float sum = 0.f;
+    for (int i = 0; i < warps; ++i) sum = __fadd_rn(sum, s_part[i][threadIdx.x]);
+    grad_w[t * k + threadIdx.x] = sum;
+  }
+}
+
+int launch_combine_grad(const Handle* h, const void* gy, const void* out_rows, const int32_t* dst_row, const float* w, int64_t T,
+                        const int32_t* counts, const int32_t* pad, int n, int64_t n_rows, void* grad_rows, float* grad_w,
+                        cudaStream_t st) {
+  const int vpr = h->d.hidden / 8;
+  int threads = 128;                       // 16 warps per SM at least, as far as a row has vectors for them
+  while (threads < 1024 && threads < vpr && T * threads < static_cast<int64_t>(h->sm_count) * 512) threads *= 2;
+  if (threads > vpr) threads = vpr;
+  const unsigned gaps = grad_rows != nullptr && counts != nullptr ? gap_zero_blocks(h, n_rows, threads / 32) : 0;
+  const int64_t blocks = (grad_rows != nullptr || grad_w != nullptr ? T : 0) + gaps;
+  if (blocks == 0) return MG_OK;
+#define MG_GRAD_CASE(R, W)                                                                                             \
+  combine_grad_kernel<R, W><<<static_cast<unsigned>(blocks), threads, 0, st>>>(                                        \
+      static_cast<const uint4*>(gy), static_cast<const uint4*>(out_rows), dst_row, w, T, h->d.top_k, vpr,              \
+      h->d.combine_mode != MG_COMBINE_FP32, n_rows, counts, pad, n, static_cast<uint4*>(grad_rows), grad_w,            \
+      Guard{h->d_status, h->guard_rows, 1})
+  if (grad_rows != nullptr && grad_w != nullptr) MG_GRAD_CASE(true, true);
+  else if (grad_rows != nullptr) MG_GRAD_CASE(true, false);
+  else MG_GRAD_CASE(false, true);
+#undef MG_GRAD_CASE
+  MG_CUDA(cudaGetLastError());
   return MG_OK;
 }
 
@@ -1289,13 +1478,13 @@ int launch_dispatch_rows(const Handle* h, const void* x, const int32_t* dst, int
   const PeerPtrs& b = backs ? *backs : peers;
   const Guard guard{h->d_status, h->guard_rows, h->d.ep_size};
   if (dups != nullptr && backs != nullptr)
-    permute_rows_kernel<true, true, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, guard);
+    permute_rows_kernel<true, true, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
   else if (dups != nullptr)
-    permute_rows_kernel<true, true, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, guard);
+    permute_rows_kernel<true, true, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
   else if (backs != nullptr)
-    permute_rows_kernel<true, false, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, guard);
+    permute_rows_kernel<true, false, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
   else
-    permute_rows_kernel<true, false, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, guard);
+    permute_rows_kernel<true, false, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
   MG_CUDA(cudaGetLastError());
   return MG_OK;
 }
@@ -1356,42 +1545,19 @@ int launch_fill_duplicates(const Handle* h, void* rows, const int32_t* dup, int6
 // ---------------------------------------------------------------------------------------
 // combine: y[t] = sum_j w[t,j] * out_rows[dst_row[t,j]] (+ shared[t])
 // ---------------------------------------------------------------------------------------
-__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
-  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 t = __bfloat1622float2(p[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
-// Rows of the kernel before this one, or of another GPU during this forward: an ordinary (coherent) load, kept in its place.
-// Free to move the loads, the compiler holds all addresses in 64 registers and half the warps fit: combine of 65536 tokens
-// of the V3 shape 2.37 ms, with 32 registers 1.43; of 32768 tokens of V2-236B 0.79 and 0.56.
-__device__ __forceinline__ uint4 ld_row(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint4 pack8(const float* f) {
-  uint4 v;
-  __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&v);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-  return v;
-}
-__device__ __forceinline__ float round_bf16(float f) {
-  return __bfloat162float(__float2bfloat16_rn(f));
-}
-
+// wide: the routed sum is not rounded to bf16 before the shared expert's row is added.  The other layers round there because the
+// reference does; int8 layers have none to follow, and it is one of four roundings of their result (V2-236B shape, 201 tokens,
+// error against 64 bits 0.0029 and 0.0025).
 // by_slot = rank + 1 (expert-parallel pushed return): a pick whose owner is another rank lies at row
 // (token * k + slot) of this rank's return buffer (bufs.p[owner] all point at it), a pick of this rank's own
 // experts is read in place from its out_rows (bufs.p[rank]); 0 = rows as dst_row says.
+// MODE kSumRows: the plain sum of the rows, a row that two picks share once (gradient of the scatter); no weights are read.
+constexpr int kSumRows = 3;
 template <int MODE, bool PEER>
 __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32_t* dst_row, const int32_t* topk_idx,
                                                       const float* topk_w, const uint4* shared, const uint4* residual,
                                                       int64_t T, int k, int vec_per_row, int v_chunk,
-                                                      uint4* y, int by_slot, const int32_t* delta, Guard guard) {
+                                                      uint4* y, int by_slot, const int32_t* delta, bool wide, Guard guard) {
   chain_wait();
   chain_go();
   const int lane = threadIdx.x & 31;
@@ -1409,9 +1575,17 @@ __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32
     // mirror of the owners' rows in this rank's own expert-sorted order (bufs.p[0]): row in the owner's
     // buffer + the expert's offset between the two layouts
     if (delta != nullptr && my_dst >= 0) my_dst = (my_dst & kPeerRowMask) + delta[topk_idx[t * k + lane]];
-    my_w = topk_w[t * k + lane];
+    my_w = MODE == kSumRows ? 1.f : topk_w[t * k + lane];
     if (MODE == MG_COMBINE_BF16_SEQ) my_e = topk_idx[t * k + lane];
-    if (MODE != MG_COMBINE_FP32) my_w = round_bf16(my_w);
+    if (MODE != MG_COMBINE_FP32 && MODE != kSumRows) my_w = round_bf16(my_w);
+  }
+  if (MODE == kSumRows) {
+    bool again = false;
+    for (int j = 0; j < k; ++j) {
+      const int32_t d = __shfl_sync(0xFFFFFFFFu, my_dst, j);
+      again = again || (j < lane && d == my_dst);
+    }
+    if (again) my_dst = -1;
   }
   // BF16_SEQ adds in ascending expert order: rank of my slot among the k picks
   int order_src = lane;  // slot visited at step `lane`
@@ -1468,7 +1642,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32
           for (int i = 0; i < 8; ++i) {
             // a skipped pick contributes w = 0 and f = 0: adding 0 changes nothing in any mode
             float p = __fmul_rn(f[i], w);
-            if (MODE == MG_COMBINE_FP32) acc[i] = __fadd_rn(acc[i], p);
+            if (MODE == MG_COMBINE_FP32 || MODE == kSumRows) acc[i] = __fadd_rn(acc[i], p);
             else if (MODE == MG_COMBINE_BF16_PROD) acc[i] = __fadd_rn(acc[i], round_bf16(p));
             else acc[i] = round_bf16(__fadd_rn(acc[i], round_bf16(p)));
           }
@@ -1479,7 +1653,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32
       float f[8];
       unpack8(ld_row(shared + t * vec_per_row + v), f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = __fadd_rn(round_bf16(acc[i]), f[i]);
+      for (int i = 0; i < 8; ++i) acc[i] = __fadd_rn(wide ? acc[i] : round_bf16(acc[i]), f[i]);
     }
     if (residual != nullptr) {
       // decoder-layer glue: the block's bf16 output is added to the bf16 residual stream (y may alias it)
@@ -1496,7 +1670,7 @@ template <bool PEER>
 static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int32_t* dst_row,
                                const int32_t* idx, const float* w, const void* shared, const void* residual,
                                int64_t T, void* y, cudaStream_t st, int by_slot = 0,
-                               const int32_t* delta = nullptr) {
+                               const int32_t* delta = nullptr, bool sum = false) {
   if (T == 0) return MG_OK;
   const int warps = 8;
   const int k = h->d.top_k, vpr = h->d.hidden / 8;
@@ -1511,8 +1685,12 @@ static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int3
 #define MG_COMBINE_CASE(M)                                                                       \
   MG_CUDA(launch_chained(h, combine_kernel<M, PEER>, grid, block, 0, st, bufs, dst_row, idx, w,   \
                          static_cast<const uint4*>(shared), static_cast<const uint4*>(residual), T, k, vpr, v_chunk, \
-                         static_cast<uint4*>(y), by_slot, delta,                                 \
+                         static_cast<uint4*>(y), by_slot, delta, h->d.weight_format == MG_WEIGHT_INT8_CHANNEL, \
                          Guard{h->d_status, h->guard_rows, PEER ? h->d.ep_size : 1}))
+  if (!PEER && sum) {
+    MG_COMBINE_CASE(kSumRows);
+    return MG_OK;
+  }
   switch (h->d.combine_mode) {
     case MG_COMBINE_FP32: MG_COMBINE_CASE(MG_COMBINE_FP32); break;
     case MG_COMBINE_BF16_PROD: MG_COMBINE_CASE(MG_COMBINE_BF16_PROD); break;
@@ -1522,6 +1700,12 @@ static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int3
 #undef MG_COMBINE_CASE
   MG_CUDA(cudaGetLastError());
   return MG_OK;
+}
+
+int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st) {
+  PeerPtrs bufs{};
+  bufs.p[0] = const_cast<void*>(grad_rows);
+  return launch_combine_impl<false>(h, bufs, dst_row, nullptr, nullptr, nullptr, nullptr, T, grad_x, st, 0, nullptr, true);
 }
 
 int launch_combine(const Handle* h, const void* out_rows, const int32_t* dst_row,
@@ -1597,6 +1781,107 @@ int launch_combine_peers(const Handle* h, const PeerPtrs& peers, const int32_t* 
                          const int32_t* idx, const float* w, const void* shared, int64_t T, void* y,
                          cudaStream_t st) {
   return launch_combine_impl<true>(h, peers, dst, idx, w, shared, nullptr, T, y, st);
+}
+
+// ---------------------------------------------------------------------------------------
+// gradient of the routing weights with respect to the logits, the picks being constants
+// ---------------------------------------------------------------------------------------
+// p_j: score (softmax s or sigmoid) of pick j.  Weights w_j = c p_j, or c p_j / d with d = sum p + eps:
+//   gp_j = c gw_j   or   (c / d) (gw_j - S), S = sum gw_j p_j / d
+//   softmax  gl_i = s_i (gs_i - D), gs the gp of the picks by expert and D = sum gp_j p_j; normalised, D = c S eps / d exactly,
+//            and is not summed up from terms that cancel
+//   sigmoid  gl_i = gs_i s_i (1 - s_i), with s (1 - s) = e / (1 + e)^2, e = exp(-|l|), which does not cancel either
+// A pick of weight 0 competed from a masked group (its score is the constant 0) and passes nothing on.  A warp per token; softmax
+// reads the row of logits once, sigmoid the picks' alone; the row of gradients is written once.
+template <bool SIGMOID>
+__global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __restrict__ logits, const int32_t* __restrict__ topk_idx,
+                                                              const float* __restrict__ topk_w, const float* __restrict__ grad_w,
+                                                              int64_t T, int E, int k, bool norm, float c, float eps,
+                                                              float* __restrict__ grad_logits) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (t >= T) return;
+  constexpr int QUADS = kMaxExperts / 128;             // of four experts, per lane
+  const float4* row = reinterpret_cast<const float4*>(logits + t * E);
+  const int quads = E >> 2;
+  int32_t e = -1;
+  float w = 0.f, gw = 0.f, l = 0.f;
+  if (lane < k) {
+    e = topk_idx[t * k + lane];
+    w = topk_w[t * k + lane];
+    gw = grad_w[t * k + lane];
+    if (e >= 0 && e < E) l = logits[t * E + e]; else e = -1;
+  }
+  float4 s[QUADS];
+  float m = 0.f, inv_sum = 0.f;
+  if (!SIGMOID) {
+    m = __int_as_float(0xff800000);
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      const int q = i * 32 + lane;
+      s[i] = make_float4(m, m, m, m);
+      if (q < quads) s[i] = __ldg(row + q);
+    }
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) m = fmaxf(m, fmaxf(fmaxf(s[i].x, s[i].y), fmaxf(s[i].z, s[i].w)));
+    m = warp_max_f(m);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+      s[i] = make_float4(expf(s[i].x - m), expf(s[i].y - m), expf(s[i].z - m), expf(s[i].w - m));
+      if (i * 32 + lane < quads) sum += (s[i].x + s[i].y) + (s[i].z + s[i].w);
+    }
+    inv_sum = 1.0f / warp_sum_f(sum);
+  }
+  const bool live = e >= 0 && w != 0.f;
+  const float ex = expf(-fabsf(l));
+  float p = 0.f;
+  if (live) p = SIGMOID ? (l >= 0.f ? 1.0f : ex) / (1.0f + ex) : expf(l - m) * inv_sum;
+  float gp = 0.f, D = 0.f;
+  if (norm) {
+    const float d = warp_sum_f(p) + eps, S = warp_sum_f(live ? gw * p : 0.f) / d;
+    if (live) gp = c * (gw - S) / d;
+    D = c * S * eps / d;
+  } else {
+    if (live) gp = c * gw;
+    D = warp_sum_f(gp * p);
+  }
+  if (SIGMOID) gp *= ex / ((1.0f + ex) * (1.0f + ex));
+  float4* out = reinterpret_cast<float4*>(grad_logits + t * E);
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) {
+    const int q = i * 32 + lane;
+    if (i * 32 >= quads) break;
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < k; ++j) {
+      const int32_t ej = __shfl_sync(0xFFFFFFFFu, e, j);
+      const float gj = __shfl_sync(0xFFFFFFFFu, gp, j);
+      if ((ej >> 2) == q) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if ((ej & 3) == u) g[u] += gj;
+      }
+    }
+    if (!SIGMOID) {
+      g[0] = s[i].x * inv_sum * (g[0] - D); g[1] = s[i].y * inv_sum * (g[1] - D);
+      g[2] = s[i].z * inv_sum * (g[2] - D); g[3] = s[i].w * inv_sum * (g[3] - D);
+    }
+    if (q < quads) out[q] = make_float4(g[0], g[1], g[2], g[3]);
+  }
+}
+
+int launch_route_topk_grad(const Handle* h, const float* logits, const int32_t* idx, const float* w, const float* grad_w, int64_t T,
+                           float* grad_logits, cudaStream_t st) {
+  if (T == 0) return MG_OK;
+  const mg_layer_desc& d = h->d;
+  const bool sig = d.gating == MG_GATE_SIGMOID_NOAUX_TC, renorm = d.gating == MG_GATE_SOFTMAX_TOPK_RENORM;
+  const bool norm = renorm || (d.norm_topk_prob && d.top_k > 1);
+  const float c = norm && !sig ? 1.0f : d.routed_scale, eps = renorm ? 0.0f : 1e-20f;
+  const unsigned grid = static_cast<unsigned>((T + 7) / 8);
+  if (sig) route_topk_grad_kernel<true><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, d.n_experts, d.top_k, norm, c, eps, grad_logits);
+  else route_topk_grad_kernel<false><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, d.n_experts, d.top_k, norm, c, eps, grad_logits);
+  MG_CUDA(cudaGetLastError());
+  return MG_OK;
 }
 
 // ---------------------------------------------------------------------------------------

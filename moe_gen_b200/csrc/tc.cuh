@@ -98,6 +98,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 // the box of a load, into L2 only
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
+}
 __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
@@ -214,6 +217,35 @@ __device__ __forceinline__ void convert16(const uint4& q, float s, uint4& lo, ui
   hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
+// ---- rows of bf16 -----------------------------------------------------------------------
+__device__ __forceinline__ void unpack8(const uint4& v, float* f) {
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 t = __bfloat1622float2(p[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+// Rows of the kernel before this one, or of another GPU during this forward: an ordinary (coherent) load, kept in its place.
+// Free to move the loads, the compiler holds all addresses in 64 registers and half the warps fit: combine of 65536 tokens
+// of the V3 shape 2.37 ms, with 32 registers 1.43; of 32768 tokens of V2-236B 0.79 and 0.56.
+__device__ __forceinline__ uint4 ld_row(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 pack8(const float* f) {
+  uint4 v;
+  __nv_bfloat162* p = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  return v;
+}
+__device__ __forceinline__ float round_bf16(float f) {
+  return __bfloat162float(__float2bfloat16_rn(f));
+}
+
 // ---- SM pairs (cta_group::2) -----------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
@@ -275,8 +307,9 @@ enum TensorMapKind : uint32_t {
   TM_OUT_16 = 3,      // boxes of 16 bf16, unswizzled: the SwiGLU stores of the weight-lane kernel
 };
 
+// ld: elements between rows (0: cols)
 int encode_2d(const Handle* h, CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
-              TensorMapKind kind);
+              TensorMapKind kind, uint64_t ld = 0);
 
 // tensor map of up to four dimensions, SWIZZLE_128B, of bytes or bf16: extents, strides in bytes of all but the inner one,
 // box (gemm.cu; not cached)

@@ -81,9 +81,11 @@ class MoELayer:
     def load_expert(self, local_expert: int, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
                     scales: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
         """Packs one expert ([I,H], [I,H], [H,I] as nn.Linear stores them).  local_expert = -1 is
-        the shared expert.  FP8 layers pass float8_e4m3fn matrices plus their fp32 scales."""
+        the shared expert.  FP8 layers pass float8_e4m3fn matrices plus their fp32 scales; int8 layers, for the shared
+        expert too, int8 matrices plus the fp32 scales of their rows ([I], [I], [H])."""
         fp8 = self.desc.weight_format == L.WEIGHT_FP8_BLOCK128 and local_expert >= 0
-        dt = torch.float8_e4m3fn if fp8 else torch.bfloat16
+        int8 = self.desc.weight_format == L.WEIGHT_INT8_CHANNEL
+        dt = torch.float8_e4m3fn if fp8 else torch.int8 if int8 else torch.bfloat16
         mats = [m.detach().to(self.device).contiguous() for m in (gate, up, down)]
         I = self.Is if local_expert < 0 else self.I
         for m, shp in zip(mats, ((I, self.H), (I, self.H), (self.H, I))):
@@ -94,14 +96,21 @@ class MoELayer:
             if scales is None:
                 raise ValueError("FP8 layer: scales=(gate_scale, up_scale, down_scale) required")
             sc = [s.detach().to(self.device, torch.float32).contiguous() for s in scales]
+        if int8:
+            if scales is None:
+                raise ValueError("int8 layer: scales=(gate_scale, up_scale, down_scale) required")
+            sc = [s.detach().to(self.device, torch.float32).reshape(-1).contiguous() for s in scales]
+            for s, m in zip(sc, mats):
+                if s.numel() != m.shape[0]:
+                    raise ValueError(f"int8 expert matrix of {m.shape[0]} rows with {s.numel()} scales")
         with torch.cuda.device(self.device):
             L.check(self.lib.mg_pack_expert(self._h, local_expert, mats[0].data_ptr(), mats[1].data_ptr(),
                                             mats[2].data_ptr(), _ptr(sc[0]), _ptr(sc[1]), _ptr(sc[2]),
                                             self.packed.data_ptr(), self._stream()))
             torch.cuda.current_stream().synchronize()   # sources may be temporaries
 
-    def load_shared(self, gate, up, down):
-        self.load_expert(-1, gate, up, down)
+    def load_shared(self, gate, up, down, scales: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
+        self.load_expert(-1, gate, up, down, scales)
 
     # ------------------------------------------------------------------ sizes
     def padded_rows(self, n_rows: int) -> int:
@@ -320,13 +329,204 @@ class MoELayer:
                                              self._stream()))
         return counts, offsets, pad, dst
 
-    def permute_rows(self, x: torch.Tensor, dst_row: torch.Tensor, rows_padded: int) -> torch.Tensor:
+    def _check_plan(self, dst_row: torch.Tensor, counts: torch.Tensor, pad_offsets: torch.Tensor):
+        self._check_in(counts, torch.int32, "counts")
+        self._check_in(pad_offsets, torch.int32, "pad_offsets")
+        if counts.numel() > self.E or pad_offsets.numel() != counts.numel() + 1:
+            raise ValueError(f"counts of {counts.numel()} and pad_offsets of {pad_offsets.numel()} entries for {self.E} experts")
+
+    def _check_rows(self, t: torch.Tensor, dtype, rows: Optional[int], cols: int, what: str):
+        self._check_in(t, dtype, what)
+        if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+            raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {('rows' if rows is None else rows, cols)}")
+
+    def permute_rows(self, x: torch.Tensor, dst_row: torch.Tensor, rows_padded: int, counts: Optional[torch.Tensor] = None,
+                     pad_offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """perm[dst_row[t, j]] = x[t], zeros in the rows no pick points at.  With the plan's counts and pad_offsets only those
+        rows are written as zeros, in the same launch, instead of all rows before it."""
         self._check_in(x, torch.bfloat16, "hidden_states")
+        if counts is not None and pad_offsets is not None:
+            self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
+            self._check_rows(dst_row, torch.int32, x.shape[0], self.k, "dst_row")
+            self._check_plan(dst_row, counts, pad_offsets)
+            perm = torch.empty(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
+            with torch.cuda.device(self.device):
+                L.check(self.lib.mg_permute_rows_padded(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
+                                                        counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), rows_padded,
+                                                        perm.data_ptr(), self._stream()))
+            return perm
         perm = torch.zeros(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
         with torch.cuda.device(self.device):
             L.check(self.lib.mg_permute_rows(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
                                              perm.data_ptr(), self._stream()))
         return perm
+
+    def permute_rows_grad(self, grad_rows: torch.Tensor, dst_row: torch.Tensor) -> torch.Tensor:
+        """Gradient of permute_rows: grad_x[t] = sum_j grad_rows[dst_row[t, j]] (fp32 sum, one rounding).  dst_row is a plan's:
+        its entries lie below grad_rows' rows."""
+        self._check_rows(grad_rows, torch.bfloat16, None, self.H, "grad_rows")
+        self._check_rows(dst_row, torch.int32, None, self.k, "dst_row")
+        T = dst_row.shape[0]
+        gx = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_permute_rows_grad(self._h, grad_rows.data_ptr(), dst_row.data_ptr(), T, gx.data_ptr(),
+                                                  self._stream()))
+        return gx
+
+    def combine_grad(self, grad_y: torch.Tensor, out_rows: torch.Tensor, dst_row: torch.Tensor, topk_w: torch.Tensor,
+                     counts: torch.Tensor, pad_offsets: torch.Tensor, need_rows: bool = True, need_w: bool = True):
+        """Gradients of combine's sum -> (grad_rows like out_rows, zeros where no pick points; grad_w [T, k] fp32), None for the
+        one that is not needed.  The gradient of shared_out is grad_y itself."""
+        T = dst_row.shape[0]
+        self._check_rows(grad_y, torch.bfloat16, T, self.H, "grad_y")
+        self._check_rows(out_rows, torch.bfloat16, None, self.H, "out_rows")
+        self._check_rows(dst_row, torch.int32, T, self.k, "dst_row")
+        self._check_rows(topk_w, torch.float32, T, self.k, "topk_w")
+        self._check_plan(dst_row, counts, pad_offsets)
+        grows = torch.empty_like(out_rows) if need_rows else None
+        gw = torch.empty(T, self.k, dtype=torch.float32, device=self.device) if need_w else None
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_combine_grad(self._h, grad_y.data_ptr(), out_rows.data_ptr(), dst_row.data_ptr(), topk_w.data_ptr(),
+                                             T, counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), out_rows.shape[0],
+                                             _ptr(grows), _ptr(gw), self._stream()))
+        return grows, gw
+
+    def route_topk_grad(self, logits: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor,
+                        grad_w: torch.Tensor) -> torch.Tensor:
+        """Gradient of route_topk's weights with respect to the logits, the picks being constants: [T, E] fp32."""
+        T = logits.shape[0]
+        self._check_rows(logits, torch.float32, None, self.E, "logits")
+        self._check_rows(topk_idx, torch.int32, T, self.k, "topk_idx")
+        self._check_rows(topk_w, torch.float32, T, self.k, "topk_w")
+        self._check_rows(grad_w, torch.float32, T, self.k, "grad_w")
+        gl = torch.empty(T, self.E, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_route_topk_grad(self._h, logits.data_ptr(), topk_idx.data_ptr(), topk_w.data_ptr(),
+                                                grad_w.data_ptr(), T, gl.data_ptr(), self._stream()))
+        return gl
+
+    # ------------------------------------------------------------------ 8-bit integers
+    def _rows_of(self, t: torch.Tensor, dtype, what: str) -> torch.Tensor:
+        """[rows, cols] with adjacent columns; rows may lie further apart."""
+        if t.device != self.device or t.dtype != dtype or t.dim() != 2:
+            raise ValueError(f"{what}: expected a [rows, cols] {dtype} tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{what}: the elements of a row must be adjacent (strides {t.stride()})")
+        return t
+
+    @staticmethod
+    def _row_stride(t: torch.Tensor) -> int:
+        """Elements between rows; of a single row, whose stride torch leaves open, enough to pass for one on any boundary."""
+        return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+    def quantize_rows(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Rows of bf16 -> (q [rows, cols] int8 with rows on 128-byte strides, scale [rows] fp32): the values are q * scale.
+        A row that holds an infinity or a NaN has scale NaN and q 0."""
+        x = self._rows_of(x, torch.bfloat16, "x")
+        n, cols = x.shape
+        q = torch.empty(n, (cols + 127) // 128 * 128, dtype=torch.int8, device=self.device)[:, :cols]
+        scale = torch.empty(n, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_quantize_rows_int8(self._h, x.data_ptr(), n, cols, self._row_stride(x), q.data_ptr(),
+                                                   (cols + 127) // 128 * 128, scale.data_ptr(), self._stream()))
+        return q, scale
+
+    def _int8_args(self, wq: torch.Tensor, w_scale: torch.Tensor, cols: int, n_rows: int, out: Optional[torch.Tensor]):
+        wq = self._rows_of(wq, torch.int8, "wq")
+        n_out = wq.shape[0]
+        if wq.shape[1] != cols:
+            raise ValueError(f"wq {tuple(wq.shape)} for rows of {cols}")
+        self._check_in(w_scale, torch.float32, "w_scale")
+        if w_scale.numel() != n_out:
+            raise ValueError(f"{w_scale.numel()} scales for {n_out} output channels")
+        if out is None:
+            out = torch.empty(n_rows, (n_out + 7) // 8 * 8, dtype=torch.bfloat16, device=self.device)[:, :n_out]
+        else:
+            out = self._rows_of(out, torch.bfloat16, "out")
+            if tuple(out.shape) != (n_rows, n_out):
+                raise ValueError(f"out {tuple(out.shape)}, expected {(n_rows, n_out)}")
+        return wq, n_out, out
+
+    def int8_matmul(self, xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """bf16(float(xq . wq^T) * x_scale[row] * w_scale[column]): xq [rows, cols] and wq [n_out, cols] int8 with rows on 16-byte
+        boundaries (views of wider tensors will do; quantize_rows gives such rows), fp32 scales.  Any layer serves."""
+        xq = self._rows_of(xq, torch.int8, "xq")
+        n, cols = xq.shape
+        self._check_in(x_scale, torch.float32, "x_scale")
+        if x_scale.numel() != n:
+            raise ValueError(f"{x_scale.numel()} scales for {n} rows")
+        wq, n_out, out = self._int8_args(wq, w_scale, cols, n, out)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_int8_matmul(self._h, xq.data_ptr(), self._row_stride(xq), x_scale.data_ptr(), n, wq.data_ptr(),
+                                            self._row_stride(wq), w_scale.data_ptr(), n_out, cols, out.data_ptr(),
+                                            self._row_stride(out), self._stream()))
+        return out
+
+    def int8_linear(self, x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """int8_matmul of bf16 rows x, quantised per token (quantize_rows) in the same call."""
+        x = self._rows_of(x, torch.bfloat16, "x")
+        n, cols = x.shape
+        wq, n_out, out = self._int8_args(wq, w_scale, cols, n, out)
+        nb = C.c_size_t()
+        L.check(self.lib.mg_int8_linear_ws_bytes(n, cols, C.byref(nb)))
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_int8_linear(self._h, x.data_ptr(), self._row_stride(x), n, wq.data_ptr(), self._row_stride(wq),
+                                            w_scale.data_ptr(), n_out, cols, ws.data_ptr(), nb.value, out.data_ptr(),
+                                            self._row_stride(out), self._stream()))
+        return out
+
+    def permute_rows_int8(self, xq: torch.Tensor, x_scale: torch.Tensor, dst_row: torch.Tensor, rows_padded: int):
+        """-> expert-sorted quantised rows [rows_padded, H] and their scales; rows no pick points at are left open."""
+        self._check_rows(xq, torch.int8, None, self.H, "xq")
+        self._check_in(x_scale, torch.float32, "x_scale")
+        self._check_rows(dst_row, torch.int32, xq.shape[0], self.k, "dst_row")
+        if x_scale.numel() != xq.shape[0]:
+            raise ValueError(f"{x_scale.numel()} scales for {xq.shape[0]} rows")
+        q = torch.empty(rows_padded, self.H, dtype=torch.int8, device=self.device)
+        s = torch.empty(rows_padded, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_permute_rows_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), dst_row.data_ptr(), xq.shape[0],
+                                                  q.data_ptr(), s.data_ptr(), self._stream()))
+        return q, s
+
+    def expert_ffn_int8(self, perm_q: torch.Tensor, perm_scale: torch.Tensor, pad_offsets: torch.Tensor, counts: torch.Tensor,
+                        dst_row: torch.Tensor):
+        """-> (h_buf [rows, I] bf16, out_rows [rows, H] bf16) of an int8 layer's experts; zeros in the rows no pick points at."""
+        rows = perm_q.shape[0]
+        self._check_rows(perm_q, torch.int8, None, self.H, "perm_q")
+        self._check_in(perm_scale, torch.float32, "perm_scale")
+        self._check_rows(dst_row, torch.int32, None, self.k, "dst_row")
+        self._check_plan(dst_row, counts, pad_offsets)
+        if perm_scale.numel() != rows or counts.numel() != self.e_local:
+            raise ValueError(f"{perm_scale.numel()} scales for {rows} rows, {counts.numel()} counts for {self.e_local} experts")
+        hbuf = torch.zeros(rows, self.I, dtype=torch.bfloat16, device=self.device)
+        out = torch.zeros(rows, self.H, dtype=torch.bfloat16, device=self.device)
+        hq = torch.empty(rows, self.I, dtype=torch.int8, device=self.device)
+        hs = torch.empty(rows, dtype=torch.float32, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_expert_ffn_int8(self._h, perm_q.data_ptr(), perm_scale.data_ptr(), pad_offsets.data_ptr(),
+                                                counts.data_ptr(), rows, dst_row.data_ptr(), dst_row.shape[0],
+                                                self.packed.data_ptr(), hbuf.data_ptr(), hq.data_ptr(), hs.data_ptr(),
+                                                out.data_ptr(), self._stream()))
+        return hbuf, out
+
+    def shared_ffn_int8(self, xq: torch.Tensor, x_scale: torch.Tensor) -> torch.Tensor:
+        self._check_rows(xq, torch.int8, None, self.H, "xq")
+        self._check_in(x_scale, torch.float32, "x_scale")
+        T = xq.shape[0]
+        if x_scale.numel() != T:
+            raise ValueError(f"{x_scale.numel()} scales for {T} rows")
+        hs = torch.empty(T, self.Is, dtype=torch.bfloat16, device=self.device)
+        hq = torch.empty(T, self.Is, dtype=torch.int8, device=self.device)
+        sc = torch.empty(T, dtype=torch.float32, device=self.device)
+        out = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
+        with torch.cuda.device(self.device):
+            L.check(self.lib.mg_shared_ffn_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), T, self.packed.data_ptr(),
+                                                hs.data_ptr(), hq.data_ptr(), sc.data_ptr(), out.data_ptr(), self._stream()))
+        return out
 
     @contextlib.contextmanager
     def job_counters(self, buf: torch.Tensor):

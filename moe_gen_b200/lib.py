@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("MOEGEN_B200_LIB") or os.path.join(_PKG, "libmoegen_b2
 
 GATE_SOFTMAX_GREEDY, GATE_SOFTMAX_GROUP_MAX, GATE_SIGMOID_NOAUX_TC, GATE_SOFTMAX_TOPK_RENORM = 0, 1, 2, 3
 COMBINE_FP32, COMBINE_BF16_PROD, COMBINE_BF16_SEQ = 0, 1, 2
-WEIGHT_BF16, WEIGHT_FP8_BLOCK128 = 0, 1
+WEIGHT_BF16, WEIGHT_FP8_BLOCK128, WEIGHT_INT8_CHANNEL = 0, 1, 2
 DEV_OK, DEV_WAIT_TIMEOUT, DEV_CAPACITY, DEV_BOUNDS = 0, 1, 2, 3
 OPT_FP8_MODE = 1
 OPT_PAIR_GEMM = 2
@@ -69,6 +69,17 @@ SIGNATURES = {
     "mg_set_job_counters": [_vp, _vp],
     "mg_shared_ffn": [_vp, _vp, _i64, _vp, _vp, _vp, _vp],
     "mg_combine": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
+    "mg_quantize_rows_int8": [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp],
+    "mg_int8_matmul": [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
+    "mg_int8_linear_ws_bytes": [_i64, _i64, _P(_sz)],
+    "mg_int8_linear": [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _sz, _vp, _i64, _vp],
+    "mg_permute_rows_int8": [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
+    "mg_expert_ffn_int8": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mg_shared_ffn_int8": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mg_permute_rows_padded": [_vp, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _vp],
+    "mg_permute_rows_grad": [_vp, _vp, _vp, _i64, _vp, _vp],
+    "mg_combine_grad": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _vp, _vp],
+    "mg_route_topk_grad": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
     "mg_moe_forward": [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
     "mg_host_chunk_plan": [_i64, _i64, _P(_i64), _i32, _P(_i32)],
     "mg_host_workspace_bytes": [_vp, _i64, _i64, _P(_sz)],
