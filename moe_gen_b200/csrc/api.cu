@@ -888,8 +888,9 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t ldq = round_up(cols, 128);
   float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
-  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_ws, ldq, scale, st);
-  if (rc != MG_OK) return rc;
+  bool quantised;
+  rc = launch_int8_linear(h, d_x, ldx, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_ws, ldq, scale, d_out, ldo, st, &quantised);
+  if (rc != MG_OK || !quantised) return rc;
   h->chain = true;
   rc = launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
   h->chain = false;

@@ -12,7 +12,7 @@ namespace mg {
 
 namespace {
 
-constexpr int kQuantVecs = 8;            // 16-byte vectors of a row a thread keeps in registers
+constexpr int kQuantVecs = 8;            // 16-byte vectors of a row a thread keeps in registers at most
 constexpr float kQuantFloor = 7.888609052210118e-31f;       // 2^-100
 
 __device__ __forceinline__ void row_scale(uint32_t amax_bits, float& scale, float& inv) {
@@ -44,6 +44,7 @@ __device__ __forceinline__ uint32_t block_amax(uint32_t pairs, uint32_t* s_max) 
 
 // A block per row, or per entry of `list` (rows of the experts' buffers; a negative one is skipped).  Rows of whole 16-byte
 // vectors; what a thread holds stays in registers between the maximum and the rounding.
+template <int VECS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int64_t ldx, int vecs, const int32_t* list,
                                                             uint2* q, int64_t ldq, float* scale) {
   chain_wait();
@@ -52,29 +53,147 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int6
   const int64_t row = list != nullptr ? list[blockIdx.x] : static_cast<int64_t>(blockIdx.x);
   if (row < 0) return;
   const uint4* src = x + row * ldx;
-  uint4 keep[kQuantVecs];
+  uint4 keep[VECS];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i) {
+  for (int i = 0; i < VECS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     keep[i] = make_uint4(0u, 0u, 0u, 0u);
     if (v < vecs) keep[i] = src[v];
   }
 #pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i)
+  for (int i = 0; i < VECS; ++i)
     m = __vmaxu2(__vmaxu2(m, keep[i].x & 0x7FFF7FFFu), __vmaxu2(keep[i].y & 0x7FFF7FFFu,
                  __vmaxu2(keep[i].z & 0x7FFF7FFFu, keep[i].w & 0x7FFF7FFFu)));
   float s, inv;
   row_scale(block_amax(m, s_max), s, inv);
   const bool dead = inv == 0.0f;
 #pragma unroll
-  for (int i = 0; i < kQuantVecs; ++i) {
+  for (int i = 0; i < VECS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v < vecs)
       q[row * ldq + v] = dead ? make_uint2(0u, 0u)
                               : make_uint2(quantise4(keep[i].x, keep[i].y, inv), quantise4(keep[i].z, keep[i].w, inv));
   }
   if (threadIdx.x == 0) scale[row] = s;
+}
+
+// A product of up to kFewRows rows of x in one launch: every block quantises them into shared memory, and a warp multiplies two
+// weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a pair
+// of SMs for 256 weight rows); here every SM streams a share of the weights.
+constexpr int kFewRows = 8, kFewWarps = 8, kFewSmem = 96 * 1024;
+template <int M>
+__global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int rows, int cols,
+                                                                       const uint8_t* __restrict__ w, int64_t ldw,
+                                                                       const float* __restrict__ w_scale, int n_out,
+                                                                       __nv_bfloat16* __restrict__ out, int64_t ldo, bool wide) {
+  extern __shared__ __align__(16) uint8_t s_q[];           // [M][chunks of 16 bytes], zeros behind the last element
+  __shared__ float s_scale[M];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (cols + 15) >> 4;
+  const int n0 = (blockIdx.x * kFewWarps + warp) * 2;
+  // this warp's weights on their way while x is quantised
+  if (n0 < n_out) {
+    const uint8_t* p = w + static_cast<int64_t>(min(n0 + (lane & 1), n_out - 1)) * ldw;
+    for (int c = (lane >> 1) * 128; c < cols; c += 16 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
+  }
+  for (int r = warp; r < M; r += kFewWarps) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(s_q + static_cast<size_t>(r) * chunks * 16);
+    if (r >= rows) {
+      for (int c = lane; c < chunks * 4; c += 32) q[c] = 0u;
+      if (lane == 0) s_scale[r] = 0.f;
+      continue;
+    }
+    const uint16_t* src = x + r * ldx;
+    uint32_t m = 0;
+    if (wide) {
+      const uint4* v = reinterpret_cast<const uint4*>(src);
+      for (int c = lane; c < cols >> 3; c += 32) {
+        const uint4 a = __ldg(v + c);
+        m = __vmaxu2(__vmaxu2(m, a.x & 0x7FFF7FFFu), __vmaxu2(a.y & 0x7FFF7FFFu, __vmaxu2(a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu)));
+      }
+      m = max(m & 0xFFFFu, m >> 16);
+    } else {
+      for (int c = lane; c < cols; c += 32) m = max(m, __ldg(src + c) & 0x7FFFu);
+    }
+    float scale, inv;
+    row_scale(__reduce_max_sync(0xFFFFFFFFu, m), scale, inv);
+    if (lane == 0) s_scale[r] = scale;
+    const bool dead = inv == 0.f;
+    if (wide) {
+      const uint4* v = reinterpret_cast<const uint4*>(src);
+      for (int c = lane; c < chunks * 2; c += 32) {
+        uint2 o = make_uint2(0u, 0u);
+        if (c < cols >> 3 && !dead) {
+          const uint4 a = __ldg(v + c);
+          o = make_uint2(quantise4(a.x, a.y, inv), quantise4(a.z, a.w, inv));
+        }
+        reinterpret_cast<uint2*>(q)[c] = o;
+      }
+    } else {
+      uint8_t* b = reinterpret_cast<uint8_t*>(q);
+      for (int c = lane; c < chunks * 16; c += 32) {
+        uint32_t lo = 0u, hi;
+        if (c < cols && !dead) quantise2(__ldg(src + c), inv, lo, hi);
+        b[c] = static_cast<uint8_t>(lo);
+      }
+    }
+  }
+  __syncthreads();
+  if (n0 >= n_out) return;
+  const bool two = n0 + 1 < n_out;
+  const uint8_t* w0 = w + static_cast<int64_t>(n0) * ldw;
+  const uint8_t* w1 = w0 + (two ? ldw : 0);
+  int acc0[M], acc1[M];
+#pragma unroll
+  for (int r = 0; r < M; ++r) acc0[r] = acc1[r] = 0;
+  auto dot = [&](int c, const uint4& a, const uint4& b) {
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      const uint4 q = *reinterpret_cast<const uint4*>(s_q + (static_cast<size_t>(r) * chunks + c) * 16);
+      acc0[r] = __dp4a(static_cast<int>(a.x), static_cast<int>(q.x), acc0[r]);
+      acc0[r] = __dp4a(static_cast<int>(a.y), static_cast<int>(q.y), acc0[r]);
+      acc0[r] = __dp4a(static_cast<int>(a.z), static_cast<int>(q.z), acc0[r]);
+      acc0[r] = __dp4a(static_cast<int>(a.w), static_cast<int>(q.w), acc0[r]);
+      acc1[r] = __dp4a(static_cast<int>(b.x), static_cast<int>(q.x), acc1[r]);
+      acc1[r] = __dp4a(static_cast<int>(b.y), static_cast<int>(q.y), acc1[r]);
+      acc1[r] = __dp4a(static_cast<int>(b.z), static_cast<int>(q.z), acc1[r]);
+      acc1[r] = __dp4a(static_cast<int>(b.w), static_cast<int>(q.w), acc1[r]);
+    }
+  };
+  const int whole = cols >> 4;
+  int c = lane;
+  for (; c + 96 < whole; c += 128) {
+    uint4 a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __ldg(reinterpret_cast<const uint4*>(w0) + c + 32 * i);
+      b[i] = __ldg(reinterpret_cast<const uint4*>(w1) + c + 32 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dot(c + 32 * i, a[i], b[i]);
+  }
+  for (; c < whole; c += 32) dot(c, __ldg(reinterpret_cast<const uint4*>(w0) + c), __ldg(reinterpret_cast<const uint4*>(w1) + c));
+  if (c == whole && whole < chunks) {                      // the bytes behind the last whole chunk, one by one
+    uint32_t a[4] = {0u, 0u, 0u, 0u}, b[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (whole * 16 + i < cols) {
+        a[i >> 2] |= static_cast<uint32_t>(w0[whole * 16 + i]) << (8 * (i & 3));
+        b[i >> 2] |= static_cast<uint32_t>(w1[whole * 16 + i]) << (8 * (i & 3));
+      }
+    }
+    dot(whole, make_uint4(a[0], a[1], a[2], a[3]), make_uint4(b[0], b[1], b[2], b[3]));
+  }
+  const float s0 = w_scale[n0], s1 = two ? w_scale[n0 + 1] : 0.f;
+#pragma unroll
+  for (int r = 0; r < M; ++r) {
+    const int a = __reduce_add_sync(0xFFFFFFFFu, acc0[r]), b = __reduce_add_sync(0xFFFFFFFFu, acc1[r]);
+    if (lane == 0 && r < rows) {
+      out[r * ldo + n0] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(a), s_scale[r]), s0));
+      if (two) out[r * ldo + n0 + 1] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(b), s_scale[r]), s1));
+    }
+  }
 }
 
 // Rows of any length, alignment and stride, element by element, read twice.
@@ -111,14 +230,55 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
     // four vectors to a thread, so that short rows do not leave most of a block idle
     int threads = static_cast<int>((vecs + 127) / 128) * 32;
     if (threads > 256) threads = 256;
-    MG_CUDA(launch_chained(h, quantize_rows_kernel, static_cast<unsigned>(n), threads, 0, st, static_cast<const uint4*>(x),
-                           ldx / 8, static_cast<int>(vecs), list, static_cast<uint2*>(q), ldq / 8, scale));
+#define MG_QUANT(V)                                                                                                          \
+  MG_CUDA(launch_chained(h, quantize_rows_kernel<V>, static_cast<unsigned>(n), threads, 0, st, static_cast<const uint4*>(x), \
+                         ldx / 8, static_cast<int>(vecs), list, static_cast<uint2*>(q), ldq / 8, scale))
+    if (vecs <= 4 * threads) MG_QUANT(4); else MG_QUANT(kQuantVecs);
+#undef MG_QUANT
     return MG_OK;
   }
   MG_REQUIRE(list == nullptr, MG_ERR_SHAPE, "quantise: listed rows of %lld elements", static_cast<long long>(cols));
   MG_CUDA(launch_chained(h, quantize_rows_any_kernel, static_cast<unsigned>(n), 256, 0, st, static_cast<const uint16_t*>(x), ldx,
                          static_cast<int>(cols), static_cast<uint8_t*>(q), ldq, scale));
   return MG_OK;
+}
+
+// true: launched (few rows, whose quantised form fits in shared memory)
+static bool few_rows(int64_t rows, int64_t cols) {
+  int m = 1;
+  while (m < rows) m *= 2;
+  return rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem;
+}
+template <int M>
+static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
+                      int64_t n_out, int64_t cols, void* out, int64_t ldo, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(M * round_up(cols, 16));
+  static bool done[64];
+  if (smem > 48 * 1024 - 64 && !(h->device >= 0 && h->device < 64 && done[h->device])) {
+    MG_CUDA(cudaFuncSetAttribute(int8_few_rows_kernel<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
+    if (h->device >= 0 && h->device < 64) done[h->device] = true;
+  }
+  const bool wide = cols % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  int8_few_rows_kernel<M><<<static_cast<unsigned>((n_out + 2 * kFewWarps - 1) / (2 * kFewWarps)), kFewWarps * 32, smem, st>>>(
+      static_cast<const uint16_t*>(x), ldx, static_cast<int>(rows), static_cast<int>(cols), static_cast<const uint8_t*>(wq), ldw,
+      w_scale, static_cast<int>(n_out), static_cast<__nv_bfloat16*>(out), ldo, wide);
+  MG_CUDA(cudaGetLastError());
+  return MG_OK;
+}
+
+// bf16 rows: few of them in one launch, else quantised into `ws` (ldq bytes apart, scales in `scale`) and multiplied there
+int launch_int8_linear(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
+                       int64_t n_out, int64_t cols, void* ws, int64_t ldq, float* scale, void* out, int64_t ldo, cudaStream_t st,
+                       bool* quantised) {
+  *quantised = false;
+  if (few_rows(rows, cols)) {
+    if (rows == 1) return launch_few<1>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+    if (rows == 2) return launch_few<2>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+    if (rows <= 4) return launch_few<4>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+    return launch_few<8>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  }
+  *quantised = true;
+  return launch_quantize_rows(h, x, rows, cols, ldx, nullptr, ws, ldq, scale, st);
 }
 
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,

@@ -929,12 +929,16 @@ __global__ void __launch_bounds__(kPlanTokens) plan_place_kernel(const int32_t* 
   }
 }
 
-constexpr int kGapRows = 8;          // consecutive rows a warp looks at before the next warp's
-// blocks of so many warps that write zeros into the gaps of n_rows rows
-static unsigned gap_zero_blocks(const Handle* h, int64_t n_rows, int warps) {
-  const int64_t runs = (n_rows + kGapRows - 1) / kGapRows, want = (runs + warps - 1) / warps;
-  const int64_t most = static_cast<int64_t>(h->sm_count) * 16 / warps * 2;
-  return n_rows <= 0 ? 0u : static_cast<unsigned>(want < most ? want : most);
+// Blocks of so many warps that write zeros into the gaps of n_rows rows, and the consecutive rows a warp looks at before the next
+// warp's: few where there are few rows, so that all SMs write (8 always: Mixtral shape, 1 token, 1152 rows, 9 blocks and 20 us)
+struct GapPlan { unsigned blocks; int run; };
+static GapPlan gap_plan(const Handle* h, int64_t n_rows, int warps) {
+  if (n_rows <= 0) return {0u, 1};
+  const int64_t most = static_cast<int64_t>(h->sm_count) * 32;
+  int run = 1;
+  while (run < 8 && n_rows > most * run) run *= 2;
+  const int64_t want = ((n_rows + run - 1) / run + warps - 1) / warps, blocks = (most + warps - 1) / warps;
+  return {static_cast<unsigned>(want < blocks ? want : blocks), run};
 }
 
 // vectors [v_begin, v_end) of a row, read once, to the k places row_of(pick, entry of the pick) names (nullptr: none); lane j
@@ -1296,13 +1300,13 @@ int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, 
 // The scatter with zeros in the rows that hold no pick: blocks behind those of the scatter write them.  A row is a gap if it
 // lies behind the rows of its expert's segment or behind the last segment; a lane looks one row up, the warp writes.
 __device__ __forceinline__ void zero_gap_rows(uint4* rows, int64_t n_rows, int vec_per_row, const int32_t* counts, const int32_t* pad,
-                                              int n, int64_t warp, int64_t n_warps, int32_t* s_pad) {
+                                              int n, int run, int64_t warp, int64_t n_warps, int32_t* s_pad) {
   for (int i = threadIdx.x; i <= n; i += blockDim.x) s_pad[i] = pad[i];
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  for (int64_t r0 = warp * kGapRows; r0 < n_rows; r0 += n_warps * kGapRows) {
+  for (int64_t r0 = warp * run; r0 < n_rows; r0 += n_warps * run) {
     const int64_t r = r0 + lane;
-    bool gap = lane < kGapRows && r < n_rows;
+    bool gap = lane < run && r < n_rows;
     if (gap && r < s_pad[n]) {
       int lo = 0, hi = n;
       while (hi - lo > 1) {
@@ -1323,11 +1327,12 @@ __global__ void __launch_bounds__(256) permute_rows_padded_kernel(const uint4* _
                                                                   int64_t T, int k, int vec_per_row, int slices, int v_chunk,
                                                                   unsigned copy_blocks, const int32_t* __restrict__ counts,
                                                                   const int32_t* __restrict__ pad, int n, int64_t n_rows,
-                                                                  uint4* __restrict__ rows, Guard guard) {
+                                                                  int run, uint4* __restrict__ rows, Guard guard) {
   __shared__ int32_t s_pad[kMaxExperts + 1];
   const int lane = threadIdx.x & 31;
   if (blockIdx.x >= copy_blocks) {
-    zero_gap_rows(rows, n_rows, vec_per_row, counts, pad, n, static_cast<int64_t>(blockIdx.x - copy_blocks) * 8 + (threadIdx.x >> 5),
+    zero_gap_rows(rows, n_rows, vec_per_row, counts, pad, n, run,
+                  static_cast<int64_t>(blockIdx.x - copy_blocks) * 8 + (threadIdx.x >> 5),
                   static_cast<int64_t>(gridDim.x - copy_blocks) * 8, s_pad);
     return;
   }
@@ -1345,10 +1350,11 @@ int launch_permute_rows_padded(const Handle* h, const void* x, const int32_t* ds
                                const int32_t* pad, int n, int64_t n_rows, void* rows, cudaStream_t st) {
   const int vpr = h->d.hidden / 8;
   const RowSlices rs = row_slices(h, T > 0 ? T : 1, vpr);
-  const unsigned copy_blocks = static_cast<unsigned>((T * rs.n + 7) / 8), gap_blocks = gap_zero_blocks(h, n_rows, 8);
-  if (copy_blocks + gap_blocks == 0) return MG_OK;
-  permute_rows_padded_kernel<<<copy_blocks + gap_blocks, 256, 0, st>>>(
-      static_cast<const uint4*>(x), dst_row, T, h->d.top_k, vpr, rs.n, rs.v_chunk, copy_blocks, counts, pad, n, n_rows,
+  const unsigned copy_blocks = static_cast<unsigned>((T * rs.n + 7) / 8);
+  const GapPlan gaps = gap_plan(h, n_rows, 8);
+  if (copy_blocks + gaps.blocks == 0) return MG_OK;
+  permute_rows_padded_kernel<<<copy_blocks + gaps.blocks, 256, 0, st>>>(
+      static_cast<const uint4*>(x), dst_row, T, h->d.top_k, vpr, rs.n, rs.v_chunk, copy_blocks, counts, pad, n, n_rows, gaps.run,
       static_cast<uint4*>(rows), Guard{h->d_status, h->guard_rows, 1});
   MG_CUDA(cudaGetLastError());
   return MG_OK;
@@ -1362,13 +1368,13 @@ __global__ void __launch_bounds__(1024) combine_grad_kernel(const uint4* __restr
                                                             const int32_t* __restrict__ dst_row, const float* __restrict__ topk_w,
                                                             int64_t T, int k, int vec_per_row, bool round_w, int64_t n_rows,
                                                             const int32_t* __restrict__ counts, const int32_t* __restrict__ pad, int n,
-                                                            uint4* __restrict__ grad_rows, float* __restrict__ grad_w, Guard guard) {
+                                                            int run, uint4* __restrict__ grad_rows, float* __restrict__ grad_w, Guard guard) {
   __shared__ int32_t s_pad[kMaxExperts + 1];
   __shared__ float s_part[32][kMaxTopK];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int64_t t = blockIdx.x;
   if (t >= T) {
-    zero_gap_rows(grad_rows, n_rows, vec_per_row, counts, pad, n, (t - T) * warps + warp, (gridDim.x - T) * warps, s_pad);
+    zero_gap_rows(grad_rows, n_rows, vec_per_row, counts, pad, n, run, (t - T) * warps + warp, (gridDim.x - T) * warps, s_pad);
     return;
   }
   int32_t my_dst = -1;
@@ -1451,13 +1457,13 @@ int launch_combine_grad(const Handle* h, const void* gy, const void* out_rows, c
   int threads = 128;                       // 16 warps per SM at least, as far as a row has vectors for them
   while (threads < 1024 && threads < vpr && T * threads < static_cast<int64_t>(h->sm_count) * 512) threads *= 2;
   if (threads > vpr) threads = vpr;
-  const unsigned gaps = grad_rows != nullptr && counts != nullptr ? gap_zero_blocks(h, n_rows, threads / 32) : 0;
-  const int64_t blocks = (grad_rows != nullptr || grad_w != nullptr ? T : 0) + gaps;
+  const GapPlan gaps = gap_plan(h, grad_rows != nullptr && counts != nullptr ? n_rows : 0, threads / 32);
+  const int64_t blocks = (grad_rows != nullptr || grad_w != nullptr ? T : 0) + gaps.blocks;
   if (blocks == 0) return MG_OK;
 #define MG_GRAD_CASE(R, W)                                                                                             \
   combine_grad_kernel<R, W><<<static_cast<unsigned>(blocks), threads, 0, st>>>(                                        \
       static_cast<const uint4*>(gy), static_cast<const uint4*>(out_rows), dst_row, w, T, h->d.top_k, vpr,              \
-      h->d.combine_mode != MG_COMBINE_FP32, n_rows, counts, pad, n, static_cast<uint4*>(grad_rows), grad_w,            \
+      h->d.combine_mode != MG_COMBINE_FP32, n_rows, counts, pad, n, gaps.run, static_cast<uint4*>(grad_rows), grad_w,            \
       Guard{h->d_status, h->guard_rows, 1})
   if (grad_rows != nullptr && grad_w != nullptr) MG_GRAD_CASE(true, true);
   else if (grad_rows != nullptr) MG_GRAD_CASE(true, false);
@@ -1792,7 +1798,9 @@ int launch_combine_peers(const Handle* h, const PeerPtrs& peers, const int32_t* 
 //            and is not summed up from terms that cancel
 //   sigmoid  gl_i = gs_i s_i (1 - s_i), with s (1 - s) = e / (1 + e)^2, e = exp(-|l|), which does not cancel either
 // A pick of weight 0 competed from a masked group (its score is the constant 0) and passes nothing on.  A warp per token; softmax
-// reads the row of logits once, sigmoid the picks' alone; the row of gradients is written once.
+// reads the row of logits once, sigmoid the picks' alone; the row of gradients is written once, from a row in shared memory that
+// the picks' lanes scatter into (every lane comparing its experts with every pick took 35 us for 65536 tokens of 256 experts
+// and 8 picks, where this takes 24).
 template <bool SIGMOID>
 __global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __restrict__ logits, const int32_t* __restrict__ topk_idx,
                                                               const float* __restrict__ topk_w, const float* __restrict__ grad_w,
@@ -1802,6 +1810,8 @@ __global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __res
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (t >= T) return;
   constexpr int QUADS = kMaxExperts / 128;             // of four experts, per lane
+  __shared__ __align__(16) float s_row[8][kMaxExperts];
+  float4* mine = reinterpret_cast<float4*>(s_row[threadIdx.x >> 5]);
   const float4* row = reinterpret_cast<const float4*>(logits + t * E);
   const int quads = E >> 2;
   int32_t e = -1;
@@ -1847,26 +1857,35 @@ __global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __res
     D = warp_sum_f(gp * p);
   }
   if (SIGMOID) gp *= ex / ((1.0f + ex) * (1.0f + ex));
+  // an expert that several picks name: the first of them carries the sum, in the order of the slots
+  const uint32_t peers = __match_any_sync(0xFFFFFFFFu, e);
+  if (__any_sync(0xFFFFFFFFu, e >= 0 && (peers & (peers - 1)) != 0)) {
+    float sum = 0.f;
+    for (int j = 0; j < k; ++j) {
+      const float gj = __shfl_sync(0xFFFFFFFFu, gp, j);
+      if ((peers >> j) & 1u) sum += gj;
+    }
+    gp = sum;
+    if ((peers & ((1u << lane) - 1u)) != 0) e = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i)
+    if (i * 32 + lane < quads) mine[i * 32 + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncwarp();
+  if (e >= 0) s_row[threadIdx.x >> 5][e] = gp;
+  __syncwarp();
   float4* out = reinterpret_cast<float4*>(grad_logits + t * E);
 #pragma unroll
   for (int i = 0; i < QUADS; ++i) {
     const int q = i * 32 + lane;
-    if (i * 32 >= quads) break;
-    float g[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < k; ++j) {
-      const int32_t ej = __shfl_sync(0xFFFFFFFFu, e, j);
-      const float gj = __shfl_sync(0xFFFFFFFFu, gp, j);
-      if ((ej >> 2) == q) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if ((ej & 3) == u) g[u] += gj;
+    if (q < quads) {
+      float4 g = mine[q];
+      if (!SIGMOID) {
+        g.x = s[i].x * inv_sum * (g.x - D); g.y = s[i].y * inv_sum * (g.y - D);
+        g.z = s[i].z * inv_sum * (g.z - D); g.w = s[i].w * inv_sum * (g.w - D);
       }
+      out[q] = g;
     }
-    if (!SIGMOID) {
-      g[0] = s[i].x * inv_sum * (g[0] - D); g[1] = s[i].y * inv_sum * (g[1] - D);
-      g[2] = s[i].z * inv_sum * (g[2] - D); g[3] = s[i].w * inv_sum * (g[3] - D);
-    }
-    if (q < quads) out[q] = make_float4(g[0], g[1], g[2], g[3]);
   }
 }
 

@@ -21,6 +21,10 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_NO_SWITCH = contextlib.nullcontext()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class MoELayer:
     def __init__(self, *, hidden: int, inter: int, n_experts: int, top_k: int, inter_shared: int = 0,
                  n_group: int = 1, topk_group: int = 1, gating: int = L.GATE_SOFTMAX_GREEDY,
@@ -31,6 +35,7 @@ class MoELayer:
             raise RuntimeError("moe_gen_b200 needs a CUDA device (sm_100a); there is no CPU path")
         self.lib = L.load()
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        self._index = torch.cuda.current_device() if self.device.index is None else self.device.index
         self.desc = L.LayerDesc(C.sizeof(L.LayerDesc), hidden, inter, inter_shared, n_experts, top_k, n_group,
                                 topk_group, gating, int(bool(norm_topk_prob)), float(routed_scale),
                                 weight_format, combine_mode, ep_rank, ep_size)
@@ -38,7 +43,7 @@ class MoELayer:
         self.e_local = n_experts // ep_size
         self.expert_lo = ep_rank * self.e_local
         self._h = C.c_void_p()
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_create(C.byref(self.desc), C.byref(self._h)))
             n = C.c_size_t()
             L.check(self.lib.mg_packed_weight_bytes(self._h, C.byref(n)))
@@ -48,6 +53,7 @@ class MoELayer:
         self.bias: Optional[torch.Tensor] = None
         self._ws: Optional[torch.Tensor] = None
         self._ws_tokens = -1
+        self._size = C.c_size_t()
         self.options = {}                       # option id -> last value set
 
     # ------------------------------------------------------------------ lifetime
@@ -62,9 +68,13 @@ class MoELayer:
         except Exception:
             pass
 
-    @staticmethod
-    def _stream() -> int:
-        return torch.cuda.current_stream().cuda_stream
+    # Entering torch.cuda.device and asking for torch.cuda.current_stream() takes 1.5 and 3.3 us of a call whose launch takes 3:
+    # the device is set where it is another one only, and the stream's handle is read without making a Stream of it.
+    def _on_device(self):
+        return _NO_SWITCH if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+
+    def _stream(self) -> int:
+        return _raw_stream(self._index)
 
     def _check_in(self, t: torch.Tensor, dtype, what: str):
         if t.device != self.device or t.dtype != dtype or not t.is_contiguous():
@@ -103,7 +113,7 @@ class MoELayer:
             for s, m in zip(sc, mats):
                 if s.numel() != m.shape[0]:
                     raise ValueError(f"int8 expert matrix of {m.shape[0]} rows with {s.numel()} scales")
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_pack_expert(self._h, local_expert, mats[0].data_ptr(), mats[1].data_ptr(),
                                             mats[2].data_ptr(), _ptr(sc[0]), _ptr(sc[1]), _ptr(sc[2]),
                                             self.packed.data_ptr(), self._stream()))
@@ -168,7 +178,7 @@ class MoELayer:
         T = x2.shape[0]
         ws = self._workspace(T)
         y = torch.empty_like(x2) if out is None else out
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_moe_forward(self._h, x2.data_ptr(), T, self.gate_w.data_ptr(), _ptr(self.bias),
                                             self.packed.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(),
                                             self._stream()))
@@ -189,7 +199,7 @@ class MoELayer:
             raise ValueError(f"logits {tuple(logits.shape)}, expected {(T, self.E)}")
         ws = self._workspace(T)
         y = torch.empty_like(x2) if out is None else out
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_moe_forward_from_logits(self._h, x2.data_ptr(), T, logits.data_ptr(), _ptr(self.bias),
                                                         self.packed.data_ptr(), ws.data_ptr(), ws.numel(),
                                                         y.data_ptr(), self._stream()))
@@ -206,7 +216,7 @@ class MoELayer:
         if weight.numel() != self.H:
             raise ValueError(f"norm weight has {weight.numel()} elements, hidden size is {self.H}")
         y = torch.empty_like(x2) if out is None else out
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_rmsnorm(self._h, x2.data_ptr(), weight.data_ptr(), float(eps), x2.shape[0],
                                         y.data_ptr(), self._stream()))
         return y.view(x.shape)
@@ -227,7 +237,7 @@ class MoELayer:
         if getattr(self, "_xnorm", None) is None or self._xnorm.shape[0] < T:
             self._xnorm = torch.empty(max(T, 1), self.H, dtype=torch.bfloat16, device=self.device)
         y = torch.empty_like(h2) if out is None else out.reshape(-1, self.H)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_moe_block_forward(self._h, h2.data_ptr(), norm_weight.data_ptr(), float(eps), T,
                                                   self.gate_w.data_ptr(), _ptr(self.bias), self.packed.data_ptr(),
                                                   self._xnorm.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(),
@@ -259,7 +269,7 @@ class MoELayer:
             y_host = torch.empty_like(x_host, pin_memory=x_host.is_pinned())
         if T == 0:
             return y_host
-        with torch.cuda.device(self.device):
+        with self._on_device():
             n = C.c_size_t()
             L.check(self.lib.mg_host_workspace_bytes(self._h, T, chunk_tokens, C.byref(n)))
             if getattr(self, "_hws", None) is None or self._hws.numel() < n.value:
@@ -276,7 +286,7 @@ class MoELayer:
         self._check_in(x, torch.bfloat16, "hidden_states")
         T = x.shape[0]
         logits = torch.empty(T, self.E, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_gate_logits(self._h, x.data_ptr(), self.gate_w.data_ptr(), T, logits.data_ptr(),
                                             self._stream()))
         return logits
@@ -286,7 +296,7 @@ class MoELayer:
         T = logits.shape[0]
         idx = torch.empty(T, self.k, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.k, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_route_topk(self._h, logits.data_ptr(), _ptr(self.bias), T, idx.data_ptr(),
                                            w.data_ptr(), self._stream()))
         return idx, w
@@ -304,7 +314,7 @@ class MoELayer:
         n = C.c_size_t()
         L.check(self.lib.mg_route_fix_bytes(T, C.byref(n)))
         fix = torch.zeros(n.value // 4, dtype=torch.int32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_gate_route_topk(self._h, x.data_ptr(), self.gate_w.data_ptr(), _ptr(self.bias), T,
                                                 logits.data_ptr(), idx.data_ptr(), w.data_ptr(), fix.data_ptr(),
                                                 self._stream()))
@@ -323,7 +333,7 @@ class MoELayer:
         nb = C.c_size_t()
         L.check(self.lib.mg_plan_ws_bytes(self._h, T, C.byref(nb)))
         ws = torch.empty(max(nb.value, 4), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
+        with self._on_device():
             L.check(self.lib.mg_permute_plan(self._h, topk_idx.data_ptr(), T, expert_lo, n, counts.data_ptr(),
                                              offsets.data_ptr(), pad.data_ptr(), dst.data_ptr(), ws.data_ptr(),
                                              self._stream()))
@@ -337,7 +347,8 @@ class MoELayer:
 
     def _check_rows(self, t: torch.Tensor, dtype, rows: Optional[int], cols: int, what: str):
         self._check_in(t, dtype, what)
-        if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+        shape = t.shape
+        if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
             raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {('rows' if rows is None else rows, cols)}")
 
     def permute_rows(self, x: torch.Tensor, dst_row: torch.Tensor, rows_padded: int, counts: Optional[torch.Tensor] = None,
@@ -350,13 +361,13 @@ class MoELayer:
             self._check_rows(dst_row, torch.int32, x.shape[0], self.k, "dst_row")
             self._check_plan(dst_row, counts, pad_offsets)
             perm = torch.empty(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
-            with torch.cuda.device(self.device):
+            with self._on_device():
                 L.check(self.lib.mg_permute_rows_padded(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
                                                         counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), rows_padded,
                                                         perm.data_ptr(), self._stream()))
             return perm
         perm = torch.zeros(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_permute_rows(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
                                              perm.data_ptr(), self._stream()))
         return perm
@@ -368,7 +379,7 @@ class MoELayer:
         self._check_rows(dst_row, torch.int32, None, self.k, "dst_row")
         T = dst_row.shape[0]
         gx = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_permute_rows_grad(self._h, grad_rows.data_ptr(), dst_row.data_ptr(), T, gx.data_ptr(),
                                                   self._stream()))
         return gx
@@ -385,7 +396,7 @@ class MoELayer:
         self._check_plan(dst_row, counts, pad_offsets)
         grows = torch.empty_like(out_rows) if need_rows else None
         gw = torch.empty(T, self.k, dtype=torch.float32, device=self.device) if need_w else None
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_combine_grad(self._h, grad_y.data_ptr(), out_rows.data_ptr(), dst_row.data_ptr(), topk_w.data_ptr(),
                                              T, counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), out_rows.shape[0],
                                              _ptr(grows), _ptr(gw), self._stream()))
@@ -400,82 +411,75 @@ class MoELayer:
         self._check_rows(topk_w, torch.float32, T, self.k, "topk_w")
         self._check_rows(grad_w, torch.float32, T, self.k, "grad_w")
         gl = torch.empty(T, self.E, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_route_topk_grad(self._h, logits.data_ptr(), topk_idx.data_ptr(), topk_w.data_ptr(),
                                                 grad_w.data_ptr(), T, gl.data_ptr(), self._stream()))
         return gl
 
     # ------------------------------------------------------------------ 8-bit integers
-    def _rows_of(self, t: torch.Tensor, dtype, what: str) -> torch.Tensor:
-        """[rows, cols] with adjacent columns; rows may lie further apart."""
-        if t.device != self.device or t.dtype != dtype or t.dim() != 2:
+    def _rows_of(self, t: torch.Tensor, dtype, what: str) -> Tuple[int, int, int]:
+        """Rows, columns and elements between rows of a [rows, cols] tensor whose columns are adjacent; rows may lie further apart.
+        torch leaves the stride of a single row open: enough is named for it to pass for one on any boundary."""
+        if t.dtype != dtype or t.dim() != 2 or t.device != self.device:
             raise ValueError(f"{what}: expected a [rows, cols] {dtype} tensor on {self.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
+        n, cols = t.shape
+        step, inner = t.stride()
+        if cols > 1 and inner != 1:
             raise ValueError(f"{what}: the elements of a row must be adjacent (strides {t.stride()})")
-        return t
-
-    @staticmethod
-    def _row_stride(t: torch.Tensor) -> int:
-        """Elements between rows; of a single row, whose stride torch leaves open, enough to pass for one on any boundary."""
-        return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+        return n, cols, step if n > 1 else (cols + 15) // 16 * 16
 
     def quantize_rows(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """Rows of bf16 -> (q [rows, cols] int8 with rows on 128-byte strides, scale [rows] fp32): the values are q * scale.
         A row that holds an infinity or a NaN has scale NaN and q 0."""
-        x = self._rows_of(x, torch.bfloat16, "x")
-        n, cols = x.shape
-        q = torch.empty(n, (cols + 127) // 128 * 128, dtype=torch.int8, device=self.device)[:, :cols]
+        n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
+        ldq = (cols + 127) // 128 * 128
+        q = torch.empty(n, ldq, dtype=torch.int8, device=self.device)
         scale = torch.empty(n, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
-            L.check(self.lib.mg_quantize_rows_int8(self._h, x.data_ptr(), n, cols, self._row_stride(x), q.data_ptr(),
-                                                   (cols + 127) // 128 * 128, scale.data_ptr(), self._stream()))
-        return q, scale
+        with self._on_device():
+            L.check(self.lib.mg_quantize_rows_int8(self._h, x.data_ptr(), n, cols, ldx, q.data_ptr(), ldq, scale.data_ptr(),
+                                                   self._stream()))
+        return (q if ldq == cols else q[:, :cols]), scale
 
     def _int8_args(self, wq: torch.Tensor, w_scale: torch.Tensor, cols: int, n_rows: int, out: Optional[torch.Tensor]):
-        wq = self._rows_of(wq, torch.int8, "wq")
-        n_out = wq.shape[0]
-        if wq.shape[1] != cols:
+        n_out, w_cols, ldw = self._rows_of(wq, torch.int8, "wq")
+        if w_cols != cols:
             raise ValueError(f"wq {tuple(wq.shape)} for rows of {cols}")
         self._check_in(w_scale, torch.float32, "w_scale")
         if w_scale.numel() != n_out:
             raise ValueError(f"{w_scale.numel()} scales for {n_out} output channels")
         if out is None:
-            out = torch.empty(n_rows, (n_out + 7) // 8 * 8, dtype=torch.bfloat16, device=self.device)[:, :n_out]
-        else:
-            out = self._rows_of(out, torch.bfloat16, "out")
-            if tuple(out.shape) != (n_rows, n_out):
-                raise ValueError(f"out {tuple(out.shape)}, expected {(n_rows, n_out)}")
-        return wq, n_out, out
+            ldo = (n_out + 7) // 8 * 8
+            out = torch.empty(n_rows, ldo, dtype=torch.bfloat16, device=self.device)
+            return n_out, ldw, out if ldo == n_out else out[:, :n_out], ldo
+        rows, o_cols, ldo = self._rows_of(out, torch.bfloat16, "out")
+        if (rows, o_cols) != (n_rows, n_out):
+            raise ValueError(f"out {tuple(out.shape)}, expected {(n_rows, n_out)}")
+        return n_out, ldw, out, ldo
 
     def int8_matmul(self, xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """bf16(float(xq . wq^T) * x_scale[row] * w_scale[column]): xq [rows, cols] and wq [n_out, cols] int8 with rows on 16-byte
         boundaries (views of wider tensors will do; quantize_rows gives such rows), fp32 scales.  Any layer serves."""
-        xq = self._rows_of(xq, torch.int8, "xq")
-        n, cols = xq.shape
+        n, cols, ldx = self._rows_of(xq, torch.int8, "xq")
         self._check_in(x_scale, torch.float32, "x_scale")
         if x_scale.numel() != n:
             raise ValueError(f"{x_scale.numel()} scales for {n} rows")
-        wq, n_out, out = self._int8_args(wq, w_scale, cols, n, out)
-        with torch.cuda.device(self.device):
-            L.check(self.lib.mg_int8_matmul(self._h, xq.data_ptr(), self._row_stride(xq), x_scale.data_ptr(), n, wq.data_ptr(),
-                                            self._row_stride(wq), w_scale.data_ptr(), n_out, cols, out.data_ptr(),
-                                            self._row_stride(out), self._stream()))
+        n_out, ldw, out, ldo = self._int8_args(wq, w_scale, cols, n, out)
+        with self._on_device():
+            L.check(self.lib.mg_int8_matmul(self._h, xq.data_ptr(), ldx, x_scale.data_ptr(), n, wq.data_ptr(), ldw,
+                                            w_scale.data_ptr(), n_out, cols, out.data_ptr(), ldo, self._stream()))
         return out
 
     def int8_linear(self, x: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """int8_matmul of bf16 rows x, quantised per token (quantize_rows) in the same call."""
-        x = self._rows_of(x, torch.bfloat16, "x")
-        n, cols = x.shape
-        wq, n_out, out = self._int8_args(wq, w_scale, cols, n, out)
-        nb = C.c_size_t()
-        L.check(self.lib.mg_int8_linear_ws_bytes(n, cols, C.byref(nb)))
-        ws = torch.empty(nb.value, dtype=torch.uint8, device=self.device)
-        with torch.cuda.device(self.device):
-            L.check(self.lib.mg_int8_linear(self._h, x.data_ptr(), self._row_stride(x), n, wq.data_ptr(), self._row_stride(wq),
-                                            w_scale.data_ptr(), n_out, cols, ws.data_ptr(), nb.value, out.data_ptr(),
-                                            self._row_stride(out), self._stream()))
+        n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
+        n_out, ldw, out, ldo = self._int8_args(wq, w_scale, cols, n, out)
+        L.check(self.lib.mg_int8_linear_ws_bytes(n, cols, C.byref(self._size)))
+        ws = torch.empty(self._size.value, dtype=torch.uint8, device=self.device)
+        with self._on_device():
+            L.check(self.lib.mg_int8_linear(self._h, x.data_ptr(), ldx, n, wq.data_ptr(), ldw, w_scale.data_ptr(), n_out, cols,
+                                            ws.data_ptr(), self._size.value, out.data_ptr(), ldo, self._stream()))
         return out
 
     def permute_rows_int8(self, xq: torch.Tensor, x_scale: torch.Tensor, dst_row: torch.Tensor, rows_padded: int):
@@ -487,7 +491,7 @@ class MoELayer:
             raise ValueError(f"{x_scale.numel()} scales for {xq.shape[0]} rows")
         q = torch.empty(rows_padded, self.H, dtype=torch.int8, device=self.device)
         s = torch.empty(rows_padded, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_permute_rows_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), dst_row.data_ptr(), xq.shape[0],
                                                   q.data_ptr(), s.data_ptr(), self._stream()))
         return q, s
@@ -506,7 +510,7 @@ class MoELayer:
         out = torch.zeros(rows, self.H, dtype=torch.bfloat16, device=self.device)
         hq = torch.empty(rows, self.I, dtype=torch.int8, device=self.device)
         hs = torch.empty(rows, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_expert_ffn_int8(self._h, perm_q.data_ptr(), perm_scale.data_ptr(), pad_offsets.data_ptr(),
                                                 counts.data_ptr(), rows, dst_row.data_ptr(), dst_row.shape[0],
                                                 self.packed.data_ptr(), hbuf.data_ptr(), hq.data_ptr(), hs.data_ptr(),
@@ -523,7 +527,7 @@ class MoELayer:
         hq = torch.empty(T, self.Is, dtype=torch.int8, device=self.device)
         sc = torch.empty(T, dtype=torch.float32, device=self.device)
         out = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_shared_ffn_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), T, self.packed.data_ptr(),
                                                 hs.data_ptr(), hq.data_ptr(), sc.data_ptr(), out.data_ptr(), self._stream()))
         return out
@@ -551,7 +555,7 @@ class MoELayer:
         nb = C.c_size_t()
         L.check(self.lib.mg_dequant_ws_bytes(self._h, C.byref(nb)))
         deq = torch.empty(nb.value, dtype=torch.uint8, device=self.device) if (nb.value and predequant) else None
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_expert_ffn(self._h, perm_x.data_ptr(), pad_offsets.data_ptr(), counts.data_ptr(),
                                            rows, self.packed.data_ptr(), hbuf.data_ptr(), out.data_ptr(),
                                            _ptr(deq), self._stream()))
@@ -564,7 +568,7 @@ class MoELayer:
         T = x.shape[0]
         hs = torch.empty(T, self.Is, dtype=torch.bfloat16, device=self.device)
         out = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_shared_ffn(self._h, x.data_ptr(), T, self.packed.data_ptr(), hs.data_ptr(),
                                            out.data_ptr(), self._stream()))
         return out
@@ -573,7 +577,7 @@ class MoELayer:
                 topk_w: torch.Tensor, shared_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         T = topk_idx.shape[0]
         y = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_combine(self._h, out_rows.data_ptr(), dst_row.data_ptr(), topk_idx.data_ptr(),
                                         topk_w.data_ptr(), _ptr(shared_out), T, y.data_ptr(), self._stream()))
         return y
@@ -583,7 +587,7 @@ class MoELayer:
         q = q.to(self.device).contiguous()
         s = scale_inv.to(self.device, torch.float32).contiguous()
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-        with torch.cuda.device(self.device):
+        with self._on_device():
             L.check(self.lib.mg_dequant_fp8_block128(q.data_ptr(), s.data_ptr(), q.shape[0], q.shape[1],
                                                      out.data_ptr(), self._stream()))
         return out

@@ -101,7 +101,9 @@ def test_rows_of_any_stride_and_alignment(any_layer):
 MATMUL = [(1, 1, 1), (1, 16, 64), (2, 8, 128), (7, 255, 127), (8, 256, 128), (9, 257, 129), (17, 300, 384), (31, 512, 640), (32, 40, 1000),
           (33, 777, 1000), (64, 128, 1024), (65, 1000, 80), (97, 777, 1000), (128, 512, 2048), (160, 513, 256), (256, 256, 896),
           (257, 264, 272), (288, 256, 512), (289, 100, 144), (320, 384, 1408), (352, 256, 256), (383, 31, 300), (384, 512, 128),
-          (385, 512, 128), (700, 1030, 520), (1153, 96, 192)]
+          (385, 512, 128), (700, 1030, 520), (1153, 96, 192),
+          # few rows: one launch, as long as their quantised form fits in a block's shared memory
+          (1, 4096, 4096), (1, 33, 98304), (1, 8, 98305), (3, 19, 5001), (4, 50, 24576), (4, 3, 24577), (6, 130, 2049), (8, 20, 12288), (8, 21, 12289)]
 
 
 @pytest.mark.parametrize("m,n,k", MATMUL)
