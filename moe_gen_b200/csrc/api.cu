@@ -770,8 +770,7 @@ static int shared_ffn(Handle* h, const void* x, int64_t T, const void* packed, v
 // are quantised for them alone.
 static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, const int32_t* pad, const int32_t* counts,
                            int64_t rows_padded, const int32_t* dst_row, int64_t T, const void* packed, void* h_buf, void* h_q,
-                           float* h_s, void* out_rows, cudaStream_t st, int* launches, bool timed, int32_t* job_counters,
-                           bool chain_down) {
+                           float* h_s, void* out_rows, cudaStream_t st, int* launches, bool timed, int32_t* job_counters) {
   const mg_layer_desc& d = h->d;
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
@@ -786,7 +785,8 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
   rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, dst_row, h_q, d.inter, h_s, st);
   if (rc != MG_OK) return rc;
-  if (!chain_down) h->chain = false;
+  // chained at every size: the quantising kernel lies between the products (kUnchainedDownTokens; layer, us, unchained and so:
+  // V2-Lite 8 tokens 102 and 98, V2-236B 8 tokens 141 and 139, 64 tokens 309 and 307)
   p.a = h_q; p.lda = d.inter; p.a_scales = h_s; p.b = base + L.w2; p.ldb = d.inter;
   p.scales = reinterpret_cast<const float*>(base + L.s2); p.n_per_group = d.hidden; p.K = d.inter;
   p.out = out_rows; p.ldo = d.hidden; p.epilogue = EPI_PLAIN_BF16;
@@ -924,7 +924,7 @@ int mg_expert_ffn_int8(mg_handle hh, const void* d_perm_q, const float* d_perm_s
   int rc = zero_job_counters(h, st);
   if (rc != MG_OK) return rc;
   return expert_ffn_int8(h, d_perm_q, d_perm_scale, d_pad, d_counts, n_rows_padded, d_dst, T, d_packed, d_h_buf, d_h_q, d_h_scale,
-                         d_out_rows, st, nullptr, false, h->job_counters, true);
+                         d_out_rows, st, nullptr, false, h->job_counters);
 }
 
 int mg_shared_ffn_int8(mg_handle hh, const void* d_xq, const float* d_x_scale, int64_t T, const void* d_packed, void* d_hs,
@@ -1151,11 +1151,10 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   if (rc != MG_OK) return rc;
   mark(h, MG_STAGE_PERMUTE_ROWS, st);
   launches += 1;
-  const bool chain_down = !(shared_early && T <= kUnchainedDownTokens);
   rc = i8 ? expert_ffn_int8(h, perm, perm_s, pad, counts, padded_rows(h, T * d.top_k), dst, T, d_packed, hbuf, ws + L.off[WS_HQ],
-                            reinterpret_cast<float*>(ws + L.off[WS_H_S]), orow, st, &launches, true, jobs, chain_down)
+                            reinterpret_cast<float*>(ws + L.off[WS_H_S]), orow, st, &launches, true, jobs)
           : expert_ffn(h, perm, pad, counts, padded_rows(h, T * d.top_k), d_packed, hbuf, orow, deq, st, &launches, true,
-                       nullptr, jobs, chain_down);
+                       nullptr, jobs, !(shared_early && T <= kUnchainedDownTokens));
   if (rc != MG_OK) return rc;
   if (shared_early) {
     MG_CUDA(cudaStreamWaitEvent(st, h->ev_shared_out, 0));
