@@ -799,18 +799,19 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
 }
 
 static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T, const void* packed, void* hs, void* hs_q,
-                           float* hs_s, void* out, cudaStream_t st, bool timed = false) {
+                           float* hs_s, void* out, cudaStream_t st, bool timed = false, bool beside = false) {
   const mg_layer_desc& d = h->d;
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
   int rc = launch_int8_matmul(h, xq, d.hidden, xs, T, base + L.sh13, d.hidden, reinterpret_cast<const float*>(base + L.shs13),
-                              2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st);
+                              2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st, beside);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_SHARED_GEMM1, st);
   rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, nullptr, hs_q, d.inter_shared, hs_s, st);
   if (rc != MG_OK) return rc;
   return launch_int8_matmul(h, hs_q, d.inter_shared, hs_s, T, base + L.sh2, d.inter_shared,
-                            reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st);
+                            reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st,
+                            beside);
 }
 
 static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -1108,7 +1109,7 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   const bool shared_early = d.inter_shared && (h->opt_shared_early == 1 ||
                                                (h->opt_shared_early == 2 && T <= (h->stage_timing ? 4096 : 16384)));
   auto run_shared = [&](cudaStream_t on, bool timed) {
-    return i8 ? shared_ffn_int8(h, xq, xs, T, d_packed, hs, ws + L.off[WS_SHQ], reinterpret_cast<float*>(ws + L.off[WS_SH_S]), sh, on, timed)
+    return i8 ? shared_ffn_int8(h, xq, xs, T, d_packed, hs, ws + L.off[WS_SHQ], reinterpret_cast<float*>(ws + L.off[WS_SH_S]), sh, on, timed, on != st)
               : shared_ffn(h, d_x, T, d_packed, hs, sh, on, timed);
   };
   if (shared_early) {

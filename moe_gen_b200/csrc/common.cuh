@@ -264,7 +264,8 @@ int launch_int8_linear(const Handle* h, const void* x, int64_t ldx, int64_t rows
                        int64_t n_out, int64_t cols, void* ws, int64_t ldq, float* scale, void* out, int64_t ldo, cudaStream_t st,
                        bool* quantised);
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
-                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st);
+                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st,
+                       bool beside = false);
 
 // weights (pack.cu) --------------------------------------------------------------------
 int launch_pack_expert(const Handle* h, int local_expert, const void* g, const void* u,
@@ -289,6 +290,7 @@ struct GemmProblem {
   bool b_i8;              // A and B hold int8: a_scales [a_rows], `scales` [rows of B]; weight-lane GEMM, grouped or dense
   const float* a_scales;
   int64_t lda, ldb;       // int8: bytes between the rows of A and of B
+  bool beside;            // int8, dense: runs beside other kernels, on few SMs where it has few jobs
   int n_groups;
   int n_per_group;        // rows of B per group (2I for SwiGLU, H for down, E for the gate)
   int K;

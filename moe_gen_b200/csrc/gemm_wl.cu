@@ -102,6 +102,7 @@ struct WlArgs {
   const float* scales;          // FP8: [rows / 128][K / 128]; int8: of every weight row
   int scale_cols;
   const float* token_scales;    // int8: of every token row
+  int dense_tiles;              // int8: token tiles of dense_rows
   int dense_rows;               // int8: > 0: one weight matrix, these token rows from 0 on; pad_offsets and counts are not read
   int w_rows;                   // int8: rows of the weights in all
   int ragged;                   // int8: K is no multiple of a step; tokens come step by step
@@ -310,6 +311,10 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
   }
   // token tiles before each expert: lane sums of runs of 16 experts, warp scan, runs written out
   auto count_tiles = [&]() {
+    if (I8 && g.dense_rows > 0) {
+      if (lane < 2) s_jp[lane] = lane * g.dense_tiles;
+      return;
+    }
     constexpr int RUN = kMaxExperts / 32;
     int sum = 0;
     for (int i = 0; i < RUN; ++i) {
@@ -897,8 +902,21 @@ int launch_gemm_wl(const Handle* h, const GemmProblem& p, cudaStream_t st) {
   a.status = h->d_status;
   a.rows = static_cast<int>(p.a_rows);
   a.chained = h->chain ? 1 : 0;
-  const int max_tokens = p.b_fp8 ? WlCfg<true>::MAX_TOKENS : WlCfg<false>::MAX_TOKENS;
-  const int64_t tiles = (p.a_rows + max_tokens - 1) / max_tokens + (dense ? 0 : p.n_groups);
+  int max_tokens = p.b_fp8 ? WlCfg<true>::MAX_TOKENS : WlCfg<false>::MAX_TOKENS;
+  if (dense && !p.beside) {
+    // One round of jobs over the pairs, if jobs of at most max_tokens make one: as small as that allows, since a job alone on
+    // its pair is bound by the latency of its rings (three token stages, which hold eight steps of 32 tokens and one of 256 or
+    // more), not by its MMAs.  us, tokens x outputs x inputs, jobs of 384 tokens and so: 128x4096x4096 14.5 and 12.5,
+    // 256x1024x8192 37 and 16.6, 256x4096x4096 22.6 and 12.5, 512x512x8192 38 and 18.6, 1024x1024x1024 14.5 and 8.3,
+    // 1024x2048x4096 24.7 and 16.5; smaller than one round: 256x4096x4096 in jobs of 32 tokens 18.6, 1024x2048x4096 of 64 20.6.
+    // Not beside the routing kernels on another stream, which wait for the SMs that more pairs take (V2-Lite layer 201 tokens
+    // 139 and 143, 512 tokens 154 and 162).
+    const int64_t per_tile = h->sm_count / 2 / a.n_tiles;
+    const int64_t fit = per_tile > 0 ? round_up((p.dense_rows + per_tile - 1) / per_tile, 32) : max_tokens;
+    if (fit < max_tokens) max_tokens = static_cast<int>(fit);
+  }
+  a.dense_tiles = dense ? static_cast<int>((p.dense_rows + max_tokens - 1) / max_tokens) : 0;
+  const int64_t tiles = dense ? a.dense_tiles : (p.a_rows + max_tokens - 1) / max_tokens + p.n_groups;
   int64_t pairs = h->sm_count / 2;
   if (tiles * a.n_tiles < pairs) pairs = tiles * a.n_tiles;
   const int grid = static_cast<int>(2 * pairs);

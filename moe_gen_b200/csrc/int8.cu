@@ -282,8 +282,10 @@ int launch_int8_linear(const Handle* h, const void* x, int64_t ldx, int64_t rows
 }
 
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
-                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st) {
+                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st,
+                       bool beside) {
   GemmProblem p{};
+  p.beside = beside;
   p.a = xq; p.a_rows = rows; p.dense_rows = rows; p.lda = ldx; p.a_scales = x_scale;
   p.b = wq; p.ldb = ldw; p.b_i8 = true; p.scales = w_scale; p.n_groups = 1; p.n_per_group = static_cast<int>(n_out);
   p.K = static_cast<int>(cols); p.out = out; p.ldo = ldo; p.epilogue = epilogue;
