@@ -1797,21 +1797,86 @@ int launch_combine_peers(const Handle* h, const PeerPtrs& peers, const int32_t* 
 //   softmax  gl_i = s_i (gs_i - D), gs the gp of the picks by expert and D = sum gp_j p_j; normalised, D = c S eps / d exactly,
 //            and is not summed up from terms that cancel
 //   sigmoid  gl_i = gs_i s_i (1 - s_i), with s (1 - s) = e / (1 + e)^2, e = exp(-|l|), which does not cancel either
-// A pick of weight 0 competed from a masked group (its score is the constant 0) and passes nothing on.  A warp per token; softmax
-// reads the row of logits once, sigmoid the picks' alone; the row of gradients is written once, from a row in shared memory that
-// the picks' lanes scatter into (every lane comparing its experts with every pick took 35 us for 65536 tokens of 256 experts
-// and 8 picks, where this takes 24).
-template <bool SIGMOID>
-__global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __restrict__ logits, const int32_t* __restrict__ topk_idx,
-                                                              const float* __restrict__ topk_w, const float* __restrict__ grad_w,
-                                                              int64_t T, int E, int k, bool norm, float c, float eps,
-                                                              float* __restrict__ grad_logits) {
+// A pick of weight 0 competed from a masked group (its score is the constant 0) and passes nothing on.
+//
+// gp of the picks, one to a lane, in a run of WIDTH lanes per token.  p: score, or 0 where nothing is passed on; D: see above.
+template <int WIDTH>
+__device__ __forceinline__ float route_pick_grad(float p, float gw, bool live, bool norm, float c, float eps, float& D) {
+  auto sum = [](float v) {
+#pragma unroll
+    for (int o = WIDTH / 2; o > 0; o >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+  };
+  float gp = 0.f;
+  if (norm) {
+    const float d = sum(p) + eps, S = sum(live ? gw * p : 0.f) / d;
+    if (live) gp = c * (gw - S) / d;
+    D = c * S * eps / d;
+  } else {
+    if (live) gp = c * gw;
+    D = sum(gp * p);
+  }
+  return gp;
+}
+// An expert that several picks of a token name: the first of them carries the sum, in the order of the slots; the others are
+// left with e = -1.  `run`: the token's first lane.
+__device__ __forceinline__ void join_repeated_picks(int32_t& e, float& g, int run, int k) {
   const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (t >= T) return;
+  const uint32_t peers = __match_any_sync(0xFFFFFFFFu, e < 0 ? -1 : run << 16 | e);
+  if (!__any_sync(0xFFFFFFFFu, e >= 0 && (peers & (peers - 1)) != 0)) return;
+  float sum = 0.f;
+  for (int j = 0; j < k; ++j) {
+    const float gj = __shfl_sync(0xFFFFFFFFu, g, run + j);
+    if ((peers >> (run + j)) & 1u) sum += gj;
+  }
+  g = sum;
+  if ((peers & ((1u << lane) - 1u)) != 0) e = -1;
+}
+
+// Sigmoid scores: nothing but the picks has a gradient.  A lane per pick, its tokens' rows written as zeros first; both stores meet
+// in L2.  us, V3, 65536 tokens: 22, where a warp per token that scattered into a row in shared memory took 24 and one that
+// compared every expert with every pick 35.
+template <int WIDTH>
+__global__ void __launch_bounds__(256) route_sigmoid_grad_kernel(const float* __restrict__ logits, const int32_t* __restrict__ topk_idx,
+                                                                 const float* __restrict__ topk_w, const float* __restrict__ grad_w,
+                                                                 int64_t T, int E, int k, bool norm, float c, float eps,
+                                                                 float* __restrict__ grad_logits) {
+  constexpr int TOKENS = 256 / WIDTH;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TOKENS, t = t0 + threadIdx.x / WIDTH;
+  const int j = threadIdx.x % WIDTH;
+  int32_t e = -1;
+  float w = 0.f, gw = 0.f, l = 0.f;
+  if (t < T && j < k) {
+    e = topk_idx[t * k + j];
+    w = topk_w[t * k + j];
+    gw = grad_w[t * k + j];
+    if (e >= 0 && e < E) l = logits[t * E + e]; else e = -1;
+  }
+  float4* rows = reinterpret_cast<float4*>(grad_logits + t0 * E);
+  const int n = static_cast<int>(min(static_cast<int64_t>(TOKENS), T - t0)) * (E >> 2);
+  for (int i = threadIdx.x; i < n; i += 256) rows[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool live = e >= 0 && w != 0.f;
+  const float ex = expf(-fabsf(l));
+  float D;
+  float g = route_pick_grad<WIDTH>(live ? (l >= 0.f ? 1.0f : ex) / (1.0f + ex) : 0.f, gw, live, norm, c, eps, D);
+  g *= ex / ((1.0f + ex) * (1.0f + ex));
+  join_repeated_picks(e, g, (threadIdx.x & 31) / WIDTH * WIDTH, k);
+  __syncthreads();
+  if (e >= 0) grad_logits[t * E + e] = g;
+}
+
+// Softmax scores: a warp per token reads the row of logits once and writes the row of gradients once, from a row in shared memory
+// that the picks' lanes scatter into.
+__global__ void __launch_bounds__(256) route_softmax_grad_kernel(const float* __restrict__ logits, const int32_t* __restrict__ topk_idx,
+                                                                 const float* __restrict__ topk_w, const float* __restrict__ grad_w,
+                                                                 int64_t T, int E, int k, bool norm, float c, float eps,
+                                                                 float* __restrict__ grad_logits) {
   constexpr int QUADS = kMaxExperts / 128;             // of four experts, per lane
   __shared__ __align__(16) float s_row[8][kMaxExperts];
-  float4* mine = reinterpret_cast<float4*>(s_row[threadIdx.x >> 5]);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float4* mine = reinterpret_cast<float4*>(s_row[warp]);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + warp;
+  if (t >= T) return;
   const float4* row = reinterpret_cast<const float4*>(logits + t * E);
   const int quads = E >> 2;
   int32_t e = -1;
@@ -1822,69 +1887,42 @@ __global__ void __launch_bounds__(256) route_topk_grad_kernel(const float* __res
     gw = grad_w[t * k + lane];
     if (e >= 0 && e < E) l = logits[t * E + e]; else e = -1;
   }
+  float m = __int_as_float(0xff800000);
   float4 s[QUADS];
-  float m = 0.f, inv_sum = 0.f;
-  if (!SIGMOID) {
-    m = __int_as_float(0xff800000);
 #pragma unroll
-    for (int i = 0; i < QUADS; ++i) {
-      const int q = i * 32 + lane;
-      s[i] = make_float4(m, m, m, m);
-      if (q < quads) s[i] = __ldg(row + q);
-    }
-#pragma unroll
-    for (int i = 0; i < QUADS; ++i) m = fmaxf(m, fmaxf(fmaxf(s[i].x, s[i].y), fmaxf(s[i].z, s[i].w)));
-    m = warp_max_f(m);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < QUADS; ++i) {
-      s[i] = make_float4(expf(s[i].x - m), expf(s[i].y - m), expf(s[i].z - m), expf(s[i].w - m));
-      if (i * 32 + lane < quads) sum += (s[i].x + s[i].y) + (s[i].z + s[i].w);
-    }
-    inv_sum = 1.0f / warp_sum_f(sum);
+  for (int i = 0; i < QUADS; ++i) {
+    const int q = i * 32 + lane;
+    s[i] = make_float4(m, m, m, m);
+    if (q < quads) s[i] = __ldg(row + q);
   }
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) m = fmaxf(m, fmaxf(fmaxf(s[i].x, s[i].y), fmaxf(s[i].z, s[i].w)));
+  m = warp_max_f(m);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) {
+    s[i] = make_float4(expf(s[i].x - m), expf(s[i].y - m), expf(s[i].z - m), expf(s[i].w - m));
+    if (i * 32 + lane < quads) {
+      sum += (s[i].x + s[i].y) + (s[i].z + s[i].w);
+      mine[i * 32 + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  const float inv_sum = 1.0f / warp_sum_f(sum);
   const bool live = e >= 0 && w != 0.f;
-  const float ex = expf(-fabsf(l));
-  float p = 0.f;
-  if (live) p = SIGMOID ? (l >= 0.f ? 1.0f : ex) / (1.0f + ex) : expf(l - m) * inv_sum;
-  float gp = 0.f, D = 0.f;
-  if (norm) {
-    const float d = warp_sum_f(p) + eps, S = warp_sum_f(live ? gw * p : 0.f) / d;
-    if (live) gp = c * (gw - S) / d;
-    D = c * S * eps / d;
-  } else {
-    if (live) gp = c * gw;
-    D = warp_sum_f(gp * p);
-  }
-  if (SIGMOID) gp *= ex / ((1.0f + ex) * (1.0f + ex));
-  // an expert that several picks name: the first of them carries the sum, in the order of the slots
-  const uint32_t peers = __match_any_sync(0xFFFFFFFFu, e);
-  if (__any_sync(0xFFFFFFFFu, e >= 0 && (peers & (peers - 1)) != 0)) {
-    float sum = 0.f;
-    for (int j = 0; j < k; ++j) {
-      const float gj = __shfl_sync(0xFFFFFFFFu, gp, j);
-      if ((peers >> j) & 1u) sum += gj;
-    }
-    gp = sum;
-    if ((peers & ((1u << lane) - 1u)) != 0) e = -1;
-  }
-#pragma unroll
-  for (int i = 0; i < QUADS; ++i)
-    if (i * 32 + lane < quads) mine[i * 32 + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float D;
+  float g = route_pick_grad<32>(live ? expf(l - m) * inv_sum : 0.f, gw, live, norm, c, eps, D);
+  join_repeated_picks(e, g, 0, k);
   __syncwarp();
-  if (e >= 0) s_row[threadIdx.x >> 5][e] = gp;
+  if (e >= 0) s_row[warp][e] = g;
   __syncwarp();
   float4* out = reinterpret_cast<float4*>(grad_logits + t * E);
 #pragma unroll
   for (int i = 0; i < QUADS; ++i) {
     const int q = i * 32 + lane;
     if (q < quads) {
-      float4 g = mine[q];
-      if (!SIGMOID) {
-        g.x = s[i].x * inv_sum * (g.x - D); g.y = s[i].y * inv_sum * (g.y - D);
-        g.z = s[i].z * inv_sum * (g.z - D); g.w = s[i].w * inv_sum * (g.w - D);
-      }
-      out[q] = g;
+      const float4 v = mine[q];
+      out[q] = make_float4(s[i].x * inv_sum * (v.x - D), s[i].y * inv_sum * (v.y - D), s[i].z * inv_sum * (v.z - D),
+                           s[i].w * inv_sum * (v.w - D));
     }
   }
 }
@@ -1896,9 +1934,11 @@ int launch_route_topk_grad(const Handle* h, const float* logits, const int32_t* 
   const bool sig = d.gating == MG_GATE_SIGMOID_NOAUX_TC, renorm = d.gating == MG_GATE_SOFTMAX_TOPK_RENORM;
   const bool norm = renorm || (d.norm_topk_prob && d.top_k > 1);
   const float c = norm && !sig ? 1.0f : d.routed_scale, eps = renorm ? 0.0f : 1e-20f;
-  const unsigned grid = static_cast<unsigned>((T + 7) / 8);
-  if (sig) route_topk_grad_kernel<true><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, d.n_experts, d.top_k, norm, c, eps, grad_logits);
-  else route_topk_grad_kernel<false><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, d.n_experts, d.top_k, norm, c, eps, grad_logits);
+  const int E = d.n_experts, k = d.top_k, per_block = sig ? (k <= 8 ? 32 : 16) : 8;
+  const unsigned grid = static_cast<unsigned>((T + per_block - 1) / per_block);
+  if (!sig) route_softmax_grad_kernel<<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, E, k, norm, c, eps, grad_logits);
+  else if (k <= 8) route_sigmoid_grad_kernel<8><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, E, k, norm, c, eps, grad_logits);
+  else route_sigmoid_grad_kernel<16><<<grid, 256, 0, st>>>(logits, idx, w, grad_w, T, E, k, norm, c, eps, grad_logits);
   MG_CUDA(cudaGetLastError());
   return MG_OK;
 }

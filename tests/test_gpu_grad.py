@@ -131,7 +131,7 @@ def test_an_expert_named_twice():
 GATES = [dict(E=64, k=6, gating=0), dict(E=64, k=6, gating=0, norm=True), dict(E=64, k=1, gating=0, norm=True, scale=2.0),
          dict(E=160, k=6, gating=1, n_group=8, topk_group=3, scale=16.0), dict(E=16, k=6, gating=1, n_group=8, topk_group=2, norm=True),
          dict(E=256, k=8, gating=2, n_group=8, topk_group=4, norm=True, scale=2.5), dict(E=32, k=4, gating=2, n_group=4, topk_group=2, scale=1.5),
-         dict(E=8, k=2, gating=3, norm=True), dict(E=512, k=16, gating=0), dict(E=4, k=4, gating=3, norm=True)]
+         dict(E=8, k=2, gating=3, norm=True), dict(E=512, k=16, gating=0), dict(E=512, k=12, gating=2, n_group=1, topk_group=1, scale=0.5), dict(E=4, k=4, gating=3, norm=True)]
 
 
 def _weights64(logits, idx, live, cfg):
@@ -203,6 +203,10 @@ def test_routing_weights_gradient_at_the_ends():
     e = torch.exp(torch.tensor(-30.0, dtype=torch.float64))
     assert abs(got[0] - e / (1 + e) ** 2) <= e * 2.0 ** -17 and abs(got[1] - e / (1 + e) ** 2) <= e * 2.0 ** -17
     assert not got[2:].any()
+    # an expert that two picks of a token name has both their gradients
+    idx = torch.tensor([[4, 4], [4, 5]], dtype=torch.int32, device=DEV)
+    got = sig.route_topk_grad(torch.zeros(2, 8, device=DEV), idx, torch.ones(2, 2, device=DEV), torch.tensor([[1.0, 2.0]] * 2, device=DEV))
+    assert got[0, 4] == 0.75 and got[1, 4] == 0.25 and got[1, 5] == 0.5 and got.abs().sum() == 1.5
     sig.close()
 
 
