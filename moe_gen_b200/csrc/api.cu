@@ -868,7 +868,7 @@ int mg_int8_linear_ws_bytes(int64_t n_rows, int64_t cols, size_t* bytes) {
   MG_REQUIRE(n_rows >= 0 && cols >= 1, MG_ERR_SHAPE, "mg_int8_linear_ws_bytes: bad size");
   MG_REQUIRE(cols <= kInt8MaxK && n_rows < (1ll << 31), MG_ERR_LIMIT, "mg_int8_linear_ws_bytes: %lld rows of %lld",
              static_cast<long long>(n_rows), static_cast<long long>(cols));
-  *bytes = int8_linear_rows_bytes(n_rows, cols) + static_cast<size_t>(round_up(4 * n_rows, 256));
+  *bytes = int8_in_one_launch(n_rows, cols) ? 0 : int8_linear_rows_bytes(n_rows, cols) + static_cast<size_t>(round_up(4 * n_rows, 256));
   return MG_OK;
 }
 
@@ -883,15 +883,15 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   size_t need = 0;
   rc = mg_int8_linear_ws_bytes(n_rows, cols, &need);
   if (rc != MG_OK) return rc;
-  MG_REQUIRE(d_x && d_ws, MG_ERR_NULL, "mg_int8_linear: null pointer");
-  MG_REQUIRE(ws_bytes >= need && aligned16(d_ws), MG_ERR_WORKSPACE, "mg_int8_linear: scratch of %zu bytes < %zu needed, or not on a 16-byte boundary",
+  MG_REQUIRE(d_x && (d_ws || need == 0), MG_ERR_NULL, "mg_int8_linear: null pointer");
+  MG_REQUIRE(ws_bytes >= need && (need == 0 || aligned16(d_ws)), MG_ERR_WORKSPACE, "mg_int8_linear: scratch of %zu bytes < %zu needed, or not on a 16-byte boundary",
              ws_bytes, need);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (need == 0) return launch_int8_few(h, d_x, ldx, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, st);
   const int64_t ldq = round_up(cols, 128);
   float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
-  bool quantised;
-  rc = launch_int8_linear(h, d_x, ldx, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_ws, ldq, scale, d_out, ldo, st, &quantised);
-  if (rc != MG_OK || !quantised) return rc;
+  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_ws, ldq, scale, st);
+  if (rc != MG_OK) return rc;
   h->chain = true;
   rc = launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
   h->chain = false;

@@ -863,6 +863,27 @@ int wl_maps(const Handle* h, const GemmProblem& p, bool swiglu, const WlMaps** o
   return keep(m);
 }
 
+// Token tiles of a dense product.  A job takes about as long as its tokens and 64 more: its MMAs, or, alone on its pair, the
+// latency of its rings (three token stages, which hold eight steps of 32 tokens and one of 256 or more).  So few tokens to a
+// job while one round of jobs holds them, and rounds that come out even beyond.  us, tokens x outputs x inputs, jobs of up to
+// 384 tokens and so: 128x4096x4096 14.5 and 12.5, 256x1024x8192 37 and 16.6, 256x4096x4096 22.6 and 12.5, 512x512x8192 38 and
+// 18.6, 1024x1024x1024 14.5 and 8.3, 1024x2048x4096 24.7 and 16.5; in more than a round 256x4096x4096 18.6, 1024x2048x4096 20.6.
+// Beside the routing kernels on another stream, which wait for the SMs that more pairs take, as few jobs as there can be
+// (V2-Lite layer 201 tokens 139 and, in more jobs, 143, 512 tokens 154 and 162).
+int dense_token_tiles(int64_t rows, int n_tiles, int pairs, bool beside) {
+  const int64_t units = (rows + 31) / 32, first = (rows + WlCfg<false>::MAX_TOKENS - 1) / WlCfg<false>::MAX_TOKENS;
+  if (beside) return static_cast<int>(first);
+  int64_t most = 2 * first > pairs / n_tiles ? 2 * first : pairs / n_tiles, best = first;
+  if (most > units) most = units;
+  if (most > first + 128) most = first + 128;
+  double best_cost = 1e30;
+  for (int64_t nt = first; nt <= most; ++nt) {
+    const double cost = static_cast<double>((n_tiles * nt + pairs - 1) / pairs) * (2.0 + static_cast<double>(units) / nt);
+    if (cost < best_cost) { best_cost = cost; best = nt; }
+  }
+  return static_cast<int>(best);
+}
+
 }  // namespace
 
 int launch_gemm_wl(const Handle* h, const GemmProblem& p, cudaStream_t st) {
@@ -902,20 +923,9 @@ int launch_gemm_wl(const Handle* h, const GemmProblem& p, cudaStream_t st) {
   a.status = h->d_status;
   a.rows = static_cast<int>(p.a_rows);
   a.chained = h->chain ? 1 : 0;
-  int max_tokens = p.b_fp8 ? WlCfg<true>::MAX_TOKENS : WlCfg<false>::MAX_TOKENS;
-  if (dense && !p.beside) {
-    // One round of jobs over the pairs, if jobs of at most max_tokens make one: as small as that allows, since a job alone on
-    // its pair is bound by the latency of its rings (three token stages, which hold eight steps of 32 tokens and one of 256 or
-    // more), not by its MMAs.  us, tokens x outputs x inputs, jobs of 384 tokens and so: 128x4096x4096 14.5 and 12.5,
-    // 256x1024x8192 37 and 16.6, 256x4096x4096 22.6 and 12.5, 512x512x8192 38 and 18.6, 1024x1024x1024 14.5 and 8.3,
-    // 1024x2048x4096 24.7 and 16.5; smaller than one round: 256x4096x4096 in jobs of 32 tokens 18.6, 1024x2048x4096 of 64 20.6.
-    // Not beside the routing kernels on another stream, which wait for the SMs that more pairs take (V2-Lite layer 201 tokens
-    // 139 and 143, 512 tokens 154 and 162).
-    const int64_t per_tile = h->sm_count / 2 / a.n_tiles;
-    const int64_t fit = per_tile > 0 ? round_up((p.dense_rows + per_tile - 1) / per_tile, 32) : max_tokens;
-    if (fit < max_tokens) max_tokens = static_cast<int>(fit);
-  }
-  a.dense_tiles = dense ? static_cast<int>((p.dense_rows + max_tokens - 1) / max_tokens) : 0;
+  const int max_tokens = p.b_fp8 ? WlCfg<true>::MAX_TOKENS : WlCfg<false>::MAX_TOKENS;
+  if (dense) a.dense_tiles = dense_token_tiles(p.dense_rows, a.n_tiles, h->sm_count / 2, p.beside);
+  else a.dense_tiles = 0;
   const int64_t tiles = dense ? a.dense_tiles : (p.a_rows + max_tokens - 1) / max_tokens + p.n_groups;
   int64_t pairs = h->sm_count / 2;
   if (tiles * a.n_tiles < pairs) pairs = tiles * a.n_tiles;

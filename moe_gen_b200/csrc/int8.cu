@@ -243,11 +243,10 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
   return MG_OK;
 }
 
-// true: launched (few rows, whose quantised form fits in shared memory)
-static bool few_rows(int64_t rows, int64_t cols) {
+bool int8_in_one_launch(int64_t rows, int64_t cols) {
   int m = 1;
-  while (m < rows) m *= 2;
-  return rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem;
+  while (m < rows && m < kFewRows) m *= 2;
+  return rows > 0 && rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem;
 }
 template <int M>
 static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
@@ -266,19 +265,12 @@ static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows,
   return MG_OK;
 }
 
-// bf16 rows: few of them in one launch, else quantised into `ws` (ldq bytes apart, scales in `scale`) and multiplied there
-int launch_int8_linear(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
-                       int64_t n_out, int64_t cols, void* ws, int64_t ldq, float* scale, void* out, int64_t ldo, cudaStream_t st,
-                       bool* quantised) {
-  *quantised = false;
-  if (few_rows(rows, cols)) {
-    if (rows == 1) return launch_few<1>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
-    if (rows == 2) return launch_few<2>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
-    if (rows <= 4) return launch_few<4>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
-    return launch_few<8>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
-  }
-  *quantised = true;
-  return launch_quantize_rows(h, x, rows, cols, ldx, nullptr, ws, ldq, scale, st);
+int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
+                    int64_t n_out, int64_t cols, void* out, int64_t ldo, cudaStream_t st) {
+  if (rows == 1) return launch_few<1>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  if (rows == 2) return launch_few<2>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  if (rows <= 4) return launch_few<4>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  return launch_few<8>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
 }
 
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,

@@ -929,16 +929,15 @@ __global__ void __launch_bounds__(kPlanTokens) plan_place_kernel(const int32_t* 
   }
 }
 
-// Blocks of so many warps that write zeros into the gaps of n_rows rows, and the consecutive rows a warp looks at before the next
-// warp's: few where there are few rows, so that all SMs write (8 always: Mixtral shape, 1 token, 1152 rows, 9 blocks and 20 us)
+// Blocks of so many warps that write zeros into the gaps of n_rows rows, and the consecutive rows a warp looks at: few where there
+// are few rows, so that all SMs write (8 always: Mixtral shape, 1 token, 1152 rows, 9 blocks and 20 us).  Every warp has one run:
+// blocks that follow one another through memory write faster than blocks that stay (a gigabyte of zeros 7.3 and 6.1 TB/s).
 struct GapPlan { unsigned blocks; int run; };
 static GapPlan gap_plan(const Handle* h, int64_t n_rows, int warps) {
   if (n_rows <= 0) return {0u, 1};
-  const int64_t most = static_cast<int64_t>(h->sm_count) * 32;
   int run = 1;
-  while (run < 8 && n_rows > most * run) run *= 2;
-  const int64_t want = ((n_rows + run - 1) / run + warps - 1) / warps, blocks = (most + warps - 1) / warps;
-  return {static_cast<unsigned>(want < blocks ? want : blocks), run};
+  while (run < 8 && n_rows > static_cast<int64_t>(h->sm_count) * 32 * run) run *= 2;
+  return {static_cast<unsigned>(((n_rows + run - 1) / run + warps - 1) / warps), run};
 }
 
 // vectors [v_begin, v_end) of a row, read once, to the k places row_of(pick, entry of the pick) names (nullptr: none); lane j

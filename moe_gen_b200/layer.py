@@ -355,7 +355,6 @@ class MoELayer:
                      pad_offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         """perm[dst_row[t, j]] = x[t], zeros in the rows no pick points at.  With the plan's counts and pad_offsets only those
         rows are written as zeros, in the same launch, instead of all rows before it."""
-        self._check_in(x, torch.bfloat16, "hidden_states")
         if counts is not None and pad_offsets is not None:
             self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
             self._check_rows(dst_row, torch.int32, x.shape[0], self.k, "dst_row")
@@ -366,6 +365,7 @@ class MoELayer:
                                                         counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), rows_padded,
                                                         perm.data_ptr(), self._stream()))
             return perm
+        self._check_in(x, torch.bfloat16, "hidden_states")
         perm = torch.zeros(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
             L.check(self.lib.mg_permute_rows(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
@@ -476,10 +476,11 @@ class MoELayer:
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
         n_out, ldw, out, ldo = self._int8_args(wq, w_scale, cols, n, out)
         L.check(self.lib.mg_int8_linear_ws_bytes(n, cols, C.byref(self._size)))
-        ws = torch.empty(self._size.value, dtype=torch.uint8, device=self.device)
+        size = self._size.value
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         with self._on_device():
             L.check(self.lib.mg_int8_linear(self._h, x.data_ptr(), ldx, n, wq.data_ptr(), ldw, w_scale.data_ptr(), n_out, cols,
-                                            ws.data_ptr(), self._size.value, out.data_ptr(), ldo, self._stream()))
+                                            _ptr(ws), size, out.data_ptr(), ldo, self._stream()))
         return out
 
     def permute_rows_int8(self, xq: torch.Tensor, x_scale: torch.Tensor, dst_row: torch.Tensor, rows_padded: int):

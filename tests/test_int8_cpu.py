@@ -22,7 +22,9 @@ def test_int8_layers_that_are_refused(built_lib, kw, code):
 
 def test_scratch_of_the_product(built_lib):
     lib, n = L.load(), C.c_size_t()
-    assert lib.mg_int8_linear_ws_bytes(5, 1000, C.byref(n)) == 0 and n.value >= 5 * 1024 + 20
+    assert lib.mg_int8_linear_ws_bytes(9, 1000, C.byref(n)) == 0 and n.value >= 9 * 1024 + 36
+    assert lib.mg_int8_linear_ws_bytes(8, 12288, C.byref(n)) == 0 and n.value == 0             # one launch, no scratch
+    assert lib.mg_int8_linear_ws_bytes(8, 12289, C.byref(n)) == 0 and n.value >= 8 * 12416
     assert lib.mg_int8_linear_ws_bytes(0, 1000, C.byref(n)) == 0 and n.value == 0
     assert lib.mg_int8_linear_ws_bytes(1 << 30, 131071, C.byref(n)) == 0 and n.value >= (1 << 30) * 131072
     assert lib.mg_int8_linear_ws_bytes(5, 131072, C.byref(n)) == -7
