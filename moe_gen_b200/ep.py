@@ -101,6 +101,8 @@ class EPMoELayer:
     def __init__(self, layer: MoELayer, group: Optional[dist.ProcessGroup] = None, capacity_factor: float = 2.0,
                  n_micro: int = 1, dedup: bool = True, min_headroom: int = 4096, push_return: Optional[bool] = None,
                  return_parts: int = 4, copy_return: bool = False):
+        if layer.desc.weight_format == L.WEIGHT_INT8_CHANNEL:
+            raise ValueError("int8 experts are not sharded over ranks: their rows travel quantised, the exchange moves bf16")
         self.layer = layer
         self.group = group
         self.rank = dist.get_rank(group)

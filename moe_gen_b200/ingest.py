@@ -31,6 +31,7 @@ DTYPES = {
     "I32": (torch.int32, 4),
     "I64": (torch.int64, 8),
     "U8": (torch.uint8, 1),
+    "I8": (torch.int8, 1),
 }
 _NAMES = {v[0]: k for k, v in DTYPES.items()}
 
@@ -171,12 +172,14 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                    prefix: str = "model.layers.{}", n_threads: int = 8) -> dict:
     """Fills `layer` (a MoELayer, any ep_rank) with block `layer_idx` of the checkpoint: router, this
     rank's experts, shared expert.  Returns byte and time counts.  Expert matrices must be stored in
-    the layer's weight format (FP8 e4m3 + `weight_scale_inv` for MG_WEIGHT_FP8_BLOCK128, else bf16); an
-    FP8-stored shared expert is de-quantised on the device, since the packed layout keeps it bf16."""
+    the layer's weight format (FP8 e4m3 + `weight_scale_inv` for MG_WEIGHT_FP8_BLOCK128, int8 + fp32 `weight_scale` per
+    row, [n] or [n, 1], for MG_WEIGHT_INT8_CHANNEL, else bf16); an FP8-stored shared expert is de-quantised on the device,
+    since the packed layout keeps it bf16, and in an int8 layer a bf16-stored one is quantised there."""
     gate_n, bias_n, exp_n, mats, shared_n = NAMING[naming]
     p = prefix.format(layer_idx)
     dev = layer.device
     fp8 = layer.desc.weight_format == L.WEIGHT_FP8_BLOCK128
+    int8 = layer.desc.weight_format == L.WEIGHT_INT8_CHANNEL
     t_start = time.perf_counter()
     nbytes = 0
 
@@ -193,17 +196,19 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
         for m in mats:
             n = exp_n.format(p=p, e=e, m=m) + ".weight"
             out.append((checkpoint.file_of(n), n))
-        if fp8:
+        if fp8 or int8:
             for m in mats:
-                n = exp_n.format(p=p, e=e, m=m) + ".weight_scale_inv"
+                n = exp_n.format(p=p, e=e, m=m) + (".weight_scale_inv" if fp8 else ".weight_scale")
                 out.append((checkpoint.file_of(n), n))
         return out
 
     I, H = layer.I, layer.H
-    wdt = torch.float8_e4m3fn if fp8 else torch.bfloat16
+    wdt = torch.float8_e4m3fn if fp8 else torch.int8 if int8 else torch.bfloat16
     want = [((I, H), wdt), ((I, H), wdt), ((H, I), wdt)]
     if fp8:
         want += [((-(-I // 128), -(-H // 128)), torch.float32)] * 2 + [((-(-H // 128), -(-I // 128)), torch.float32)]
+    if int8:
+        want += [((I,), torch.float32), ((I,), torch.float32), ((H,), torch.float32)]
     sizes = [int(np.prod(s)) * torch.empty(0, dtype=d).element_size() for s, d in want]
     offs = np.concatenate([[0], np.cumsum([(s + 255) // 256 * 256 for s in sizes])]).astype(np.int64)
     total = int(offs[-1])
@@ -221,6 +226,8 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                 src = pieces(e)
                 for (f, n), (shape, dt) in zip(src, want):
                     got_dt, got_shape = f.info(n)
+                    if len(shape) == 1 and tuple(got_shape) == (shape[0], 1):
+                        got_shape = shape                  # a scale per row, stored as a column
                     if got_dt != dt or tuple(got_shape) != tuple(shape):
                         raise ValueError(f"{n}: stored as {tuple(got_shape)} {got_dt}, the layer needs {tuple(shape)} {dt}")
                 if i >= 2:
@@ -244,7 +251,7 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                 comp.wait_event(copied[b])
                 base = staged[b].data_ptr()
                 ptrs = [base + int(o) for o in offs[:-1]]
-                sc = ptrs[3:6] if fp8 else [None, None, None]
+                sc = ptrs[3:6] if fp8 or int8 else [None, None, None]
                 L.check(layer.lib.mg_pack_expert(layer._h, i, ptrs[0], ptrs[1], ptrs[2], sc[0], sc[1], sc[2],
                                                  layer.packed.data_ptr(), comp.cuda_stream))
                 packed[b].record(comp)
@@ -253,9 +260,9 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
         finally:
             pool.shutdown(wait=True)
 
-    # ---- shared expert (bf16 in the packed layout)
+    # ---- shared expert (bf16 in the packed layout, int8 in that of an int8 layer)
     if layer.Is and shared_n is not None:
-        ws = []
+        ws, scales = [], []
         for m in mats:
             n = shared_n.format(p=p, m=m) + ".weight"
             f = checkpoint.file_of(n)
@@ -265,8 +272,17 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                 sn = shared_n.format(p=p, m=m) + ".weight_scale_inv"
                 s = checkpoint.file_of(sn).tensor(sn)
                 t = layer.dequant_fp8(t.to(dev), s.to(dev))
-            ws.append(t.to(torch.bfloat16))
-        layer.load_shared(*ws)
+            if int8:
+                if t.dtype == torch.int8:
+                    sn = shared_n.format(p=p, m=m) + ".weight_scale"
+                    s = checkpoint.file_of(sn).tensor(sn)
+                else:
+                    t, s = layer.quantize_rows(t.to(dev, torch.bfloat16))
+                scales.append(s)
+                ws.append(t)
+            else:
+                ws.append(t.to(torch.bfloat16))
+        layer.load_shared(*ws, tuple(scales) if int8 else None)
     dt = time.perf_counter() - t_start
     return {"bytes": int(nbytes), "seconds": dt, "gb_per_s": nbytes / dt / 1e9, "experts": layer.e_local}
 
@@ -276,7 +292,7 @@ def export_moe_layer(path: str, layer_idx: int, gate_w: torch.Tensor, bias: Opti
                      prefix: str = "model.layers.{}"):
     """Writes one MoE block in the checkpoint's naming (tests, and tools that build synthetic
     checkpoints).  experts: per expert (gate, up, down) bf16 matrices, or for FP8 checkpoints
-    ((q, scale_inv), (q, scale_inv), (q, scale_inv))."""
+    ((q, scale_inv), (q, scale_inv), (q, scale_inv)), for int8 ones ((q, scale), ...), shared likewise."""
     gate_n, bias_n, exp_n, mats, shared_n = NAMING[naming]
     p = prefix.format(layer_idx)
     out = {gate_n.format(p=p): gate_w}
@@ -286,10 +302,14 @@ def export_moe_layer(path: str, layer_idx: int, gate_w: torch.Tensor, bias: Opti
         for m, w in zip(mats, ws):
             n = exp_n.format(p=p, e=e, m=m)
             if isinstance(w, (tuple, list)):
-                out[n + ".weight"], out[n + ".weight_scale_inv"] = w[0], w[1]
+                out[n + ".weight"], out[n + (".weight_scale" if w[0].dtype == torch.int8 else ".weight_scale_inv")] = w[0], w[1]
             else:
                 out[n + ".weight"] = w
     if shared is not None and shared_n is not None:
         for m, w in zip(mats, shared):
-            out[shared_n.format(p=p, m=m) + ".weight"] = w
+            n = shared_n.format(p=p, m=m)
+            if isinstance(w, (tuple, list)):
+                out[n + ".weight"], out[n + ".weight_scale"] = w
+            else:
+                out[n + ".weight"] = w
     write_safetensors(path, out)

@@ -107,7 +107,7 @@ class MoELayer:
                 raise ValueError("FP8 layer: scales=(gate_scale, up_scale, down_scale) required")
             sc = [s.detach().to(self.device, torch.float32).contiguous() for s in scales]
         if int8:
-            if scales is None:
+            if scales is None or any(s is None for s in scales):
                 raise ValueError("int8 layer: scales=(gate_scale, up_scale, down_scale) required")
             sc = [s.detach().to(self.device, torch.float32).reshape(-1).contiguous() for s in scales]
             for s, m in zip(sc, mats):

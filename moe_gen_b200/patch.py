@@ -25,8 +25,12 @@ def _unwrap(expert):
 
 def _lin_weight(lin):
     w = lin.weight
-    s = getattr(lin, "weight_scale_inv", None)
+    s = getattr(lin, "weight_scale" if w.dtype == torch.int8 else "weight_scale_inv", None)
     return w, s
+
+
+def _format_of(w) -> int:
+    return {torch.float8_e4m3fn: L.WEIGHT_FP8_BLOCK128, torch.int8: L.WEIGHT_INT8_CHANNEL}.get(w.dtype, L.WEIGHT_BF16)
 
 
 def layer_from_deepseek(module, device=None, ep_rank: int = 0, ep_size: int = 1) -> MoELayer:
@@ -46,27 +50,31 @@ def layer_from_deepseek(module, device=None, ep_rank: int = 0, ep_size: int = 1)
     n_shared = getattr(cfg, "n_shared_experts", None) or 0
     experts = [_unwrap(e) for e in module.experts]
     first = next(e for e in experts if e is not None)
-    fp8 = first.gate_proj.weight.dtype == torch.float8_e4m3fn
+    fmt = _format_of(first.gate_proj.weight)
     dev = device if device is not None else first.gate_proj.weight.device
     layer = MoELayer(hidden=cfg.hidden_size, inter=cfg.moe_intermediate_size, n_experts=cfg.n_routed_experts,
                      top_k=cfg.num_experts_per_tok, inter_shared=n_shared * cfg.moe_intermediate_size,
                      n_group=getattr(cfg, "n_group", 1) or 1, topk_group=getattr(cfg, "topk_group", 1) or 1,
                      gating=gating, norm_topk_prob=bool(cfg.norm_topk_prob),
                      routed_scale=float(cfg.routed_scaling_factor),
-                     weight_format=L.WEIGHT_FP8_BLOCK128 if fp8 else L.WEIGHT_BF16, combine_mode=combine,
+                     weight_format=fmt, combine_mode=combine,
                      ep_rank=ep_rank, ep_size=ep_size, device=dev)
     layer.set_router(gate.weight, getattr(gate, "e_score_correction_bias", None))
     for i in range(layer.e_local):
         ex = experts[layer.expert_lo + i]
         (g, gs), (u, us), (d, ds) = _lin_weight(ex.gate_proj), _lin_weight(ex.up_proj), _lin_weight(ex.down_proj)
-        layer.load_expert(i, g, u, d, (gs, us, ds) if fp8 else None)
+        layer.load_expert(i, g, u, d, None if fmt == L.WEIGHT_BF16 else (gs, us, ds))
     if n_shared:
         sh = _unwrap(module.shared_experts)
-        mats = []
+        mats, scales = [], []
         for lin in (sh.gate_proj, sh.up_proj, sh.down_proj):
             w, s = _lin_weight(lin)
-            mats.append(layer.dequant_fp8(w, s) if w.dtype == torch.float8_e4m3fn else w)
-        layer.load_shared(*mats)
+            w = layer.dequant_fp8(w, s) if w.dtype == torch.float8_e4m3fn else w
+            if fmt == L.WEIGHT_INT8_CHANNEL and w.dtype != torch.int8:       # kept in bf16 by the checkpoint
+                w, s = layer.quantize_rows(w.detach().to(layer.device, torch.bfloat16))
+            mats.append(w)
+            scales.append(s)
+        layer.load_shared(*mats, tuple(scales) if fmt == L.WEIGHT_INT8_CHANNEL else None)
     return layer
 
 
@@ -80,12 +88,22 @@ def layer_from_mixtral(module, device=None) -> MoELayer:
         I = dn.shape[2]
         mats = [(gu[e, :I], gu[e, I:], dn[e]) for e in range(E)]
     else:                                          # transformers 4.42: per-expert w1, w3, w2
-        mats = [(ex.w1.weight, ex.w3.weight, ex.w2.weight) for ex in (_unwrap(e) for e in experts)]
+        lins = [(ex.w1, ex.w3, ex.w2) for ex in (_unwrap(e) for e in experts)]
+        mats = [tuple(lin.weight for lin in t) for t in lins]
         I = mats[0][0].shape[0]
     dev = device if device is not None else gate_w.device
+    int8 = mats[0][0].dtype == torch.int8
     layer = MoELayer(hidden=H, inter=I, n_experts=E, top_k=top_k, gating=L.GATE_SOFTMAX_TOPK_RENORM,
+                     weight_format=L.WEIGHT_INT8_CHANNEL if int8 else L.WEIGHT_BF16,
                      norm_topk_prob=True, routed_scale=1.0, combine_mode=L.COMBINE_BF16_SEQ, device=dev)
     layer.set_router(gate_w)
+    if int8:
+        if hasattr(experts, "gate_up_proj"):
+            raise NotImplementedError("int8 experts are read per expert (w1, w3, w2 with a weight_scale each)")
+        for e, t in enumerate(lins):
+            (g, gs), (u, us), (d, ds) = (_lin_weight(lin) for lin in t)
+            layer.load_expert(e, g, u, d, (gs, us, ds))
+        return layer
     for e, (g, u, d) in enumerate(mats):
         layer.load_expert(e, g.to(torch.bfloat16), u.to(torch.bfloat16), d.to(torch.bfloat16))
     return layer

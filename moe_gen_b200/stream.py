@@ -26,6 +26,8 @@ class StreamedMoELayer:
     def __init__(self, *, group_experts: int, slots: int = 2, routing_aware: bool = False, device=None,
                  **layer_kwargs):
         E = layer_kwargs["n_experts"]
+        if layer_kwargs.get("weight_format") == L.WEIGHT_INT8_CHANNEL:
+            raise ValueError("int8 experts are not streamed: their products take quantised rows (MoELayer.expert_ffn_int8)")
         if group_experts < 1 or E % group_experts:
             raise ValueError(f"group_experts={group_experts} must divide n_experts={E}")
         if slots < 2:

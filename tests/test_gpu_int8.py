@@ -442,3 +442,89 @@ def test_refusals(any_layer):
         bf.shared_ffn_int8(q, sc)
     layer.close()
     bf.close()
+
+
+# ------------------------------------------------------------------ checkpoints and modules
+def _checkpoint_weights(seed, E=8, H=256, I=128, Is=128):
+    """Per expert ((q, scale), ...) with scales as a column, as such checkpoints store them; the shared expert in bf16."""
+    def mats(n, s):
+        return [(q.contiguous(), sc[:, None]) for q, sc in (_weights(a, b, s + i) for i, (a, b) in enumerate(((n, H), (n, H), (H, n))))]
+    g = torch.Generator().manual_seed(seed)
+    shared = [torch.randn(a, b, generator=g).mul(0.05).to(torch.bfloat16) for a, b in ((Is, H), (Is, H), (H, Is))]
+    return [mats(I, seed + 10 * e) for e in range(E)], shared, torch.randn(E, H, generator=g).to(torch.bfloat16)
+
+
+def _direct(experts, shared, router):
+    layer = _layer(Is=128, norm=True)
+    layer.set_router(router)
+    for e, m in enumerate(experts):
+        layer.load_expert(e, *[q for q, _ in m], scales=tuple(s for _, s in m))
+    q = [quantise(w) for w in shared]
+    layer.load_shared(*[a.to(torch.int8) for a, _ in q], tuple(s for _, s in q))
+    return layer
+
+
+@pytest.mark.parametrize("shared_int8", (False, True))
+def test_int8_checkpoint(tmp_path, shared_int8):
+    from moe_gen_b200 import ingest
+    experts, shared, router = _checkpoint_weights(300)
+    want = _direct(experts, shared, router)
+    stored = [(q.to(torch.int8), s[:, None]) for q, s in map(quantise, shared)] if shared_int8 else shared
+    ingest.export_moe_layer(str(tmp_path / "model.safetensors"), 2, router, None, experts, shared=stored)
+    got = _layer(Is=128, norm=True)
+    ingest.load_moe_layer(got, ingest.Checkpoint(str(tmp_path)), 2, n_threads=2)
+    assert torch.equal(got.packed, want.packed) and torch.equal(got.gate_w, want.gate_w)
+    bf = _layer(Is=128, int8=False)
+    with pytest.raises(ValueError, match="int8"):
+        ingest.load_moe_layer(bf, ingest.Checkpoint(str(tmp_path)), 2)
+    for layer in (want, got, bf):
+        layer.close()
+
+
+def test_patched_modules_of_int8_experts():
+    from types import SimpleNamespace as NS
+    from moe_gen_b200 import patch_moe_module
+
+    class Lin(torch.nn.Module):
+        def __init__(self, w, s=None):
+            super().__init__()
+            self.weight = torch.nn.Parameter(w.to(DEV), requires_grad=False)
+            if s is not None:
+                self.weight_scale = torch.nn.Parameter(s.to(DEV), requires_grad=False)
+
+    experts, shared, router = _checkpoint_weights(400)
+    x = torch.randn(2, 33, 256, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    want = _direct(experts, shared, router)
+    DeepseekV2MoE = type("DeepseekV2MoE", (torch.nn.Module,), {})
+    mod = DeepseekV2MoE()
+    mod.config = NS(hidden_size=256, moe_intermediate_size=128, n_routed_experts=8, num_experts_per_tok=2, n_shared_experts=1,
+                    norm_topk_prob=True, routed_scaling_factor=1.0, scoring_func="softmax", topk_method="greedy")
+    names = ("gate_proj", "up_proj", "down_proj")
+    mod.gate = Lin(router)
+    mod.experts = [NS(**{n: Lin(*m) for n, m in zip(names, e)}) for e in experts]
+    mod.shared_experts = NS(**{n: Lin(w) for n, w in zip(names, shared)})
+    mod.eval()
+    layer = patch_moe_module(mod)
+    assert torch.equal(layer.packed, want.packed)
+    # the module's combine mode rounds products to bf16, which the directly built layer does not: compared through the patched one
+    assert torch.equal(mod.forward(x), layer.forward(x)) and layer.desc.weight_format == 2
+    MixtralSparseMoeBlock = type("MixtralSparseMoeBlock", (torch.nn.Module,), {})
+    mix = MixtralSparseMoeBlock()
+    mix.gate, mix.top_k = Lin(router), 2
+    mix.experts = [NS(w1=Lin(*e[0]), w3=Lin(*e[1]), w2=Lin(*e[2])) for e in experts]
+    y, logits = (patch_moe_module(mix), mix.forward(x))[1]
+    assert y.shape == x.shape and logits.shape == (66, 8) and bool(torch.isfinite(y.float()).all())
+    lay = mix._moegen_b200_layer
+    assert torch.equal(y.view(-1, 256), _staged(lay, x.view(-1, 256), lay.gate_logits(x.view(-1, 256))))
+
+
+def test_layers_that_stream_or_shard_refuse_int8_experts():
+    from moe_gen_b200 import WEIGHT_INT8_CHANNEL
+    from moe_gen_b200.ep import EPMoELayer
+    from moe_gen_b200.stream import StreamedMoELayer
+    with pytest.raises(ValueError, match="int8"):
+        StreamedMoELayer(group_experts=4, hidden=256, inter=128, n_experts=8, top_k=2, weight_format=WEIGHT_INT8_CHANNEL)
+    layer = _layer()
+    with pytest.raises(ValueError, match="int8"):
+        EPMoELayer(layer)
+    layer.close()
