@@ -1079,17 +1079,22 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     if (rc != MG_OK) return rc;
   }
   // int8 experts: the tokens are quantised once, for the scatter and for the shared expert.  Ahead of the chain: the kernel
-  // behind it is launched by an ordinary dependence, so that the scatter may read the quantised rows as older memory.
+  // behind it is launched by an ordinary dependence, so that the scatter may read the quantised rows as older memory.  Up to 128
+  // tokens the plan that copies the rows quantises them itself, and the shared expert has its own on its own stream (layer, us,
+  // V2-Lite 8 tokens in a graph 96 and 82).
   const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
   uint8_t* xq = ws + L.off[WS_XQ];
   float* xs = reinterpret_cast<float*>(ws + L.off[WS_XS]);
   float* perm_s = i8 ? reinterpret_cast<float*>(ws + L.off[WS_PERM_S]) : nullptr;
-  if (i8) {
-    rc = launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, nullptr, xq, d.hidden, xs, st);
-    if (rc != MG_OK) return rc;
+  auto quantise = [&](cudaStream_t on) {
     launches += 1;
+    return launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, nullptr, xq, d.hidden, xs, on);
+  };
+  const bool copies = plan_copies(h, T) && !h->stage_timing;        // while stage times are recorded plan and scatter have their own
+  if (i8 && !copies) {
+    rc = quantise(st);
+    if (rc != MG_OK) return rc;
   }
-  const void* rows_in = i8 ? xq : d_x;
   if (d_logits_in != nullptr) {
     logits = const_cast<float*>(d_logits_in);      // only read from here on
   } else {
@@ -1122,7 +1127,8 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     MG_CUDA(cudaStreamWaitEvent(h->side2, h->ev_shared_in, 0));
     const bool keep = h->chain;
     h->chain = false;
-    rc = run_shared(h->side2, false);
+    rc = i8 && copies ? quantise(h->side2) : MG_OK;
+    if (rc == MG_OK) rc = run_shared(h->side2, false);
     h->chain = keep;
     if (rc != MG_OK) return rc;
     MG_CUDA(cudaEventRecord(h->ev_shared_out, h->side2));
@@ -1141,13 +1147,13 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   h->chain = chain;
   mark(h, MG_STAGE_ROUTE_TOPK, st);
   int32_t* jobs = reinterpret_cast<int32_t*>(ws + L.off[WS_JOBS]);
-  if (plan_copies(h, T) && !h->stage_timing) {      // while stage times are recorded each has its own
-    rc = launch_plan_and_rows(h, idx, T, counts, offsets, pad, dst, jobs, rows_in, perm, i8 ? xs : nullptr, perm_s, st);
+  if (copies) {
+    rc = launch_plan_and_rows(h, idx, T, counts, offsets, pad, dst, jobs, d_x, perm, perm_s, st);
   } else {
     rc = launch_permute_plan(h, idx, T, 0, d.n_experts, counts, offsets, pad, dst, plan, st, &launches, jobs);
     if (rc != MG_OK) return rc;
     mark(h, MG_STAGE_PERMUTE_PLAN, st);
-    rc = launch_permute_rows(h, rows_in, dst, T, perm, st, i8 ? xs : nullptr, perm_s);
+    rc = launch_permute_rows(h, i8 ? xq : d_x, dst, T, perm, st, i8 ? xs : nullptr, perm_s);
   }
   if (rc != MG_OK) return rc;
   mark(h, MG_STAGE_PERMUTE_ROWS, st);
@@ -1162,7 +1168,8 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     h->chain = false;
     mark(h, MG_STAGE_SHARED_GEMM1, st);
   } else if (d.inter_shared) {
-    rc = run_shared(st, true);
+    rc = i8 && copies ? quantise(st) : MG_OK;
+    if (rc == MG_OK) rc = run_shared(st, true);
     if (rc != MG_OK) return rc;
     launches += i8 ? 3 : 2;
   } else {

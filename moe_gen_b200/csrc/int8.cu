@@ -1,37 +1,12 @@
 // 8-bit integer activations: quantisation of rows, and the dense product as the library's callers reach it.  The product
-// itself is the weight-lane GEMM (gemm_wl.cu).
-//
-// A row x is held as integers q in [-127, 127] and one scale: m = max(max|x|, 2^-100), scale = m / 127, inv = 127 / m (fp32,
-// correctly rounded quotients), q = the integer nearest to x * inv, ties to even.  The product is rounded once: the fused
-// multiply-add with 1.5 * 2^23 leaves the integer of the exact product in its low bits.  2^-100 keeps inv finite; rows below
-// it, rows of zeros among them, come out as zeros.  A row that holds an infinity or a NaN has scale NaN and q = 0, so that
-// every product of the row is NaN.
-#include "common.cuh"
+// itself is the weight-lane GEMM (gemm_wl.cu), the arithmetic of a row in tc.cuh.
+#include "tc.cuh"
 
 namespace mg {
 
 namespace {
 
 constexpr int kQuantVecs = 8;            // 16-byte vectors of a row a thread keeps in registers at most
-constexpr float kQuantFloor = 7.888609052210118e-31f;       // 2^-100
-
-__device__ __forceinline__ void row_scale(uint32_t amax_bits, float& scale, float& inv) {
-  const float m = fmaxf(__uint_as_float(amax_bits << 16), kQuantFloor);
-  const bool finite = amax_bits < 0x7F80u;
-  scale = finite ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7FC00000);
-  inv = finite ? __fdiv_rn(127.0f, m) : 0.0f;
-}
-// the two bf16 of a word -> their integers in the low bytes of lo and hi
-__device__ __forceinline__ void quantise2(uint32_t pair, float inv, uint32_t& lo, uint32_t& hi) {
-  lo = __float_as_uint(__fmaf_rn(__uint_as_float(pair << 16), inv, 12582912.0f));
-  hi = __float_as_uint(__fmaf_rn(__uint_as_float(pair & 0xFFFF0000u), inv, 12582912.0f));
-}
-__device__ __forceinline__ uint32_t quantise4(uint32_t a, uint32_t b, float inv) {
-  uint32_t q[4];
-  quantise2(a, inv, q[0], q[1]);
-  quantise2(b, inv, q[2], q[3]);
-  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-}
 // largest |x| of the block's row as bf16 bits (an infinity or NaN is larger than any number)
 __device__ __forceinline__ uint32_t block_amax(uint32_t pairs, uint32_t* s_max) {
   const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, max(pairs & 0xFFFFu, pairs >> 16));
@@ -62,18 +37,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int6
     if (v < vecs) keep[i] = src[v];
   }
 #pragma unroll
-  for (int i = 0; i < VECS; ++i)
-    m = __vmaxu2(__vmaxu2(m, keep[i].x & 0x7FFF7FFFu), __vmaxu2(keep[i].y & 0x7FFF7FFFu,
-                 __vmaxu2(keep[i].z & 0x7FFF7FFFu, keep[i].w & 0x7FFF7FFFu)));
+  for (int i = 0; i < VECS; ++i) m = amax8(m, keep[i]);
   float s, inv;
   row_scale(block_amax(m, s_max), s, inv);
-  const bool dead = inv == 0.0f;
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
-    if (v < vecs)
-      q[row * ldq + v] = dead ? make_uint2(0u, 0u)
-                              : make_uint2(quantise4(keep[i].x, keep[i].y, inv), quantise4(keep[i].z, keep[i].w, inv));
+    if (v < vecs) q[row * ldq + v] = quantise8(keep[i], inv);
   }
   if (threadIdx.x == 0) scale[row] = s;
 }
@@ -108,10 +78,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uin
     uint32_t m = 0;
     if (wide) {
       const uint4* v = reinterpret_cast<const uint4*>(src);
-      for (int c = lane; c < cols >> 3; c += 32) {
-        const uint4 a = __ldg(v + c);
-        m = __vmaxu2(__vmaxu2(m, a.x & 0x7FFF7FFFu), __vmaxu2(a.y & 0x7FFF7FFFu, __vmaxu2(a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu)));
-      }
+      for (int c = lane; c < cols >> 3; c += 32) m = amax8(m, __ldg(v + c));
       m = max(m & 0xFFFFu, m >> 16);
     } else {
       for (int c = lane; c < cols; c += 32) m = max(m, __ldg(src + c) & 0x7FFFu);
@@ -119,22 +86,16 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uin
     float scale, inv;
     row_scale(__reduce_max_sync(0xFFFFFFFFu, m), scale, inv);
     if (lane == 0) s_scale[r] = scale;
-    const bool dead = inv == 0.f;
     if (wide) {
       const uint4* v = reinterpret_cast<const uint4*>(src);
       for (int c = lane; c < chunks * 2; c += 32) {
-        uint2 o = make_uint2(0u, 0u);
-        if (c < cols >> 3 && !dead) {
-          const uint4 a = __ldg(v + c);
-          o = make_uint2(quantise4(a.x, a.y, inv), quantise4(a.z, a.w, inv));
-        }
-        reinterpret_cast<uint2*>(q)[c] = o;
+        reinterpret_cast<uint2*>(q)[c] = c < cols >> 3 ? quantise8(__ldg(v + c), inv) : make_uint2(0u, 0u);
       }
     } else {
       uint8_t* b = reinterpret_cast<uint8_t*>(q);
       for (int c = lane; c < chunks * 16; c += 32) {
         uint32_t lo = 0u, hi;
-        if (c < cols && !dead) quantise2(__ldg(src + c), inv, lo, hi);
+        if (c < cols && inv != 0.f) quantise2(__ldg(src + c), inv, lo, hi);
         b[c] = static_cast<uint8_t>(lo);
       }
     }

@@ -929,14 +929,14 @@ __global__ void __launch_bounds__(kPlanTokens) plan_place_kernel(const int32_t* 
   }
 }
 
-// Blocks of so many warps that write zeros into the gaps of n_rows rows, and the consecutive rows a warp looks at: few where there
-// are few rows, so that all SMs write (8 always: Mixtral shape, 1 token, 1152 rows, 9 blocks and 20 us).  Every warp has one run:
-// blocks that follow one another through memory write faster than blocks that stay (a gigabyte of zeros 7.3 and 6.1 TB/s).
+// Blocks of so many warps that write zeros into the gaps of n_rows rows, and the consecutive rows a warp looks at: few, so that all
+// SMs write (8 always: Mixtral shape, 1 token, 1152 rows, 9 blocks and 20 us), and every warp has one run: blocks that follow one
+// another through memory write faster than blocks that stay (a gigabyte of zeros 7.3 and 6.1 TB/s).  V3, 8192 tokens, sort and
+// return's gradient, us, runs of 8, 2 and 1 rows: 266, 252 and 258, 390, 369 and 375.
 struct GapPlan { unsigned blocks; int run; };
 static GapPlan gap_plan(const Handle* h, int64_t n_rows, int warps) {
   if (n_rows <= 0) return {0u, 1};
-  int run = 1;
-  while (run < 8 && n_rows > static_cast<int64_t>(h->sm_count) * 32 * run) run *= 2;
+  const int run = n_rows > static_cast<int64_t>(h->sm_count) * 32 ? 2 : 1;
   return {static_cast<unsigned>(((n_rows + run - 1) / run + warps - 1) / warps), run};
 }
 
@@ -963,6 +963,29 @@ __device__ __forceinline__ void copy_row(const uint4* src, int32_t my_dst, int k
   }
 }
 
+// The same for a row that is quantised on its way: x is its bf16 (two vectors to one of bytes), read whole by every warp that has a
+// slice of it, for its scale.
+__device__ __forceinline__ void quantise_row(const uint4* src, uint4* rows, float* row_scales, int32_t my_dst, int k, int vec_per_row,
+                                             int v_begin, int v_end, int lane) {
+  uint32_t m = 0;
+  for (int v = lane; v < 2 * vec_per_row; v += 32) m = amax8(m, __ldg(src + v));
+  float scale, inv;
+  row_scale(__reduce_max_sync(0xFFFFFFFFu, max(m & 0xFFFFu, m >> 16)), scale, inv);
+  if (v_begin == 0 && my_dst >= 0) row_scales[my_dst] = scale;
+  for (int o = v_begin; o < v_end; o += 32) {
+    const int at = o + lane, v = 2 * at;
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (at < v_end) {
+      const uint2 a = quantise8(__ldg(src + v), inv), b = quantise8(__ldg(src + v + 1), inv);
+      q = make_uint4(a.x, a.y, b.x, b.y);
+    }
+    for (int j = 0; j < k; ++j) {
+      const int32_t d = __shfl_sync(0xFFFFFFFFu, my_dst, j);
+      if (d >= 0 && at < v_end) rows[static_cast<int64_t>(d) * vec_per_row + at] = q;
+    }
+  }
+}
+
 // The whole plan in one block, for batches of up to kPlanSmallTokens tokens: a bitmap per (32 tokens, expert) gives
 // the counts and the stable ranks, one block scan the offsets.  Same results as the four kernels above, which cost a
 // launch each: 20 -> 8 us at 8 tokens, 23 -> 10 us at 512.  The limit is one token per thread of the block.
@@ -982,8 +1005,7 @@ struct PlanCopy {
   const uint4* x;
   uint4* rows;
   int vec_per_row, slices, v_chunk;
-  const float* scale;           // int8 rows: of every token, nullptr else
-  float* row_scale;
+  float* row_scale;             // != nullptr: x is bf16, rows are its quantised rows, and this their scales
 };
 template <bool COPY>
 __global__ void __launch_bounds__(1024) plan_small_kernel(const int32_t* idx, int T, int k, int lo, int n,
@@ -1057,7 +1079,11 @@ __global__ void __launch_bounds__(1024) plan_small_kernel(const int32_t* idx, in
     const int e = lane < k ? idx[t * k + lane] - lo : -1, at = (t >> 5) * n + e;
     int32_t dst = e >= 0 && e < n ? wbase[at] + __popc(bm[at] & ((1u << (t & 31)) - 1u)) : -1;
     if (dst >= 0 && !MG_GUARD(dst < guard.rows_bound, guard, 103)) dst = -1;
-    if (copy.scale != nullptr && v == 0 && dst >= 0) copy.row_scale[dst] = copy.scale[t];
+    if (copy.row_scale != nullptr) {
+      quantise_row(copy.x + static_cast<int64_t>(t) * copy.vec_per_row * 2, copy.rows, copy.row_scale, dst, k, copy.vec_per_row, v,
+                   min(copy.vec_per_row, v + copy.v_chunk), lane);
+      return;
+    }
     copy_row(copy.x + static_cast<int64_t>(t) * copy.vec_per_row, dst, k, v, min(copy.vec_per_row, v + copy.v_chunk), lane,
              [&](int, int32_t d) { return d < 0 ? nullptr : copy.rows + static_cast<int64_t>(d) * copy.vec_per_row; });
   }
@@ -1080,7 +1106,7 @@ static_assert(plan_small_smem(kPlanCopyTokens, kMaxExperts) <= 48 * 1024, "the c
 // x == nullptr: the plan alone
 static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo, int n, int32_t* counts,
                              int32_t* offsets, int32_t* pad_offsets, int32_t* dst_row, int32_t* job_counters,
-                             const void* x, void* perm_x, const float* x_scale, float* perm_scale, cudaStream_t st) {
+                             const void* x, void* perm_x, float* perm_scale, cudaStream_t st) {
   const size_t smem = plan_small_smem(T, n);
   static bool done[64];
   if (smem > 48 * 1024 && !(h->device >= 0 && h->device < 64 && done[h->device])) {
@@ -1096,12 +1122,12 @@ static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo,
     return MG_OK;
   }
   if (threads < 256) threads = 256;
-  const int vpr = h->d.hidden / (x_scale != nullptr ? 16 : 8);
+  const int vpr = h->d.hidden / (perm_scale != nullptr ? 16 : 8);
   const RowSlices rs = row_slices(h, T, vpr);
   const int warps = threads / 32;
   MG_CUDA(launch_chained(h, plan_small_kernel<true>, (T * rs.n + warps - 1) / warps, threads, smem, st, idx, T, h->d.top_k, lo, n,
                          counts, offsets, pad_offsets, dst_row, job_counters,
-                         PlanCopy{static_cast<const uint4*>(x), static_cast<uint4*>(perm_x), vpr, rs.n, rs.v_chunk, x_scale, perm_scale},
+                         PlanCopy{static_cast<const uint4*>(x), static_cast<uint4*>(perm_x), vpr, rs.n, rs.v_chunk, perm_scale},
                          guard));
   return MG_OK;
 }
@@ -1112,10 +1138,9 @@ static int launch_plan_small(const Handle* h, const int32_t* idx, int T, int lo,
 // and 467.7; V2-236B 8 tokens 359 and 357, 128 1170 and 1171, 512 1230 and 1239; V3 1 token 149.7 and 146.5, 256 2562 and 2570.
 bool plan_copies(const Handle* h, int64_t T) { return T > 0 && T <= kPlanCopyTokens && T * h->d.hidden >= 4096; }
 int launch_plan_and_rows(const Handle* h, const int32_t* idx, int64_t T, int32_t* counts, int32_t* offsets, int32_t* pad_offsets,
-                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, const float* x_scale,
-                         float* perm_scale, cudaStream_t st) {
+                         int32_t* dst_row, int32_t* job_counters, const void* x, void* perm_x, float* perm_scale, cudaStream_t st) {
   return launch_plan_small(h, idx, static_cast<int>(T), 0, h->d.n_experts, counts, offsets, pad_offsets, dst_row, job_counters, x,
-                           perm_x, x_scale, perm_scale, st);
+                           perm_x, perm_scale, st);
 }
 
 size_t plan_ws_bytes(const Handle* h, int64_t T) {
@@ -1132,7 +1157,7 @@ int launch_permute_plan(const Handle* h, const int32_t* idx, int64_t T, int expe
   if (T > 0 && T <= kPlanSmallTokens) {
     if (launches) *launches += 1;
     return launch_plan_small(h, idx, static_cast<int>(T), expert_lo, n_exp, counts, offsets, pad_offsets, dst_row,
-                             job_counters, nullptr, nullptr, nullptr, nullptr, st);
+                             job_counters, nullptr, nullptr, nullptr, st);
   }
   int nblk = static_cast<int>((T + kPlanTokens - 1) / kPlanTokens);
   int32_t* bc = static_cast<int32_t*>(ws);

@@ -246,6 +246,40 @@ __device__ __forceinline__ float round_bf16(float f) {
   return __bfloat162float(__float2bfloat16_rn(f));
 }
 
+// ---- rows of bytes ----------------------------------------------------------------------
+// A row x is held as integers q in [-127, 127] and one scale: m = max(max|x|, 2^-100), scale = m / 127, inv = 127 / m (fp32,
+// correctly rounded quotients), q = the integer nearest to x * inv, ties to even.  The product is rounded once: the fused
+// multiply-add with 1.5 * 2^23 leaves the integer of the exact product in its low bits.  2^-100 keeps inv finite; rows below
+// it, rows of zeros among them, come out as zeros.  A row that holds an infinity or a NaN has scale NaN and q = 0, so that
+// every product of the row is NaN.
+constexpr float kQuantFloor = 7.888609052210118e-31f;       // 2^-100
+
+__device__ __forceinline__ void row_scale(uint32_t amax_bits, float& scale, float& inv) {
+  const float m = fmaxf(__uint_as_float(amax_bits << 16), kQuantFloor);
+  const bool finite = amax_bits < 0x7F80u;
+  scale = finite ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7FC00000);
+  inv = finite ? __fdiv_rn(127.0f, m) : 0.0f;
+}
+// the two bf16 of a word -> their integers in the low bytes of lo and hi
+__device__ __forceinline__ void quantise2(uint32_t pair, float inv, uint32_t& lo, uint32_t& hi) {
+  lo = __float_as_uint(__fmaf_rn(__uint_as_float(pair << 16), inv, 12582912.0f));
+  hi = __float_as_uint(__fmaf_rn(__uint_as_float(pair & 0xFFFF0000u), inv, 12582912.0f));
+}
+__device__ __forceinline__ uint32_t quantise4(uint32_t a, uint32_t b, float inv) {
+  uint32_t q[4];
+  quantise2(a, inv, q[0], q[1]);
+  quantise2(b, inv, q[2], q[3]);
+  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
+// largest |x| of a 16-byte vector's halves and m's, as bf16 bits (an infinity or NaN is larger than any number)
+__device__ __forceinline__ uint32_t amax8(uint32_t m, const uint4& a) {
+  return __vmaxu2(__vmaxu2(m, a.x & 0x7FFF7FFFu),
+                  __vmaxu2(a.y & 0x7FFF7FFFu, __vmaxu2(a.z & 0x7FFF7FFFu, a.w & 0x7FFF7FFFu)));
+}
+__device__ __forceinline__ uint2 quantise8(const uint4& a, float inv) {
+  return inv == 0.0f ? make_uint2(0u, 0u) : make_uint2(quantise4(a.x, a.y, inv), quantise4(a.z, a.w, inv));
+}
+
 // ---- SM pairs (cta_group::2) -----------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
