@@ -863,12 +863,12 @@ int mg_int8_matmul(mg_handle hh, const void* d_xq, int64_t ldx, const float* d_x
 static size_t int8_linear_rows_bytes(int64_t n_rows, int64_t cols) {
   return static_cast<size_t>(round_up(n_rows * round_up(cols, 128), 256));
 }
-int mg_int8_linear_ws_bytes(int64_t n_rows, int64_t cols, size_t* bytes) {
+int mg_int8_linear_ws_bytes(int64_t n_rows, int64_t n_out, int64_t cols, size_t* bytes) {
   MG_REQUIRE(bytes, MG_ERR_NULL, "null argument");
-  MG_REQUIRE(n_rows >= 0 && cols >= 1, MG_ERR_SHAPE, "mg_int8_linear_ws_bytes: bad size");
+  MG_REQUIRE(n_rows >= 0 && n_out >= 1 && cols >= 1, MG_ERR_SHAPE, "mg_int8_linear_ws_bytes: bad size");
   MG_REQUIRE(cols <= kInt8MaxK && n_rows < (1ll << 31), MG_ERR_LIMIT, "mg_int8_linear_ws_bytes: %lld rows of %lld",
              static_cast<long long>(n_rows), static_cast<long long>(cols));
-  *bytes = int8_in_one_launch(n_rows, cols) ? 0 : int8_linear_rows_bytes(n_rows, cols) + static_cast<size_t>(round_up(4 * n_rows, 256));
+  *bytes = int8_in_one_launch(n_rows, n_out, cols) ? 0 : int8_linear_rows_bytes(n_rows, cols) + static_cast<size_t>(round_up(4 * n_rows, 256));
   return MG_OK;
 }
 
@@ -881,7 +881,7 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   if (rc != MG_OK || n_rows == 0) return rc;
   MG_REQUIRE(ldx >= cols, MG_ERR_SHAPE, "mg_int8_linear: rows of x are %lld elements apart", static_cast<long long>(ldx));
   size_t need = 0;
-  rc = mg_int8_linear_ws_bytes(n_rows, cols, &need);
+  rc = mg_int8_linear_ws_bytes(n_rows, n_out, cols, &need);
   if (rc != MG_OK) return rc;
   MG_REQUIRE(d_x && (d_ws || need == 0), MG_ERR_NULL, "mg_int8_linear: null pointer");
   MG_REQUIRE(ws_bytes >= need && (need == 0 || aligned16(d_ws)), MG_ERR_WORKSPACE, "mg_int8_linear: scratch of %zu bytes < %zu needed, or not on a 16-byte boundary",

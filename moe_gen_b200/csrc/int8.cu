@@ -51,108 +51,120 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int6
 // A product of up to kFewRows rows of x in one launch: every block quantises them into shared memory, and a warp multiplies two
 // weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a pair
 // of SMs for 256 weight rows); here every SM streams a share of the weights.
-constexpr int kFewRows = 8, kFewWarps = 8, kFewSmem = 96 * 1024;
+constexpr int kFewRows = 8, kFewWarps = 16, kFewSmem = 96 * 1024;
 template <int M>
 __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int rows, int cols,
                                                                        const uint8_t* __restrict__ w, int64_t ldw,
                                                                        const float* __restrict__ w_scale, int n_out,
                                                                        __nv_bfloat16* __restrict__ out, int64_t ldo, bool wide) {
   extern __shared__ __align__(16) uint8_t s_q[];           // [M][chunks of 16 bytes], zeros behind the last element
+  __shared__ uint32_t s_max[kFewWarps];
   __shared__ float s_scale[M];
+  constexpr int ROW_WARPS = kFewWarps / M, STEP = ROW_WARPS * 32, KEEP = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int chunks = (cols + 15) >> 4;
-  const int n0 = (blockIdx.x * kFewWarps + warp) * 2;
-  // this warp's weights on their way while x is quantised
+  int n0 = (blockIdx.x * kFewWarps + warp) * 2;
+  // this warp's first weights on their way while x is quantised
   if (n0 < n_out) {
     const uint8_t* p = w + static_cast<int64_t>(min(n0 + (lane & 1), n_out - 1)) * ldw;
     for (int c = (lane >> 1) * 128; c < cols; c += 16 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + c));
   }
-  for (int r = warp; r < M; r += kFewWarps) {
-    uint32_t* q = reinterpret_cast<uint32_t*>(s_q + static_cast<size_t>(r) * chunks * 16);
-    if (r >= rows) {
-      for (int c = lane; c < chunks * 4; c += 32) q[c] = 0u;
-      if (lane == 0) s_scale[r] = 0.f;
-      continue;
-    }
-    const uint16_t* src = x + r * ldx;
+  {
+    const int r = warp / ROW_WARPS, t = threadIdx.x - r * STEP;          // ROW_WARPS warps to a row
+    const bool live = r < rows;
+    const uint16_t* src = x + (live ? r : 0) * ldx;
+    const uint4* v4 = reinterpret_cast<const uint4*>(src);
+    const int vecs = wide && live ? cols >> 3 : 0;
+    uint4 keep[KEEP];
     uint32_t m = 0;
-    if (wide) {
-      const uint4* v = reinterpret_cast<const uint4*>(src);
-      for (int c = lane; c < cols >> 3; c += 32) m = amax8(m, __ldg(v + c));
-      m = max(m & 0xFFFFu, m >> 16);
-    } else {
-      for (int c = lane; c < cols; c += 32) m = max(m, __ldg(src + c) & 0x7FFFu);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+      keep[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (t + i * STEP < vecs) keep[i] = __ldg(v4 + t + i * STEP);
     }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) m = amax8(m, keep[i]);
+    for (int c = t + KEEP * STEP; c < vecs; c += STEP) m = amax8(m, __ldg(v4 + c));
+    m = max(m & 0xFFFFu, m >> 16);
+    if (!wide && live)
+      for (int c = t; c < cols; c += STEP) m = max(m, __ldg(src + c) & 0x7FFFu);
+    m = __reduce_max_sync(0xFFFFFFFFu, m);
+    if (lane == 0) s_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROW_WARPS; ++i) m = max(m, s_max[r * ROW_WARPS + i]);
     float scale, inv;
-    row_scale(__reduce_max_sync(0xFFFFFFFFu, m), scale, inv);
-    if (lane == 0) s_scale[r] = scale;
+    row_scale(m, scale, inv);
+    if (t == 0) s_scale[r] = scale;
+    uint8_t* q = s_q + static_cast<size_t>(r) * chunks * 16;
     if (wide) {
-      const uint4* v = reinterpret_cast<const uint4*>(src);
-      for (int c = lane; c < chunks * 2; c += 32) {
-        reinterpret_cast<uint2*>(q)[c] = c < cols >> 3 ? quantise8(__ldg(v + c), inv) : make_uint2(0u, 0u);
-      }
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (t + i * STEP < chunks * 2) reinterpret_cast<uint2*>(q)[t + i * STEP] = quantise8(keep[i], inv);      // zeros behind the row
+      for (int c = t + KEEP * STEP; c < chunks * 2; c += STEP)
+        reinterpret_cast<uint2*>(q)[c] = c < vecs ? quantise8(__ldg(v4 + c), inv) : make_uint2(0u, 0u);
     } else {
-      uint8_t* b = reinterpret_cast<uint8_t*>(q);
-      for (int c = lane; c < chunks * 16; c += 32) {
+      for (int c = t; c < chunks * 16; c += STEP) {
         uint32_t lo = 0u, hi;
-        if (c < cols && inv != 0.f) quantise2(__ldg(src + c), inv, lo, hi);
-        b[c] = static_cast<uint8_t>(lo);
+        if (live && c < cols && inv != 0.f) quantise2(__ldg(src + c), inv, lo, hi);
+        q[c] = static_cast<uint8_t>(lo);
       }
     }
   }
   __syncthreads();
-  if (n0 >= n_out) return;
-  const bool two = n0 + 1 < n_out;
-  const uint8_t* w0 = w + static_cast<int64_t>(n0) * ldw;
-  const uint8_t* w1 = w0 + (two ? ldw : 0);
-  int acc0[M], acc1[M];
+  for (; n0 < n_out; n0 += gridDim.x * kFewWarps * 2) {
+    const bool two = n0 + 1 < n_out;
+    const uint8_t* w0 = w + static_cast<int64_t>(n0) * ldw;
+    const uint8_t* w1 = w0 + (two ? ldw : 0);
+    int acc0[M], acc1[M];
 #pragma unroll
-  for (int r = 0; r < M; ++r) acc0[r] = acc1[r] = 0;
-  auto dot = [&](int c, const uint4& a, const uint4& b) {
+    for (int r = 0; r < M; ++r) acc0[r] = acc1[r] = 0;
+    auto dot = [&](int c, const uint4& a, const uint4& b) {
+#pragma unroll
+      for (int r = 0; r < M; ++r) {
+        const uint4 q = *reinterpret_cast<const uint4*>(s_q + (static_cast<size_t>(r) * chunks + c) * 16);
+        acc0[r] = __dp4a(static_cast<int>(a.x), static_cast<int>(q.x), acc0[r]);
+        acc0[r] = __dp4a(static_cast<int>(a.y), static_cast<int>(q.y), acc0[r]);
+        acc0[r] = __dp4a(static_cast<int>(a.z), static_cast<int>(q.z), acc0[r]);
+        acc0[r] = __dp4a(static_cast<int>(a.w), static_cast<int>(q.w), acc0[r]);
+        acc1[r] = __dp4a(static_cast<int>(b.x), static_cast<int>(q.x), acc1[r]);
+        acc1[r] = __dp4a(static_cast<int>(b.y), static_cast<int>(q.y), acc1[r]);
+        acc1[r] = __dp4a(static_cast<int>(b.z), static_cast<int>(q.z), acc1[r]);
+        acc1[r] = __dp4a(static_cast<int>(b.w), static_cast<int>(q.w), acc1[r]);
+      }
+    };
+    const int whole = cols >> 4;
+    int c = lane;
+    for (; c + 96 < whole; c += 128) {
+      uint4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[i] = __ldg(reinterpret_cast<const uint4*>(w0) + c + 32 * i);
+        b[i] = __ldg(reinterpret_cast<const uint4*>(w1) + c + 32 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dot(c + 32 * i, a[i], b[i]);
+    }
+    for (; c < whole; c += 32) dot(c, __ldg(reinterpret_cast<const uint4*>(w0) + c), __ldg(reinterpret_cast<const uint4*>(w1) + c));
+    if (c == whole && whole < chunks) {                      // the bytes behind the last whole chunk, one by one
+      uint32_t a[4] = {0u, 0u, 0u, 0u}, b[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (whole * 16 + i < cols) {
+          a[i >> 2] |= static_cast<uint32_t>(w0[whole * 16 + i]) << (8 * (i & 3));
+          b[i >> 2] |= static_cast<uint32_t>(w1[whole * 16 + i]) << (8 * (i & 3));
+        }
+      }
+      dot(whole, make_uint4(a[0], a[1], a[2], a[3]), make_uint4(b[0], b[1], b[2], b[3]));
+    }
+    const float s0 = w_scale[n0], s1 = two ? w_scale[n0 + 1] : 0.f;
 #pragma unroll
     for (int r = 0; r < M; ++r) {
-      const uint4 q = *reinterpret_cast<const uint4*>(s_q + (static_cast<size_t>(r) * chunks + c) * 16);
-      acc0[r] = __dp4a(static_cast<int>(a.x), static_cast<int>(q.x), acc0[r]);
-      acc0[r] = __dp4a(static_cast<int>(a.y), static_cast<int>(q.y), acc0[r]);
-      acc0[r] = __dp4a(static_cast<int>(a.z), static_cast<int>(q.z), acc0[r]);
-      acc0[r] = __dp4a(static_cast<int>(a.w), static_cast<int>(q.w), acc0[r]);
-      acc1[r] = __dp4a(static_cast<int>(b.x), static_cast<int>(q.x), acc1[r]);
-      acc1[r] = __dp4a(static_cast<int>(b.y), static_cast<int>(q.y), acc1[r]);
-      acc1[r] = __dp4a(static_cast<int>(b.z), static_cast<int>(q.z), acc1[r]);
-      acc1[r] = __dp4a(static_cast<int>(b.w), static_cast<int>(q.w), acc1[r]);
-    }
-  };
-  const int whole = cols >> 4;
-  int c = lane;
-  for (; c + 96 < whole; c += 128) {
-    uint4 a[4], b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = __ldg(reinterpret_cast<const uint4*>(w0) + c + 32 * i);
-      b[i] = __ldg(reinterpret_cast<const uint4*>(w1) + c + 32 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) dot(c + 32 * i, a[i], b[i]);
-  }
-  for (; c < whole; c += 32) dot(c, __ldg(reinterpret_cast<const uint4*>(w0) + c), __ldg(reinterpret_cast<const uint4*>(w1) + c));
-  if (c == whole && whole < chunks) {                      // the bytes behind the last whole chunk, one by one
-    uint32_t a[4] = {0u, 0u, 0u, 0u}, b[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (whole * 16 + i < cols) {
-        a[i >> 2] |= static_cast<uint32_t>(w0[whole * 16 + i]) << (8 * (i & 3));
-        b[i >> 2] |= static_cast<uint32_t>(w1[whole * 16 + i]) << (8 * (i & 3));
+      const int a = __reduce_add_sync(0xFFFFFFFFu, acc0[r]), b = __reduce_add_sync(0xFFFFFFFFu, acc1[r]);
+      if (lane == 0 && r < rows) {
+        out[r * ldo + n0] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(a), s_scale[r]), s0));
+        if (two) out[r * ldo + n0 + 1] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(b), s_scale[r]), s1));
       }
-    }
-    dot(whole, make_uint4(a[0], a[1], a[2], a[3]), make_uint4(b[0], b[1], b[2], b[3]));
-  }
-  const float s0 = w_scale[n0], s1 = two ? w_scale[n0 + 1] : 0.f;
-#pragma unroll
-  for (int r = 0; r < M; ++r) {
-    const int a = __reduce_add_sync(0xFFFFFFFFu, acc0[r]), b = __reduce_add_sync(0xFFFFFFFFu, acc1[r]);
-    if (lane == 0 && r < rows) {
-      out[r * ldo + n0] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(a), s_scale[r]), s0));
-      if (two) out[r * ldo + n0 + 1] = __float2bfloat16_rn(__fmul_rn(__fmul_rn(__int2float_rn(b), s_scale[r]), s1));
     }
   }
 }
@@ -204,10 +216,13 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
   return MG_OK;
 }
 
-bool int8_in_one_launch(int64_t rows, int64_t cols) {
+// us with x and weights in L2, one launch, and two (quantised, then on the tensor cores): 1 row 4096x4096 4.4 and 12, 8192x8192 8.6
+// and 18; 4 rows 8192x8192 14.0 and 18; 8 rows 1024x1024 4.6 and 8.5, 4096x4096 8.5 and 12.5, 8192x2048 10.3 and 10.2, 8192x8192
+// 25.5 and 18.4 (every weight meets eight rows from shared memory, which bounds it).  So beyond four rows up to 2^24 weights.
+bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols) {
   int m = 1;
   while (m < rows && m < kFewRows) m *= 2;
-  return rows > 0 && rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem;
+  return rows > 0 && rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem && (rows <= 4 || n_out <= (1 << 24) / cols);
 }
 template <int M>
 static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
@@ -219,7 +234,9 @@ static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows,
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
   const bool wide = cols % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  int8_few_rows_kernel<M><<<static_cast<unsigned>((n_out + 2 * kFewWarps - 1) / (2 * kFewWarps)), kFewWarps * 32, smem, st>>>(
+  // no more blocks than run at once, since each quantises all of x
+  const int64_t want = (n_out + 2 * kFewWarps - 1) / (2 * kFewWarps), most = static_cast<int64_t>(h->sm_count) * (smem > 64 * 1024 ? 2 : 3);
+  int8_few_rows_kernel<M><<<static_cast<unsigned>(want < most ? want : most), kFewWarps * 32, smem, st>>>(
       static_cast<const uint16_t*>(x), ldx, static_cast<int>(rows), static_cast<int>(cols), static_cast<const uint8_t*>(wq), ldw,
       w_scale, static_cast<int>(n_out), static_cast<__nv_bfloat16*>(out), ldo, wide);
   MG_CUDA(cudaGetLastError());

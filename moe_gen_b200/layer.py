@@ -475,7 +475,7 @@ class MoELayer:
         """int8_matmul of bf16 rows x, quantised per token (quantize_rows) in the same call."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
         n_out, ldw, out, ldo = self._int8_args(wq, w_scale, cols, n, out)
-        L.check(self.lib.mg_int8_linear_ws_bytes(n, cols, C.byref(self._size)))
+        L.check(self.lib.mg_int8_linear_ws_bytes(n, n_out, cols, C.byref(self._size)))
         size = self._size.value
         ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         with self._on_device():

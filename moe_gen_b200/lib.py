@@ -71,7 +71,7 @@ SIGNATURES = {
     "mg_combine": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
     "mg_quantize_rows_int8": [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp],
     "mg_int8_matmul": [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp],
-    "mg_int8_linear_ws_bytes": [_i64, _i64, _P(_sz)],
+    "mg_int8_linear_ws_bytes": [_i64, _i64, _i64, _P(_sz)],
     "mg_int8_linear": [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _sz, _vp, _i64, _vp],
     "mg_permute_rows_int8": [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
     "mg_expert_ffn_int8": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],

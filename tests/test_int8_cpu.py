@@ -22,14 +22,17 @@ def test_int8_layers_that_are_refused(built_lib, kw, code):
 
 def test_scratch_of_the_product(built_lib):
     lib, n = L.load(), C.c_size_t()
-    assert lib.mg_int8_linear_ws_bytes(9, 1000, C.byref(n)) == 0 and n.value >= 9 * 1024 + 36
-    assert lib.mg_int8_linear_ws_bytes(8, 12288, C.byref(n)) == 0 and n.value == 0             # one launch, no scratch
-    assert lib.mg_int8_linear_ws_bytes(8, 12289, C.byref(n)) == 0 and n.value >= 8 * 12416
-    assert lib.mg_int8_linear_ws_bytes(0, 1000, C.byref(n)) == 0 and n.value == 0
-    assert lib.mg_int8_linear_ws_bytes(1 << 30, 131071, C.byref(n)) == 0 and n.value >= (1 << 30) * 131072
-    assert lib.mg_int8_linear_ws_bytes(5, 131072, C.byref(n)) == -7
-    assert lib.mg_int8_linear_ws_bytes(5, 0, C.byref(n)) == -2 and lib.mg_int8_linear_ws_bytes(-1, 8, C.byref(n)) == -2
-    assert lib.mg_int8_linear_ws_bytes(5, 8, None) == -1
+    assert lib.mg_int8_linear_ws_bytes(9, 4, 1000, C.byref(n)) == 0 and n.value >= 9 * 1024 + 36
+    assert lib.mg_int8_linear_ws_bytes(8, 20, 12288, C.byref(n)) == 0 and n.value == 0             # one launch, no scratch
+    assert lib.mg_int8_linear_ws_bytes(8, 20, 12289, C.byref(n)) == 0 and n.value >= 8 * 12416
+    assert lib.mg_int8_linear_ws_bytes(4, 1 << 30, 4096, C.byref(n)) == 0 and n.value == 0
+    assert lib.mg_int8_linear_ws_bytes(5, 4096, 4096, C.byref(n)) == 0 and n.value == 0
+    assert lib.mg_int8_linear_ws_bytes(5, 4097, 4096, C.byref(n)) == 0 and n.value >= 5 * 4096
+    assert lib.mg_int8_linear_ws_bytes(0, 8, 1000, C.byref(n)) == 0 and n.value == 0
+    assert lib.mg_int8_linear_ws_bytes(1 << 30, 8, 131071, C.byref(n)) == 0 and n.value >= (1 << 30) * 131072
+    assert lib.mg_int8_linear_ws_bytes(5, 8, 131072, C.byref(n)) == -7
+    assert lib.mg_int8_linear_ws_bytes(5, 8, 0, C.byref(n)) == -2 and lib.mg_int8_linear_ws_bytes(-1, 8, 8, C.byref(n)) == -2
+    assert lib.mg_int8_linear_ws_bytes(5, 0, 8, C.byref(n)) == -2 and lib.mg_int8_linear_ws_bytes(5, 8, 8, None) == -1
 
 
 @pytest.mark.parametrize("name", ["mg_quantize_rows_int8", "mg_int8_matmul", "mg_int8_linear", "mg_permute_rows_int8", "mg_expert_ffn_int8",
