@@ -783,7 +783,7 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   int rc = launch_grouped_gemm(h, p, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
-  rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, dst_row, h_q, d.inter, h_s, st);
+  rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, h_q, d.inter, h_s, st, dst_row, rows_padded);
   if (rc != MG_OK) return rc;
   // chained at every size: the quantising kernel lies between the products (kUnchainedDownTokens; layer, us, unchained and so:
   // V2-Lite 8 tokens 102 and 98, V2-236B 8 tokens 141 and 139, 64 tokens 309 and 307)
@@ -807,7 +807,7 @@ static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T
                               2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st, beside);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_SHARED_GEMM1, st);
-  rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, nullptr, hs_q, d.inter_shared, hs_s, st);
+  rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, hs_q, d.inter_shared, hs_s, st);
   if (rc != MG_OK) return rc;
   return launch_int8_matmul(h, hs_q, d.inter_shared, hs_s, T, base + L.sh2, d.inter_shared,
                             reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st,
@@ -826,7 +826,7 @@ int mg_quantize_rows_int8(mg_handle hh, const void* d_x, int64_t n_rows, int64_t
   MG_REQUIRE(cols <= kInt8MaxK, MG_ERR_LIMIT, "mg_quantize_rows_int8: rows of %lld, at most %d", static_cast<long long>(cols), kInt8MaxK);
   if (n_rows == 0) return MG_OK;
   MG_REQUIRE(d_x && d_q && d_scale, MG_ERR_NULL, "mg_quantize_rows_int8: null pointer");
-  return launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_q, ldq, d_scale, static_cast<cudaStream_t>(stream));
+  return launch_quantize_rows(h, d_x, n_rows, cols, ldx, d_q, ldq, d_scale, static_cast<cudaStream_t>(stream));
 }
 
 static int check_int8_product(int64_t n_rows, int64_t n_out, int64_t cols, const void* d_w, int64_t ldw, const float* d_ws,
@@ -890,7 +890,7 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   if (need == 0) return launch_int8_few(h, d_x, ldx, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, st);
   const int64_t ldq = round_up(cols, 128);
   float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
-  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, nullptr, d_ws, ldq, scale, st);
+  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, d_ws, ldq, scale, st);
   if (rc != MG_OK) return rc;
   h->chain = true;
   rc = launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
@@ -906,6 +906,7 @@ int mg_permute_rows_int8(mg_handle hh, const void* d_q, const float* d_scale, co
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   if (T == 0) return MG_OK;
   MG_REQUIRE(d_q && d_scale && d_dst && d_perm_q && d_perm_scale, MG_ERR_NULL, "mg_permute_rows_int8: null pointer");
+  MG_REQUIRE(aligned16(d_q) && aligned16(d_perm_q), MG_ERR_SHAPE, "mg_permute_rows_int8: rows must begin on a 16-byte boundary");
   return launch_permute_rows(h, d_q, d_dst, T, d_perm_q, static_cast<cudaStream_t>(stream), d_scale, d_perm_scale);
 }
 
@@ -921,6 +922,8 @@ int mg_expert_ffn_int8(mg_handle hh, const void* d_perm_q, const float* d_perm_s
   if (T == 0 || n_rows_padded == 0) return MG_OK;
   MG_REQUIRE(d_perm_q && d_perm_scale && d_pad && d_counts && d_dst && d_packed && d_h_buf && d_h_q && d_h_scale && d_out_rows,
              MG_ERR_NULL, "mg_expert_ffn_int8: null pointer");
+  MG_REQUIRE(aligned16(d_perm_q) && aligned16(d_h_buf) && aligned16(d_h_q) && aligned16(d_out_rows) && aligned16(d_packed), MG_ERR_SHAPE,
+             "mg_expert_ffn_int8: rows and weights must begin on a 16-byte boundary");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc = zero_job_counters(h, st);
   if (rc != MG_OK) return rc;
@@ -938,6 +941,8 @@ int mg_shared_ffn_int8(mg_handle hh, const void* d_xq, const float* d_x_scale, i
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   if (T == 0) return MG_OK;
   MG_REQUIRE(d_xq && d_x_scale && d_packed && d_hs && d_hs_q && d_hs_scale && d_out, MG_ERR_NULL, "mg_shared_ffn_int8: null pointer");
+  MG_REQUIRE(aligned16(d_xq) && aligned16(d_hs) && aligned16(d_hs_q) && aligned16(d_out) && aligned16(d_packed), MG_ERR_SHAPE,
+             "mg_shared_ffn_int8: rows and weights must begin on a 16-byte boundary");
   return shared_ffn_int8(h, d_xq, d_x_scale, T, d_packed, d_hs, d_hs_q, d_hs_scale, d_out, static_cast<cudaStream_t>(stream));
 }
 
@@ -951,6 +956,7 @@ int mg_permute_rows_padded(mg_handle hh, const void* d_x, const int32_t* d_dst, 
              "mg_permute_rows_padded: %lld tokens, %lld rows, %d experts", static_cast<long long>(T), static_cast<long long>(n_rows), n_plan);
   if (n_rows == 0) return MG_OK;
   MG_REQUIRE((T == 0 || (d_x && d_dst)) && d_counts && d_pad && d_perm, MG_ERR_NULL, "mg_permute_rows_padded: null pointer");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_perm), MG_ERR_SHAPE, "mg_permute_rows_padded: rows must begin on a 16-byte boundary");
   return launch_permute_rows_padded(h, d_x, d_dst, T, d_counts, d_pad, n_plan, n_rows, d_perm, static_cast<cudaStream_t>(stream));
 }
 
@@ -961,6 +967,7 @@ int mg_permute_rows_grad(mg_handle hh, const void* d_grad_rows, const int32_t* d
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   if (T == 0) return MG_OK;
   MG_REQUIRE(d_grad_rows && d_dst && d_grad_x, MG_ERR_NULL, "mg_permute_rows_grad: null pointer");
+  MG_REQUIRE(aligned16(d_grad_rows) && aligned16(d_grad_x), MG_ERR_SHAPE, "mg_permute_rows_grad: rows must begin on a 16-byte boundary");
   return launch_permute_rows_grad(h, d_grad_rows, d_dst, T, d_grad_x, static_cast<cudaStream_t>(stream));
 }
 
@@ -974,6 +981,8 @@ int mg_combine_grad(mg_handle hh, const void* d_grad_y, const void* d_out_rows, 
              "mg_combine_grad: %lld tokens, %lld rows, %d experts", static_cast<long long>(T), static_cast<long long>(n_rows), n_plan);
   MG_REQUIRE((d_counts == nullptr) == (d_pad == nullptr), MG_ERR_NULL, "mg_combine_grad: counts and pad_offsets come together");
   MG_REQUIRE(T == 0 || (d_grad_y && d_dst && d_w && (d_out_rows || d_grad_w == nullptr)), MG_ERR_NULL, "mg_combine_grad: null pointer");
+  MG_REQUIRE(aligned16(d_grad_y) && aligned16(d_out_rows) && aligned16(d_grad_rows), MG_ERR_SHAPE,
+             "mg_combine_grad: rows must begin on a 16-byte boundary");
   return launch_combine_grad(h, d_grad_y, d_out_rows, d_dst, d_w, T, d_counts, d_pad, n_plan, n_rows, d_grad_rows, d_grad_w,
                              static_cast<cudaStream_t>(stream));
 }
@@ -1088,7 +1097,7 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   float* perm_s = i8 ? reinterpret_cast<float*>(ws + L.off[WS_PERM_S]) : nullptr;
   auto quantise = [&](cudaStream_t on) {
     launches += 1;
-    return launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, nullptr, xq, d.hidden, xs, on);
+    return launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, xq, d.hidden, xs, on);
   };
   const bool copies = plan_copies(h, T) && !h->stage_timing;        // while stage times are recorded plan and scatter have their own
   if (i8 && !copies) {

@@ -17,16 +17,16 @@ __device__ __forceinline__ uint32_t block_amax(uint32_t pairs, uint32_t* s_max) 
   return a;
 }
 
-// A block per row, or per entry of `list` (rows of the experts' buffers; a negative one is skipped).  Rows of whole 16-byte
+// A block per row, or per entry of `list` (rows of the experts' buffers; one outside their list_rows rows is skipped).  Rows of whole 16-byte
 // vectors; what a thread holds stays in registers between the maximum and the rounding.
 template <int VECS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int64_t ldx, int vecs, const int32_t* list,
-                                                            uint2* q, int64_t ldq, float* scale) {
+                                                            int64_t list_rows, uint2* q, int64_t ldq, float* scale) {
   chain_wait();
   chain_go();
   __shared__ uint32_t s_max[8];
   const int64_t row = list != nullptr ? list[blockIdx.x] : static_cast<int64_t>(blockIdx.x);
-  if (row < 0) return;
+  if (row < 0 || row >= list_rows) return;
   const uint4* src = x + row * ldx;
   uint4 keep[VECS];
   uint32_t m = 0;
@@ -191,9 +191,9 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* 
 
 }  // namespace
 
-// ldx in elements, ldq in bytes; list: nullptr, or the n rows to quantise (cols a multiple of 8 then)
-int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, const int32_t* list, void* q,
-                         int64_t ldq, float* scale, cudaStream_t st) {
+// ldx in elements, ldq in bytes; list: nullptr, or the n rows to quantise of list_rows (cols a multiple of 8 then)
+int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
+                         cudaStream_t st, const int32_t* list, int64_t list_rows) {
   if (n == 0) return MG_OK;
   MG_REQUIRE(n < (1ll << 31), MG_ERR_LIMIT, "quantise: %lld rows", static_cast<long long>(n));
   const int64_t vecs = cols / 8;
@@ -205,7 +205,7 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
     if (threads > 256) threads = 256;
 #define MG_QUANT(V)                                                                                                          \
   MG_CUDA(launch_chained(h, quantize_rows_kernel<V>, static_cast<unsigned>(n), threads, 0, st, static_cast<const uint4*>(x), \
-                         ldx / 8, static_cast<int>(vecs), list, static_cast<uint2*>(q), ldq / 8, scale))
+                         ldx / 8, static_cast<int>(vecs), list, list == nullptr ? n : list_rows, static_cast<uint2*>(q), ldq / 8, scale))
     if (vecs <= 4 * threads) MG_QUANT(4); else MG_QUANT(kQuantVecs);
 #undef MG_QUANT
     return MG_OK;

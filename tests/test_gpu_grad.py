@@ -341,4 +341,13 @@ def test_refusals():
                 lambda: layer.route_topk_grad(torch.zeros(10, 8, device=DEV), idx, w, w[:4])):
         with pytest.raises(ValueError):
             bad()
+    # contiguous views that begin off a 16-byte boundary
+    from moe_gen_b200 import MoeGenError
+    off = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)      # noqa: E731
+    lg = torch.zeros(10, 8, device=DEV)
+    for bad in (lambda: layer.permute_rows(off(x), dst, rows, counts, pad), lambda: layer.permute_rows_grad(off(out), dst),
+                lambda: layer.combine_grad(off(x), out, dst, w, counts, pad), lambda: layer.combine_grad(x, off(out), dst, w, counts, pad),
+                lambda: layer.route_topk_grad(off(lg), idx, w, w)):
+        with pytest.raises(MoeGenError, match="16-byte"):
+            bad()
     layer.close()

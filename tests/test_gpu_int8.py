@@ -435,6 +435,13 @@ def test_refusals(any_layer):
         layer.expert_ffn(torch.zeros(256, 256, dtype=torch.bfloat16, device=DEV), pad, counts)
     with pytest.raises(MoeGenError, match="int8"):
         layer.shared_ffn(x)
+    off = lambda t: torch.zeros(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape)      # noqa: E731
+    q, sc = layer.quantize_rows(x)
+    pq, ps = layer.permute_rows_int8(q, sc, dst, 256)
+    for bad in (lambda: layer.permute_rows_int8(off(q), sc, dst, 256), lambda: layer.expert_ffn_int8(off(pq), ps, pad, counts, dst),
+                lambda: layer.shared_ffn_int8(off(q), sc), lambda: layer.int8_matmul(off(q), sc, w, s)):
+        with pytest.raises(MoeGenError, match="16-byte"):
+            bad()
     bf = _layer(int8=False)
     q, sc = bf.quantize_rows(x)
     with pytest.raises(MoeGenError, match="not int8"):
