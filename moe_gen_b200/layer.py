@@ -433,12 +433,12 @@ class MoELayer:
         A row that holds an infinity or a NaN has scale NaN and q 0."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
         ldq = (cols + 127) // 128 * 128
-        q = torch.empty(n, ldq, dtype=torch.int8, device=self.device)
+        q = torch.empty_strided((n, cols), (ldq, 1), dtype=torch.int8, device=self.device)
         scale = torch.empty(n, dtype=torch.float32, device=self.device)
         with self._on_device():
             L.check(self.lib.mg_quantize_rows_int8(self._h, x.data_ptr(), n, cols, ldx, q.data_ptr(), ldq, scale.data_ptr(),
                                                    self._stream()))
-        return (q if ldq == cols else q[:, :cols]), scale
+        return q, scale
 
     def _int8_args(self, wq: torch.Tensor, w_scale: torch.Tensor, cols: int, n_rows: int, out: Optional[torch.Tensor]):
         n_out, w_cols, ldw = self._rows_of(wq, torch.int8, "wq")
@@ -449,8 +449,7 @@ class MoELayer:
             raise ValueError(f"{w_scale.numel()} scales for {n_out} output channels")
         if out is None:
             ldo = (n_out + 7) // 8 * 8
-            out = torch.empty(n_rows, ldo, dtype=torch.bfloat16, device=self.device)
-            return n_out, ldw, out if ldo == n_out else out[:, :n_out], ldo
+            return n_out, ldw, torch.empty_strided((n_rows, n_out), (ldo, 1), dtype=torch.bfloat16, device=self.device), ldo
         rows, o_cols, ldo = self._rows_of(out, torch.bfloat16, "out")
         if (rows, o_cols) != (n_rows, n_out):
             raise ValueError(f"out {tuple(out.shape)}, expected {(n_rows, n_out)}")
