@@ -43,6 +43,8 @@ static Handle* check(mg_handle hh) {
 
 Handle* check_handle(mg_handle hh) { return check(hh); }
 
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
 static int64_t padded_rows(const Handle* h, int64_t rows) {
   return ((rows + kTileM - 1) / kTileM + h->e_local) * kTileM;
 }
@@ -814,8 +816,6 @@ static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T
                             beside);
 }
 
-static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
 int mg_quantize_rows_int8(mg_handle hh, const void* d_x, int64_t n_rows, int64_t cols, int64_t ldx, void* d_q, int64_t ldq,
                           float* d_scale, void* stream) {
   MG_TRACE("mg_quantize_rows_int8", n_rows);
@@ -1045,6 +1045,8 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   if (T == 0) { h->last_launches = 0; return MG_OK; }   // empty batch: nothing to read or write
   MG_REQUIRE(d_x && (d_gate_w || d_logits_in) && d_packed && d_ws && d_y, MG_ERR_NULL, "mg_moe_forward: null pointer");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_y) && aligned16(d_residual), MG_ERR_SHAPE,
+             "mg_moe_forward: hidden states and output must begin on a 16-byte boundary");
   MG_REQUIRE(h->d.ep_size == 1, MG_ERR_CONFIG, "mg_moe_forward is the single-GPU path (ep_size == 1)");
   MG_REQUIRE(h->d.gating != MG_GATE_SIGMOID_NOAUX_TC || d_bias != nullptr, MG_ERR_NULL,
              "noaux_tc gating needs e_score_correction_bias");

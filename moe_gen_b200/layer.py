@@ -354,7 +354,8 @@ class MoELayer:
     def permute_rows(self, x: torch.Tensor, dst_row: torch.Tensor, rows_padded: int, counts: Optional[torch.Tensor] = None,
                      pad_offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         """perm[dst_row[t, j]] = x[t], zeros in the rows no pick points at.  With the plan's counts and pad_offsets only those
-        rows are written as zeros, in the same launch, instead of all rows before it."""
+        rows are written as zeros, in the same launch, instead of all rows before it (a plan of distinct experts per token: one
+        that a token names twice leaves a counted row without a pick, which then stays as it was)."""
         if counts is not None and pad_offsets is not None:
             self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
             self._check_rows(dst_row, torch.int32, x.shape[0], self.k, "dst_row")
@@ -386,8 +387,9 @@ class MoELayer:
 
     def combine_grad(self, grad_y: torch.Tensor, out_rows: torch.Tensor, dst_row: torch.Tensor, topk_w: torch.Tensor,
                      counts: torch.Tensor, pad_offsets: torch.Tensor, need_rows: bool = True, need_w: bool = True):
-        """Gradients of combine's sum -> (grad_rows like out_rows, zeros where no pick points; grad_w [T, k] fp32), None for the
-        one that is not needed.  The gradient of shared_out is grad_y itself."""
+        """Gradients of combine's sum -> (grad_rows like out_rows, zeros where no pick points, by a plan of distinct experts per
+        token as in permute_rows; grad_w [T, k] fp32), None for the one that is not needed.  The gradient of shared_out is
+        grad_y itself."""
         T = dst_row.shape[0]
         self._check_rows(grad_y, torch.bfloat16, T, self.H, "grad_y")
         self._check_rows(out_rows, torch.bfloat16, None, self.H, "out_rows")

@@ -442,6 +442,10 @@ def test_refusals(any_layer):
                 lambda: layer.shared_ffn_int8(off(q), sc), lambda: layer.int8_matmul(off(q), sc, w, s)):
         with pytest.raises(MoeGenError, match="16-byte"):
             bad()
+    lg = torch.zeros(4, 8, device=DEV)
+    for bad in (lambda: layer.forward_from_logits(off(x), lg), lambda: layer.forward_from_logits(x, lg, out=off(x))):
+        with pytest.raises(MoeGenError, match="16-byte"):
+            bad()
     bf = _layer(int8=False)
     q, sc = bf.quantize_rows(x)
     with pytest.raises(MoeGenError, match="not int8"):
