@@ -351,3 +351,31 @@ def test_refusals():
         with pytest.raises(MoeGenError, match="16-byte"):
             bad()
     layer.close()
+
+
+def test_offsets_beyond_32_bits():
+    """Buffers of rows of more than 2^31 elements: the last tokens, whose picks fill the last expert's segment."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    E, k, H, T = 8, 8, 7168, 37600                                     # 301824 padded rows of 7168: 2.16e9 elements
+    layer = _layer(E=E, k=k, H=H)
+    idx = torch.arange(8, dtype=torch.int32, device=DEV).repeat(T, 1)
+    counts, _, pad, dst = layer.permute_plan(idx)
+    rows = layer.padded_rows(T * k)
+    assert rows * H > 1 << 31 and int(dst.max()) * H > 1 << 31
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device=DEV)
+    x[-5:] = torch.randn(5, H, device=DEV).to(torch.bfloat16)
+    perm = layer.permute_rows(x, dst, rows, counts, pad)
+    assert torch.equal(perm[dst[-5:].long()], x[-5:, None, :].expand(5, k, H)) and not perm[dst[:-5, 7].long()].any()
+    assert not perm[int(pad[-1]):].any()
+    gx = layer.permute_rows_grad(perm, dst)
+    assert torch.equal(gx[-5:], (x[-5:].float() * 8).to(torch.bfloat16)) and not gx[:-5].any()
+    w = torch.full((T, k), 0.5, device=DEV)
+    gr, gw = layer.combine_grad(x, perm, dst, w, counts, pad)
+    assert torch.equal(gr[dst[-5:].long()].float(), perm[dst[-5:].long()].float() * 0.5) and not gr[int(pad[-1]):].any()
+    norm = (x[-5:].double() ** 2).sum(dim=1, keepdim=True)
+    assert ((gw[-5:].double() - norm).abs() <= norm * 96 * 2.0 ** -24).all() and not gw[:-5].any()
+    layer.close()
+    del perm, gr, gx, x
+    torch.cuda.empty_cache()

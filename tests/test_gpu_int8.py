@@ -540,3 +540,31 @@ def test_layers_that_stream_or_shard_refuse_int8_experts():
     with pytest.raises(ValueError, match="int8"):
         EPMoELayer(layer)
     layer.close()
+
+
+def test_offsets_beyond_32_bits(any_layer):
+    """Rows, products and outputs of more than 2^31 elements: the last rows against the first rows' own call."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    m, k, n = 262160, 8200, 16
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)              # 2.15e9 elements
+    tail = torch.randn(33, k, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    x[-33:] = tail.to(DEV)
+    q, s = any_layer.quantize_rows(x)
+    want_q, want_s = quantise(tail)
+    assert torch.equal(q[-33:].cpu().long(), want_q) and torch.equal(s[-33:].cpu(), want_s) and not q[:40].any()
+    wq, ws = _weights(n, k, 2)
+    y = any_layer.int8_matmul(q, s, _strided(wq), ws.to(DEV))
+    assert same(y[-33:].cpu(), product(want_q, want_s, wq, ws)) and not y[:-33].any()
+    del x, q, y
+    torch.cuda.empty_cache()
+    m, k, n = 300000, 64, 7400                                          # 2.2e9 outputs
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+    x[-33:] = tail[:, :k].to(DEV)
+    wq, ws = _weights(n, k, 3)
+    y = any_layer.int8_linear(x, _strided(wq), ws.to(DEV))
+    assert same(y[-33:].cpu(), product(*quantise(tail[:, :k]), wq, ws)) and not y[:64].any()
+    assert any_layer.device_status() == (0, 0)
+    del x, y
+    torch.cuda.empty_cache()
