@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(256) quantize_short_rows_kernel(const uint4* x
 // A product of up to kFewRows rows of x in one launch: every block quantises them into shared memory, and a warp multiplies two
 // weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a pair
 // of SMs for 256 weight rows); here every SM streams a share of the weights.
-constexpr int kFewRows = 8, kFewWarps = 16, kFewSmem = 96 * 1024;
+constexpr int kFewRows = 16, kFewWarps = 16, kFewSmem = 96 * 1024;
 template <int M>
 __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int rows, int cols,
                                                                        const uint8_t* __restrict__ w, int64_t ldw,
@@ -263,11 +263,14 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
 
 // us with x and weights in L2, one launch, and two (quantised, then on the tensor cores): 1 row 4096x4096 4.4 and 12, 8192x8192 8.6
 // and 18; 4 rows 8192x8192 14.0 and 18; 8 rows 1024x1024 4.6 and 8.5, 4096x4096 8.5 and 12.5, 8192x2048 10.3 and 10.2, 8192x8192
-// 25.5 and 18.4 (every weight meets eight rows from shared memory, which bounds it).  So beyond four rows up to 2^24 weights.
+// 25.5 and 18.4 (every weight meets eight rows from shared memory, which bounds it); 16 rows 512x512 5.7 and 8.1, 1024x2048
+// (outputs x inputs) 8.7 and 10.1, 4096x2048 8.9 and 10.2, 8192x1024 12.2 and 9.0, 2048x4096 12.9 and 12.9 (a warp quantises a row
+// by itself there, which takes as long as the row).  So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.
 bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols) {
   int m = 1;
   while (m < rows && m < kFewRows) m *= 2;
-  return rows > 0 && rows <= kFewRows && m * round_up(cols, 16) <= kFewSmem && (rows <= 4 || n_out <= (1 << 24) / cols);
+  if (rows < 1 || rows > kFewRows || m * round_up(cols, 16) > kFewSmem) return false;
+  return rows <= 4 || (rows <= 8 ? n_out <= (1 << 24) / cols : cols <= 2048 && n_out <= (1 << 23) / cols);
 }
 template <int M>
 static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
@@ -293,7 +296,8 @@ int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, c
   if (rows == 1) return launch_few<1>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
   if (rows == 2) return launch_few<2>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
   if (rows <= 4) return launch_few<4>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
-  return launch_few<8>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  if (rows <= 8) return launch_few<8>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
+  return launch_few<16>(h, x, ldx, rows, wq, ldw, w_scale, n_out, cols, out, ldo, st);
 }
 
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,

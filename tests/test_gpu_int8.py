@@ -104,7 +104,8 @@ MATMUL = [(1, 1, 1), (1, 16, 64), (2, 8, 128), (7, 255, 127), (8, 256, 128), (9,
           (385, 512, 128), (700, 1030, 520), (1153, 96, 192),
           # few rows: one launch, as long as their quantised form fits in a block's shared memory
           (1, 4096, 4096), (1, 33, 98304), (1, 8, 98305), (3, 19, 5001), (4, 50, 24576), (4, 3, 24577), (6, 130, 2049), (8, 20, 12288), (8, 21, 12289),
-          (1, 20000, 64), (2, 19001, 72), (7, 4097, 4096), (8, 4096, 1024)]
+          (1, 20000, 64), (2, 19001, 72), (7, 4097, 4096), (8, 4096, 1024), (9, 700, 567), (11, 4096, 2048), (16, 33, 2047),
+          (16, 4097, 2048), (13, 16, 2049), (15, 1030, 72)]
 
 
 @pytest.mark.parametrize("m,n,k", MATMUL)

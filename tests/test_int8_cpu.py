@@ -22,7 +22,10 @@ def test_int8_layers_that_are_refused(built_lib, kw, code):
 
 def test_scratch_of_the_product(built_lib):
     lib, n = L.load(), C.c_size_t()
-    assert lib.mg_int8_linear_ws_bytes(9, 4, 1000, C.byref(n)) == 0 and n.value >= 9 * 1024 + 36
+    assert lib.mg_int8_linear_ws_bytes(17, 4, 1000, C.byref(n)) == 0 and n.value >= 17 * 1024 + 68
+    assert lib.mg_int8_linear_ws_bytes(16, 4096, 2048, C.byref(n)) == 0 and n.value == 0
+    assert lib.mg_int8_linear_ws_bytes(16, 4097, 2048, C.byref(n)) == 0 and n.value >= 16 * 2048
+    assert lib.mg_int8_linear_ws_bytes(9, 8, 2049, C.byref(n)) == 0 and n.value >= 9 * 2176
     assert lib.mg_int8_linear_ws_bytes(8, 20, 12288, C.byref(n)) == 0 and n.value == 0             # one launch, no scratch
     assert lib.mg_int8_linear_ws_bytes(8, 20, 12289, C.byref(n)) == 0 and n.value >= 8 * 12416
     assert lib.mg_int8_linear_ws_bytes(4, 1 << 30, 4096, C.byref(n)) == 0 and n.value == 0
