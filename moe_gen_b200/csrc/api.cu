@@ -787,8 +787,6 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
   rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, h_q, d.inter, h_s, st, dst_row, rows_padded);
   if (rc != MG_OK) return rc;
-  // chained at every size: the quantising kernel lies between the products (kUnchainedDownTokens; layer, us, unchained and so:
-  // V2-Lite 8 tokens 102 and 98, V2-236B 8 tokens 141 and 139, 64 tokens 309 and 307)
   p.a = h_q; p.lda = d.inter; p.a_scales = h_s; p.b = base + L.w2; p.ldb = d.inter;
   p.scales = reinterpret_cast<const float*>(base + L.s2); p.n_per_group = d.hidden; p.K = d.inter;
   p.out = out_rows; p.ldo = d.hidden; p.epilogue = EPI_PLAIN_BF16;
@@ -801,19 +799,18 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
 }
 
 static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T, const void* packed, void* hs, void* hs_q,
-                           float* hs_s, void* out, cudaStream_t st, bool timed = false, bool beside = false) {
+                           float* hs_s, void* out, cudaStream_t st, bool timed = false) {
   const mg_layer_desc& d = h->d;
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
   int rc = launch_int8_matmul(h, xq, d.hidden, xs, T, base + L.sh13, d.hidden, reinterpret_cast<const float*>(base + L.shs13),
-                              2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st, beside);
+                              2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_SHARED_GEMM1, st);
   rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, hs_q, d.inter_shared, hs_s, st);
   if (rc != MG_OK) return rc;
   return launch_int8_matmul(h, hs_q, d.inter_shared, hs_s, T, base + L.sh2, d.inter_shared,
-                            reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st,
-                            beside);
+                            reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st);
 }
 
 int mg_quantize_rows_int8(mg_handle hh, const void* d_x, int64_t n_rows, int64_t cols, int64_t ldx, void* d_q, int64_t ldq,
@@ -892,10 +889,7 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
   rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, d_ws, ldq, scale, st);
   if (rc != MG_OK) return rc;
-  h->chain = true;
-  rc = launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
-  h->chain = false;
-  return rc;
+  return launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
 }
 
 int mg_permute_rows_int8(mg_handle hh, const void* d_q, const float* d_scale, const int32_t* d_dst, int64_t T, void* d_perm_q,
@@ -1077,8 +1071,8 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   h->guard_rows = padded_rows(h, T * d.top_k);     // what this call's dst_row entries may address
   struct RestoreGuard { Handle* h; long long v; ~RestoreGuard() { h->guard_rows = v; h->chain = false; } } restore_guard{h, guard_keep};
   // the launches behind the first one follow by programmatic dependence, unless events of the de-quantisation lie between
-  // them or their times are asked for one by one
-  const bool chain = deq == nullptr && !h->stage_timing;
+  // them or their times are asked for one by one; the int8 products are launched by ordinary dependence
+  const bool chain = deq == nullptr && !h->stage_timing && d.weight_format != MG_WEIGHT_INT8_CHANNEL;
   if (h->stage_timing) MG_CUDA(cudaEventRecord(h->stage_ev[h->stage_calls % kStageSlots][0], st));
   int rc;
   const bool deq_same = h->deq_scratch == deq && h->deq_packed == d_packed && h->deq_stream == st;
@@ -1125,7 +1119,7 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   const bool shared_early = d.inter_shared && (h->opt_shared_early == 1 ||
                                                (h->opt_shared_early == 2 && T <= (h->stage_timing ? 4096 : 16384)));
   auto run_shared = [&](cudaStream_t on, bool timed) {
-    return i8 ? shared_ffn_int8(h, xq, xs, T, d_packed, hs, ws + L.off[WS_SHQ], reinterpret_cast<float*>(ws + L.off[WS_SH_S]), sh, on, timed, on != st)
+    return i8 ? shared_ffn_int8(h, xq, xs, T, d_packed, hs, ws + L.off[WS_SHQ], reinterpret_cast<float*>(ws + L.off[WS_SH_S]), sh, on, timed)
               : shared_ffn(h, d_x, T, d_packed, hs, sh, on, timed);
   };
   if (shared_early) {

@@ -43,7 +43,7 @@ struct TensorMapCache {
   static constexpr int kEntries = 96;
   struct Entry {
     const void* base;
-    uint64_t rows, cols, ld;
+    uint64_t rows, cols;
     uint32_t box_rows, kind;
     CUtensorMap map;
   };
@@ -55,7 +55,7 @@ struct TensorMapCache {
 // fetches all steps of a stage: with a copy per step and per 64 or 16 tokens the kernel's token role was late at 32 to 128
 // tokens per expert (V3, 4096 skewed tokens 4.89 against 4.77 ms).
 struct WlMaps {
-  CUtensorMap w;                // FP8: weights [blocks of 128 rows][128][K]; bf16, int8 gate/up: [8][blocks][16][K]; int8: [rows][K]
+  CUtensorMap w;                // FP8: weights [blocks of 128 rows][128][K]; bf16: [8][blocks][16][K]
   CUtensorMap t[8];             // 16 .. 128 tokens
   CUtensorMap t8;               // 8 tokens: jobs of up to 32 leave out groups of eight without a live one
   CUtensorMap t2[5];            // 16 .. 80 tokens, one step: the parts of a job of more than 256
@@ -65,12 +65,12 @@ struct WlMapCache {
   static constexpr int kEntries = 24;      // a forward launches 2, with weights de-quantised first 16
   struct Key {
     const void *a, *b, *out;
-    int64_t a_rows, w_rows, ldo, lda, ldb;
-    int K, type;
-    bool swiglu;
+    int64_t a_rows, w_rows, ldo;
+    int K;
+    bool fp8, swiglu;
     bool operator==(const Key& o) const {
-      return a == o.a && b == o.b && out == o.out && a_rows == o.a_rows && w_rows == o.w_rows && ldo == o.ldo &&
-             lda == o.lda && ldb == o.ldb && K == o.K && type == o.type && swiglu == o.swiglu;
+      return a == o.a && b == o.b && out == o.out && a_rows == o.a_rows && w_rows == o.w_rows && ldo == o.ldo && K == o.K &&
+             fp8 == o.fp8 && swiglu == o.swiglu;
     }
   };
   struct Entry { Key key; WlMaps maps; };
@@ -263,8 +263,7 @@ bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols);        // fe
 int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
                     int64_t n_out, int64_t cols, void* out, int64_t ldo, cudaStream_t st);
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
-                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st,
-                       bool beside = false);
+                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st);
 
 // weights (pack.cu) --------------------------------------------------------------------
 int launch_pack_expert(const Handle* h, int local_expert, const void* g, const void* u,
@@ -286,10 +285,9 @@ struct GemmProblem {
   const void* b;          // [n_groups * n_per_group, K] row-major ("N x K, K-major"), bf16 or FP8 e4m3
   bool b_fp8;             // B holds e4m3 bytes; `scales` holds fp32 [rows/128][K/128]
   const float* scales;
-  bool b_i8;              // A and B hold int8: a_scales [a_rows], `scales` [rows of B]; weight-lane GEMM, grouped or dense
+  bool b_i8;              // A and B hold int8: a_scales [a_rows], `scales` [rows of B]; grouped or dense (gemm_i8.cu)
   const float* a_scales;
   int64_t lda, ldb;       // int8: bytes between the rows of A and of B
-  bool beside;            // int8, dense: runs beside other kernels, on few SMs where it has few jobs
   int n_groups;
   int n_per_group;        // rows of B per group (2I for SwiGLU, H for down, E for the gate)
   int K;
@@ -316,6 +314,7 @@ struct RingPlan {
 };
 RingPlan ring_plan(int n_per_group, int K, int64_t a_rows, int n_groups, size_t budget_bytes);
 int launch_grouped_gemm(const Handle* h, const GemmProblem& p, cudaStream_t st);
+int launch_gemm_i8(const Handle* h, const GemmProblem& p, cudaStream_t st);     // int8 (gemm_i8.cu)
 int launch_gemm_wl(const Handle* h, const GemmProblem& p, cudaStream_t st);     // weights on the lanes (gemm_wl.cu)
 int launch_wait_probe(const Handle* h, int limit_ms, cudaStream_t st);
 

@@ -1380,13 +1380,12 @@ static EncodeTiledFn get_encode_fn() {
 // A layer calls the same few (pointer, shape) combinations on every forward, so the encoded maps
 // are kept in the handle: a forward at decode sizes is short enough for ~60 driver calls to show.
 int encode_2d(const Handle* h, CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows,
-              TensorMapKind kind, uint64_t ld) {
-  if (ld == 0) ld = cols;
+              TensorMapKind kind) {
   const bool fp8 = kind == TM_FP8_ROWS;
   TensorMapCache& c = h->tmaps;
   for (int i = 0; i < c.used; ++i) {
     const TensorMapCache::Entry& e = c.e[i];
-    if (e.base == base && e.rows == rows && e.cols == cols && e.ld == ld && e.box_rows == box_rows && e.kind == kind) {
+    if (e.base == base && e.rows == rows && e.cols == cols && e.box_rows == box_rows && e.kind == kind) {
       *map = e.map;
       return MG_OK;
     }
@@ -1394,7 +1393,7 @@ int encode_2d(const Handle* h, CUtensorMap* map, const void* base, uint64_t rows
   EncodeTiledFn fn = get_encode_fn();
   MG_REQUIRE(fn != nullptr, MG_ERR_DRIVER, "cuTensorMapEncodeTiled not available from the driver");
   cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld * (fp8 ? 1 : 2)};
+  cuuint64_t strides[1] = {cols * (fp8 ? 1 : 2)};
   cuuint32_t box[2] = {static_cast<cuuint32_t>(kind == TM_OUT_PIECE ? 32 : kind == TM_OUT_16 ? 16 : BK), box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
@@ -1406,7 +1405,7 @@ int encode_2d(const Handle* h, CUtensorMap* map, const void* base, uint64_t rows
              static_cast<int>(r), static_cast<unsigned long long>(rows), static_cast<unsigned long long>(cols),
              box_rows);
   TensorMapCache::Entry& e = c.e[c.next];
-  e.base = base; e.rows = rows; e.cols = cols; e.ld = ld; e.box_rows = box_rows; e.kind = kind; e.map = *map;
+  e.base = base; e.rows = rows; e.cols = cols; e.box_rows = box_rows; e.kind = kind; e.map = *map;
   c.next = (c.next + 1) % TensorMapCache::kEntries;
   if (c.used < TensorMapCache::kEntries) ++c.used;
   return MG_OK;
@@ -1560,7 +1559,7 @@ static int launch_ring_gemm(const Handle* h, const GemmProblem& p, cudaStream_t 
 int launch_grouped_gemm(const Handle* h, const GemmProblem& p, cudaStream_t st) {
   const bool dense = p.pad_offsets == nullptr;
   if (p.a_rows <= 0 || (dense && p.dense_rows <= 0)) return MG_OK;
-  if (p.b_i8) return launch_gemm_wl(h, p, st);
+  if (p.b_i8) return launch_gemm_i8(h, p, st);
   MG_REQUIRE(p.K % BK == 0, MG_ERR_SHAPE, "GEMM K=%d must be a multiple of %d", p.K, BK);
   MG_REQUIRE(p.n_groups >= 1 && p.n_groups <= kMaxExperts, MG_ERR_SHAPE, "n_groups=%d out of range", p.n_groups);
   int bn;

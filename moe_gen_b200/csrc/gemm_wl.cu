@@ -1,9 +1,6 @@
 // Grouped GEMM with the weights on the accumulator's lanes: D[weight row, token] = W_e[N, K] . X_e[rows, K]^T, with FP8
-// weights (W8A16), with bf16 weights, and with int8 weights and tokens (W8A8).  What follows is about the FP8 form; the bf16
-// form has no converters, takes both operands from shared memory and uses all 512 columns of tensor memory for accumulators.
-// The int8 form is the bf16 form with 128 elements to a step of 128 bytes and kind::i8 MMAs: the sums are exact in 32 bits,
-// and the epilogue multiplies them by the scale of the weight row (lane) and that of the token (column).  It also takes one
-// dense weight matrix of any size (the last tile of rows and the last step of K arrive padded with zeros).
+// weights (W8A16) and with bf16 weights.  What follows is about the FP8 form; the bf16 form has no converters, takes both
+// operands from shared memory and uses all 512 columns of tensor memory for accumulators.
 //
 // A cluster of two CTAs (one SM pair, tcgen05 cta_group::2, M = 256) computes 256 weight rows against up to
 // 384 tokens of one expert.  Compared with tokens on the lanes (gemm.cu):
@@ -73,7 +70,6 @@ constexpr int WL_PIECE = 1024;                 // epilogue staging: 32 tokens x 
 constexpr int WL_JOBS = 1;                     // announced ahead: few, so that the last jobs go to whoever is free
 constexpr int WL_AHEAD = 8;                     // weight stages brought into L2 while the kernel before still runs
 constexpr int WL_MAIL = 4;                     // job numbers on their way from the leader to the other CTA
-enum WlType { WL_BF16 = 0, WL_FP8 = 1, WL_INT8 = 2 };
 template <bool FP8>
 struct WlCfg {
   static constexpr int MAX_TOKENS = 384;                       // per job
@@ -99,15 +95,8 @@ struct WlArgs {
   int n_tiles;                  // 256-row weight tiles per group
   int n_per_group;
   int k_steps;                  // K / 64
-  const float* scales;          // FP8: [rows / 128][K / 128]; int8: of every weight row
+  const float* scales;          // [rows / 128][K / 128]
   int scale_cols;
-  const float* token_scales;    // int8: of every token row
-  int dense_tiles;              // int8: token tiles of dense_rows
-  int dense_rows;               // int8: > 0: one weight matrix, these token rows from 0 on; pad_offsets and counts are not read
-  int w_rows;                   // int8: rows of the weights in all
-  int ragged;                   // int8: K is no multiple of a step; tokens come step by step
-  uint16_t* out;                // int8: for the columns behind the last whole 16 bytes of a row
-  long long ldo;
   int32_t* next_job;            // counts the jobs handed out beyond each pair's first; nullptr: every n_pairs-th job
   int32_t* status;
   int rows;                     // of the token matrix: the first row number behind it
@@ -174,16 +163,6 @@ __device__ __forceinline__ Job locate_job(int job, const int* s_pad, const int* 
   return j;
 }
 
-// D (int32) += A * B of signed bytes on the SM pair, 32 of K
-__device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 // D += A(tensor memory) * B(shared memory) on the SM pair
 __device__ __forceinline__ void tc_mma_pair_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                uint32_t accumulate) {
@@ -254,16 +233,9 @@ __device__ __forceinline__ int peek(const int32_t* p) {
   return v;
 }
 
-// the sum scaled by its weight row's and its token's scale, as fp32 bits
-__device__ __forceinline__ uint32_t scaled(uint32_t sum, float w, float t) {
-  return __float_as_uint(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int>(sum)), t), w));
-}
-
-template <int EPI, int TYPE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WlCfg<TYPE == WL_FP8>::THREADS, 1)
+template <int EPI, bool FP8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WlCfg<FP8>::THREADS, 1)
 grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
-  constexpr bool FP8 = TYPE == WL_FP8, I8 = TYPE == WL_INT8;
-  constexpr int STEP_ELEMS = I8 ? 128 : WL_K;        // K elements of a 128-byte step
   using C = WlCfg<FP8>;
   constexpr bool SWIGLU = EPI == EPI_SWIGLU_BF16;
   extern __shared__ uint8_t smem_raw[];
@@ -311,10 +283,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
   }
   // token tiles before each expert: lane sums of runs of 16 experts, warp scan, runs written out
   auto count_tiles = [&]() {
-    if (I8 && g.dense_rows > 0) {
-      if (lane < 2) s_jp[lane] = lane * g.dense_tiles;
-      return;
-    }
     constexpr int RUN = kMaxExperts / 32;
     int sum = 0;
     for (int i = 0; i < RUN; ++i) {
@@ -353,8 +321,7 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
   // and 137.0, 512 tokens 257, 237, 237 and 239; Mixtral 61 tokens 469, 465, 465 and 465; V2-236B 512 tokens 1241, 1228, 1225
   // and 1228; V3, where converting bounds it, 8 tokens 591, 595, 595 and 596, 64 tokens 2124, 2143, 2149 and 2143.
   if (g.chained) {
-    for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x)
-      s_cnt[i] = I8 && g.dense_rows > 0 ? g.dense_rows : min(max(peek(g.counts + i), 0), 1 << 16);
+    for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x) s_cnt[i] = min(max(peek(g.counts + i), 0), 1 << 16);
     __syncthreads();
     if (warp == 3) count_tiles();
     __syncthreads();
@@ -364,20 +331,18 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
     const int steps = min(g.k_steps / (FP8 ? 2 : 1), WL_AHEAD);
     for (int kb = 0; kb < steps; ++kb) {
       if (FP8) tma_prefetch_3d(&maps.w, kb * 128, SWIGLU ? r0 * 64 : 0, SWIGLU ? blk : blk + r0);
-      else if (I8 && !SWIGLU) tma_prefetch_2d(&maps.w, kb * STEP_ELEMS, (blk + r0) * 128);
-      else tma_prefetch_4d(&maps.w, kb * STEP_ELEMS, 0, SWIGLU ? blk : blk + r0, SWIGLU ? r0 * 4 : 0);
+      else tma_prefetch_4d(&maps.w, kb * WL_K, 0, SWIGLU ? blk : blk + r0, SWIGLU ? r0 * 4 : 0);
     }
   }
   chain_wait();
   chain_go();
   bool same = g.chained;
-  const bool dense = I8 && g.dense_rows > 0;
   for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x) {
-    s_pad[i] = dense ? 0 : g.pad_offsets[i];
-    same = same && (dense || g.counts[i] == s_cnt[i]);
+    s_pad[i] = g.pad_offsets[i];
+    same = same && g.counts[i] == s_cnt[i];
   }
   if (!__syncthreads_and(same)) {
-    for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x) s_cnt[i] = dense ? g.dense_rows : g.counts[i];
+    for (int i = threadIdx.x; i < g.n_groups; i += blockDim.x) s_cnt[i] = g.counts[i];
     __syncthreads();
     if (warp == 3) count_tiles();
     __syncthreads();
@@ -426,9 +391,8 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
             const uint32_t fb = smem_u32(&wfull[r.i]), dst = w_base + r.i * WL_W_STAGE;
             if (rank == 0) mbar_expect_tx(fb, 2 * WL_W_STAGE);           // of both CTAs
             // SwiGLU: 16 gate rows, the 16 up rows of the same outputs, the next 16 gate rows ...
-            if (SWIGLU) tma_load_4d_pair(dst, &maps.w, kb * STEP_ELEMS, 0, blk, r0 * 4, fb);
-            else if (I8) tma_load_2d_pair(dst, &maps.w, kb * STEP_ELEMS, (blk + r0) * 128, fb);
-            else tma_load_4d_pair(dst, &maps.w, kb * STEP_ELEMS, 0, blk + r0, 0, fb);
+            if (SWIGLU) tma_load_4d_pair(dst, &maps.w, kb * WL_K, 0, blk, r0 * 4, fb);
+            else tma_load_4d_pair(dst, &maps.w, kb * WL_K, 0, blk + r0, 0, fb);
           }
         }
       }
@@ -455,13 +419,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
             const uint32_t fb = smem_u32(&tfull[r.i]);
             const uint32_t dst = t_base + r.i * C::T_STAGE;
             if (rank == 0) mbar_expect_tx(fb, kpt * 32 * 128);
-            if (I8 && g.ragged) {
-              for (int i = 0; i < kpt; ++i) {
-                tma_load_2d_pair(dst + i * 1024, &maps.t8, (kb + i) * STEP_ELEMS, g0, fb);
-                tma_load_2d_pair(dst + (kpt + i) * 1024, &maps.t8, (kb + i) * STEP_ELEMS, g1, fb);
-              }
-              continue;
-            }
             tma_load_3d_pair(dst, &maps.t8, 0, g0, kb, fb);
             tma_load_3d_pair(dst + kpt * 1024, &maps.t8, 0, g1, kb, fb);
           }
@@ -474,11 +431,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
           const uint32_t fb = smem_u32(&tfull[r.i]);
           const uint32_t dst = t_base + r.i * C::T_STAGE;
           if (rank == 0) mbar_expect_tx(fb, kpt * j.n_tok * 128);      // steps beyond K arrive as zeros
-          if (I8 && g.ragged) {
-            for (int i = 0; i < kpt; ++i) tma_load_2d_pair(dst + i * j.n_tok * 64, m1, (kb + i) * STEP_ELEMS, row1, fb);
-            if (h2 > 0) tma_load_2d_pair(dst + h1 * 128, m2, kb * STEP_ELEMS, row2, fb);
-            continue;
-          }
           tma_load_3d_pair(dst, m1, 0, row1, kb, fb);
           if (h2 > 0) tma_load_3d_pair(dst + h1 * 128, m2, 0, row2, kb, fb);
         }
@@ -490,9 +442,8 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
       Ring rt, ra, rj;
       uint32_t seq = 0u, parts = 0u;       // jobs, and waits for a part of the accumulator
       int n_before = 0;
-      // kind::f16: D fp32 (1 at bit 4), A bf16 (bit 7), B bf16 (bit 10); kind::i8: D int32 (2 at bit 4), A and B signed (the
-      // same bits); both K-major, N>>3 at 17, M>>4 at 24
-      const uint32_t id0 = ((I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(256 >> 4) << 24);
+      // kind::f16: D fp32 (bit 4), A bf16 (bit 7), B bf16 (bit 10), both K-major, N>>3 at 17, M>>4 at 24
+      const uint32_t id0 = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(256 >> 4) << 24);
       bool ok = true;
       Job j;
       while (take_job(j, rj)) {
@@ -554,11 +505,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
 #pragma unroll
             for (int k = 0; k < WL_K / 16; ++k) {
               const uint32_t accumulate = (kb | k) != 0 ? 1u : 0u;
-              if (I8) {
-                tc_mma_i8_pair(d, da + 2 * k, db + 2 * k, id1, accumulate);
-                if (n2 > 0) tc_mma_i8_pair(d + n1, da + 2 * k, db2 + 2 * k, id2, accumulate);
-                continue;
-              }
               tc_mma_bf16_pair(d, da + 2 * k, db + 2 * k, id1, accumulate);
               if (n2 > 0) tc_mma_bf16_pair(d + n1, da + 2 * k, db2 + 2 * k, id2, accumulate);
             }
@@ -619,18 +565,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
       return piece0 + piece * WL_PIECE;
     };
     auto send_piece = [&](int col, int row) {
-      if (I8 && !SWIGLU && (g.n_per_group & 7) != 0 && col + 32 > g.n_per_group) {
-        // a dense product's last columns: the copy engine stores whole 16 bytes, and would write zeros behind the row's end
-        __syncwarp();
-        if (col + lane < g.n_per_group) {
-          const uint8_t* p = pieces + (warp - 4) * 2 * WL_PIECE + piece * WL_PIECE;
-          for (int t = 0; t < 16 && row + t < g.rows; ++t)
-            g.out[(row + t) * g.ldo + col + lane] =
-                *reinterpret_cast<const uint16_t*>(p + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2);
-        }
-        __syncwarp();
-        return;
-      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) tma_store_2d(&maps.c, col, row, piece0 + piece * WL_PIECE);
@@ -643,16 +577,6 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
     while (more) {
       const Job j = next;
       more = take_job_warp(next, rj);
-      // int8: scales of the weight rows of this lane's registers (va: lane / 4 and 8 further, vb: the up rows or 16 further)
-      float ws[4];
-      if (I8) {
-        const int r = j.b_row + static_cast<int>(rank) * (SWIGLU ? 64 : 128) + quarter * (SWIGLU ? 16 : 32) + (lane >> 2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int ri = r + 8 * (i & 1) + (i >> 1) * (SWIGLU ? 128 : 16);
-          ws[i] = ri < g.w_rows ? g.scales[ri] : 0.f;
-        }
-      }
       const uint32_t h = seq & 1u;
       if (!wait_warp(smem_u32(&dfull[h]), (seq >> 1) & 1u, abort_flag, g.status, 56)) break;
       ++seq;
@@ -674,30 +598,12 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
       for (int i = i0; i < chunks; i += 2) {
         const int c = 32 * (h ? i : chunks - 1 - i);
         uint32_t va[16], vb[16];                // lanes 0-15 and 16-31 of the quarter
-        float2 ts[4];                           // int8: scales of this lane's tokens
-        if (I8) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = j.row0 + c + 8 * x + 2 * (lane & 3);
-            ts[x].x = r < g.rows ? g.token_scales[r] : 0.f;
-            ts[x].y = r + 1 < g.rows ? g.token_scales[r + 1] : 0.f;
-          }
-        }
         tc_ld_16x32(taddr + c, va);
         tc_ld_16x32(taddr + (16u << 16) + c, vb);
         tc_ld_wait();
         // this warp's share is in registers
         if (i < shared && i + 2 >= shared) release(dpart);
         if (i + 2 >= chunks) release(&dempty[h]);
-        if (I8) {
-          if (!SWIGLU && col0 >= g.n_per_group) continue;        // behind the last row of a dense weight matrix
-#pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const float t = x & 1 ? ts[x >> 2].y : ts[x >> 2].x;
-            va[x] = scaled(va[x], ws[(x >> 1) & 1], t);
-            vb[x] = scaled(vb[x], ws[2 + ((x >> 1) & 1)], t);
-          }
-        }
         if (SWIGLU) {
           // va: gate rows, vb: the up rows of the same 16 outputs; a piece is 32 tokens x 16 outputs
           uint32_t p[8];
@@ -792,61 +698,30 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
   }
 }
 
-template <int EPI, int TYPE>
+template <int EPI, bool FP8>
 int launch_kernel(const Handle* h, const WlMaps& maps, const WlArgs& a, int grid, cudaStream_t st) {
-  using C = WlCfg<TYPE == WL_FP8>;
+  using C = WlCfg<FP8>;
   static bool done[64];
   if (!(h->device >= 0 && h->device < 64 && done[h->device])) {
-    MG_CUDA(cudaFuncSetAttribute(grouped_gemm_wl_kernel<EPI, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    MG_CUDA(cudaFuncSetAttribute(grouped_gemm_wl_kernel<EPI, FP8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  static_cast<int>(C::SMEM)));
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
-  MG_CUDA(launch_chained(h, grouped_gemm_wl_kernel<EPI, TYPE>, grid, C::THREADS, C::SMEM, st, maps, a));
+  MG_CUDA(launch_chained(h, grouped_gemm_wl_kernel<EPI, FP8>, grid, C::THREADS, C::SMEM, st, maps, a));
   return MG_OK;
 }
 
 // From the handle's cache, by what the maps are made of: a forward's launches are few and the same ones again.  Encoding the
 // maps anew, as for a batch size not seen lately, takes a forward 3 us more on the host (V2-Lite 36 and 39 us).
-template <int TYPE>
+template <bool FP8>
 int wl_maps(const Handle* h, const GemmProblem& p, bool swiglu, const WlMaps** out) {
-  constexpr bool FP8 = TYPE == WL_FP8, I8 = TYPE == WL_INT8;
   WlMapCache& cache = h->wl_maps;
-  const WlMapCache::Key key{p.a, p.b, p.out, p.a_rows, static_cast<int64_t>(p.n_groups) * p.n_per_group, p.ldo, p.lda, p.ldb, p.K,
-                            TYPE, swiglu};
+  const WlMapCache::Key key{p.a, p.b, p.out, p.a_rows, static_cast<int64_t>(p.n_groups) * p.n_per_group, p.ldo, p.K, FP8, swiglu};
   for (int i = 0; i < cache.used; ++i)
     if (cache.e[i].key == key) { *out = &cache.e[i].maps; return MG_OK; }
-  auto keep = [&](const WlMaps& maps) {
-    WlMapCache::Entry& e = cache.e[cache.next];
-    e.key = key;
-    e.maps = maps;
-    cache.next = (cache.next + 1) % WlMapCache::kEntries;
-    if (cache.used < WlMapCache::kEntries) ++cache.used;
-    *out = &e.maps;
-    return MG_OK;
-  };
   WlMaps m;
   const uint64_t K = static_cast<uint64_t>(p.K), blocks = static_cast<uint64_t>(key.w_rows) / 128;
   const uint32_t both = swiglu ? 2 : 1;
-  if (I8) {
-    // bytes; tokens of a ragged K are fetched step by step, so that what lies behind a row's end is not read
-    const uint64_t rows = static_cast<uint64_t>(p.a_rows), w_rows = static_cast<uint64_t>(key.w_rows);
-    const uint64_t lda = static_cast<uint64_t>(p.lda), ldb = static_cast<uint64_t>(p.ldb);
-    const bool ragged = K % 128 != 0;
-    int rc = swiglu ? encode_map(&m.w, p.b, true, 4, {K, 16, blocks, 8}, {ldb, 128 * ldb, 16 * ldb}, {128, 16, 2, 4})
-                    : encode_map(&m.w, p.b, true, 2, {K, w_rows}, {ldb}, {128, 128});
-    for (int i = 0; i < 14 && rc == MG_OK; ++i) {
-      const uint32_t n = i == 13 ? 8 : 16 * (i < 8 ? i + 1 : i - 7);
-      const uint32_t kpt = i < 8 ? steps_per_stage<false>(n) : i == 13 ? steps_per_stage<false>(16) : 1;
-      CUtensorMap* map = i < 8 ? &m.t[i] : i < 13 ? &m.t2[i - 8] : &m.t8;
-      rc = ragged ? encode_map(map, p.a, true, 2, {K, rows}, {lda}, {128, n})
-                  : encode_map(map, p.a, true, 3, {128, rows, K / 128}, {lda, 128}, {128, n, kpt});
-    }
-    if (rc == MG_OK)
-      rc = encode_2d(h, &m.c, p.out, rows, swiglu ? static_cast<uint64_t>(p.ldo) : w_rows / p.n_groups, swiglu ? 32 : 16,
-                     swiglu ? TM_OUT_16 : TM_OUT_PIECE, static_cast<uint64_t>(p.ldo));
-    if (rc != MG_OK) return rc;
-    return keep(m);
-  }
   int rc = FP8 ? encode_map(&m.w, p.b, true, 3, {K, 128, blocks}, {K, 128 * K}, {128, 128 / both, both})
                : encode_map(&m.w, p.b, false, 4, {K, 16, blocks, 8}, {2 * K, 256 * K, 32 * K}, {WL_K, 16, both, 8 / both});
   const uint64_t rows = static_cast<uint64_t>(p.a_rows), steps = K / WL_K;
@@ -860,84 +735,49 @@ int wl_maps(const Handle* h, const GemmProblem& p, bool swiglu, const WlMaps** o
   if (rc == MG_OK)
     rc = encode_2d(h, &m.c, p.out, rows, static_cast<uint64_t>(p.ldo), swiglu ? 32 : 16, swiglu ? TM_OUT_16 : TM_OUT_PIECE);
   if (rc != MG_OK) return rc;
-  return keep(m);
-}
-
-// Token tiles of a dense product.  A job takes about as long as its tokens and 64 more: its MMAs, or, alone on its pair, the
-// latency of its rings (three token stages, which hold eight steps of 32 tokens and one of 256 or more).  So few tokens to a
-// job while one round of jobs holds them, and rounds that come out even beyond.  us, tokens x outputs x inputs, jobs of up to
-// 384 tokens and so: 128x4096x4096 14.5 and 12.5, 256x1024x8192 37 and 16.6, 256x4096x4096 22.6 and 12.5, 512x512x8192 38 and
-// 18.6, 1024x1024x1024 14.5 and 8.3, 1024x2048x4096 24.7 and 16.5; in more than a round 256x4096x4096 18.6, 1024x2048x4096 20.6.
-// Beside the routing kernels on another stream, which wait for the SMs that more pairs take, as few jobs as there can be
-// (V2-Lite layer 201 tokens 139 and, in more jobs, 143, 512 tokens 154 and 162).
-int dense_token_tiles(int64_t rows, int n_tiles, int pairs, bool beside) {
-  const int64_t units = (rows + 31) / 32, first = (rows + WlCfg<false>::MAX_TOKENS - 1) / WlCfg<false>::MAX_TOKENS;
-  if (beside) return static_cast<int>(first);
-  int64_t most = 2 * first > pairs / n_tiles ? 2 * first : pairs / n_tiles, best = first;
-  if (most > units) most = units;
-  if (most > first + 128) most = first + 128;
-  double best_cost = 1e30;
-  for (int64_t nt = first; nt <= most; ++nt) {
-    const double cost = static_cast<double>((n_tiles * nt + pairs - 1) / pairs) * (2.0 + static_cast<double>(units) / nt);
-    if (cost < best_cost) { best_cost = cost; best = nt; }
-  }
-  return static_cast<int>(best);
+  WlMapCache::Entry& e = cache.e[cache.next];
+  e.key = key;
+  e.maps = m;
+  cache.next = (cache.next + 1) % WlMapCache::kEntries;
+  if (cache.used < WlMapCache::kEntries) ++cache.used;
+  *out = &e.maps;
+  return MG_OK;
 }
 
 }  // namespace
 
 int launch_gemm_wl(const Handle* h, const GemmProblem& p, cudaStream_t st) {
-  const bool swiglu = p.epilogue == EPI_SWIGLU_BF16, dense = p.pad_offsets == nullptr;
-  MG_REQUIRE((!dense || p.b_i8) && ((!p.b_fp8 && !p.b_i8) || p.scales != nullptr) && (!p.b_i8 || p.a_scales != nullptr) &&
-             (swiglu || p.epilogue == EPI_PLAIN_BF16),
-             MG_ERR_CONFIG, "weight-lane GEMM: grouped weights, FP8 and int8 with scales, and bf16 outputs only");
-  if (p.b_i8) {
-    MG_REQUIRE(p.K >= 1 && p.K <= kInt8MaxK && p.lda % 16 == 0 && p.ldb % 16 == 0 && p.lda >= p.K && p.ldb >= p.K && p.ldo % 8 == 0 &&
-               (dense || p.n_per_group % 256 == 0) && (!swiglu || (p.n_per_group % 256 == 0 && p.ldo % 16 == 0)),
-               MG_ERR_SHAPE, "int8 GEMM: K=%d, N=%d, row strides %lld, %lld and %lld", p.K, p.n_per_group,
-               static_cast<long long>(p.lda), static_cast<long long>(p.ldb), static_cast<long long>(p.ldo));
-  } else {
-    MG_REQUIRE(p.K % (p.b_fp8 ? 128 : WL_K) == 0 && p.n_per_group % 256 == 0 && p.ldo % 16 == 0, MG_ERR_SHAPE,
-               "weight-lane GEMM: K=%d, N per expert=%d", p.K, p.n_per_group);
-  }
+  const bool swiglu = p.epilogue == EPI_SWIGLU_BF16;
+  MG_REQUIRE(p.pad_offsets != nullptr && (!p.b_fp8 || p.scales != nullptr) && (swiglu || p.epilogue == EPI_PLAIN_BF16),
+             MG_ERR_CONFIG, "weight-lane GEMM: grouped weights, FP8 with scales, and bf16 outputs only");
+  MG_REQUIRE(p.K % (p.b_fp8 ? 128 : WL_K) == 0 && p.n_per_group % 256 == 0 && p.ldo % 16 == 0, MG_ERR_SHAPE,
+             "weight-lane GEMM: K=%d, N per expert=%d", p.K, p.n_per_group);
   const WlMaps* maps = nullptr;
-  const int rc = p.b_fp8 ? wl_maps<WL_FP8>(h, p, swiglu, &maps)
-                 : p.b_i8 ? wl_maps<WL_INT8>(h, p, swiglu, &maps) : wl_maps<WL_BF16>(h, p, swiglu, &maps);
+  const int rc = p.b_fp8 ? wl_maps<true>(h, p, swiglu, &maps) : wl_maps<false>(h, p, swiglu, &maps);
   if (rc != MG_OK) return rc;
   WlArgs a;
   a.pad_offsets = p.pad_offsets;
   a.counts = p.counts;
   a.n_groups = p.n_groups;
-  a.n_tiles = (p.n_per_group + 255) / 256;
+  a.n_tiles = p.n_per_group / 256;
   a.n_per_group = p.n_per_group;
-  a.k_steps = p.b_i8 ? (p.K + 127) / 128 : p.K / WL_K;
+  a.k_steps = p.K / WL_K;
   a.scales = p.scales;
   a.scale_cols = p.K / 128;
-  a.token_scales = p.a_scales;
-  a.dense_rows = dense ? static_cast<int>(p.dense_rows) : 0;
-  a.w_rows = p.n_groups * p.n_per_group;
-  a.ragged = p.b_i8 && p.K % 128 != 0 ? 1 : 0;
-  a.out = static_cast<uint16_t*>(p.out);
-  a.ldo = p.ldo;
   a.next_job = p.next_job;
   a.status = h->d_status;
   a.rows = static_cast<int>(p.a_rows);
   a.chained = h->chain ? 1 : 0;
   const int max_tokens = p.b_fp8 ? WlCfg<true>::MAX_TOKENS : WlCfg<false>::MAX_TOKENS;
-  if (dense) a.dense_tiles = dense_token_tiles(p.dense_rows, a.n_tiles, h->sm_count / 2, p.beside);
-  else a.dense_tiles = 0;
-  const int64_t tiles = dense ? a.dense_tiles : (p.a_rows + max_tokens - 1) / max_tokens + p.n_groups;
+  const int64_t tiles = (p.a_rows + max_tokens - 1) / max_tokens + p.n_groups;
   int64_t pairs = h->sm_count / 2;
   if (tiles * a.n_tiles < pairs) pairs = tiles * a.n_tiles;
   const int grid = static_cast<int>(2 * pairs);
   if (p.b_fp8)
-    return swiglu ? launch_kernel<EPI_SWIGLU_BF16, WL_FP8>(h, *maps, a, grid, st)
-                  : launch_kernel<EPI_PLAIN_BF16, WL_FP8>(h, *maps, a, grid, st);
-  if (p.b_i8)
-    return swiglu ? launch_kernel<EPI_SWIGLU_BF16, WL_INT8>(h, *maps, a, grid, st)
-                  : launch_kernel<EPI_PLAIN_BF16, WL_INT8>(h, *maps, a, grid, st);
-  return swiglu ? launch_kernel<EPI_SWIGLU_BF16, WL_BF16>(h, *maps, a, grid, st)
-                : launch_kernel<EPI_PLAIN_BF16, WL_BF16>(h, *maps, a, grid, st);
+    return swiglu ? launch_kernel<EPI_SWIGLU_BF16, true>(h, *maps, a, grid, st)
+                  : launch_kernel<EPI_PLAIN_BF16, true>(h, *maps, a, grid, st);
+  return swiglu ? launch_kernel<EPI_SWIGLU_BF16, false>(h, *maps, a, grid, st)
+                : launch_kernel<EPI_PLAIN_BF16, false>(h, *maps, a, grid, st);
 }
 
 }  // namespace mg

@@ -1,5 +1,5 @@
 // 8-bit integer activations: quantisation of rows, and the dense product as the library's callers reach it.  The product
-// itself is the weight-lane GEMM (gemm_wl.cu), the arithmetic of a row in tc.cuh.
+// itself is in gemm_i8.cu, the arithmetic of a row in tc.cuh.
 #include "tc.cuh"
 
 namespace mg {
@@ -301,10 +301,8 @@ int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, c
 }
 
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
-                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st,
-                       bool beside) {
+                       const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st) {
   GemmProblem p{};
-  p.beside = beside;
   p.a = xq; p.a_rows = rows; p.dense_rows = rows; p.lda = ldx; p.a_scales = x_scale;
   p.b = wq; p.ldb = ldw; p.b_i8 = true; p.scales = w_scale; p.n_groups = 1; p.n_per_group = static_cast<int>(n_out);
   p.K = static_cast<int>(cols); p.out = out; p.ldo = ldo; p.epilogue = epilogue;
