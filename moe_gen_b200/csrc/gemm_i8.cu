@@ -19,13 +19,14 @@ constexpr int I8_GROUP = 8;       // token tiles that share a weight tile throug
 
 template <int BN>
 struct I8Cfg {
-  static constexpr int STAGES = BN == 128 ? 3 : BN == 64 ? 4 : 5;        // two blocks per SM
+  static constexpr int BLOCKS = BN == 256 ? 1 : 2;                        // per SM
+  static constexpr int STAGES = BN == 128 ? 3 : BN <= 32 ? 5 : 4;
   static constexpr int STAGE = (I8_BM + BN) * I8_STEP;
-  static constexpr int WN = BN == 128 ? 2 : 1, WM = 8 / WN;               // warps over tokens and over weight rows
+  static constexpr int WN = BN == 256 ? 4 : BN == 128 ? 2 : 1, WM = 8 / WN;               // warps over tokens and over weight rows
   static constexpr int MT = I8_BM / (16 * WM), NT = BN / (8 * WN);
   static constexpr int PITCH = 2 * I8_BM + 16;                            // bytes of a token's outputs on their way out
   static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE;
-  static_assert(BN * PITCH <= STAGES * STAGE && 2 * (SMEM + 4096) <= 227 * 1024, "shared memory");
+  static_assert(BN * PITCH <= STAGES * STAGE && BLOCKS * (SMEM + 4096) <= 227 * 1024, "shared memory");
 };
 
 struct I8Args {
@@ -60,7 +61,7 @@ __device__ __forceinline__ float scaled(int sum, float w, float t) { return __fm
 __device__ __forceinline__ uint16_t bf16_bits(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
 template <bool SWIGLU, int BN>
-__global__ void __launch_bounds__(I8_THREADS, 2) gemm_i8_kernel(const I8Args g) {
+__global__ void __launch_bounds__(I8_THREADS, I8Cfg<BN>::BLOCKS) gemm_i8_kernel(const I8Args g) {
   using C = I8Cfg<BN>;
   constexpr int OUTS = SWIGLU ? I8_BM / 2 : I8_BM;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -235,7 +236,7 @@ int launch(const Handle* h, const I8Args& a, int64_t tiles, cudaStream_t st) {
     MG_CUDA(cudaFuncSetAttribute(gemm_i8_kernel<SWIGLU, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::SMEM)));
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
-  const int64_t most = 2ll * h->sm_count, jobs = tiles * a.n_tiles;
+  const int64_t most = static_cast<int64_t>(C::BLOCKS) * h->sm_count, jobs = tiles * a.n_tiles;
   gemm_i8_kernel<SWIGLU, BN><<<static_cast<unsigned>(jobs < most ? jobs : most), I8_THREADS, C::SMEM, st>>>(a);
   MG_CUDA(cudaGetLastError());
   return MG_OK;
@@ -266,7 +267,8 @@ int launch_gemm_i8(const Handle* h, const GemmProblem& p, cudaStream_t st) {
   if (mean <= 16) return launch<16>(h, a, rows, swiglu, st);
   if (mean <= 32) return launch<32>(h, a, rows, swiglu, st);
   if (mean <= 64) return launch<64>(h, a, rows, swiglu, st);
-  return launch<128>(h, a, rows, swiglu, st);
+  if (mean <= 192) return launch<128>(h, a, rows, swiglu, st);
+  return launch<256>(h, a, rows, swiglu, st);
 }
 
 }  // namespace mg
