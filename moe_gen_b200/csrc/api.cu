@@ -1086,7 +1086,7 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   // int8 experts: the tokens are quantised once, for the scatter and for the shared expert.  Ahead of the chain: the kernel
   // behind it is launched by an ordinary dependence, so that the scatter may read the quantised rows as older memory.  Up to 128
   // tokens the plan that copies the rows quantises them itself, and the shared expert has its own on its own stream (layer, us,
-  // V2-Lite 8 tokens in a graph 96 and 82).
+  // V2-Lite 8 tokens in a graph 96 and 82, measured with the kernels chained).
   const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
   uint8_t* xq = ws + L.off[WS_XQ];
   float* xs = reinterpret_cast<float*>(ws + L.off[WS_XS]);

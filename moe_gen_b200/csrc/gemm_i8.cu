@@ -5,6 +5,9 @@
 // 128-byte steps filled by asynchronous copies.  Few tokens: a warp per 16 weight rows, so that a weight is read from shared memory
 // once; 128 tokens: 32 rows x 64 tokens per warp.  For SwiGLU a warp's sixteen rows are eight gate rows and the up rows of the same
 // outputs, which then meet in one thread.
+// What bounds it: with few tokens the weights' bytes (V2-236B layer, 64 tokens, 5.7 TB/s); with many the warp-wide integer MMAs, whose
+// pipe runs 60 % of the cycles at one block of 256 tokens per SM (4096 x 4096 x 7168 367 us, 0.65 POP/s; 8192 601 us, 0.80), between
+// the filling of the ring at the start of a tile and the last round of tiles; shared memory 31 %.
 // It is deliberately of plain parts: warp-wide MMAs, copies counted by the thread that issued them and block barriers, so nothing in
 // it waits for another block, another kernel or a flag.  An earlier form on SM pairs (tensor memory, copies by the tensor engine,
 // launched by programmatic dependence) was faster for large batches and stalled without end once in some million passes.
@@ -262,13 +265,21 @@ int launch_gemm_i8(const Handle* h, const GemmProblem& p, cudaStream_t st) {
   I8Args a{static_cast<const uint8_t*>(p.a), p.lda, p.a_scales, rows, static_cast<const uint8_t*>(p.b), p.ldb, p.scales,
            static_cast<uint16_t*>(p.out), p.ldo, p.pad_offsets, p.counts, p.n_groups, p.n_per_group,
            (p.n_per_group + I8_BM - 1) / I8_BM, p.K, reinterpret_cast<uintptr_t>(p.out) % 16 == 0};
-  // tokens of a tile: what a group has on average, whose rows are padded to whole tiles of 128 and one more
+  // Tokens of a tile: what a group has on average, whose rows are padded to whole tiles of 128 and one more; of a dense matrix less
+  // while fewer than three quarters of the SMs would have a block.  us, 4096 x 4096, by the mean alone and so: 64 tokens 23.1 and
+  // 13.9, 256 52.7 and 24.0, 512 52.8 and 35.8; 256 tokens of 1024 x 8192 98 and 24.5; 1024 tokens in 128 blocks of 256 53.8, in 256
+  // of 128 60.6.  256 against 128 tokens at most: 8192 x 4096 x 7168 with its rows 631 and 716, Mixtral layer 8192 tokens 8.6 and 9.0 ms.
+  // Tiles of 32 tokens from a mean of 5 on, layer: V2-Lite 64 tokens 138 and 143, V2-236B 201 625 and 631, Mixtral 61 273 and 278.
   const int64_t mean = dense ? rows : (rows - 128ll * p.n_groups) / p.n_groups;
-  if (mean <= 16) return launch<16>(h, a, rows, swiglu, st);
-  if (mean <= 32) return launch<32>(h, a, rows, swiglu, st);
-  if (mean <= 64) return launch<64>(h, a, rows, swiglu, st);
-  if (mean <= 192) return launch<128>(h, a, rows, swiglu, st);
-  return launch<256>(h, a, rows, swiglu, st);
+  int bn = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : mean <= 192 ? 128 : 256;
+  while (dense && bn > 16 && (rows + bn - 1) / bn * a.n_tiles * 4 < 3ll * h->sm_count) bn /= 2;
+  switch (bn) {
+    case 16: return launch<16>(h, a, rows, swiglu, st);
+    case 32: return launch<32>(h, a, rows, swiglu, st);
+    case 64: return launch<64>(h, a, rows, swiglu, st);
+    case 128: return launch<128>(h, a, rows, swiglu, st);
+    default: return launch<256>(h, a, rows, swiglu, st);
+  }
 }
 
 }  // namespace mg

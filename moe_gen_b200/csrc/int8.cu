@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(256) quantize_short_rows_kernel(const uint4* x
 }
 
 // A product of up to kFewRows rows of x in one launch: every block quantises them into shared memory, and a warp multiplies two
-// weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a pair
-// of SMs for 256 weight rows); here every SM streams a share of the weights.
+// weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a
+// block for 128 weight rows); here every SM streams a share of the weights.
 constexpr int kFewRows = 16, kFewWarps = 16, kFewSmem = 96 * 1024;
 template <int M>
 __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int rows, int cols,
@@ -261,11 +261,12 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
   return MG_OK;
 }
 
-// us with x and weights in L2, one launch, and two (quantised, then on the tensor cores): 1 row 4096x4096 4.4 and 12, 8192x8192 8.6
-// and 18; 4 rows 8192x8192 14.0 and 18; 8 rows 1024x1024 4.6 and 8.5, 4096x4096 8.5 and 12.5, 8192x2048 10.3 and 10.2, 8192x8192
-// 25.5 and 18.4 (every weight meets eight rows from shared memory, which bounds it); 16 rows 512x512 5.7 and 8.1, 1024x2048
-// (outputs x inputs) 8.7 and 10.1, 4096x2048 8.9 and 10.2, 8192x1024 12.2 and 9.0, 2048x4096 12.9 and 12.9 (a warp quantises a row
-// by itself there, which takes as long as the row).  So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.
+// us with x and weights in L2, in a graph, one launch, and two (quantised, then on the tensor cores): 1 row 4096x4096 4.4 and 15.0,
+// 8192x8192 8.9 and 25.9; 4 rows 8192x8192 14.1 and 25.5; 8 rows 1024x1024 4.7 and 7.0, 4096x4096 8.6 and 14.6, 8192x2048 10.4 and
+// 9.6; 16 rows 512x512 5.7 and 5.7, 1024x2048 (outputs x inputs) 8.8 and 9.5, 4096x2048 9.0 and 9.6, 8192x1024 12.3 and 7.0 (a warp
+// quantises a row by itself, and every weight meets all rows from shared memory).  A launch takes 3 to 4 us of the call's host side,
+// which bounds these.  Beyond the line, 8 rows 8192x8192 25 in two launches as in one.
+// So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.
 bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols) {
   int m = 1;
   while (m < rows && m < kFewRows) m *= 2;
