@@ -772,7 +772,7 @@ static int shared_ffn(Handle* h, const void* x, int64_t T, const void* packed, v
 // are quantised for them alone.
 static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, const int32_t* pad, const int32_t* counts,
                            int64_t rows_padded, const int32_t* dst_row, int64_t T, const void* packed, void* h_buf, void* h_q,
-                           float* h_s, void* out_rows, cudaStream_t st, int* launches, bool timed, int32_t* job_counters) {
+                           float* h_s, void* out_rows, cudaStream_t st, int* launches, bool timed) {
   const mg_layer_desc& d = h->d;
   const PackedLayout L = packed_layout(h);
   const uint8_t* base = static_cast<const uint8_t*>(packed);
@@ -781,7 +781,7 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   if (timed) mark(h, MG_STAGE_DEQUANT, st);
   p.a = perm_q; p.lda = d.hidden; p.a_scales = perm_s; p.b = base + L.w13; p.ldb = d.hidden;
   p.scales = reinterpret_cast<const float*>(base + L.s13); p.n_per_group = 2 * d.inter; p.K = d.hidden;
-  p.out = h_buf; p.ldo = d.inter; p.epilogue = EPI_SWIGLU_BF16; p.next_job = job_counters;
+  p.out = h_buf; p.ldo = d.inter; p.epilogue = EPI_SWIGLU_BF16;
   int rc = launch_grouped_gemm(h, p, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
@@ -790,7 +790,6 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   p.a = h_q; p.lda = d.inter; p.a_scales = h_s; p.b = base + L.w2; p.ldb = d.inter;
   p.scales = reinterpret_cast<const float*>(base + L.s2); p.n_per_group = d.hidden; p.K = d.inter;
   p.out = out_rows; p.ldo = d.hidden; p.epilogue = EPI_PLAIN_BF16;
-  p.next_job = job_counters != nullptr ? job_counters + 1 : nullptr;
   rc = launch_grouped_gemm(h, p, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM2, st);
@@ -919,10 +918,8 @@ int mg_expert_ffn_int8(mg_handle hh, const void* d_perm_q, const float* d_perm_s
   MG_REQUIRE(aligned16(d_perm_q) && aligned16(d_h_buf) && aligned16(d_h_q) && aligned16(d_out_rows) && aligned16(d_packed), MG_ERR_SHAPE,
              "mg_expert_ffn_int8: rows and weights must begin on a 16-byte boundary");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  int rc = zero_job_counters(h, st);
-  if (rc != MG_OK) return rc;
   return expert_ffn_int8(h, d_perm_q, d_perm_scale, d_pad, d_counts, n_rows_padded, d_dst, T, d_packed, d_h_buf, d_h_q, d_h_scale,
-                         d_out_rows, st, nullptr, false, h->job_counters);
+                         d_out_rows, st, nullptr, false);
 }
 
 int mg_shared_ffn_int8(mg_handle hh, const void* d_xq, const float* d_x_scale, int64_t T, const void* d_packed, void* d_hs,
@@ -1164,7 +1161,7 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   mark(h, MG_STAGE_PERMUTE_ROWS, st);
   launches += 1;
   rc = i8 ? expert_ffn_int8(h, perm, perm_s, pad, counts, padded_rows(h, T * d.top_k), dst, T, d_packed, hbuf, ws + L.off[WS_HQ],
-                            reinterpret_cast<float*>(ws + L.off[WS_H_S]), orow, st, &launches, true, jobs)
+                            reinterpret_cast<float*>(ws + L.off[WS_H_S]), orow, st, &launches, true)
           : expert_ffn(h, perm, pad, counts, padded_rows(h, T * d.top_k), d_packed, hbuf, orow, deq, st, &launches, true,
                        nullptr, jobs, !(shared_early && T <= kUnchainedDownTokens));
   if (rc != MG_OK) return rc;
