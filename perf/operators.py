@@ -226,9 +226,8 @@ def prepare(case, seed):
 def _quantise(x, dt):
     """int8 values of x's rows (in type dt) and the fp32 scales."""
     m = x.float().abs().amax(dim=1, keepdim=True).clamp_min(2.0 ** -100)
-    top = torch.full_like(m, 127.0)                # quotients of tensors: a number's would be a product with its reciprocal
-    inv = top / m
-    return torch.round(x.double() * inv.double()).to(dt), m / top        # the product has 32 bits: exact in 64
+    inv = 127.0 / m
+    return torch.round(x.double() * inv.double()).to(dt), m / 127.0      # the product has 32 bits: exact in 64
 
 
 def _linear(x, q, s):
@@ -344,8 +343,7 @@ def work(case):
 def _x_quant(x):
     x = x.double()
     m = torch.clamp(x.abs().max(dim=1)[0], min=2.0 ** -100).float()
-    c = torch.full_like(m, 127.0)
-    inv, scale = (c / m).double(), (m / c).double()
+    inv, scale = (127.0 / m).double(), (m / 127.0).double()
     return torch.round(x * inv[:, None]), scale[:, None]
 
 
