@@ -1007,6 +1007,8 @@ int mg_combine(mg_handle hh, const void* d_out_rows, const int32_t* d_dst, const
   if (!h) return MG_ERR_STATE;
   MG_REQUIRE(d_out_rows && d_dst && d_idx && d_w && d_y, MG_ERR_NULL, "mg_combine: null pointer");
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  MG_REQUIRE(aligned16(d_out_rows) && aligned16(d_shared) && aligned16(d_y), MG_ERR_SHAPE,
+             "mg_combine: rows must begin on a 16-byte boundary");
   return launch_combine(h, d_out_rows, d_dst, d_idx, d_w, d_shared, nullptr, T, d_y, static_cast<cudaStream_t>(stream));
 }
 

@@ -577,7 +577,15 @@ class MoELayer:
 
     def combine(self, out_rows: torch.Tensor, dst_row: torch.Tensor, topk_idx: torch.Tensor,
                 topk_w: torch.Tensor, shared_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """y[t] = sum_j topk_w[t, j] * out_rows[dst_row[t, j]] (+ shared_out[t]) in the layer's combine mode: rows in bf16, the plan and
+        the picks in int32, weights in fp32."""
         T = topk_idx.shape[0]
+        self._check_rows(out_rows, torch.bfloat16, None, self.H, "out_rows")
+        self._check_rows(dst_row, torch.int32, T, self.k, "dst_row")
+        self._check_rows(topk_idx, torch.int32, T, self.k, "topk_idx")
+        self._check_rows(topk_w, torch.float32, T, self.k, "topk_w")
+        if shared_out is not None:
+            self._check_rows(shared_out, torch.bfloat16, T, self.H, "shared_out")
         y = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
             L.check(self.lib.mg_combine(self._h, out_rows.data_ptr(), dst_row.data_ptr(), topk_idx.data_ptr(),
