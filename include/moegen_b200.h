@@ -373,6 +373,10 @@ int mg_shared_ffn_int8(mg_handle h, const void* d_xq, const float* d_x_scale, in
  * mg_permute_plan over n_plan_experts experts, with the experts a token names distinct, as every routing here gives them; entries
  * of dst_row that are negative, or not below n_rows_padded where that is given, are left out.
  *
+ * The _bounded calls take the number of rows of the buffer that dst_row points into, and leave out the entries that are not below
+ * it as they do the negative ones; the calls of the same names without it rely on a plan whose rows all lie inside.
+ *
+ * mg_permute_rows_bounded: mg_permute_rows; with d_x_scale and d_perm_scale (else both NULL) mg_permute_rows_int8.
  * mg_permute_rows_padded: mg_permute_rows with zeros in the rows of perm_x [n_rows_padded, H] that hold no pick: behind an
  *   expert's rows and behind the last segment.
  * mg_permute_rows_grad: grad_x[t] = sum_j grad_rows[dst_row[t, j]], summed in fp32 in the order of the slots, rounded once.
@@ -392,6 +396,12 @@ int mg_permute_rows_grad(mg_handle h, const void* d_grad_rows, const int32_t* d_
 int mg_combine_grad(mg_handle h, const void* d_grad_y, const void* d_out_rows, const int32_t* d_dst_row, const float* d_topk_w,
                     int64_t n_tokens, const int32_t* d_counts, const int32_t* d_pad_offsets, int32_t n_plan_experts,
                     int64_t n_rows_padded, void* d_grad_rows, float* d_grad_w, void* stream);
+int mg_permute_rows_bounded(mg_handle h, const void* d_x, const float* d_x_scale, const int32_t* d_dst_row, int64_t n_tokens,
+                            int64_t n_rows, void* d_perm_x, float* d_perm_scale, void* stream);
+int mg_permute_rows_grad_bounded(mg_handle h, const void* d_grad_rows, int64_t n_rows, const int32_t* d_dst_row, int64_t n_tokens,
+                                 void* d_grad_x, void* stream);
+int mg_combine_bounded(mg_handle h, const void* d_out_rows, int64_t n_rows, const int32_t* d_dst_row, const int32_t* d_topk_idx,
+                       const float* d_topk_w, const void* d_shared_out, int64_t n_tokens, void* d_y, void* stream);
 int mg_route_topk_grad(mg_handle h, const float* d_logits, const int32_t* d_topk_idx, const float* d_topk_w, const float* d_grad_w,
                        int64_t n_tokens, float* d_grad_logits, void* stream);
 

@@ -903,6 +903,20 @@ int mg_permute_rows_int8(mg_handle hh, const void* d_q, const float* d_scale, co
   return launch_permute_rows(h, d_q, d_dst, T, d_perm_q, static_cast<cudaStream_t>(stream), d_scale, d_perm_scale);
 }
 
+int mg_permute_rows_bounded(mg_handle hh, const void* d_x, const float* d_scale, const int32_t* d_dst, int64_t T, int64_t n_rows,
+                            void* d_perm, float* d_perm_scale, void* stream) {
+  MG_TRACE("mg_permute_rows_bounded", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0 && n_rows >= 0, MG_ERR_SHAPE, "mg_permute_rows_bounded: %lld tokens, %lld rows", static_cast<long long>(T),
+             static_cast<long long>(n_rows));
+  if (T == 0 || n_rows == 0) return MG_OK;
+  MG_REQUIRE(d_x && d_dst && d_perm && (d_scale == nullptr) == (d_perm_scale == nullptr), MG_ERR_NULL,
+             "mg_permute_rows_bounded: null pointer, or scales on one side only");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_perm), MG_ERR_SHAPE, "mg_permute_rows_bounded: rows must begin on a 16-byte boundary");
+  return launch_permute_rows(h, d_x, d_dst, T, d_perm, static_cast<cudaStream_t>(stream), d_scale, d_perm_scale, n_rows);
+}
+
 int mg_expert_ffn_int8(mg_handle hh, const void* d_perm_q, const float* d_perm_scale, const int32_t* d_pad, const int32_t* d_counts,
                        int64_t n_rows_padded, const int32_t* d_dst, int64_t T, const void* d_packed, void* d_h_buf, void* d_h_q,
                        float* d_h_scale, void* d_out_rows, void* stream) {
@@ -962,6 +976,20 @@ int mg_permute_rows_grad(mg_handle hh, const void* d_grad_rows, const int32_t* d
   return launch_permute_rows_grad(h, d_grad_rows, d_dst, T, d_grad_x, static_cast<cudaStream_t>(stream));
 }
 
+int mg_permute_rows_grad_bounded(mg_handle hh, const void* d_grad_rows, int64_t n_rows, const int32_t* d_dst, int64_t T, void* d_grad_x,
+                                 void* stream) {
+  MG_TRACE("mg_permute_rows_grad_bounded", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0 && n_rows >= 0, MG_ERR_SHAPE, "mg_permute_rows_grad_bounded: %lld tokens, %lld rows", static_cast<long long>(T),
+             static_cast<long long>(n_rows));
+  if (T == 0) return MG_OK;
+  MG_REQUIRE((d_grad_rows || n_rows == 0) && d_dst && d_grad_x, MG_ERR_NULL, "mg_permute_rows_grad_bounded: null pointer");
+  MG_REQUIRE(aligned16(d_grad_rows) && aligned16(d_grad_x), MG_ERR_SHAPE,
+             "mg_permute_rows_grad_bounded: rows must begin on a 16-byte boundary");
+  return launch_permute_rows_grad(h, d_grad_rows, d_dst, T, d_grad_x, static_cast<cudaStream_t>(stream), n_rows);
+}
+
 int mg_combine_grad(mg_handle hh, const void* d_grad_y, const void* d_out_rows, const int32_t* d_dst, const float* d_w, int64_t T,
                     const int32_t* d_counts, const int32_t* d_pad, int32_t n_plan, int64_t n_rows, void* d_grad_rows, float* d_grad_w,
                     void* stream) {
@@ -971,7 +999,7 @@ int mg_combine_grad(mg_handle hh, const void* d_grad_y, const void* d_out_rows, 
   MG_REQUIRE(T >= 0 && n_rows >= 0 && (d_counts == nullptr || (n_plan >= 1 && n_plan <= h->d.n_experts)), MG_ERR_SHAPE,
              "mg_combine_grad: %lld tokens, %lld rows, %d experts", static_cast<long long>(T), static_cast<long long>(n_rows), n_plan);
   MG_REQUIRE((d_counts == nullptr) == (d_pad == nullptr), MG_ERR_NULL, "mg_combine_grad: counts and pad_offsets come together");
-  MG_REQUIRE(T == 0 || (d_grad_y && d_dst && d_w && (d_out_rows || d_grad_w == nullptr)), MG_ERR_NULL, "mg_combine_grad: null pointer");
+  MG_REQUIRE(T == 0 || (d_grad_y && d_dst && d_w && (d_out_rows || d_grad_w == nullptr || n_rows == 0)), MG_ERR_NULL, "mg_combine_grad: null pointer");
   MG_REQUIRE(aligned16(d_grad_y) && aligned16(d_out_rows) && aligned16(d_grad_rows), MG_ERR_SHAPE,
              "mg_combine_grad: rows must begin on a 16-byte boundary");
   return launch_combine_grad(h, d_grad_y, d_out_rows, d_dst, d_w, T, d_counts, d_pad, n_plan, n_rows, d_grad_rows, d_grad_w,
@@ -1010,6 +1038,20 @@ int mg_combine(mg_handle hh, const void* d_out_rows, const int32_t* d_dst, const
   MG_REQUIRE(aligned16(d_out_rows) && aligned16(d_shared) && aligned16(d_y), MG_ERR_SHAPE,
              "mg_combine: rows must begin on a 16-byte boundary");
   return launch_combine(h, d_out_rows, d_dst, d_idx, d_w, d_shared, nullptr, T, d_y, static_cast<cudaStream_t>(stream));
+}
+
+int mg_combine_bounded(mg_handle hh, const void* d_out_rows, int64_t n_rows, const int32_t* d_dst, const int32_t* d_idx, const float* d_w,
+                       const void* d_shared, int64_t T, void* d_y, void* stream) {
+  MG_TRACE("mg_combine_bounded", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0 && n_rows >= 0, MG_ERR_SHAPE, "mg_combine_bounded: %lld tokens, %lld rows", static_cast<long long>(T),
+             static_cast<long long>(n_rows));
+  if (T == 0) return MG_OK;
+  MG_REQUIRE((d_out_rows || n_rows == 0) && d_dst && d_idx && d_w && d_y, MG_ERR_NULL, "mg_combine_bounded: null pointer");
+  MG_REQUIRE(aligned16(d_out_rows) && aligned16(d_shared) && aligned16(d_y), MG_ERR_SHAPE,
+             "mg_combine_bounded: rows must begin on a 16-byte boundary");
+  return launch_combine(h, d_out_rows, d_dst, d_idx, d_w, d_shared, nullptr, T, d_y, static_cast<cudaStream_t>(stream), n_rows);
 }
 
 int mg_workspace_ptr(mg_handle hh, void* d_ws, int64_t max_tokens, int64_t max_rows, int32_t which, void** ptr) {

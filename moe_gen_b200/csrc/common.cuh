@@ -191,12 +191,14 @@ int launch_plan_and_rows(const Handle* h, const int32_t* idx, int64_t T, int32_t
 int launch_permute_plan_static(const Handle* h, const int32_t* idx, int64_t T, int expert_lo, int n_exp,
                                int32_t* counts, int32_t* offsets, int32_t* pad_offsets, int32_t* dst_row,
                                cudaStream_t st);
-// x_scale != nullptr: int8 rows and their scales, else bf16 rows
-int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, int64_t T,
-                        void* perm_x, cudaStream_t st, const float* x_scale = nullptr, float* perm_scale = nullptr);
+constexpr int64_t kAnyRows = INT64_MAX;   // rows of a buffer that its caller does not name: every entry of dst_row lies below
+// x_scale != nullptr: int8 rows and their scales, else bf16 rows; entries of dst_row not below n_rows are left out
+int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, int64_t T, void* perm_x, cudaStream_t st,
+                        const float* x_scale = nullptr, float* perm_scale = nullptr, int64_t n_rows = kAnyRows);
 int launch_permute_rows_padded(const Handle* h, const void* x, const int32_t* dst_row, int64_t T, const int32_t* counts,
                                const int32_t* pad, int n, int64_t n_rows, void* rows, cudaStream_t st);
-int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st);
+int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st,
+                             int64_t n_rows = kAnyRows);
 int launch_combine_grad(const Handle* h, const void* gy, const void* out_rows, const int32_t* dst_row, const float* w, int64_t T,
                         const int32_t* counts, const int32_t* pad, int n, int64_t n_rows, void* grad_rows, float* grad_w,
                         cudaStream_t st);
@@ -204,7 +206,7 @@ int launch_route_topk_grad(const Handle* h, const float* logits, const int32_t* 
                            float* grad_logits, cudaStream_t st);
 int launch_combine(const Handle* h, const void* out_rows, const int32_t* dst_row,
                    const int32_t* idx, const float* w, const void* shared, const void* residual, int64_t T,
-                   void* y, cudaStream_t st);
+                   void* y, cudaStream_t st, int64_t n_rows = kAnyRows);
 int launch_rmsnorm(const Handle* h, const void* x, const void* weight, float eps, int64_t T, void* out,
                    cudaStream_t st);
 

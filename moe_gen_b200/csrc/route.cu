@@ -1241,7 +1241,7 @@ template <bool PEER, bool DEDUP, bool BACK>
 __global__ void __launch_bounds__(256) permute_rows_kernel(const uint4* __restrict__ x, const int32_t* dst_row,
                                                            int64_t T, int k, int vec_per_row, int slices, int v_chunk,
                                                            PeerPtrs bufs, PeerPtrs dups, PeerPtrs backs, int my_rank,
-                                                           const float* scale, float* row_scale, Guard guard) {
+                                                           const float* scale, float* row_scale, int64_t n_rows, Guard guard) {
   chain_wait();
   chain_go();
   const int lane = threadIdx.x & 31;
@@ -1254,6 +1254,7 @@ __global__ void __launch_bounds__(256) permute_rows_kernel(const uint4* __restri
   if (my_dst >= 0 && !MG_GUARD((PEER ? (my_dst & kPeerRowMask) : my_dst) < guard.rows_bound &&
                                (!PEER || (my_dst >> kPeerShift) < guard.n_peers), guard, 103))
     my_dst = -1;
+  if (!PEER && my_dst >= n_rows) my_dst = -1;
   if (!PEER && scale != nullptr && v_begin == 0 && my_dst >= 0) row_scale[my_dst] = scale[t];      // int8 rows
   if (BACK && my_dst >= 0)
     static_cast<int32_t*>(backs.p[my_dst >> kPeerShift])[my_dst & kPeerRowMask] =
@@ -1308,7 +1309,7 @@ __global__ void __launch_bounds__(256) fill_duplicate_rows_kernel(uint4* __restr
 }
 
 int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, int64_t T,
-                        void* perm_x, cudaStream_t st, const float* x_scale, float* perm_scale) {
+                        void* perm_x, cudaStream_t st, const float* x_scale, float* perm_scale, int64_t n_rows) {
   if (T == 0) return MG_OK;
   const int warps = 8, vpr = h->d.hidden / (x_scale != nullptr ? 16 : 8);
   const RowSlices rs = row_slices(h, T, vpr);
@@ -1316,7 +1317,7 @@ int launch_permute_rows(const Handle* h, const void* x, const int32_t* dst_row, 
   PeerPtrs bufs{};
   bufs.p[0] = perm_x;
   MG_CUDA(launch_chained(h, permute_rows_kernel<false, false, false>, grid, block, 0, st, static_cast<const uint4*>(x), dst_row,
-                         T, h->d.top_k, vpr, rs.n, rs.v_chunk, bufs, bufs, bufs, 0, x_scale, perm_scale,
+                         T, h->d.top_k, vpr, rs.n, rs.v_chunk, bufs, bufs, bufs, 0, x_scale, perm_scale, n_rows,
                          Guard{h->d_status, h->guard_rows, 1}));
   return MG_OK;
 }
@@ -1509,13 +1510,13 @@ int launch_dispatch_rows(const Handle* h, const void* x, const int32_t* dst, int
   const PeerPtrs& b = backs ? *backs : peers;
   const Guard guard{h->d_status, h->guard_rows, h->d.ep_size};
   if (dups != nullptr && backs != nullptr)
-    permute_rows_kernel<true, true, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
+    permute_rows_kernel<true, true, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, kAnyRows, guard);
   else if (dups != nullptr)
-    permute_rows_kernel<true, true, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
+    permute_rows_kernel<true, true, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, kAnyRows, guard);
   else if (backs != nullptr)
-    permute_rows_kernel<true, false, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
+    permute_rows_kernel<true, false, true><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, kAnyRows, guard);
   else
-    permute_rows_kernel<true, false, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, guard);
+    permute_rows_kernel<true, false, false><<<grid, block, 0, st>>>(xs, dst, T, k, vpr, 1, vpr, peers, d, b, me, nullptr, nullptr, kAnyRows, guard);
   MG_CUDA(cudaGetLastError());
   return MG_OK;
 }
@@ -1588,7 +1589,8 @@ template <int MODE, bool PEER>
 __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32_t* dst_row, const int32_t* topk_idx,
                                                       const float* topk_w, const uint4* shared, const uint4* residual,
                                                       int64_t T, int k, int vec_per_row, int v_chunk,
-                                                      uint4* y, int by_slot, const int32_t* delta, bool wide, Guard guard) {
+                                                      uint4* y, int by_slot, const int32_t* delta, bool wide, int64_t n_rows,
+                                                      Guard guard) {
   chain_wait();
   chain_go();
   const int lane = threadIdx.x & 31;
@@ -1601,6 +1603,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PeerPtrs bufs, const int32
     if (my_dst >= 0 && !MG_GUARD((PEER ? (my_dst & kPeerRowMask) : my_dst) < guard.rows_bound &&
                                  (!PEER || (my_dst >> kPeerShift) < guard.n_peers), guard, 104))
       my_dst = -1;
+    if (!PEER && my_dst >= n_rows) my_dst = -1;
     if (by_slot > 0 && my_dst >= 0 && (my_dst >> kPeerShift) != by_slot - 1)
       my_dst = (my_dst & ~kPeerRowMask) | static_cast<int32_t>(t * k + lane);
     // mirror of the owners' rows in this rank's own expert-sorted order (bufs.p[0]): row in the owner's
@@ -1701,7 +1704,7 @@ template <bool PEER>
 static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int32_t* dst_row,
                                const int32_t* idx, const float* w, const void* shared, const void* residual,
                                int64_t T, void* y, cudaStream_t st, int by_slot = 0,
-                               const int32_t* delta = nullptr, bool sum = false) {
+                               const int32_t* delta = nullptr, bool sum = false, int64_t n_rows = kAnyRows) {
   if (T == 0) return MG_OK;
   const int warps = 8;
   const int k = h->d.top_k, vpr = h->d.hidden / 8;
@@ -1717,7 +1720,7 @@ static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int3
 #define MG_COMBINE_CASE(M)                                                                       \
   MG_CUDA(launch_chained(h, combine_kernel<M, PEER>, grid, block, 0, st, bufs, dst_row, idx, w,   \
                          static_cast<const uint4*>(shared), static_cast<const uint4*>(residual), T, k, vpr, v_chunk, \
-                         static_cast<uint4*>(y), by_slot, delta, h->d.weight_format == MG_WEIGHT_INT8_CHANNEL, \
+                         static_cast<uint4*>(y), by_slot, delta, h->d.weight_format == MG_WEIGHT_INT8_CHANNEL, n_rows, \
                          Guard{h->d_status, h->guard_rows, PEER ? h->d.ep_size : 1}))
   if (!PEER && sum) {
     MG_COMBINE_CASE(kSumRows);
@@ -1734,18 +1737,19 @@ static int launch_combine_impl(const Handle* h, const PeerPtrs& bufs, const int3
   return MG_OK;
 }
 
-int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st) {
+int launch_permute_rows_grad(const Handle* h, const void* grad_rows, const int32_t* dst_row, int64_t T, void* grad_x, cudaStream_t st,
+                             int64_t n_rows) {
   PeerPtrs bufs{};
   bufs.p[0] = const_cast<void*>(grad_rows);
-  return launch_combine_impl<false>(h, bufs, dst_row, nullptr, nullptr, nullptr, nullptr, T, grad_x, st, 0, nullptr, true);
+  return launch_combine_impl<false>(h, bufs, dst_row, nullptr, nullptr, nullptr, nullptr, T, grad_x, st, 0, nullptr, true, n_rows);
 }
 
 int launch_combine(const Handle* h, const void* out_rows, const int32_t* dst_row,
                    const int32_t* idx, const float* w, const void* shared, const void* residual, int64_t T,
-                   void* y, cudaStream_t st) {
+                   void* y, cudaStream_t st, int64_t n_rows) {
   PeerPtrs bufs{};
   bufs.p[0] = const_cast<void*>(out_rows);
-  return launch_combine_impl<false>(h, bufs, dst_row, idx, w, shared, residual, T, y, st);
+  return launch_combine_impl<false>(h, bufs, dst_row, idx, w, shared, residual, T, y, st, 0, nullptr, false, n_rows);
 }
 
 int launch_combine_slots(const Handle* h, const void* ret_rows, const void* own_out_rows, const int32_t* dst,

@@ -366,23 +366,24 @@ class MoELayer:
                                                         counts.data_ptr(), pad_offsets.data_ptr(), counts.numel(), rows_padded,
                                                         perm.data_ptr(), self._stream()))
             return perm
-        self._check_in(x, torch.bfloat16, "hidden_states")
+        self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
+        self._check_rows(dst_row, torch.int32, x.shape[0], self.k, "dst_row")
         perm = torch.zeros(rows_padded, self.H, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
-            L.check(self.lib.mg_permute_rows(self._h, x.data_ptr(), dst_row.data_ptr(), x.shape[0],
-                                             perm.data_ptr(), self._stream()))
+            L.check(self.lib.mg_permute_rows_bounded(self._h, x.data_ptr(), None, dst_row.data_ptr(), x.shape[0], rows_padded,
+                                                     perm.data_ptr(), None, self._stream()))
         return perm
 
     def permute_rows_grad(self, grad_rows: torch.Tensor, dst_row: torch.Tensor) -> torch.Tensor:
-        """Gradient of permute_rows: grad_x[t] = sum_j grad_rows[dst_row[t, j]] (fp32 sum, one rounding).  dst_row is a plan's:
-        its entries lie below grad_rows' rows."""
+        """Gradient of permute_rows: grad_x[t] = sum_j grad_rows[dst_row[t, j]] (fp32 sum, one rounding).  Entries of dst_row that
+        are negative or not below grad_rows' rows are left out."""
         self._check_rows(grad_rows, torch.bfloat16, None, self.H, "grad_rows")
         self._check_rows(dst_row, torch.int32, None, self.k, "dst_row")
         T = dst_row.shape[0]
         gx = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
-            L.check(self.lib.mg_permute_rows_grad(self._h, grad_rows.data_ptr(), dst_row.data_ptr(), T, gx.data_ptr(),
-                                                  self._stream()))
+            L.check(self.lib.mg_permute_rows_grad_bounded(self._h, grad_rows.data_ptr(), grad_rows.shape[0], dst_row.data_ptr(), T,
+                                                          gx.data_ptr(), self._stream()))
         return gx
 
     def combine_grad(self, grad_y: torch.Tensor, out_rows: torch.Tensor, dst_row: torch.Tensor, topk_w: torch.Tensor,
@@ -494,8 +495,8 @@ class MoELayer:
         q = torch.empty(rows_padded, self.H, dtype=torch.int8, device=self.device)
         s = torch.empty(rows_padded, dtype=torch.float32, device=self.device)
         with self._on_device():
-            L.check(self.lib.mg_permute_rows_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), dst_row.data_ptr(), xq.shape[0],
-                                                  q.data_ptr(), s.data_ptr(), self._stream()))
+            L.check(self.lib.mg_permute_rows_bounded(self._h, xq.data_ptr(), x_scale.data_ptr(), dst_row.data_ptr(), xq.shape[0],
+                                                     rows_padded, q.data_ptr(), s.data_ptr(), self._stream()))
         return q, s
 
     def expert_ffn_int8(self, perm_q: torch.Tensor, perm_scale: torch.Tensor, pad_offsets: torch.Tensor, counts: torch.Tensor,
@@ -578,7 +579,7 @@ class MoELayer:
     def combine(self, out_rows: torch.Tensor, dst_row: torch.Tensor, topk_idx: torch.Tensor,
                 topk_w: torch.Tensor, shared_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """y[t] = sum_j topk_w[t, j] * out_rows[dst_row[t, j]] (+ shared_out[t]) in the layer's combine mode: rows in bf16, the plan and
-        the picks in int32, weights in fp32."""
+        the picks in int32, weights in fp32.  Entries of dst_row that are negative or not below out_rows' rows are left out."""
         T = topk_idx.shape[0]
         self._check_rows(out_rows, torch.bfloat16, None, self.H, "out_rows")
         self._check_rows(dst_row, torch.int32, T, self.k, "dst_row")
@@ -588,8 +589,9 @@ class MoELayer:
             self._check_rows(shared_out, torch.bfloat16, T, self.H, "shared_out")
         y = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
-            L.check(self.lib.mg_combine(self._h, out_rows.data_ptr(), dst_row.data_ptr(), topk_idx.data_ptr(),
-                                        topk_w.data_ptr(), _ptr(shared_out), T, y.data_ptr(), self._stream()))
+            L.check(self.lib.mg_combine_bounded(self._h, out_rows.data_ptr(), out_rows.shape[0], dst_row.data_ptr(),
+                                                topk_idx.data_ptr(), topk_w.data_ptr(), _ptr(shared_out), T, y.data_ptr(),
+                                                self._stream()))
         return y
 
     def dequant_fp8(self, q: torch.Tensor, scale_inv: torch.Tensor) -> torch.Tensor:

@@ -78,6 +78,9 @@ SIGNATURES = {
     "mg_shared_ffn_int8": [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
     "mg_permute_rows_padded": [_vp, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _vp],
     "mg_permute_rows_grad": [_vp, _vp, _vp, _i64, _vp, _vp],
+    "mg_permute_rows_bounded": [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp],
+    "mg_permute_rows_grad_bounded": [_vp, _vp, _i64, _vp, _i64, _vp, _vp],
+    "mg_combine_bounded": [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
     "mg_combine_grad": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _vp, _vp],
     "mg_route_topk_grad": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp],
     "mg_moe_forward": [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
