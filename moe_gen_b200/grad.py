@@ -16,6 +16,13 @@ import torch
 from .layer import MoELayer
 
 
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and on a 16-byte boundary, as the kernels read rows.  torch hands a gradient over as it comes: the backward of cat
+    and of flat views cuts it out of a larger tensor at any element."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, layer):
@@ -29,7 +36,7 @@ class _Route(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, grad_w):
         logits, idx, w = ctx.saved_tensors
-        return ctx.layer.route_topk_grad(logits, idx, w, grad_w.contiguous()), None
+        return ctx.layer.route_topk_grad(_whole(logits), idx, w, grad_w.contiguous()), None
 
 
 class _SortRows(torch.autograd.Function):
@@ -42,7 +49,7 @@ class _SortRows(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_rows):
-        return ctx.layer.permute_rows_grad(grad_rows.contiguous(), ctx.saved_tensors[0]), None, None, None, None, None
+        return ctx.layer.permute_rows_grad(_whole(grad_rows), ctx.saved_tensors[0]), None, None, None, None, None
 
 
 class _CombineRows(torch.autograd.Function):
@@ -56,7 +63,7 @@ class _CombineRows(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_y):
         out_rows, topk_w, dst_row, counts, pad_offsets = ctx.saved_tensors
-        grad_y = grad_y.contiguous()
+        grad_y = _whole(grad_y)
         grows = gw = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
             grows, gw = ctx.layer.combine_grad(grad_y, out_rows, dst_row, topk_w, counts, pad_offsets,
