@@ -393,10 +393,11 @@ int mg_route_topk(mg_handle hh, const float* d_logits, const float* d_bias, int6
   MG_TRACE("mg_route_topk", T);
   Handle* h = check(hh);
   if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
   MG_REQUIRE(d_logits && d_idx && d_w, MG_ERR_NULL, "mg_route_topk: null pointer");
   MG_REQUIRE(h->d.gating != MG_GATE_SIGMOID_NOAUX_TC || d_bias != nullptr, MG_ERR_NULL,
              "noaux_tc gating needs e_score_correction_bias");
-  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   return launch_route_topk(h, d_logits, d_bias, T, d_idx, d_w, static_cast<cudaStream_t>(stream));
 }
 
@@ -413,7 +414,7 @@ int mg_permute_plan(mg_handle hh, const int32_t* d_idx, int64_t T, int32_t exper
   MG_TRACE("mg_permute_plan", T);
   Handle* h = check(hh);
   if (!h) return MG_ERR_STATE;
-  MG_REQUIRE(d_idx && d_counts && d_offsets && d_pad && d_dst && d_ws, MG_ERR_NULL, "mg_permute_plan: null pointer");
+  MG_REQUIRE(((d_idx && d_dst) || T == 0) && d_counts && d_offsets && d_pad && d_ws, MG_ERR_NULL, "mg_permute_plan: null pointer");
   MG_REQUIRE(T >= 0 && expert_lo >= 0 && n_plan >= 1 && expert_lo + n_plan <= h->d.n_experts, MG_ERR_SHAPE,
              "expert range [%d,%d) outside [0,%d)", expert_lo, expert_lo + n_plan, h->d.n_experts);
   return launch_permute_plan(h, d_idx, T, expert_lo, n_plan, d_counts, d_offsets, d_pad, d_dst, d_ws,
@@ -1033,8 +1034,9 @@ int mg_combine(mg_handle hh, const void* d_out_rows, const int32_t* d_dst, const
   MG_TRACE("mg_combine", T);
   Handle* h = check(hh);
   if (!h) return MG_ERR_STATE;
-  MG_REQUIRE(d_out_rows && d_dst && d_idx && d_w && d_y, MG_ERR_NULL, "mg_combine: null pointer");
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) return MG_OK;
+  MG_REQUIRE(d_out_rows && d_dst && d_idx && d_w && d_y, MG_ERR_NULL, "mg_combine: null pointer");
   MG_REQUIRE(aligned16(d_out_rows) && aligned16(d_shared) && aligned16(d_y), MG_ERR_SHAPE,
              "mg_combine: rows must begin on a 16-byte boundary");
   return launch_combine(h, d_out_rows, d_dst, d_idx, d_w, d_shared, nullptr, T, d_y, static_cast<cudaStream_t>(stream));
