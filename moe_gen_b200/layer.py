@@ -292,7 +292,7 @@ class MoELayer:
         return logits
 
     def route_topk(self, logits: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-        self._check_in(logits, torch.float32, "logits")
+        self._check_rows(logits, torch.float32, None, self.E, "logits")
         T = logits.shape[0]
         idx = torch.empty(T, self.k, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.k, dtype=torch.float32, device=self.device)
@@ -322,7 +322,7 @@ class MoELayer:
 
     def permute_plan(self, topk_idx: torch.Tensor, expert_lo: int = 0, n_plan: Optional[int] = None):
         """-> counts [n], offsets [n+1], pad_offsets [n+1], dst_row [T,k] (all int32)."""
-        self._check_in(topk_idx, torch.int32, "topk_idx")
+        self._check_rows(topk_idx, torch.int32, None, self.k, "topk_idx")
         n = self.E if n_plan is None else n_plan
         T = topk_idx.shape[0]
         dev = self.device
