@@ -183,7 +183,12 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
     t_start = time.perf_counter()
     nbytes = 0
 
-    gw = checkpoint.file_of(gate_n.format(p=p)).tensor(gate_n.format(p=p))
+    def not_int8(name: str, t: torch.Tensor) -> torch.Tensor:
+        if t.dtype == torch.int8:               # its integers are no weights without their scales
+            raise ValueError(f"{name}: stored as int8, the layer keeps it in bf16")
+        return t
+
+    gw = not_int8(gate_n.format(p=p), checkpoint.file_of(gate_n.format(p=p)).tensor(gate_n.format(p=p)))
     bias = None
     if bias_n is not None and bias_n.format(p=p) in checkpoint:
         bias = checkpoint.file_of(bias_n.format(p=p)).tensor(bias_n.format(p=p)).float()
@@ -281,7 +286,7 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                 scales.append(s)
                 ws.append(t)
             else:
-                ws.append(t.to(torch.bfloat16))
+                ws.append(not_int8(n, t).to(torch.bfloat16))
         layer.load_shared(*ws, tuple(scales) if int8 else None)
     dt = time.perf_counter() - t_start
     return {"bytes": int(nbytes), "seconds": dt, "gb_per_s": nbytes / dt / 1e9, "experts": layer.e_local}

@@ -1,0 +1,23 @@
+"""GPU: what an int8 checkpoint may hold its scales in, and layers of other formats that are given int8 tensors."""
+import pytest
+import torch
+
+from tests.test_gpu_int8 import _checkpoint_weights, _layer, quantise
+
+pytestmark = pytest.mark.gpu
+
+
+def test_int8_tensors_where_the_layer_keeps_bf16_are_refused(tmp_path):
+    """A shared expert or a router stored in int8 is no bf16 matrix: its bytes without their scales mean nothing."""
+    from moe_gen_b200 import ingest
+    experts, shared, router = _checkpoint_weights(700)
+    bf = [[torch.randn(q.shape).to(torch.bfloat16) for q, _ in e] for e in experts]
+    q8 = [(q.to(torch.int8), s) for q, s in map(quantise, shared)]
+    for name, kw in (("shared", dict(gate_w=router, shared=q8)), ("router", dict(gate_w=router.to(torch.int8), shared=shared))):
+        d = tmp_path / name
+        d.mkdir()
+        ingest.export_moe_layer(str(d / "model.safetensors"), 0, kw["gate_w"], None, bf, shared=kw["shared"])
+        layer = _layer(Is=128, int8=False)
+        with pytest.raises(ValueError, match="int8"):
+            ingest.load_moe_layer(layer, ingest.Checkpoint(str(d)), 0, n_threads=2)
+        layer.close()
