@@ -53,7 +53,6 @@ class MoELayer:
         self.bias: Optional[torch.Tensor] = None
         self._ws: Optional[torch.Tensor] = None
         self._ws_tokens = -1
-        self._size = C.c_size_t()
         self.options = {}                       # option id -> last value set
 
     # ------------------------------------------------------------------ lifetime
@@ -477,8 +476,9 @@ class MoELayer:
         """int8_matmul of bf16 rows x, quantised per token (quantize_rows) in the same call."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
         n_out, ldw, out, ldo = self._int8_args(wq, w_scale, cols, n, out)
-        L.check(self.lib.mg_int8_linear_ws_bytes(n, n_out, cols, C.byref(self._size)))
-        size = self._size.value
+        need = C.c_size_t()
+        L.check(self.lib.mg_int8_linear_ws_bytes(n, n_out, cols, C.byref(need)))
+        size = need.value
         ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         with self._on_device():
             L.check(self.lib.mg_int8_linear(self._h, x.data_ptr(), ldx, n, wq.data_ptr(), ldw, w_scale.data_ptr(), n_out, cols,
