@@ -172,7 +172,7 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                    prefix: str = "model.layers.{}", n_threads: int = 8) -> dict:
     """Fills `layer` (a MoELayer, any ep_rank) with block `layer_idx` of the checkpoint: router, this
     rank's experts, shared expert.  Returns byte and time counts.  Expert matrices must be stored in
-    the layer's weight format (FP8 e4m3 + `weight_scale_inv` for MG_WEIGHT_FP8_BLOCK128, int8 + fp32 `weight_scale` per
+    the layer's weight format (FP8 e4m3 + `weight_scale_inv` for MG_WEIGHT_FP8_BLOCK128, int8 + a `weight_scale` of any floating type per
     row, [n] or [n, 1], for MG_WEIGHT_INT8_CHANNEL, else bf16); an FP8-stored shared expert is de-quantised on the device,
     since the packed layout keeps it bf16, and in an int8 layer a bf16-stored one is quantised there."""
     gate_n, bias_n, exp_n, mats, shared_n = NAMING[naming]
@@ -233,6 +233,8 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                     got_dt, got_shape = f.info(n)
                     if len(shape) == 1 and tuple(got_shape) == (shape[0], 1):
                         got_shape = shape                  # a scale per row, stored as a column
+                    if int8 and dt == torch.float32 and got_dt.is_floating_point:
+                        got_dt = dt                        # in the model's own type: converted as they are copied
                     if got_dt != dt or tuple(got_shape) != tuple(shape):
                         raise ValueError(f"{n}: stored as {tuple(got_shape)} {got_dt}, the layer needs {tuple(shape)} {dt}")
                 if i >= 2:
@@ -241,6 +243,8 @@ def load_moe_layer(layer, checkpoint: Checkpoint, layer_idx: int, naming: str = 
                 futs = []
                 for j, (f, n) in enumerate(src):
                     raw = f.raw(n)
+                    if f.info(n)[0] != want[j][1]:
+                        raw = f.tensor(n).float().reshape(-1).numpy().view(np.uint8)
                     # large matrices in slices so that the pool's threads share them
                     step = max(1 << 20, -(-raw.size // max(1, n_threads)))
                     for a in range(0, raw.size, step):
