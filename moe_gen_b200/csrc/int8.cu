@@ -204,13 +204,14 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uin
   }
 }
 
-// Rows of any length, alignment and stride, element by element, read twice.
-__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* x, int64_t ldx, int cols, uint8_t* q, int64_t ldq,
-                                                                float* scale) {
+// Rows (or listed rows) of any length, alignment and stride, element by element, read twice.
+__global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* x, int64_t ldx, int cols, const int32_t* list,
+                                                                int64_t list_rows, uint8_t* q, int64_t ldq, float* scale) {
   chain_wait();
   chain_go();
   __shared__ uint32_t s_max[8];
-  const int64_t row = blockIdx.x;
+  const int64_t row = list != nullptr ? list[blockIdx.x] : static_cast<int64_t>(blockIdx.x);
+  if (row < 0 || row >= list_rows) return;
   const uint16_t* src = x + row * ldx;
   uint32_t m = 0;
   for (int c = threadIdx.x; c < cols; c += blockDim.x) m = max(m, src[c] & 0x7FFFu);
@@ -226,19 +227,18 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* 
 
 }  // namespace
 
-// ldx in elements, ldq in bytes; list: nullptr, or the n rows to quantise of list_rows (cols a multiple of 8 then)
+// ldx in elements, ldq in bytes; list: nullptr, or the n rows to quantise of list_rows
 int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
                          cudaStream_t st, const int32_t* list, int64_t list_rows) {
   if (n == 0) return MG_OK;
   MG_REQUIRE(n < (1ll << 31), MG_ERR_LIMIT, "quantise: %lld rows", static_cast<long long>(n));
-  const int64_t vecs = cols / 8;
+  const int64_t vecs = cols / 8, bound = list == nullptr ? n : list_rows;
   const bool wide = cols % 8 == 0 && ldx % 8 == 0 && ldq % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(q) % 8 == 0 && vecs <= 256 * kQuantVecs;
   if (wide) {
     // four vectors to a thread, so that short rows do not leave most of a block idle
     int threads = static_cast<int>((vecs + 127) / 128) * 32;
     if (threads > 256) threads = 256;
-    const int64_t bound = list == nullptr ? n : list_rows;
     if (vecs <= 32 * kQuantVecs && n >= kWarpRows) {
 #define MG_QUANT(V)                                                                                                          \
   MG_CUDA(launch_chained(h, quantize_short_rows_kernel<V>, static_cast<unsigned>((n + 7) / 8), 256, 0, st,                   \
@@ -255,9 +255,8 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
 #undef MG_QUANT
     return MG_OK;
   }
-  MG_REQUIRE(list == nullptr, MG_ERR_SHAPE, "quantise: listed rows of %lld elements", static_cast<long long>(cols));
   MG_CUDA(launch_chained(h, quantize_rows_any_kernel, static_cast<unsigned>(n), 256, 0, st, static_cast<const uint16_t*>(x), ldx,
-                         static_cast<int>(cols), static_cast<uint8_t*>(q), ldq, scale));
+                         static_cast<int>(cols), list, bound, static_cast<uint8_t*>(q), ldq, scale));
   return MG_OK;
 }
 
