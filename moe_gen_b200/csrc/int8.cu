@@ -276,8 +276,8 @@ template <int M>
 static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,
                       int64_t n_out, int64_t cols, void* out, int64_t ldo, cudaStream_t st) {
   const size_t smem = static_cast<size_t>(M * round_up(cols, 16));
-  static bool done[64];
-  if (smem > 48 * 1024 - 64 && !(h->device >= 0 && h->device < 64 && done[h->device])) {
+  static bool done[64];       // asked for whatever this call's rows take: what the kernel declares by itself counts against the default
+  if (!(h->device >= 0 && h->device < 64 && done[h->device])) {
     MG_CUDA(cudaFuncSetAttribute(int8_few_rows_kernel<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem));
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
