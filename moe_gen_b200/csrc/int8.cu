@@ -265,11 +265,12 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
 // 9.6; 16 rows 512x512 5.7 and 5.7, 1024x2048 (outputs x inputs) 8.8 and 9.5, 4096x2048 9.0 and 9.6, 8192x1024 12.3 and 7.0 (a warp
 // quantises a row by itself, and every weight meets all rows from shared memory).  A launch takes 3 to 4 us of the call's host side,
 // which bounds these.  Beyond the line, 8 rows 8192x8192 25 in two launches as in one.
-// So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.
+// So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.  Never beyond 2^30 outputs, which the kernel
+// counts in 32 bits, a whole grid's step past the last one included.
 bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols) {
   int m = 1;
   while (m < rows && m < kFewRows) m *= 2;
-  if (rows < 1 || rows > kFewRows || m * round_up(cols, 16) > kFewSmem) return false;
+  if (rows < 1 || rows > kFewRows || m * round_up(cols, 16) > kFewSmem || n_out > 1 << 30) return false;
   return rows <= 4 || (rows <= 8 ? n_out <= (1 << 24) / cols : cols <= 2048 && n_out <= (1 << 23) / cols);
 }
 template <int M>
