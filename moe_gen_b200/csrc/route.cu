@@ -696,10 +696,9 @@ int launch_route_topk_fixup(const Handle* h, const void* x, const void* gate_w, 
   dim3 grid(static_cast<unsigned>((T + warps - 1) / warps)), block(warps * 32);
   const int sms = h->sm_count > 0 ? h->sm_count : 148;
   const size_t smem = static_cast<size_t>(kFixTokens) * d.hidden * 2;
-  static bool done[64];
+  static bool done[64];                              // all that a block may have: a later layer's rows may be longer
   if (smem > 48 * 1024 && !(h->device >= 0 && h->device < 64 && done[h->device])) {
-    MG_CUDA(cudaFuncSetAttribute(route_fix_logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem)));
+    MG_CUDA(cudaFuncSetAttribute(route_fix_logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
   const __nv_bfloat16* xb = static_cast<const __nv_bfloat16*>(x);

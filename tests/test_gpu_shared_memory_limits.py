@@ -40,3 +40,25 @@ print("SAME")
 @pytest.mark.parametrize("experts,tokens", [(512, [288, 320, 321, 352, 353]), (384, [448, 449, 480, 481])])
 def test_plans_whose_bitmaps_fill_the_default(experts, tokens):
     _run(PLAN.replace("EXPERTS", str(experts)).replace("TOKENS", repr(tokens)))
+
+
+ROUTE = r"""
+import torch
+from tests.test_gpu_grad import DEV, _layer
+for H in (6400, 7168, 8192, 6656):             # a larger row after a smaller one
+    layer = _layer(E=64, k=6, H=H)
+    g = torch.Generator().manual_seed(H)
+    layer.set_router(torch.randn(64, H, generator=g) * 0.1)
+    x = torch.randn(40, H, generator=g).to(torch.bfloat16).to(DEV)
+    idx, w, logits, fix = layer.gate_route(x)
+    torch.cuda.synchronize()
+    exact = x.double() @ layer.gate_w.double().t()
+    assert ((logits.double() - exact).abs() <= 1e-4 * (x.double().abs() @ layer.gate_w.double().abs().t())).all()
+    assert torch.equal(idx.long().sort(dim=1)[0], exact.topk(6, dim=1)[1].sort(dim=1)[0])
+    layer.close()
+print("SAME")
+"""
+
+
+def test_routing_of_a_larger_hidden_size_after_a_smaller_one():
+    _run(ROUTE)
