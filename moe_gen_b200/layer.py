@@ -53,6 +53,7 @@ class MoELayer:
         self.bias: Optional[torch.Tensor] = None
         self._ws: Optional[torch.Tensor] = None
         self._ws_tokens = -1
+        self._captured: list = []               # buffers that captured graphs go on using
         self.options = {}                       # option id -> last value set
 
     # ------------------------------------------------------------------ lifetime
@@ -127,6 +128,14 @@ class MoELayer:
         L.check(self.lib.mg_padded_rows(self._h, n_rows, C.byref(out)))
         return out.value
 
+    def _kept(self, buf: torch.Tensor) -> torch.Tensor:
+        """buf, kept for the layer's life where the call is being captured: a graph writes to it at every replay, also after a larger
+        batch has been given another."""
+        with self._on_device():
+            if torch.cuda.is_current_stream_capturing() and all(b is not buf for b in self._captured):
+                self._captured.append(buf)
+        return buf
+
     def _workspace(self, T: int) -> torch.Tensor:
         if self._ws is None or T > self._ws_tokens:
             n = C.c_size_t()
@@ -134,7 +143,7 @@ class MoELayer:
             self._ws = None
             self._ws = torch.empty(max(n.value, 256), dtype=torch.uint8, device=self.device)
             self._ws_tokens = T
-        return self._ws
+        return self._kept(self._ws)
 
     def workspace_view(self, which: int, T: int) -> int:
         p = C.c_void_p()
@@ -235,11 +244,12 @@ class MoELayer:
         ws = self._workspace(T)
         if getattr(self, "_xnorm", None) is None or self._xnorm.shape[0] < T:
             self._xnorm = torch.empty(max(T, 1), self.H, dtype=torch.bfloat16, device=self.device)
+        xnorm = self._kept(self._xnorm)
         y = torch.empty_like(h2) if out is None else out.reshape(-1, self.H)
         with self._on_device():
             L.check(self.lib.mg_moe_block_forward(self._h, h2.data_ptr(), norm_weight.data_ptr(), float(eps), T,
                                                   self.gate_w.data_ptr(), _ptr(self.bias), self.packed.data_ptr(),
-                                                  self._xnorm.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(),
+                                                  xnorm.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(),
                                                   self._stream()))
         return y.view(shape)
 
