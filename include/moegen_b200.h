@@ -342,7 +342,7 @@ int mg_moe_forward_from_logits(mg_handle h, const void* d_x, int64_t n_tokens, c
  *   [n_rows, n_out] bf16 with rows ldo elements apart, ldo a multiple of 8; any sizes otherwise.
  * mg_int8_linear: both in one call, for bf16 rows; d_ws is scratch of mg_int8_linear_ws_bytes bytes on a 16-byte boundary (0 bytes
  *   for the few rows that one launch takes: d_ws may be NULL then).
- * The handle may be any layer's: it gives the device, its status word and its cache of tensor maps. */
+ * The handle may be any layer's: it gives the device. */
 int mg_quantize_rows_int8(mg_handle h, const void* d_x, int64_t n_rows, int64_t cols, int64_t ldx, void* d_q, int64_t ldq,
                           float* d_scale, void* stream);
 int mg_int8_matmul(mg_handle h, const void* d_xq, int64_t ldx, const float* d_x_scale, int64_t n_rows, const void* d_wq,

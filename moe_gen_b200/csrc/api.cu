@@ -786,7 +786,7 @@ static int expert_ffn_int8(Handle* h, const void* perm_q, const float* perm_s, c
   int rc = launch_grouped_gemm(h, p, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_EXPERT_GEMM1, st);
-  rc = launch_quantize_rows(h, h_buf, T * d.top_k, d.inter, d.inter, h_q, d.inter, h_s, st, dst_row, rows_padded);
+  rc = launch_quantize_rows(h_buf, T * d.top_k, d.inter, d.inter, h_q, d.inter, h_s, st, dst_row, rows_padded);
   if (rc != MG_OK) return rc;
   p.a = h_q; p.lda = d.inter; p.a_scales = h_s; p.b = base + L.w2; p.ldb = d.inter;
   p.scales = reinterpret_cast<const float*>(base + L.s2); p.n_per_group = d.hidden; p.K = d.inter;
@@ -807,7 +807,7 @@ static int shared_ffn_int8(Handle* h, const void* xq, const float* xs, int64_t T
                               2 * d.inter_shared, d.hidden, hs, d.inter_shared, EPI_SWIGLU_BF16, st);
   if (rc != MG_OK) return rc;
   if (timed) mark(h, MG_STAGE_SHARED_GEMM1, st);
-  rc = launch_quantize_rows(h, hs, T, d.inter_shared, d.inter_shared, hs_q, d.inter_shared, hs_s, st);
+  rc = launch_quantize_rows(hs, T, d.inter_shared, d.inter_shared, hs_q, d.inter_shared, hs_s, st);
   if (rc != MG_OK) return rc;
   return launch_int8_matmul(h, hs_q, d.inter_shared, hs_s, T, base + L.sh2, d.inter_shared,
                             reinterpret_cast<const float*>(base + L.shs2), d.hidden, d.inter_shared, out, d.hidden, EPI_PLAIN_BF16, st);
@@ -823,7 +823,7 @@ int mg_quantize_rows_int8(mg_handle hh, const void* d_x, int64_t n_rows, int64_t
   MG_REQUIRE(cols <= kInt8MaxK, MG_ERR_LIMIT, "mg_quantize_rows_int8: rows of %lld, at most %d", static_cast<long long>(cols), kInt8MaxK);
   if (n_rows == 0) return MG_OK;
   MG_REQUIRE(d_x && d_q && d_scale, MG_ERR_NULL, "mg_quantize_rows_int8: null pointer");
-  return launch_quantize_rows(h, d_x, n_rows, cols, ldx, d_q, ldq, d_scale, static_cast<cudaStream_t>(stream));
+  return launch_quantize_rows(d_x, n_rows, cols, ldx, d_q, ldq, d_scale, static_cast<cudaStream_t>(stream));
 }
 
 static int check_int8_product(int64_t n_rows, int64_t n_out, int64_t cols, const void* d_w, int64_t ldw, const float* d_ws,
@@ -887,7 +887,7 @@ int mg_int8_linear(mg_handle hh, const void* d_x, int64_t ldx, int64_t n_rows, c
   if (need == 0) return launch_int8_few(h, d_x, ldx, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, st);
   const int64_t ldq = round_up(cols, 128);
   float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(d_ws) + int8_linear_rows_bytes(n_rows, cols));
-  rc = launch_quantize_rows(h, d_x, n_rows, cols, ldx, d_ws, ldq, scale, st);
+  rc = launch_quantize_rows(d_x, n_rows, cols, ldx, d_ws, ldq, scale, st);
   if (rc != MG_OK) return rc;
   return launch_int8_matmul(h, d_ws, ldq, scale, n_rows, d_wq, ldw, d_w_scale, n_out, cols, d_out, ldo, EPI_PLAIN_BF16, st);
 }
@@ -1126,17 +1126,16 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
     rc = start_dequant(h, d_packed, deq, st, &launches);
     if (rc != MG_OK) return rc;
   }
-  // int8 experts: the tokens are quantised once, for the scatter and for the shared expert.  Ahead of the chain: the kernel
-  // behind it is launched by an ordinary dependence, so that the scatter may read the quantised rows as older memory.  Up to 128
-  // tokens the plan that copies the rows quantises them itself, and the shared expert has its own on its own stream (layer, us,
-  // V2-Lite 8 tokens in a graph 96 and 82, measured with the kernels chained).
+  // int8 experts: the tokens are quantised once, for the scatter and for the shared expert.  Up to 128 tokens the plan that copies
+  // the rows quantises them itself, and the shared expert's are quantised once more on its own stream: a kernel less in a row
+  // (layer in a graph, us, V2-Lite 8 tokens 82 and 78, 64 tokens 131.6 and 127.5).
   const bool i8 = d.weight_format == MG_WEIGHT_INT8_CHANNEL;
   uint8_t* xq = ws + L.off[WS_XQ];
   float* xs = reinterpret_cast<float*>(ws + L.off[WS_XS]);
   float* perm_s = i8 ? reinterpret_cast<float*>(ws + L.off[WS_PERM_S]) : nullptr;
   auto quantise = [&](cudaStream_t on) {
     launches += 1;
-    return launch_quantize_rows(h, d_x, T, d.hidden, d.hidden, xq, d.hidden, xs, on);
+    return launch_quantize_rows(d_x, T, d.hidden, d.hidden, xq, d.hidden, xs, on);
   };
   const bool copies = plan_copies(h, T) && !h->stage_timing;        // while stage times are recorded plan and scatter have their own
   if (i8 && !copies) {

@@ -259,7 +259,7 @@ int launch_ep_place(const Handle* h, const int32_t* idx, int64_t T, const int32_
                     cudaStream_t st);
 
 // 8-bit integers (int8.cu) ---------------------------------------------------------------
-int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
+int launch_quantize_rows(const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
                          cudaStream_t st, const int32_t* list = nullptr, int64_t list_rows = 0);
 bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols);        // few bf16 rows, quantised and multiplied by launch_int8_few
 int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, const void* wq, int64_t ldw, const float* w_scale,

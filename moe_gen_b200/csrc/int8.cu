@@ -24,8 +24,6 @@ __device__ __forceinline__ uint32_t block_amax(uint32_t pairs, uint32_t* s_max) 
 template <int VECS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int64_t ldx, int vecs, const int32_t* list,
                                                             int64_t list_rows, uint2* q, int64_t ldq, float* scale) {
-  chain_wait();
-  chain_go();
   __shared__ uint32_t s_max[8];
   const int64_t row = list != nullptr ? list[blockIdx.x] : static_cast<int64_t>(blockIdx.x);
   if (row < 0 || row >= list_rows) return;
@@ -55,8 +53,6 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const uint4* x, int6
 template <int VECS>
 __global__ void __launch_bounds__(256) quantize_short_rows_kernel(const uint4* x, int64_t ldx, int vecs, int64_t n, const int32_t* list,
                                                                   int64_t list_rows, uint2* q, int64_t ldq, float* scale) {
-  chain_wait();
-  chain_go();
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (item >= n) return;
@@ -207,8 +203,6 @@ __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uin
 // Rows (or listed rows) of any length, alignment and stride, element by element, read twice.
 __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* x, int64_t ldx, int cols, const int32_t* list,
                                                                 int64_t list_rows, uint8_t* q, int64_t ldq, float* scale) {
-  chain_wait();
-  chain_go();
   __shared__ uint32_t s_max[8];
   const int64_t row = list != nullptr ? list[blockIdx.x] : static_cast<int64_t>(blockIdx.x);
   if (row < 0 || row >= list_rows) return;
@@ -228,7 +222,7 @@ __global__ void __launch_bounds__(256) quantize_rows_any_kernel(const uint16_t* 
 }  // namespace
 
 // ldx in elements, ldq in bytes; list: nullptr, or the n rows to quantise of list_rows
-int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
+int launch_quantize_rows(const void* x, int64_t n, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
                          cudaStream_t st, const int32_t* list, int64_t list_rows) {
   if (n == 0) return MG_OK;
   MG_REQUIRE(n < (1ll << 31), MG_ERR_LIMIT, "quantise: %lld rows", static_cast<long long>(n));
@@ -241,22 +235,25 @@ int launch_quantize_rows(const Handle* h, const void* x, int64_t n, int64_t cols
     if (threads > 256) threads = 256;
     if (vecs <= 32 * kQuantVecs && n >= kWarpRows) {
 #define MG_QUANT(V)                                                                                                          \
-  MG_CUDA(launch_chained(h, quantize_short_rows_kernel<V>, static_cast<unsigned>((n + 7) / 8), 256, 0, st,                   \
-                         static_cast<const uint4*>(x), ldx / 8, static_cast<int>(vecs), n, list, bound, static_cast<uint2*>(q), \
-                         ldq / 8, scale))
+  quantize_short_rows_kernel<V><<<static_cast<unsigned>((n + 7) / 8), 256, 0, st>>>(                                         \
+      static_cast<const uint4*>(x), ldx / 8, static_cast<int>(vecs), n, list, bound, static_cast<uint2*>(q), ldq / 8, scale)
       if (vecs <= 128) MG_QUANT(4); else MG_QUANT(kQuantVecs);
+      MG_CUDA(cudaGetLastError());
       return MG_OK;
     }
 #undef MG_QUANT
 #define MG_QUANT(V)                                                                                                          \
-  MG_CUDA(launch_chained(h, quantize_rows_kernel<V>, static_cast<unsigned>(n), threads, 0, st, static_cast<const uint4*>(x), \
-                         ldx / 8, static_cast<int>(vecs), list, bound, static_cast<uint2*>(q), ldq / 8, scale))
+  quantize_rows_kernel<V><<<static_cast<unsigned>(n), threads, 0, st>>>(static_cast<const uint4*>(x), ldx / 8,               \
+                                                                        static_cast<int>(vecs), list, bound, static_cast<uint2*>(q), \
+                                                                        ldq / 8, scale)
     if (vecs <= 4 * threads) MG_QUANT(4); else MG_QUANT(kQuantVecs);
 #undef MG_QUANT
+    MG_CUDA(cudaGetLastError());
     return MG_OK;
   }
-  MG_CUDA(launch_chained(h, quantize_rows_any_kernel, static_cast<unsigned>(n), 256, 0, st, static_cast<const uint16_t*>(x), ldx,
-                         static_cast<int>(cols), list, bound, static_cast<uint8_t*>(q), ldq, scale));
+  quantize_rows_any_kernel<<<static_cast<unsigned>(n), 256, 0, st>>>(static_cast<const uint16_t*>(x), ldx, static_cast<int>(cols), list,
+                                                                     bound, static_cast<uint8_t*>(q), ldq, scale);
+  MG_CUDA(cudaGetLastError());
   return MG_OK;
 }
 

@@ -1577,8 +1577,9 @@ int launch_fill_duplicates(const Handle* h, void* rows, const int32_t* dup, int6
 // combine: y[t] = sum_j w[t,j] * out_rows[dst_row[t,j]] (+ shared[t])
 // ---------------------------------------------------------------------------------------
 // wide: the routed sum is not rounded to bf16 before the shared expert's row is added.  The other layers round there because the
-// reference does; int8 layers have none to follow, and it is one of four roundings of their result (V2-236B shape, 201 tokens,
-// error against 64 bits 0.0029 and 0.0025).
+// reference does; int8 layers have none to follow, and it is one of their result's roundings to bf16, behind those of the rows between
+// the products, of the experts' rows and of the shared expert's (V2-236B shape, 201 tokens under a skewed load, error against 64 bits
+// with it 0.0029, without 0.0023; V2-Lite 300 tokens 0.0024 and 0.0023).
 // by_slot = rank + 1 (expert-parallel pushed return): a pick whose owner is another rank lies at row
 // (token * k + slot) of this rank's return buffer (bufs.p[owner] all point at it), a pick of this rank's own
 // experts is read in place from its out_rows (bufs.p[rank]); 0 = rows as dst_row says.
