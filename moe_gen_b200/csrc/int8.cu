@@ -83,6 +83,9 @@ __global__ void __launch_bounds__(256) quantize_short_rows_kernel(const uint4* x
 // weight rows at a time by them with four-way dot products.  Few rows leave the tensor cores idle and their tiles few (a
 // block for 128 weight rows); here every SM streams a share of the weights.
 constexpr int kFewRows = 16, kFewWarps = 16, kFewSmem = 96 * 1024;
+// Blocks that run at once on an SM, by their registers: 60 to 64 a thread for up to four rows, 108 and 128 for eight and sixteen.  Asked
+// of the compiler as a launch bound, it spills: 2 rows 16384x4096 8.6 us without, 10.1 with it.
+constexpr int few_blocks(int m) { return m <= 4 ? 2 : 1; }
 template <int M>
 __global__ void __launch_bounds__(kFewWarps * 32) int8_few_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int rows, int cols,
                                                                        const uint8_t* __restrict__ w, int64_t ldw,
@@ -257,11 +260,11 @@ int launch_quantize_rows(const void* x, int64_t n, int64_t cols, int64_t ldx, vo
   return MG_OK;
 }
 
-// us with x and weights in L2, in a graph, one launch, and two (quantised, then on the tensor cores): 1 row 4096x4096 4.4 and 15.0,
-// 8192x8192 8.9 and 25.9; 4 rows 8192x8192 14.1 and 25.5; 8 rows 1024x1024 4.7 and 7.0, 4096x4096 8.6 and 14.6, 8192x2048 10.4 and
-// 9.6; 16 rows 512x512 5.7 and 5.7, 1024x2048 (outputs x inputs) 8.8 and 9.5, 4096x2048 9.0 and 9.6, 8192x1024 12.3 and 7.0 (a warp
-// quantises a row by itself, and every weight meets all rows from shared memory).  A launch takes 3 to 4 us of the call's host side,
-// which bounds these.  Beyond the line, 8 rows 8192x8192 25 in two launches as in one.
+// us with x and weights in L2, in a graph, one launch, and two (quantised, then by gemm_i8.cu): 1 row 4096x4096 4.0 and 14.8,
+// 8192x8192 8.7 and 25.7; 4 rows 8192x8192 13.8 and 25.3; 8 rows 1024x1024 4.6 and 6.7, 4096x4096 8.3 and 14.5, 8192x2048 (outputs x
+// inputs) 8.3 and 9.4, 16384x1024 10.9 and 7.0; 16 rows 512x512 5.5 and 5.4, 1024x2048 8.6 and 9.2, 4096x2048 8.7 and 9.5, 8192x1024
+// 10.4 and 7.0 (a warp quantises a row by itself, and every weight meets all rows from shared memory).  A launch takes 3 to 4 us of
+// the call's host side, which bounds a call that waits for nothing.
 // So beyond four rows up to 2^24 weights, beyond eight up to 2^23 and 2048 inputs.  Never beyond 2^30 outputs, which the kernel
 // counts in 32 bits, a whole grid's step past the last one included.
 bool int8_in_one_launch(int64_t rows, int64_t n_out, int64_t cols) {
@@ -280,8 +283,9 @@ static int launch_few(const Handle* h, const void* x, int64_t ldx, int64_t rows,
     if (h->device >= 0 && h->device < 64) done[h->device] = true;
   }
   const bool wide = cols % 8 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  // no more blocks than run at once, since each quantises all of x
-  const int64_t want = (n_out + 2 * kFewWarps - 1) / (2 * kFewWarps), most = static_cast<int64_t>(h->sm_count) * (smem > 64 * 1024 ? 2 : 3);
+  // no more blocks than run at once, since each quantises all of x: us, up to three blocks per SM and so, 8 rows 8192x2048 10.2 and
+  // 8.3, 2 rows 16384x4096 (outputs x inputs) 10.8 and 8.6, 16 rows 8192x1024 12.1 and 10.4; level where the outputs are few
+  const int64_t want = (n_out + 2 * kFewWarps - 1) / (2 * kFewWarps), most = static_cast<int64_t>(h->sm_count) * few_blocks(M);
   int8_few_rows_kernel<M><<<static_cast<unsigned>(want < most ? want : most), kFewWarps * 32, smem, st>>>(
       static_cast<const uint16_t*>(x), ldx, static_cast<int>(rows), static_cast<int>(cols), static_cast<const uint8_t*>(wq), ldw,
       w_scale, static_cast<int>(n_out), static_cast<__nv_bfloat16*>(out), ldo, wide);
