@@ -580,6 +580,7 @@ grouped_gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           }
         }
       }
+      drain_slots(empty, it % STAGES2, (it / STAGES2) & 1u, STAGES2, abort_flag, g.status, 11);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
@@ -653,6 +654,7 @@ grouped_gemm2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       }
       if (!ok) break;
     }
+    if (lane == 0) drain_slots(bfree, it % B2_SLOTS, (it / B2_SLOTS) & 1u, B2_SLOTS, abort_flag, g.status, 17);
   } else if (warp >= 2 && warp < 6) {
     // ---------------- epilogue (both CTAs, own 128 rows) ----------------
     const int quarter = warp & 3;

@@ -396,6 +396,7 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
           }
         }
       }
+      drain_slots(wempty, r.i, r.ph, C::SW, abort_flag, g.status, 51);
     }
   } else if (warp == 1) {
     // ---------------- token TMA (both CTAs, own half of each MMA's N) ----------------
@@ -435,6 +436,7 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
           if (h2 > 0) tma_load_3d_pair(dst + h1 * 128, m2, 0, row2, kb, fb);
         }
       }
+      drain_slots(tempty, r.i, r.ph, C::ST, abort_flag, g.status, 52);
     }
   } else if (warp == 2) {
     // ---------------- MMA issuer (leader CTA only) ----------------
@@ -686,6 +688,7 @@ grouped_gemm_wl_kernel(const __grid_constant__ WlMaps maps, const WlArgs g) {
       }
       first = (first + stages) & 1;
     }
+    if (lane == 0) drain_slots(afree + grp, 0u, ph, 1u, abort_flag, g.status, 58);
   }
 
   tc_fence_before();

@@ -320,6 +320,13 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
       ::"r"(bar), "h"(static_cast<uint16_t>(3))
       : "memory");
 }
+// A CTA of a pair leaves only when the releases of all its slots have arrived: the leader's commits signal both CTAs, and one still
+// on its way would find another block's shared memory.  Waits as if the n slots were filled once more, from slot i and phase ph on.
+__device__ __forceinline__ void drain_slots(uint64_t* released, uint32_t i, uint32_t ph, uint32_t n, volatile int* abort_flag,
+                                            int32_t* status, int where) {
+  for (uint32_t left = n; left > 0 && mbar_wait(smem_u32(&released[i]), ph ^ 1u, abort_flag, status, where); --left)
+    if (++i == n) { i = 0; ph ^= 1u; }
+}
 __device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                                  uint32_t accumulate) {
   asm volatile(
