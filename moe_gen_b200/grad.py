@@ -8,6 +8,9 @@ modeling_deepseek_v3.py:614-626).
     rows = sort_rows(layer, x, dst, layer.padded_rows(idx.numel()), counts, pad)
     ...                                                          # experts, adapters on rows
     y = combine_rows(layer, out_rows, dst, idx, w, counts, pad, shared_out)
+
+A step can be captured into a CUDA graph, its backward pass too; as with any torch step, no eager graph of the same leaves may be alive
+then (torch's accumulation nodes belong to the stream that they were made on).
 """
 from typing import Optional, Tuple
 
