@@ -330,6 +330,8 @@ int mg_pack_expert(mg_handle hh, int32_t local_expert, const void* d_gate, const
   Handle* h = check(hh);
   if (!h) return MG_ERR_STATE;
   MG_REQUIRE(d_gate && d_up && d_down && d_packed, MG_ERR_NULL, "mg_pack_expert: null pointer");
+  MG_REQUIRE(aligned16(d_gate) && aligned16(d_up) && aligned16(d_down) && aligned16(d_packed), MG_ERR_SHAPE,
+             "mg_pack_expert: matrices must begin on a 16-byte boundary");
   h->deq_valid = false;
   h->deq_inflight = false;
   return launch_pack_expert(h, local_expert, d_gate, d_up, d_down, gs, us, ds, d_packed,
@@ -341,6 +343,7 @@ int mg_dequant_fp8_block128(const void* d_q, const float* d_scale_inv, int64_t r
   MG_TRACE("mg_dequant_fp8_block128", rows);
   MG_REQUIRE(d_q && d_scale_inv && d_out, MG_ERR_NULL, "mg_dequant_fp8_block128: null pointer");
   MG_REQUIRE(rows >= 0 && cols >= 0, MG_ERR_SHAPE, "negative size");
+  MG_REQUIRE(aligned16(d_q) && aligned16(d_out), MG_ERR_SHAPE, "mg_dequant_fp8_block128: matrices must begin on a 16-byte boundary");
   return launch_dequant(d_q, d_scale_inv, rows, cols, d_out, static_cast<cudaStream_t>(stream));
 }
 
@@ -439,6 +442,7 @@ int mg_permute_rows(mg_handle hh, const void* d_x, const int32_t* d_dst, int64_t
   if (!h) return MG_ERR_STATE;
   MG_REQUIRE(d_x && d_dst && d_perm, MG_ERR_NULL, "mg_permute_rows: null pointer");
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_perm), MG_ERR_SHAPE, "mg_permute_rows: rows must begin on a 16-byte boundary");
   return launch_permute_rows(h, d_x, d_dst, T, d_perm, static_cast<cudaStream_t>(stream));
 }
 
@@ -1403,6 +1407,8 @@ int mg_rmsnorm(mg_handle hh, const void* d_x, const void* d_weight, float eps, i
   if (T == 0) return MG_OK;
   MG_REQUIRE(d_x && d_weight && d_out, MG_ERR_NULL, "mg_rmsnorm: null pointer");
   MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_rmsnorm: negative eps");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_weight) && aligned16(d_out), MG_ERR_SHAPE,
+             "mg_rmsnorm: rows and weight must begin on a 16-byte boundary");
   return launch_rmsnorm(h, d_x, d_weight, eps, T, d_out, static_cast<cudaStream_t>(stream));
 }
 

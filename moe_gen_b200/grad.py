@@ -16,16 +16,11 @@ from typing import Optional, Tuple
 
 import torch
 
-from .layer import MoELayer
+from .layer import MoELayer, _whole
 
 
-def _whole(t: torch.Tensor) -> torch.Tensor:
-    """t contiguous and on a 16-byte boundary, as the kernels read rows.  torch hands a gradient over as it comes: the backward of cat
-    and of flat views cuts it out of a larger tensor at any element."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
+# Gradients are taken through _whole: torch hands them over as they come, and the backward of cat and of flat views cuts them out of a
+# larger tensor at any element.
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, layer):

@@ -21,6 +21,12 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and on a 16-byte boundary, as the kernels read rows: a copy where it is a view that begins elsewhere."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 _NO_SWITCH = contextlib.nullcontext()
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -84,7 +90,7 @@ class MoELayer:
     # ------------------------------------------------------------------ weights
     def set_router(self, gate_weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
         """gate.weight [E,H] (kept as bf16) and, for noaux_tc, e_score_correction_bias [E] (fp32)."""
-        self.gate_w = gate_weight.detach().to(self.device, torch.bfloat16).contiguous()
+        self.gate_w = _whole(gate_weight.detach().to(self.device, torch.bfloat16))
         assert self.gate_w.shape == (self.E, self.H)
         self.bias = None if bias is None else bias.detach().to(self.device, torch.float32).contiguous()
 
@@ -96,7 +102,7 @@ class MoELayer:
         fp8 = self.desc.weight_format == L.WEIGHT_FP8_BLOCK128 and local_expert >= 0
         int8 = self.desc.weight_format == L.WEIGHT_INT8_CHANNEL
         dt = torch.float8_e4m3fn if fp8 else torch.int8 if int8 else torch.bfloat16
-        mats = [m.detach().to(self.device).contiguous() for m in (gate, up, down)]
+        mats = [_whole(m.detach().to(self.device)) for m in (gate, up, down)]
         I = self.Is if local_expert < 0 else self.I
         for m, shp in zip(mats, ((I, self.H), (I, self.H), (self.H, I))):
             if m.dtype != dt or tuple(m.shape) != shp:
@@ -606,7 +612,7 @@ class MoELayer:
 
     def dequant_fp8(self, q: torch.Tensor, scale_inv: torch.Tensor) -> torch.Tensor:
         """bf16(float(q) * scale[r/128][c/128]) (moe_gen/models/Wrapper.py:109-138)."""
-        q = q.to(self.device).contiguous()
+        q = _whole(q.to(self.device))
         s = scale_inv.to(self.device, torch.float32).contiguous()
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
         with self._on_device():
