@@ -87,6 +87,12 @@ class MoELayer:
             raise ValueError(f"{what}: expected contiguous {dtype} tensor on {self.device}, got "
                              f"{t.dtype} on {t.device} contiguous={t.is_contiguous()}")
 
+    def _check_out(self, out: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+        self._check_in(out, like.dtype, "out")
+        if out.numel() != like.numel():
+            raise ValueError(f"out: {tuple(out.shape)} for results of {tuple(like.shape)}")
+        return out
+
     # ------------------------------------------------------------------ weights
     def set_router(self, gate_weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
         """gate.weight [E,H] (kept as bf16) and, for noaux_tc, e_score_correction_bias [E] (fp32)."""
@@ -191,7 +197,7 @@ class MoELayer:
         self._check_in(x2, torch.bfloat16, "hidden_states")
         T = x2.shape[0]
         ws = self._workspace(T)
-        y = torch.empty_like(x2) if out is None else out
+        y = torch.empty_like(x2) if out is None else self._check_out(out, x2)
         with self._on_device():
             L.check(self.lib.mg_moe_forward(self._h, x2.data_ptr(), T, self.gate_w.data_ptr(), _ptr(self.bias),
                                             self.packed.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(),
@@ -212,7 +218,7 @@ class MoELayer:
         if tuple(logits.shape) != (T, self.E):
             raise ValueError(f"logits {tuple(logits.shape)}, expected {(T, self.E)}")
         ws = self._workspace(T)
-        y = torch.empty_like(x2) if out is None else out
+        y = torch.empty_like(x2) if out is None else self._check_out(out, x2)
         with self._on_device():
             L.check(self.lib.mg_moe_forward_from_logits(self._h, x2.data_ptr(), T, logits.data_ptr(), _ptr(self.bias),
                                                         self.packed.data_ptr(), ws.data_ptr(), ws.numel(),
@@ -229,7 +235,7 @@ class MoELayer:
         self._check_in(weight, torch.bfloat16, "norm weight")
         if weight.numel() != self.H:
             raise ValueError(f"norm weight has {weight.numel()} elements, hidden size is {self.H}")
-        y = torch.empty_like(x2) if out is None else out
+        y = torch.empty_like(x2) if out is None else self._check_out(out, x2)
         with self._on_device():
             L.check(self.lib.mg_rmsnorm(self._h, x2.data_ptr(), weight.data_ptr(), float(eps), x2.shape[0],
                                         y.data_ptr(), self._stream()))
@@ -251,7 +257,7 @@ class MoELayer:
         if getattr(self, "_xnorm", None) is None or self._xnorm.shape[0] < T:
             self._xnorm = torch.empty(max(T, 1), self.H, dtype=torch.bfloat16, device=self.device)
         xnorm = self._kept(self._xnorm)
-        y = torch.empty_like(h2) if out is None else out.reshape(-1, self.H)
+        y = torch.empty_like(h2) if out is None else self._check_out(out, h2)
         with self._on_device():
             L.check(self.lib.mg_moe_block_forward(self._h, h2.data_ptr(), norm_weight.data_ptr(), float(eps), T,
                                                   self.gate_w.data_ptr(), _ptr(self.bias), self.packed.data_ptr(),
