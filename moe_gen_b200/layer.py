@@ -304,7 +304,7 @@ class MoELayer:
 
     # ------------------------------------------------------------------ stages
     def gate_logits(self, x: torch.Tensor) -> torch.Tensor:
-        self._check_in(x, torch.bfloat16, "hidden_states")
+        self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
         T = x.shape[0]
         logits = torch.empty(T, self.E, dtype=torch.float32, device=self.device)
         with self._on_device():
@@ -327,7 +327,7 @@ class MoELayer:
         re-routed from exactly recomputed logits.  -> topk_idx, topk_w, logits (recomputed entries included),
         fix (int32: [0] tokens routed again, [1] of which with the whole row recomputed, [2] single logits
         recomputed; tokens from [4], row tokens from [4+T], (token, expert) pairs from [4+2T])."""
-        self._check_in(x, torch.bfloat16, "hidden_states")
+        self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
         T = x.shape[0]
         logits = torch.empty(T, self.E, dtype=torch.float32, device=self.device)
         idx = torch.empty(T, self.k, dtype=torch.int32, device=self.device)
@@ -574,6 +574,11 @@ class MoELayer:
                    predequant: bool = False):
         """-> (h_buf [rows,I], out_rows [rows,H]) over the padded expert-sorted rows.
         predequant=True (FP8 layers) de-quantises the weights into scratch first."""
+        self._check_rows(perm_x, torch.bfloat16, None, self.H, "perm_x")
+        self._check_in(counts, torch.int32, "counts")
+        self._check_in(pad_offsets, torch.int32, "pad_offsets")
+        if counts.numel() != self.e_local or pad_offsets.numel() != self.e_local + 1:
+            raise ValueError(f"counts of {counts.numel()} and pad_offsets of {pad_offsets.numel()} entries for {self.e_local} experts")
         rows = perm_x.shape[0]
         hbuf = torch.zeros(rows, self.I, dtype=torch.bfloat16, device=self.device)
         out = torch.zeros(rows, self.H, dtype=torch.bfloat16, device=self.device)
@@ -589,7 +594,7 @@ class MoELayer:
         return hbuf, out
 
     def shared_ffn(self, x: torch.Tensor) -> torch.Tensor:
-        self._check_in(x, torch.bfloat16, "hidden_states")
+        self._check_rows(x, torch.bfloat16, None, self.H, "hidden_states")
         T = x.shape[0]
         hs = torch.empty(T, self.Is, dtype=torch.bfloat16, device=self.device)
         out = torch.empty(T, self.H, dtype=torch.bfloat16, device=self.device)
