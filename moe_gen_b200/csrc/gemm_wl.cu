@@ -53,7 +53,8 @@
 // warp-wide role leave by the vote on a wait only, all at once: a lane that read the abort flag on its own would wait
 // at the closing barrier for lanes that wait for it in a warp-wide instruction, without a limit.  A role that gives
 // up has waited for the limit while the others could run ahead by a ring's length at most, so the loads still in
-// flight then were issued about as long ago and have landed.
+// flight then were issued about as long ago and have landed.  The roles that fill the rings leave only after the last
+// releases (drain_slots), which the leader's commits bring to both CTAs.
 #include "tc.cuh"
 
 namespace mg {

@@ -191,7 +191,8 @@ class MoELayer:
 
     # ------------------------------------------------------------------ whole layer
     def forward(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x: [..., H] bf16 on the layer's device -> same shape.  Asynchronous on the current stream."""
+        """x: [..., H] bf16 on the layer's device -> same shape.  Asynchronous on the current stream.  A layer's forwards share its
+        workspace: they follow one another on the GPU, replays of captured ones included."""
         shape = x.shape
         x2 = x.reshape(-1, self.H)
         self._check_in(x2, torch.bfloat16, "hidden_states")
