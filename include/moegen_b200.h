@@ -536,6 +536,84 @@ int mg_moe_block_forward(mg_handle h, const void* d_hidden, const void* d_norm_w
                          int64_t n_tokens, const void* d_gate_w, const float* d_bias, const void* d_packed,
                          void* d_xnorm, void* d_workspace, size_t workspace_bytes, void* d_out, void* stream);
 
+/* mg_moe_block_forward_add: mg_moe_block_forward of hidden + residual, the addition that precedes it in the decoder layer
+ * (modeling_deepseek_v3.py:1348-1359): h = bf16(hidden + residual), out = h + moe(rmsnorm(h)), h and its normalised rows from
+ * one launch (mg_add_rmsnorm).  d_out holds h meanwhile; it may be d_hidden or d_residual.
+ *
+ * The rows of the calls below are bf16, of any length, with columns adjacent and rows ld* elements apart; where lengths, strides
+ * and addresses are multiples of 8 elements they are read in 16-byte vectors.  The handle may be any layer's: it gives the
+ * device.
+ *
+ * mg_add_rmsnorm: sum = h = bf16(x + residual), out = mg_rmsnorm's rows of h, bit for bit.  Without a residual (NULL) h is x and d_sum is
+ *   not written.  d_sum and d_out may each be d_x or d_residual with its stride, not one another, and overlap nothing otherwise.
+ * mg_add_rmsnorm_int8: the rows v = weight * (h * rstd) in fp32, quantised as mg_quantize_rows_int8 does a row: bytes ldq apart
+ *   and one scale.  There is no rounding to bf16 in between.  d_q overlaps nothing.
+ * mg_add_rmsnorm_grad: with n = h * rstd, the forward's roundings counting as the identity,
+ *     grad_x = rstd * (weight grad_y - n mean(weight grad_y n)) + grad_h,   grad_w[cols] = sum over rows of grad_y n  (fp32)
+ *   grad_x is the gradient of x and of the residual alike.  d_grad_h, which reaches h by other ways, may be NULL; d_grad_x or
+ *   d_grad_w may be NULL and is then not computed; d_grad_x may be d_grad_y or d_grad_h with its stride.  At most 16384 columns.
+ *   d_ws: scratch of mg_add_rmsnorm_grad_ws_bytes bytes on a 4-byte boundary, for grad_w only.  The same rows, columns and device give
+ *   the same bits. */
+int mg_moe_block_forward_add(mg_handle h, const void* d_hidden, const void* d_residual, const void* d_norm_weight, float eps,
+                             int64_t n_tokens, const void* d_gate_w, const float* d_bias, const void* d_packed, void* d_xnorm,
+                             void* d_workspace, size_t workspace_bytes, void* d_out, void* stream);
+int mg_add_rmsnorm(mg_handle h, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, float eps,
+                   int64_t n_rows, int64_t cols, void* d_sum, int64_t lds, void* d_out, int64_t ldo, void* stream);
+int mg_add_rmsnorm_int8(mg_handle h, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, float eps,
+                        int64_t n_rows, int64_t cols, void* d_sum, int64_t lds, void* d_q, int64_t ldq, float* d_scale, void* stream);
+int mg_add_rmsnorm_grad_ws_bytes(mg_handle h, int64_t n_rows, int64_t cols, size_t* bytes);
+int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const void* d_h, int64_t ldh, const void* d_weight, float eps,
+                        int64_t n_rows, int64_t cols, const void* d_grad_h, int64_t ldgh, void* d_grad_x, int64_t ldgx, float* d_grad_w,
+                        void* d_ws, size_t ws_bytes, void* stream);
+
+/* ---- low-rank adapters beside a projection --------------------------------------------------- */
+/* For rows that belong to different requests, or to different experts, each with an adapter of its own beside the weights that
+ * all share (mg_int8_linear, mg_expert_ffn, ...).  No counterpart in the reference.  For the rows t of adapter g:
+ *   s[t] = bf16(x[t] . down[g]^T),   out[t] = y[t] + f[g] * s[t] . up[g]^T,   f[g] = factor * d_scale[g] (d_scale NULL: factor)
+ * with fp32 sums, out rounded once; out[t] = y[t] for rows without an adapter.
+ * down is [n_adapters][rank][cols], up [n_adapters][n_out][rank], bf16, with the rows of either matrix ld_* and the matrices *_stride
+ * elements apart.  All rows (x, y, out, gradients, down, up) begin on 16-byte boundaries: strides are multiples of 8.  Adapters of
+ * a lower rank are filled up with zeros.  rank <= 128, n_adapters <= MG_ADAPTER_MAX, cols and n_out <= 2^24, rows < 2^28.
+ *
+ * mg_adapter_plan: the rows sorted by adapter, from ids[n_rows]; an id that is negative or not below n_adapters means none.
+ *   d_plan: mg_adapter_plan_bytes bytes on a 16-byte boundary.  One plan serves all calls on these rows (with n_adapters
+ *   adapters), and is only read by them.
+ * mg_adapter_plan_sorted: the same for rows that lie sorted, by mg_permute_plan's counts[n_adapters] and
+ *   pad_offsets[n_adapters + 1]: adapter g has the rows [pad_offsets[g], pad_offsets[g] + counts[g]).  Offsets that leave
+ *   [0, n_rows] or descend are cut off.
+ * mg_adapter_add: with d_ids and no plan (NULL) up to MG_ADAPTER_DIRECT rows in one launch; with a plan any number, and d_ids is not
+ *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s: [n_rows]
+ *   rows of mg_adapter_rank_stride(rank) elements, zeros behind the rank and for rows without an adapter.
+ * mg_adapter_grad: the gradients, s and gs = bf16(f[g] * grad_out . up[g]) counting as unrounded:
+ *     grad_x[t] = gs[t] . down[g],   grad_down[g] = sum_t gs[t]^T x[t],   grad_up[g] = f[g] * sum_t grad_out[t]^T s[t]
+ *   grad_x is zero in rows without an adapter, grad_down [n_adapters][rank][cols] and grad_up [n_adapters][n_out][rank] (bf16, contiguous,
+ *   rounded once) in adapters without rows.  Each may be NULL and is then not computed.  The gradient of y is grad_out itself.  d_gs:
+ *   scratch like d_s.  d_s is read for grad_up alone.  The same rows and plan give the same bits. */
+#define MG_ADAPTER_MAX     1024
+#define MG_ADAPTER_DIRECT   256
+typedef struct mg_adapters {
+  int32_t struct_bytes;    /* = sizeof(mg_adapters), for versioning */
+  int32_t n_adapters;
+  int32_t rank;
+  float   factor;
+  int64_t cols, n_out;
+  const void* d_down;
+  int64_t down_stride, ld_down;
+  const void* d_up;
+  int64_t up_stride, ld_up;
+  const float* d_scale;    /* [n_adapters] or NULL */
+} mg_adapters;
+int mg_adapter_rank_stride(int32_t rank, int32_t* elements);
+int mg_adapter_plan_bytes(int64_t n_rows, int32_t n_adapters, size_t* bytes);
+int mg_adapter_plan(mg_handle h, const int32_t* d_ids, int64_t n_rows, int32_t n_adapters, void* d_plan, void* stream);
+int mg_adapter_plan_sorted(mg_handle h, const int32_t* d_counts, const int32_t* d_pad_offsets, int64_t n_rows, int32_t n_adapters,
+                           void* d_plan, void* stream);
+int mg_adapter_add(mg_handle h, const mg_adapters* adapters, const void* d_x, int64_t ldx, const void* d_y, int64_t ldy, int64_t n_rows,
+                   const int32_t* d_ids, const void* d_plan, void* d_out, int64_t ldo, void* d_s, void* stream);
+int mg_adapter_grad(mg_handle h, const mg_adapters* adapters, const void* d_grad_out, int64_t ldg, const void* d_x, int64_t ldx,
+                    int64_t n_rows, const void* d_plan, const void* d_s, void* d_gs, void* d_grad_x, int64_t ldgx, void* d_grad_down,
+                    void* d_grad_up, void* stream);
+
 /* Pointers into a workspace laid out by mg_moe_forward, for tests and tools:
  * which = 0 logits, 1 topk_idx, 2 topk_w, 3 counts, 4 offsets, 5 pad_offsets,
  * 6 dst_row, 7 perm_x, 8 h_buf, 9 out_rows. */

@@ -1430,6 +1430,228 @@ int mg_moe_block_forward(mg_handle hh, const void* d_hidden, const void* d_norm_
   return rc;
 }
 
+int mg_moe_block_forward_add(mg_handle hh, const void* d_hidden, const void* d_residual, const void* d_norm_weight, float eps, int64_t T,
+                             const void* d_gate_w, const float* d_bias, const void* d_packed, void* d_xnorm, void* d_ws, size_t ws_bytes,
+                             void* d_out, void* stream) {
+  MG_TRACE("mg_moe_block_forward_add", T);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
+  if (T == 0) { h->last_launches = 0; return MG_OK; }
+  MG_REQUIRE(d_hidden && d_residual && d_norm_weight && d_xnorm && d_out, MG_ERR_NULL, "mg_moe_block_forward_add: null pointer");
+  MG_REQUIRE(d_xnorm != d_hidden && d_xnorm != d_residual && d_xnorm != d_out, MG_ERR_CONFIG,
+             "mg_moe_block_forward_add: the normalised rows need a buffer of their own");
+  MG_REQUIRE(aligned16(d_hidden) && aligned16(d_residual) && aligned16(d_norm_weight) && aligned16(d_xnorm) && aligned16(d_out),
+             MG_ERR_SHAPE, "mg_moe_block_forward_add: rows and weight must begin on a 16-byte boundary");
+  const int64_t H = h->d.hidden;
+  int rc = mg_add_rmsnorm(hh, d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, stream);
+  if (rc != MG_OK) return rc;
+  rc = moe_forward_impl(hh, d_xnorm, T, d_gate_w, d_bias, d_packed, d_ws, ws_bytes, d_out, d_out, stream);
+  if (rc == MG_OK) h->last_launches += 1;
+  return rc;
+}
+
+// ---- norm with the residual's addition ----------------------------------------------------------------
+static int check_add_norm(const char* what, const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, float eps, int64_t n,
+                          int64_t cols, const void* sum, int64_t lds, const void* out, int64_t ldo) {
+  MG_REQUIRE(n >= 0 && cols >= 1 && ldx >= cols && ldo >= cols && (res == nullptr || (ldr >= cols && lds >= cols)), MG_ERR_SHAPE,
+             "%s: %lld rows of %lld, strides %lld, %lld, %lld and %lld", what, static_cast<long long>(n), static_cast<long long>(cols),
+             static_cast<long long>(ldx), static_cast<long long>(ldr), static_cast<long long>(lds), static_cast<long long>(ldo));
+  MG_REQUIRE(cols <= (1 << 24) && n < (1ll << 31), MG_ERR_LIMIT, "%s: %lld rows of %lld", what, static_cast<long long>(n),
+             static_cast<long long>(cols));
+  MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "%s: negative eps", what);
+  if (n == 0) return MG_OK;
+  MG_REQUIRE(x && w && out && (res == nullptr || sum), MG_ERR_NULL, "%s: null pointer", what);
+  MG_REQUIRE(res == nullptr || sum != out, MG_ERR_CONFIG, "%s: the sum and the normalised rows need a buffer each", what);
+  MG_REQUIRE(res == nullptr || ((sum != x || lds == ldx) && (sum != res || lds == ldr)), MG_ERR_CONFIG,
+             "%s: the sum's rows lie otherwise than those of the input that it replaces", what);
+  return MG_OK;
+}
+
+int mg_add_rmsnorm(mg_handle hh, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, float eps,
+                   int64_t n_rows, int64_t cols, void* d_sum, int64_t lds, void* d_out, int64_t ldo, void* stream) {
+  MG_TRACE("mg_add_rmsnorm", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_add_norm("mg_add_rmsnorm", d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_out, ldo);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(n_rows == 0 || ((d_out != d_x || ldo == ldx) && (d_out != d_residual || ldo == ldr)), MG_ERR_CONFIG,
+             "mg_add_rmsnorm: the normalised rows lie otherwise than those of the input that they replace");
+  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_out, ldo, nullptr,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int mg_add_rmsnorm_int8(mg_handle hh, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, float eps,
+                        int64_t n_rows, int64_t cols, void* d_sum, int64_t lds, void* d_q, int64_t ldq, float* d_scale, void* stream) {
+  MG_TRACE("mg_add_rmsnorm_int8", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_add_norm("mg_add_rmsnorm_int8", d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_q, ldq);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(n_rows == 0 || d_scale, MG_ERR_NULL, "mg_add_rmsnorm_int8: null pointer");
+  MG_REQUIRE(n_rows == 0 || (d_q != d_x && d_q != d_residual), MG_ERR_CONFIG, "mg_add_rmsnorm_int8: the bytes need a buffer of their own");
+  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_q, ldq, d_scale,
+                         static_cast<cudaStream_t>(stream));
+}
+
+static int check_norm_grad(const char* what, int64_t n, int64_t cols) {
+  MG_REQUIRE(n >= 0 && cols >= 1, MG_ERR_SHAPE, "%s: %lld rows of %lld", what, static_cast<long long>(n), static_cast<long long>(cols));
+  MG_REQUIRE(cols <= norm_grad_max_cols() && n < (1ll << 31), MG_ERR_LIMIT, "%s: %lld rows of %lld, at most %lld columns", what,
+             static_cast<long long>(n), static_cast<long long>(cols), static_cast<long long>(norm_grad_max_cols()));
+  return MG_OK;
+}
+
+int mg_add_rmsnorm_grad_ws_bytes(mg_handle hh, int64_t n_rows, int64_t cols, size_t* bytes) {
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  MG_REQUIRE(bytes, MG_ERR_NULL, "null argument");
+  int rc = check_norm_grad("mg_add_rmsnorm_grad_ws_bytes", n_rows, cols);
+  if (rc != MG_OK) return rc;
+  *bytes = norm_grad_ws_bytes(h, n_rows, cols);
+  return MG_OK;
+}
+
+int mg_add_rmsnorm_grad(mg_handle hh, const void* d_gy, int64_t ldgy, const void* d_h, int64_t ldh, const void* d_weight, float eps,
+                        int64_t n_rows, int64_t cols, const void* d_gh, int64_t ldgh, void* d_gx, int64_t ldgx, float* d_gw, void* d_ws,
+                        size_t ws_bytes, void* stream) {
+  MG_TRACE("mg_add_rmsnorm_grad", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_norm_grad("mg_add_rmsnorm_grad", n_rows, cols);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(ldgy >= cols && ldh >= cols && (d_gh == nullptr || ldgh >= cols) && (d_gx == nullptr || ldgx >= cols), MG_ERR_SHAPE,
+             "mg_add_rmsnorm_grad: rows of %lld, strides %lld, %lld, %lld and %lld", static_cast<long long>(cols),
+             static_cast<long long>(ldgy), static_cast<long long>(ldh), static_cast<long long>(ldgh), static_cast<long long>(ldgx));
+  MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_add_rmsnorm_grad: negative eps");
+  MG_REQUIRE(d_gx || d_gw, MG_ERR_NULL, "mg_add_rmsnorm_grad: no gradient asked for");
+  if (n_rows > 0) {
+    MG_REQUIRE(d_gy && d_h && d_weight && (d_gw == nullptr || d_ws), MG_ERR_NULL, "mg_add_rmsnorm_grad: null pointer");
+    MG_REQUIRE((d_gx != d_gy || ldgx == ldgy) && (d_gx != d_gh || d_gh == nullptr || ldgx == ldgh) && d_gx != d_h, MG_ERR_CONFIG,
+               "mg_add_rmsnorm_grad: grad_x lies otherwise than the gradient that it replaces, or over h");
+    const size_t need = norm_grad_ws_bytes(h, n_rows, cols);
+    MG_REQUIRE(d_gw == nullptr || ws_bytes >= need, MG_ERR_WORKSPACE, "mg_add_rmsnorm_grad: workspace %zu bytes, need %zu", ws_bytes, need);
+    MG_REQUIRE(d_gw == nullptr || reinterpret_cast<uintptr_t>(d_ws) % 4 == 0, MG_ERR_SHAPE,
+               "mg_add_rmsnorm_grad: the workspace must begin on a 4-byte boundary");
+  }
+  return launch_norm_grad(h, d_gy, ldgy, d_h, ldh, d_weight, eps, n_rows, cols, d_gh, ldgh, d_gx, ldgx, d_gw, d_ws,
+                          static_cast<cudaStream_t>(stream));
+}
+
+// ---- low-rank adapters -----------------------------------------------------------------------------------
+static bool row_stride(int64_t ld, int64_t cols) { return ld >= cols && ld % 8 == 0; }
+
+static int check_adapters(const char* what, const mg_adapters* a) {
+  MG_REQUIRE(a, MG_ERR_NULL, "%s: null pointer", what);
+  MG_REQUIRE(a->struct_bytes == static_cast<int32_t>(sizeof(mg_adapters)), MG_ERR_CONFIG, "%s: mg_adapters of %d bytes, expected %zu", what,
+             a->struct_bytes, sizeof(mg_adapters));
+  MG_REQUIRE(a->n_adapters >= 1 && a->rank >= 1 && a->cols >= 1 && a->n_out >= 1, MG_ERR_SHAPE, "%s: %d adapters of rank %d, %lld by %lld",
+             what, a->n_adapters, a->rank, static_cast<long long>(a->n_out), static_cast<long long>(a->cols));
+  MG_REQUIRE(a->n_adapters <= MG_ADAPTER_MAX && a->rank <= 128 && a->cols <= (1 << 24) && a->n_out <= (1 << 24), MG_ERR_LIMIT,
+             "%s: %d adapters of rank %d, %lld by %lld; at most %d of rank 128", what, a->n_adapters, a->rank,
+             static_cast<long long>(a->n_out), static_cast<long long>(a->cols), MG_ADAPTER_MAX);
+  MG_REQUIRE(a->d_down && a->d_up, MG_ERR_NULL, "%s: null adapters", what);
+  MG_REQUIRE(aligned16(a->d_down) && aligned16(a->d_up) && row_stride(a->ld_down, a->cols) && row_stride(a->ld_up, a->rank) &&
+                 (a->n_adapters == 1 || (a->down_stride >= 0 && a->up_stride >= 0 && a->down_stride % 8 == 0 && a->up_stride % 8 == 0)),
+             MG_ERR_SHAPE, "%s: the adapters' rows must begin on 16-byte boundaries (strides %lld, %lld, %lld, %lld)", what,
+             static_cast<long long>(a->down_stride), static_cast<long long>(a->ld_down), static_cast<long long>(a->up_stride),
+             static_cast<long long>(a->ld_up));
+  return MG_OK;
+}
+
+int mg_adapter_rank_stride(int32_t rank, int32_t* elements) {
+  MG_REQUIRE(elements, MG_ERR_NULL, "null argument");
+  MG_REQUIRE(rank >= 1 && rank <= 128, MG_ERR_LIMIT, "mg_adapter_rank_stride: rank %d, at most 128", rank);
+  *elements = adapter_padded_rank(rank);
+  return MG_OK;
+}
+
+static int check_adapter_rows(const char* what, int64_t n_rows, int32_t n_adapters) {
+  MG_REQUIRE(n_rows >= 0 && n_adapters >= 1, MG_ERR_SHAPE, "%s: %lld rows, %d adapters", what, static_cast<long long>(n_rows), n_adapters);
+  MG_REQUIRE(n_rows < (1 << 28) && n_adapters <= MG_ADAPTER_MAX, MG_ERR_LIMIT, "%s: %lld rows, %d adapters", what,
+             static_cast<long long>(n_rows), n_adapters);
+  return MG_OK;
+}
+
+int mg_adapter_plan_bytes(int64_t n_rows, int32_t n_adapters, size_t* bytes) {
+  MG_REQUIRE(bytes, MG_ERR_NULL, "null argument");
+  int rc = check_adapter_rows("mg_adapter_plan_bytes", n_rows, n_adapters);
+  if (rc != MG_OK) return rc;
+  *bytes = adapter_plan_bytes(n_rows, n_adapters);
+  return MG_OK;
+}
+
+int mg_adapter_plan(mg_handle hh, const int32_t* d_ids, int64_t n_rows, int32_t n_adapters, void* d_plan, void* stream) {
+  MG_TRACE("mg_adapter_plan", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_adapter_rows("mg_adapter_plan", n_rows, n_adapters);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(d_plan && (d_ids || n_rows == 0), MG_ERR_NULL, "mg_adapter_plan: null pointer");
+  MG_REQUIRE(aligned16(d_plan), MG_ERR_SHAPE, "mg_adapter_plan: the plan must begin on a 16-byte boundary");
+  // no rows: the empty segments come from this kernel as well, which reads no id then
+  return launch_adapter_plan(h, n_rows == 0 ? static_cast<const int32_t*>(d_plan) : d_ids, nullptr, nullptr, n_rows, n_adapters, d_plan,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int mg_adapter_plan_sorted(mg_handle hh, const int32_t* d_counts, const int32_t* d_pad, int64_t n_rows, int32_t n_adapters, void* d_plan,
+                           void* stream) {
+  MG_TRACE("mg_adapter_plan_sorted", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_adapter_rows("mg_adapter_plan_sorted", n_rows, n_adapters);
+  if (rc != MG_OK) return rc;
+  MG_REQUIRE(d_plan && d_counts && d_pad, MG_ERR_NULL, "mg_adapter_plan_sorted: null pointer");
+  MG_REQUIRE(aligned16(d_plan), MG_ERR_SHAPE, "mg_adapter_plan_sorted: the plan must begin on a 16-byte boundary");
+  return launch_adapter_plan(h, nullptr, d_counts, d_pad, n_rows, n_adapters, d_plan, static_cast<cudaStream_t>(stream));
+}
+
+int mg_adapter_add(mg_handle hh, const mg_adapters* ad, const void* d_x, int64_t ldx, const void* d_y, int64_t ldy, int64_t n_rows,
+                   const int32_t* d_ids, const void* d_plan, void* d_out, int64_t ldo, void* d_s, void* stream) {
+  MG_TRACE("mg_adapter_add", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_adapters("mg_adapter_add", ad);
+  if (rc == MG_OK) rc = check_adapter_rows("mg_adapter_add", n_rows, ad->n_adapters);
+  if (rc != MG_OK || n_rows == 0) return rc;
+  MG_REQUIRE(d_x && d_y && d_out && (d_ids || d_plan), MG_ERR_NULL, "mg_adapter_add: null pointer");
+  MG_REQUIRE(d_plan || n_rows <= MG_ADAPTER_DIRECT, MG_ERR_LIMIT, "mg_adapter_add: %lld rows without a plan, at most %d",
+             static_cast<long long>(n_rows), MG_ADAPTER_DIRECT);
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_y) && aligned16(d_out) && aligned16(d_s) && aligned16(d_plan) && row_stride(ldx, ad->cols) &&
+                 row_stride(ldy, ad->n_out) && row_stride(ldo, ad->n_out),
+             MG_ERR_SHAPE, "mg_adapter_add: rows must begin on 16-byte boundaries (strides %lld, %lld, %lld)", static_cast<long long>(ldx),
+             static_cast<long long>(ldy), static_cast<long long>(ldo));
+  MG_REQUIRE((d_out != d_y || ldo == ldy) && d_out != d_x, MG_ERR_CONFIG,
+             "mg_adapter_add: the results lie otherwise than the rows that they replace, or over x");
+  return launch_adapter_add(h, ad, d_x, ldx, d_y, ldy, n_rows, d_ids, d_plan, d_out, ldo, d_s, static_cast<cudaStream_t>(stream));
+}
+
+int mg_adapter_grad(mg_handle hh, const mg_adapters* ad, const void* d_gout, int64_t ldg, const void* d_x, int64_t ldx, int64_t n_rows,
+                    const void* d_plan, const void* d_s, void* d_gs, void* d_gx, int64_t ldgx, void* d_gdown, void* d_gup, void* stream) {
+  MG_TRACE("mg_adapter_grad", n_rows);
+  Handle* h = check(hh);
+  if (!h) return MG_ERR_STATE;
+  int rc = check_adapters("mg_adapter_grad", ad);
+  if (rc == MG_OK) rc = check_adapter_rows("mg_adapter_grad", n_rows, ad->n_adapters);
+  if (rc != MG_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (n_rows == 0) {
+    const size_t per = static_cast<size_t>(ad->n_adapters) * ad->rank * 2;
+    if (d_gdown) MG_CUDA(cudaMemsetAsync(d_gdown, 0, per * ad->cols, st));
+    if (d_gup) MG_CUDA(cudaMemsetAsync(d_gup, 0, per * ad->n_out, st));
+    return MG_OK;
+  }
+  MG_REQUIRE(d_gx || d_gdown || d_gup, MG_ERR_NULL, "mg_adapter_grad: no gradient asked for");
+  MG_REQUIRE(d_gout && d_plan && (d_x || !d_gdown) && (d_s || !d_gup) && (d_gs || (!d_gx && !d_gdown)), MG_ERR_NULL,
+             "mg_adapter_grad: null pointer");
+  MG_REQUIRE(aligned16(d_gout) && aligned16(d_x) && aligned16(d_s) && aligned16(d_gs) && aligned16(d_gx) && aligned16(d_plan) &&
+                 row_stride(ldg, ad->n_out) && (d_gdown == nullptr || row_stride(ldx, ad->cols)) &&
+                 (d_gx == nullptr || row_stride(ldgx, ad->cols)),
+             MG_ERR_SHAPE, "mg_adapter_grad: rows must begin on 16-byte boundaries (strides %lld, %lld, %lld)", static_cast<long long>(ldg),
+             static_cast<long long>(ldx), static_cast<long long>(ldgx));
+  MG_REQUIRE(d_gx == nullptr || (d_gx != d_gout && d_gx != d_x), MG_ERR_CONFIG, "mg_adapter_grad: grad_x needs a buffer of its own");
+  return launch_adapter_grad(h, ad, d_gout, ldg, d_x, ldx, n_rows, d_plan, d_s, d_gs, d_gx, ldgx, d_gdown, d_gup, st);
+}
+
 int mg_set_option(mg_handle hh, int32_t option, int32_t value) {
   Handle* h = check(hh);
   if (!h) return MG_ERR_STATE;

@@ -267,6 +267,25 @@ int launch_int8_few(const Handle* h, const void* x, int64_t ldx, int64_t rows, c
 int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float* x_scale, int64_t rows, const void* wq, int64_t ldw,
                        const float* w_scale, int64_t n_out, int64_t cols, void* out, int64_t ldo, int epilogue, cudaStream_t st);
 
+// norm with the residual's addition, and its gradient (norm.cu) ------------------------------
+int launch_add_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, float eps, int64_t n, int64_t cols,
+                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, cudaStream_t st);
+int64_t norm_grad_max_cols();
+size_t norm_grad_ws_bytes(const Handle* h, int64_t n, int64_t cols);
+int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* hrows, int64_t ldh, const void* w, float eps, int64_t n,
+                     int64_t cols, const void* gh, int64_t ldgh, void* gx, int64_t ldgx, float* gw, void* ws, cudaStream_t st);
+
+// low-rank adapters (adapter.cu) ---------------------------------------------------------------
+int adapter_padded_rank(int rank);       // elements between the rows of s and of gs
+int64_t adapter_direct_rows();           // rows of a call without a plan, at most
+size_t adapter_plan_bytes(int64_t rows, int64_t adapters);
+int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* counts, const int32_t* pad, int64_t rows, int adapters,
+                        void* plan, cudaStream_t st);
+int launch_adapter_add(const Handle* h, const mg_adapters* d, const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t rows,
+                       const int32_t* ids, const void* plan, void* out, int64_t ldo, void* s, cudaStream_t st);
+int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout, int64_t ldg, const void* x, int64_t ldx, int64_t rows,
+                        const void* plan, const void* s, void* gs, void* gx, int64_t ldgx, void* gdown, void* gup, cudaStream_t st);
+
 // weights (pack.cu) --------------------------------------------------------------------
 int launch_pack_expert(const Handle* h, int local_expert, const void* g, const void* u,
                        const void* dn, const float* gs, const float* us, const float* ds,

@@ -1,0 +1,512 @@
+// The residual's addition and the RMS norm behind it in one pass, rows out in bf16 or in 8-bit integers, and the gradient.
+//   h = bf16(x + residual), rstd = 1 / sqrt(mean(h^2) + eps), y = bf16(w * bf16(h * rstd))         (mg_rmsnorm's y of h)
+//   8 bits: v = w * (h * rstd) in fp32, m = max(max|v|, 2^-100), scale = m / 127, q = v * (127 / m) to the nearest, ties to even
+// h is rounded because it is stored so, and the norm is of what is stored.  y has the two roundings of the reference's module;
+// the 8-bit form has none before its own.
+#include "tc.cuh"
+
+namespace mg {
+
+namespace {
+
+constexpr int kNormLanes = 256;          // lanes over which a row's squares are summed, whatever the kernel (as in rmsnorm_kernel)
+constexpr int64_t kNormWarpRows = 2048;  // fewer rows than this have a block each, and its latency
+
+struct NormArgs {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint16_t* res;       // nullptr: h = x
+  int64_t ldr;
+  const uint16_t* w;
+  float eps;
+  int64_t n;
+  int cols;
+  uint16_t* sum;             // h, where there is a residual
+  int64_t lds;
+  void* out;                 // bf16 rows, or bytes with their scales
+  int64_t ldo;
+  float* scale;
+};
+
+__device__ __forceinline__ uint4 add8(const uint4& a, const uint4& b) {
+  float f[8], g[8];
+  unpack8(a, f);
+  unpack8(b, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(f[i], g[i]);
+  return pack8(f);
+}
+__device__ __forceinline__ float squares8(const uint4& q, float sum) {
+  float f[8];
+  unpack8(q, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+  return sum;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ float rstd_of(float sum, int cols, float eps) { return 1.0f / sqrtf(sum / static_cast<float>(cols) + eps); }
+// w * (h * rstd) of eight elements
+__device__ __forceinline__ void normal8(const uint4& h, const uint4& w, float rstd, float* f) {
+  float g[8];
+  unpack8(h, f);
+  unpack8(w, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(g[i], __fmul_rn(f[i], rstd));
+}
+__device__ __forceinline__ uint4 rounded8(const uint4& h, const uint4& w, float rstd) {
+  float f[8], g[8];
+  unpack8(h, f);
+  unpack8(w, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(g[i], round_bf16(__fmul_rn(f[i], rstd)));
+  return pack8(f);
+}
+// |v| as bits, which order as the numbers do; infinities and NaN are larger than any number
+__device__ __forceinline__ uint32_t amax_bits8(uint32_t m, const float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7FFFFFFFu);
+  return m;
+}
+__device__ __forceinline__ void row_scale_f32(uint32_t amax, float& scale, float& inv) {
+  const float m = fmaxf(__uint_as_float(amax), kQuantFloor);
+  const bool finite = amax < 0x7F800000u;
+  scale = finite ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7FC00000);
+  inv = finite ? __fdiv_rn(127.0f, m) : 0.0f;
+}
+__device__ __forceinline__ uint32_t byte_of(float v, float inv) { return __float_as_uint(__fmaf_rn(v, inv, 12582912.0f)); }
+__device__ __forceinline__ uint2 bytes8(const float* f, float inv) {
+  if (inv == 0.0f) return make_uint2(0u, 0u);
+  uint32_t q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = byte_of(f[i], inv);
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
+  return make_uint2(w[0], w[1]);
+}
+
+// A block per row of whole 16-byte vectors, which stay in registers between the sum and the output.
+template <int VECS, bool INT8>
+__global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) {
+  __shared__ float s_sum[kNormLanes / 32];
+  __shared__ uint32_t s_max[kNormLanes / 32];
+  const int64_t row = blockIdx.x;
+  const int vecs = a.cols >> 3, warp = threadIdx.x >> 5;
+  const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+  const uint4* w = reinterpret_cast<const uint4*>(a.w);
+  uint4 keep[VECS], wk[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = threadIdx.x + i * kNormLanes;
+    keep[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (v < vecs) keep[i] = x[v];
+  }
+  if (a.res != nullptr) {
+    const uint4* r = reinterpret_cast<const uint4*>(a.res + row * a.ldr);
+    uint4* h = reinterpret_cast<uint4*>(a.sum + row * a.lds);
+    uint4 other[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = threadIdx.x + i * kNormLanes;
+      if (v < vecs) other[i] = r[v];
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = threadIdx.x + i * kNormLanes;
+      if (v < vecs) h[v] = keep[i] = add8(keep[i], other[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = threadIdx.x + i * kNormLanes;
+    wk[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (v < vecs) wk[i] = w[v];
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) sum = squares8(keep[i], sum);
+  sum = warp_sum(sum);
+  if ((threadIdx.x & 31) == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kNormLanes / 32; ++i) sum += s_sum[i];
+  const float rstd = rstd_of(sum, a.cols, a.eps);
+  if (!INT8) {
+    uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ldo);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = threadIdx.x + i * kNormLanes;
+      if (v < vecs) y[v] = rounded8(keep[i], wk[i], rstd);
+    }
+    return;
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    float f[8];
+    normal8(keep[i], wk[i], rstd, f);
+    m = amax_bits8(m, f);
+  }
+  m = __reduce_max_sync(0xFFFFFFFFu, m);
+  if ((threadIdx.x & 31) == 0) s_max[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kNormLanes / 32; ++i) m = max(m, s_max[i]);
+  float scale, inv;
+  row_scale_f32(m, scale, inv);
+  uint2* q = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row * a.ldo);
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = threadIdx.x + i * kNormLanes;
+    float f[8];
+    normal8(keep[i], wk[i], rstd, f);
+    if (v < vecs) q[v] = bytes8(f, inv);
+  }
+  if (threadIdx.x == 0) a.scale[row] = scale;
+}
+
+// A warp per row, for many short rows.  Its lanes hold what lanes 32 apart would hold in a block, summed in the same order.
+template <int VECS, bool INT8>
+__global__ void __launch_bounds__(256) add_norm_short_kernel(const NormArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= a.n) return;
+  const int vecs = a.cols >> 3;
+  const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+  const uint4* w = reinterpret_cast<const uint4*>(a.w);
+  uint4 keep[VECS];
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = lane + i * 32;
+    keep[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (v < vecs) keep[i] = x[v];
+  }
+  if (a.res != nullptr) {
+    const uint4* r = reinterpret_cast<const uint4*>(a.res + row * a.ldr);
+    uint4* h = reinterpret_cast<uint4*>(a.sum + row * a.lds);
+    uint4 other[VECS];
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = lane + i * 32;
+      if (v < vecs) other[i] = r[v];
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = lane + i * 32;
+      if (v < vecs) h[v] = keep[i] = add8(keep[i], other[i]);
+    }
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) sum += warp_sum(squares8(keep[i], 0.f));
+  const float rstd = rstd_of(sum, a.cols, a.eps);
+  if (!INT8) {
+    uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ldo);
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int v = lane + i * 32;
+      if (v < vecs) y[v] = rounded8(keep[i], __ldg(w + v), rstd);
+    }
+    return;
+  }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = lane + i * 32;
+    float f[8];
+    if (v < vecs) {
+      normal8(keep[i], __ldg(w + v), rstd, f);
+      m = amax_bits8(m, f);
+    }
+  }
+  float scale, inv;
+  row_scale_f32(__reduce_max_sync(0xFFFFFFFFu, m), scale, inv);
+  uint2* q = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + row * a.ldo);
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    const int v = lane + i * 32;
+    float f[8];
+    if (v < vecs) {
+      normal8(keep[i], __ldg(w + v), rstd, f);
+      q[v] = bytes8(f, inv);
+    }
+  }
+  if (lane == 0) a.scale[row] = scale;
+}
+
+// Rows of any length, alignment and stride, element by element.  What is not kept is read again: h, where it was written, by
+// the thread that wrote it, so that x or the residual may be where it goes.
+template <bool INT8>
+__global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs a) {
+  __shared__ float s_sum[kNormLanes / 32];
+  __shared__ uint32_t s_max[kNormLanes / 32];
+  const int64_t row = blockIdx.x;
+  const int warp = threadIdx.x >> 5;
+  const uint16_t* x = a.x + row * a.ldx;
+  auto f32 = [](uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); };
+  float sum = 0.f;
+  for (int64_t v = threadIdx.x; v * 8 < a.cols; v += kNormLanes)
+    for (int c = static_cast<int>(v) * 8; c < a.cols && c < static_cast<int>(v) * 8 + 8; ++c) {
+      float f = f32(x[c]);
+      if (a.res != nullptr) {
+        const uint16_t b = __bfloat16_as_ushort(__float2bfloat16_rn(__fadd_rn(f, f32(a.res[row * a.ldr + c]))));
+        a.sum[row * a.lds + c] = b;
+        f = f32(b);
+      }
+      sum = fmaf(f, f, sum);
+    }
+  const uint16_t* h = a.res != nullptr ? a.sum + row * a.lds : x;
+  sum = warp_sum(sum);
+  if ((threadIdx.x & 31) == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+  for (int i = 0; i < kNormLanes / 32; ++i) sum += s_sum[i];
+  const float rstd = rstd_of(sum, a.cols, a.eps);
+  uint32_t m = 0;
+  for (int64_t v = threadIdx.x; v * 8 < a.cols; v += kNormLanes)
+    for (int c = static_cast<int>(v) * 8; c < a.cols && c < static_cast<int>(v) * 8 + 8; ++c) {
+      const float n = __fmul_rn(f32(h[c]), rstd), w = f32(a.w[c]);
+      if (INT8)
+        m = max(m, __float_as_uint(__fmul_rn(w, n)) & 0x7FFFFFFFu);
+      else
+        static_cast<uint16_t*>(a.out)[row * a.ldo + c] = __bfloat16_as_ushort(__float2bfloat16_rn(__fmul_rn(w, round_bf16(n))));
+    }
+  if (!INT8) return;
+  m = __reduce_max_sync(0xFFFFFFFFu, m);
+  if ((threadIdx.x & 31) == 0) s_max[warp] = m;
+  __syncthreads();
+  for (int i = 0; i < kNormLanes / 32; ++i) m = max(m, s_max[i]);
+  float scale, inv;
+  row_scale_f32(m, scale, inv);
+  for (int64_t v = threadIdx.x; v * 8 < a.cols; v += kNormLanes)
+    for (int c = static_cast<int>(v) * 8; c < a.cols && c < static_cast<int>(v) * 8 + 8; ++c)
+      static_cast<uint8_t*>(a.out)[row * a.ldo + c] =
+          inv == 0.0f ? 0 : static_cast<uint8_t>(byte_of(__fmul_rn(f32(a.w[c]), __fmul_rn(f32(h[c]), rstd)), inv));
+  if (threadIdx.x == 0) a.scale[row] = scale;
+}
+
+// ---- gradient ----------------------------------------------------------------------------
+// With n = h * rstd (the forward's roundings count as the identity):
+//   gx = rstd * (w gy - n mean(w gy n)) + gh,   gw = sum over rows of gy n
+// mean(w gy n) = rstd sum(w gy h) / cols, so that both sums of a row come from one reading.  Blocks stay and take rows in turn; a
+// thread holds the same columns of every row, and its share of gw in fp32.  The shares are summed by a second launch, in the
+// order of the blocks: the same rows and columns give the same bits.
+struct NormGradArgs {
+  const uint16_t* gy;
+  int64_t ldgy;
+  const uint16_t* h;
+  int64_t ldh;
+  const uint16_t* w;
+  float eps;
+  int64_t n;
+  int cols;
+  const uint16_t* gh;        // nullptr: none
+  int64_t ldgh;
+  uint16_t* gx;              // nullptr: not wanted
+  int64_t ldgx;
+  float* parts;              // [shares][cols], nullptr: gw is not wanted
+  int lanes;                 // threads to a row
+};
+constexpr int kGradThreads = 1024, kGradMaxCols = 2 * 8 * kGradThreads;      // up to two vectors of a row to a thread
+
+template <bool WIDE>
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int c, int cols) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (WIDE) {
+    if (c < cols) v = *reinterpret_cast<const uint4*>(p + c);
+  } else {
+    uint32_t* u = &v.x;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) u[i >> 1] |= static_cast<uint32_t>(p[c + i]) << (16 * (i & 1));
+  }
+  return v;
+}
+
+template <int VECS, bool WIDE>
+__global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGradArgs a) {
+  __shared__ float2 s_sum[2][kGradThreads / 32];
+  const int lanes = a.lanes, sub = threadIdx.x / lanes, t = threadIdx.x - sub * lanes, rows = blockDim.x / lanes;
+  const int warp = threadIdx.x >> 5, warps = lanes >> 5;
+  uint4 w[VECS], h[VECS], gy[VECS], gh[VECS];
+  float acc[VECS][8];
+  auto load = [&](int64_t row) {
+    const int cols = row < a.n ? a.cols : 0;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int c = (t + i * lanes) * 8;
+      h[i] = load8<WIDE>(a.h + row * a.ldh, c, cols);
+      gy[i] = load8<WIDE>(a.gy + row * a.ldgy, c, cols);
+      gh[i] = load8<WIDE>(a.gh + row * a.ldgh, c, a.gh != nullptr ? cols : 0);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < VECS; ++i) {
+    w[i] = load8<WIDE>(a.w, (t + i * lanes) * 8, a.cols);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * rows; base < a.n; base += static_cast<int64_t>(gridDim.x) * rows, turn ^= 1) {
+    const int64_t row = base + sub;
+    const bool live = row < a.n;
+    load(row);
+    float ss = 0.f, sp = 0.f;
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      float fh[8], fg[8], fw[8];
+      unpack8(h[i], fh);
+      unpack8(gy[i], fg);
+      unpack8(w[i], fw);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ss = fmaf(fh[j], fh[j], ss);
+        sp = fmaf(__fmul_rn(fw[j], fg[j]), fh[j], sp);
+      }
+    }
+    ss = warp_sum(ss);
+    sp = warp_sum(sp);
+    if (warps > 1) {
+      if ((threadIdx.x & 31) == 0) s_sum[turn][warp] = make_float2(ss, sp);
+      __syncthreads();               // the other half of s_sum is written in the next turn: no thread is two turns ahead
+      ss = sp = 0.f;
+      for (int i = 0; i < warps; ++i) {
+        const float2 v = s_sum[turn][sub * warps + i];
+        ss += v.x;
+        sp += v.y;
+      }
+    }
+    const float rstd = rstd_of(ss, a.cols, a.eps);
+    const float c2 = __fmul_rn(__fmul_rn(rstd, rstd), sp / static_cast<float>(a.cols));
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) {
+      const int c = (t + i * lanes) * 8;
+      float fh[8], fg[8], fw[8], fr[8];
+      unpack8(h[i], fh);
+      unpack8(gy[i], fg);
+      unpack8(w[i], fw);
+      unpack8(gh[i], fr);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (live) acc[i][j] = fmaf(fg[j], __fmul_rn(fh[j], rstd), acc[i][j]);
+        fr[j] = fmaf(rstd, fmaf(-fh[j], c2, __fmul_rn(fw[j], fg[j])), fr[j]);
+      }
+      if (a.gx == nullptr || !live) continue;
+      uint16_t* dst = a.gx + row * a.ldgx;
+      const uint4 v = pack8(fr);
+      if (WIDE) {
+        if (c < a.cols) *reinterpret_cast<uint4*>(dst + c) = v;
+      } else {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < a.cols) dst[c + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+  }
+  if (a.parts == nullptr) return;
+  float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * rows + sub) * a.cols;
+#pragma unroll
+  for (int i = 0; i < VECS; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = (t + i * lanes) * 8 + j;
+      if (c < a.cols) part[c] = acc[i][j];
+    }
+}
+
+// gw[c] = the sum of the shares of column c: 32 columns and 32 shares at a time to a block
+__global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* parts, int shares, int cols, float* gw) {
+  __shared__ float s[32][33];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
+  float v = 0.f;
+  if (c < cols)
+    for (int p = y; p < shares; p += 32) v += parts[static_cast<int64_t>(p) * cols + c];
+  s[y][x] = v;
+  __syncthreads();
+  v = warp_sum(s[x][y]);             // warp y: the 32 sums of column y of the block
+  if (x == 0 && blockIdx.x * 32 + y < cols) gw[blockIdx.x * 32 + y] = v;
+}
+
+struct NormGradPlan { int vecs, lanes, threads, blocks, shares; };
+NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
+  NormGradPlan p;
+  const int vecs = static_cast<int>((cols + 7) / 8);
+  p.vecs = vecs <= kGradThreads ? 1 : 2;
+  p.lanes = (vecs + 32 * p.vecs - 1) / (32 * p.vecs) * 32;
+  p.threads = p.lanes >= 256 ? p.lanes : 256 / p.lanes * p.lanes;
+  const int rows = p.threads / p.lanes;
+  const int64_t want = (n + rows - 1) / rows, most = static_cast<int64_t>(h->sm_count) * (kGradThreads / p.threads);
+  p.blocks = static_cast<int>(want < most ? want : most);
+  p.shares = p.blocks * rows;
+  return p;
+}
+
+bool on16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+
+template <bool INT8>
+int launch_add_norm_as(const NormArgs& a, cudaStream_t st) {
+  const int vecs = a.cols / 8;
+  const bool wide = a.cols % 8 == 0 && on16(a.x, a.ldx) && (a.res == nullptr || (on16(a.res, a.ldr) && on16(a.sum, a.lds))) &&
+                    on16(a.w, 0) && vecs <= 8 * kNormLanes && reinterpret_cast<uintptr_t>(a.out) % (INT8 ? 8 : 16) == 0 && a.ldo % 8 == 0;
+  const unsigned rows = static_cast<unsigned>(a.n), eighth = static_cast<unsigned>((a.n + 7) / 8);
+  if (!wide) add_norm_any_kernel<INT8><<<rows, kNormLanes, 0, st>>>(a);
+  else if (a.n >= kNormWarpRows && vecs <= 64) add_norm_short_kernel<2, INT8><<<eighth, 256, 0, st>>>(a);
+  else if (a.n >= kNormWarpRows && vecs <= 256) add_norm_short_kernel<8, INT8><<<eighth, 256, 0, st>>>(a);
+  else if (vecs <= kNormLanes) add_norm_kernel<1, INT8><<<rows, kNormLanes, 0, st>>>(a);
+  else if (vecs <= 2 * kNormLanes) add_norm_kernel<2, INT8><<<rows, kNormLanes, 0, st>>>(a);
+  else if (vecs <= 4 * kNormLanes) add_norm_kernel<4, INT8><<<rows, kNormLanes, 0, st>>>(a);
+  else add_norm_kernel<8, INT8><<<rows, kNormLanes, 0, st>>>(a);
+  MG_CUDA(cudaGetLastError());
+  return MG_OK;
+}
+
+}  // namespace
+
+// scale: nullptr for bf16 rows, ldo in elements of out either way
+int launch_add_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, float eps, int64_t n, int64_t cols,
+                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, cudaStream_t st) {
+  if (n == 0) return MG_OK;
+  NormArgs a{static_cast<const uint16_t*>(x), ldx, static_cast<const uint16_t*>(res), ldr, static_cast<const uint16_t*>(w), eps, n,
+             static_cast<int>(cols), static_cast<uint16_t*>(sum), lds, out, ldo, scale};
+  return scale != nullptr ? launch_add_norm_as<true>(a, st) : launch_add_norm_as<false>(a, st);
+}
+
+int64_t norm_grad_max_cols() { return kGradMaxCols; }
+
+size_t norm_grad_ws_bytes(const Handle* h, int64_t n, int64_t cols) {
+  return static_cast<size_t>(norm_grad_plan(h, n, cols).shares) * cols * sizeof(float);
+}
+
+int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* hrows, int64_t ldh, const void* w, float eps, int64_t n,
+                     int64_t cols, const void* gh, int64_t ldgh, void* gx, int64_t ldgx, float* gw, void* ws, cudaStream_t st) {
+  if (n == 0) {
+    if (gw != nullptr) MG_CUDA(cudaMemsetAsync(gw, 0, cols * sizeof(float), st));
+    return MG_OK;
+  }
+  const NormGradPlan p = norm_grad_plan(h, n, cols);
+  NormGradArgs a{static_cast<const uint16_t*>(gy), ldgy, static_cast<const uint16_t*>(hrows), ldh, static_cast<const uint16_t*>(w), eps, n,
+                 static_cast<int>(cols), static_cast<const uint16_t*>(gh), ldgh, static_cast<uint16_t*>(gx), ldgx,
+                 gw != nullptr ? static_cast<float*>(ws) : nullptr, p.lanes};
+  const bool wide = cols % 8 == 0 && on16(gy, ldgy) && on16(hrows, ldh) && on16(w, 0) && (gh == nullptr || on16(gh, ldgh)) &&
+                    (gx == nullptr || on16(gx, ldgx));
+  if (wide && p.vecs == 1) norm_grad_kernel<1, true><<<p.blocks, p.threads, 0, st>>>(a);
+  else if (wide) norm_grad_kernel<2, true><<<p.blocks, p.threads, 0, st>>>(a);
+  else if (p.vecs == 1) norm_grad_kernel<1, false><<<p.blocks, p.threads, 0, st>>>(a);
+  else norm_grad_kernel<2, false><<<p.blocks, p.threads, 0, st>>>(a);
+  MG_CUDA(cudaGetLastError());
+  if (gw != nullptr) {
+    norm_grad_sum_kernel<<<static_cast<unsigned>((cols + 31) / 32), 1024, 0, st>>>(static_cast<const float*>(ws), p.shares,
+                                                                                 static_cast<int>(cols), gw);
+    MG_CUDA(cudaGetLastError());
+  }
+  return MG_OK;
+}
+
+}  // namespace mg

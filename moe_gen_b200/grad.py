@@ -9,14 +9,17 @@ modeling_deepseek_v3.py:614-626).
     ...                                                          # experts, adapters on rows
     y = combine_rows(layer, out_rows, dst, idx, w, counts, pad, shared_out)
 
+    h, y = add_norm(layer, x, residual, weight, eps)             # the norm in front of the block, and the residual stream
+    out_rows = adapt_rows(layer, out_rows, rows, down, up, layer.adapter_plan_sorted(counts, pad, rows.shape[0]), scale)
+
 A step can be captured into a CUDA graph, its backward pass too; as with any torch step, no eager graph of the same leaves may be alive
 then (torch's accumulation nodes belong to the stream that they were made on).
 """
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
-from .layer import MoELayer, _whole
+from .layer import AdapterPlan, MoELayer, _whole
 
 
 # Gradients are taken through _whole: torch hands them over as they come, and the backward of cat and of flat views cuts them out of a
@@ -69,6 +72,56 @@ class _CombineRows(torch.autograd.Function):
         return grows, gw, grad_y if ctx.needs_input_grad[2] else None, None, None, None, None, None
 
 
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, layer, eps):
+        y, h = layer.add_rmsnorm(x, residual, weight, eps)
+        if residual is None:
+            h = x.clone()               # an output of its own: what is done to it in place is not done to x
+        ctx.layer, ctx.eps = layer, eps
+        ctx.save_for_backward(x if residual is None else h, weight)
+        ctx.set_materialize_grads(False)
+        return h, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_h, grad_y):
+        h, weight = ctx.saved_tensors
+        need_x, need_w = ctx.needs_input_grad[0] or ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        gw = None
+        if grad_y is None:
+            gx = grad_h
+        else:
+            gx, gw = ctx.layer.add_rmsnorm_grad(grad_y.contiguous(), h, weight, ctx.eps, None if grad_h is None else grad_h.contiguous(),
+                                                need_x, need_w)
+            gw = None if gw is None else gw.to(weight.dtype)
+        return gx if ctx.needs_input_grad[0] else None, gx if ctx.needs_input_grad[1] else None, gw, None, None
+
+
+class _AdaptRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, down, up, layer, plan, scale):
+        out, s = layer.adapter_add(y, x, down, up, plan, scale, keep=True)
+        ctx.layer, ctx.plan, ctx.scale = layer, plan, scale
+        ctx.save_for_backward(x, down, up, s)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        x, down, up, s = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gx = gdown = gup = None
+        if any(need[1:4]):
+            n_out = grad_out.shape[1]
+            rows = _whole(grad_out)
+            if n_out % 8:               # rows on 16-byte boundaries
+                rows = torch.empty_strided(grad_out.shape, ((n_out + 7) // 8 * 8, 1), dtype=grad_out.dtype, device=grad_out.device)
+                rows.copy_(grad_out)
+            gx, gdown, gup = ctx.layer.adapter_grad(rows, x, down, up, ctx.plan, ctx.scale, s, *need[1:4])
+        return grad_out if need[0] else None, gx, gdown, gup, None, None, None
+
+
 def route(layer: MoELayer, logits: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """MoELayer.route_topk, its weights differentiable in the logits (the picks are constants)."""
     return _Route.apply(logits, layer)
@@ -84,3 +137,16 @@ def combine_rows(layer: MoELayer, out_rows: torch.Tensor, dst_row: torch.Tensor,
                  counts: torch.Tensor, pad_offsets: torch.Tensor, shared_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """MoELayer.combine, differentiable in out_rows, topk_w and shared_out (its bf16 modes' roundings count as the identity)."""
     return _CombineRows.apply(out_rows, topk_w, shared_out, layer, dst_row, topk_idx, counts, pad_offsets)
+
+
+def add_norm(layer: MoELayer, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
+             eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """MoELayer.add_rmsnorm -> (h, y), differentiable in x, residual and weight: h = x + residual goes on as the residual stream, y is its
+    norm.  Without a residual h is a copy of x."""
+    return _AddNorm.apply(x, residual, weight, layer, eps)
+
+
+def adapt_rows(layer: MoELayer, y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan: AdapterPlan,
+               scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
+    """MoELayer.adapter_add by a plan, differentiable in y, x, down and up (the scales are constants)."""
+    return _AdaptRows.apply(y, x, down, up, layer, plan, scale)

@@ -27,6 +27,14 @@ def _whole(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+class AdapterPlan:
+    """Rows sorted by their adapters (MoELayer.adapter_plan, .adapter_plan_sorted), for every adapter call on these rows."""
+    __slots__ = ("buf", "rows", "n_adapters")
+
+    def __init__(self, buf: torch.Tensor, rows: int, n_adapters: int):
+        self.buf, self.rows, self.n_adapters = buf, rows, n_adapters
+
+
 _NO_SWITCH = contextlib.nullcontext()
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -242,11 +250,90 @@ class MoELayer:
                                         y.data_ptr(), self._stream()))
         return y.view(x.shape)
 
+    def _norm_args(self, x, residual, weight, sum_out):
+        """Rows, columns and strides of x, the residual and their sum; the sum's tensor."""
+        n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
+        self._check_in(weight, torch.bfloat16, "norm weight")
+        if weight.numel() != cols:
+            raise ValueError(f"norm weight has {weight.numel()} elements, rows have {cols}")
+        if residual is None:
+            if sum_out is not None:
+                raise ValueError("sum_out: there is no residual to add")
+            return n, cols, ldx, 0, x, 0
+        nr, rcols, ldr = self._rows_of(residual, torch.bfloat16, "residual")
+        if (nr, rcols) != (n, cols):
+            raise ValueError(f"residual {tuple(residual.shape)} for rows of {tuple(x.shape)}")
+        sum_out, lds = self._out_rows(sum_out, n, cols, "sum_out")
+        return n, cols, ldx, ldr, sum_out, lds
+
+    def _out_rows(self, out: Optional[torch.Tensor], n: int, cols: int, what: str):
+        """out and the elements between its rows; a new one has its rows on 16-byte boundaries."""
+        if out is None:
+            ld = (cols + 7) // 8 * 8
+            return torch.empty_strided((n, cols), (ld, 1), dtype=torch.bfloat16, device=self.device), ld
+        rows, o_cols, ld = self._rows_of(out, torch.bfloat16, what)
+        if (rows, o_cols) != (n, cols):
+            raise ValueError(f"{what} {tuple(out.shape)}, expected {(n, cols)}")
+        return out, ld
+
+    def add_rmsnorm(self, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
+                    out: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
+        """-> (rmsnorm(h), h) with h = bf16(x + residual), in one launch; h = x without a residual.  x, residual and weight bf16,
+        [rows, cols] with adjacent columns (any cols, rows may lie further apart).  out and sum_out may each be x or the residual,
+        not one another, and overlap nothing otherwise.  Any layer serves."""
+        n, cols, ldx, ldr, h, lds = self._norm_args(x, residual, weight, sum_out)
+        y, ldo = self._out_rows(out, n, cols, "out")
+        with self._on_device():
+            L.check(self.lib.mg_add_rmsnorm(self._h, x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), eps, n, cols,
+                                            None if residual is None else h.data_ptr(), lds, y.data_ptr(), ldo, self._stream()))
+        return y, h
+
+    def add_rmsnorm_int8(self, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
+                         sum_out: Optional[torch.Tensor] = None):
+        """-> (q, scale, h): add_rmsnorm with its rows quantised as quantize_rows does (int8 on 128-byte strides, fp32 scales), from
+        their fp32 values; what int8_matmul and permute_rows_int8 take."""
+        n, cols, ldx, ldr, h, lds = self._norm_args(x, residual, weight, sum_out)
+        ldq = (cols + 127) // 128 * 128
+        q = torch.empty_strided((n, cols), (ldq, 1), dtype=torch.int8, device=self.device)
+        scale = torch.empty(n, dtype=torch.float32, device=self.device)
+        with self._on_device():
+            L.check(self.lib.mg_add_rmsnorm_int8(self._h, x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), eps, n, cols,
+                                                 None if residual is None else h.data_ptr(), lds, q.data_ptr(), ldq, scale.data_ptr(),
+                                                 self._stream()))
+        return q, scale, h
+
+    def add_rmsnorm_grad(self, grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                         grad_h: Optional[torch.Tensor] = None, need_x: bool = True, need_w: bool = True):
+        """Gradients of add_rmsnorm for grad_y and for grad_h, which reaches h by other ways -> (grad_x, which is the residual's too,
+        bf16; grad_weight [cols] fp32), None for the one that is not needed.  At most 16384 columns."""
+        n, cols, ldh = self._rows_of(h, torch.bfloat16, "h")
+        self._check_in(weight, torch.bfloat16, "norm weight")
+        if weight.numel() != cols:
+            raise ValueError(f"norm weight has {weight.numel()} elements, rows have {cols}")
+        ng, gcols, ldgy = self._rows_of(grad_y, torch.bfloat16, "grad_y")
+        nh, hcols, ldgh = (n, cols, 0) if grad_h is None else self._rows_of(grad_h, torch.bfloat16, "grad_h")
+        if (ng, gcols) != (n, cols) or (nh, hcols) != (n, cols):
+            raise ValueError(f"gradients of {(ng, gcols)} and {(nh, hcols)} for rows of {(n, cols)}")
+        gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
+        gw = ws = None
+        size = C.c_size_t()
+        if need_w:
+            gw = torch.empty(cols, dtype=torch.float32, device=self.device)
+            L.check(self.lib.mg_add_rmsnorm_grad_ws_bytes(self._h, n, cols, C.byref(size)))
+            ws = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+        if not (need_x or need_w):
+            return None, None
+        with self._on_device():
+            L.check(self.lib.mg_add_rmsnorm_grad(self._h, grad_y.data_ptr(), ldgy, h.data_ptr(), ldh, weight.data_ptr(), eps, n, cols,
+                                                 _ptr(grad_h), ldgh, _ptr(gx), ldgx, _ptr(gw), _ptr(ws), size.value, self._stream()))
+        return gx, gw
+
     def block_forward(self, hidden: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,
-                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         """hidden + moe(rmsnorm(hidden)): the decoder layer's second half
         (modeling_deepseek_v3.py:1361-1365) with the residual add done by the combine kernel.
-        out may be hidden itself (in-place update of the residual stream)."""
+        out may be hidden itself (in-place update of the residual stream).  With a residual (same shape) the block runs on
+        bf16(hidden + residual), as if that had been handed in, added by the norm's launch (add_rmsnorm); out may be either."""
         shape = hidden.shape
         h2 = hidden.reshape(-1, self.H)
         self._check_in(h2, torch.bfloat16, "hidden_states")
@@ -259,6 +346,15 @@ class MoELayer:
             self._xnorm = torch.empty(max(T, 1), self.H, dtype=torch.bfloat16, device=self.device)
         xnorm = self._kept(self._xnorm)
         y = torch.empty_like(h2) if out is None else self._check_out(out, h2)
+        if residual is not None:
+            self._check_in(residual, torch.bfloat16, "residual")
+            if residual.shape != shape:
+                raise ValueError(f"residual {tuple(residual.shape)} for hidden states of {tuple(shape)}")
+            with self._on_device():
+                L.check(self.lib.mg_moe_block_forward_add(self._h, h2.data_ptr(), residual.data_ptr(), norm_weight.data_ptr(), float(eps), T,
+                                                          self.gate_w.data_ptr(), _ptr(self.bias), self.packed.data_ptr(),
+                                                          xnorm.data_ptr(), ws.data_ptr(), ws.numel(), y.data_ptr(), self._stream()))
+            return y.view(shape)
         with self._on_device():
             L.check(self.lib.mg_moe_block_forward(self._h, h2.data_ptr(), norm_weight.data_ptr(), float(eps), T,
                                                   self.gate_w.data_ptr(), _ptr(self.bias), self.packed.data_ptr(),
@@ -557,6 +653,127 @@ class MoELayer:
             L.check(self.lib.mg_shared_ffn_int8(self._h, xq.data_ptr(), x_scale.data_ptr(), T, self.packed.data_ptr(),
                                                 hs.data_ptr(), hq.data_ptr(), sc.data_ptr(), out.data_ptr(), self._stream()))
         return out
+
+    # ------------------------------------------------------------------ low-rank adapters
+    def _plan_buffer(self, rows: int, n_adapters: int) -> torch.Tensor:
+        size = C.c_size_t()
+        L.check(self.lib.mg_adapter_plan_bytes(rows, n_adapters, C.byref(size)))
+        return torch.empty(size.value, dtype=torch.uint8, device=self.device)
+
+    def adapter_plan(self, ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
+        """The rows of a batch sorted by adapter: ids [rows] int32, an id outside [0, n_adapters) for none."""
+        self._check_in(ids, torch.int32, "ids")
+        rows = ids.numel()
+        buf = self._plan_buffer(rows, n_adapters)
+        with self._on_device():
+            L.check(self.lib.mg_adapter_plan(self._h, ids.data_ptr(), rows, n_adapters, buf.data_ptr(), self._stream()))
+        return AdapterPlan(buf, rows, n_adapters)
+
+    def adapter_plan_sorted(self, counts: torch.Tensor, pad_offsets: torch.Tensor, rows: int) -> AdapterPlan:
+        """The plan of expert-sorted rows (permute_plan's counts and pad_offsets, buffers of `rows` rows), an adapter to an expert."""
+        self._check_in(counts, torch.int32, "counts")
+        self._check_in(pad_offsets, torch.int32, "pad_offsets")
+        n = counts.numel()
+        if pad_offsets.numel() != n + 1:
+            raise ValueError(f"counts of {n} and pad_offsets of {pad_offsets.numel()} entries")
+        buf = self._plan_buffer(rows, n)
+        with self._on_device():
+            L.check(self.lib.mg_adapter_plan_sorted(self._h, counts.data_ptr(), pad_offsets.data_ptr(), rows, n, buf.data_ptr(),
+                                                    self._stream()))
+        return AdapterPlan(buf, rows, n)
+
+    def _adapters(self, down: torch.Tensor, up: torch.Tensor, scale) -> L.Adapters:
+        for t, what in ((down, "down"), (up, "up")):
+            if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != self.device:
+                raise ValueError(f"{what}: expected [adapters, rows, cols] bfloat16 on {self.device}, got {tuple(t.shape)} {t.dtype} on "
+                                 f"{t.device}")
+        n, rank, cols = down.shape
+        n_up, n_out, rank_up = up.shape
+        if n_up != n or rank_up != rank:
+            raise ValueError(f"down {tuple(down.shape)} and up {tuple(up.shape)}")
+        (sd, ld, one), (su, lu, one_up) = down.stride(), up.stride()
+        if (cols > 1 and one != 1) or (rank > 1 and one_up != 1):
+            raise ValueError(f"the elements of an adapter's row must be adjacent (strides {down.stride()}, {up.stride()})")
+        factor, d_scale = 1.0, None
+        if isinstance(scale, torch.Tensor):
+            self._check_in(scale, torch.float32, "scale")
+            if scale.numel() != n:
+                raise ValueError(f"{scale.numel()} scales for {n} adapters")
+            d_scale = scale.data_ptr()
+        else:
+            factor = float(scale)
+        # torch leaves the strides of single rows open
+        return L.Adapters(C.sizeof(L.Adapters), n, rank, factor, cols, n_out, down.data_ptr(), sd,
+                          ld if rank > 1 else (cols + 7) // 8 * 8, up.data_ptr(), su, lu if n_out > 1 else (rank + 7) // 8 * 8, d_scale)
+
+    def _adapter_plan_of(self, who, rows: int, n_adapters: int):
+        """ids or a plan -> the two pointers of the call (what the ids lie in is the caller's)."""
+        if isinstance(who, AdapterPlan):
+            if who.rows != rows or who.n_adapters != n_adapters or who.buf.device != self.device:
+                raise ValueError(f"plan of {who.rows} rows and {who.n_adapters} adapters on {who.buf.device} for {rows} and {n_adapters}")
+            return who
+        self._check_in(who, torch.int32, "ids")
+        if who.numel() != rows:
+            raise ValueError(f"{who.numel()} ids for {rows} rows")
+        return who if rows <= L.ADAPTER_DIRECT else self.adapter_plan(who, n_adapters)
+
+    def _rank_rows(self, rows: int, rank: int) -> torch.Tensor:
+        n = C.c_int32()
+        L.check(self.lib.mg_adapter_rank_stride(rank, C.byref(n)))
+        return torch.empty(rows, n.value, dtype=torch.bfloat16, device=self.device)
+
+    def adapter_add(self, y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, who, scale=1.0,
+                    out: Optional[torch.Tensor] = None, keep: bool = False):
+        """out[t] = y[t] + scale[g] * (x[t] . down[g]^T) . up[g]^T, g being row t's adapter; out[t] = y[t] for a row without one.
+        x [rows, cols] and y [rows, n_out], down [adapters, rank, cols] and up [adapters, n_out, rank], bf16 with rows on 16-byte
+        boundaries (views will do); rank at most 128, a lower one filled up with zeros.  who: int32 ids [rows], outside [0, adapters)
+        for none, or the plan made of them (adapter_plan, adapter_plan_sorted), once for all of a batch's projections.  scale: a number or
+        fp32 [adapters].  out may be y, and overlaps nothing otherwise.  With keep also the rows between the two products, bf16,
+        for adapter_grad: (out, s).  Any layer serves."""
+        n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
+        ad = self._adapters(down, up, scale)
+        if cols != ad.cols:
+            raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
+        ny, n_out, ldy = self._rows_of(y, torch.bfloat16, "y")
+        if (ny, n_out) != (n, ad.n_out):
+            raise ValueError(f"y {tuple(y.shape)}, expected {(n, ad.n_out)}")
+        who = self._adapter_plan_of(who, n, ad.n_adapters)
+        ids, plan = (None, who.buf) if isinstance(who, AdapterPlan) else (who, None)
+        out, ldo = self._out_rows(out, n, n_out, "out")
+        s = self._rank_rows(n, ad.rank) if keep else None
+        with self._on_device():
+            L.check(self.lib.mg_adapter_add(self._h, C.byref(ad), x.data_ptr(), ldx, y.data_ptr(), ldy, n, _ptr(ids), _ptr(plan),
+                                            out.data_ptr(), ldo, _ptr(s), self._stream()))
+        return (out, s) if keep else out
+
+    def adapter_grad(self, grad_out: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, who, scale, s: torch.Tensor,
+                     need_x: bool = True, need_down: bool = True, need_up: bool = True):
+        """Gradients of adapter_add -> (grad_x, grad_down, grad_up), bf16, None for what is not needed; s is what adapter_add kept.
+        grad_x is zero in rows without an adapter, the others in adapters without rows.  The gradient of y is grad_out itself."""
+        n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
+        ad = self._adapters(down, up, scale)
+        if cols != ad.cols:
+            raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
+        ng, n_out, ldg = self._rows_of(grad_out, torch.bfloat16, "grad_out")
+        if (ng, n_out) != (n, ad.n_out):
+            raise ValueError(f"grad_out {tuple(grad_out.shape)}, expected {(n, ad.n_out)}")
+        if isinstance(who, torch.Tensor):
+            self._check_in(who, torch.int32, "ids")
+            if who.numel() != n:
+                raise ValueError(f"{who.numel()} ids for {n} rows")
+            who = self.adapter_plan(who, ad.n_adapters)
+        who = self._adapter_plan_of(who, n, ad.n_adapters)
+        gs = self._rank_rows(n, ad.rank)
+        self._check_rows(s, torch.bfloat16, n, gs.shape[1], "s")
+        if not (need_x or need_down or need_up):
+            return None, None, None
+        gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
+        gdown = torch.empty(down.shape, dtype=torch.bfloat16, device=self.device) if need_down else None
+        gup = torch.empty(up.shape, dtype=torch.bfloat16, device=self.device) if need_up else None
+        with self._on_device():
+            L.check(self.lib.mg_adapter_grad(self._h, C.byref(ad), grad_out.data_ptr(), ldg, x.data_ptr(), ldx, n, who.buf.data_ptr(),
+                                             s.data_ptr(), gs.data_ptr(), _ptr(gx), ldgx, _ptr(gdown), _ptr(gup), self._stream()))
+        return gx, gdown, gup
 
     @contextlib.contextmanager
     def job_counters(self, buf: torch.Tensor):

@@ -40,6 +40,16 @@ class LayerDesc(C.Structure):
                 ("ep_rank", C.c_int32), ("ep_size", C.c_int32)]
 
 
+ADAPTER_MAX, ADAPTER_DIRECT = 1024, 256
+
+
+class Adapters(C.Structure):
+    _fields_ = [("struct_bytes", C.c_int32), ("n_adapters", C.c_int32), ("rank", C.c_int32), ("factor", C.c_float),
+                ("cols", C.c_int64), ("n_out", C.c_int64),
+                ("d_down", C.c_void_p), ("down_stride", C.c_int64), ("ld_down", C.c_int64),
+                ("d_up", C.c_void_p), ("up_stride", C.c_int64), ("ld_up", C.c_int64), ("d_scale", C.c_void_p)]
+
+
 _vp, _i64, _i32, _sz = C.c_void_p, C.c_int64, C.c_int32, C.c_size_t
 _P = C.POINTER
 
@@ -111,6 +121,17 @@ SIGNATURES = {
     "mg_ep_combine": [_vp, _P(_vp), _vp, _vp, _vp, _vp, _i64, _vp, _vp],
     "mg_rmsnorm": [_vp, _vp, _vp, C.c_float, _i64, _vp, _vp],
     "mg_moe_block_forward": [_vp, _vp, _vp, C.c_float, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
+    "mg_moe_block_forward_add": [_vp, _vp, _vp, _vp, C.c_float, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp],
+    "mg_add_rmsnorm": [_vp, _vp, _i64, _vp, _i64, _vp, C.c_float, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
+    "mg_add_rmsnorm_int8": [_vp, _vp, _i64, _vp, _i64, _vp, C.c_float, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp],
+    "mg_add_rmsnorm_grad_ws_bytes": [_vp, _i64, _i64, _P(_sz)],
+    "mg_add_rmsnorm_grad": [_vp, _vp, _i64, _vp, _i64, _vp, C.c_float, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _sz, _vp],
+    "mg_adapter_rank_stride": [_i32, _P(_i32)],
+    "mg_adapter_plan_bytes": [_i64, _i32, _P(_sz)],
+    "mg_adapter_plan": [_vp, _vp, _i64, _i32, _vp, _vp],
+    "mg_adapter_plan_sorted": [_vp, _vp, _vp, _i64, _i32, _vp, _vp],
+    "mg_adapter_add": [_vp, _P(Adapters), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp],
+    "mg_adapter_grad": [_vp, _P(Adapters), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
     "mg_set_option": [_vp, _i32, _i32],
     "mg_set_stage_timing": [_vp, _i32],
     "mg_stage_times": [_vp, _P(C.c_float), _i32],
