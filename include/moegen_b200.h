@@ -537,15 +537,15 @@ int mg_moe_block_forward(mg_handle h, const void* d_hidden, const void* d_norm_w
                          void* d_xnorm, void* d_workspace, size_t workspace_bytes, void* d_out, void* stream);
 
 /* mg_moe_block_forward_add: mg_moe_block_forward of hidden + residual, the addition that precedes it in the decoder layer
- * (modeling_deepseek_v3.py:1348-1359): h = bf16(hidden + residual), out = h + moe(rmsnorm(h)), h and its normalised rows from
- * one launch (mg_add_rmsnorm).  d_out holds h meanwhile; it may be d_hidden or d_residual.
+ * (modeling_deepseek_v3.py:1348-1359): h = bf16(hidden + residual), out = h + moe(rmsnorm(h)), h and mg_rmsnorm's rows of it from
+ * one launch.  d_out holds h meanwhile; it may be d_hidden or d_residual.
  *
  * The rows of the calls below are bf16, of any length, with columns adjacent and rows ld* elements apart; where lengths, strides
  * and addresses are multiples of 8 elements they are read in 16-byte vectors.  The handle may be any layer's: it gives the
  * device.
  *
- * mg_add_rmsnorm: sum = h = bf16(x + residual), out = mg_rmsnorm's rows of h, bit for bit.  Without a residual (NULL) h is x and d_sum is
- *   not written.  d_sum and d_out may each be d_x or d_residual with its stride, not one another, and overlap nothing otherwise.
+ * mg_add_rmsnorm: sum = h = bf16(x + residual), out = bf16(weight * (h * rstd)), rstd = 1 / sqrt(mean(h^2) + eps): one rounding, where
+ *   mg_rmsnorm has its module's second one before the weight.  Without a residual (NULL) h is x and d_sum is not written.  d_sum and d_out may each be d_x or d_residual with its stride, not one another, and overlap nothing otherwise.
  * mg_add_rmsnorm_int8: the rows v = weight * (h * rstd) in fp32, quantised as mg_quantize_rows_int8 does a row: bytes ldq apart
  *   and one scale.  There is no rounding to bf16 in between.  d_q overlaps nothing.
  * mg_add_rmsnorm_grad: with n = h * rstd, the forward's roundings counting as the identity,

@@ -60,9 +60,40 @@ __device__ __forceinline__ uint4 load_tail(const uint16_t* row, int c, int end) 
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+// BYTES of a row from element c on, into shared memory; what lies at `end` or behind arrives as zeros and is not read.  Rows begin on
+// 16-byte boundaries.
+template <int BYTES>
+__device__ __forceinline__ void copy_row(uint32_t to, const uint16_t* row, int c, int end) {
+  const int have = min(max(2 * (end - c), 0), BYTES);
+  const uint16_t* from = have > 0 ? row + c : row;          // an address inside the row for a copy of nothing
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
+  else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
+}
+// BYTES of a row, all of them there
+template <int BYTES>
+__device__ __forceinline__ void copy_whole(uint32_t to, const uint16_t* from) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -70,8 +101,6 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 struct AdapterArgs {
   const uint16_t* x;          // rows of the first product, K elements
@@ -97,18 +126,34 @@ struct AdapterArgs {
 
 // NT: n tiles of a warp in the first product, NG: groups of warps over the rank.  BACK: the gradient's two products, whose adapters
 // are transposed.
+template <int NT, int NG>
+struct AdapterCfg {
+  static constexpr int RP = NT * NG * 8;                       // the rank, filled up
+  static constexpr int V1 = 8 + NT, V2 = 8 + RP / 8;           // 16-byte pieces of a thread and a step: rows and adapters, in either product
+  static constexpr int BLOCKS = NT >= 8 ? 1 : 2;               // per SM
+  static constexpr int S1 = NT >= 8 ? 3 : 2, S2 = RP == 64 ? 3 : 2;        // steps on their way
+  static constexpr int PIECES = S1 * V1 > S2 * V2 ? S1 * V1 : S2 * V2;
+  static constexpr size_t RING = static_cast<size_t>(PIECES) * kAdapterThreads * 16;
+  static constexpr size_t SMEM = RING + kAdapterTile * RP * 2;
+  static_assert(8 / NG * kAdapterTile * RP * 4 <= RING && BLOCKS * (SMEM + 2048) <= 227 * 1024, "shared memory");
+};
+
 template <int NT, int NG, bool BACK>
-__global__ void __launch_bounds__(kAdapterThreads, NT >= 8 ? 1 : 2) adapter_kernel(const AdapterArgs a) {
-  constexpr int RP = NT * NG * 8, KS = RP / 16;
-  constexpr int UNROLL = NT == 2 ? 4 : NT == 4 ? 2 : 1;
+__global__ void __launch_bounds__(kAdapterThreads, AdapterCfg<NT, NG>::BLOCKS) adapter_kernel(const AdapterArgs a) {
+  using C = AdapterCfg<NT, NG>;
+  constexpr int RP = C::RP, KS = RP / 16, KGS = 8 / NG, MT = kAdapterTile / 16;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem);                                   // [groups over K][rows][RP]
-  uint4* frag = reinterpret_cast<uint4*>(smem + 1024 / NG * RP);                 // s: [m tile][k step][lane]
+  float* red = reinterpret_cast<float*>(smem);                                   // between the products: [groups over K][rows][RP]
+  uint4* frag = reinterpret_cast<uint4*>(smem + C::RING);                        // s: [m tile][k step][lane]
   __shared__ int s_rows[kAdapterTile];
   __shared__ int s_before[kAdapterThreads / 32], s_first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, q = lane & 3;
   const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / cs;
+  // A thread copies what it reads itself: piece j of a stage of V lies beside the other threads' piece j, and it waits for its own copies
+  // only.
+  const uint32_t ring = smem_u32(smem) + tid * 16;
+  auto piece = [&](int j) { return ring + static_cast<uint32_t>(j) * (kAdapterThreads * 16); };
   int g, live, len;
   if (a.tiles != nullptr) {
     const int4 t = a.tiles[tile];
@@ -139,210 +184,280 @@ __global__ void __launch_bounds__(kAdapterThreads, NT >= 8 ? 1 : 2) adapter_kern
     __syncthreads();
   }
   const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
+  const int live_mts = (live + 15) / 16;
 
   if (live > 0) {
-    const uint16_t* w1 = a.w1 + g * a.g1;
-    const int rgs = live > 32 ? 2 : 1, kgs = 8 / (rgs * NG);
-    const int ng = warp % NG, rg = (warp / NG) % rgs, kg = warp / (NG * rgs);
-    const bool both = live - rg * 32 > 16;                                        // the second m tile holds a row
-    const uint16_t* xp[2][2];
+    const int ng = warp % NG, kg = warp / NG;
+    const uint16_t* w1 = a.w1 + g * a.g1 + (BACK ? 0 : static_cast<int64_t>(ng * NT * 8 + i) * a.ld1);
+    const uint16_t* xp[MT][2];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) xp[m][hf] = a.x + static_cast<int64_t>(s_rows[min(rg * 32 + m * 16 + hf * 8 + i, live - 1)]) * a.ldx;
-    float acc[2][NT][4];
+      for (int hf = 0; hf < 2; ++hf) xp[m][hf] = a.x + static_cast<int64_t>(s_rows[min(m * 16 + hf * 8 + i, live - 1)]) * a.ldx;
+    float acc[MT][NT][4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[m][t][e] = 0.f;
     const int slices = (a.K + 31) / 32, per = (slices + cs - 1) / cs;
     const int lo = cr * per, hi = min(slices, lo + per);
-    for (int sl = lo + kg; sl < hi; sl += kgs * UNROLL) {
-      uint4 av[UNROLL][2][2];
-      uint32_t bv[UNROLL][NT * 4];
+    const bool filled = a.rank == RP;
+    auto fetch = [&](int stage, int sl) {
+      const int c = sl * 32 + 8 * q;
+      if (sl < hi && filled && sl * 32 + 32 <= a.K) {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int c = (sl + u * kgs) * 32 + 8 * q, end = sl + u * kgs < hi ? a.K : 0;
-        if (c + 8 <= end) {
+        for (int m = 0; m < MT; ++m)
+          if (m < live_mts)
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            av[u][0][hf] = ld_once(xp[0][hf] + c);
-            if (both) av[u][1][hf] = ld_once(xp[1][hf] + c);
-          }
-        } else {
+            for (int hf = 0; hf < 2; ++hf) copy_whole<16>(piece(stage * C::V1 + m * 2 + hf), xp[m][hf] + c);
+        const uint16_t* w = BACK ? w1 + c * a.ld1 + ng * NT * 8 + i * NT : w1 + c;
+        const int64_t next = BACK ? a.ld1 : 8 * a.ld1;
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            av[u][0][hf] = load_tail(xp[0][hf], c, end);
-            av[u][1][hf] = load_tail(xp[1][hf], c, end);
-          }
+        for (int r = 0; r < (BACK ? 8 : NT); ++r, w += next) {
+          if (!BACK) copy_whole<16>(piece(stage * C::V1 + 8 + r), w);
+          else copy_whole<NT * 2>(piece(stage * C::V1 + 8 + r * NT / 8) + r * NT % 8 * 2, w);
         }
+      } else if (sl < hi) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (m < live_mts)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V1 + m * 2 + hf), xp[m][hf], c, a.K);
         if (!BACK) {
-          // four words of each of NT rows of w1: the n tiles' row i
+          // eight elements of each of NT rows of w1: row i of the n tiles
 #pragma unroll
           for (int t = 0; t < NT; ++t)
-            load_words<4>(w1 + static_cast<int64_t>(min((ng * NT + t) * 8 + i, a.rank - 1)) * a.ld1, c, end, &bv[u][t * 4]);
+            copy_row<16>(piece(stage * C::V1 + 8 + t), (ng * NT + t) * 8 + i < a.rank ? w1 + t * 8 * a.ld1 : a.w1, c,
+                         (ng * NT + t) * 8 + i < a.rank ? a.K : 0);
         } else {
           // NT elements of each of eight rows of w1: element i * NT + t is row i of n tile t
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            load_words<NT / 2>(w1 + static_cast<int64_t>(min(c + r, a.K - 1)) * a.ld1, ng * NT * 8 + i * NT, c + r < end ? a.rank : 0,
-                               &bv[u][r * (NT / 2)]);
+            copy_row<NT * 2>(piece(stage * C::V1 + 8 + r * NT / 8) + r * NT % 8 * 2, w1 + static_cast<int64_t>(min(c + r, a.K - 1)) * a.ld1,
+                             ng * NT * 8 + i * NT, c + r < a.K ? a.rank : 0);
         }
       }
+      copies_commit();
+    };
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
+    for (int k = 0; k < C::S1 - 1; ++k) fetch(k, lo + kg + k * KGS);
+    int stage = 0;
+    for (int sl = lo + kg; sl < hi; sl += KGS) {
+      fetch(stage == 0 ? C::S1 - 1 : stage - 1, sl + (C::S1 - 1) * KGS);
+      copies_wait<C::S1 - 1>();
+      uint32_t bv[NT * 4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const uint4 v = ld_shared(piece(stage * C::V1 + 8 + t));
+        bv[4 * t] = v.x; bv[4 * t + 1] = v.y; bv[4 * t + 2] = v.z; bv[4 * t + 3] = v.w;
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m >= live_mts) break;
+        const uint4 u0 = ld_shared(piece(stage * C::V1 + m * 2)), u1 = ld_shared(piece(stage * C::V1 + m * 2 + 1));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           uint32_t b[4];
-          if (!BACK) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = bv[u][t * 4 + e];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t r0 = bv[u][2 * e * (NT / 2) + t / 2], r1 = bv[u][(2 * e + 1) * (NT / 2) + t / 2];
-              b[e] = t % 2 ? highs(r0, r1) : lows(r0, r1);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t r0 = bv[BACK ? 2 * e * (NT / 2) + t / 2 : 0], r1 = bv[BACK ? (2 * e + 1) * (NT / 2) + t / 2 : 0];
+            b[e] = !BACK ? bv[t * 4 + e] : t % 2 ? highs(r0, r1) : lows(r0, r1);
           }
-          mma_bf16(acc[0][t], av[u][0][0].x, av[u][0][1].x, av[u][0][0].y, av[u][0][1].y, b[0], b[1]);
-          mma_bf16(acc[0][t], av[u][0][0].z, av[u][0][1].z, av[u][0][0].w, av[u][0][1].w, b[2], b[3]);
-          if (both) {
-            mma_bf16(acc[1][t], av[u][1][0].x, av[u][1][1].x, av[u][1][0].y, av[u][1][1].y, b[0], b[1]);
-            mma_bf16(acc[1][t], av[u][1][0].z, av[u][1][1].z, av[u][1][0].w, av[u][1][1].w, b[2], b[3]);
-          }
+          mma_bf16(acc[m][t], u0.x, u1.x, u0.y, u1.y, b[0], b[1]);
+          mma_bf16(acc[m][t], u0.z, u1.z, u0.w, u1.w, b[2], b[3]);
         }
       }
+      if (++stage == C::S1) stage = 0;
     }
-    const int rows = rgs * 32;
+    copies_wait<0>();
+    __syncthreads();                                  // the ring is free: the warps' sums go there
+    const int rows = live_mts * 16;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < MT; ++m) {
+      if (m >= live_mts) break;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int n = 2 * q + (e & 1);
           const int r = ng * NT * 8 + (BACK ? n * NT + t : t * 8 + n);
-          red[(kg * rows + rg * 32 + m * 16 + (e >> 1) * 8 + i) * RP + r] = acc[m][t][e];
+          red[(kg * rows + m * 16 + (e >> 1) * 8 + i) * RP + r] = acc[m][t][e];
         }
+    }
     __syncthreads();
     // The sums of this block over its warps, then over the blocks of the cluster, always in the same order; the columns behind the rank
     // and the rows behind the tile's are zeros.
-    const int mts = (live + 15) / 16;
-    if (cs > 1) {
-      for (int e = tid; e < mts * 16 * RP; e += kAdapterThreads) {
-        float v = 0.f;
-        for (int k = 0; k < kgs; ++k) v += red[k * rows * RP + e];
-        red[e] = v;
+    const float4* parts = reinterpret_cast<const float4*>(red);
+    const int quads = rows * RP / 4;
+    auto block_sum = [&](int p) {
+      float4 v = parts[p];
+#pragma unroll
+      for (int k = 1; k < KGS; ++k) {
+        const float4 u = parts[k * quads + p];
+        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
       }
+      return v;
+    };
+    if (cs > 1) {
+      for (int p = tid; p < quads; p += kAdapterThreads) reinterpret_cast<float4*>(red)[p] = block_sum(p);
       cluster_sync_all();
     }
-    for (int p = tid; p < mts * 16 * RP / 2; p += kAdapterThreads) {
-      const int row = 2 * p / RP, r = 2 * p % RP;
-      float v[2] = {0.f, 0.f};
+    for (int p = tid; p < quads; p += kAdapterThreads) {
+      const int row = 4 * p / RP, r = 4 * p % RP;
+      float4 u;
       if (cs > 1) {
-        const uint32_t at = smem_u32(red + 2 * p);
-        for (int c = 0; c < cs; ++c) {
-          const uint32_t there = map_to_cta(at, c);
-          v[0] += ld_cluster_f32(there);
-          v[1] += ld_cluster_f32(there + 4);
-        }
-      } else {
-        for (int k = 0; k < kgs; ++k) {
-          v[0] += red[k * rows * RP + 2 * p];
-          v[1] += red[k * rows * RP + 2 * p + 1];
-        }
-      }
+        const uint32_t at = smem_u32(parts + p);
+        float4 there[8];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) v[e] = row < live && r + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(&b);
-      // which thread's fragment holds (row, r): see the loads of w2 below
-      const int fi = row & 7, hf = (row >> 3) & 1, in = RP == 16 ? r : r & 31;
-      const int fq = RP == 16 ? in >> 2 : in >> 3, part = (in >> 1) & 1;
-      const int ks = RP == 16 ? 0 : (r >> 5) * 2 + ((in >> 2) & 1);
-      reinterpret_cast<uint32_t*>(frag + ((row >> 4) * KS + ks) * 32 + fi * 4 + fq)[part * 2 + hf] = word;
-      if (a.s != nullptr && cr == 0 && row < len) *reinterpret_cast<uint32_t*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + r) = word;
+        for (int c = 0; c < 8; ++c)
+          if (c < cs) there[c] = ld_cluster_f32x4(map_to_cta(at, c));
+        u = there[0];
+#pragma unroll
+        for (int c = 1; c < 8; ++c)
+          if (c < cs) { u.x += there[c].x; u.y += there[c].y; u.z += there[c].z; u.w += there[c].w; }
+      } else {
+        u = block_sum(p);
+      }
+      float v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = row < live && r + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
+      const __nv_bfloat162 b0 = __floats2bfloat162_rn(v[0], v[1]), b1 = __floats2bfloat162_rn(v[2], v[3]);
+      const uint2 words = make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1));
+      // the fragments that hold (row, r) to (row, r + 3): see the loads of w2 below
+      const int fi = row & 7, hf = (row >> 3) & 1, fq = RP == 16 ? r >> 2 : (r & 31) >> 3;
+      const int ks = RP == 16 ? 0 : (r >> 5) * 2 + ((r >> 2) & 1);
+      uint32_t* f = reinterpret_cast<uint32_t*>(frag + ((row >> 4) * KS + ks) * 32 + fi * 4 + fq);
+      f[hf] = words.x;
+      f[2 + hf] = words.y;
+      if (a.s != nullptr && cr == 0 && row < len) *reinterpret_cast<uint2*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + r) = words;
     }
-    if (cs > 1) cluster_arrive();                    // done with the other blocks' shared memory
-    __syncthreads();
+    if (cs > 1) cluster_sync_all();                   // the ring is free again, here and in the blocks that have read it
+    else __syncthreads();
   }
-  if (a.s != nullptr && cr == 0) {                   // rows without an adapter
-    const int from = (live + 15) / 16 * 16;
+  if (a.s != nullptr && cr == 0) {                    // rows without an adapter
+    const int from = live_mts * 16;
     for (int p = tid; p < (len - from) * RP / 2; p += kAdapterThreads)
       *reinterpret_cast<uint32_t*>(a.s + static_cast<int64_t>(s_rows[from + 2 * p / RP]) * RP + 2 * p % RP) = 0u;
   }
 
-  const int units = (a.N + 31) / 32, each = (units + cs - 1) / cs;
-  const int mts = (len + 15) / 16, live_mts = (live + 15) / 16;
+  const int units = (a.N + 31) / 32, each = (units + cs - 1) / cs, last = min(units, (cr + 1) * each);
+  const int mts = (len + 15) / 16;
   const bool in_place = a.y == a.out && a.ldy == a.ldo;
-  const uint16_t* w2 = g >= 0 ? a.w2 + g * a.g2 : nullptr;
-  for (int unit = cr * each + warp; unit < min(units, (cr + 1) * each); unit += kAdapterThreads / 32) {
-    const int c0 = unit * 32;
-    uint32_t b[KS][4][2];
-    if (live > 0) {
-      if (!BACK) {
+  const uint16_t* w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
+  const uint16_t* yp[MT][2];
+  uint16_t* op[MT][2];                                // nullptr: not written
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint16_t* row = w2 + static_cast<int64_t>(min(c0 + 4 * i + t, a.N - 1)) * a.ld2;
-          if (RP == 16) {
-            load_words<2>(row, 4 * q, a.rank, b[0][t]);
-          } else {
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int p = 0; p < RP / 32; ++p) {
-              uint32_t v[4];
-              load_words<4>(row, 32 * p + 8 * q, a.rank, v);
-              b[(2 * p) % KS][t][0] = v[0]; b[(2 * p) % KS][t][1] = v[1];
-              b[(2 * p + 1) % KS][t][0] = v[2]; b[(2 * p + 1) % KS][t][1] = v[3];
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = m * 16 + hf * 8 + i;
+      const int64_t row = s_rows[min(r, len - 1)];
+      yp[m][hf] = a.y + row * a.ldy;
+      op[m][hf] = r < len && !(in_place && r >= live) ? a.out + row * a.ldo : nullptr;
+    }
+  const bool filled = a.rank == RP;
+  auto fetch = [&](int stage, int unit) {
+    const int c0 = unit * 32, c = c0 + 8 * q;
+    if (unit < last && filled && c0 + 32 <= a.N) {
+      if (a.y != nullptr)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (m < mts)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) copy_whole<16>(piece(stage * C::V2 + m * 2 + hf), yp[m][hf] + c);
+      if (live > 0 && !BACK) {
+        const uint16_t* w = w2 + (c0 + 4 * i) * a.ld2 + (RP == 16 ? 4 : 8) * q;
+#pragma unroll
+        for (int t = 0; t < 4; ++t, w += a.ld2) {
+          if (RP == 16) copy_whole<8>(piece(stage * C::V2 + 8 + t / 2) + t % 2 * 8, w);
+          else
+#pragma unroll
+            for (int p = 0; p < RP / 32; ++p) copy_whole<16>(piece(stage * C::V2 + 8 + t * (RP / 32) + p), w + 32 * p);
+        }
+      } else if (live > 0) {
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          const uint16_t* w = w2 + (RP == 16 ? 4 * q : k * 16 + 8 * q) * a.ld2 + c0 + 4 * i;
+#pragma unroll
+          for (int e = 0; e < (RP == 16 ? 4 : 8); ++e, w += a.ld2) copy_whole<8>(piece(stage * C::V2 + 8 + k * 2 + e / 2) + e % 2 * 8, w);
+        }
+      }
+    } else if (unit < last) {
+      if (a.y != nullptr)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (m < mts)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V2 + m * 2 + hf), yp[m][hf], c, a.N);
+      if (live > 0) {
+        if (!BACK) {
+          // of row 4 i + t of the unit's 32 rows of w2, n tile t's row i: the elements of this thread's fragments
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int col = c0 + 4 * i + t, end = col < a.N ? a.rank : 0;
+            const uint16_t* row = w2 + (col < a.N ? col : 0) * a.ld2;
+            if (RP == 16) {
+              copy_row<8>(piece(stage * C::V2 + 8 + t / 2) + t % 2 * 8, row, 4 * q, end);
+            } else {
+#pragma unroll
+              for (int p = 0; p < RP / 32; ++p) copy_row<16>(piece(stage * C::V2 + 8 + t * (RP / 32) + p), row, 32 * p + 8 * q, end);
             }
           }
-        }
-      } else {
+        } else {
+          // four columns, of n tiles 0 to 3, of the rows of w2 that this thread's fragments hold
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int r0 = RP == 16 ? 4 * q : (ks >> 1) * 32 + 8 * q + (ks & 1) * 4;
-          uint32_t v[4][2];
+          for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            load_words<2>(w2 + static_cast<int64_t>(min(r0 + e, a.rank - 1)) * a.ld2, c0 + 4 * i, r0 + e < a.rank ? a.N : 0, v[e]);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-              b[ks][t][p] = t % 2 ? highs(v[2 * p][t / 2], v[2 * p + 1][t / 2]) : lows(v[2 * p][t / 2], v[2 * p + 1][t / 2]);
+            for (int e = 0; e < 4; ++e) {
+              const int r = (RP == 16 ? 4 * q : (ks >> 1) * 32 + 8 * q + (ks & 1) * 4) + e;
+              copy_row<8>(piece(stage * C::V2 + 8 + ks * 2 + e / 2) + e % 2 * 8, w2 + (r < a.rank ? r : 0) * a.ld2, c0 + 4 * i,
+                          r < a.rank ? a.N : 0);
+            }
         }
       }
     }
-    const int c = c0 + 8 * q;
-    for (int m = 0; m < mts; ++m) {
+    copies_commit();
+  };
+  const int unit0 = cr * each + warp;
+#pragma unroll
+  for (int k = 0; k < C::S2 - 1; ++k) fetch(k, unit0 + k * (kAdapterThreads / 32));
+  int stage = 0;
+  for (int unit = unit0; unit < last; unit += kAdapterThreads / 32) {
+    fetch(stage == 0 ? C::S2 - 1 : stage - 1, unit + (C::S2 - 1) * (kAdapterThreads / 32));
+    copies_wait<C::S2 - 1>();
+    const int c = unit * 32 + 8 * q;
+    uint32_t b[KS][4][2];
+    if (live > 0) {
+      uint32_t v[KS * 8];
+#pragma unroll
+      for (int j = 0; j < KS * 2; ++j) {
+        const uint4 u = ld_shared(piece(stage * C::V2 + 8 + j));
+        v[4 * j] = u.x; v[4 * j + 1] = u.y; v[4 * j + 2] = u.z; v[4 * j + 3] = u.w;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            if (!BACK)
+              b[ks][t][p] = RP == 16 ? v[t * 2 + p] : v[(t * (RP / 32) + ks / 2) * 4 + ks % 2 * 2 + p];
+            else {
+              const uint32_t r0 = v[ks * 8 + p * 4 + t / 2], r1 = v[ks * 8 + p * 4 + 2 + t / 2];
+              b[ks][t][p] = t % 2 ? highs(r0, r1) : lows(r0, r1);
+            }
+          }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m >= mts) break;
       float acc[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-      uint4 base[2];
-      bool there[2];
-      uint16_t* dst[2];
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int r = m * 16 + hf * 8 + i;
-        there[hf] = r < len && c < a.N && !(in_place && r >= live);
-        const int64_t row = s_rows[min(r, len - 1)];
-        dst[hf] = a.out + row * a.ldo;
-        base[hf] = make_uint4(0u, 0u, 0u, 0u);
-        if (a.y != nullptr && there[hf]) {
-          const uint16_t* src = a.y + row * a.ldy;
-          if (c + 8 <= a.N) {
-            base[hf] = ld_row(reinterpret_cast<const uint4*>(src + c));
-          } else {
-            uint32_t* u = &base[hf].x;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (c + e < a.N) u[e >> 1] |= static_cast<uint32_t>(src[c + e]) << (16 * (e & 1));
-          }
-        }
-      }
       if (m < live_mts) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -353,30 +468,31 @@ __global__ void __launch_bounds__(kAdapterThreads, NT >= 8 ? 1 : 2) adapter_kern
       }
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        if (!there[hf]) continue;
-        uint4 v = base[hf];
+        if (op[m][hf] == nullptr || c >= a.N) continue;
+        uint4 v = a.y != nullptr ? ld_shared(piece(stage * C::V2 + m * 2 + hf)) : make_uint4(0u, 0u, 0u, 0u);
         if (m * 16 + hf * 8 + i < live) {
           float o[8];
           unpack8(v, o);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float p = acc[e & 3][hf * 2 + (e >> 2)];                        // column c0 + 4 * (2q + (e >> 2)) + (e & 3)
+            const float p = acc[e & 3][hf * 2 + (e >> 2)];                        // column 4 * (2q + (e >> 2)) + (e & 3) of the unit
             o[e] = BACK ? p : fmaf(scale, p, o[e]);
           }
           v = pack8(o);
         }
+        uint16_t* dst = op[m][hf] + c;
         if (c + 8 <= a.N) {
-          *reinterpret_cast<uint4*>(dst[hf] + c) = v;
+          *reinterpret_cast<uint4*>(dst) = v;
         } else {
           const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (c + e < a.N) dst[hf][c + e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+            if (c + e < a.N) dst[e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
         }
       }
     }
+    if (++stage == C::S2) stage = 0;
   }
-  if (live > 0 && cs > 1) cluster_wait();            // no block leaves while another reads its sums
 }
 
 // ---- gradients of the adapters ---------------------------------------------------------------
@@ -643,8 +759,7 @@ int allow_smem(const Handle* h, K* kernel, size_t smem, bool (&done)[64]) {
 
 template <int NT, int NG, bool BACK>
 int launch_adapter_as(const Handle* h, const AdapterArgs& a, int64_t jobs, int cs, cudaStream_t st) {
-  constexpr int RP = NT * NG * 8;
-  constexpr size_t smem = 1024 / NG * RP + kAdapterTile * RP * 2;
+  constexpr size_t smem = AdapterCfg<NT, NG>::SMEM;
   static bool done[64];
   if (int rc = allow_smem(h, adapter_kernel<NT, NG, BACK>, smem, done)) return rc;
   MG_CUDA(launch_clusters(adapter_kernel<NT, NG, BACK>, jobs, cs, smem, st, a));
@@ -653,10 +768,10 @@ int launch_adapter_as(const Handle* h, const AdapterArgs& a, int64_t jobs, int c
 template <bool BACK>
 int launch_adapter_rank(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   const int64_t jobs = a.tiles != nullptr ? (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile + a.n_adapters + 1 : a.n_rows;
-  // as many blocks to a tile as fill the SMs twice, were all tiles full
+  // as many blocks to a tile as run at once, were all tiles full
   const int64_t full = a.tiles != nullptr ? (a.n_rows + kAdapterTile - 1) / kAdapterTile : a.n_rows;
   int cs = 8;
-  while (cs > 1 && full * cs > 4 * h->sm_count) cs /= 2;
+  while (cs > 1 && full * cs > (a.rank > 32 ? 1 : 2) * h->sm_count) cs /= 2;
   switch (padded_rank(a.rank)) {
     case 16: return launch_adapter_as<2, 1, BACK>(h, a, jobs, cs, st);
     case 32: return launch_adapter_as<4, 1, BACK>(h, a, jobs, cs, st);

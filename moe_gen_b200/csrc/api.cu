@@ -1444,7 +1444,9 @@ int mg_moe_block_forward_add(mg_handle hh, const void* d_hidden, const void* d_r
   MG_REQUIRE(aligned16(d_hidden) && aligned16(d_residual) && aligned16(d_norm_weight) && aligned16(d_xnorm) && aligned16(d_out),
              MG_ERR_SHAPE, "mg_moe_block_forward_add: rows and weight must begin on a 16-byte boundary");
   const int64_t H = h->d.hidden;
-  int rc = mg_add_rmsnorm(hh, d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, stream);
+  MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_moe_block_forward_add: negative eps");
+  int rc = launch_add_norm(d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, nullptr, true,
+                           static_cast<cudaStream_t>(stream));
   if (rc != MG_OK) return rc;
   rc = moe_forward_impl(hh, d_xnorm, T, d_gate_w, d_bias, d_packed, d_ws, ws_bytes, d_out, d_out, stream);
   if (rc == MG_OK) h->last_launches += 1;
@@ -1477,7 +1479,7 @@ int mg_add_rmsnorm(mg_handle hh, const void* d_x, int64_t ldx, const void* d_res
   if (rc != MG_OK) return rc;
   MG_REQUIRE(n_rows == 0 || ((d_out != d_x || ldo == ldx) && (d_out != d_residual || ldo == ldr)), MG_ERR_CONFIG,
              "mg_add_rmsnorm: the normalised rows lie otherwise than those of the input that they replace");
-  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_out, ldo, nullptr,
+  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_out, ldo, nullptr, false,
                          static_cast<cudaStream_t>(stream));
 }
 
@@ -1490,7 +1492,7 @@ int mg_add_rmsnorm_int8(mg_handle hh, const void* d_x, int64_t ldx, const void* 
   if (rc != MG_OK) return rc;
   MG_REQUIRE(n_rows == 0 || d_scale, MG_ERR_NULL, "mg_add_rmsnorm_int8: null pointer");
   MG_REQUIRE(n_rows == 0 || (d_q != d_x && d_q != d_residual), MG_ERR_CONFIG, "mg_add_rmsnorm_int8: the bytes need a buffer of their own");
-  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_q, ldq, d_scale,
+  return launch_add_norm(d_x, ldx, d_residual, ldr, d_weight, eps, n_rows, cols, d_sum, lds, d_q, ldq, d_scale, false,
                          static_cast<cudaStream_t>(stream));
 }
 

@@ -269,7 +269,7 @@ int launch_int8_matmul(const Handle* h, const void* xq, int64_t ldx, const float
 
 // norm with the residual's addition, and its gradient (norm.cu) ------------------------------
 int launch_add_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, float eps, int64_t n, int64_t cols,
-                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, cudaStream_t st);
+                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, bool as_module, cudaStream_t st);
 int64_t norm_grad_max_cols();
 size_t norm_grad_ws_bytes(const Handle* h, int64_t n, int64_t cols);
 int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* hrows, int64_t ldh, const void* w, float eps, int64_t n,

@@ -1,8 +1,8 @@
 // The residual's addition and the RMS norm behind it in one pass, rows out in bf16 or in 8-bit integers, and the gradient.
-//   h = bf16(x + residual), rstd = 1 / sqrt(mean(h^2) + eps), y = bf16(w * bf16(h * rstd))         (mg_rmsnorm's y of h)
-//   8 bits: v = w * (h * rstd) in fp32, m = max(max|v|, 2^-100), scale = m / 127, q = v * (127 / m) to the nearest, ties to even
-// h is rounded because it is stored so, and the norm is of what is stored.  y has the two roundings of the reference's module;
-// the 8-bit form has none before its own.
+//   h = bf16(x + residual), rstd = 1 / sqrt(mean(h^2) + eps), v = w * (h * rstd) in fp32, y = bf16(v)
+//   8 bits: m = max(max|v|, 2^-100), scale = m / 127, q = v * (127 / m) to the nearest, ties to even
+// h is rounded because it is stored so, and the norm is of what is stored; v is rounded once.  In front of the block
+// y = bf16(w * bf16(h * rstd)), mg_rmsnorm's bits, whose module the block's parity is with.
 #include "tc.cuh"
 
 namespace mg {
@@ -12,6 +12,7 @@ namespace {
 constexpr int kNormLanes = 256;          // lanes over which a row's squares are summed, whatever the kernel (as in rmsnorm_kernel)
 constexpr int64_t kNormWarpRows = 2048;  // fewer rows than this have a block each, and its latency
 
+enum NormOut { NORM_BF16, NORM_AS_MODULE, NORM_INT8 };
 struct NormArgs {
   const uint16_t* x;
   int64_t ldx;
@@ -49,21 +50,26 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 __device__ __forceinline__ float rstd_of(float sum, int cols, float eps) { return 1.0f / sqrtf(sum / static_cast<float>(cols) + eps); }
-// w * (h * rstd) of eight elements
-__device__ __forceinline__ void normal8(const uint4& h, const uint4& w, float rstd, float* f) {
-  float g[8];
-  unpack8(h, f);
-  unpack8(w, g);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(g[i], __fmul_rn(f[i], rstd));
+template <int OUT>
+__device__ __forceinline__ float normal(float h, float w, float rstd) {
+  const float n = __fmul_rn(h, rstd);
+  return __fmul_rn(w, OUT == NORM_AS_MODULE ? round_bf16(n) : n);
 }
+template <int OUT>
 __device__ __forceinline__ uint4 rounded8(const uint4& h, const uint4& w, float rstd) {
   float f[8], g[8];
   unpack8(h, f);
   unpack8(w, g);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = __fmul_rn(g[i], round_bf16(__fmul_rn(f[i], rstd)));
+  for (int i = 0; i < 8; ++i) f[i] = normal<OUT>(f[i], g[i], rstd);
   return pack8(f);
+}
+__device__ __forceinline__ void normal8(const uint4& h, const uint4& w, float rstd, float* f) {
+  float g[8];
+  unpack8(h, f);
+  unpack8(w, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = normal<NORM_INT8>(f[i], g[i], rstd);
 }
 // |v| as bits, which order as the numbers do; infinities and NaN are larger than any number
 __device__ __forceinline__ uint32_t amax_bits8(uint32_t m, const float* f) {
@@ -91,7 +97,7 @@ __device__ __forceinline__ uint2 bytes8(const float* f, float inv) {
 }
 
 // A block per row of whole 16-byte vectors, which stay in registers between the sum and the output.
-template <int VECS, bool INT8>
+template <int VECS, int OUT>
 __global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) {
   __shared__ float s_sum[kNormLanes / 32];
   __shared__ uint32_t s_max[kNormLanes / 32];
@@ -137,12 +143,12 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) 
 #pragma unroll
   for (int i = 0; i < kNormLanes / 32; ++i) sum += s_sum[i];
   const float rstd = rstd_of(sum, a.cols, a.eps);
-  if (!INT8) {
+  if (OUT != NORM_INT8) {
     uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ldo);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = threadIdx.x + i * kNormLanes;
-      if (v < vecs) y[v] = rounded8(keep[i], wk[i], rstd);
+      if (v < vecs) y[v] = rounded8<OUT>(keep[i], wk[i], rstd);
     }
     return;
   }
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) 
 }
 
 // A warp per row, for many short rows.  Its lanes hold what lanes 32 apart would hold in a block, summed in the same order.
-template <int VECS, bool INT8>
+template <int VECS, int OUT>
 __global__ void __launch_bounds__(256) add_norm_short_kernel(const NormArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -206,12 +212,12 @@ __global__ void __launch_bounds__(256) add_norm_short_kernel(const NormArgs a) {
 #pragma unroll
   for (int i = 0; i < VECS; ++i) sum += warp_sum(squares8(keep[i], 0.f));
   const float rstd = rstd_of(sum, a.cols, a.eps);
-  if (!INT8) {
+  if (OUT != NORM_INT8) {
     uint4* y = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ldo);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = lane + i * 32;
-      if (v < vecs) y[v] = rounded8(keep[i], __ldg(w + v), rstd);
+      if (v < vecs) y[v] = rounded8<OUT>(keep[i], __ldg(w + v), rstd);
     }
     return;
   }
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(256) add_norm_short_kernel(const NormArgs a) {
 
 // Rows of any length, alignment and stride, element by element.  What is not kept is read again: h, where it was written, by
 // the thread that wrote it, so that x or the residual may be where it goes.
-template <bool INT8>
+template <int OUT>
 __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs a) {
   __shared__ float s_sum[kNormLanes / 32];
   __shared__ uint32_t s_max[kNormLanes / 32];
@@ -271,13 +277,13 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs
   uint32_t m = 0;
   for (int64_t v = threadIdx.x; v * 8 < a.cols; v += kNormLanes)
     for (int c = static_cast<int>(v) * 8; c < a.cols && c < static_cast<int>(v) * 8 + 8; ++c) {
-      const float n = __fmul_rn(f32(h[c]), rstd), w = f32(a.w[c]);
-      if (INT8)
-        m = max(m, __float_as_uint(__fmul_rn(w, n)) & 0x7FFFFFFFu);
+      const float v = normal<OUT>(f32(h[c]), f32(a.w[c]), rstd);
+      if (OUT == NORM_INT8)
+        m = max(m, __float_as_uint(v) & 0x7FFFFFFFu);
       else
-        static_cast<uint16_t*>(a.out)[row * a.ldo + c] = __bfloat16_as_ushort(__float2bfloat16_rn(__fmul_rn(w, round_bf16(n))));
+        static_cast<uint16_t*>(a.out)[row * a.ldo + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
     }
-  if (!INT8) return;
+  if (OUT != NORM_INT8) return;
   m = __reduce_max_sync(0xFFFFFFFFu, m);
   if ((threadIdx.x & 31) == 0) s_max[warp] = m;
   __syncthreads();
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs
   for (int64_t v = threadIdx.x; v * 8 < a.cols; v += kNormLanes)
     for (int c = static_cast<int>(v) * 8; c < a.cols && c < static_cast<int>(v) * 8 + 8; ++c)
       static_cast<uint8_t*>(a.out)[row * a.ldo + c] =
-          inv == 0.0f ? 0 : static_cast<uint8_t>(byte_of(__fmul_rn(f32(a.w[c]), __fmul_rn(f32(h[c]), rstd)), inv));
+          inv == 0.0f ? 0 : static_cast<uint8_t>(byte_of(normal<OUT>(f32(h[c]), f32(a.w[c]), rstd), inv));
   if (threadIdx.x == 0) a.scale[row] = scale;
 }
 
@@ -314,6 +320,9 @@ struct NormGradArgs {
   int lanes;                 // threads to a row
 };
 constexpr int kGradThreads = 1024, kGradMaxCols = 2 * 8 * kGradThreads;      // up to two vectors of a row to a thread
+// rows on their way at once: 48 bytes to a thread, a vector and a row
+template <int VECS>
+constexpr int kGradStages = VECS == 1 ? 4 : 2;
 
 template <bool WIDE>
 __device__ __forceinline__ uint4 load8(const uint16_t* p, int c, int cols) {
@@ -329,86 +338,133 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int c, int cols) {
   return v;
 }
 
+__device__ __forceinline__ void pairs8(const uint4& v, float2* f) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
+}
+__device__ __forceinline__ void copy_vec(uint4* to, const uint16_t* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+
+// WIDE: rows of whole 16-byte vectors, several of them on their way to shared memory at a time.  A thread copies what it reads itself, so
+// that it waits for its own copies only.
 template <int VECS, bool WIDE>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGradArgs a) {
+  constexpr int STAGES = kGradStages<VECS>;
+  extern __shared__ __align__(16) uint4 s_rows[];                // [stage][h, gy, gh][vector][thread]
   __shared__ float2 s_sum[2][kGradThreads / 32];
   const int lanes = a.lanes, sub = threadIdx.x / lanes, t = threadIdx.x - sub * lanes, rows = blockDim.x / lanes;
   const int warp = threadIdx.x >> 5, warps = lanes >> 5;
-  uint4 w[VECS], h[VECS], gy[VECS], gh[VECS];
-  float acc[VECS][8];
-  auto load = [&](int64_t row) {
-    const int cols = row < a.n ? a.cols : 0;
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int c = (t + i * lanes) * 8;
-      h[i] = load8<WIDE>(a.h + row * a.ldh, c, cols);
-      gy[i] = load8<WIDE>(a.gy + row * a.ldgy, c, cols);
-      gh[i] = load8<WIDE>(a.gh + row * a.ldgh, c, a.gh != nullptr ? cols : 0);
-    }
-  };
+  const bool with_h = a.gh != nullptr && a.gx != nullptr;
+  float2 w[VECS][4], acc[VECS][4];
 #pragma unroll
   for (int i = 0; i < VECS; ++i) {
-    w[i] = load8<WIDE>(a.w, (t + i * lanes) * 8, a.cols);
+    pairs8(load8<WIDE>(a.w, (t + i * lanes) * 8, a.cols), w[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
   }
-  int turn = 0;
-  for (int64_t base = static_cast<int64_t>(blockIdx.x) * rows; base < a.n; base += static_cast<int64_t>(gridDim.x) * rows, turn ^= 1) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * rows, first = static_cast<int64_t>(blockIdx.x) * rows;
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  uint4* mine = s_rows + threadIdx.x;
+  auto slot = [&](int stage, int which, int i) { return mine + ((stage * 3 + which) * VECS + i) * blockDim.x; };
+  // the next row to fetch, and this thread's columns of it
+  int64_t ahead = first + sub;
+  const uint16_t *ph = a.h + ahead * a.ldh + t * 8, *pg = a.gy + ahead * a.ldgy + t * 8, *pr = a.gh + ahead * a.ldgh + t * 8;
+  const int64_t sh = step * a.ldh, sg = step * a.ldgy, sr = step * a.ldgh;
+  auto fetch = [&](int stage) {
+    if (ahead < a.n) {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i)
+        if ((t + i * lanes) * 8 < a.cols) {
+          copy_vec(slot(stage, 0, i), ph + i * lanes * 8);
+          copy_vec(slot(stage, 1, i), pg + i * lanes * 8);
+          if (with_h) copy_vec(slot(stage, 2, i), pr + i * lanes * 8);
+        }
+    }
+    ahead += step; ph += sh; pg += sg; pr += sr;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (WIDE)
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+  int turn = 0, stage = 0;
+  for (int64_t base = first; base < a.n; base += step, turn ^= 1) {
     const int64_t row = base + sub;
     const bool live = row < a.n;
-    load(row);
-    float ss = 0.f, sp = 0.f;
+    const int cols = live ? a.cols : 0;
+    if (WIDE) {
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    }
+    auto take = [&](const uint16_t* from, int64_t ld, int which, int i) {
+      const int c = (t + i * lanes) * 8;
+      if (!WIDE) return load8<false>(from + row * ld, c, which == 2 && !with_h ? 0 : cols);
+      return c < cols && (which != 2 || with_h) ? *slot(stage, which, i) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    float2 s2 = make_float2(0.f, 0.f), p2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      float fh[8], fg[8], fw[8];
-      unpack8(h[i], fh);
-      unpack8(gy[i], fg);
-      unpack8(w[i], fw);
+      float2 fh[4], fg[4];
+      pairs8(take(a.h, a.ldh, 0, i), fh);
+      pairs8(take(a.gy, a.ldgy, 1, i), fg);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ss = fmaf(fh[j], fh[j], ss);
-        sp = fmaf(__fmul_rn(fw[j], fg[j]), fh[j], sp);
+      for (int j = 0; j < 4; ++j) {
+        s2 = __ffma2_rn(fh[j], fh[j], s2);
+        p2 = __ffma2_rn(__fmul2_rn(w[i][j], fg[j]), fh[j], p2);
       }
     }
-    ss = warp_sum(ss);
-    sp = warp_sum(sp);
+    float ss = warp_sum(s2.x + s2.y), sp = warp_sum(p2.x + p2.y);
     if (warps > 1) {
       if ((threadIdx.x & 31) == 0) s_sum[turn][warp] = make_float2(ss, sp);
       __syncthreads();               // the other half of s_sum is written in the next turn: no thread is two turns ahead
-      ss = sp = 0.f;
-      for (int i = 0; i < warps; ++i) {
-        const float2 v = s_sum[turn][sub * warps + i];
-        ss += v.x;
-        sp += v.y;
+      const int lane = threadIdx.x & 31;
+      const float2 v = lane < warps ? s_sum[turn][sub * warps + lane] : make_float2(0.f, 0.f);
+      ss = v.x;
+      sp = v.y;
+#pragma unroll
+      for (int o = kGradThreads / 64; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+        sp += __shfl_xor_sync(0xFFFFFFFFu, sp, o);
+      }
+      if (kGradThreads / 32 < 32) {  // lanes behind the last warp's have summed zeros
+        ss = __shfl_sync(0xFFFFFFFFu, ss, 0);
+        sp = __shfl_sync(0xFFFFFFFFu, sp, 0);
       }
     }
-    const float rstd = rstd_of(ss, a.cols, a.eps);
-    const float c2 = __fmul_rn(__fmul_rn(rstd, rstd), sp / static_cast<float>(a.cols));
+    const float rstd = live ? rsqrtf(fmaf(ss, inv_cols, a.eps)) : 0.f;
+    const float2 r2 = make_float2(rstd, rstd);
+    const float c = -rstd * rstd * (sp * inv_cols);
+    const float2 c2 = make_float2(c, c);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int c = (t + i * lanes) * 8;
-      float fh[8], fg[8], fw[8], fr[8];
-      unpack8(h[i], fh);
-      unpack8(gy[i], fg);
-      unpack8(w[i], fw);
-      unpack8(gh[i], fr);
+      float2 fh[4], fg[4], fr[4];
+      pairs8(take(a.h, a.ldh, 0, i), fh);
+      pairs8(take(a.gy, a.ldgy, 1, i), fg);
+      pairs8(take(a.gh, a.ldgh, 2, i), fr);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (live) acc[i][j] = fmaf(fg[j], __fmul_rn(fh[j], rstd), acc[i][j]);
-        fr[j] = fmaf(rstd, fmaf(-fh[j], c2, __fmul_rn(fw[j], fg[j])), fr[j]);
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = __ffma2_rn(fg[j], __fmul2_rn(fh[j], r2), acc[i][j]);
+        fr[j] = __ffma2_rn(r2, __ffma2_rn(fh[j], c2, __fmul2_rn(w[i][j], fg[j])), fr[j]);
       }
       if (a.gx == nullptr || !live) continue;
+      const int at = (t + i * lanes) * 8;
       uint16_t* dst = a.gx + row * a.ldgx;
-      const uint4 v = pack8(fr);
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(fr[j].x, fr[j].y);
+        u[j] = *reinterpret_cast<const uint32_t*>(&v);
+      }
       if (WIDE) {
-        if (c < a.cols) *reinterpret_cast<uint4*>(dst + c) = v;
+        if (at < a.cols) *reinterpret_cast<uint4*>(dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
       } else {
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (c + j < a.cols) dst[c + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+          if (at + j < a.cols) dst[at + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
       }
     }
+    if (++stage == STAGES) stage = 0;
   }
   if (a.parts == nullptr) return;
   float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * rows + sub) * a.cols;
@@ -417,7 +473,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGr
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int c = (t + i * lanes) * 8 + j;
-      if (c < a.cols) part[c] = acc[i][j];
+      if (c < a.cols) part[c] = j & 1 ? acc[i][j >> 1].y : acc[i][j >> 1].x;
     }
 }
 
@@ -442,7 +498,7 @@ NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
   p.lanes = (vecs + 32 * p.vecs - 1) / (32 * p.vecs) * 32;
   p.threads = p.lanes >= 256 ? p.lanes : 256 / p.lanes * p.lanes;
   const int rows = p.threads / p.lanes;
-  const int64_t want = (n + rows - 1) / rows, most = static_cast<int64_t>(h->sm_count) * (kGradThreads / p.threads);
+  const int64_t want = (n + rows - 1) / rows, most = static_cast<int64_t>(h->sm_count) * (p.threads > 512 ? 1 : p.threads > 256 ? 2 : 4);
   p.blocks = static_cast<int>(want < most ? want : most);
   p.shares = p.blocks * rows;
   return p;
@@ -450,32 +506,55 @@ NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
 
 bool on16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
 
-template <bool INT8>
+template <int OUT>
 int launch_add_norm_as(const NormArgs& a, cudaStream_t st) {
   const int vecs = a.cols / 8;
   const bool wide = a.cols % 8 == 0 && on16(a.x, a.ldx) && (a.res == nullptr || (on16(a.res, a.ldr) && on16(a.sum, a.lds))) &&
-                    on16(a.w, 0) && vecs <= 8 * kNormLanes && reinterpret_cast<uintptr_t>(a.out) % (INT8 ? 8 : 16) == 0 && a.ldo % 8 == 0;
+                    on16(a.w, 0) && vecs <= 8 * kNormLanes && reinterpret_cast<uintptr_t>(a.out) % (OUT == NORM_INT8 ? 8 : 16) == 0 && a.ldo % 8 == 0;
   const unsigned rows = static_cast<unsigned>(a.n), eighth = static_cast<unsigned>((a.n + 7) / 8);
-  if (!wide) add_norm_any_kernel<INT8><<<rows, kNormLanes, 0, st>>>(a);
-  else if (a.n >= kNormWarpRows && vecs <= 64) add_norm_short_kernel<2, INT8><<<eighth, 256, 0, st>>>(a);
-  else if (a.n >= kNormWarpRows && vecs <= 256) add_norm_short_kernel<8, INT8><<<eighth, 256, 0, st>>>(a);
-  else if (vecs <= kNormLanes) add_norm_kernel<1, INT8><<<rows, kNormLanes, 0, st>>>(a);
-  else if (vecs <= 2 * kNormLanes) add_norm_kernel<2, INT8><<<rows, kNormLanes, 0, st>>>(a);
-  else if (vecs <= 4 * kNormLanes) add_norm_kernel<4, INT8><<<rows, kNormLanes, 0, st>>>(a);
-  else add_norm_kernel<8, INT8><<<rows, kNormLanes, 0, st>>>(a);
+  if (!wide) add_norm_any_kernel<OUT><<<rows, kNormLanes, 0, st>>>(a);
+  else if (a.n >= kNormWarpRows && vecs <= 64) add_norm_short_kernel<2, OUT><<<eighth, 256, 0, st>>>(a);
+  else if (a.n >= kNormWarpRows && vecs <= 256) add_norm_short_kernel<8, OUT><<<eighth, 256, 0, st>>>(a);
+  else if (vecs <= kNormLanes) add_norm_kernel<1, OUT><<<rows, kNormLanes, 0, st>>>(a);
+  else if (vecs <= 2 * kNormLanes) add_norm_kernel<2, OUT><<<rows, kNormLanes, 0, st>>>(a);
+  else if (vecs <= 4 * kNormLanes) add_norm_kernel<4, OUT><<<rows, kNormLanes, 0, st>>>(a);
+  else add_norm_kernel<8, OUT><<<rows, kNormLanes, 0, st>>>(a);
   MG_CUDA(cudaGetLastError());
+  return MG_OK;
+}
+
+template <int VECS>
+int launch_norm_grad_as(const Handle* h, const NormGradArgs& a, const NormGradPlan& p, bool wide, float* gw, cudaStream_t st) {
+  if (wide) {
+    const size_t smem = static_cast<size_t>(p.threads) * kGradStages<VECS> * 3 * VECS * sizeof(uint4);
+    static bool done[64];
+    if (!(h->device >= 0 && h->device < 64 && done[h->device])) {
+      MG_CUDA(cudaFuncSetAttribute(norm_grad_kernel<VECS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   static_cast<int>(kGradThreads * kGradStages<VECS> * 3 * VECS * sizeof(uint4))));
+      if (h->device >= 0 && h->device < 64) done[h->device] = true;
+    }
+    norm_grad_kernel<VECS, true><<<p.blocks, p.threads, smem, st>>>(a);
+  } else {
+    norm_grad_kernel<VECS, false><<<p.blocks, p.threads, 0, st>>>(a);
+  }
+  MG_CUDA(cudaGetLastError());
+  if (gw != nullptr) {
+    norm_grad_sum_kernel<<<static_cast<unsigned>((a.cols + 31) / 32), 1024, 0, st>>>(a.parts, p.shares, a.cols, gw);
+    MG_CUDA(cudaGetLastError());
+  }
   return MG_OK;
 }
 
 }  // namespace
 
-// scale: nullptr for bf16 rows, ldo in elements of out either way
+// scale: nullptr for bf16 rows, ldo in elements of out either way; as_module: bf16 rows rounded as mg_rmsnorm's
 int launch_add_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, float eps, int64_t n, int64_t cols,
-                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, cudaStream_t st) {
+                    void* sum, int64_t lds, void* out, int64_t ldo, float* scale, bool as_module, cudaStream_t st) {
   if (n == 0) return MG_OK;
   NormArgs a{static_cast<const uint16_t*>(x), ldx, static_cast<const uint16_t*>(res), ldr, static_cast<const uint16_t*>(w), eps, n,
              static_cast<int>(cols), static_cast<uint16_t*>(sum), lds, out, ldo, scale};
-  return scale != nullptr ? launch_add_norm_as<true>(a, st) : launch_add_norm_as<false>(a, st);
+  if (scale != nullptr) return launch_add_norm_as<NORM_INT8>(a, st);
+  return as_module ? launch_add_norm_as<NORM_AS_MODULE>(a, st) : launch_add_norm_as<NORM_BF16>(a, st);
 }
 
 int64_t norm_grad_max_cols() { return kGradMaxCols; }
@@ -496,17 +575,8 @@ int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* 
                  gw != nullptr ? static_cast<float*>(ws) : nullptr, p.lanes};
   const bool wide = cols % 8 == 0 && on16(gy, ldgy) && on16(hrows, ldh) && on16(w, 0) && (gh == nullptr || on16(gh, ldgh)) &&
                     (gx == nullptr || on16(gx, ldgx));
-  if (wide && p.vecs == 1) norm_grad_kernel<1, true><<<p.blocks, p.threads, 0, st>>>(a);
-  else if (wide) norm_grad_kernel<2, true><<<p.blocks, p.threads, 0, st>>>(a);
-  else if (p.vecs == 1) norm_grad_kernel<1, false><<<p.blocks, p.threads, 0, st>>>(a);
-  else norm_grad_kernel<2, false><<<p.blocks, p.threads, 0, st>>>(a);
-  MG_CUDA(cudaGetLastError());
-  if (gw != nullptr) {
-    norm_grad_sum_kernel<<<static_cast<unsigned>((cols + 31) / 32), 1024, 0, st>>>(static_cast<const float*>(ws), p.shares,
-                                                                                 static_cast<int>(cols), gw);
-    MG_CUDA(cudaGetLastError());
-  }
-  return MG_OK;
+  if (p.vecs == 1) return launch_norm_grad_as<1>(h, a, p, wide, gw, st);
+  return launch_norm_grad_as<2>(h, a, p, wide, gw, st);
 }
 
 }  // namespace mg

@@ -278,8 +278,9 @@ class MoELayer:
 
     def add_rmsnorm(self, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-6,
                     out: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
-        """-> (rmsnorm(h), h) with h = bf16(x + residual), in one launch; h = x without a residual.  x, residual and weight bf16,
-        [rows, cols] with adjacent columns (any cols, rows may lie further apart).  out and sum_out may each be x or the residual,
+        """-> (y, h) with h = bf16(x + residual), y = bf16(weight * h * rsqrt(mean(h^2) + eps)), in one launch; h = x without a residual.
+        y is rounded once, where rmsnorm rounds a second time before the weight.  x, residual and weight bf16, [rows, cols] with
+        adjacent columns (any cols, rows may lie further apart).  out and sum_out may each be x or the residual,
         not one another, and overlap nothing otherwise.  Any layer serves."""
         n, cols, ldx, ldr, h, lds = self._norm_args(x, residual, weight, sum_out)
         y, ldo = self._out_rows(out, n, cols, "out")
@@ -333,7 +334,7 @@ class MoELayer:
         """hidden + moe(rmsnorm(hidden)): the decoder layer's second half
         (modeling_deepseek_v3.py:1361-1365) with the residual add done by the combine kernel.
         out may be hidden itself (in-place update of the residual stream).  With a residual (same shape) the block runs on
-        bf16(hidden + residual), as if that had been handed in, added by the norm's launch (add_rmsnorm); out may be either."""
+        bf16(hidden + residual), as if that had been handed in, added by the norm's launch; out may be either."""
         shape = hidden.shape
         h2 = hidden.reshape(-1, self.H)
         self._check_in(h2, torch.bfloat16, "hidden_states")
