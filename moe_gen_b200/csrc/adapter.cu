@@ -16,7 +16,7 @@ namespace mg {
 
 namespace {
 
-constexpr int kAdapterTile = 64;            // rows of a tile of a plan
+constexpr int kAdapterTile = 128;           // rows of a tile of a plan
 constexpr int kDirectTile = 16;             // rows of a tile that the kernel finds by itself
 constexpr int kDirectRows = 256;            // rows of a call without a plan, at most: one to a thread
 constexpr int kAdapterThreads = 256;
@@ -70,12 +70,9 @@ __device__ __forceinline__ void copy_row(uint32_t to, const uint16_t* row, int c
   else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
 }
-// BYTES of a row, all of them there
-template <int BYTES>
+// 16 bytes of a row, all of them there
 __device__ __forceinline__ void copy_whole(uint32_t to, const uint16_t* from) {
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -95,6 +92,75 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// the sum of four numbers over the blocks of the cluster, in the order of the blocks
+__device__ __forceinline__ float4 cluster_sum(uint32_t at, int cs) {
+  float4 there[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    if (c < cs) there[c] = ld_cluster_f32x4(map_to_cta(at, c));
+  float4 u = there[0];
+#pragma unroll
+  for (int c = 1; c < 8; ++c)
+    if (c < cs) { u.x += there[c].x; u.y += there[c].y; u.z += there[c].z; u.w += there[c].w; }
+  return u;
+}
+// eight numbers, the second four `next` bytes behind the first
+template <int CS>
+__device__ __forceinline__ void cluster_sum8(uint32_t at, uint32_t next, float* v) {
+  float4 a[CS], b[CS];
+#pragma unroll
+  for (int c = 0; c < CS; ++c) {
+    const uint32_t there = map_to_cta(at, c);
+    a[c] = ld_cluster_f32x4(there);
+    b[c] = ld_cluster_f32x4(there + next);
+  }
+#pragma unroll
+  for (int c = 1; c < CS; ++c) {
+    a[0].x += a[c].x; a[0].y += a[c].y; a[0].z += a[c].z; a[0].w += a[c].w;
+    b[0].x += b[c].x; b[0].y += b[c].y; b[0].z += b[c].z; b[0].w += b[c].w;
+  }
+  v[0] = a[0].x; v[1] = a[0].y; v[2] = a[0].z; v[3] = a[0].w;
+  v[4] = b[0].x; v[5] = b[0].y; v[6] = b[0].z; v[7] = b[0].w;
+}
+__device__ __forceinline__ void st_cluster16(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// two numbers as bf16 and what that leaves of them as bf16
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& high, uint32_t& low) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  const float2 f = __bfloat1622float2(h);
+  // what is not finite has no rest: it would make a NaN of an infinity
+  const __nv_bfloat162 l = __floats2bfloat162_rn(isfinite(f.x) ? a - f.x : 0.f, isfinite(f.y) ? b - f.y : 0.f);
+  high = *reinterpret_cast<const uint32_t*>(&h);
+  low = *reinterpret_cast<const uint32_t*>(&l);
+}
+template <int N>
+__device__ __forceinline__ uint32_t word_of(const uint4 (&v)[N], int w) {      // w is a constant wherever this is inlined
+  const uint4& u = v[w / 4];
+  return w % 4 == 0 ? u.x : w % 4 == 1 ? u.y : w % 4 == 2 ? u.z : u.w;
+}
+// eight elements of a row of n from column c on
+__device__ __forceinline__ void store_row(uint16_t* row, int c, int n, const uint4& v) {
+  if (c + 8 <= n) {
+    *reinterpret_cast<uint4*>(row + c) = v;
+  } else {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < n) row[c + e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+  }
+}
+__device__ __forceinline__ void tc_ld8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+  tc_ld_wait();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[e]);
 }
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
@@ -122,376 +188,530 @@ struct AdapterArgs {
   const int32_t* ids;         // a call without a plan
   const int4* tiles;          // adapter (-1: none), first entry of order, rows with it, rows
   const int32_t* order;
+  int32_t* status;
 };
 
-// NT: n tiles of a warp in the first product, NG: groups of warps over the rank.  BACK: the gradient's two products, whose adapters
-// are transposed.
-template <int NT, int NG>
-struct AdapterCfg {
-  static constexpr int RP = NT * NG * 8;                       // the rank, filled up
-  static constexpr int V1 = 8 + NT, V2 = 8 + RP / 8;           // 16-byte pieces of a thread and a step: rows and adapters, in either product
-  static constexpr int BLOCKS = NT >= 8 ? 1 : 2;               // per SM
-  static constexpr int S1 = NT >= 8 ? 3 : 2, S2 = RP == 64 ? 3 : 2;        // steps on their way
-  static constexpr int PIECES = S1 * V1 > S2 * V2 ? S1 * V1 : S2 * V2;
+// ---- few rows, without a plan ------------------------------------------------------------------
+// Tiles of sixteen rows, which the kernel finds by itself: what counts is the latency and the adapters' bytes.  Operands go through a ring
+// that every thread fills for itself, in the layout of its MMA fragments: the inner index of a product may be permuted at will, so a
+// thread takes 16 adjacent bytes of a row where the fragment names two and two elements apart, and the outputs' index too, so that it
+// ends with 16 adjacent bytes of a row of out.
+template <int RP>                                              // the rank, filled up
+struct DirectCfg {
+  static constexpr int NG = RP == 128 ? 2 : 1, NT = RP / 8 / NG;               // groups of warps over the rank, n tiles of a warp
+  static constexpr int V1 = 2 + NT, V2 = 2 + RP / 8;           // 16-byte pieces of a thread and a step: rows and adapters, in either product
+  static constexpr int STAGES = RP == 16 ? 4 : RP == 128 ? 2 : 3;              // steps on their way
+  static constexpr int PIECES = STAGES * (V1 > V2 ? V1 : V2);
   static constexpr size_t RING = static_cast<size_t>(PIECES) * kAdapterThreads * 16;
-  static constexpr size_t SMEM = RING + kAdapterTile * RP * 2;
-  static_assert(8 / NG * kAdapterTile * RP * 4 <= RING && BLOCKS * (SMEM + 2048) <= 227 * 1024, "shared memory");
+  static constexpr size_t SMEM = RING + 2 * kDirectTile * RP * 2;
+  static_assert(8 / NG * kDirectTile * RP * 4 <= RING && SMEM <= 224 * 1024, "shared memory");
 };
 
-template <int NT, int NG, bool BACK>
-__global__ void __launch_bounds__(kAdapterThreads, AdapterCfg<NT, NG>::BLOCKS) adapter_kernel(const AdapterArgs a) {
-  using C = AdapterCfg<NT, NG>;
-  constexpr int RP = C::RP, KS = RP / 16, KGS = 8 / NG, MT = kAdapterTile / 16;
+template <int RP>
+__global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_direct_kernel(const AdapterArgs a) {
+  using C = DirectCfg<RP>;
+  constexpr int NT = C::NT, NG = C::NG, KS = RP / 16, KGS = 8 / NG, S = C::STAGES;
   extern __shared__ __align__(16) uint8_t smem[];
   float* red = reinterpret_cast<float*>(smem);                                   // between the products: [groups over K][rows][RP]
-  uint4* frag = reinterpret_cast<uint4*>(smem + C::RING);                        // s: [m tile][k step][lane]
-  __shared__ int s_rows[kAdapterTile];
+  uint4* frag = reinterpret_cast<uint4*>(smem + C::RING);                        // s: [high, low part][k step][lane]
+  __shared__ int s_rows[kDirectTile];
   __shared__ int s_before[kAdapterThreads / 32], s_first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, q = lane & 3;
   const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / cs;
-  // A thread copies what it reads itself: piece j of a stage of V lies beside the other threads' piece j, and it waits for its own copies
-  // only.
   const uint32_t ring = smem_u32(smem) + tid * 16;
   auto piece = [&](int j) { return ring + static_cast<uint32_t>(j) * (kAdapterThreads * 16); };
-  int g, live, len;
-  if (a.tiles != nullptr) {
-    const int4 t = a.tiles[tile];
-    g = t.x; live = t.z; len = t.w;
-    if (len == 0) return;
-    if (tid < len) s_rows[tid] = a.order[t.y + tid];
-    __syncthreads();
-  } else {
-    // Row `tile` begins a tile if as many rows of its adapter lie before it as whole tiles take; the tile is it and the next ones.
-    auto id_of = [&](int r) { const int v = a.ids[r]; return v >= 0 && v < a.n_adapters ? v : -1; };
-    g = id_of(tile);
+  // Row `tile` begins a tile if as many rows of its adapter lie before it as whole tiles take; the tile is it and the next ones.
+  auto id_of = [&](int r) { const int v = a.ids[r]; return v >= 0 && v < a.n_adapters ? v : -1; };
+  const int g = id_of(tile);
+  {
     const bool same = tid < a.n_rows && id_of(tid) == g;
     const uint32_t votes = __ballot_sync(0xFFFFFFFFu, same);
     if (lane == 0) s_before[warp] = __popc(votes);
     __syncthreads();
-    int before = __popc(votes & ((1u << lane) - 1u)), all = 0;
-    for (int w = 0; w < kAdapterThreads / 32; ++w) {
-      if (w < warp) before += s_before[w];
-      all += s_before[w];
-    }
+    int before = __popc(votes & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) before += s_before[w];
     if (tid == tile) s_first = before;
     __syncthreads();
     const int first = s_first;
-    if (first % kDirectTile != 0) return;
-    len = min(all - first, kDirectTile);
-    live = g >= 0 ? len : 0;
-    if (same && before >= first && before < first + len) s_rows[before - first] = tid;
-    __syncthreads();
+    if (first % kDirectTile != 0) return;              // the whole cluster
+    if (same && before >= first && before < first + kDirectTile) s_rows[before - first] = tid;
   }
+  int all = 0;
+  for (int w = 0; w < kAdapterThreads / 32; ++w) all += s_before[w];
+  const int len = min(all - s_first, kDirectTile), live = g >= 0 ? len : 0;
   const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
-  const int live_mts = (live + 15) / 16;
+  __syncthreads();
+  int64_t row_of[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) row_of[hf] = s_rows[min(hf * 8 + i, len - 1)];
 
   if (live > 0) {
     const int ng = warp % NG, kg = warp / NG;
-    const uint16_t* w1 = a.w1 + g * a.g1 + (BACK ? 0 : static_cast<int64_t>(ng * NT * 8 + i) * a.ld1);
-    const uint16_t* xp[MT][2];
+    const uint16_t* w1 = a.w1 + g * a.g1;
+    const uint16_t* xp[2] = {a.x + row_of[0] * a.ldx, a.x + row_of[1] * a.ldx};
+    float acc[NT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) xp[m][hf] = a.x + static_cast<int64_t>(s_rows[min(m * 16 + hf * 8 + i, live - 1)]) * a.ldx;
-    float acc[MT][NT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][t][e] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
     const int slices = (a.K + 31) / 32, per = (slices + cs - 1) / cs;
     const int lo = cr * per, hi = min(slices, lo + per);
-    const bool filled = a.rank == RP;
     auto fetch = [&](int stage, int sl) {
-      const int c = sl * 32 + 8 * q;
-      if (sl < hi && filled && sl * 32 + 32 <= a.K) {
+      if (sl < hi) {
+        const int c = sl * 32 + 8 * q;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m < live_mts)
+        for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V1 + hf), xp[hf], c, a.K);
+        // eight elements of each of NT rows of w1: row i of the n tiles
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) copy_whole<16>(piece(stage * C::V1 + m * 2 + hf), xp[m][hf] + c);
-        const uint16_t* w = BACK ? w1 + c * a.ld1 + ng * NT * 8 + i * NT : w1 + c;
-        const int64_t next = BACK ? a.ld1 : 8 * a.ld1;
-#pragma unroll
-        for (int r = 0; r < (BACK ? 8 : NT); ++r, w += next) {
-          if (!BACK) copy_whole<16>(piece(stage * C::V1 + 8 + r), w);
-          else copy_whole<NT * 2>(piece(stage * C::V1 + 8 + r * NT / 8) + r * NT % 8 * 2, w);
-        }
-      } else if (sl < hi) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m < live_mts)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V1 + m * 2 + hf), xp[m][hf], c, a.K);
-        if (!BACK) {
-          // eight elements of each of NT rows of w1: row i of the n tiles
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            copy_row<16>(piece(stage * C::V1 + 8 + t), (ng * NT + t) * 8 + i < a.rank ? w1 + t * 8 * a.ld1 : a.w1, c,
-                         (ng * NT + t) * 8 + i < a.rank ? a.K : 0);
-        } else {
-          // NT elements of each of eight rows of w1: element i * NT + t is row i of n tile t
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            copy_row<NT * 2>(piece(stage * C::V1 + 8 + r * NT / 8) + r * NT % 8 * 2, w1 + static_cast<int64_t>(min(c + r, a.K - 1)) * a.ld1,
-                             ng * NT * 8 + i * NT, c + r < a.K ? a.rank : 0);
+        for (int t = 0; t < NT; ++t) {
+          const int n = (ng * NT + t) * 8 + i;
+          copy_row<16>(piece(stage * C::V1 + 2 + t), w1 + (n < a.rank ? n : 0) * a.ld1, c, n < a.rank ? a.K : 0);
         }
       }
       copies_commit();
     };
 #pragma unroll
-    for (int k = 0; k < C::S1 - 1; ++k) fetch(k, lo + kg + k * KGS);
+    for (int k = 0; k < S - 1; ++k) fetch(k, lo + kg + k * KGS);
     int stage = 0;
     for (int sl = lo + kg; sl < hi; sl += KGS) {
-      fetch(stage == 0 ? C::S1 - 1 : stage - 1, sl + (C::S1 - 1) * KGS);
-      copies_wait<C::S1 - 1>();
-      uint32_t bv[NT * 4];
+      fetch(stage == 0 ? S - 1 : stage - 1, sl + (S - 1) * KGS);
+      copies_wait<S - 1>();
+      const uint4 u0 = ld_shared(piece(stage * C::V1)), u1 = ld_shared(piece(stage * C::V1 + 1));
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint4 v = ld_shared(piece(stage * C::V1 + 8 + t));
-        bv[4 * t] = v.x; bv[4 * t + 1] = v.y; bv[4 * t + 2] = v.z; bv[4 * t + 3] = v.w;
+        const uint4 v = ld_shared(piece(stage * C::V1 + 2 + t));
+        mma_bf16(acc[t], u0.x, u1.x, u0.y, u1.y, v.x, v.y);
+        mma_bf16(acc[t], u0.z, u1.z, u0.w, u1.w, v.z, v.w);
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m >= live_mts) break;
-        const uint4 u0 = ld_shared(piece(stage * C::V1 + m * 2)), u1 = ld_shared(piece(stage * C::V1 + m * 2 + 1));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint32_t b[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t r0 = bv[BACK ? 2 * e * (NT / 2) + t / 2 : 0], r1 = bv[BACK ? (2 * e + 1) * (NT / 2) + t / 2 : 0];
-            b[e] = !BACK ? bv[t * 4 + e] : t % 2 ? highs(r0, r1) : lows(r0, r1);
-          }
-          mma_bf16(acc[m][t], u0.x, u1.x, u0.y, u1.y, b[0], b[1]);
-          mma_bf16(acc[m][t], u0.z, u1.z, u0.w, u1.w, b[2], b[3]);
-        }
-      }
-      if (++stage == C::S1) stage = 0;
+      if (++stage == S) stage = 0;
     }
     copies_wait<0>();
     __syncthreads();                                  // the ring is free: the warps' sums go there
-    const int rows = live_mts * 16;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m >= live_mts) break;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = 2 * q + (e & 1);
-          const int r = ng * NT * 8 + (BACK ? n * NT + t : t * 8 + n);
-          red[(kg * rows + m * 16 + (e >> 1) * 8 + i) * RP + r] = acc[m][t][e];
-        }
-    }
+      for (int e = 0; e < 4; ++e) red[(kg * kDirectTile + (e >> 1) * 8 + i) * RP + ng * NT * 8 + t * 8 + 2 * q + (e & 1)] = acc[t][e];
     __syncthreads();
     // The sums of this block over its warps, then over the blocks of the cluster, always in the same order; the columns behind the rank
     // and the rows behind the tile's are zeros.
     const float4* parts = reinterpret_cast<const float4*>(red);
-    const int quads = rows * RP / 4;
+    constexpr int QUADS = kDirectTile * RP / 4;
     auto block_sum = [&](int p) {
       float4 v = parts[p];
 #pragma unroll
       for (int k = 1; k < KGS; ++k) {
-        const float4 u = parts[k * quads + p];
-        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        const float4 w = parts[k * QUADS + p];
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
       }
       return v;
     };
     if (cs > 1) {
-      for (int p = tid; p < quads; p += kAdapterThreads) reinterpret_cast<float4*>(red)[p] = block_sum(p);
+      for (int p = tid; p < QUADS; p += kAdapterThreads) reinterpret_cast<float4*>(red)[p] = block_sum(p);
       cluster_sync_all();
     }
-    for (int p = tid; p < quads; p += kAdapterThreads) {
+    for (int p = tid; p < QUADS; p += kAdapterThreads) {
       const int row = 4 * p / RP, r = 4 * p % RP;
-      float4 u;
-      if (cs > 1) {
-        const uint32_t at = smem_u32(parts + p);
-        float4 there[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c < cs) there[c] = ld_cluster_f32x4(map_to_cta(at, c));
-        u = there[0];
-#pragma unroll
-        for (int c = 1; c < 8; ++c)
-          if (c < cs) { u.x += there[c].x; u.y += there[c].y; u.z += there[c].z; u.w += there[c].w; }
-      } else {
-        u = block_sum(p);
-      }
+      const float4 u = cs > 1 ? cluster_sum(smem_u32(parts + p), cs) : block_sum(p);
       float v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = row < live && r + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
-      const __nv_bfloat162 b0 = __floats2bfloat162_rn(v[0], v[1]), b1 = __floats2bfloat162_rn(v[2], v[3]);
-      const uint2 words = make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1));
-      // the fragments that hold (row, r) to (row, r + 3): see the loads of w2 below
+      for (int e = 0; e < 4; ++e) v[e] = row < live && r + e < a.rank ? v[e] : 0.f;
+      uint2 high, low;
+      split_pair(v[0], v[1], high.x, low.x);
+      split_pair(v[2], v[3], high.y, low.y);
+      // the fragments that hold (row, r) to (row, r + 3): see the copies of w2
       const int fi = row & 7, hf = (row >> 3) & 1, fq = RP == 16 ? r >> 2 : (r & 31) >> 3;
       const int ks = RP == 16 ? 0 : (r >> 5) * 2 + ((r >> 2) & 1);
-      uint32_t* f = reinterpret_cast<uint32_t*>(frag + ((row >> 4) * KS + ks) * 32 + fi * 4 + fq);
-      f[hf] = words.x;
-      f[2 + hf] = words.y;
-      if (a.s != nullptr && cr == 0 && row < len) *reinterpret_cast<uint2*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + r) = words;
+      uint32_t* f = reinterpret_cast<uint32_t*>(frag + ks * 32 + fi * 4 + fq);
+      f[hf] = high.x;
+      f[2 + hf] = high.y;
+      f[KS * 128 + hf] = low.x;
+      f[KS * 128 + 2 + hf] = low.y;
+      if (a.s != nullptr && cr == 0 && row < len) *reinterpret_cast<uint2*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + r) = high;
     }
     if (cs > 1) cluster_sync_all();                   // the ring is free again, here and in the blocks that have read it
     else __syncthreads();
-  }
-  if (a.s != nullptr && cr == 0) {                    // rows without an adapter
-    const int from = live_mts * 16;
-    for (int p = tid; p < (len - from) * RP / 2; p += kAdapterThreads)
-      *reinterpret_cast<uint32_t*>(a.s + static_cast<int64_t>(s_rows[from + 2 * p / RP]) * RP + 2 * p % RP) = 0u;
+  } else if (a.s != nullptr && cr == 0) {
+    for (int p = tid; p < len * RP / 2; p += kAdapterThreads)
+      *reinterpret_cast<uint32_t*>(a.s + static_cast<int64_t>(s_rows[2 * p / RP]) * RP + 2 * p % RP) = 0u;
   }
 
   const int units = (a.N + 31) / 32, each = (units + cs - 1) / cs, last = min(units, (cr + 1) * each);
-  const int mts = (len + 15) / 16;
-  const bool in_place = a.y == a.out && a.ldy == a.ldo;
+  if (live == 0 && a.y == a.out && a.ldy == a.ldo) return;            // after the last barrier of the cluster
   const uint16_t* w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
-  const uint16_t* yp[MT][2];
-  uint16_t* op[MT][2];                                // nullptr: not written
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = m * 16 + hf * 8 + i;
-      const int64_t row = s_rows[min(r, len - 1)];
-      yp[m][hf] = a.y + row * a.ldy;
-      op[m][hf] = r < len && !(in_place && r >= live) ? a.out + row * a.ldo : nullptr;
-    }
-  const bool filled = a.rank == RP;
   auto fetch = [&](int stage, int unit) {
-    const int c0 = unit * 32, c = c0 + 8 * q;
-    if (unit < last && filled && c0 + 32 <= a.N) {
-      if (a.y != nullptr)
+    if (unit < last) {
+      const int c0 = unit * 32;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m < mts)
+      for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V2 + hf), a.y + row_of[hf] * a.ldy, c0 + 8 * q, hf * 8 + i < len ? a.N : 0);
+      if (live > 0)
+        // of row 4 i + t of the unit's 32 rows of w2, n tile t's row i: the elements of this thread's fragments
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) copy_whole<16>(piece(stage * C::V2 + m * 2 + hf), yp[m][hf] + c);
-      if (live > 0 && !BACK) {
-        const uint16_t* w = w2 + (c0 + 4 * i) * a.ld2 + (RP == 16 ? 4 : 8) * q;
-#pragma unroll
-        for (int t = 0; t < 4; ++t, w += a.ld2) {
-          if (RP == 16) copy_whole<8>(piece(stage * C::V2 + 8 + t / 2) + t % 2 * 8, w);
+        for (int t = 0; t < 4; ++t) {
+          const int col = c0 + 4 * i + t, end = col < a.N ? a.rank : 0;
+          const uint16_t* row = w2 + (col < a.N ? col : 0) * a.ld2;
+          if (RP == 16) copy_row<8>(piece(stage * C::V2 + 2 + t / 2) + t % 2 * 8, row, 4 * q, end);
           else
 #pragma unroll
-            for (int p = 0; p < RP / 32; ++p) copy_whole<16>(piece(stage * C::V2 + 8 + t * (RP / 32) + p), w + 32 * p);
+            for (int p = 0; p < RP / 32; ++p) copy_row<16>(piece(stage * C::V2 + 2 + t * (RP / 32) + p), row, 32 * p + 8 * q, end);
         }
-      } else if (live > 0) {
-#pragma unroll
-        for (int k = 0; k < KS; k += 2) {
-          const uint16_t* w = w2 + (RP == 16 ? 4 * q : k * 16 + 8 * q) * a.ld2 + c0 + 4 * i;
-#pragma unroll
-          for (int e = 0; e < (RP == 16 ? 4 : 8); ++e, w += a.ld2) copy_whole<8>(piece(stage * C::V2 + 8 + k * 2 + e / 2) + e % 2 * 8, w);
-        }
-      }
-    } else if (unit < last) {
-      if (a.y != nullptr)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (m < mts)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) copy_row<16>(piece(stage * C::V2 + m * 2 + hf), yp[m][hf], c, a.N);
-      if (live > 0) {
-        if (!BACK) {
-          // of row 4 i + t of the unit's 32 rows of w2, n tile t's row i: the elements of this thread's fragments
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int col = c0 + 4 * i + t, end = col < a.N ? a.rank : 0;
-            const uint16_t* row = w2 + (col < a.N ? col : 0) * a.ld2;
-            if (RP == 16) {
-              copy_row<8>(piece(stage * C::V2 + 8 + t / 2) + t % 2 * 8, row, 4 * q, end);
-            } else {
-#pragma unroll
-              for (int p = 0; p < RP / 32; ++p) copy_row<16>(piece(stage * C::V2 + 8 + t * (RP / 32) + p), row, 32 * p + 8 * q, end);
-            }
-          }
-        } else {
-          // four columns, of n tiles 0 to 3, of the rows of w2 that this thread's fragments hold
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = (RP == 16 ? 4 * q : (ks >> 1) * 32 + 8 * q + (ks & 1) * 4) + e;
-              copy_row<8>(piece(stage * C::V2 + 8 + ks * 2 + e / 2) + e % 2 * 8, w2 + (r < a.rank ? r : 0) * a.ld2, c0 + 4 * i,
-                          r < a.rank ? a.N : 0);
-            }
-        }
-      }
     }
     copies_commit();
   };
   const int unit0 = cr * each + warp;
 #pragma unroll
-  for (int k = 0; k < C::S2 - 1; ++k) fetch(k, unit0 + k * (kAdapterThreads / 32));
+  for (int k = 0; k < S - 1; ++k) fetch(k, unit0 + k * (kAdapterThreads / 32));
   int stage = 0;
   for (int unit = unit0; unit < last; unit += kAdapterThreads / 32) {
-    fetch(stage == 0 ? C::S2 - 1 : stage - 1, unit + (C::S2 - 1) * (kAdapterThreads / 32));
-    copies_wait<C::S2 - 1>();
+    fetch(stage == 0 ? S - 1 : stage - 1, unit + (S - 1) * (kAdapterThreads / 32));
+    copies_wait<S - 1>();
     const int c = unit * 32 + 8 * q;
-    uint32_t b[KS][4][2];
-    if (live > 0) {
-      uint32_t v[KS * 8];
+    float acc[4][4];
 #pragma unroll
-      for (int j = 0; j < KS * 2; ++j) {
-        const uint4 u = ld_shared(piece(stage * C::V2 + 8 + j));
-        v[4 * j] = u.x; v[4 * j + 1] = u.y; v[4 * j + 2] = u.z; v[4 * j + 3] = u.w;
-      }
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    if (live > 0) {
+      uint4 v[KS * 2];
+#pragma unroll
+      for (int j = 0; j < KS * 2; ++j) v[j] = ld_shared(piece(stage * C::V2 + 2 + j));
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int part = 0; part < 2; ++part) {
+          const uint4 f = frag[(part * KS + ks) * 32 + lane];
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            if (!BACK)
-              b[ks][t][p] = RP == 16 ? v[t * 2 + p] : v[(t * (RP / 32) + ks / 2) * 4 + ks % 2 * 2 + p];
-            else {
-              const uint32_t r0 = v[ks * 8 + p * 4 + t / 2], r1 = v[ks * 8 + p * 4 + 2 + t / 2];
-              b[ks][t][p] = t % 2 ? highs(r0, r1) : lows(r0, r1);
-            }
+          for (int t = 0; t < 4; ++t) {
+            const int w = RP == 16 ? t * 2 : (t * (RP / 32) + ks / 2) * 4 + ks % 2 * 2;
+            mma_bf16(acc[t], f.x, f.y, f.z, f.w, word_of(v, w), word_of(v, w + 1));
           }
+        }
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m >= mts) break;
-      float acc[4][4];
+    for (int hf = 0; hf < 2; ++hf) {
+      if (hf * 8 + i >= len || c >= a.N) continue;
+      uint4 v = ld_shared(piece(stage * C::V2 + hf));
+      if (live > 0) {
+        float o[8];
+        unpack8(v, o);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(scale, acc[e & 3][hf * 2 + (e >> 2)], o[e]);          // column 4 * (2q + (e >> 2)) + (e & 3) of the unit
+        v = pack8(o);
+      }
+      store_row(a.out + row_of[hf] * a.ldo, c, a.N, v);
+    }
+    if (++stage == S) stage = 0;
+  }
+  copies_wait<0>();
+}
+
+// ---- tiles of a plan ---------------------------------------------------------------------------
+// 128 rows of one adapter on the accumulator's lanes.  Eight warps copy the tiles of either product to shared memory as the tensor core reads
+// them, a few steps ahead (rows wherever the order says, zeros behind what a row or the rank has), and finish the outputs; a ninth has the
+// products done, into tensor memory.  A step is 64 columns of x, or 64 columns of out.  s passes through shared memory in two parts of
+// bf16, so that it has 16 bits of mantissa in the second product.  A cluster of up to eight blocks shares a tile where there are few: each sums
+// s over its columns of x, then over the blocks for its share of the rows, and hands that to all.
+constexpr int kTileThreads = kAdapterThreads + 32;
+template <int RP>
+struct TileCfg {
+  static constexpr int BLOCKS = RP <= 64 ? 2 : 1;              // per SM
+  static constexpr int STAGES = RP <= 64 ? 3 : 4;
+  static constexpr int ROWS = kAdapterTile * 128;              // bytes of a stage: the rows' tile, then the adapter's
+  static constexpr int STAGE = ROWS + (RP <= 64 ? 8192 : 16384);
+  static constexpr int PART = ROWS * (RP <= 64 ? 1 : 2);       // either part of s: blocks of 64 columns
+  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + 2 * PART + 1024;
+  static constexpr int COLS = 256, SECOND = 128;               // of tensor memory; the second product's two accumulators of 64
+  static_assert(kAdapterTile * RP * 4 <= STAGES * STAGE && BLOCKS * (SMEM + 2048) <= 227 * 1024, "shared memory");
+};
+// operand whose inner index goes over rows of 128 bytes (64 outer elements each), swizzled: 64 outer elements outer_bytes apart
+__device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t outer_bytes) {
+  return (make_smem_desc(saddr) & ~(0x3FFFull << 16)) | static_cast<uint64_t>(outer_bytes >> 4) << 16;
+}
+__host__ __device__ constexpr uint32_t mma_shape(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n) >> 3 << 17) | (8u << 24); }
+constexpr uint32_t kRowsB = 1u << 16;           // operand B by rows_desc
+
+template <int RP, bool BACK>
+__global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_tile_kernel(const AdapterArgs a) {
+  using C = TileCfg<RP>;
+  constexpr int S = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t s_full[S], s_done[S];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  __shared__ int s_rows[kAdapterTile];
+  const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u, s_at = ring + S * C::STAGE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, quarter = warp & 3, side = warp >> 2;
+  const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
+  const int4 job = a.tiles[blockIdx.x / cs];
+  const int g = job.x, live = job.z, len = job.w;
+  if (len == 0) return;                                // the whole cluster
+  if (tid < len) s_rows[tid] = a.order[job.y + tid];
+  if (tid == 0) {
+    for (int k = 0; k < S; ++k) { mbar_init(smem_u32(&s_full[k]), kAdapterThreads / 32); mbar_init(smem_u32(&s_done[k]), 1); }
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(C::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
+  const int slices = live > 0 ? (a.K + 63) / 64 : 0, per = (slices + cs - 1) / cs;
+  const int units = (a.N + 63) / 64, each = (units + cs - 1) / cs;
+  const int lo1 = cr * per, n1 = max(min(slices, lo1 + per) - lo1, 0), lo2 = cr * each, n2 = max(min(units, lo2 + each) - lo2, 0);
+  const int steps = n1 + n2;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 8) {
+    // ---- products: a step's as soon as its tiles are there; the stage is free when they are done ----
+    auto arrived = [&](int k) {
+      mbar_wait(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 121);
+      tc_fence_after();
+      return ring + k % S * C::STAGE;
+    };
+    if (live > 0 && elect_one())
+      for (int k = 0; k < n1; ++k) {
+        const uint32_t at = arrived(k);
+        const uint64_t da = make_smem_desc(at), db = BACK ? rows_desc(at + C::ROWS, 8192) : make_smem_desc(at + C::ROWS);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-      if (m < live_mts) {
+        for (int j = 0; j < 4; ++j)
+          tc_mma_bf16(tmem, da + 2 * j, db + (BACK ? 128 : 2) * j, mma_shape(RP) | (BACK ? kRowsB : 0u), k + j > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&s_done[k % S]));
+      }
+    __syncwarp();
+    if (live > 0 && cs > 1) {
+      cluster_sync_all();
+      cluster_sync_all();
+    }
+    if (live > 0 && elect_one())
+      for (int m = 0; m < n2; ++m) {
+        const uint32_t at = arrived(n1 + m) + C::ROWS, d = tmem + C::SECOND + (m & 1) * 64;
+        const uint64_t da = make_smem_desc(s_at), db = BACK ? rows_desc(at, 8192) : make_smem_desc(at);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const uint4 f = frag[(m * KS + ks) * 32 + lane];
+        for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) mma_bf16(acc[t], f.x, f.y, f.z, f.w, b[ks][t][0], b[ks][t][1]);
+          for (int k = 0; k < RP / 16; ++k)
+            tc_mma_bf16(d, da + (part * C::PART + (k >> 2) * C::ROWS) / 16 + 2 * (k & 3), db + (BACK ? 128 * k : (k >> 2) * 512 + 2 * (k & 3)),
+                        mma_shape(64) | (BACK ? kRowsB : 0u), part + k > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&s_done[(n1 + m) % S]));
+      }
+    __syncwarp();
+  } else {
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const bool in_place = a.y == a.out && a.ldy == a.ldo, filled = a.rank == RP;
+    const uint16_t* w1 = a.w1 + (g >= 0 ? g * a.g1 : 0);
+    const uint16_t* w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
+    // A warp copies, finishes and stores 32 rows by 64 bytes of a tile: this thread 16 bytes of rows i, i + 8, i + 16 and i + 24 of them.
+    // Rows that are not there are the last one again, and not stored.
+    const int piece = side * 4 + (lane & 3);
+    const uint32_t mine = (quarter * 32 + i) * 128 + ((piece ^ i) << 4);         // in a tile of rows; 1024 bytes to the next one
+    const uint16_t *xp[4], *yp[4];
+    uint16_t* op[4];
+    uint32_t stored = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = quarter * 32 + j * 8 + i;
+      const int64_t row = s_rows[min(r, len - 1)];
+      xp[j] = a.x + (live > 0 ? static_cast<int64_t>(s_rows[min(r, live - 1)]) : 0) * a.ldx + piece * 8;
+      yp[j] = a.y + row * a.ldy + piece * 8;
+      op[j] = a.out + row * a.ldo + piece * 8;
+      stored |= (r < len && !(in_place && r >= live) ? 1u : 0u) << j;
+    }
+    // The adapter's tile: RP rows of 64 elements (wide), or 64 rows of RP (narrow).  This thread's 16-byte pieces, in pairs of rows so far apart that
+    // their place is the same one
+    constexpr int WIDE = RP / 32 > 0 ? RP / 32 : 1, NARROW_ROWS = kAdapterThreads / (RP / 8);
+    const bool mine_too = RP >= 32 || tid < 128;
+    const int wr = tid >> 3, wp = tid & 7, nr = tid / (RP / 8), np = tid % (RP / 8);
+    const uint32_t wide_at = C::ROWS + wr * 128 + ((wp ^ (wr & 7)) << 4);
+    const uint32_t narrow_at = C::ROWS + (np >> 3) * 8192 + nr * 128 + (((np & 7) ^ (nr & 7)) << 4);
+    const uint16_t* wide = BACK ? w2 + wr * a.ld2 + wp * 8 : w1 + wr * a.ld1 + wp * 8;
+    const uint16_t* narrow = BACK ? w1 + nr * a.ld1 + np * 8 : w2 + nr * a.ld2 + np * 8;
+    const int64_t wide_ld = BACK ? a.ld2 : a.ld1, narrow_ld = BACK ? a.ld1 : a.ld2;
+    auto fetch_adapter = [&](uint32_t to, int c, bool first, bool whole) {
+      if (!mine_too) return;
+      if (first != BACK) {                             // wide
+        if (whole) {
+          const uint16_t* w = wide + c;
+#pragma unroll
+          for (int j = 0; j < WIDE; ++j, w += 32 * wide_ld) copy_whole(to + wide_at + j * 4096, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < WIDE; ++j) {
+            const int r = wr + j * 32;
+            copy_row<16>(to + wide_at + j * 4096, (BACK ? w2 : w1) + (r < a.rank ? r : 0) * wide_ld, c + wp * 8, r < a.rank ? (BACK ? a.N : a.K) : 0);
+          }
+        }
+      } else {
+        const int end = BACK ? a.K : a.N;
+        if (whole) {
+          const uint16_t* w = narrow + c * narrow_ld;
+#pragma unroll
+          for (int j = 0; j < WIDE; ++j, w += NARROW_ROWS * narrow_ld) copy_whole(to + narrow_at + j * NARROW_ROWS * 128, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < WIDE; ++j) {
+            const int r = c + nr + j * NARROW_ROWS;
+            copy_row<16>(to + narrow_at + j * NARROW_ROWS * 128, (BACK ? w1 : w2) + (r < end ? r : 0) * narrow_ld, np * 8, r < end ? a.rank : 0);
+          }
         }
       }
+    };
+    int ahead = 0;                                     // the next step to fetch, into stage `filling`
+    uint32_t filling = ring;
+    auto fetch = [&](int end) {
+      if (ahead < end) {
+        const bool first = ahead < n1;
+        const int c = (first ? lo1 + ahead : lo2 + ahead - n1) * 64, n = first ? a.K : a.N;
+        const bool inside = c + 64 <= n;
+        if (first ? quarter * 32 < live : !BACK && quarter * 32 < len) {
+          if (inside) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        if (op[m][hf] == nullptr || c >= a.N) continue;
-        uint4 v = a.y != nullptr ? ld_shared(piece(stage * C::V2 + m * 2 + hf)) : make_uint4(0u, 0u, 0u, 0u);
-        if (m * 16 + hf * 8 + i < live) {
+            for (int j = 0; j < 4; ++j) copy_whole(filling + mine + j * 1024, (first ? xp[j] : yp[j]) + c);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) copy_row<16>(filling + mine + j * 1024, (first ? xp[j] : yp[j]) - piece * 8, c + piece * 8, n);
+          }
+        }
+        if (live > 0) fetch_adapter(filling, c, first, inside && filled);
+      }
+      copies_commit();
+      ++ahead;
+      filling = filling == ring + (S - 1) * C::STAGE ? ring : filling + C::STAGE;
+    };
+    // this warp's copies of step k are there, and what it has written before, for the tensor core too
+    auto arrive = [&](int k) {
+      copies_wait<S - 2>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (live > 0 && lane == 0) mbar_arrive(smem_u32(&s_full[k % S]));
+    };
+    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 120); };
+    const int end1 = cs == 1 ? steps : n1;             // in a cluster the blocks' sums of s go where the ring is
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k) fetch(end1);
+
+    if (live > 0) {
+      for (int k = 0; k < n1; ++k) {
+        arrive(k);
+        if (k > 0) done(k - 1);
+        fetch(end1);
+      }
+      if (n1 > 0) done(n1 - 1);
+      tc_fence_after();
+      // eight columns of a row of s, zeros behind the tile's rows and the rank, in two parts
+      auto parts = [&](int row, int col, float* v, uint4& high, uint4& low) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = row < live && col + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
+        split_pair(v[0], v[1], high.x, low.x);
+        split_pair(v[2], v[3], high.y, low.y);
+        split_pair(v[4], v[5], high.z, low.z);
+        split_pair(v[6], v[7], high.w, low.w);
+        if (a.s != nullptr && row < len) *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + col) = high;
+        return s_at + (col >> 6) * C::ROWS + row * 128 + (((col >> 3 & 7) ^ (row & 7)) << 4);
+      };
+      // the accumulator's row of this thread, half of the columns to either side's warps
+#pragma unroll
+      for (int k = 0; k < RP / 2; k += 8) {
+        float v[8];
+        const int row = quarter * 32 + lane, col = side * (RP / 2) + k;
+        tc_ld8(lanes + col, v);
+        if (n1 == 0)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (cs == 1) {
+          uint4 high, low;
+          const uint32_t to = parts(row, col, v, high, low);
+          st_shared(to, high);
+          st_shared(to + C::PART, low);
+        } else {                                       // [groups of four columns][row]
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            st_shared(ring + ((col / 4 + e) * kAdapterTile + row) * 16,
+                      make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
+        }
+      }
+      if (cs > 1) {
+        cluster_sync_all();
+        const int share = kAdapterTile / cs;
+        for (int p = tid; p < share * RP / 8; p += kAdapterThreads) {
+          const int row = cr * share + p % share, col = p / share * 8;
+          float v[8];
+          const uint32_t at = ring + (col / 4 * kAdapterTile + row) * 16;
+          if (cs == 8) cluster_sum8<8>(at, kAdapterTile * 16, v);
+          else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, v);
+          else cluster_sum8<2>(at, kAdapterTile * 16, v);
+          uint4 high, low;
+          const uint32_t to = parts(row, col, v, high, low);
+          for (int c = 0; c < cs; ++c) {
+            const uint32_t there = map_to_cta(to, c);
+            st_cluster16(there, high);
+            st_cluster16(there + C::PART, low);
+          }
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        cluster_sync_all();                            // s is whole; the ring is free again, here and in the blocks that have read it
+      }
+    } else if (a.s != nullptr && cr == 0) {
+      for (int p = tid; p < len * RP / 8; p += kAdapterThreads)
+        *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[p / (RP / 8)]) * RP + p % (RP / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (cs > 1) {
+      ahead = n1;
+      filling = ring + n1 % S * C::STAGE;
+#pragma unroll
+      for (int k = 0; k < S - 1; ++k) fetch(steps);
+    }
+
+    // finishes unit m in the place of y, from where the warp stores 64 bytes of eight rows at a time
+    auto finish = [&](int m) {
+      const uint32_t at = ring + (n1 + m) % S * C::STAGE;
+      const int c0 = (lo2 + m) * 64, row = quarter * 32 + lane;
+      if (live > 0) {
+        done(n1 + m);
+        tc_fence_after();
+        uint32_t acc[32];
+        tc_ld32(lanes + C::SECOND + (m & 1) * 64 + side * 32, acc);
+        tc_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t to = at + row * 128 + (((side * 4 + k) ^ (row & 7)) << 4);
           float o[8];
-          unpack8(v, o);
+          if (!BACK) unpack8(ld_shared(to), o);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float p = acc[e & 3][hf * 2 + (e >> 2)];                        // column 4 * (2q + (e >> 2)) + (e & 3) of the unit
+            const float p = __uint_as_float(acc[8 * k + e]);
             o[e] = BACK ? p : fmaf(scale, p, o[e]);
           }
-          v = pack8(o);
-        }
-        uint16_t* dst = op[m][hf] + c;
-        if (c + 8 <= a.N) {
-          *reinterpret_cast<uint4*>(dst) = v;
-        } else {
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c + e < a.N) dst[e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+          if (row < live) st_shared(to, pack8(o));
+          else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
         }
       }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u) : ld_shared(at + mine + j * 1024);
+        if (stored >> j & 1u) store_row(op[j] + c0, 0, a.N - c0 - piece * 8, v);
+      }
+    };
+    for (int m = 0; m < n2; ++m) {
+      arrive(n1 + m);
+      if (m > 0) finish(m - 1);
+      fetch(steps);
     }
-    if (++stage == C::S2) stage = 0;
+    if (n2 > 0) finish(n2 - 1);
+    copies_wait<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
   }
 }
 
@@ -732,14 +952,14 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
 int padded_rank(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 template <typename... P, typename... A>
-cudaError_t launch_clusters(void (*kernel)(P...), int64_t jobs, int cs, size_t smem, cudaStream_t st, A&&... args) {
+cudaError_t launch_clusters(void (*kernel)(P...), int64_t jobs, int cs, int threads, size_t smem, cudaStream_t st, A&&... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = cs;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(jobs * cs));
-  cfg.blockDim = dim3(kAdapterThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &attr;
@@ -757,26 +977,42 @@ int allow_smem(const Handle* h, K* kernel, size_t smem, bool (&done)[64]) {
   return MG_OK;
 }
 
-template <int NT, int NG, bool BACK>
-int launch_adapter_as(const Handle* h, const AdapterArgs& a, int64_t jobs, int cs, cudaStream_t st) {
-  constexpr size_t smem = AdapterCfg<NT, NG>::SMEM;
+template <int RP>
+int launch_direct_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   static bool done[64];
-  if (int rc = allow_smem(h, adapter_kernel<NT, NG, BACK>, smem, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_kernel<NT, NG, BACK>, jobs, cs, smem, st, a));
+  if (int rc = allow_smem(h, adapter_direct_kernel<RP>, DirectCfg<RP>::SMEM, done)) return rc;
+  int cs = 8;
+  while (cs > 2 && static_cast<int64_t>(a.n_rows) * cs > 4 * h->sm_count) cs /= 2;
+  MG_CUDA(launch_clusters(adapter_direct_kernel<RP>, a.n_rows, cs, kAdapterThreads, DirectCfg<RP>::SMEM, st, a));
+  return MG_OK;
+}
+template <int RP, bool BACK>
+int launch_tiles_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
+  using C = TileCfg<RP>;
+  static bool done[64];
+  if (int rc = allow_smem(h, adapter_tile_kernel<RP, BACK>, C::SMEM, done)) return rc;
+  // as many blocks to a tile as run at once, were all tiles full
+  const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile;
+  int cs = 8;
+  while (cs > 1 && full * cs > C::BLOCKS * h->sm_count) cs /= 2;
+  MG_CUDA(launch_clusters(adapter_tile_kernel<RP, BACK>, full + a.n_adapters + 1, cs, kTileThreads, C::SMEM, st, a));
   return MG_OK;
 }
 template <bool BACK>
-int launch_adapter_rank(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
-  const int64_t jobs = a.tiles != nullptr ? (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile + a.n_adapters + 1 : a.n_rows;
-  // as many blocks to a tile as run at once, were all tiles full
-  const int64_t full = a.tiles != nullptr ? (a.n_rows + kAdapterTile - 1) / kAdapterTile : a.n_rows;
-  int cs = 8;
-  while (cs > 1 && full * cs > (a.rank > 32 ? 1 : 2) * h->sm_count) cs /= 2;
+int launch_tiles(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   switch (padded_rank(a.rank)) {
-    case 16: return launch_adapter_as<2, 1, BACK>(h, a, jobs, cs, st);
-    case 32: return launch_adapter_as<4, 1, BACK>(h, a, jobs, cs, st);
-    case 64: return launch_adapter_as<8, 1, BACK>(h, a, jobs, cs, st);
-    default: return launch_adapter_as<8, 2, BACK>(h, a, jobs, cs, st);
+    case 16: return launch_tiles_as<16, BACK>(h, a, st);
+    case 32: return launch_tiles_as<32, BACK>(h, a, st);
+    case 64: return launch_tiles_as<64, BACK>(h, a, st);
+    default: return launch_tiles_as<128, BACK>(h, a, st);
+  }
+}
+int launch_direct(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
+  switch (padded_rank(a.rank)) {
+    case 16: return launch_direct_as<16>(h, a, st);
+    case 32: return launch_direct_as<32>(h, a, st);
+    case 64: return launch_direct_as<64>(h, a, st);
+    default: return launch_direct_as<128>(h, a, st);
   }
 }
 template <int NT, int NG>
@@ -784,7 +1020,7 @@ int launch_adapter_grad_as(const Handle* h, const AdapterGradArgs& a, int64_t jo
   constexpr size_t smem = 256 * (NT * NG * 8 + 1) * sizeof(float);
   static bool done[64];
   if (int rc = allow_smem(h, adapter_grad_kernel<NT, NG>, smem, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_grad_kernel<NT, NG>, jobs, cs, smem, st, a));
+  MG_CUDA(launch_clusters(adapter_grad_kernel<NT, NG>, jobs, cs, kAdapterThreads, smem, st, a));
   return MG_OK;
 }
 
@@ -815,8 +1051,9 @@ int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* coun
   return MG_OK;
 }
 
-static AdapterArgs adapter_args(const mg_adapters* d, int64_t rows, const int32_t* ids, const void* plan) {
+static AdapterArgs adapter_args(const Handle* h, const mg_adapters* d, int64_t rows, const int32_t* ids, const void* plan) {
   AdapterArgs a{};
+  a.status = h->d_status;
   a.scale = d->d_scale;
   a.factor = d->factor;
   a.rank = d->rank;
@@ -835,26 +1072,26 @@ static AdapterArgs adapter_args(const mg_adapters* d, int64_t rows, const int32_
 
 int launch_adapter_add(const Handle* h, const mg_adapters* d, const void* x, int64_t ldx, const void* y, int64_t ldy, int64_t rows,
                        const int32_t* ids, const void* plan, void* out, int64_t ldo, void* s, cudaStream_t st) {
-  AdapterArgs a = adapter_args(d, rows, ids, plan);
+  AdapterArgs a = adapter_args(h, d, rows, ids, plan);
   a.x = static_cast<const uint16_t*>(x); a.ldx = ldx; a.K = static_cast<int>(d->cols);
   a.w1 = static_cast<const uint16_t*>(d->d_down); a.g1 = d->down_stride; a.ld1 = d->ld_down;
   a.w2 = static_cast<const uint16_t*>(d->d_up); a.g2 = d->up_stride; a.ld2 = d->ld_up;
   a.y = static_cast<const uint16_t*>(y); a.ldy = ldy;
   a.out = static_cast<uint16_t*>(out); a.ldo = ldo; a.N = static_cast<int>(d->n_out);
   a.s = static_cast<uint16_t*>(s);
-  return launch_adapter_rank<false>(h, a, st);
+  return plan != nullptr ? launch_tiles<false>(h, a, st) : launch_direct(h, a, st);
 }
 
 int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout, int64_t ldg, const void* x, int64_t ldx, int64_t rows,
                         const void* plan, const void* s, void* gs, void* gx, int64_t ldgx, void* gdown, void* gup, cudaStream_t st) {
-  AdapterArgs a = adapter_args(d, rows, nullptr, plan);
+  AdapterArgs a = adapter_args(h, d, rows, nullptr, plan);
   a.x = static_cast<const uint16_t*>(gout); a.ldx = ldg; a.K = static_cast<int>(d->n_out);
   a.w1 = static_cast<const uint16_t*>(d->d_up); a.g1 = d->up_stride; a.ld1 = d->ld_up;
   a.w2 = static_cast<const uint16_t*>(d->d_down); a.g2 = d->down_stride; a.ld2 = d->ld_down;
   a.out = static_cast<uint16_t*>(gx); a.ldo = ldgx; a.N = gx != nullptr ? static_cast<int>(d->cols) : 0;
   a.s = static_cast<uint16_t*>(gs);
   if (gx != nullptr || gdown != nullptr)
-    if (int rc = launch_adapter_rank<true>(h, a, st)) return rc;
+    if (int rc = launch_tiles<true>(h, a, st)) return rc;
   if (gdown == nullptr && gup == nullptr) return MG_OK;
   AdapterGradArgs b{};
   b.wide[0] = static_cast<const uint16_t*>(gout); b.ldw[0] = ldg; b.cols[0] = static_cast<int>(d->n_out);
