@@ -25,41 +25,6 @@ __device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uin
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
-// rows that are read once: not kept in L1, where the adapters are
-__device__ __forceinline__ uint4 ld_once(const uint16_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-// W 32-bit words of a row from element c on; what lies at `end` or behind is 0 and not read.  Rows begin on 16-byte boundaries.
-template <int W>
-__device__ __forceinline__ void load_words(const uint16_t* row, int c, int end, uint32_t* v) {
-  if (c + 2 * W <= end) {
-    if (W == 1) v[0] = __ldg(reinterpret_cast<const uint32_t*>(row + c));
-    else if (W == 2) {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(row + c));
-      v[0] = u.x; v[W - 1] = u.y;
-    } else {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + c));
-      v[0] = u.x; v[1 % W] = u.y; v[2 % W] = u.z; v[3 % W] = u.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      v[i] = 0u;
-      if (c + 2 * i < end) v[i] = __ldg(row + c + 2 * i);
-      if (c + 2 * i + 1 < end) v[i] |= static_cast<uint32_t>(__ldg(row + c + 2 * i + 1)) << 16;
-    }
-  }
-}
-__device__ __forceinline__ uint4 load_tail(const uint16_t* row, int c, int end) {
-  uint32_t v[4];
-  load_words<4>(row, c, end, v);
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-
 // BYTES of a row from element c on, into shared memory; what lies at `end` or behind arrives as zeros and is not read.  Rows begin on
 // 16-byte boundaries.
 template <int BYTES>
@@ -83,11 +48,6 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
   return v;
 }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -428,7 +388,7 @@ __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t outer_byt
   return (make_smem_desc(saddr) & ~(0x3FFFull << 16)) | static_cast<uint64_t>(outer_bytes >> 4) << 16;
 }
 __host__ __device__ constexpr uint32_t mma_shape(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n) >> 3 << 17) | (8u << 24); }
-constexpr uint32_t kRowsB = 1u << 16;           // operand B by rows_desc
+constexpr uint32_t kRowsA = 1u << 15, kRowsB = 1u << 16;        // operand A, B by rows_desc
 
 template <int RP, bool BACK>
 __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_tile_kernel(const AdapterArgs a) {
@@ -716,113 +676,195 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 }
 
 // ---- gradients of the adapters ---------------------------------------------------------------
-// Both are W[c][r] = sum over an adapter's rows of wide[t][c] * narrow[t][r]: rows of gout and s, of x and gs.  A block holds 256
-// columns of one adapter for all of the rank and goes through the rows, which a cluster's blocks take in turn; the sums meet in
-// shared memory in a fixed order.  The wide rows are read once.
+// Both are W[c][r] = sum over an adapter's rows t of wide[t][c] * narrow[t][r]: rows of gout and s, of x and gs.  A block holds 128
+// columns c of one adapter on the accumulator's lanes, for all of the rank, and goes through the rows 64 at a time (a cluster's blocks in
+// turn, where there are few blocks); the inner index is the rows', so both operands are read as they lie.  The blocks' sums meet in a fixed
+// order.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
-  int cols[2], blocks[2];       // columns, and blocks of 256 of them
+  int cols[2], blocks[2];       // columns, and blocks of 128 of them
   const uint16_t* narrow[2];    // [n_rows][RP]
-  uint16_t* out[2];             // [adapters][cols][rank], [adapters][rank][cols]; nullptr: not wanted
+  uint16_t* out[2];             // [adapters][cols][rank], [adapters][rank][cols]
   const float* scale;
   float factor;
   int rank;
   const int2* segs;             // first entry of order and rows of every adapter
   const int32_t* order;
+  int32_t* status;
 };
 
-template <int NT, int NG>
-__global__ void __launch_bounds__(kAdapterThreads, NT >= 8 ? 1 : 2) adapter_grad_kernel(const AdapterGradArgs a) {
-  constexpr int RP = NT * NG * 8, PITCH = RP + 1, RGS = 2 / NG;
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* buf = reinterpret_cast<float*>(smem);       // [256 columns][PITCH]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, q = lane & 3;
+template <int RP>
+struct GradCfg {
+  static constexpr int BLOCKS = 2, STAGES = RP <= 64 ? 4 : 3;
+  static constexpr int WIDE = 16384;                           // bytes of a stage: two blocks of 64 columns by 64 rows, then the narrow rows
+  static constexpr int STAGE = WIDE + (RP <= 64 ? 8192 : 16384);
+  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + 1024;
+  static constexpr int COLS = 128;                             // of tensor memory
+  static_assert(128 * RP * 4 <= STAGES * STAGE && BLOCKS * (SMEM + 1536) <= 227 * 1024, "shared memory");
+};
+
+template <int RP>
+__global__ void __launch_bounds__(kTileThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
+  using C = GradCfg<RP>;
+  constexpr int S = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t s_full[S], s_done[S];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quarter = warp & 3, side = warp >> 2;
   const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
   const int job = blockIdx.x / cs, per = a.blocks[0] + a.blocks[1];
-  const int g = job / per, which = job % per >= a.blocks[0], cb = job % per - (which ? a.blocks[0] : 0);
+  const int g = job / per, block = job % per;
+  const bool which = block >= a.blocks[0];
+  const int c0 = (block - (which ? a.blocks[0] : 0)) * 128, cols = which ? a.cols[1] : a.cols[0];
   const int2 seg = a.segs[g];
-  const int live = seg.y, cols = which ? a.cols[1] : a.cols[0];
-  const int cg = warp & 3, other = warp >> 2, ng = NG == 2 ? other : 0, rg = NG == 2 ? 0 : other;
-  const int c = cb * 256 + cg * 64 + i * 8, r0 = ng * NT * 8 + i * NT;
-  const uint16_t* wide = which ? a.wide[1] : a.wide[0];
-  const uint16_t* narrow = which ? a.narrow[1] : a.narrow[0];
-  const int64_t ldw = which ? a.ldw[1] : a.ldw[0];
-  float acc[4][NT][4];
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][t][e] = 0.f;
-  const int step = RGS * cs * 16;
-  auto row_of = [&](int t) { return t < live ? a.order[seg.x + t] : -1; };
-  int rows[4];
-  int t0 = (rg + RGS * cr) * 16;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) rows[e] = row_of(t0 + 4 * q + e);
-  for (; t0 < live; t0 += step) {
-    uint4 v[4];
-    uint32_t w[4][NT / 2];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t row = rows[e];
-      v[e] = make_uint4(0u, 0u, 0u, 0u);
-      if (row >= 0) v[e] = c + 8 <= cols ? ld_once(wide + row * ldw + c) : load_tail(wide + row * ldw, c, cols);
-      load_words<NT / 2>(narrow + (row >= 0 ? row : 0) * RP, r0, row >= 0 ? RP : 0, w[e]);
+  const int live = seg.y;
+  const int64_t stride = static_cast<int64_t>(a.rank) * cols;
+  uint16_t* out = (which ? a.out[1] : a.out[0]) + g * stride;
+  if (live == 0) {                                     // the whole cluster
+    for (int e = cr * kTileThreads + tid; e < 128 * a.rank; e += cs * kTileThreads) {
+      const int c = c0 + (which ? e % 128 : e / a.rank), r = which ? e / 128 : e % a.rank;
+      if (c < cols) out[which ? r * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r] = 0;
     }
+    return;
+  }
+  if (tid == 0) {
+    for (int k = 0; k < S; ++k) { mbar_init(smem_u32(&s_full[k]), kAdapterThreads / 32); mbar_init(smem_u32(&s_done[k]), 1); }
+    s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(C::COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  const int all = (live + 63) / 64, steps = cr < all ? (all - cr + cs - 1) / cs : 0;       // steps cr, cr + cs, ...
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+
+  if (warp == 8) {
+    if (elect_one())
+      for (int k = 0; k < steps; ++k) {
+        mbar_wait(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 123);
+        tc_fence_after();
+        const uint32_t at = ring + k % S * C::STAGE;
+        const uint64_t da = rows_desc(at, 8192), db = rows_desc(at + C::WIDE, 8192);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) rows[e] = row_of(t0 + step + 4 * q + e);
+        for (int j = 0; j < 4; ++j) tc_mma_bf16(tmem, da + 128 * j, db + 128 * j, mma_shape(RP) | kRowsA | kRowsB, k + j > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&s_done[k % S]));
+      }
+    __syncwarp();
+  } else {
+    const uint16_t* wide = which ? a.wide[1] : a.wide[0];
+    const uint16_t* narrow = which ? a.narrow[1] : a.narrow[0];
+    const int64_t ldw = which ? a.ldw[1] : a.ldw[0];
+    const int r0 = tid >> 3, p = tid & 7;              // this thread's 16 bytes of rows r0 and r0 + 32, of 128 bytes each
+    const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
+    int rows[2];
+    auto look = [&](int k) {                           // rows of step k
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint32_t b0 = t % 2 ? highs(w[0][t / 2], w[1][t / 2]) : lows(w[0][t / 2], w[1][t / 2]);
-      const uint32_t b1 = t % 2 ? highs(w[2][t / 2], w[3][t / 2]) : lows(w[2][t / 2], w[3][t / 2]);
+      for (int j = 0; j < 2; ++j) {
+        const int t = (cr + k * cs) * 64 + j * 32 + r0;
+        rows[j] = k < steps && t < live ? a.order[seg.x + t] : -1;
+      }
+    };
+    int ahead = 0;
+    uint32_t filling = ring;
+    look(0);
+    auto fetch = [&]() {                               // what lies behind the last row or column arrives as zeros
+      if (ahead < steps) {
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        auto word = [m](const uint4& u) { return m == 0 ? u.x : m == 1 ? u.y : m == 2 ? u.z : u.w; };
-        const uint32_t x0 = word(v[0]), x1 = word(v[1]), x2 = word(v[2]), x3 = word(v[3]);
-        mma_bf16(acc[m][t], lows(x0, x1), highs(x0, x1), lows(x2, x3), highs(x2, x3), b0, b1);
+        for (int j = 0; j < 2; ++j) {
+          const int64_t row = max(rows[j], 0);
+          const int c = c0 + p * 8, end = rows[j] >= 0 ? cols : 0;
+          const uint16_t* w = wide + row * ldw;
+          const uint16_t* n = narrow + row * RP;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) copy_row<16>(filling + mine + j * 4096 + b * 8192, w, c + b * 64, end);
+#pragma unroll
+          for (int b = 0; b < (RP <= 64 ? 1 : 2); ++b)
+            if (p < RP / 8) copy_row<16>(filling + C::WIDE + mine + j * 4096 + b * 8192, n, p * 8 + b * 64, rows[j] >= 0 ? RP : 0);
+        }
+        look(ahead + 1);
+      }
+      copies_commit();
+      ++ahead;
+      filling = filling == ring + (S - 1) * C::STAGE ? ring : filling + C::STAGE;
+    };
+    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 122); };
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k) fetch();
+    for (int k = 0; k < steps; ++k) {
+      copies_wait<S - 2>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s_full[k % S]));
+      if (k > 0) done(k - 1);
+      fetch();
+    }
+    if (steps > 0) done(steps - 1);
+    tc_fence_after();
+    const float scale = which ? 1.0f : a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f);
+    auto store8 = [&](int c, int r, float* v) {        // eight of the rank of one column
+      if (c >= cols) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= scale;
+      if (!which && r + 8 <= a.rank && a.rank % 8 == 0) {
+        *reinterpret_cast<uint4*>(out + static_cast<int64_t>(c) * a.rank + r) = pack8(v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (r + e < a.rank)
+            out[which ? (r + e) * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r + e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < RP / 2; k += 8) {
+      float v[8];
+      const int col = quarter * 32 + lane, r = side * (RP / 2) + k;
+      tc_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r, v);
+      if (steps == 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (cs == 1) {
+        store8(c0 + col, r, v);
+      } else {                                         // [groups of four of the rank][column]
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          st_shared(ring + ((r / 4 + e) * 128 + col) * 16,
+                    make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
       }
     }
-  }
-  // row i of m tile m is column 2m of the thread's eight, row i + 8 the one behind it
-  auto at = [&](int m, int t, int e) -> float& {
-    return buf[(cg * 64 + i * 8 + 2 * m + (e >> 1)) * PITCH + ng * NT * 8 + (2 * q + (e & 1)) * NT + t];
-  };
-  if (rg == 1)
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) at(m, t, e) = acc[m][t][e];
-  __syncthreads();
-  if (rg == 0)
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) at(m, t, e) = RGS == 2 ? acc[m][t][e] + at(m, t, e) : acc[m][t][e];
-  if (cs > 1) cluster_sync_all();
-  else __syncthreads();
-  const float scale = which ? 1.0f : a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f);
-  uint16_t* out = (which ? a.out[1] : a.out[0]) + static_cast<int64_t>(g) * a.rank * cols;
-  const int mine = 256 / cs, first = cr * mine;
-  for (int e = tid; e < mine * a.rank; e += kAdapterThreads) {
-    const int col = first + (which ? e % mine : e / a.rank), r = which ? e / mine : e % a.rank;
-    if (cb * 256 + col >= cols) continue;
-    float v = 0.f;
     if (cs > 1) {
-      const uint32_t p = smem_u32(buf + col * PITCH + r);
-      for (int k = 0; k < cs; ++k) v += ld_cluster_f32(map_to_cta(p, k));
-    } else {
-      v = buf[col * PITCH + r];
+      cluster_sync_all();
+      const int share = 128 / cs;
+      for (int q = tid; q < share * RP / 8; q += kAdapterThreads) {
+        const int col = cr * share + q % share, r = q / share * 8;
+        float v[8];
+        const uint32_t at = ring + (r / 4 * 128 + col) * 16;
+        if (cs == 8) cluster_sum8<8>(at, 128 * 16, v);
+        else if (cs == 4) cluster_sum8<4>(at, 128 * 16, v);
+        else cluster_sum8<2>(at, 128 * 16, v);
+        store8(c0 + col, r, v);
+      }
     }
-    const int64_t cc = cb * 256 + col;
-    out[which ? r * static_cast<int64_t>(cols) + cc : cc * a.rank + r] = __bfloat16_as_ushort(__float2bfloat16_rn(live > 0 ? scale * v : 0.f));
+    copies_wait<0>();
   }
-  if (cs > 1) cluster_sync_all();                    // no block leaves while another reads its sums
+  if (cs > 1) {                                        // no block leaves while another reads its sums
+    if (warp == 8) cluster_sync_all();
+    cluster_sync_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+  }
 }
 
 // ---- plans -----------------------------------------------------------------------------------
@@ -1015,12 +1057,11 @@ int launch_direct(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
     default: return launch_direct_as<128>(h, a, st);
   }
 }
-template <int NT, int NG>
-int launch_adapter_grad_as(const Handle* h, const AdapterGradArgs& a, int64_t jobs, int cs, cudaStream_t st) {
-  constexpr size_t smem = 256 * (NT * NG * 8 + 1) * sizeof(float);
+template <int RP>
+int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int64_t jobs, int cs, cudaStream_t st) {
   static bool done[64];
-  if (int rc = allow_smem(h, adapter_grad_kernel<NT, NG>, smem, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_grad_kernel<NT, NG>, jobs, cs, kAdapterThreads, smem, st, a));
+  if (int rc = allow_smem(h, adapter_grad_kernel<RP>, GradCfg<RP>::SMEM, done)) return rc;
+  MG_CUDA(launch_clusters(adapter_grad_kernel<RP>, jobs, cs, kTileThreads, GradCfg<RP>::SMEM, st, a));
   return MG_OK;
 }
 
@@ -1098,21 +1139,22 @@ int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout,
   b.narrow[0] = static_cast<const uint16_t*>(s); b.out[0] = static_cast<uint16_t*>(gup);
   b.wide[1] = static_cast<const uint16_t*>(x); b.ldw[1] = ldx; b.cols[1] = static_cast<int>(d->cols);
   b.narrow[1] = static_cast<const uint16_t*>(gs); b.out[1] = static_cast<uint16_t*>(gdown);
-  for (int i = 0; i < 2; ++i) b.blocks[i] = b.out[i] != nullptr ? (b.cols[i] + 255) / 256 : 0;
+  for (int i = 0; i < 2; ++i) b.blocks[i] = b.out[i] != nullptr ? (b.cols[i] + 127) / 128 : 0;
+  b.status = h->d_status;
   b.scale = a.scale;
   b.factor = a.factor;
   b.rank = a.rank;
   b.order = a.order;
   b.segs = reinterpret_cast<const int2*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
   const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);
-  // rows of an adapter shared among blocks while each has two steps of 64 rows, were all adapters alike
+  // an adapter's rows among several blocks where there are few blocks, while each has two steps, were all adapters alike
   int cs = 8;
-  while (cs > 1 && rows / d->n_adapters < 128 * cs) cs /= 2;
+  while (cs > 1 && (rows / d->n_adapters < 128 * cs || jobs * cs > 4 * GradCfg<16>::BLOCKS * h->sm_count)) cs /= 2;
   switch (padded_rank(a.rank)) {
-    case 16: return launch_adapter_grad_as<2, 1>(h, b, jobs, cs, st);
-    case 32: return launch_adapter_grad_as<4, 1>(h, b, jobs, cs, st);
-    case 64: return launch_adapter_grad_as<8, 1>(h, b, jobs, cs, st);
-    default: return launch_adapter_grad_as<8, 2>(h, b, jobs, cs, st);
+    case 16: return launch_grad_as<16>(h, b, jobs, cs, st);
+    case 32: return launch_grad_as<32>(h, b, jobs, cs, st);
+    case 64: return launch_grad_as<64>(h, b, jobs, cs, st);
+    default: return launch_grad_as<128>(h, b, jobs, cs, st);
   }
 }
 
