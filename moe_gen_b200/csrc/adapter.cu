@@ -98,6 +98,8 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& high, uin
   high = *reinterpret_cast<const uint32_t*>(&h);
   low = *reinterpret_cast<const uint32_t*>(&l);
 }
+// two warps wait for one another
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(pair + 1) : "memory"); }
 template <int N>
 __device__ __forceinline__ uint32_t word_of(const uint4 (&v)[N], int w) {      // w is a constant wherever this is inlined
   const uint4& u = v[w / 4];
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
   __shared__ int s_abort;
   __shared__ int s_rows[kAdapterTile];
   const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u, s_at = ring + S * C::STAGE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane >> 2, quarter = warp & 3, side = warp >> 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quarter = warp & 3, side = warp >> 2;
   const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
   const int4 job = a.tiles[blockIdx.x / cs];
   const int g = job.x, live = job.z, len = job.w;
@@ -465,16 +467,18 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     const bool in_place = a.y == a.out && a.ldy == a.ldo, filled = a.rank == RP;
     const uint16_t* w1 = a.w1 + (g >= 0 ? g * a.g1 : 0);
     const uint16_t* w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
-    // A warp copies, finishes and stores 32 rows by 64 bytes of a tile: this thread 16 bytes of rows i, i + 8, i + 16 and i + 24 of them.
-    // Rows that are not there are the last one again, and not stored.
-    const int piece = side * 4 + (lane & 3);
-    const uint32_t mine = (quarter * 32 + i) * 128 + ((piece ^ i) << 4);         // in a tile of rows; 1024 bytes to the next one
+    // A warp copies and stores 16 rows of a tile: this thread 16 bytes of every fourth of them.  (128 bytes of a row side by side: with 64, the
+    // load and store unit was what 8192 rows of 4096 x 4096 waited for.)  Rows that are not there are the last one again, and not stored.
+    // Outputs are finished by rows to a lane, 64 bytes to a warp, so that two warps share 32 rows.
+    const int first_row = quarter * 32 + side * 16, piece = lane & 7;
+    const uint32_t mine = (first_row + (lane >> 3)) * 128;
+    auto mine_at = [&](int j) { return mine + j * 512 + ((piece ^ (lane >> 3) ^ ((j & 1) << 2)) << 4); };
     const uint16_t *xp[4], *yp[4];
     uint16_t* op[4];
     uint32_t stored = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int r = quarter * 32 + j * 8 + i;
+      const int r = first_row + j * 4 + (lane >> 3);
       const int64_t row = s_rows[min(r, len - 1)];
       xp[j] = a.x + (live > 0 ? static_cast<int64_t>(s_rows[min(r, live - 1)]) : 0) * a.ldx + piece * 8;
       yp[j] = a.y + row * a.ldy + piece * 8;
@@ -527,13 +531,13 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
         const bool first = ahead < n1;
         const int c = (first ? lo1 + ahead : lo2 + ahead - n1) * 64, n = first ? a.K : a.N;
         const bool inside = c + 64 <= n;
-        if (first ? quarter * 32 < live : !BACK && quarter * 32 < len) {
+        if (first ? first_row < live : !BACK && first_row < len) {
           if (inside) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) copy_whole(filling + mine + j * 1024, (first ? xp[j] : yp[j]) + c);
+            for (int j = 0; j < 4; ++j) copy_whole(filling + mine_at(j), (first ? xp[j] : yp[j]) + c);
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) copy_row<16>(filling + mine + j * 1024, (first ? xp[j] : yp[j]) - piece * 8, c + piece * 8, n);
+            for (int j = 0; j < 4; ++j) copy_row<16>(filling + mine_at(j), (first ? xp[j] : yp[j]) - piece * 8, c + piece * 8, n);
           }
         }
         if (live > 0) fetch_adapter(filling, c, first, inside && filled);
@@ -627,10 +631,11 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       for (int k = 0; k < S - 1; ++k) fetch(steps);
     }
 
-    // finishes unit m in the place of y, from where the warp stores 64 bytes of eight rows at a time
+    // finishes unit m in the place of y, from where the warps store 128 bytes of four rows at a time
     auto finish = [&](int m) {
       const uint32_t at = ring + (n1 + m) % S * C::STAGE;
       const int c0 = (lo2 + m) * 64, row = quarter * 32 + lane;
+      pair_sync(quarter);                              // the other warp's copies too
       if (live > 0) {
         done(n1 + m);
         tc_fence_after();
@@ -651,10 +656,10 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
           else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
         }
       }
-      __syncwarp();
+      pair_sync(quarter);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u) : ld_shared(at + mine + j * 1024);
+        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u) : ld_shared(at + mine_at(j));
         if (stored >> j & 1u) store_row(op[j] + c0, 0, a.N - c0 - piece * 8, v);
       }
     };
