@@ -552,8 +552,9 @@ int mg_moe_block_forward(mg_handle h, const void* d_hidden, const void* d_norm_w
  *     grad_x = rstd * (weight grad_y - n mean(weight grad_y n)) + grad_h,   grad_w[cols] = sum over rows of grad_y n  (fp32)
  *   grad_x is the gradient of x and of the residual alike.  d_grad_h, which reaches h by other ways, may be NULL; d_grad_x or
  *   d_grad_w may be NULL and is then not computed; d_grad_x may be d_grad_y or d_grad_h with its stride.  At most 16384 columns.
- *   d_ws: scratch of mg_add_rmsnorm_grad_ws_bytes bytes on a 4-byte boundary, for grad_w only.  The same rows, columns and device give
- *   the same bits. */
+ *   d_ws: scratch of mg_add_rmsnorm_grad_ws_bytes bytes on a 4-byte boundary, for grad_w only (0 bytes up to MG_NORM_GRAD_FEW rows,
+ *   which one launch takes: d_ws may be NULL then).  The same rows, columns and device give the same bits. */
+#define MG_NORM_GRAD_FEW 64
 int mg_moe_block_forward_add(mg_handle h, const void* d_hidden, const void* d_residual, const void* d_norm_weight, float eps,
                              int64_t n_tokens, const void* d_gate_w, const float* d_bias, const void* d_packed, void* d_xnorm,
                              void* d_workspace, size_t workspace_bytes, void* d_out, void* stream);

@@ -48,11 +48,6 @@ __device__ __forceinline__ uint4 ld_shared(uint32_t at) {
   return v;
 }
 
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ void st_shared(uint32_t at, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -124,12 +119,6 @@ __device__ __forceinline__ void tc_ld8(uint32_t taddr, float* v) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[e]);
 }
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
 struct AdapterArgs {
   const uint16_t* x;          // rows of the first product, K elements
   int64_t ldx;
@@ -998,38 +987,12 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
 
 int padded_rank(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
-template <typename... P, typename... A>
-cudaError_t launch_clusters(void (*kernel)(P...), int64_t jobs, int cs, int threads, size_t smem, cudaStream_t st, A&&... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cs;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(jobs * cs));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
-}
-
-// a kernel's dynamic shared memory above the default, once to a device
-template <typename K>
-int allow_smem(const Handle* h, K* kernel, size_t smem, bool (&done)[64]) {
-  const bool known = h->device >= 0 && h->device < 64;
-  if (known && done[h->device]) return MG_OK;
-  MG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  if (known) done[h->device] = true;
-  return MG_OK;
-}
-
 template <int RP>
 int launch_direct_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   static bool done[64];
   if (int rc = allow_smem(h, adapter_direct_kernel<RP>, DirectCfg<RP>::SMEM, done)) return rc;
   int cs = 8;
-  while (cs > 2 && static_cast<int64_t>(a.n_rows) * cs > 4 * h->sm_count) cs /= 2;
+  while (cs > 2 && static_cast<int64_t>(a.n_rows) * cs > 8 * h->sm_count) cs /= 2;
   MG_CUDA(launch_clusters(adapter_direct_kernel<RP>, a.n_rows, cs, kAdapterThreads, DirectCfg<RP>::SMEM, st, a));
   return MG_OK;
 }

@@ -1527,10 +1527,10 @@ int mg_add_rmsnorm_grad(mg_handle hh, const void* d_gy, int64_t ldgy, const void
   MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_add_rmsnorm_grad: negative eps");
   MG_REQUIRE(d_gx || d_gw, MG_ERR_NULL, "mg_add_rmsnorm_grad: no gradient asked for");
   if (n_rows > 0) {
-    MG_REQUIRE(d_gy && d_h && d_weight && (d_gw == nullptr || d_ws), MG_ERR_NULL, "mg_add_rmsnorm_grad: null pointer");
+    const size_t need = norm_grad_ws_bytes(h, n_rows, cols);
+    MG_REQUIRE(d_gy && d_h && d_weight && (d_gw == nullptr || d_ws || need == 0), MG_ERR_NULL, "mg_add_rmsnorm_grad: null pointer");
     MG_REQUIRE((d_gx != d_gy || ldgx == ldgy) && (d_gx != d_gh || d_gh == nullptr || ldgx == ldgh) && d_gx != d_h, MG_ERR_CONFIG,
                "mg_add_rmsnorm_grad: grad_x lies otherwise than the gradient that it replaces, or over h");
-    const size_t need = norm_grad_ws_bytes(h, n_rows, cols);
     MG_REQUIRE(d_gw == nullptr || ws_bytes >= need, MG_ERR_WORKSPACE, "mg_add_rmsnorm_grad: workspace %zu bytes, need %zu", ws_bytes, need);
     MG_REQUIRE(d_gw == nullptr || reinterpret_cast<uintptr_t>(d_ws) % 4 == 0, MG_ERR_SHAPE,
                "mg_add_rmsnorm_grad: the workspace must begin on a 4-byte boundary");

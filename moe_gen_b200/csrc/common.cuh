@@ -163,6 +163,32 @@ inline cudaError_t launch_chained(const Handle* h, void (*kernel)(P...), dim3 gr
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// jobs of cs blocks each, a cluster to a job
+template <typename... P, typename... A>
+inline cudaError_t launch_clusters(void (*kernel)(P...), int64_t jobs, int cs, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cs;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(jobs * cs));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+// a kernel's dynamic shared memory above the default, once to a device
+template <typename K>
+inline int allow_smem(const Handle* h, K* kernel, size_t smem, bool (&done)[64]) {
+  const bool known = h->device >= 0 && h->device < 64;
+  if (known && done[h->device]) return MG_OK;
+  MG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  if (known) done[h->device] = true;
+  return MG_OK;
+}
+
 static inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // packed weight buffer offsets (bytes) ------------------------------------------------

@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs
 // With n = h * rstd (the forward's roundings count as the identity):
 //   gx = rstd * (w gy - n mean(w gy n)) + gh,   gw = sum over rows of gy n
 // mean(w gy n) = rstd sum(w gy h) / cols, so that both sums of a row come from one reading.  Blocks stay and take rows in turn; a
-// thread holds the same columns of every row, and its share of gw in fp32.  The shares are summed by a second launch, in the
-// order of the blocks: the same rows and columns give the same bits.
+// thread holds the same columns of every row, and its share of gw in fp32.  The shares are summed by a second launch, in the order of
+// the blocks, or, few rows, in the same one by a cluster's blocks, so that the same rows and columns give the same bits.
 struct NormGradArgs {
   const uint16_t* gy;
   int64_t ldgy;
@@ -316,7 +316,8 @@ struct NormGradArgs {
   int64_t ldgh;
   uint16_t* gx;              // nullptr: not wanted
   int64_t ldgx;
-  float* parts;              // [shares][cols], nullptr: gw is not wanted
+  float* parts;              // [shares][cols], nullptr: gw is not wanted, or
+  float* gw;                 // summed here, by one cluster
   int lanes;                 // threads to a row
 };
 constexpr int kGradThreads = 1024, kGradMaxCols = 2 * 8 * kGradThreads;      // up to two vectors of a row to a thread
@@ -347,9 +348,17 @@ __device__ __forceinline__ void copy_vec(uint4* to, const uint16_t* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
 
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // WIDE: rows of whole 16-byte vectors, several of them on their way to shared memory at a time.  A thread copies what it reads itself, so
 // that it waits for its own copies only.
-template <int VECS, bool WIDE>
+// FEW: the grid is one cluster, which sums the shares too.
+template <int VECS, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGradArgs a) {
   constexpr int STAGES = kGradStages<VECS>;
   extern __shared__ __align__(16) uint4 s_rows[];                // [stage][h, gy, gh][vector][thread]
@@ -466,6 +475,31 @@ __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGr
     }
     if (++stage == STAGES) stage = 0;
   }
+  if (FEW) {
+    if (a.gw == nullptr) return;
+    float* part = reinterpret_cast<float*>(s_rows);              // [rows][cols], where the ring is
+    copies_done();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VECS; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int c = (t + i * lanes) * 8 + j;
+        if (c < a.cols) part[sub * a.cols + c] = j & 1 ? acc[i][j >> 1].y : acc[i][j >> 1].x;
+      }
+    cluster_sync_all();
+    const int blocks = static_cast<int>(gridDim.x);
+    for (int c = blockIdx.x * blockDim.x + threadIdx.x; c < a.cols; c += blocks * blockDim.x) {
+      float v = 0.f;
+      for (int k = 0; k < blocks; ++k) {
+        const uint32_t there = map_to_cta(smem_u32(part + c), k);
+        for (int r = 0; r < rows; ++r) v += ld_cluster_f32(there + r * a.cols * 4);
+      }
+      a.gw[c] = v;
+    }
+    cluster_sync_all();              // no block leaves while another reads its share
+    return;
+  }
   if (a.parts == nullptr) return;
   float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * rows + sub) * a.cols;
 #pragma unroll
@@ -490,7 +524,9 @@ __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* parts,
   if (x == 0 && blockIdx.x * 32 + y < cols) gw[blockIdx.x * 32 + y] = v;
 }
 
-struct NormGradPlan { int vecs, lanes, threads, blocks, shares; };
+// us in a graph, and on their way from Python, by two launches and by one: 1 row of 2048 columns X
+constexpr int kGradCluster = 8;
+struct NormGradPlan { int vecs, lanes, threads, blocks, shares; bool few; };
 NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
   NormGradPlan p;
   const int vecs = static_cast<int>((cols + 7) / 8);
@@ -499,8 +535,9 @@ NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
   p.threads = p.lanes >= 256 ? p.lanes : 256 / p.lanes * p.lanes;
   const int rows = p.threads / p.lanes;
   const int64_t want = (n + rows - 1) / rows, most = static_cast<int64_t>(h->sm_count) * (p.threads > 512 ? 1 : p.threads > 256 ? 2 : 4);
-  p.blocks = static_cast<int>(want < most ? want : most);
-  p.shares = p.blocks * rows;
+  p.few = n <= MG_NORM_GRAD_FEW;
+  p.blocks = p.few ? kGradCluster : static_cast<int>(want < most ? want : most);
+  p.shares = p.few ? 0 : p.blocks * rows;
   return p;
 }
 
@@ -523,25 +560,21 @@ int launch_add_norm_as(const NormArgs& a, cudaStream_t st) {
   return MG_OK;
 }
 
-template <int VECS>
-int launch_norm_grad_as(const Handle* h, const NormGradArgs& a, const NormGradPlan& p, bool wide, float* gw, cudaStream_t st) {
-  if (wide) {
-    const size_t smem = static_cast<size_t>(p.threads) * kGradStages<VECS> * 3 * VECS * sizeof(uint4);
+template <int VECS, bool WIDE>
+int launch_norm_grad_as(const Handle* h, const NormGradArgs& a, const NormGradPlan& p, cudaStream_t st) {
+  const size_t ring = WIDE ? static_cast<size_t>(p.threads) * kGradStages<VECS> * 3 * VECS * sizeof(uint4) : 0;
+  constexpr size_t most = kGradThreads * kGradStages<VECS> * 3 * VECS * sizeof(uint4);
+  if (p.few) {
+    const size_t part = static_cast<size_t>(p.threads / p.lanes) * a.cols * sizeof(float);
     static bool done[64];
-    if (!(h->device >= 0 && h->device < 64 && done[h->device])) {
-      MG_CUDA(cudaFuncSetAttribute(norm_grad_kernel<VECS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   static_cast<int>(kGradThreads * kGradStages<VECS> * 3 * VECS * sizeof(uint4))));
-      if (h->device >= 0 && h->device < 64) done[h->device] = true;
-    }
-    norm_grad_kernel<VECS, true><<<p.blocks, p.threads, smem, st>>>(a);
-  } else {
-    norm_grad_kernel<VECS, false><<<p.blocks, p.threads, 0, st>>>(a);
+    if (int rc = allow_smem(h, norm_grad_kernel<VECS, WIDE, true>, most, done)) return rc;
+    MG_CUDA(launch_clusters(norm_grad_kernel<VECS, WIDE, true>, 1, p.blocks, p.threads, ring > part ? ring : part, st, a));
+    return MG_OK;
   }
+  static bool done[64];
+  if (int rc = allow_smem(h, norm_grad_kernel<VECS, WIDE, false>, most, done)) return rc;
+  norm_grad_kernel<VECS, WIDE, false><<<p.blocks, p.threads, ring, st>>>(a);
   MG_CUDA(cudaGetLastError());
-  if (gw != nullptr) {
-    norm_grad_sum_kernel<<<static_cast<unsigned>((a.cols + 31) / 32), 1024, 0, st>>>(a.parts, p.shares, a.cols, gw);
-    MG_CUDA(cudaGetLastError());
-  }
   return MG_OK;
 }
 
@@ -572,11 +605,15 @@ int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* 
   const NormGradPlan p = norm_grad_plan(h, n, cols);
   NormGradArgs a{static_cast<const uint16_t*>(gy), ldgy, static_cast<const uint16_t*>(hrows), ldh, static_cast<const uint16_t*>(w), eps, n,
                  static_cast<int>(cols), static_cast<const uint16_t*>(gh), ldgh, static_cast<uint16_t*>(gx), ldgx,
-                 gw != nullptr ? static_cast<float*>(ws) : nullptr, p.lanes};
+                 gw != nullptr && !p.few ? static_cast<float*>(ws) : nullptr, p.few ? gw : nullptr, p.lanes};
   const bool wide = cols % 8 == 0 && on16(gy, ldgy) && on16(hrows, ldh) && on16(w, 0) && (gh == nullptr || on16(gh, ldgh)) &&
                     (gx == nullptr || on16(gx, ldgx));
-  if (p.vecs == 1) return launch_norm_grad_as<1>(h, a, p, wide, gw, st);
-  return launch_norm_grad_as<2>(h, a, p, wide, gw, st);
+  const int rc = p.vecs == 1 ? (wide ? launch_norm_grad_as<1, true>(h, a, p, st) : launch_norm_grad_as<1, false>(h, a, p, st))
+                             : (wide ? launch_norm_grad_as<2, true>(h, a, p, st) : launch_norm_grad_as<2, false>(h, a, p, st));
+  if (rc != MG_OK || a.parts == nullptr) return rc;
+  norm_grad_sum_kernel<<<static_cast<unsigned>((cols + 31) / 32), 1024, 0, st>>>(a.parts, p.shares, static_cast<int>(cols), gw);
+  MG_CUDA(cudaGetLastError());
+  return MG_OK;
 }
 
 }  // namespace mg

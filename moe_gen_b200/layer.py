@@ -316,17 +316,18 @@ class MoELayer:
         if (ng, gcols) != (n, cols) or (nh, hcols) != (n, cols):
             raise ValueError(f"gradients of {(ng, gcols)} and {(nh, hcols)} for rows of {(n, cols)}")
         gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
-        gw = ws = None
-        size = C.c_size_t()
-        if need_w:
-            gw = torch.empty(cols, dtype=torch.float32, device=self.device)
-            L.check(self.lib.mg_add_rmsnorm_grad_ws_bytes(self._h, n, cols, C.byref(size)))
-            ws = torch.empty(size.value, dtype=torch.uint8, device=self.device)
         if not (need_x or need_w):
             return None, None
+        gw = torch.empty(cols, dtype=torch.float32, device=self.device) if need_w else None
+        ws, size = None, 0
+        if need_w and n > L.NORM_GRAD_FEW:
+            need = C.c_size_t()
+            L.check(self.lib.mg_add_rmsnorm_grad_ws_bytes(self._h, n, cols, C.byref(need)))
+            size = need.value
+            ws = torch.empty(size, dtype=torch.uint8, device=self.device)
         with self._on_device():
             L.check(self.lib.mg_add_rmsnorm_grad(self._h, grad_y.data_ptr(), ldgy, h.data_ptr(), ldh, weight.data_ptr(), eps, n, cols,
-                                                 _ptr(grad_h), ldgh, _ptr(gx), ldgx, _ptr(gw), _ptr(ws), size.value, self._stream()))
+                                                 _ptr(grad_h), ldgh, _ptr(gx), ldgx, _ptr(gw), _ptr(ws), size, self._stream()))
         return gx, gw
 
     def block_forward(self, hidden: torch.Tensor, norm_weight: torch.Tensor, eps: float = 1e-6,

@@ -41,6 +41,7 @@ class LayerDesc(C.Structure):
 
 
 ADAPTER_MAX, ADAPTER_DIRECT = 1024, 256
+NORM_GRAD_FEW = 64
 
 
 class Adapters(C.Structure):

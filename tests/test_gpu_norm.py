@@ -174,7 +174,7 @@ def _grad_ref(gy, h, w, eps, gh):
     return gx, mag, (gy * n).sum(dim=0), (gy * n).abs().sum(dim=0)
 
 
-@pytest.mark.parametrize("n,cols", [(1, 256), (1, 1), (37, 2048), (5, 7168), (300, 4096), (1000, 512), (777, 1000), (50, 1001), (601, 8192), (9, 8200),
+@pytest.mark.parametrize("n,cols", [(1, 256), (1, 1), (37, 2048), (5, 7168), (64, 8200), (65, 77), (64, 16384), (63, 40), (300, 4096), (1000, 512), (777, 1000), (50, 1001), (601, 8192), (9, 8200),
                                     (301, 16384), (3, 16383), (3000, 40), (2500, 256)])
 @pytest.mark.parametrize("with_h", (True, False))
 def test_gradients(layer, n, cols, with_h):
@@ -190,6 +190,27 @@ def test_gradients(layer, n, cols, with_h):
     assert torch.equal(layer.add_rmsnorm_grad(gy, h, w, 1e-6, gh, need_x=False)[1], gw)
     again = layer.add_rmsnorm_grad(gy, h, w, 1e-6, gh)
     assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
+
+
+@pytest.mark.parametrize("n", (64, 65))
+def test_scratch_of_the_gradient(layer, n):
+    """None up to 64 rows, refused where it is missing or too small beyond."""
+    import ctypes as C
+    from moe_gen_b200 import lib as L
+    assert L.NORM_GRAD_FEW == 64
+    x, w, gw, need = _rows(n, 512, 1), _weight(512, 2), torch.zeros(512, device=DEV), C.c_size_t()
+    assert layer.lib.mg_add_rmsnorm_grad_ws_bytes(layer._h, n, 512, C.byref(need)) == 0 and (need.value > 0) == (n > 64)
+    ws = torch.empty(max(need.value, 4), dtype=torch.uint8, device=DEV)
+
+    def call(ptr, size):
+        return layer.lib.mg_add_rmsnorm_grad(layer._h, x.data_ptr(), 512, x.data_ptr(), 512, w.data_ptr(), 1e-6, n, 512, None, 0, None, 0,
+                                             gw.data_ptr(), ptr, size, layer._stream())
+    if n > 64:
+        assert call(None, 0) == -1 and call(ws.data_ptr(), need.value - 1) == -4 and call(ws.data_ptr() + 2, need.value) == -2
+        assert call(ws.data_ptr(), need.value) == 0
+    else:
+        assert call(None, 0) == 0
+    assert torch.equal(gw, layer.add_rmsnorm_grad(x, x, w)[1])
 
 
 @pytest.mark.parametrize("ld,off", [(600, 0), (600, 8), (513, 0), (512, 1)])

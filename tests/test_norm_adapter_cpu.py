@@ -49,7 +49,7 @@ def test_quantised_norms_that_are_refused(handle, kw, code):
 @pytest.mark.parametrize("kw,code", [(dict(n=-1), -2), (dict(cols=0), -2), (dict(cols=16385, ldgy=16392, ldh=16392, ldgh=16392, ldgx=16392), -7),
                                      (dict(ldgy=63), -2), (dict(ldh=63), -2), (dict(ldgh=63), -2), (dict(ldgx=63), -2), (dict(eps=-1.0), -3),
                                      (dict(gx=None, gw=None), -1), (dict(gy=None), -1), (dict(h=None), -1), (dict(w=None), -1),
-                                     (dict(ws=None), -1), (dict(gx=P, ldgx=72), -3), (dict(gx=4 * P, ldgx=72), -3), (dict(gx=2 * P), -3)])
+                                     (dict(gx=P, ldgx=72), -3), (dict(gx=4 * P, ldgx=72), -3), (dict(gx=2 * P), -3)])
 def test_norm_gradients_that_are_refused(handle, kw, code):
     a = dict(gy=P, ldgy=64, h=2 * P, ldh=64, w=3 * P, eps=1e-6, n=4, cols=64, gh=4 * P, ldgh=64, gx=5 * P, ldgx=64, gw=6 * P, ws=7 * P)
     a.update(kw)
@@ -115,10 +115,10 @@ def test_plans_that_are_refused(handle):
 
 @pytest.mark.parametrize("rows,adapters", [(0, 1), (1, 1), (63, 3), (64, 4), (65, 1024), (100000, 7)])
 def test_a_plan_holds_its_tiles_segments_and_order(built_lib, rows, adapters):
-    """16 bytes to a tile of 64 rows or a part of one, for every adapter and for none, 8 to an adapter, 4 to a row."""
+    """16 bytes to a tile of 128 rows or a part of one, for every adapter and for none, 8 to an adapter, 4 to a row."""
     n = C.c_size_t()
     assert L.load().mg_adapter_plan_bytes(rows, adapters, C.byref(n)) == 0
-    assert n.value >= 16 * ((rows + 63) // 64 + adapters + 1) + 8 * adapters + 4 * rows
+    assert n.value >= 16 * ((rows + 127) // 128 + adapters + 1) + 8 * adapters + 4 * rows
 
 
 def test_adapters_struct_matches_the_header():
