@@ -111,6 +111,13 @@ __device__ __forceinline__ void store_row(uint16_t* row, int c, int n, const uin
       if (c + e < n) row[c + e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
   }
 }
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+  tc_ld_wait();
+}
 __device__ __forceinline__ void tc_ld8(uint32_t taddr, float* v) {
   uint32_t r[8];
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
@@ -357,22 +364,23 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
 }
 
 // ---- tiles of a plan ---------------------------------------------------------------------------
-// 128 rows of one adapter on the accumulator's lanes.  Eight warps copy the tiles of either product to shared memory as the tensor core reads
-// them, a few steps ahead (rows wherever the order says, zeros behind what a row or the rank has), and finish the outputs; a ninth has the
-// products done, into tensor memory.  A step is 64 columns of x, or 64 columns of out.  s passes through shared memory in two parts of
-// bf16, so that it has 16 bits of mantissa in the second product.  A cluster of up to eight blocks shares a tile where there are few: each sums
-// s over its columns of x, then over the blocks for its share of the rows, and hands that to all.
-constexpr int kTileThreads = kAdapterThreads + 32;
+// 128 rows of one adapter on the accumulator's lanes.  A step is 64 columns of x, or 64 columns of out; its tiles are copied to shared memory as
+// the tensor core reads them, a few steps ahead (rows wherever the order says, zeros behind what a row or the rank has).  Eight warps copy
+// the first product's, then finish s and the outputs, while four others copy the second product's; one has the products done, into tensor
+// memory.  s passes through shared memory in two parts of bf16, so that it has 16 bits of mantissa in the second product.  A cluster of up
+// to eight blocks shares a tile where there are few: each sums s over its columns of x, then over the blocks for its share of the rows, and
+// hands that to all.
+constexpr int kFinishWarps = 8, kCopyWarps = 4, kTileThreads = 32 * (kFinishWarps + kCopyWarps + 1);
 template <int RP>
 struct TileCfg {
   static constexpr int BLOCKS = RP <= 64 ? 2 : 1;              // per SM
-  static constexpr int STAGES = RP <= 64 ? 3 : 4;
+  static constexpr int STAGES = RP == 64 ? 3 : 4;
   static constexpr int ROWS = kAdapterTile * 128;              // bytes of a stage: the rows' tile, then the adapter's
   static constexpr int STAGE = ROWS + (RP <= 64 ? 8192 : 16384);
-  static constexpr int PART = ROWS * (RP <= 64 ? 1 : 2);       // either part of s: blocks of 64 columns
-  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + 2 * PART + 1024;
+  static constexpr int PART = RP <= 32 ? 64 : ROWS * (RP / 64);                  // from one part of s to the other: blocks of 64 columns, or half a row
+  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + (RP <= 32 ? ROWS : 2 * PART);
   static constexpr int COLS = 256, SECOND = 128;               // of tensor memory; the second product's two accumulators of 64
-  static_assert(kAdapterTile * RP * 4 <= STAGES * STAGE && BLOCKS * (SMEM + 2048) <= 227 * 1024, "shared memory");
+  static_assert(kAdapterTile * RP * 4 <= (RP <= 32 ? ROWS : 2 * PART) && BLOCKS * (SMEM + 2048) <= 228 * 1024, "shared memory");
 };
 // operand whose inner index goes over rows of 128 bytes (64 outer elements each), swizzled: 64 outer elements outer_bytes apart
 __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t outer_bytes) {
@@ -381,66 +389,150 @@ __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t outer_byt
 __host__ __device__ constexpr uint32_t mma_shape(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n) >> 3 << 17) | (8u << 24); }
 constexpr uint32_t kRowsA = 1u << 15, kRowsB = 1u << 16;        // operand A, B by rows_desc
 
+// What one of WARPS warps' threads copies of a step: 16 bytes of some rows of the tile of rows, 128 bytes of a row side by side (with 64 the load and
+// store unit was what 8192 rows of 4096 x 4096 waited for; rows that are not there are the last one again), and pieces of the adapter's tile,
+// RP rows of 64 elements (wide) or 64 rows of RP (narrow).
+// for the tensor core: this warp's copies but those of the last LEFT steps, and what it has written before
+template <int LEFT>
+__device__ __forceinline__ void arrive(uint64_t* full) {
+  copies_wait<LEFT>();
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(full));
+}
+template <int RP, bool BACK, int WARPS>
+struct TileCopies {
+  using C = TileCfg<RP>;
+  static constexpr int ROWS = WARPS * 4, EACH = kAdapterTile / ROWS;             // rows of an instruction of all warps, rows of a thread
+  static constexpr int PIECES = RP * 8 / (WARPS * 32) > 0 ? RP * 8 / (WARPS * 32) : 1, NARROW_ROWS = WARPS * 32 / (RP / 8);
+  const AdapterArgs& a;
+  const uint16_t *wide, *narrow;
+  int t;
+  const uint16_t* from[EACH];
+  __device__ TileCopies(const AdapterArgs& args, int g, int thread) : a(args), t(thread) {
+    const uint16_t *w1 = a.w1 + (g >= 0 ? g * a.g1 : 0), *w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
+    wide = BACK ? w2 : w1;
+    narrow = BACK ? w1 : w2;
+  }
+  __device__ __forceinline__ void rows_of(const uint16_t* base, int64_t ld, const int* rows, int n) {
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) from[j] = base + static_cast<int64_t>(rows[min((t >> 3) + j * ROWS, n - 1)]) * ld + (t & 7) * 8;
+  }
+  // into the stage at `to`: columns c to c + 63 of n of the first `rows` rows, and of the adapter
+  __device__ __forceinline__ void step(uint32_t to, bool first, int c, int n, int rows, bool adapter) const {
+    const int r0 = t >> 3, p = t & 7, first_row = t / 32 * 4;
+    const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
+    const bool inside = c + 64 <= n, filled = a.rank == RP;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+      if (first_row + j * ROWS < rows) {
+        if (inside) copy_whole(to + mine + j * ROWS * 128, from[j] + c);
+        else copy_row<16>(to + mine + j * ROWS * 128, from[j] - p * 8, c + p * 8, n);
+      }
+    if (!adapter || (RP * 8 < WARPS * 32 && t >= RP * 8)) return;
+    if (first != BACK) {
+      const int64_t ld = BACK ? a.ld2 : a.ld1;
+      if (inside && filled) {
+        const uint16_t* w = wide + r0 * ld + p * 8 + c;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j, w += ROWS * ld) copy_whole(to + C::ROWS + mine + j * ROWS * 128, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int r = r0 + j * ROWS;
+          copy_row<16>(to + C::ROWS + mine + j * ROWS * 128, wide + (r < a.rank ? r : 0) * ld, c + p * 8, r < a.rank ? n : 0);
+        }
+      }
+    } else {
+      const int64_t ld = BACK ? a.ld1 : a.ld2;
+      const int nr = t / (RP / 8), np = t % (RP / 8);
+      const uint32_t at = to + C::ROWS + (np >> 3) * 8192 + nr * 128 + (((np & 7) ^ (nr & 7)) << 4);
+      if (inside && filled) {
+        const uint16_t* w = narrow + (c + nr) * ld + np * 8;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j, w += NARROW_ROWS * ld) copy_whole(at + j * NARROW_ROWS * 128, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int r = c + nr + j * NARROW_ROWS;
+          copy_row<16>(at + j * NARROW_ROWS * 128, narrow + (r < n ? r : 0) * ld, np * 8, r < n ? a.rank : 0);
+        }
+      }
+    }
+  }
+};
+
 template <int RP, bool BACK>
 __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_tile_kernel(const AdapterArgs a) {
   using C = TileCfg<RP>;
   constexpr int S = C::STAGES;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_full[S], s_done[S];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint64_t s_full[S], s_done[S], s_empty[S], s_first, s_ready, s_met[3];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ int s_rows[kAdapterTile];
-  const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u, s_at = ring + S * C::STAGE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quarter = warp & 3, side = warp >> 2;
+  const uint32_t ring = smem_u32(smem_raw), s_at = ring + S * C::STAGE;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
   const int4 job = a.tiles[blockIdx.x / cs];
   const int g = job.x, live = job.z, len = job.w;
   if (len == 0) return;                                // the whole cluster
   if (tid < len) s_rows[tid] = a.order[job.y + tid];
   if (tid == 0) {
-    for (int k = 0; k < S; ++k) { mbar_init(smem_u32(&s_full[k]), kAdapterThreads / 32); mbar_init(smem_u32(&s_done[k]), 1); }
+    for (int k = 0; k < S; ++k) {
+      mbar_init(smem_u32(&s_full[k]), kFinishWarps);
+      mbar_init(smem_u32(&s_done[k]), 1);
+      mbar_init(smem_u32(&s_empty[k]), kFinishWarps);
+    }
+    mbar_init(smem_u32(&s_first), 1);
+    mbar_init(smem_u32(&s_ready), kFinishWarps);
+    for (int k = 0; k < 3; ++k) mbar_init(smem_u32(&s_met[k]), kFinishWarps * cs);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == kFinishWarps + kCopyWarps) {
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(C::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
   const int slices = live > 0 ? (a.K + 63) / 64 : 0, per = (slices + cs - 1) / cs;
   const int units = (a.N + 63) / 64, each = (units + cs - 1) / cs;
   const int lo1 = cr * per, n1 = max(min(slices, lo1 + per) - lo1, 0), lo2 = cr * each, n2 = max(min(units, lo2 + each) - lo2, 0);
-  const int steps = n1 + n2;
   tc_fence_before();
-  __syncthreads();
+  if (cs > 1) cluster_sync_all();                      // the other blocks' barriers are set up
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  // Steps are numbered through both products; step k fills stage k % S for the k / S-th time, and the m-th of the second product empties its stage
+  // for the m / S-th.
+  auto full = [&](int k) { return wait_warp(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 120); };
+  auto done = [&](int k) { return wait_warp(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 121); };
+  auto empty = [&](int m) { return wait_warp(smem_u32(&s_empty[(n1 + m) % S]), (m / S) & 1, &s_abort, a.status, 122); };
 
-  if (warp == 8) {
-    // ---- products: a step's as soon as its tiles are there; the stage is free when they are done ----
-    auto arrived = [&](int k) {
-      mbar_wait(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 121);
+  if (warp == kFinishWarps + kCopyWarps) {
+    // ---- products ----
+    for (int k = 0; live > 0 && k < n1; ++k) {
+      full(k);
       tc_fence_after();
-      return ring + k % S * C::STAGE;
-    };
-    if (live > 0 && elect_one())
-      for (int k = 0; k < n1; ++k) {
-        const uint32_t at = arrived(k);
+      if (elect_one()) {
+        const uint32_t at = ring + k % S * C::STAGE;
         const uint64_t da = make_smem_desc(at), db = BACK ? rows_desc(at + C::ROWS, 8192) : make_smem_desc(at + C::ROWS);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           tc_mma_bf16(tmem, da + 2 * j, db + (BACK ? 128 : 2) * j, mma_shape(RP) | (BACK ? kRowsB : 0u), k + j > 0 ? 1u : 0u);
         tc_commit(smem_u32(&s_done[k % S]));
+        if (k == n1 - 1) tc_commit(smem_u32(&s_first));          // for who has not waited for every phase before
       }
-    __syncwarp();
-    if (live > 0 && cs > 1) {
-      cluster_sync_all();
-      cluster_sync_all();
+      __syncwarp();
     }
-    if (live > 0 && elect_one())
-      for (int m = 0; m < n2; ++m) {
-        const uint32_t at = arrived(n1 + m) + C::ROWS, d = tmem + C::SECOND + (m & 1) * 64;
+    if (live > 0) wait_warp(smem_u32(&s_ready), 0, &s_abort, a.status, 123);
+    for (int m = 0; live > 0 && m < n2; ++m) {
+      full(n1 + m);
+      if (m >= 2) empty(m - 2);                        // the accumulator has been read
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t at = ring + (n1 + m) % S * C::STAGE + C::ROWS, d = tmem + C::SECOND + (m & 1) * 64;
         const uint64_t da = make_smem_desc(s_at), db = BACK ? rows_desc(at, 8192) : make_smem_desc(at);
 #pragma unroll
         for (int part = 0; part < 2; ++part)
@@ -450,128 +542,72 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
                         mma_shape(64) | (BACK ? kRowsB : 0u), part + k > 0 ? 1u : 0u);
         tc_commit(smem_u32(&s_done[(n1 + m) % S]));
       }
-    __syncwarp();
-  } else {
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const bool in_place = a.y == a.out && a.ldy == a.ldo, filled = a.rank == RP;
-    const uint16_t* w1 = a.w1 + (g >= 0 ? g * a.g1 : 0);
-    const uint16_t* w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
-    // A warp copies and stores 16 rows of a tile: this thread 16 bytes of every fourth of them.  (128 bytes of a row side by side: with 64, the
-    // load and store unit was what 8192 rows of 4096 x 4096 waited for.)  Rows that are not there are the last one again, and not stored.
-    // Outputs are finished by rows to a lane, 64 bytes to a warp, so that two warps share 32 rows.
-    const int first_row = quarter * 32 + side * 16, piece = lane & 7;
-    const uint32_t mine = (first_row + (lane >> 3)) * 128;
-    auto mine_at = [&](int j) { return mine + j * 512 + ((piece ^ (lane >> 3) ^ ((j & 1) << 2)) << 4); };
-    const uint16_t *xp[4], *yp[4];
-    uint16_t* op[4];
-    uint32_t stored = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = first_row + j * 4 + (lane >> 3);
-      const int64_t row = s_rows[min(r, len - 1)];
-      xp[j] = a.x + (live > 0 ? static_cast<int64_t>(s_rows[min(r, live - 1)]) : 0) * a.ldx + piece * 8;
-      yp[j] = a.y + row * a.ldy + piece * 8;
-      op[j] = a.out + row * a.ldo + piece * 8;
-      stored |= (r < len && !(in_place && r >= live) ? 1u : 0u) << j;
+      __syncwarp();
     }
-    // The adapter's tile: RP rows of 64 elements (wide), or 64 rows of RP (narrow).  This thread's 16-byte pieces, in pairs of rows so far apart that
-    // their place is the same one
-    constexpr int WIDE = RP / 32 > 0 ? RP / 32 : 1, NARROW_ROWS = kAdapterThreads / (RP / 8);
-    const bool mine_too = RP >= 32 || tid < 128;
-    const int wr = tid >> 3, wp = tid & 7, nr = tid / (RP / 8), np = tid % (RP / 8);
-    const uint32_t wide_at = C::ROWS + wr * 128 + ((wp ^ (wr & 7)) << 4);
-    const uint32_t narrow_at = C::ROWS + (np >> 3) * 8192 + nr * 128 + (((np & 7) ^ (nr & 7)) << 4);
-    const uint16_t* wide = BACK ? w2 + wr * a.ld2 + wp * 8 : w1 + wr * a.ld1 + wp * 8;
-    const uint16_t* narrow = BACK ? w1 + nr * a.ld1 + np * 8 : w2 + nr * a.ld2 + np * 8;
-    const int64_t wide_ld = BACK ? a.ld2 : a.ld1, narrow_ld = BACK ? a.ld1 : a.ld2;
-    auto fetch_adapter = [&](uint32_t to, int c, bool first, bool whole) {
-      if (!mine_too) return;
-      if (first != BACK) {                             // wide
-        if (whole) {
-          const uint16_t* w = wide + c;
-#pragma unroll
-          for (int j = 0; j < WIDE; ++j, w += 32 * wide_ld) copy_whole(to + wide_at + j * 4096, w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < WIDE; ++j) {
-            const int r = wr + j * 32;
-            copy_row<16>(to + wide_at + j * 4096, (BACK ? w2 : w1) + (r < a.rank ? r : 0) * wide_ld, c + wp * 8, r < a.rank ? (BACK ? a.N : a.K) : 0);
-          }
-        }
-      } else {
-        const int end = BACK ? a.K : a.N;
-        if (whole) {
-          const uint16_t* w = narrow + c * narrow_ld;
-#pragma unroll
-          for (int j = 0; j < WIDE; ++j, w += NARROW_ROWS * narrow_ld) copy_whole(to + narrow_at + j * NARROW_ROWS * 128, w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < WIDE; ++j) {
-            const int r = c + nr + j * NARROW_ROWS;
-            copy_row<16>(to + narrow_at + j * NARROW_ROWS * 128, (BACK ? w1 : w2) + (r < end ? r : 0) * narrow_ld, np * 8, r < end ? a.rank : 0);
-          }
-        }
-      }
-    };
-    int ahead = 0;                                     // the next step to fetch, into stage `filling`
-    uint32_t filling = ring;
-    auto fetch = [&](int end) {
-      if (ahead < end) {
-        const bool first = ahead < n1;
-        const int c = (first ? lo1 + ahead : lo2 + ahead - n1) * 64, n = first ? a.K : a.N;
-        const bool inside = c + 64 <= n;
-        if (first ? first_row < live : !BACK && first_row < len) {
-          if (inside) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) copy_whole(filling + mine_at(j), (first ? xp[j] : yp[j]) + c);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) copy_row<16>(filling + mine_at(j), (first ? xp[j] : yp[j]) - piece * 8, c + piece * 8, n);
-          }
-        }
-        if (live > 0) fetch_adapter(filling, c, first, inside && filled);
+  } else if (warp >= kFinishWarps) {
+    // ---- copies of the second product, from step n1 + S - 1 on ----
+    TileCopies<RP, BACK, kCopyWarps> copies(a, g, tid - kFinishWarps * 32);
+    if (!BACK) copies.rows_of(a.y, a.ldy, s_rows, len);
+    if (n1 > 0) wait_warp(smem_u32(&s_first), 0, &s_abort, a.status, 126);       // the first product has left its last stage
+    for (int m = S - 1; m < n2 + S - 2; ++m) {
+      if (m < n2) {
+        if (m >= S) empty(m - S);
+        copies.step(ring + (n1 + m) % S * C::STAGE, false, (lo2 + m) * 64, a.N, BACK ? 0 : len, live > 0);
       }
       copies_commit();
-      ++ahead;
-      filling = filling == ring + (S - 1) * C::STAGE ? ring : filling + C::STAGE;
-    };
-    // this warp's copies of step k are there, and what it has written before, for the tensor core too
-    auto arrive = [&](int k) {
-      copies_wait<S - 2>();
+      copies_wait<S - 2>();                            // step m - (S - 2) is there, for the tensor core too
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc_fence_before();
       __syncwarp();
-      if (live > 0 && lane == 0) mbar_arrive(smem_u32(&s_full[k % S]));
-    };
-    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 120); };
-    const int end1 = cs == 1 ? steps : n1;             // in a cluster the blocks' sums of s go where the ring is
-#pragma unroll
-    for (int k = 0; k < S - 1; ++k) fetch(end1);
-
-    if (live > 0) {
+      if (m >= 2 * S - 3 && lane < kFinishWarps / kCopyWarps) mbar_arrive(smem_u32(&s_full[(n1 + m - (S - 2)) % S]));
+    }
+  } else {
+    // ---- s, and the outputs ----
+    // A lane finishes a row, 64 bytes to a warp, so that two warps share 32 rows; each stores 16 of them, 128 bytes of a row side by side.
+    const int quarter = warp & 3, side = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
+    const bool in_place = a.y == a.out && a.ldy == a.ldo;
+    {
+      // ---- copies of the first product and of the second's first S - 1 steps ----
+      TileCopies<RP, BACK, kFinishWarps> copies(a, g, tid);
+      if (n1 > 0) copies.rows_of(a.x, a.ldx, s_rows, live);
+      auto fetch = [&](int k) {
+        if (k < n1) {
+          copies.step(ring + k % S * C::STAGE, true, (lo1 + k) * 64, a.K, live, true);
+        } else if (k < n1 + n2) {
+          if (!BACK && k == n1) copies.rows_of(a.y, a.ldy, s_rows, len);
+          copies.step(ring + k % S * C::STAGE, false, (lo2 + k - n1) * 64, a.N, BACK ? 0 : len, live > 0);
+        }
+        copies_commit();
+      };
+#pragma unroll 1
+      for (int k = 0; k < S - 1; ++k) fetch(k);
       for (int k = 0; k < n1; ++k) {
-        arrive(k);
+        arrive<S - 2>(&s_full[k % S]);
         if (k > 0) done(k - 1);
-        fetch(end1);
+        fetch(k + S - 1);
       }
       if (n1 > 0) done(n1 - 1);
-      tc_fence_after();
+    }
+    if (live > 0) {
       // eight columns of a row of s, zeros behind the tile's rows and the rank, in two parts
-      auto parts = [&](int row, int col, float* v, uint4& high, uint4& low) {
+      auto parts = [&](int r, int col, float* v, uint4& high, uint4& low) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = row < live && col + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
+        for (int e = 0; e < 8; ++e) v[e] = r < live && col + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
         split_pair(v[0], v[1], high.x, low.x);
         split_pair(v[2], v[3], high.y, low.y);
         split_pair(v[4], v[5], high.z, low.z);
         split_pair(v[6], v[7], high.w, low.w);
-        if (a.s != nullptr && row < len) *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[row]) * RP + col) = high;
-        return s_at + (col >> 6) * C::ROWS + row * 128 + (((col >> 3 & 7) ^ (row & 7)) << 4);
+        if (a.s != nullptr && r < len) *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[r]) * RP + col) = high;
+        return s_at + (col >> 6) * C::ROWS + r * 128;
       };
+      auto low_piece = [&](int r, int col) { return (((RP <= 32 ? 4 : 0) + (col >> 3 & 7)) ^ (r & 7)) << 4; };      // in the second part's row
+      tc_fence_after();
       // the accumulator's row of this thread, half of the columns to either side's warps
 #pragma unroll
       for (int k = 0; k < RP / 2; k += 8) {
         float v[8];
-        const int row = quarter * 32 + lane, col = side * (RP / 2) + k;
+        const int col = side * (RP / 2) + k;
         tc_ld8(lanes + col, v);
         if (n1 == 0)
 #pragma unroll
@@ -579,90 +615,113 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
         if (cs == 1) {
           uint4 high, low;
           const uint32_t to = parts(row, col, v, high, low);
-          st_shared(to, high);
-          st_shared(to + C::PART, low);
-        } else {                                       // [groups of four columns][row]
+          st_shared(to + (((col >> 3 & 7) ^ (row & 7)) << 4), high);
+          st_shared(to + (RP <= 32 ? 0 : C::PART) + low_piece(row, col), low);
+        } else {                                       // [groups of four columns][row], where s will be
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            st_shared(ring + ((col / 4 + e) * kAdapterTile + row) * 16,
+            st_shared(s_at + ((col / 4 + e) * kAdapterTile + row) * 16,
                       make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
         }
       }
       if (cs > 1) {
-        cluster_sync_all();
+        auto meet = [&](int k) {                       // all blocks' warps that finish have come so far
+          __syncwarp();
+          if (lane < cs) mbar_arrive_cluster(map_to_cta(smem_u32(&s_met[k]), lane));
+          mbar_wait_cluster(smem_u32(&s_met[k]), 0, &s_abort, a.status, 124);
+          __syncwarp();
+        };
+        constexpr int ITEMS = RP <= 32 ? 1 : RP / 32;
         const int share = kAdapterTile / cs;
-        for (int p = tid; p < share * RP / 8; p += kAdapterThreads) {
-          const int row = cr * share + p % share, col = p / share * 8;
-          float v[8];
-          const uint32_t at = ring + (col / 4 * kAdapterTile + row) * 16;
-          if (cs == 8) cluster_sum8<8>(at, kAdapterTile * 16, v);
-          else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, v);
-          else cluster_sum8<2>(at, kAdapterTile * 16, v);
+        float v[ITEMS][8];
+        meet(0);
+#pragma unroll
+        for (int n = 0; n < ITEMS; ++n) {
+          const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
+          const uint32_t at = s_at + (col / 4 * kAdapterTile + r) * 16;
+          if (q >= share * RP / 8) continue;
+          if (cs == 8) cluster_sum8<8>(at, kAdapterTile * 16, v[n]);
+          else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, v[n]);
+          else cluster_sum8<2>(at, kAdapterTile * 16, v[n]);
+        }
+        meet(1);
+#pragma unroll
+        for (int n = 0; n < ITEMS; ++n) {
+          const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
+          if (q >= share * RP / 8) continue;
           uint4 high, low;
-          const uint32_t to = parts(row, col, v, high, low);
+          const uint32_t to = parts(r, col, v[n], high, low);
           for (int c = 0; c < cs; ++c) {
             const uint32_t there = map_to_cta(to, c);
-            st_cluster16(there, high);
-            st_cluster16(there + C::PART, low);
+            st_cluster16(there + (((col >> 3 & 7) ^ (r & 7)) << 4), high);
+            st_cluster16(there + (RP <= 32 ? 0 : C::PART) + low_piece(r, col), low);
           }
         }
         asm volatile("fence.proxy.async;" ::: "memory");
-        cluster_sync_all();                            // s is whole; the ring is free again, here and in the blocks that have read it
+        meet(2);
       }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s_ready));
     } else if (a.s != nullptr && cr == 0) {
-      for (int p = tid; p < len * RP / 8; p += kAdapterThreads)
+      for (int p = tid; p < len * RP / 8; p += kFinishWarps * 32)
         *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[p / (RP / 8)]) * RP + p % (RP / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
-    if (cs > 1) {
-      ahead = n1;
-      filling = ring + n1 % S * C::STAGE;
+    const int first_row = quarter * 32 + side * 16, piece = lane & 7;
+    uint16_t* op[4];
+    uint32_t stored = 0;
 #pragma unroll
-      for (int k = 0; k < S - 1; ++k) fetch(steps);
+    for (int j = 0; j < 4; ++j) {
+      const int r = first_row + j * 4 + (lane >> 3);
+      op[j] = a.out + static_cast<int64_t>(s_rows[min(r, len - 1)]) * a.ldo + piece * 8;
+      stored |= (r < len && !(in_place && r >= live) ? 1u : 0u) << j;
     }
-
-    // finishes unit m in the place of y, from where the warps store 128 bytes of four rows at a time
-    auto finish = [&](int m) {
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k)
+      if (k < n2) arrive<0>(&s_full[(n1 + k) % S]);
+    for (int m = 0; m < n2; ++m) {
       const uint32_t at = ring + (n1 + m) % S * C::STAGE;
-      const int c0 = (lo2 + m) * 64, row = quarter * 32 + lane;
-      pair_sync(quarter);                              // the other warp's copies too
+      const int c0 = (lo2 + m) * 64;
+      full(n1 + m);
       if (live > 0) {
         done(n1 + m);
         tc_fence_after();
-        uint32_t acc[32];
-        tc_ld32(lanes + C::SECOND + (m & 1) * 64 + side * 32, acc);
-        tc_ld_wait();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t to = at + row * 128 + (((side * 4 + k) ^ (row & 7)) << 4);
-          float o[8];
-          if (!BACK) unpack8(ld_shared(to), o);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t acc[16];
+          tc_ld16(lanes + C::SECOND + (m & 1) * 64 + side * 32 + h * 16, acc);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float p = __uint_as_float(acc[8 * k + e]);
-            o[e] = BACK ? p : fmaf(scale, p, o[e]);
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t to = at + row * 128 + (((side * 4 + h * 2 + k) ^ (row & 7)) << 4);
+            float o[8];
+            if (!BACK) unpack8(ld_shared(to), o);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = __uint_as_float(acc[8 * k + e]);
+              o[e] = BACK ? v : fmaf(scale, v, o[e]);
+            }
+            if (row < live) st_shared(to, pack8(o));
+            else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
           }
-          if (row < live) st_shared(to, pack8(o));
-          else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
         }
+        tc_fence_before();
+        pair_sync(quarter);
       }
-      pair_sync(quarter);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u) : ld_shared(at + mine_at(j));
+        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u)
+                                          : ld_shared(at + (first_row + j * 4 + (lane >> 3)) * 128 + ((piece ^ (lane >> 3) ^ ((j & 1) << 2)) << 4));
         if (stored >> j & 1u) store_row(op[j] + c0, 0, a.N - c0 - piece * 8, v);
       }
-    };
-    for (int m = 0; m < n2; ++m) {
-      arrive(n1 + m);
-      if (m > 0) finish(m - 1);
-      fetch(steps);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&s_empty[(n1 + m) % S]));
     }
-    if (n2 > 0) finish(n2 - 1);
-    copies_wait<0>();
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 8) {
+  if (cs > 1) cluster_sync_all();                      // no block leaves while another may reach for its memory, also where a wait has run out
+  else __syncthreads();
+  if (warp == kFinishWarps + kCopyWarps) {
     __syncwarp();
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
@@ -688,6 +747,7 @@ struct AdapterGradArgs {
   int32_t* status;
 };
 
+constexpr int kGradThreads = kAdapterThreads + 32;
 template <int RP>
 struct GradCfg {
   static constexpr int BLOCKS = 2, STAGES = RP <= 64 ? 4 : 3;
@@ -699,7 +759,7 @@ struct GradCfg {
 };
 
 template <int RP>
-__global__ void __launch_bounds__(kTileThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
   using C = GradCfg<RP>;
   constexpr int S = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -718,7 +778,7 @@ __global__ void __launch_bounds__(kTileThreads, GradCfg<RP>::BLOCKS) adapter_gra
   const int64_t stride = static_cast<int64_t>(a.rank) * cols;
   uint16_t* out = (which ? a.out[1] : a.out[0]) + g * stride;
   if (live == 0) {                                     // the whole cluster
-    for (int e = cr * kTileThreads + tid; e < 128 * a.rank; e += cs * kTileThreads) {
+    for (int e = cr * kGradThreads + tid; e < 128 * a.rank; e += cs * kGradThreads) {
       const int c = c0 + (which ? e % 128 : e / a.rank), r = which ? e / 128 : e % a.rank;
       if (c < cols) out[which ? r * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r] = 0;
     }
@@ -1029,7 +1089,7 @@ template <int RP>
 int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int64_t jobs, int cs, cudaStream_t st) {
   static bool done[64];
   if (int rc = allow_smem(h, adapter_grad_kernel<RP>, GradCfg<RP>::SMEM, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_grad_kernel<RP>, jobs, cs, kTileThreads, GradCfg<RP>::SMEM, st, a));
+  MG_CUDA(launch_clusters(adapter_grad_kernel<RP>, jobs, cs, kGradThreads, GradCfg<RP>::SMEM, st, a));
   return MG_OK;
 }
 

@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import lib as L
-from .layer import MoELayer
+from .layer import MoELayer, _whole
 
 
 def _unwrap(expert):
@@ -139,11 +139,10 @@ def patch_moe_module(module, device=None, return_router_logits: Optional[bool] =
 
 def patch_decoder_layer(decoder_layer, device=None) -> MoELayer:
     """Replaces the forward of a reference DeepseekV2/V3DecoderLayer whose `.mlp` is a MoE block
-    (modeling_deepseek_v3.py:1302-1375).  Attention and its residual add stay as they are; the three
-    steps behind them - post_attention_layernorm, mlp, residual add - become one call,
-    `MoELayer.block_forward`, which normalises, runs the block and adds the residual inside the
-    combine kernel, updating the hidden states in place.  Same arguments and return tuple as the
-    reference's forward."""
+    (modeling_deepseek_v3.py:1302-1375).  Attention stays as it is; the four steps behind it - residual
+    add, post_attention_layernorm, mlp, residual add - become one call, `MoELayer.block_forward`, which
+    adds and normalises in one launch, runs the block and adds the residual inside the combine kernel.
+    Same arguments and return tuple as the reference's forward."""
     layer = patch_moe_module(decoder_layer.mlp, device)
     norm = decoder_layer.post_attention_layernorm
     eps = float(getattr(norm, "variance_epsilon", getattr(norm, "eps", 1e-6)))
@@ -155,11 +154,14 @@ def patch_decoder_layer(decoder_layer, device=None) -> MoELayer:
         hidden_states, self_attn_weights, present_key_value = decoder_layer.self_attn(
             hidden_states=hidden_states, attention_mask=attention_mask, position_ids=position_ids,
             past_key_value=past_key_value, output_attentions=output_attentions, use_cache=use_cache, **kwargs)
-        hidden_states = (residual + hidden_states).contiguous()
         w = norm.weight
         if w.dtype != torch.bfloat16 or w.device != hidden_states.device:
             w = w.detach().to(hidden_states.device, torch.bfloat16)
-        hidden_states = layer.block_forward(hidden_states, w, eps, out=hidden_states)
+        if hidden_states.shape == residual.shape and hidden_states.dtype == residual.dtype == torch.bfloat16:
+            hidden_states = layer.block_forward(_whole(hidden_states), w, eps, residual=_whole(residual))
+        else:                               # what the addition broadcasts or promotes is the module's
+            hidden_states = (residual + hidden_states).contiguous()
+            hidden_states = layer.block_forward(hidden_states, w, eps, out=hidden_states)
         outputs = (hidden_states,)
         if output_attentions:
             outputs += (self_attn_weights,)
