@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
   using C = TileCfg<RP>;
   constexpr int S = C::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ uint64_t s_full[S], s_done[S], s_empty[S], s_first, s_ready, s_met[3];
+  __shared__ uint64_t s_full[S], s_done[S], s_empty[S], s_first, s_ready;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   __shared__ int s_rows[kAdapterTile];
@@ -487,7 +487,6 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     }
     mbar_init(smem_u32(&s_first), 1);
     mbar_init(smem_u32(&s_ready), kFinishWarps);
-    for (int k = 0; k < 3; ++k) mbar_init(smem_u32(&s_met[k]), kFinishWarps * cs);
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -500,8 +499,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
   const int units = (a.N + 63) / 64, each = (units + cs - 1) / cs;
   const int lo1 = cr * per, n1 = max(min(slices, lo1 + per) - lo1, 0), lo2 = cr * each, n2 = max(min(units, lo2 + each) - lo2, 0);
   tc_fence_before();
-  if (cs > 1) cluster_sync_all();                      // the other blocks' barriers are set up
-  else __syncthreads();
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   // Steps are numbered through both products; step k fills stage k % S for the k / S-th time, and the m-th of the second product empties its stage
@@ -526,6 +524,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       }
       __syncwarp();
     }
+    if (live > 0 && cs > 1)
+      for (int k = 0; k < 3; ++k) cluster_sync_all();
     if (live > 0) wait_warp(smem_u32(&s_ready), 0, &s_abort, a.status, 123);
     for (int m = 0; live > 0 && m < n2; ++m) {
       full(n1 + m);
@@ -549,7 +549,12 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     TileCopies<RP, BACK, kCopyWarps> copies(a, g, tid - kFinishWarps * 32);
     if (!BACK) copies.rows_of(a.y, a.ldy, s_rows, len);
     if (n1 > 0) wait_warp(smem_u32(&s_first), 0, &s_abort, a.status, 126);       // the first product has left its last stage
+    bool met = live == 0 || cs == 1;
     for (int m = S - 1; m < n2 + S - 2; ++m) {
+      if (m >= S && !met) {                            // the blocks' exchange, which comes before any stage is emptied
+        for (int k = 0; k < 3; ++k) cluster_sync_all();
+        met = true;
+      }
       if (m < n2) {
         if (m >= S) empty(m - S);
         copies.step(ring + (n1 + m) % S * C::STAGE, false, (lo2 + m) * 64, a.N, BACK ? 0 : len, live > 0);
@@ -560,6 +565,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       __syncwarp();
       if (m >= 2 * S - 3 && lane < kFinishWarps / kCopyWarps) mbar_arrive(smem_u32(&s_full[(n1 + m - (S - 2)) % S]));
     }
+    if (!met)
+      for (int k = 0; k < 3; ++k) cluster_sync_all();
   } else {
     // ---- s, and the outputs ----
     // A lane finishes a row, 64 bytes to a warp, so that two warps share 32 rows; each stores 16 of them, 128 bytes of a row side by side.
@@ -625,16 +632,10 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
         }
       }
       if (cs > 1) {
-        auto meet = [&](int k) {                       // all blocks' warps that finish have come so far
-          __syncwarp();
-          if (lane < cs) mbar_arrive_cluster(map_to_cta(smem_u32(&s_met[k]), lane));
-          mbar_wait_cluster(smem_u32(&s_met[k]), 0, &s_abort, a.status, 124);
-          __syncwarp();
-        };
         constexpr int ITEMS = RP <= 32 ? 1 : RP / 32;
         const int share = kAdapterTile / cs;
         float v[ITEMS][8];
-        meet(0);
+        cluster_sync_all();                            // the blocks' sums are there
 #pragma unroll
         for (int n = 0; n < ITEMS; ++n) {
           const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
@@ -644,21 +645,21 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
           else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, v[n]);
           else cluster_sum8<2>(at, kAdapterTile * 16, v[n]);
         }
-        meet(1);
+        cluster_sync_all();                            // and have been read: s takes their place
 #pragma unroll
         for (int n = 0; n < ITEMS; ++n) {
           const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
           if (q >= share * RP / 8) continue;
           uint4 high, low;
           const uint32_t to = parts(r, col, v[n], high, low);
-          for (int c = 0; c < cs; ++c) {
-            const uint32_t there = map_to_cta(to, c);
+          for (int c = 0; c < cs; ++c) {                // every block begins with itself
+            const uint32_t there = map_to_cta(to, (cr + c) & (cs - 1));
             st_cluster16(there + (((col >> 3 & 7) ^ (r & 7)) << 4), high);
             st_cluster16(there + (RP <= 32 ? 0 : C::PART) + low_piece(r, col), low);
           }
         }
         asm volatile("fence.proxy.async;" ::: "memory");
-        meet(2);
+        cluster_sync_all();
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
@@ -719,8 +720,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     }
   }
   tc_fence_before();
-  if (cs > 1) cluster_sync_all();                      // no block leaves while another may reach for its memory, also where a wait has run out
-  else __syncthreads();
+  __syncthreads();                                     // other blocks reach for this one's memory between their joint barriers only
   if (warp == kFinishWarps + kCopyWarps) {
     __syncwarp();
     tc_fence_after();
