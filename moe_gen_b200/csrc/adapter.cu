@@ -922,15 +922,16 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
 }
 
 // ---- plans -----------------------------------------------------------------------------------
-constexpr int kPlanWarps = 32;
-struct PlanLayout { int64_t tiles, segs, order, words; };          // offsets in words
+constexpr int kPlanWarps = 32, kPlanAhead = 8;
+struct PlanLayout { int64_t tiles, segs, order, place, words; };          // offsets in words
 PlanLayout plan_layout(int64_t rows, int64_t adapters) {
   PlanLayout p;
   const int64_t n = (rows + kAdapterTile - 1) / kAdapterTile + adapters + 1;
   p.tiles = 0;
   p.segs = 4 * n;
   p.order = p.segs + 2 * (adapters + (adapters & 1));
-  p.words = p.order + rows;
+  p.place = p.order + rows;                // while the plan is made
+  p.words = p.place + rows;
   return p;
 }
 
@@ -940,7 +941,7 @@ PlanLayout plan_layout(int64_t rows, int64_t adapters) {
 template <bool SORTED>
 __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int32_t* ids, const int32_t* counts, const int32_t* pad,
                                                                        int rows, int adapters, int n_tiles, int4* tiles, int2* segs,
-                                                                       int32_t* order) {
+                                                                       int32_t* order, int32_t* place) {
   extern __shared__ __align__(16) int s_mem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, groups = adapters + 1;
   if (SORTED && blockIdx.x > 0) {
@@ -953,29 +954,49 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
   int* s_live = s_len + groups;            // of which with the adapter
   int* s_tile = s_live + groups;           // [groups + 1] tiles before
   int* s_hist = s_tile + groups + 1;       // [warps][groups]
+  auto id_of = [&](int64_t j) {            // -1: no row
+    const int v = j < rows ? ids[j] : 0;
+    return j < rows ? (v >= 0 && v < adapters ? v : adapters) : -1;
+  };
   const int per = ((rows + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
   const int64_t from = static_cast<int64_t>(warp) * per;
   if (!SORTED) {
     for (int e = tid; e < kPlanWarps * groups; e += blockDim.x) s_hist[e] = 0;
     __syncthreads();
-    for (int k = 0; k < per; k += 32) {
-      const int64_t j = from + k + lane;
-      const int v = j < rows ? ids[j] : -1;
-      const int id = j < rows ? (v >= 0 && v < adapters ? v : adapters) : -1;
-      const uint32_t peers = __match_any_sync(0xFFFFFFFFu, id);
-      if (id >= 0 && lane == __ffs(peers) - 1) s_hist[warp * groups + id] += __popc(peers);
-      __syncwarp();
+    for (int k = 0; k < per; k += 32 * kPlanAhead) {
+      int ids_of[kPlanAhead];                          // on their way together
+#pragma unroll
+      for (int n = 0; n < kPlanAhead; ++n) ids_of[n] = k + n * 32 < per ? id_of(from + k + n * 32 + lane) : -1;
+#pragma unroll
+      for (int n = 0; n < kPlanAhead; ++n) {
+        if (k + n * 32 >= per) break;
+        const int id = ids_of[n];
+        const uint32_t peers = __match_any_sync(0xFFFFFFFFu, id);
+        const int before = __popc(peers & ((1u << lane) - 1u));
+        int at = 0;
+        if (id >= 0 && before == 0) {
+          at = s_hist[warp * groups + id];
+          s_hist[warp * groups + id] = at + __popc(peers);
+        }
+        at = __shfl_sync(0xFFFFFFFFu, at, __ffs(peers) - 1) + before;
+        if (id >= 0) place[from + k + n * 32 + lane] = at;             // among the warp's rows of the adapter
+        __syncwarp();
+      }
     }
     __syncthreads();
-    for (int e = tid; e < groups; e += blockDim.x) {
-      int run = 0;
-      for (int w = 0; w < kPlanWarps; ++w) {
-        const int n = s_hist[w * groups + e];
-        s_hist[w * groups + e] = run;
-        run += n;
+    for (int e = warp; e < groups; e += kPlanWarps) {  // lane: a warp's count
+      const int n = s_hist[lane * groups + e];
+      int in = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, in, o);
+        if (lane >= o) in += u;
       }
-      s_len[e] = run;
-      s_live[e] = e < adapters ? run : 0;
+      s_hist[lane * groups + e] = in - n;
+      if (lane == 31) {
+        s_len[e] = in;
+        s_live[e] = e < adapters ? in : 0;
+      }
     }
   } else {
     for (int e = tid; e < groups; e += blockDim.x) {
@@ -1029,19 +1050,11 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
     tiles[e] = t;
   }
   if (!SORTED)
+#pragma unroll 4
     for (int k = 0; k < per; k += 32) {
       const int64_t j = from + k + lane;
-      const int v = j < rows ? ids[j] : -1;
-      const int id = j < rows ? (v >= 0 && v < adapters ? v : adapters) : -1;
-      const uint32_t peers = __match_any_sync(0xFFFFFFFFu, id);
-      const int before = __popc(peers & ((1u << lane) - 1u));
-      const int at = id >= 0 ? s_start[id] + s_hist[warp * groups + id] + before : 0;
-      __syncwarp();
-      if (id >= 0) {
-        order[at] = static_cast<int32_t>(j);
-        if (before == 0) s_hist[warp * groups + id] += __popc(peers);
-      }
-      __syncwarp();
+      const int id = id_of(j);
+      if (id >= 0) order[s_start[id] + s_hist[warp * groups + id] + place[j]] = static_cast<int32_t>(j);
     }
 }
 
@@ -1110,11 +1123,11 @@ int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* coun
   if (ids != nullptr) {
     if (int rc = allow_smem(h, adapter_plan_kernel<false>, most, done[0])) return rc;
     adapter_plan_kernel<false><<<1, kPlanWarps * 32, smem, st>>>(ids, nullptr, nullptr, static_cast<int>(rows), adapters, n_tiles,
-                                                                reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order);
+                                                                reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order, w + p.place);
   } else {
     const unsigned blocks = static_cast<unsigned>(1 + (rows + kPlanWarps * 32 - 1) / (kPlanWarps * 32));
     adapter_plan_kernel<true><<<blocks, kPlanWarps * 32, smem, st>>>(nullptr, counts, pad, static_cast<int>(rows), adapters, n_tiles,
-                                                                    reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order);
+                                                                    reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order, w + p.place);
   }
   MG_CUDA(cudaGetLastError());
   return MG_OK;

@@ -342,3 +342,65 @@ def test_rows_beyond_32_bits(layer):
     del q, s
     gx, _ = layer.add_rmsnorm_grad(x, x, w)
     assert torch.equal(gx[-3:], layer.add_rmsnorm_grad(last, last, w)[0])
+
+
+@pytest.mark.parametrize("shape", [(1, 1), (2, 19), (1, 2100)])
+def test_the_patched_decoder_layer_adds_in_the_norms_launch(built_lib, shape):
+    """What a patched decoder layer returns is the block on the rounded sum, bit for bit, also where attention hands over rows that
+    are not contiguous, begin off a boundary, or have another type (which the addition promotes, and the block refuses)."""
+    import types
+
+    import torch.nn as nn
+    from moe_gen_b200 import patch_decoder_layer
+    g = torch.Generator().manual_seed(3)
+
+    class DeepseekV3MoE(nn.Module):
+        pass
+
+    class Layer(nn.Module):
+        pass
+
+    class Norm(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.weight, self.variance_epsilon = nn.Parameter((1 + 0.1 * torch.randn(256, generator=g)).to(torch.bfloat16).to(DEV)), 1e-6
+
+        def forward(self, h):
+            return h
+
+    def lin(rows, cols):
+        m = nn.Linear(cols, rows, bias=False)
+        m.weight = nn.Parameter((torch.randn(rows, cols, generator=g) * 0.05).to(torch.bfloat16).to(DEV), requires_grad=False)
+        return m
+
+    def mlp():
+        m = nn.Module()
+        m.gate_proj, m.up_proj, m.down_proj = lin(128, 256), lin(128, 256), lin(256, 128)
+        return m
+
+    moe = DeepseekV3MoE().eval()
+    moe.config = types.SimpleNamespace(hidden_size=256, moe_intermediate_size=128, n_routed_experts=8, num_experts_per_tok=2, n_shared_experts=1,
+                                       n_group=2, topk_group=1, topk_method="noaux_tc", scoring_func="sigmoid", norm_topk_prob=True,
+                                       routed_scaling_factor=2.5)
+    moe.gate = nn.Module()
+    moe.gate.weight = nn.Parameter(torch.randn(8, 256, generator=g) * 0.05)
+    moe.gate.e_score_correction_bias = nn.Parameter(torch.zeros(8))
+    moe.experts, moe.shared_experts = nn.ModuleList([mlp() for _ in range(8)]), mlp()
+    dl = Layer().eval()
+    dl.input_layernorm, dl.post_attention_layernorm, dl.mlp = Norm(), Norm(), moe
+    B, S = shape
+    kinds = {"plain": lambda t: t * 0.5, "turned": lambda t: (t * 0.5).transpose(0, 1).contiguous().transpose(0, 1),
+             "off": lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)[1:].view(t.shape).copy_(t * 0.5), "float": lambda t: t.float() * 0.5}
+    dl.self_attn = nn.Module()
+    layer = patch_decoder_layer(dl, device=DEV)
+    x = _rows(B * S, 256, 4).clone().view(B, S, 256)
+    want = layer.block_forward(x + x * 0.5, dl.post_attention_layernorm.weight.detach(), 1e-6)
+    for name, make in kinds.items():
+        dl.self_attn.forward = lambda hidden_states, make=make, **kw: (make(hidden_states), None, None)
+        before = x.clone()
+        if name == "float":
+            with pytest.raises(ValueError):
+                dl(x)
+        else:
+            assert torch.equal(dl(x)[0], want), name
+        assert torch.equal(x, before)
