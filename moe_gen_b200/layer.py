@@ -36,6 +36,7 @@ class AdapterPlan:
 
 
 _NO_SWITCH = contextlib.nullcontext()
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
@@ -85,7 +86,7 @@ class MoELayer:
     # Entering torch.cuda.device and asking for torch.cuda.current_stream() takes 1.5 and 3.3 us of a call whose launch takes 3:
     # the device is set where it is another one only, and the stream's handle is read without making a Stream of it.
     def _on_device(self):
-        return _NO_SWITCH if torch.cuda.current_device() == self._index else torch.cuda.device(self._index)
+        return _NO_SWITCH if _raw_device() == self._index else torch.cuda.device(self._index)
 
     def _stream(self) -> int:
         return _raw_stream(self._index)
@@ -684,7 +685,8 @@ class MoELayer:
                                                     self._stream()))
         return AdapterPlan(buf, rows, n)
 
-    def _adapters(self, down: torch.Tensor, up: torch.Tensor, scale) -> L.Adapters:
+    def _adapters(self, down: torch.Tensor, up: torch.Tensor, scale):
+        """-> (mg_adapters as bytes, adapters, rank, cols, n_out)"""
         for t, what in ((down, "down"), (up, "up")):
             if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != self.device:
                 raise ValueError(f"{what}: expected [adapters, rows, cols] bfloat16 on {self.device}, got {tuple(t.shape)} {t.dtype} on "
@@ -705,8 +707,8 @@ class MoELayer:
         else:
             factor = float(scale)
         # torch leaves the strides of single rows open
-        return L.Adapters(C.sizeof(L.Adapters), n, rank, factor, cols, n_out, down.data_ptr(), sd,
-                          ld if rank > 1 else (cols + 7) // 8 * 8, up.data_ptr(), su, lu if n_out > 1 else (rank + 7) // 8 * 8, d_scale)
+        return L.ADAPTERS.pack(L.ADAPTERS.size, n, rank, factor, cols, n_out, down.data_ptr(), sd, ld if rank > 1 else (cols + 7) // 8 * 8,
+                               up.data_ptr(), su, lu if n_out > 1 else (rank + 7) // 8 * 8, d_scale or 0), n, rank, cols, n_out
 
     def _adapter_plan_of(self, who, rows: int, n_adapters: int):
         """ids or a plan -> the two pointers of the call (what the ids lie in is the caller's)."""
@@ -733,18 +735,18 @@ class MoELayer:
         fp32 [adapters].  out may be y, and overlaps nothing otherwise.  With keep also the rows between the two products, bf16,
         for adapter_grad: (out, s).  Any layer serves."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
-        ad = self._adapters(down, up, scale)
-        if cols != ad.cols:
+        ad, n_adapters, rank, a_cols, a_out = self._adapters(down, up, scale)
+        if cols != a_cols:
             raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
         ny, n_out, ldy = self._rows_of(y, torch.bfloat16, "y")
-        if (ny, n_out) != (n, ad.n_out):
-            raise ValueError(f"y {tuple(y.shape)}, expected {(n, ad.n_out)}")
-        who = self._adapter_plan_of(who, n, ad.n_adapters)
+        if (ny, n_out) != (n, a_out):
+            raise ValueError(f"y {tuple(y.shape)}, expected {(n, a_out)}")
+        who = self._adapter_plan_of(who, n, n_adapters)
         ids, plan = (None, who.buf) if isinstance(who, AdapterPlan) else (who, None)
         out, ldo = self._out_rows(out, n, n_out, "out")
-        s = self._rank_rows(n, ad.rank) if keep else None
+        s = self._rank_rows(n, rank) if keep else None
         with self._on_device():
-            L.check(self.lib.mg_adapter_add(self._h, C.byref(ad), x.data_ptr(), ldx, y.data_ptr(), ldy, n, _ptr(ids), _ptr(plan),
+            L.check(self.lib.mg_adapter_add(self._h, ad, x.data_ptr(), ldx, y.data_ptr(), ldy, n, _ptr(ids), _ptr(plan),
                                             out.data_ptr(), ldo, _ptr(s), self._stream()))
         return (out, s) if keep else out
 
@@ -753,19 +755,19 @@ class MoELayer:
         """Gradients of adapter_add -> (grad_x, grad_down, grad_up), bf16, None for what is not needed; s is what adapter_add kept.
         grad_x is zero in rows without an adapter, the others in adapters without rows.  The gradient of y is grad_out itself."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
-        ad = self._adapters(down, up, scale)
-        if cols != ad.cols:
+        ad, n_adapters, rank, a_cols, a_out = self._adapters(down, up, scale)
+        if cols != a_cols:
             raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
         ng, n_out, ldg = self._rows_of(grad_out, torch.bfloat16, "grad_out")
-        if (ng, n_out) != (n, ad.n_out):
-            raise ValueError(f"grad_out {tuple(grad_out.shape)}, expected {(n, ad.n_out)}")
+        if (ng, n_out) != (n, a_out):
+            raise ValueError(f"grad_out {tuple(grad_out.shape)}, expected {(n, a_out)}")
         if isinstance(who, torch.Tensor):
             self._check_in(who, torch.int32, "ids")
             if who.numel() != n:
                 raise ValueError(f"{who.numel()} ids for {n} rows")
-            who = self.adapter_plan(who, ad.n_adapters)
-        who = self._adapter_plan_of(who, n, ad.n_adapters)
-        gs = self._rank_rows(n, ad.rank)
+            who = self.adapter_plan(who, n_adapters)
+        who = self._adapter_plan_of(who, n, n_adapters)
+        gs = self._rank_rows(n, rank)
         self._check_rows(s, torch.bfloat16, n, gs.shape[1], "s")
         if not (need_x or need_down or need_up):
             return None, None, None
@@ -773,7 +775,7 @@ class MoELayer:
         gdown = torch.empty(down.shape, dtype=torch.bfloat16, device=self.device) if need_down else None
         gup = torch.empty(up.shape, dtype=torch.bfloat16, device=self.device) if need_up else None
         with self._on_device():
-            L.check(self.lib.mg_adapter_grad(self._h, C.byref(ad), grad_out.data_ptr(), ldg, x.data_ptr(), ldx, n, who.buf.data_ptr(),
+            L.check(self.lib.mg_adapter_grad(self._h, ad, grad_out.data_ptr(), ldg, x.data_ptr(), ldx, n, who.buf.data_ptr(),
                                              s.data_ptr(), gs.data_ptr(), _ptr(gx), ldgx, _ptr(gdown), _ptr(gup), self._stream()))
         return gx, gdown, gup
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 # MOEGEN_B200_LIB selects another build of the same library (the -DMG_BOUNDS_CHECK one, for test runs)
@@ -49,6 +50,10 @@ class Adapters(C.Structure):
                 ("cols", C.c_int64), ("n_out", C.c_int64),
                 ("d_down", C.c_void_p), ("down_stride", C.c_int64), ("ld_down", C.c_int64),
                 ("d_up", C.c_void_p), ("up_stride", C.c_int64), ("ld_up", C.c_int64), ("d_scale", C.c_void_p)]
+
+
+ADAPTERS = struct.Struct("@iiifqqPqqPqqP")      # the same, packed in a fifth of the time that ctypes takes to fill one
+assert ADAPTERS.size == C.sizeof(Adapters)
 
 
 _vp, _i64, _i32, _sz = C.c_void_p, C.c_int64, C.c_int32, C.c_size_t
@@ -131,8 +136,8 @@ SIGNATURES = {
     "mg_adapter_plan_bytes": [_i64, _i32, _P(_sz)],
     "mg_adapter_plan": [_vp, _vp, _i64, _i32, _vp, _vp],
     "mg_adapter_plan_sorted": [_vp, _vp, _vp, _i64, _i32, _vp, _vp],
-    "mg_adapter_add": [_vp, _P(Adapters), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp],
-    "mg_adapter_grad": [_vp, _P(Adapters), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
+    "mg_adapter_add": [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp],
+    "mg_adapter_grad": [_vp, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp],
     "mg_set_option": [_vp, _i32, _i32],
     "mg_set_stage_timing": [_vp, _i32],
     "mg_stage_times": [_vp, _P(C.c_float), _i32],
