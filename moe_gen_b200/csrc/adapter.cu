@@ -729,10 +729,10 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 }
 
 // ---- gradients of the adapters ---------------------------------------------------------------
-// Both are W[c][r] = sum over an adapter's rows t of wide[t][c] * narrow[t][r]: rows of gout and s, of x and gs.  A block holds 128
-// columns c of one adapter on the accumulator's lanes, for all of the rank, and goes through the rows 64 at a time (a cluster's blocks in
-// turn, where there are few blocks); the inner index is the rows', so both operands are read as they lie.  The blocks' sums meet in a fixed
-// order.
+// Both are W[c][r] = sum over an adapter's rows t of wide[t][c] * narrow[t][r]: rows of gout and s, of x and gs.  A job is 128 columns c of one
+// adapter, on the accumulator's lanes, for all of the rank; a block goes through its rows 64 at a time, then to its next job, whose first
+// copies are on their way meanwhile.  Where there are few jobs a cluster's blocks take the steps of one in turn, and their sums meet in a
+// fixed order.  The inner index is the rows', so both operands are read as they lie.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
@@ -741,7 +741,7 @@ struct AdapterGradArgs {
   uint16_t* out[2];             // [adapters][cols][rank], [adapters][rank][cols]
   const float* scale;
   float factor;
-  int rank;
+  int rank, jobs;
   const int2* segs;             // first entry of order and rows of every adapter
   const int32_t* order;
   int32_t* status;
@@ -754,36 +754,41 @@ struct GradCfg {
   static constexpr int WIDE = 16384;                           // bytes of a stage: two blocks of 64 columns by 64 rows, then the narrow rows
   static constexpr int STAGE = WIDE + (RP <= 64 ? 8192 : 16384);
   static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE + 1024;
-  static constexpr int COLS = 128;                             // of tensor memory
+  static constexpr int COLS = RP < 32 ? 32 : RP;               // of tensor memory
   static_assert(128 * RP * 4 <= STAGES * STAGE && BLOCKS * (SMEM + 1536) <= 227 * 1024, "shared memory");
 };
 
-template <int RP>
+// ONE: a job to a block (to a cluster), else every gridDim.x-th
+template <int RP, bool ONE>
 __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
   using C = GradCfg<RP>;
   constexpr int S = C::STAGES;
-  extern __shared__ uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t s_full[S], s_done[S];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const uint32_t ring = (smem_u32(smem_raw) + 1023) & ~1023u;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quarter = warp & 3, side = warp >> 2;
-  const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
-  const int job = blockIdx.x / cs, per = a.blocks[0] + a.blocks[1];
-  const int g = job / per, block = job % per;
-  const bool which = block >= a.blocks[0];
-  const int c0 = (block - (which ? a.blocks[0] : 0)) * 128, cols = which ? a.cols[1] : a.cols[0];
-  const int2 seg = a.segs[g];
-  const int live = seg.y;
-  const int64_t stride = static_cast<int64_t>(a.rank) * cols;
-  uint16_t* out = (which ? a.out[1] : a.out[0]) + g * stride;
-  if (live == 0) {                                     // the whole cluster
-    for (int e = cr * kGradThreads + tid; e < 128 * a.rank; e += cs * kGradThreads) {
-      const int c = c0 + (which ? e % 128 : e / a.rank), r = which ? e / 128 : e % a.rank;
-      if (c < cols) out[which ? r * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r] = 0;
-    }
-    return;
-  }
+  const int cs = ONE ? static_cast<int>(cluster_size()) : 1, cr = ONE ? static_cast<int>(cluster_ctarank()) : 0;
+  struct Job {
+    int g, c0, start, live, steps;                     // steps: of this block, cr, cr + cs, ...
+    bool which;
+  };
+  auto job_of = [&](int n) {
+    Job j;
+    const int per = a.blocks[0] + a.blocks[1];
+    j.g = n / per;
+    const int block = n - j.g * per;
+    j.which = block >= a.blocks[0];
+    j.c0 = (block - (j.which ? a.blocks[0] : 0)) * 128;
+    const int2 seg = a.segs[j.g];
+    j.start = seg.x;
+    j.live = seg.y;
+    const int all = (seg.y + 63) / 64;
+    j.steps = cr < all ? (all - cr + cs - 1) / cs : 0;
+    return j;
+  };
+  const int first = ONE ? static_cast<int>(blockIdx.x) / cs : static_cast<int>(blockIdx.x), last = ONE ? first + 1 : a.jobs;
   if (tid == 0) {
     for (int k = 0; k < S; ++k) { mbar_init(smem_u32(&s_full[k]), kAdapterThreads / 32); mbar_init(smem_u32(&s_done[k]), 1); }
     s_abort = 0;
@@ -794,47 +799,61 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(C::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const int all = (live + 63) / 64, steps = cr < all ? (all - cr + cs - 1) / cs : 0;       // steps cr, cr + cs, ...
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
 
   if (warp == 8) {
-    if (elect_one())
-      for (int k = 0; k < steps; ++k) {
-        mbar_wait(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 123);
+    int k = 0;
+    for (int n = first; n < last; n += ONE ? 1 : gridDim.x) {
+      const int steps = job_of(n).steps;
+      for (int i = 0; i < steps; ++i, ++k) {
+        wait_warp(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 127);       // a job's first: also that the accumulator has been read
         tc_fence_after();
-        const uint32_t at = ring + k % S * C::STAGE;
-        const uint64_t da = rows_desc(at, 8192), db = rows_desc(at + C::WIDE, 8192);
+        if (elect_one()) {
+          const uint32_t at = ring + k % S * C::STAGE;
+          const uint64_t da = rows_desc(at, 8192), db = rows_desc(at + C::WIDE, 8192);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) tc_mma_bf16(tmem, da + 128 * j, db + 128 * j, mma_shape(RP) | kRowsA | kRowsB, k + j > 0 ? 1u : 0u);
-        tc_commit(smem_u32(&s_done[k % S]));
+          for (int j = 0; j < 4; ++j) tc_mma_bf16(tmem, da + 128 * j, db + 128 * j, mma_shape(RP) | kRowsA | kRowsB, i + j > 0 ? 1u : 0u);
+          tc_commit(smem_u32(&s_done[k % S]));
+        }
+        __syncwarp();
       }
-    __syncwarp();
+    }
   } else {
-    const uint16_t* wide = which ? a.wide[1] : a.wide[0];
-    const uint16_t* narrow = which ? a.narrow[1] : a.narrow[0];
-    const int64_t ldw = which ? a.ldw[1] : a.ldw[0];
     const int r0 = tid >> 3, p = tid & 7;              // this thread's 16 bytes of rows r0 and r0 + 32, of 128 bytes each
     const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
-    int rows[2];
-    auto look = [&](int k) {                           // rows of step k
+    // the next step to fetch: its job, its number in it, its rows
+    int ahead = first, in = 0, rows[2];
+    Job f = job_of(first);
+    uint32_t filling = ring;
+    auto look = [&]() {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int t = (cr + k * cs) * 64 + j * 32 + r0;
-        rows[j] = k < steps && t < live ? a.order[seg.x + t] : -1;
+        const int t = (cr + in * cs) * 64 + j * 32 + r0;
+        rows[j] = in < f.steps && t < f.live ? a.order[f.start + t] : -1;
       }
     };
-    int ahead = 0;
-    uint32_t filling = ring;
-    look(0);
+    auto next_job = [&]() {
+      do {
+        ahead += gridDim.x;
+        if (ahead < last) f = job_of(ahead);
+      } while (ahead < last && f.steps == 0);
+      in = 0;
+    };
+    if (!ONE && f.steps == 0) next_job();
+    look();
     auto fetch = [&]() {                               // what lies behind the last row or column arrives as zeros
-      if (ahead < steps) {
+      if (ONE ? in < f.steps : ahead < last) {
+        const int cols = f.which ? a.cols[1] : a.cols[0], c = f.c0 + p * 8;
+        const uint16_t* wide = f.which ? a.wide[1] : a.wide[0];
+        const uint16_t* narrow = f.which ? a.narrow[1] : a.narrow[0];
+        const int64_t ldw = f.which ? a.ldw[1] : a.ldw[0];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int64_t row = max(rows[j], 0);
-          const int c = c0 + p * 8, end = rows[j] >= 0 ? cols : 0;
+          const int end = rows[j] >= 0 ? cols : 0;
           const uint16_t* w = wide + row * ldw;
           const uint16_t* n = narrow + row * RP;
 #pragma unroll
@@ -843,73 +862,87 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
           for (int b = 0; b < (RP <= 64 ? 1 : 2); ++b)
             if (p < RP / 8) copy_row<16>(filling + C::WIDE + mine + j * 4096 + b * 8192, n, p * 8 + b * 64, rows[j] >= 0 ? RP : 0);
         }
-        look(ahead + 1);
+        ++in;
+        if (!ONE && in == f.steps) next_job();
+        look();
       }
       copies_commit();
-      ++ahead;
       filling = filling == ring + (S - 1) * C::STAGE ? ring : filling + C::STAGE;
     };
-    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 122); };
-#pragma unroll
+    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 128); };
+#pragma unroll 1
     for (int k = 0; k < S - 1; ++k) fetch();
-    for (int k = 0; k < steps; ++k) {
-      copies_wait<S - 2>();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s_full[k % S]));
-      if (k > 0) done(k - 1);
-      fetch();
-    }
-    if (steps > 0) done(steps - 1);
-    tc_fence_after();
-    const float scale = which ? 1.0f : a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f);
-    auto store8 = [&](int c, int r, float* v) {        // eight of the rank of one column
-      if (c >= cols) return;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= scale;
-      if (!which && r + 8 <= a.rank && a.rank % 8 == 0) {
-        *reinterpret_cast<uint4*>(out + static_cast<int64_t>(c) * a.rank + r) = pack8(v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (r + e < a.rank)
-            out[which ? (r + e) * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r + e] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+    int k = 0;
+    for (int n = first; n < last; n += ONE ? 1 : gridDim.x) {
+      const Job j = job_of(n);
+      const int cols = j.which ? a.cols[1] : a.cols[0];
+      uint16_t* out = (j.which ? a.out[1] : a.out[0]) + static_cast<int64_t>(j.g) * a.rank * cols;
+      for (int i = 0; i < j.steps; ++i, ++k) {
+        arrive<S - 2>(&s_full[k % S]);
+        if (k > 0) done(k - 1);
+        fetch();
       }
-    };
-#pragma unroll
-    for (int k = 0; k < RP / 2; k += 8) {
-      float v[8];
-      const int col = quarter * 32 + lane, r = side * (RP / 2) + k;
-      tc_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r, v);
-      if (steps == 0)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
-      if (cs == 1) {
-        store8(c0 + col, r, v);
-      } else {                                         // [groups of four of the rank][column]
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          st_shared(ring + ((r / 4 + e) * 128 + col) * 16,
-                    make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
+      if (j.live == 0) {
+        for (int e = cr * kAdapterThreads + tid; e < 128 * a.rank; e += cs * kAdapterThreads) {
+          const int c = j.c0 + (j.which ? e % 128 : e / a.rank), r = j.which ? e / 128 : e % a.rank;
+          if (c < cols) out[j.which ? r * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r] = 0;
+        }
+        continue;
       }
-    }
-    if (cs > 1) {
-      cluster_sync_all();
-      const int share = 128 / cs;
-      for (int q = tid; q < share * RP / 8; q += kAdapterThreads) {
-        const int col = cr * share + q % share, r = q / share * 8;
+      if (j.steps > 0) done(k - 1);
+      tc_fence_after();
+      const float scale = j.which ? 1.0f : a.factor * (a.scale != nullptr ? a.scale[j.g] : 1.0f);
+      auto store8 = [&](int c, int r, float* v) {      // eight of the rank of one column
+        if (c >= cols) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= scale;
+        if (!j.which && r + 8 <= a.rank && a.rank % 8 == 0) {
+          *reinterpret_cast<uint4*>(out + static_cast<int64_t>(c) * a.rank + r) = pack8(v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (r + e < a.rank)
+              out[j.which ? (r + e) * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r + e] =
+                  __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+        }
+      };
+      // a lane a column, half of the rank to either side's warps
+      const int col = quarter * 32 + lane;
+#pragma unroll
+      for (int q = 0; q < RP / 2; q += 8) {
         float v[8];
-        const uint32_t at = ring + (r / 4 * 128 + col) * 16;
-        if (cs == 8) cluster_sum8<8>(at, 128 * 16, v);
-        else if (cs == 4) cluster_sum8<4>(at, 128 * 16, v);
-        else cluster_sum8<2>(at, 128 * 16, v);
-        store8(c0 + col, r, v);
+        const int r = side * (RP / 2) + q;
+        tc_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r, v);
+        if (j.steps == 0)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (cs == 1) {
+          store8(j.c0 + col, r, v);
+        } else {                                       // [groups of four of the rank][column]
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            st_shared(ring + ((r / 4 + e) * 128 + col) * 16,
+                      make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
+        }
+      }
+      if (cs > 1) {
+        cluster_sync_all();
+        const int share = 128 / cs;
+        for (int q = tid; q < share * RP / 8; q += kAdapterThreads) {
+          const int c = cr * share + q % share, r = q / share * 8;
+          float v[8];
+          const uint32_t at = ring + (r / 4 * 128 + c) * 16;
+          if (cs == 8) cluster_sum8<8>(at, 128 * 16, v);
+          else if (cs == 4) cluster_sum8<4>(at, 128 * 16, v);
+          else cluster_sum8<2>(at, 128 * 16, v);
+          store8(j.c0 + c, r, v);
+        }
       }
     }
     copies_wait<0>();
   }
   if (cs > 1) {                                        // no block leaves while another reads its sums
-    if (warp == 8) cluster_sync_all();
+    if (job_of(first).live > 0 && warp == 8) cluster_sync_all();
     cluster_sync_all();
   }
   tc_fence_before();
@@ -1098,12 +1131,20 @@ int launch_direct(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
     default: return launch_direct_as<128>(h, a, st);
   }
 }
-template <int RP>
-int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int64_t jobs, int cs, cudaStream_t st) {
+template <int RP, bool ONE>
+int launch_grad_jobs(const Handle* h, const AdapterGradArgs& a, int64_t clusters, int cs, cudaStream_t st) {
   static bool done[64];
-  if (int rc = allow_smem(h, adapter_grad_kernel<RP>, GradCfg<RP>::SMEM, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_grad_kernel<RP>, jobs, cs, kGradThreads, GradCfg<RP>::SMEM, st, a));
+  if (int rc = allow_smem(h, adapter_grad_kernel<RP, ONE>, GradCfg<RP>::SMEM, done)) return rc;
+  MG_CUDA(launch_clusters(adapter_grad_kernel<RP, ONE>, clusters, cs, kGradThreads, GradCfg<RP>::SMEM, st, a));
   return MG_OK;
+}
+template <int RP>
+int launch_grad_as(const Handle* h, const AdapterGradArgs& a, bool few, int cs, cudaStream_t st) {
+  // Blocks that stay and take job after job where a job is a step or two, more of a block's setting up than of copies: 64 adapters of 4
+  // rows, 2 x 16 blocks of columns, us, a job to a block 22, so 11.  Where jobs are long the SMs' shares come out too unequal: 768 rows,
+  // 16 blocks, 52 and 83.
+  const int most = GradCfg<RP>::BLOCKS * h->sm_count;
+  return few && cs == 1 && a.jobs > most ? launch_grad_jobs<RP, false>(h, a, most, 1, st) : launch_grad_jobs<RP, true>(h, a, a.jobs, cs, st);
 }
 
 }  // namespace
@@ -1187,15 +1228,17 @@ int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout,
   b.rank = a.rank;
   b.order = a.order;
   b.segs = reinterpret_cast<const int2*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
-  const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);
+  const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);       // below 2^28
+  b.jobs = static_cast<int>(jobs);
   // an adapter's rows among several blocks where there are few blocks, while each has two steps, were all adapters alike
   int cs = 8;
   while (cs > 1 && (rows / d->n_adapters < 128 * cs || jobs * cs > 4 * GradCfg<16>::BLOCKS * h->sm_count)) cs /= 2;
+  const bool few = rows / d->n_adapters <= 2 * kAdapterTile;        // rows that lie sorted have 128 and more to an adapter
   switch (padded_rank(a.rank)) {
-    case 16: return launch_grad_as<16>(h, b, jobs, cs, st);
-    case 32: return launch_grad_as<32>(h, b, jobs, cs, st);
-    case 64: return launch_grad_as<64>(h, b, jobs, cs, st);
-    default: return launch_grad_as<128>(h, b, jobs, cs, st);
+    case 16: return launch_grad_as<16>(h, b, few, cs, st);
+    case 32: return launch_grad_as<32>(h, b, few, cs, st);
+    case 64: return launch_grad_as<64>(h, b, few, cs, st);
+    default: return launch_grad_as<128>(h, b, few, cs, st);
   }
 }
 
