@@ -545,7 +545,8 @@ int mg_moe_block_forward(mg_handle h, const void* d_hidden, const void* d_norm_w
  * device.
  *
  * mg_add_rmsnorm: sum = h = bf16(x + residual), out = bf16(weight * (h * rstd)), rstd = 1 / sqrt(mean(h^2) + eps): one rounding, where
- *   mg_rmsnorm has its module's second one before the weight.  Without a residual (NULL) h is x and d_sum is not written.  d_sum and d_out may each be d_x or d_residual with its stride, not one another, and overlap nothing otherwise.
+ *   mg_rmsnorm has its module's second one before the weight.  Without a residual (NULL) h is x and d_sum is not written.  d_sum and
+ *   d_out may each be d_x or d_residual with its stride, not one another, and overlap nothing otherwise.
  * mg_add_rmsnorm_int8: the rows v = weight * (h * rstd) in fp32, quantised as mg_quantize_rows_int8 does a row: bytes ldq apart
  *   and one scale.  There is no rounding to bf16 in between.  d_q overlaps nothing.
  * mg_add_rmsnorm_grad: with n = h * rstd, the forward's roundings counting as the identity,
@@ -570,8 +571,8 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
 /* ---- low-rank adapters beside a projection --------------------------------------------------- */
 /* For rows that belong to different requests, or to different experts, each with an adapter of its own beside the weights that
  * all share (mg_int8_linear, mg_expert_ffn, ...).  No counterpart in the reference.  For the rows t of adapter g:
- *   s[t] = bf16(x[t] . down[g]^T),   out[t] = y[t] + f[g] * s[t] . up[g]^T,   f[g] = factor * d_scale[g] (d_scale NULL: factor)
- * with fp32 sums, out rounded once; out[t] = y[t] for rows without an adapter.
+ *   s[t] = x[t] . down[g]^T,   out[t] = y[t] + f[g] * s[t] . up[g]^T,   f[g] = factor * d_scale[g] (d_scale NULL: factor)
+ * with fp32 sums, s taken to 16 bits, out rounded once; out[t] = y[t] for rows without an adapter.
  * down is [n_adapters][rank][cols], up [n_adapters][n_out][rank], bf16, with the rows of either matrix ld_* and the matrices *_stride
  * elements apart.  All rows (x, y, out, gradients, down, up) begin on 16-byte boundaries: strides are multiples of 8.  Adapters of
  * a lower rank are filled up with zeros.  rank <= 128, n_adapters <= MG_ADAPTER_MAX, cols and n_out <= 2^24, rows < 2^28.
@@ -583,13 +584,13 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
  *   pad_offsets[n_adapters + 1]: adapter g has the rows [pad_offsets[g], pad_offsets[g] + counts[g]).  Offsets that leave
  *   [0, n_rows] or descend are cut off.
  * mg_adapter_add: with d_ids and no plan (NULL) up to MG_ADAPTER_DIRECT rows in one launch; with a plan any number, and d_ids is not
- *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s: [n_rows]
+ *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s in bf16: [n_rows]
  *   rows of mg_adapter_rank_stride(rank) elements, zeros behind the rank and for rows without an adapter.
- * mg_adapter_grad: the gradients, s and gs = bf16(f[g] * grad_out . up[g]) counting as unrounded:
+ * mg_adapter_grad: the gradients, with gs[t] = f[g] * grad_out[t] . up[g], taken to 16 bits for grad_x, and like s to bf16 for the others:
  *     grad_x[t] = gs[t] . down[g],   grad_down[g] = sum_t gs[t]^T x[t],   grad_up[g] = f[g] * sum_t grad_out[t]^T s[t]
  *   grad_x is zero in rows without an adapter, grad_down [n_adapters][rank][cols] and grad_up [n_adapters][n_out][rank] (bf16, contiguous,
  *   rounded once) in adapters without rows.  Each may be NULL and is then not computed.  The gradient of y is grad_out itself.  d_gs:
- *   scratch like d_s.  d_s is read for grad_up alone.  The same rows and plan give the same bits. */
+ *   scratch like d_s.  d_s is read for grad_up alone.  What is written overlaps nothing.  The same rows and plan give the same bits. */
 #define MG_ADAPTER_MAX     1024
 #define MG_ADAPTER_DIRECT   256
 typedef struct mg_adapters {

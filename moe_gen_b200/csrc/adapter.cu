@@ -1,15 +1,15 @@
 // Low-rank adapters beside a projection, an adapter to a row, and their gradients.  For the rows t of adapter g:
-//   s[t] = bf16(x[t] . down[g]^T)                 out[t] = y[t] + scale[g] * s[t] . up[g]^T
-//   gs[t] = bf16(scale[g] * gout[t] . up[g])      gx[t] = gs[t] . down[g]
+//   s[t] = x[t] . down[g]^T                       out[t] = y[t] + scale[g] * s[t] . up[g]^T
+//   gs[t] = scale[g] * gout[t] . up[g]            gx[t] = gs[t] . down[g]
 //   gdown[g] = sum_t gs[t]^T x[t]                 gup[g] = scale[g] * sum_t gout[t]^T s[t]
-// Sums are in fp32; s and gs are rounded to bf16, the type that the matrix instructions take and that an adapter of bf16 modules
-// has between its two products.
+// Sums are in fp32.  s and gs enter the second product as two bf16 numbers each, the nearest and what it leaves, so that they have 16
+// bits there: rounded to 8 they would add an error of their own, as large as that of the outputs' rounding.  They are kept for gdown and
+// gup in 8 bits, where the other factor, x or gout, has no more.
 //
-// Rows of one adapter are worked on in tiles, by the plan's order.  One launch does both products of a tile: a cluster of one to
-// eight blocks splits the first product over its inner size and the second over its outputs, and joins s through distributed
-// shared memory.  Operands go from global memory into registers in the layout of the MMA's fragments: the inner index of a product
-// may be permuted at will, so a thread takes 16 adjacent bytes of a row where the fragment names two and two elements apart, and
-// the outputs' index too, so that it ends with 16 adjacent bytes of a row of out.
+// Rows of one adapter are worked on in tiles, and one launch does both products of a tile: a cluster of one to eight blocks splits the
+// first over its inner size and the second over its outputs, and joins s through distributed shared memory, always in the blocks' order.
+// What has to be moved is x, y and out once and each adapter once; a tile of few rows is bound by the latency of its two chains of copies,
+// one of many by the bytes.
 #include "tc.cuh"
 
 namespace mg {
@@ -150,7 +150,13 @@ struct AdapterArgs {
 };
 
 // ---- few rows, without a plan ------------------------------------------------------------------
-// Tiles of sixteen rows, which the kernel finds by itself: what counts is the latency and the adapters' bytes.  Operands go through a ring
+// Tiles of sixteen rows, which the kernel finds by itself: what counts is the latency and the adapters' bytes.  In us, here and by a plan
+// that is made already (making it takes 2 to 5 more), K = N = 4096, rank 16: 1 row 6.0 and 16.1, 32 rows with 64 adapters 7.8 and 19.4,
+// 128 rows 14.4 and 35.6, 256 rows 14.9 and 37.4, with 8 adapters 12.5 and 17.3; rank 64, 64 adapters 35.3 and 50.3; rank 128, 8 adapters
+// 27.9 and 22.0.  Beyond 256 rows there is no thread to a row for the search, and the plan's larger tiles read the adapters less often.
+// 201 rows of 64 adapters, 5120 to 1000 columns, rank 12: 11.5 us for 12 MB; bound by two chains of copy, wait and product with a meeting
+// of the cluster between them.
+// Operands go through a ring
 // that every thread fills for itself, in the layout of its MMA fragments: the inner index of a product may be permuted at will, so a
 // thread takes 16 adjacent bytes of a row where the fragment names two and two elements apart, and the outputs' index too, so that it
 // ends with 16 adjacent bytes of a row of out.
@@ -367,9 +373,11 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
 // 128 rows of one adapter on the accumulator's lanes.  A step is 64 columns of x, or 64 columns of out; its tiles are copied to shared memory as
 // the tensor core reads them, a few steps ahead (rows wherever the order says, zeros behind what a row or the rank has).  Eight warps copy
 // the first product's, then finish s and the outputs, while four others copy the second product's; one has the products done, into tensor
-// memory.  s passes through shared memory in two parts of bf16, so that it has 16 bits of mantissa in the second product.  A cluster of up
-// to eight blocks shares a tile where there are few: each sums s over its columns of x, then over the blocks for its share of the rows, and
-// hands that to all.
+// memory.  s passes through shared memory in two parts of bf16.  A cluster of up to eight blocks shares a tile where there are few: each sums
+// s over its columns of x, then over the blocks for its share of the rows, and hands that to all.
+// 8192 rows of 4096 to 4096 columns, rank 64, 8 adapters: 54 us for 210 MB, 3.9 TB/s; 49152 rows of 2048 to 2048, rank 16, 64 adapters:
+// 145 us for 600 MB, 4.2 TB/s, the way back 111 us for 400 MB.  What bounds it is the chain within a block, fill, first product, s, second
+// product, drain: two blocks to an SM cover one another's gaps in part.  By MMAs of warps on tiles of 16 rows the first took 88 us.
 constexpr int kFinishWarps = 8, kCopyWarps = 4, kTileThreads = 32 * (kFinishWarps + kCopyWarps + 1);
 template <int RP>
 struct TileCfg {
@@ -389,9 +397,6 @@ __device__ __forceinline__ uint64_t rows_desc(uint32_t saddr, uint32_t outer_byt
 __host__ __device__ constexpr uint32_t mma_shape(int n) { return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n) >> 3 << 17) | (8u << 24); }
 constexpr uint32_t kRowsA = 1u << 15, kRowsB = 1u << 16;        // operand A, B by rows_desc
 
-// What one of WARPS warps' threads copies of a step: 16 bytes of some rows of the tile of rows, 128 bytes of a row side by side (with 64 the load and
-// store unit was what 8192 rows of 4096 x 4096 waited for; rows that are not there are the last one again), and pieces of the adapter's tile,
-// RP rows of 64 elements (wide) or 64 rows of RP (narrow).
 // for the tensor core: this warp's copies but those of the last LEFT steps, and what it has written before
 template <int LEFT>
 __device__ __forceinline__ void arrive(uint64_t* full) {
@@ -401,6 +406,9 @@ __device__ __forceinline__ void arrive(uint64_t* full) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(full));
 }
+// What one of WARPS warps' threads copies of a step: 16 bytes of some rows of the tile of rows, 128 bytes of a row side by side (with 64 the load and
+// store unit was what 8192 rows of 4096 x 4096 waited for; rows that are not there are the last one again), and pieces of the adapter's tile,
+// RP rows of 64 elements (wide) or 64 rows of RP (narrow).
 template <int RP, bool BACK, int WARPS>
 struct TileCopies {
   using C = TileCfg<RP>;
@@ -733,6 +741,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 // adapter, on the accumulator's lanes, for all of the rank; a block goes through its rows 64 at a time, then to its next job, whose first
 // copies are on their way meanwhile.  Where there are few jobs a cluster's blocks take the steps of one in turn, and their sums meet in a
 // fixed order.  The inner index is the rows', so both operands are read as they lie.
+// 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 85 us for 410 MB, 4.8 TB/s; a job's end, its last product and its sums on their
+// way out, is what two blocks to an SM do not quite cover.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
@@ -1097,6 +1107,7 @@ template <int RP>
 int launch_direct_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   static bool done[64];
   if (int rc = allow_smem(h, adapter_direct_kernel<RP>, DirectCfg<RP>::SMEM, done)) return rc;
+  // Blocks to a row's cluster; those whose row begins no tile end at once.  201 rows, us, with 2: 13.3, 4: 11.2, 8: 14.6.
   int cs = 8;
   while (cs > 2 && static_cast<int64_t>(a.n_rows) * cs > 8 * h->sm_count) cs /= 2;
   MG_CUDA(launch_clusters(adapter_direct_kernel<RP>, a.n_rows, cs, kAdapterThreads, DirectCfg<RP>::SMEM, st, a));
@@ -1107,7 +1118,9 @@ int launch_tiles_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   using C = TileCfg<RP>;
   static bool done[64];
   if (int rc = allow_smem(h, adapter_tile_kernel<RP, BACK>, C::SMEM, done)) return rc;
-  // as many blocks to a tile as run at once, were all tiles full
+  // As many blocks to a tile as run at once, were all tiles full.  K = N = 4096, 8 adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16
+  // 92, 50, 29, 18; 4096 rows 93, 52, 34, 36; 8192 rows rank 64 107, 65, 55, 68; 16384 rows rank 16 101, 83, 90, 98; 32768 rows 151,
+  // 161, 164, 179.
   const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile;
   int cs = 8;
   while (cs > 1 && full * cs > C::BLOCKS * h->sm_count) cs /= 2;

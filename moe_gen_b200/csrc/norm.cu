@@ -10,7 +10,11 @@ namespace mg {
 namespace {
 
 constexpr int kNormLanes = 256;          // lanes over which a row's squares are summed, whatever the kernel (as in rmsnorm_kernel)
-constexpr int64_t kNormWarpRows = 2048;  // fewer rows than this have a block each, and its latency
+// From this many rows of at most 1024 columns on a warp takes a row; us, a warp to a row and a block to a row, bf16 rows (8-bit rows):
+//   512 columns: 1024 rows 2.6 (2.8) and 2.5 (3.3), 2048 rows 2.8 (3.1) and 3.6 (5.1), 16384 rows 10.1 (11.0) and 20.7 (29.5)
+//   1024 columns: 1024 rows 3.4 (3.7) and 2.7 (3.4), 2048 rows 3.8 (4.2) and 4.1 (5.3), 16384 rows 21.4 (21.3) and 26.7 (33.6)
+//   2048 columns: 2048 rows 7.4 (8.6) and 6.0 (7.0), 8192 rows 25.1 (26.1) and 21.5 (22.6): the block, at any number of rows
+constexpr int64_t kNormWarpRows = 2048;
 
 enum NormOut { NORM_BF16, NORM_AS_MODULE, NORM_INT8 };
 struct NormArgs {
@@ -96,7 +100,9 @@ __device__ __forceinline__ uint2 bytes8(const float* f, float inv) {
   return make_uint2(w[0], w[1]);
 }
 
-// A block per row of whole 16-byte vectors, which stay in registers between the sum and the output.
+// A block per row of whole 16-byte vectors, which stay in registers between the sum and the output: each byte is moved once, and
+// memory is what bounds it.  16384 rows of 7168 columns with a residual (four rows' bytes moved per row): 136.5 us, 6.9 TB/s; 8-bit
+// rows, 8192 of them: 66.7 us, 6.2 TB/s; one row of 2048 columns: 1.8 us, a launch and one trip to memory.
 template <int VECS, int OUT>
 __global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) {
   __shared__ float s_sum[kNormLanes / 32];
@@ -177,7 +183,8 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_kernel(const NormArgs a) 
   if (threadIdx.x == 0) a.scale[row] = scale;
 }
 
-// A warp per row, for many short rows.  Its lanes hold what lanes 32 apart would hold in a block, summed in the same order.
+// A warp per row, for many short rows, where a block's start and its meeting cost more than its bytes.  Its lanes hold what lanes 32
+// apart would hold in a block, summed in the same order.
 template <int VECS, int OUT>
 __global__ void __launch_bounds__(256) add_norm_short_kernel(const NormArgs a) {
   const int lane = threadIdx.x & 31;
@@ -303,6 +310,8 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs
 // mean(w gy n) = rstd sum(w gy h) / cols, so that both sums of a row come from one reading.  Blocks stay and take rows in turn; a
 // thread holds the same columns of every row, and its share of gw in fp32.  The shares are summed by a second launch, in the order of
 // the blocks, or, few rows, in the same one by a cluster's blocks, so that the same rows and columns give the same bits.
+// 8192 rows of 7168 columns with gh: 85 us for 470 MB, 5.5 TB/s.  What bounds it is the time between a row's arrival and its block's
+// meeting, so that rows are copied ahead into a ring; loads into registers and products one by one took 152 us.
 struct NormGradArgs {
   const uint16_t* gy;
   int64_t ldgy;
@@ -524,7 +533,9 @@ __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* parts,
   if (x == 0 && blockIdx.x * 32 + y < cols) gw[blockIdx.x * 32 + y] = v;
 }
 
-// us in a graph, and on their way from Python, by two launches and by one: 1 row of 2048 columns X
+// Two launches and one, us in a graph: 1 row of 2048 columns 4.2 and 4.8, 16 rows 4.4 and 5.4, 37 rows 4.8 and 7.2, 64 rows 5.4 and 9.2,
+// 128 rows 5.3 and 14.0.  A call from Python at 37 rows: 18.0 and 12.2, since two launches and their scratch cost the host more than
+// the device gains; from MG_NORM_GRAD_FEW rows on the device's side wins.
 constexpr int kGradCluster = 8;
 struct NormGradPlan { int vecs, lanes, threads, blocks, shares; bool few; };
 NormGradPlan norm_grad_plan(const Handle* h, int64_t n, int64_t cols) {
@@ -551,7 +562,7 @@ int launch_add_norm_as(const NormArgs& a, cudaStream_t st) {
   const unsigned rows = static_cast<unsigned>(a.n), eighth = static_cast<unsigned>((a.n + 7) / 8);
   if (!wide) add_norm_any_kernel<OUT><<<rows, kNormLanes, 0, st>>>(a);
   else if (a.n >= kNormWarpRows && vecs <= 64) add_norm_short_kernel<2, OUT><<<eighth, 256, 0, st>>>(a);
-  else if (a.n >= kNormWarpRows && vecs <= 256) add_norm_short_kernel<8, OUT><<<eighth, 256, 0, st>>>(a);
+  else if (a.n >= kNormWarpRows && vecs <= 128) add_norm_short_kernel<4, OUT><<<eighth, 256, 0, st>>>(a);
   else if (vecs <= kNormLanes) add_norm_kernel<1, OUT><<<rows, kNormLanes, 0, st>>>(a);
   else if (vecs <= 2 * kNormLanes) add_norm_kernel<2, OUT><<<rows, kNormLanes, 0, st>>>(a);
   else if (vecs <= 4 * kNormLanes) add_norm_kernel<4, OUT><<<rows, kNormLanes, 0, st>>>(a);

@@ -102,14 +102,15 @@ class _AdaptRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, down, up, layer, plan, scale):
         out, s = layer.adapter_add(y, x, down, up, plan, scale, keep=True)
-        ctx.layer, ctx.plan, ctx.scale = layer, plan, scale
-        ctx.save_for_backward(x, down, up, s)
+        ctx.layer, ctx.plan = layer, plan
+        ctx.scale, kept = (None, (scale,)) if isinstance(scale, torch.Tensor) else (scale, ())
+        ctx.save_for_backward(x, down, up, s, *kept)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        x, down, up, s = ctx.saved_tensors
+        x, down, up, s, *kept = ctx.saved_tensors
         need = ctx.needs_input_grad
         gx = gdown = gup = None
         if any(need[1:4]):
@@ -118,7 +119,7 @@ class _AdaptRows(torch.autograd.Function):
             if n_out % 8:               # rows on 16-byte boundaries
                 rows = torch.empty_strided(grad_out.shape, ((n_out + 7) // 8 * 8, 1), dtype=grad_out.dtype, device=grad_out.device)
                 rows.copy_(grad_out)
-            gx, gdown, gup = ctx.layer.adapter_grad(rows, x, down, up, ctx.plan, ctx.scale, s, *need[1:4])
+            gx, gdown, gup = ctx.layer.adapter_grad(rows, x, down, up, ctx.plan, kept[0] if kept else ctx.scale, s, *need[1:4])
         return grad_out if need[0] else None, gx, gdown, gup, None, None, None
 
 
@@ -149,4 +150,6 @@ def add_norm(layer: MoELayer, x: torch.Tensor, residual: Optional[torch.Tensor],
 def adapt_rows(layer: MoELayer, y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan: AdapterPlan,
                scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """MoELayer.adapter_add by a plan, differentiable in y, x, down and up (the scales are constants)."""
+    if isinstance(scale, torch.Tensor) and scale.requires_grad:
+        raise ValueError("adapt_rows has no gradient for its scales: detach them")
     return _AdaptRows.apply(y, x, down, up, layer, plan, scale)

@@ -297,6 +297,45 @@ def test_autograd(layer):
         assert torch.equal(got[0], want[1])
 
 
+def test_scales_stay_what_they_were(layer):
+    from moe_gen_b200 import adapt_rows
+    x, y = _rows(20, 64, 1), _rows(20, 64, 2)
+    down, up, scale = _adapters(3, 8, 64, 64, 4)
+    plan = layer.adapter_plan(_ids(20, 3, 5), 3)
+    with pytest.raises(ValueError, match="detach"):
+        adapt_rows(layer, y, x, down, up, plan, scale.clone().requires_grad_(True))
+    leaf = x.clone().requires_grad_(True)
+    out = adapt_rows(layer, y, leaf, down, up, plan, scale)
+    scale.mul_(2.0)                         # the gradient would be another product's
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, leaf, y)
+
+
+@pytest.mark.parametrize("n", (1, 100, 900))
+def test_a_replayed_call_takes_the_ids_that_are_there(layer, n):
+    x, y, go = _rows(n, 512, 1).clone(), _rows(n, 384, 2).clone(), _rows(n, 384, 6).clone()
+    down, up, scale = _adapters(6, 32, 512, 384, 3)
+    ids = _ids(n, 6, 4).clone()
+
+    def step():
+        out, s = layer.adapter_add(y, x, down, up, ids, scale, keep=True)
+        return (out, s) + layer.adapter_grad(go, x, down, up, ids, scale, s)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (5, 6, 7):
+        ids.copy_(_ids(n, 6, seed) if seed < 7 else torch.full_like(ids, -1))
+        x.copy_(_rows(n, 512, 10 + seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(kept, step()))
+        assert seed < 7 or (torch.equal(kept[0], y) and not any(t.any() for t in kept[1:]))
+
+
 def test_gradient_against_differences(layer):
     """L = sum(go * out) is linear in down and in up by themselves: its difference along a direction is the gradient's product with it, up to
     the gradients' roundings."""

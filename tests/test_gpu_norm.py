@@ -73,7 +73,7 @@ def test_rows_and_sum(layer, n, cols, residual):
     assert q.to(torch.int32).abs().max() <= 127
 
 
-@pytest.mark.parametrize("n,H", [(1, 256), (37, 2048), (2300, 1024), (2300, 2048), (64, 4096), (16, 7168), (5, 8192), (2, 16384)])
+@pytest.mark.parametrize("n,H", [(1, 256), (37, 2048), (2300, 512), (2300, 1024), (2300, 2048), (64, 4096), (16, 7168), (5, 8192), (2, 16384)])
 def test_the_same_bits_by_every_kernel(layer, n, H):
     """A row's bits do not depend on the batch, the strides or the alignment."""
     w = _weight(H, 5)
