@@ -584,9 +584,10 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
  *   pad_offsets[n_adapters + 1]: adapter g has the rows [pad_offsets[g], pad_offsets[g] + counts[g]).  Offsets that leave
  *   [0, n_rows] or descend are cut off.
  * mg_adapter_add: with d_ids and no plan (NULL) up to MG_ADAPTER_DIRECT rows in one launch; with a plan any number, and d_ids is not
- *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s in bf16: [n_rows]
- *   rows of mg_adapter_rank_stride(rank) elements, zeros behind the rank and for rows without an adapter.
- * mg_adapter_grad: the gradients, with gs[t] = f[g] * grad_out[t] . up[g], taken to 16 bits for grad_x, and like s to bf16 for the others:
+ *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s for mg_adapter_grad:
+ *   [n_rows] rows of mg_adapter_rank_stride(rank) elements, s rounded to bf16 in their first half and what that leaves in the
+ *   second, zeros behind the rank and for rows without an adapter.
+ * mg_adapter_grad: the gradients, with gs[t] = f[g] * grad_out[t] . up[g], taken to 16 bits like s:
  *     grad_x[t] = gs[t] . down[g],   grad_down[g] = sum_t gs[t]^T x[t],   grad_up[g] = f[g] * sum_t grad_out[t]^T s[t]
  *   grad_x is zero in rows without an adapter, grad_down [n_adapters][rank][cols] and grad_up [n_adapters][n_out][rank] (bf16, contiguous,
  *   rounded once) in adapters without rows.  Each may be NULL and is then not computed.  The gradient of y is grad_out itself.  d_gs:

@@ -1563,7 +1563,7 @@ static int check_adapters(const char* what, const mg_adapters* a) {
 int mg_adapter_rank_stride(int32_t rank, int32_t* elements) {
   MG_REQUIRE(elements, MG_ERR_NULL, "null argument");
   MG_REQUIRE(rank >= 1 && rank <= 128, MG_ERR_LIMIT, "mg_adapter_rank_stride: rank %d, at most 128", rank);
-  *elements = adapter_padded_rank(rank);
+  *elements = adapter_rank_stride(rank);
   return MG_OK;
 }
 

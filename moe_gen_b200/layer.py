@@ -732,8 +732,8 @@ class MoELayer:
         x [rows, cols] and y [rows, n_out], down [adapters, rank, cols] and up [adapters, n_out, rank], bf16 with rows on 16-byte
         boundaries (views will do); rank at most 128, a lower one filled up with zeros.  who: int32 ids [rows], outside [0, adapters)
         for none, or the plan made of them (adapter_plan, adapter_plan_sorted), once for all of a batch's projections.  scale: a number or
-        fp32 [adapters].  out may be y, and overlaps nothing otherwise.  With keep also the rows between the two products, bf16,
-        for adapter_grad: (out, s).  Any layer serves."""
+        fp32 [adapters].  out may be y, and overlaps nothing otherwise.  With keep also the rows between the two products, in two
+        parts of bf16, for adapter_grad: (out, s).  Any layer serves."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
         ad, n_adapters, rank, a_cols, a_out = self._adapters(down, up, scale)
         if cols != a_cols:

@@ -108,7 +108,7 @@ def test_plans_that_are_refused(handle):
     assert lib.mg_adapter_plan_sorted(handle[0], None, P, 4, 4, P, None) == -1
     assert lib.mg_adapter_plan_sorted(handle[0], P, None, 4, 4, P, None) == -1
     assert lib.mg_adapter_plan_sorted(handle[0], P, P, 4, 4, P + 8, None) == -2
-    for rank, stride in ((1, 16), (16, 16), (17, 32), (33, 64), (65, 128), (128, 128)):
+    for rank, stride in ((1, 32), (16, 32), (17, 64), (33, 128), (65, 256), (128, 256)):
         assert lib.mg_adapter_rank_stride(rank, C.byref(r)) == 0 and r.value == stride
     assert lib.mg_adapter_rank_stride(0, C.byref(r)) == -7 and lib.mg_adapter_rank_stride(129, C.byref(r)) == -7
 
