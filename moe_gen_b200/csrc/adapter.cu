@@ -750,8 +750,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 // copies are on their way meanwhile.  Where there are few jobs a cluster's blocks take the steps of one in turn, and their sums meet in a
 // fixed order.  The inner index is the rows', so both operands are read as they lie.  The narrow rows' two parts are columns side by side,
 // whose sums are added at the end.
-// 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 85 us for 410 MB, 4.8 TB/s; a job's end, its last product and its sums on their
-// way out, is what two blocks to an SM do not quite cover.
+// 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 77 us for 410 MB, 5.3 TB/s, by three blocks to an SM with rings of three stages
+// (two with four: 84); a job's end, its last product and its sums on their way out, is what they do not quite cover.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
@@ -761,7 +761,7 @@ struct AdapterGradArgs {
   const float* scale;
   float factor;
   int rank, jobs;
-  const int2* segs;             // first entry of order and rows of every adapter
+  const int4* segs;             // first entry of order, rows and number of every adapter, those of most rows first
   const int32_t* order;
   int32_t* status;
 };
@@ -769,7 +769,7 @@ struct AdapterGradArgs {
 constexpr int kGradThreads = kAdapterThreads + 32;
 template <int RP>
 struct GradCfg {
-  static constexpr int BLOCKS = RP <= 64 ? 2 : 1, STAGES = RP == 64 ? 3 : 4;
+  static constexpr int BLOCKS = RP <= 32 ? 3 : RP <= 64 ? 2 : 1, STAGES = RP <= 64 ? 3 : 4;
   static constexpr int NR = 2 * RP, HALVES = NR <= 64 ? 1 : NR / 64;             // columns of a narrow row, in blocks of 64
   static constexpr int WIDE = 16384;                           // bytes of a stage: two blocks of 64 columns by 64 rows, then the narrow rows
   static constexpr int STAGE = WIDE + HALVES * 8192;
@@ -778,7 +778,7 @@ struct GradCfg {
   static_assert(128 * RP * 4 <= STAGES * STAGE && BLOCKS * (SMEM + 1536) <= 227 * 1024, "shared memory");
 };
 
-// ONE: a job to a block (to a cluster), else every gridDim.x-th
+// ONE: a job to a block (to a cluster), else one of every gridDim.x
 template <int RP, bool ONE>
 __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
   using C = GradCfg<RP>;
@@ -797,18 +797,20 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
   auto job_of = [&](int n) {
     Job j;
     const int per = a.blocks[0] + a.blocks[1];
-    j.g = n / per;
-    const int block = n - j.g * per;
+    const int at = n / per, block = n - at * per;
     j.which = block >= a.blocks[0];
     j.c0 = (block - (j.which ? a.blocks[0] : 0)) * 128;
-    const int2 seg = a.segs[j.g];
+    const int4 seg = a.segs[at];
     j.start = seg.x;
     j.live = seg.y;
+    j.g = seg.z;
     const int all = (seg.y + 63) / 64;
     j.steps = cr < all ? (all - cr + cs - 1) / cs : 0;
     return j;
   };
   const int first = ONE ? static_cast<int>(blockIdx.x) / cs : static_cast<int>(blockIdx.x), last = ONE ? first + 1 : a.jobs;
+  // the jobs' lengths descend: turns go to and fro, the last block of one being the first of the next
+  const int both = 2 * static_cast<int>(gridDim.x), hop0 = ONE ? 1 : both - 1 - 2 * first;
   if (tid == 0) {
     for (int k = 0; k < S; ++k) { mbar_init(smem_u32(&s_full[k]), kAdapterThreads / 32); mbar_init(smem_u32(&s_done[k]), 1); }
     s_abort = 0;
@@ -826,7 +828,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
 
   if (warp == 8) {
     int k = 0;
-    for (int n = first; n < last; n += ONE ? 1 : gridDim.x) {
+    for (int n = first, hop = hop0; n < last; n += hop, hop = both - hop) {
       const int steps = job_of(n).steps;
       for (int i = 0; i < steps; ++i, ++k) {
         wait_warp(smem_u32(&s_full[k % S]), (k / S) & 1, &s_abort, a.status, 127);       // a job's first: also that the accumulator has been read
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
     const int r0 = tid >> 3, p = tid & 7;              // this thread's 16 bytes of rows r0 and r0 + 32, of 128 bytes each
     const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
     // the next step to fetch: its job, its number in it, its rows
-    int ahead = first, in = 0, rows[2];
+    int ahead = first, ahead_hop = hop0, in = 0, rows[2];
     Job f = job_of(first);
     uint32_t filling = ring;
     auto look = [&]() {
@@ -857,7 +859,8 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
     };
     auto next_job = [&]() {
       do {
-        ahead += gridDim.x;
+        ahead += ahead_hop;
+        ahead_hop = both - ahead_hop;
         if (ahead < last) f = job_of(ahead);
       } while (ahead < last && f.steps == 0);
       in = 0;
@@ -893,7 +896,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_gra
 #pragma unroll 1
     for (int k = 0; k < S - 1; ++k) fetch();
     int k = 0;
-    for (int n = first; n < last; n += ONE ? 1 : gridDim.x) {
+    for (int n = first, hop = hop0; n < last; n += hop, hop = both - hop) {
       const Job j = job_of(n);
       const int cols = j.which ? a.cols[1] : a.cols[0];
       uint16_t* out = (j.which ? a.out[1] : a.out[0]) + static_cast<int64_t>(j.g) * a.rank * cols;
@@ -986,7 +989,7 @@ PlanLayout plan_layout(int64_t rows, int64_t adapters) {
   const int64_t n = (rows + kAdapterTile - 1) / kAdapterTile + adapters + 1;
   p.tiles = 0;
   p.segs = 4 * n;
-  p.order = p.segs + 2 * (adapters + (adapters & 1));
+  p.order = p.segs + 4 * adapters;
   p.place = p.order + rows;                // while the plan is made
   p.words = p.place + rows;
   return p;
@@ -997,7 +1000,7 @@ PlanLayout plan_layout(int64_t rows, int64_t adapters) {
 // SORTED: the rows lie in segments already (pad_offsets, counts); the order is the rows' own, written by the other blocks.
 template <bool SORTED>
 __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int32_t* ids, const int32_t* counts, const int32_t* pad,
-                                                                       int rows, int adapters, int n_tiles, int4* tiles, int2* segs,
+                                                                       int rows, int adapters, int n_tiles, int4* tiles, int4* segs,
                                                                        int32_t* order, int32_t* place) {
   extern __shared__ __align__(16) int s_mem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, groups = adapters + 1;
@@ -1091,7 +1094,17 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
     }
   }
   __syncthreads();
-  for (int e = tid; e < adapters; e += blockDim.x) segs[e] = make_int2(s_start[e], s_live[e]);
+  static_assert(MG_ADAPTER_MAX <= kPlanWarps * 32, "a thread to an adapter");
+  {                                        // the adapters by their rows: 2^bits neighbouring threads compare one with all
+    int bits = 5;
+    while (bits > 0 && adapters << bits > kPlanWarps * 32) --bits;
+    const int e = tid >> bits, n = e < adapters ? s_live[e] : 0;
+    int before = 0;
+    if (e < adapters)
+      for (int f = tid & ((1 << bits) - 1); f < adapters; f += 1 << bits) before += s_live[f] > n || (s_live[f] == n && f < e);
+    for (int o = 1 << bits >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+    if (e < adapters && (tid & ((1 << bits) - 1)) == 0) segs[before] = make_int4(s_start[e], n, e, 0);
+  }
   for (int e = tid; e < n_tiles; e += blockDim.x) {
     int4 t = make_int4(-1, 0, 0, 0);
     if (e < s_tile[groups]) {
@@ -1166,12 +1179,12 @@ int launch_grad_jobs(const Handle* h, const AdapterGradArgs& a, int64_t clusters
   return MG_OK;
 }
 template <int RP>
-int launch_grad_as(const Handle* h, const AdapterGradArgs& a, bool few, int cs, cudaStream_t st) {
-  // Blocks that stay and take job after job where a job is a step or two, more of a block's setting up than of copies: 64 adapters of 4
-  // rows, 2 x 16 blocks of columns, us, a job to a block 22, so 11.  Where jobs are long the SMs' shares come out too unequal: 768 rows,
-  // 16 blocks, 52 and 83.
+int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int cs, cudaStream_t st) {
+  // Blocks that stay where there are more jobs than places: the next job's copies are on their way while one ends.  2048 and 2048 columns,
+  // 64 adapters, rank 16, us, a job to a block and so: 4 rows each 19.5 and 14.0, 128 rows 27 and 22, 512 rows 55.8 and 52; 768 rows of a
+  // skewed routing 79 and 79, if the plan names the adapters of most rows first and the turns go to and fro (in the adapters' order 91 and 122).
   const int most = GradCfg<RP>::BLOCKS * h->sm_count;
-  return few && cs == 1 && a.jobs > most ? launch_grad_jobs<RP, false>(h, a, most, 1, st) : launch_grad_jobs<RP, true>(h, a, a.jobs, cs, st);
+  return cs == 1 && a.jobs > most ? launch_grad_jobs<RP, false>(h, a, most, 1, st) : launch_grad_jobs<RP, true>(h, a, a.jobs, cs, st);
 }
 
 }  // namespace
@@ -1191,11 +1204,11 @@ int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* coun
   if (ids != nullptr) {
     if (int rc = allow_smem(h, adapter_plan_kernel<false>, most, done[0])) return rc;
     adapter_plan_kernel<false><<<1, kPlanWarps * 32, smem, st>>>(ids, nullptr, nullptr, static_cast<int>(rows), adapters, n_tiles,
-                                                                reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order, w + p.place);
+                                                                reinterpret_cast<int4*>(w), reinterpret_cast<int4*>(w + p.segs), w + p.order, w + p.place);
   } else {
     const unsigned blocks = static_cast<unsigned>(1 + (rows + kPlanWarps * 32 - 1) / (kPlanWarps * 32));
     adapter_plan_kernel<true><<<blocks, kPlanWarps * 32, smem, st>>>(nullptr, counts, pad, static_cast<int>(rows), adapters, n_tiles,
-                                                                    reinterpret_cast<int4*>(w), reinterpret_cast<int2*>(w + p.segs), w + p.order, w + p.place);
+                                                                    reinterpret_cast<int4*>(w), reinterpret_cast<int4*>(w + p.segs), w + p.order, w + p.place);
   }
   MG_CUDA(cudaGetLastError());
   return MG_OK;
@@ -1254,18 +1267,17 @@ int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout,
   b.factor = a.factor;
   b.rank = a.rank;
   b.order = a.order;
-  b.segs = reinterpret_cast<const int2*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
+  b.segs = reinterpret_cast<const int4*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
   const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);       // below 2^28
   b.jobs = static_cast<int>(jobs);
   // an adapter's rows among several blocks where there are few blocks, while each has two steps, were all adapters alike
   int cs = 8;
   while (cs > 1 && (rows / d->n_adapters < 128 * cs || jobs * cs > 4 * GradCfg<16>::BLOCKS * h->sm_count)) cs /= 2;
-  const bool few = rows / d->n_adapters <= 2 * kAdapterTile;        // rows that lie sorted have 128 and more to an adapter
   switch (padded_rank(a.rank)) {
-    case 16: return launch_grad_as<16>(h, b, few, cs, st);
-    case 32: return launch_grad_as<32>(h, b, few, cs, st);
-    case 64: return launch_grad_as<64>(h, b, few, cs, st);
-    default: return launch_grad_as<128>(h, b, few, cs, st);
+    case 16: return launch_grad_as<16>(h, b, cs, st);
+    case 32: return launch_grad_as<32>(h, b, cs, st);
+    case 64: return launch_grad_as<64>(h, b, cs, st);
+    default: return launch_grad_as<128>(h, b, cs, st);
   }
 }
 
