@@ -750,8 +750,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 // copies are on their way meanwhile.  Where there are few jobs a cluster's blocks take the steps of one in turn, and their sums meet in a
 // fixed order.  The inner index is the rows', so both operands are read as they lie.  The narrow rows' two parts are columns side by side,
 // whose sums are added at the end.
-// 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 77 us for 410 MB, 5.3 TB/s, by three blocks to an SM with rings of three stages
-// (two with four: 84); a job's end, its last product and its sums on their way out, is what they do not quite cover.
+// 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 77 us for 410 MB, 5.3 TB/s; a job's end, its last product and its sums on their
+// way out, is what the SM's other blocks do not quite cover.  Rank 128: 139 us, the narrow rows, twice the wide ones' bytes, from L2.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
@@ -767,9 +767,11 @@ struct AdapterGradArgs {
 };
 
 constexpr int kGradThreads = kAdapterThreads + 32;
-template <int RP>
+// DEEP: two blocks to an SM in the place of three, each with a step more on its way, where no more than two come to an SM anyway.  us, so and
+// with three: 65536 rows of one adapter, 2048 and 2048 columns, rank 16 103 and 139; 49152 rows of 64 adapters 84 and 77.
+template <int RP, bool DEEP>
 struct GradCfg {
-  static constexpr int BLOCKS = RP <= 32 ? 3 : RP <= 64 ? 2 : 1, STAGES = RP <= 64 ? 3 : 4;
+  static constexpr int BLOCKS = RP <= 32 && !DEEP ? 3 : 2, STAGES = RP <= 32 ? (DEEP ? 4 : 3) : RP <= 64 ? 3 : 2;
   static constexpr int NR = 2 * RP, HALVES = NR <= 64 ? 1 : NR / 64;             // columns of a narrow row, in blocks of 64
   static constexpr int WIDE = 16384;                           // bytes of a stage: two blocks of 64 columns by 64 rows, then the narrow rows
   static constexpr int STAGE = WIDE + HALVES * 8192;
@@ -779,9 +781,9 @@ struct GradCfg {
 };
 
 // ONE: a job to a block (to a cluster), else one of every gridDim.x
-template <int RP, bool ONE>
-__global__ void __launch_bounds__(kGradThreads, GradCfg<RP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
-  using C = GradCfg<RP>;
+template <int RP, bool ONE, bool DEEP>
+__global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapter_grad_kernel(const AdapterGradArgs a) {
+  using C = GradCfg<RP, DEEP>;
   constexpr int S = C::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ uint64_t s_full[S], s_done[S];
@@ -1171,11 +1173,11 @@ int launch_direct(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
     default: return launch_direct_as<128>(h, a, st);
   }
 }
-template <int RP, bool ONE>
+template <int RP, bool ONE, bool DEEP>
 int launch_grad_jobs(const Handle* h, const AdapterGradArgs& a, int64_t clusters, int cs, cudaStream_t st) {
   static bool done[64];
-  if (int rc = allow_smem(h, adapter_grad_kernel<RP, ONE>, GradCfg<RP>::SMEM, done)) return rc;
-  MG_CUDA(launch_clusters(adapter_grad_kernel<RP, ONE>, clusters, cs, kGradThreads, GradCfg<RP>::SMEM, st, a));
+  if (int rc = allow_smem(h, adapter_grad_kernel<RP, ONE, DEEP>, GradCfg<RP, DEEP>::SMEM, done)) return rc;
+  MG_CUDA(launch_clusters(adapter_grad_kernel<RP, ONE, DEEP>, clusters, cs, kGradThreads, GradCfg<RP, DEEP>::SMEM, st, a));
   return MG_OK;
 }
 template <int RP>
@@ -1183,8 +1185,11 @@ int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int cs, cudaStream
   // Blocks that stay where there are more jobs than places: the next job's copies are on their way while one ends.  2048 and 2048 columns,
   // 64 adapters, rank 16, us, a job to a block and so: 4 rows each 19.5 and 14.0, 128 rows 27 and 22, 512 rows 55.8 and 52; 768 rows of a
   // skewed routing 79 and 79, if the plan names the adapters of most rows first and the turns go to and fro (in the adapters' order 91 and 122).
-  const int most = GradCfg<RP>::BLOCKS * h->sm_count;
-  return cs == 1 && a.jobs > most ? launch_grad_jobs<RP, false>(h, a, most, 1, st) : launch_grad_jobs<RP, true>(h, a, a.jobs, cs, st);
+  const int most = GradCfg<RP, false>::BLOCKS * h->sm_count;
+  if (cs == 1 && a.jobs > most) return launch_grad_jobs<RP, false, false>(h, a, most, 1, st);
+  constexpr bool choice = GradCfg<RP, true>::BLOCKS < GradCfg<RP, false>::BLOCKS;
+  const bool deep = choice && static_cast<int64_t>(a.jobs) * cs <= 2 * h->sm_count;
+  return deep ? launch_grad_jobs<RP, true, choice>(h, a, a.jobs, cs, st) : launch_grad_jobs<RP, true, false>(h, a, a.jobs, cs, st);
 }
 
 }  // namespace
@@ -1270,9 +1275,11 @@ int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout,
   b.segs = reinterpret_cast<const int4*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
   const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);       // below 2^28
   b.jobs = static_cast<int>(jobs);
-  // an adapter's rows among several blocks where there are few blocks, while each has two steps, were all adapters alike
+  // An adapter's rows among several blocks while all of them run at once, two to an SM, and each has two steps, were all adapters alike.
+  // 2048 and 2048 columns, us, within 2 blocks to an SM, within 4, within 8: 4096 rows of 4 adapters, rank 16 12.7, 15.3, 22.6; 16384 rows
+  // of 8 30.5, 37.1, 39.2; 4096 columns, rank 64 70, 70, 76.
   int cs = 8;
-  while (cs > 1 && (rows / d->n_adapters < 128 * cs || jobs * cs > 4 * GradCfg<16>::BLOCKS * h->sm_count)) cs /= 2;
+  while (cs > 1 && (rows / d->n_adapters < 128 * cs || jobs * cs > 2 * h->sm_count)) cs /= 2;
   switch (padded_rank(a.rank)) {
     case 16: return launch_grad_as<16>(h, b, cs, st);
     case 32: return launch_grad_as<32>(h, b, cs, st);
