@@ -18,22 +18,21 @@ namespace {
 
 constexpr int kAdapterTile = 128;           // rows of a tile of a plan
 constexpr int kDirectTile = 16;             // rows of a tile that the kernel finds by itself
-constexpr int kDirectRows = 256;            // rows of a call without a plan, at most: one to a thread
 constexpr int kAdapterThreads = 256;
+static_assert(MG_ADAPTER_DIRECT <= kAdapterThreads, "rows of a call without a plan: one to a thread");
 
 __device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// BYTES of a row from element c on, into shared memory; what lies at `end` or behind arrives as zeros and is not read.  Rows begin on
+// BYTES (16 or 8) of a row from element c on, into shared memory; what lies at `end` or behind arrives as zeros and is not read.  Rows begin on
 // 16-byte boundaries.
 template <int BYTES>
 __device__ __forceinline__ void copy_row(uint32_t to, const uint16_t* row, int c, int end) {
   const int have = min(max(2 * (end - c), 0), BYTES);
   const uint16_t* from = have > 0 ? row + c : row;          // an address inside the row for a copy of nothing
   if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
-  else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(have) : "memory");
 }
 // 16 bytes of a row, all of them there
 __device__ __forceinline__ void copy_whole(uint32_t to, const uint16_t* from) {
@@ -1195,7 +1194,6 @@ int launch_grad_as(const Handle* h, const AdapterGradArgs& a, int cs, cudaStream
 }  // namespace
 
 int adapter_rank_stride(int rank) { return 2 * padded_rank(rank); }
-int64_t adapter_direct_rows() { return kDirectRows; }
 size_t adapter_plan_bytes(int64_t rows, int64_t adapters) { return static_cast<size_t>(plan_layout(rows, adapters).words) * 4; }
 
 int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* counts, const int32_t* pad, int64_t rows, int adapters,

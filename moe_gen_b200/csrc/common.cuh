@@ -303,7 +303,6 @@ int launch_norm_grad(const Handle* h, const void* gy, int64_t ldgy, const void* 
 
 // low-rank adapters (adapter.cu) ---------------------------------------------------------------
 int adapter_rank_stride(int rank);       // elements between the rows of s and of gs
-int64_t adapter_direct_rows();           // rows of a call without a plan, at most
 size_t adapter_plan_bytes(int64_t rows, int64_t adapters);
 int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* counts, const int32_t* pad, int64_t rows, int adapters,
                         void* plan, cudaStream_t st);

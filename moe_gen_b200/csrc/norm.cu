@@ -310,8 +310,9 @@ __global__ void __launch_bounds__(kNormLanes) add_norm_any_kernel(const NormArgs
 // mean(w gy n) = rstd sum(w gy h) / cols, so that both sums of a row come from one reading.  Blocks stay and take rows in turn; a
 // thread holds the same columns of every row, and its share of gw in fp32.  The shares are summed by a second launch, in the order of
 // the blocks, or, few rows, in the same one by a cluster's blocks, so that the same rows and columns give the same bits.
-// 8192 rows of 7168 columns with gh: 85 us for 470 MB, 5.5 TB/s.  What bounds it is the time between a row's arrival and its block's
-// meeting, so that rows are copied ahead into a ring; loads into registers and products one by one took 152 us.
+// 8192 rows of 7168 columns with gh: 77 us for 470 MB, 6.1 TB/s, where instructions are what it waits for next to memory: two rows meet at
+// once, by sums of which a warp's halves take one each (one row to a meeting and ten exchanges to its sums: 86 us), and what no copy fills
+// is zeros in the ring, so that nothing is selected (rows of 16384 columns 145 and 115 us).  Loads into registers took 152 us.
 struct NormGradArgs {
   const uint16_t* gy;
   int64_t ldgy;
@@ -353,8 +354,9 @@ __device__ __forceinline__ void pairs8(const uint4& v, float2* f) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xFFFF0000u));
 }
-__device__ __forceinline__ void copy_vec(uint4* to, const uint16_t* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+// bytes: 16, or 0 for zeros
+__device__ __forceinline__ void copy_vec(uint4* to, const uint16_t* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
@@ -364,14 +366,36 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// Sums over a warp of two numbers of each of R rows: the lanes of a 2 R-th of the warp end with one of them, first a[0], then b[0], a[1], b[1].
+// Halves of the warp hand each other what they do not go on with, so that there are 5 or 6 exchanges and not 10 R.
+template <int R>
+__device__ __forceinline__ float warp_sums(const float (&a)[R], const float (&b)[R]) {
+  const int lane = threadIdx.x & 31;
+  float v;
+  if (R == 1) {
+    v = lane & 16 ? b[0] : a[0];
+    v += __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? a[0] : b[0], 16);
+    v += __shfl_xor_sync(0xFFFFFFFFu, v, 8);
+  } else {
+    float x = lane & 16 ? a[R - 1] : a[0], y = lane & 16 ? b[R - 1] : b[0];
+    x += __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? a[0] : a[R - 1], 16);
+    y += __shfl_xor_sync(0xFFFFFFFFu, lane & 16 ? b[0] : b[R - 1], 16);
+    v = lane & 8 ? y : x;
+    v += __shfl_xor_sync(0xFFFFFFFFu, lane & 8 ? x : y, 8);
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
 // WIDE: rows of whole 16-byte vectors, several of them on their way to shared memory at a time.  A thread copies what it reads itself, so
 // that it waits for its own copies only.
 // FEW: the grid is one cluster, which sums the shares too.
 template <int VECS, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGradArgs a) {
-  constexpr int STAGES = kGradStages<VECS>;
+  constexpr int STAGES = kGradStages<VECS>, R = WIDE ? STAGES / 2 : 1;          // R: rows to a turn, which meet once
   extern __shared__ __align__(16) uint4 s_rows[];                // [stage][h, gy, gh][vector][thread]
-  __shared__ float2 s_sum[2][kGradThreads / 32];
+  __shared__ float s_sum[2][2 * R][kGradThreads / 32];
   const int lanes = a.lanes, sub = threadIdx.x / lanes, t = threadIdx.x - sub * lanes, rows = blockDim.x / lanes;
   const int warp = threadIdx.x >> 5, warps = lanes >> 5;
   const bool with_h = a.gh != nullptr && a.gx != nullptr;
@@ -388,101 +412,118 @@ __global__ void __launch_bounds__(kGradThreads, 1) norm_grad_kernel(const NormGr
   auto slot = [&](int stage, int which, int i) { return mine + ((stage * 3 + which) * VECS + i) * blockDim.x; };
   // the next row to fetch, and this thread's columns of it
   int64_t ahead = first + sub;
-  const uint16_t *ph = a.h + ahead * a.ldh + t * 8, *pg = a.gy + ahead * a.ldgy + t * 8, *pr = a.gh + ahead * a.ldgh + t * 8;
+  const int64_t there = ahead < a.n ? ahead : 0;
+  const uint16_t *ph = a.h + there * a.ldh + t * 8, *pg = a.gy + there * a.ldgy + t * 8, *pr = a.gh + there * a.ldgh + t * 8;
   const int64_t sh = step * a.ldh, sg = step * a.ldgy, sr = step * a.ldgh;
   auto fetch = [&](int stage) {
-    if (ahead < a.n) {
+    const int bytes = ahead < a.n ? 16 : 0;                      // rows behind the last: zeros, by the address of one before
 #pragma unroll
-      for (int i = 0; i < VECS; ++i)
-        if ((t + i * lanes) * 8 < a.cols) {
-          copy_vec(slot(stage, 0, i), ph + i * lanes * 8);
-          copy_vec(slot(stage, 1, i), pg + i * lanes * 8);
-          if (with_h) copy_vec(slot(stage, 2, i), pr + i * lanes * 8);
-        }
-    }
-    ahead += step; ph += sh; pg += sg; pr += sr;
+    for (int i = 0; i < VECS; ++i)
+      if ((t + i * lanes) * 8 < a.cols) {
+        copy_vec(slot(stage, 0, i), ph + i * lanes * 8, bytes);
+        copy_vec(slot(stage, 1, i), pg + i * lanes * 8, bytes);
+        if (with_h) copy_vec(slot(stage, 2, i), pr + i * lanes * 8, bytes);
+      }
+    ahead += step;
+    if (ahead < a.n) { ph += sh; pg += sg; pr += sr; }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (WIDE)
+  if (WIDE) {                                                    // what no copy fills: columns behind the last, and rows that are not given
+    for (int k = 0; k < STAGES; ++k)
 #pragma unroll
-    for (int k = 0; k < STAGES - 1; ++k) fetch(k);
-  int turn = 0, stage = 0;
-  for (int64_t base = first; base < a.n; base += step, turn ^= 1) {
-    const int64_t row = base + sub;
-    const bool live = row < a.n;
-    const int cols = live ? a.cols : 0;
+      for (int i = 0; i < VECS; ++i)
+#pragma unroll
+        for (int which = 0; which < 3; ++which)
+          if ((t + i * lanes) * 8 >= a.cols || (which == 2 && !with_h)) *slot(k, which, i) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int k = 0; k < STAGES - R; ++k) fetch(k);
+  }
+  int turn = 0, stage = 0;                                       // of the turn's first row
+  for (int64_t base = first; base < a.n; base += R * step, turn ^= 1) {
     if (WIDE) {
-      fetch(stage == 0 ? STAGES - 1 : stage - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+#pragma unroll
+      for (int j = 0; j < R; ++j) fetch((stage + STAGES - R + j) % STAGES);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - R) : "memory");
     }
-    auto take = [&](const uint16_t* from, int64_t ld, int which, int i) {
-      const int c = (t + i * lanes) * 8;
-      if (!WIDE) return load8<false>(from + row * ld, c, which == 2 && !with_h ? 0 : cols);
-      return c < cols && (which != 2 || with_h) ? *slot(stage, which, i) : make_uint4(0u, 0u, 0u, 0u);
+    auto take = [&](const uint16_t* from, int64_t ld, int which, int i, int j) {
+      if (WIDE) return *slot((stage + j) % STAGES, which, i);
+      const int64_t row = base + j * step + sub;
+      return load8<false>(from + row * ld, (t + i * lanes) * 8, row < a.n && (which != 2 || with_h) ? a.cols : 0);
     };
-    float2 s2 = make_float2(0.f, 0.f), p2 = make_float2(0.f, 0.f);
+    float ss[R], sp[R];
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      float2 fh[4], fg[4];
-      pairs8(take(a.h, a.ldh, 0, i), fh);
-      pairs8(take(a.gy, a.ldgy, 1, i), fg);
+    for (int j = 0; j < R; ++j) {
+      float2 s2 = make_float2(0.f, 0.f), p2 = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s2 = __ffma2_rn(fh[j], fh[j], s2);
-        p2 = __ffma2_rn(__fmul2_rn(w[i][j], fg[j]), fh[j], p2);
+      for (int i = 0; i < VECS; ++i) {
+        float2 fh[4], fg[4];
+        pairs8(take(a.h, a.ldh, 0, i, j), fh);
+        pairs8(take(a.gy, a.ldgy, 1, i, j), fg);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s2 = __ffma2_rn(fh[e], fh[e], s2);
+          p2 = __ffma2_rn(__fmul2_rn(w[i][e], fg[e]), fh[e], p2);
+        }
       }
+      ss[j] = s2.x + s2.y;
+      sp[j] = p2.x + p2.y;
     }
-    float ss = warp_sum(s2.x + s2.y), sp = warp_sum(p2.x + p2.y);
+    const int lane = threadIdx.x & 31;
+    constexpr int EACH = 16 / R;                                 // lanes that end with a sum
+    float v = warp_sums<R>(ss, sp);
     if (warps > 1) {
-      if ((threadIdx.x & 31) == 0) s_sum[turn][warp] = make_float2(ss, sp);
+      if (lane % EACH == 0) s_sum[turn][lane / EACH][warp] = v;
       __syncthreads();               // the other half of s_sum is written in the next turn: no thread is two turns ahead
-      const int lane = threadIdx.x & 31;
-      const float2 v = lane < warps ? s_sum[turn][sub * warps + lane] : make_float2(0.f, 0.f);
-      ss = v.x;
-      sp = v.y;
 #pragma unroll
-      for (int o = kGradThreads / 64; o > 0; o >>= 1) {
-        ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-        sp += __shfl_xor_sync(0xFFFFFFFFu, sp, o);
+      for (int j = 0; j < R; ++j) {
+        ss[j] = lane < warps ? s_sum[turn][2 * j][sub * warps + lane] : 0.f;
+        sp[j] = lane < warps ? s_sum[turn][2 * j + 1][sub * warps + lane] : 0.f;
       }
-      if (kGradThreads / 32 < 32) {  // lanes behind the last warp's have summed zeros
-        ss = __shfl_sync(0xFFFFFFFFu, ss, 0);
-        sp = __shfl_sync(0xFFFFFFFFu, sp, 0);
+      v = warp_sums<R>(ss, sp);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      ss[j] = __shfl_sync(0xFFFFFFFFu, v, 2 * j * EACH);
+      sp[j] = __shfl_sync(0xFFFFFFFFu, v, (2 * j + 1) * EACH);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int64_t row = base + j * step + sub;
+      const bool live = row < a.n;
+      const float rstd = live ? rsqrtf(fmaf(ss[j], inv_cols, a.eps)) : 0.f;
+      const float2 r2 = make_float2(rstd, rstd);
+      const float c = -rstd * rstd * (sp[j] * inv_cols);
+      const float2 c2 = make_float2(c, c);
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        float2 fh[4], fg[4], fr[4];
+        pairs8(take(a.h, a.ldh, 0, i, j), fh);
+        pairs8(take(a.gy, a.ldgy, 1, i, j), fg);
+        pairs8(take(a.gh, a.ldgh, 2, i, j), fr);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[i][e] = __ffma2_rn(fg[e], __fmul2_rn(fh[e], r2), acc[i][e]);
+          fr[e] = __ffma2_rn(r2, __ffma2_rn(fh[e], c2, __fmul2_rn(w[i][e], fg[e])), fr[e]);
+        }
+        if (a.gx == nullptr || !live) continue;
+        const int at = (t + i * lanes) * 8;
+        uint16_t* dst = a.gx + row * a.ldgx;
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(fr[e].x, fr[e].y);
+          u[e] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        if (WIDE) {
+          if (at < a.cols) *reinterpret_cast<uint4*>(dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (at + e < a.cols) dst[at + e] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+        }
       }
     }
-    const float rstd = live ? rsqrtf(fmaf(ss, inv_cols, a.eps)) : 0.f;
-    const float2 r2 = make_float2(rstd, rstd);
-    const float c = -rstd * rstd * (sp * inv_cols);
-    const float2 c2 = make_float2(c, c);
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      float2 fh[4], fg[4], fr[4];
-      pairs8(take(a.h, a.ldh, 0, i), fh);
-      pairs8(take(a.gy, a.ldgy, 1, i), fg);
-      pairs8(take(a.gh, a.ldgh, 2, i), fr);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[i][j] = __ffma2_rn(fg[j], __fmul2_rn(fh[j], r2), acc[i][j]);
-        fr[j] = __ffma2_rn(r2, __ffma2_rn(fh[j], c2, __fmul2_rn(w[i][j], fg[j])), fr[j]);
-      }
-      if (a.gx == nullptr || !live) continue;
-      const int at = (t + i * lanes) * 8;
-      uint16_t* dst = a.gx + row * a.ldgx;
-      uint32_t u[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(fr[j].x, fr[j].y);
-        u[j] = *reinterpret_cast<const uint32_t*>(&v);
-      }
-      if (WIDE) {
-        if (at < a.cols) *reinterpret_cast<uint4*>(dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (at + j < a.cols) dst[at + j] = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
-      }
-    }
-    if (++stage == STAGES) stage = 0;
+    stage = (stage + R) % STAGES;
   }
   if (FEW) {
     if (a.gw == nullptr) return;
@@ -533,8 +574,8 @@ __global__ void __launch_bounds__(1024) norm_grad_sum_kernel(const float* parts,
   if (x == 0 && blockIdx.x * 32 + y < cols) gw[blockIdx.x * 32 + y] = v;
 }
 
-// Two launches and one, us in a graph: 1 row of 2048 columns 4.2 and 4.8, 16 rows 4.4 and 5.4, 37 rows 4.8 and 7.2, 64 rows 5.4 and 9.2,
-// 128 rows 5.3 and 14.0.  A call from Python at 37 rows: 18.0 and 12.2, since two launches and their scratch cost the host more than
+// Two launches and one, us in a graph: 1 row of 2048 columns 4.8 and 5.2, 16 rows 5.0 and 5.3, 37 rows 5.3 and 7.2, 64 rows 6.0 and 8.5,
+// 128 rows 5.9 and 12.5.  A call from Python at 37 rows: 18.0 and 12.2, since two launches and their scratch cost the host more than
 // the device gains; from MG_NORM_GRAD_FEW rows on the device's side wins.
 constexpr int kGradCluster = 8;
 struct NormGradPlan { int vecs, lanes, threads, blocks, shares; bool few; };
