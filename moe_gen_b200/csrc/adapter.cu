@@ -38,6 +38,10 @@ __device__ __forceinline__ void copy_row(uint32_t to, const uint16_t* row, int c
 __device__ __forceinline__ void copy_whole(uint32_t to, const uint16_t* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// the same, or zeros
+__device__ __forceinline__ void copy_or_zeros(uint32_t to, const uint16_t* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -877,14 +881,17 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int64_t row = max(rows[j], 0);
-          const int end = rows[j] >= 0 ? cols : 0;
+          const bool there = rows[j] >= 0;
           const uint16_t* w = wide + row * ldw;
-          const uint16_t* n = narrow + row * C::NR;
+          const uint16_t* n = narrow + row * C::NR + p * 8;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) copy_row<16>(filling + mine + j * 4096 + b * 8192, w, c + b * 64, end);
+          for (int b = 0; b < 2; ++b) {
+            if (f.c0 + 128 <= cols) copy_or_zeros(filling + mine + j * 4096 + b * 8192, w + c + b * 64, there);
+            else copy_row<16>(filling + mine + j * 4096 + b * 8192, w, c + b * 64, there ? cols : 0);
+          }
 #pragma unroll
           for (int b = 0; b < C::HALVES; ++b)
-            if (p < C::NR / 8) copy_row<16>(filling + C::WIDE + mine + j * 4096 + b * 8192, n, p * 8 + b * 64, rows[j] >= 0 ? C::NR : 0);
+            if (p < C::NR / 8) copy_or_zeros(filling + C::WIDE + mine + j * 4096 + b * 8192, n + b * 64, there);
         }
         ++in;
         if (!ONE && in == f.steps) next_job();
