@@ -1028,11 +1028,12 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
   };
   const int per = ((rows + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
   const int64_t from = static_cast<int64_t>(warp) * per;
+  const bool kept = per <= 32 * kPlanAhead;            // a lane's rows stay in its registers
+  int ids_of[kPlanAhead], place_of[kPlanAhead];
   if (!SORTED) {
     for (int e = tid; e < kPlanWarps * groups; e += blockDim.x) s_hist[e] = 0;
     __syncthreads();
-    for (int k = 0; k < per; k += 32 * kPlanAhead) {
-      int ids_of[kPlanAhead];                          // on their way together
+    for (int k = 0; k < per; k += 32 * kPlanAhead) {   // the ids of a run on their way together
 #pragma unroll
       for (int n = 0; n < kPlanAhead; ++n) ids_of[n] = k + n * 32 < per ? id_of(from + k + n * 32 + lane) : -1;
 #pragma unroll
@@ -1047,7 +1048,8 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
           s_hist[warp * groups + id] = at + __popc(peers);
         }
         at = __shfl_sync(0xFFFFFFFFu, at, __ffs(peers) - 1) + before;
-        if (id >= 0) place[from + k + n * 32 + lane] = at;             // among the warp's rows of the adapter
+        place_of[n] = at;                              // among the warp's rows of the adapter
+        if (!kept && id >= 0) place[from + k + n * 32 + lane] = at;
         __syncwarp();
       }
     }
@@ -1127,13 +1129,19 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
     }
     tiles[e] = t;
   }
-  if (!SORTED)
+  if (!SORTED && kept) {
+#pragma unroll
+    for (int n = 0; n < kPlanAhead; ++n)
+      if (n * 32 < per && ids_of[n] >= 0)
+        order[s_start[ids_of[n]] + s_hist[warp * groups + ids_of[n]] + place_of[n]] = static_cast<int32_t>(from + n * 32 + lane);
+  } else if (!SORTED) {
 #pragma unroll 4
     for (int k = 0; k < per; k += 32) {
       const int64_t j = from + k + lane;
       const int id = id_of(j);
       if (id >= 0) order[s_start[id] + s_hist[warp * groups + id] + place[j]] = static_cast<int32_t>(j);
     }
+  }
 }
 
 int padded_rank(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
