@@ -66,13 +66,13 @@ __device__ __forceinline__ float4 cluster_sum(uint32_t at, int cs) {
     if (c < cs) { u.x += there[c].x; u.y += there[c].y; u.z += there[c].z; u.w += there[c].w; }
   return u;
 }
-// eight numbers, the second four `next` bytes behind the first
+// eight numbers, the second four `next` bytes behind the first, over CS blocks from block `base` on
 template <int CS>
-__device__ __forceinline__ void cluster_sum8(uint32_t at, uint32_t next, float* v) {
+__device__ __forceinline__ void cluster_sum8(uint32_t at, uint32_t next, int base, float* v) {
   float4 a[CS], b[CS];
 #pragma unroll
   for (int c = 0; c < CS; ++c) {
-    const uint32_t there = map_to_cta(at, c);
+    const uint32_t there = map_to_cta(at, base + c);
     a[c] = ld_cluster_f32x4(there);
     b[c] = ld_cluster_f32x4(there + next);
   }
@@ -147,7 +147,8 @@ struct AdapterArgs {
   float factor;
   int rank, n_adapters, n_rows;
   const int32_t* ids;         // a call without a plan
-  const int4* tiles;          // adapter (-1: none), first entry of order, rows with it, rows
+  const int4* tiles;          // adapter (-1: none), first entry of order, rows with it, rows; behind them, the tiles of adapters and all
+  int n_tiles, slots;         // tiles there is room for; blocks that run at once, a multiple of a cluster's
   const int32_t* order;
   int32_t* status;
 };
@@ -426,7 +427,7 @@ struct TileCopies {
   int t;
   const uint16_t* from[EACH];
   __device__ TileCopies(const AdapterArgs& args, int g, int thread) : a(args), t(thread) {
-    const uint16_t *w1 = a.w1 + (g >= 0 ? g * a.g1 : 0), *w2 = a.w2 + (g >= 0 ? g * a.g2 : 0);
+    const uint16_t *w1 = a.w1 + g * a.g1, *w2 = a.w2 + g * a.g2;
     wide = BACK ? w2 : w1;
     narrow = BACK ? w1 : w2;
   }
@@ -435,7 +436,7 @@ struct TileCopies {
     for (int j = 0; j < EACH; ++j) from[j] = base + static_cast<int64_t>(rows[min((t >> 3) + j * ROWS, n - 1)]) * ld + (t & 7) * 8;
   }
   // into the stage at `to`: columns c to c + 63 of n of the first `rows` rows, and of the adapter
-  __device__ __forceinline__ void step(uint32_t to, bool first, int c, int n, int rows, bool adapter) const {
+  __device__ __forceinline__ void step(uint32_t to, bool first, int c, int n, int rows) const {
     const int r0 = t >> 3, p = t & 7, first_row = t / 32 * 4;
     const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
     const bool inside = c + 64 <= n, filled = a.rank == RP;
@@ -445,7 +446,7 @@ struct TileCopies {
         if (inside) copy_whole(to + mine + j * ROWS * 128, from[j] + c);
         else copy_row<16>(to + mine + j * ROWS * 128, from[j] - p * 8, c + p * 8, n);
       }
-    if (!adapter || (RP * 8 < WARPS * 32 && t >= RP * 8)) return;
+    if (RP * 8 < WARPS * 32 && t >= RP * 8) return;
     if (first != BACK) {
       const int64_t ld = BACK ? a.ld2 : a.ld1;
       if (inside && filled) {
@@ -478,6 +479,35 @@ struct TileCopies {
   }
 };
 
+// The rows of a tile none of which has an adapter: out = y, and s zeros, or gx zeros; columns lo to hi of each.  A warp to a row, 4 KB of it at a
+// time.
+template <int RP, bool BACK>
+__device__ __forceinline__ void rows_without(const AdapterArgs& a, const int32_t* order, int len, int lo, int hi, bool first) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool in_place = !BACK && a.y == a.out && a.ldy == a.ldo;
+  for (int r = warp; r < len; r += kTileThreads / 32) {
+    const int64_t row = order[r];
+    if (!BACK && a.s != nullptr && first)              // gs is read for rows with an adapter only
+      for (int p = lane; p < RP / 4; p += 32) reinterpret_cast<uint4*>(a.s + row * (2 * RP))[p] = make_uint4(0u, 0u, 0u, 0u);
+    if (in_place) continue;
+    uint16_t* to = a.out + row * a.ldo;
+    const uint16_t* from = BACK ? nullptr : a.y + row * a.ldy;
+    for (int c = lo + lane * 8; c < hi; c += 8 * 32 * 8) {
+      uint4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        v[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (!BACK && c + k * 256 + 8 <= hi) v[k] = *reinterpret_cast<const uint4*>(from + c + k * 256);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k * 256 + 8 <= hi) *reinterpret_cast<uint4*>(to + c + k * 256) = v[k];
+    }
+    const int rest = hi & ~7;                          // hi is the rows' end where it is not a multiple of 8
+    if (lo < hi && rest + lane < hi) to[rest + lane] = BACK ? static_cast<uint16_t>(0) : from[rest + lane];
+  }
+}
+
 template <int RP, bool BACK>
 __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_tile_kernel(const AdapterArgs a) {
   using C = TileCfg<RP>;
@@ -489,10 +519,43 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
   __shared__ int s_rows[kAdapterTile];
   const uint32_t ring = smem_u32(smem_raw), s_at = ring + S * C::STAGE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int cs = static_cast<int>(cluster_size()), cr = static_cast<int>(cluster_ctarank());
-  const int4 job = a.tiles[blockIdx.x / cs];
+  // The blocks of a cluster, 2^most of them, share a tile among cs, or take one each.  Tiles of adapters that fill all places take one each; the
+  // rest of them are shared by as many as let them all run at once; then come those of rows without an adapter, shared by P.
+  const int most = 31 - __clz(cluster_size()), P = 1 << most, pr = static_cast<int>(cluster_ctarank()), cl = blockIdx.x >> most;
+  const int4 total = a.tiles[a.n_tiles];
+  int4 guess[4];                                       // the tile if there is no full round, by 1, 2, 4 and 8 blocks, on its way beside the numbers
+#pragma unroll
+  for (int k = 0; k < 4; ++k) guess[k] = a.tiles[min((cl << most >> k) + (pr >> k), a.n_tiles - 1)];
+  const int solo = total.x / a.slots * a.slots, rem = total.x - solo;
+  int by = most;
+  while (by > 0 && rem << by > a.slots) --by;
+  const int c1 = solo >> most, c2 = c1 + (((rem << by) + P - 1) >> most);
+  const int shift = cl < c1 ? 0 : cl < c2 ? by : a.N > 0 ? most : 0;
+  const int first = cl < c1 ? 0 : cl < c2 ? c1 : c2, before = cl < c1 ? 0 : cl < c2 ? solo : total.x;
+  const int tile = before + ((cl - first) << most >> shift) + (pr >> shift), end = cl < c2 ? (cl < c1 ? solo : total.x) : total.y;
+  const int cs = 1 << shift, cr = pr & (cs - 1), base = pr - cr;
+  auto meet = [&]() {                                  // who has nothing to share meets the others of its cluster all the same
+    for (int k = 0; cs > 1 && cl < c2 && k < 3; ++k) cluster_sync_all();
+  };
+  int4 job = make_int4(-1, 0, 0, 0);
+  if (tile < end) {
+    if (solo == 0 && cl < c2) {
+      job = guess[0];
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (shift == k) job = guess[k];
+    } else {
+      job = a.tiles[tile];
+    }
+  }
   const int g = job.x, live = job.z, len = job.w;
-  if (len == 0) return;                                // the whole cluster
+  const int units = (a.N + 63) / 64, each = (units + cs - 1) / cs;
+  const int lo2 = cr * each, n2 = max(min(units, lo2 + each) - lo2, 0);
+  if (live == 0) {
+    if (len > 0) rows_without<RP, BACK>(a, a.order + job.y, len, lo2 * 64, min(a.N, (lo2 + n2) * 64), cr == 0);
+    meet();
+    return;
+  }
   if (tid < len) s_rows[tid] = a.order[job.y + tid];
   if (tid == 0) {
     for (int k = 0; k < S; ++k) {
@@ -510,9 +573,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(C::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  const int slices = live > 0 ? (a.K + 63) / 64 : 0, per = (slices + cs - 1) / cs;
-  const int units = (a.N + 63) / 64, each = (units + cs - 1) / cs;
-  const int lo1 = cr * per, n1 = max(min(slices, lo1 + per) - lo1, 0), lo2 = cr * each, n2 = max(min(units, lo2 + each) - lo2, 0);
+  const int slices = (a.K + 63) / 64, per = (slices + cs - 1) / cs;
+  const int lo1 = cr * per, n1 = max(min(slices, lo1 + per) - lo1, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -525,7 +587,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 
   if (warp == kFinishWarps + kCopyWarps) {
     // ---- products ----
-    for (int k = 0; live > 0 && k < n1; ++k) {
+    for (int k = 0; k < n1; ++k) {
       full(k);
       tc_fence_after();
       if (elect_one()) {
@@ -539,10 +601,10 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       }
       __syncwarp();
     }
-    if (live > 0 && cs > 1)
+    if (cs > 1)
       for (int k = 0; k < 3; ++k) cluster_sync_all();
-    if (live > 0) wait_warp(smem_u32(&s_ready), 0, &s_abort, a.status, 123);
-    for (int m = 0; live > 0 && m < n2; ++m) {
+    wait_warp(smem_u32(&s_ready), 0, &s_abort, a.status, 123);
+    for (int m = 0; m < n2; ++m) {
       full(n1 + m);
       if (m >= 2) empty(m - 2);                        // the accumulator has been read
       tc_fence_after();
@@ -564,7 +626,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     TileCopies<RP, BACK, kCopyWarps> copies(a, g, tid - kFinishWarps * 32);
     if (!BACK) copies.rows_of(a.y, a.ldy, s_rows, len);
     if (n1 > 0) wait_warp(smem_u32(&s_first), 0, &s_abort, a.status, 126);       // the first product has left its last stage
-    bool met = live == 0 || cs == 1;
+    bool met = cs == 1;
     for (int m = S - 1; m < n2 + S - 2; ++m) {
       if (m >= S && !met) {                            // the blocks' exchange, which comes before any stage is emptied
         for (int k = 0; k < 3; ++k) cluster_sync_all();
@@ -572,7 +634,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       }
       if (m < n2) {
         if (m >= S) empty(m - S);
-        copies.step(ring + (n1 + m) % S * C::STAGE, false, (lo2 + m) * 64, a.N, BACK ? 0 : len, live > 0);
+        copies.step(ring + (n1 + m) % S * C::STAGE, false, (lo2 + m) * 64, a.N, BACK ? 0 : len);
       }
       copies_commit();
       copies_wait<S - 2>();                            // step m - (S - 2) is there, for the tensor core too
@@ -587,7 +649,7 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
     // A lane finishes a row, 64 bytes to a warp, so that two warps share 32 rows; each stores 16 of them, 128 bytes of a row side by side.
     const int quarter = warp & 3, side = warp >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const float scale = g >= 0 ? a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f) : 0.0f;
+    const float scale = a.factor * (a.scale != nullptr ? a.scale[g] : 1.0f);
     const bool in_place = a.y == a.out && a.ldy == a.ldo;
     {
       // ---- copies of the first product and of the second's first S - 1 steps ----
@@ -595,10 +657,10 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       if (n1 > 0) copies.rows_of(a.x, a.ldx, s_rows, live);
       auto fetch = [&](int k) {
         if (k < n1) {
-          copies.step(ring + k % S * C::STAGE, true, (lo1 + k) * 64, a.K, live, true);
+          copies.step(ring + k % S * C::STAGE, true, (lo1 + k) * 64, a.K, live);
         } else if (k < n1 + n2) {
           if (!BACK && k == n1) copies.rows_of(a.y, a.ldy, s_rows, len);
-          copies.step(ring + k % S * C::STAGE, false, (lo2 + k - n1) * 64, a.N, BACK ? 0 : len, live > 0);
+          copies.step(ring + k % S * C::STAGE, false, (lo2 + k - n1) * 64, a.N, BACK ? 0 : len);
         }
         copies_commit();
       };
@@ -611,83 +673,78 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       }
       if (n1 > 0) done(n1 - 1);
     }
-    if (live > 0) {
-      // eight columns of a row of s, zeros behind the tile's rows and the rank, in two parts
-      auto parts = [&](int r, int col, float* v, uint4& high, uint4& low) {
+    // eight columns of a row of s, zeros behind the tile's rows and the rank, in two parts
+    auto parts = [&](int r, int col, float* v, uint4& high, uint4& low) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = r < live && col + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
-        split_pair(v[0], v[1], high.x, low.x);
-        split_pair(v[2], v[3], high.y, low.y);
-        split_pair(v[4], v[5], high.z, low.z);
-        split_pair(v[6], v[7], high.w, low.w);
-        if (a.s != nullptr && r < len) {
-          uint16_t* kept = a.s + static_cast<int64_t>(s_rows[r]) * (2 * RP) + col;
-          *reinterpret_cast<uint4*>(kept) = high;
-          *reinterpret_cast<uint4*>(kept + RP) = low;
-        }
-        return s_at + (col >> 6) * C::ROWS + r * 128;
-      };
-      auto low_piece = [&](int r, int col) { return (((RP <= 32 ? 4 : 0) + (col >> 3 & 7)) ^ (r & 7)) << 4; };      // in the second part's row
-      tc_fence_after();
-      // the accumulator's row of this thread, half of the columns to either side's warps
-#pragma unroll
-      for (int k = 0; k < RP / 2; k += 8) {
-        float v[8];
-        const int col = side * (RP / 2) + k;
-        tc_ld8(lanes + col, v);
-        if (n1 == 0)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        if (cs == 1) {
-          uint4 high, low;
-          const uint32_t to = parts(row, col, v, high, low);
-          st_shared(to + (((col >> 3 & 7) ^ (row & 7)) << 4), high);
-          st_shared(to + (RP <= 32 ? 0 : C::PART) + low_piece(row, col), low);
-        } else {                                       // [groups of four columns][row], where s will be
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            st_shared(s_at + ((col / 4 + e) * kAdapterTile + row) * 16,
-                      make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
-        }
+      for (int e = 0; e < 8; ++e) v[e] = r < live && col + e < a.rank ? (BACK ? scale * v[e] : v[e]) : 0.f;
+      split_pair(v[0], v[1], high.x, low.x);
+      split_pair(v[2], v[3], high.y, low.y);
+      split_pair(v[4], v[5], high.z, low.z);
+      split_pair(v[6], v[7], high.w, low.w);
+      if (a.s != nullptr && r < len) {
+        uint16_t* kept = a.s + static_cast<int64_t>(s_rows[r]) * (2 * RP) + col;
+        *reinterpret_cast<uint4*>(kept) = high;
+        *reinterpret_cast<uint4*>(kept + RP) = low;
       }
-      if (cs > 1) {
-        constexpr int ITEMS = RP <= 32 ? 1 : RP / 32;
-        const int share = kAdapterTile / cs;
-        float v[ITEMS][8];
-        cluster_sync_all();                            // the blocks' sums are there
+      return s_at + (col >> 6) * C::ROWS + r * 128;
+    };
+    auto low_piece = [&](int r, int col) { return (((RP <= 32 ? 4 : 0) + (col >> 3 & 7)) ^ (r & 7)) << 4; };      // in the second part's row
+    tc_fence_after();
+    // the accumulator's row of this thread, half of the columns to either side's warps
 #pragma unroll
-        for (int n = 0; n < ITEMS; ++n) {
-          const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
-          const uint32_t at = s_at + (col / 4 * kAdapterTile + r) * 16;
-          if (q >= share * RP / 8) continue;
-          if (cs == 8) cluster_sum8<8>(at, kAdapterTile * 16, v[n]);
-          else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, v[n]);
-          else cluster_sum8<2>(at, kAdapterTile * 16, v[n]);
-        }
-        cluster_sync_all();                            // and have been read: s takes their place
+    for (int k = 0; k < RP / 2; k += 8) {
+      float v[8];
+      const int col = side * (RP / 2) + k;
+      tc_ld8(lanes + col, v);
+      if (n1 == 0)
 #pragma unroll
-        for (int n = 0; n < ITEMS; ++n) {
-          const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
-          if (q >= share * RP / 8) continue;
-          uint4 high, low;
-          const uint32_t to = parts(r, col, v[n], high, low);
-          for (int c = 0; c < cs; ++c) {                // every block begins with itself
-            const uint32_t there = map_to_cta(to, (cr + c) & (cs - 1));
-            st_cluster16(there + (((col >> 3 & 7) ^ (r & 7)) << 4), high);
-            st_cluster16(there + (RP <= 32 ? 0 : C::PART) + low_piece(r, col), low);
-          }
-        }
-        asm volatile("fence.proxy.async;" ::: "memory");
-        cluster_sync_all();
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      if (cs == 1) {
+        uint4 high, low;
+        const uint32_t to = parts(row, col, v, high, low);
+        st_shared(to + (((col >> 3 & 7) ^ (row & 7)) << 4), high);
+        st_shared(to + (RP <= 32 ? 0 : C::PART) + low_piece(row, col), low);
+      } else {                                       // [groups of four columns][row], where s will be
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          st_shared(s_at + ((col / 4 + e) * kAdapterTile + row) * 16,
+                    make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&s_ready));
-    } else if (a.s != nullptr && cr == 0) {
-      for (int p = tid; p < len * RP / 4; p += kFinishWarps * 32)
-        *reinterpret_cast<uint4*>(a.s + static_cast<int64_t>(s_rows[p / (RP / 4)]) * (2 * RP) + p % (RP / 4) * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
+    if (cs > 1) {
+      constexpr int ITEMS = RP <= 32 ? 1 : RP / 32;
+      const int share = kAdapterTile / cs;
+      float v[ITEMS][8];
+      cluster_sync_all();                            // the blocks' sums are there
+#pragma unroll
+      for (int n = 0; n < ITEMS; ++n) {
+        const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
+        const uint32_t at = s_at + (col / 4 * kAdapterTile + r) * 16;
+        if (q >= share * RP / 8) continue;
+        if (cs == 8) cluster_sum8<8>(at, kAdapterTile * 16, base, v[n]);
+        else if (cs == 4) cluster_sum8<4>(at, kAdapterTile * 16, base, v[n]);
+        else cluster_sum8<2>(at, kAdapterTile * 16, base, v[n]);
+      }
+      cluster_sync_all();                            // and have been read: s takes their place
+#pragma unroll
+      for (int n = 0; n < ITEMS; ++n) {
+        const int q = tid + n * kFinishWarps * 32, r = cr * share + q % share, col = q / share * 8;
+        if (q >= share * RP / 8) continue;
+        uint4 high, low;
+        const uint32_t to = parts(r, col, v[n], high, low);
+        for (int c = 0; c < cs; ++c) {                // every block begins with itself
+          const uint32_t there = map_to_cta(to, base + ((cr + c) & (cs - 1)));
+          st_cluster16(there + (((col >> 3 & 7) ^ (r & 7)) << 4), high);
+          st_cluster16(there + (RP <= 32 ? 0 : C::PART) + low_piece(r, col), low);
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      cluster_sync_all();
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&s_ready));
     const int first_row = quarter * 32 + side * 16, piece = lane & 7;
     uint16_t* op[4];
     uint32_t stored = 0;
@@ -704,34 +761,31 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
       const uint32_t at = ring + (n1 + m) % S * C::STAGE;
       const int c0 = (lo2 + m) * 64;
       full(n1 + m);
-      if (live > 0) {
-        done(n1 + m);
-        tc_fence_after();
+      done(n1 + m);
+      tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t acc[16];
-          tc_ld16(lanes + C::SECOND + (m & 1) * 64 + side * 32 + h * 16, acc);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t acc[16];
+        tc_ld16(lanes + C::SECOND + (m & 1) * 64 + side * 32 + h * 16, acc);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t to = at + row * 128 + (((side * 4 + h * 2 + k) ^ (row & 7)) << 4);
-            float o[8];
-            if (!BACK) unpack8(ld_shared(to), o);
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t to = at + row * 128 + (((side * 4 + h * 2 + k) ^ (row & 7)) << 4);
+          float o[8];
+          if (!BACK) unpack8(ld_shared(to), o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float v = __uint_as_float(acc[8 * k + e]);
-              o[e] = BACK ? v : fmaf(scale, v, o[e]);
-            }
-            if (row < live) st_shared(to, pack8(o));
-            else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
+          for (int e = 0; e < 8; ++e) {
+            const float v = __uint_as_float(acc[8 * k + e]);
+            o[e] = BACK ? v : fmaf(scale, v, o[e]);
           }
+          if (row < live) st_shared(to, pack8(o));
+          else if (BACK) st_shared(to, make_uint4(0u, 0u, 0u, 0u));
         }
-        tc_fence_before();
-        pair_sync(quarter);
       }
+      tc_fence_before();
+      pair_sync(quarter);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 v = BACK && live == 0 ? make_uint4(0u, 0u, 0u, 0u)
-                                          : ld_shared(at + (first_row + j * 4 + (lane >> 3)) * 128 + ((piece ^ (lane >> 3) ^ ((j & 1) << 2)) << 4));
+        const uint4 v = ld_shared(at + (first_row + j * 4 + (lane >> 3)) * 128 + ((piece ^ (lane >> 3) ^ ((j & 1) << 2)) << 4));
         if (stored >> j & 1u) store_row(op[j] + c0, 0, a.N - c0 - piece * 8, v);
       }
       __syncwarp();
@@ -914,9 +968,18 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
         fetch();
       }
       if (j.live == 0) {
-        for (int e = cr * kAdapterThreads + tid; e < 128 * a.rank; e += cs * kAdapterThreads) {
-          const int c = j.c0 + (j.which ? e % 128 : e / a.rank), r = j.which ? e / 128 : e % a.rank;
-          if (c < cols) out[j.which ? r * static_cast<int64_t>(cols) + c : static_cast<int64_t>(c) * a.rank + r] = 0;
+        // zeros, 16 bytes at a time where rows begin so: 128 columns of every one of the rank, or the rank of 128 columns in a piece
+        const int have = min(cols - j.c0, 128);
+        const int lines = j.which ? a.rank : 1, width = j.which ? have : have * a.rank;
+        const int64_t ld = j.which ? cols : 0;
+        uint16_t* zeros = out + (j.which ? j.c0 : static_cast<int64_t>(j.c0) * a.rank);
+        const bool wide = reinterpret_cast<uintptr_t>(zeros) % 16 == 0 && ld % 8 == 0 && width % 8 == 0;
+        const int each = wide ? 8 : 1, pieces = width / each;
+        for (int e = cr * kAdapterThreads + tid; e < lines * pieces; e += cs * kAdapterThreads) {
+          const int line = lines == 1 ? 0 : e / pieces;
+          uint16_t* at = zeros + line * ld + static_cast<int64_t>(e - line * pieces) * each;
+          if (wide) *reinterpret_cast<uint4*>(at) = make_uint4(0u, 0u, 0u, 0u);
+          else *at = 0;
         }
         continue;
       }
@@ -967,9 +1030,9 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
           const int c = cr * share + q % share, r = q / share * 8;
           float v[8];
           const uint32_t at = ring + (r / 4 * 128 + c) * 16;
-          if (cs == 8) cluster_sum8<8>(at, 128 * 16, v);
-          else if (cs == 4) cluster_sum8<4>(at, 128 * 16, v);
-          else cluster_sum8<2>(at, 128 * 16, v);
+          if (cs == 8) cluster_sum8<8>(at, 128 * 16, 0, v);
+          else if (cs == 4) cluster_sum8<4>(at, 128 * 16, 0, v);
+          else cluster_sum8<2>(at, 128 * 16, 0, v);
           store8(j.c0 + c, r, v);
         }
       }
@@ -996,7 +1059,7 @@ PlanLayout plan_layout(int64_t rows, int64_t adapters) {
   PlanLayout p;
   const int64_t n = (rows + kAdapterTile - 1) / kAdapterTile + adapters + 1;
   p.tiles = 0;
-  p.segs = 4 * n;
+  p.segs = 4 * (n + 1);
   p.order = p.segs + 4 * adapters;
   p.place = p.order + rows;                // while the plan is made
   p.words = p.place + rows;
@@ -1115,6 +1178,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
     for (int o = 1 << bits >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
     if (e < adapters && (tid & ((1 << bits) - 1)) == 0) segs[before] = make_int4(s_start[e], n, e, 0);
   }
+  if (tid == 0) tiles[n_tiles] = make_int4(min(s_tile[adapters], n_tiles), min(s_tile[groups], n_tiles), 0, 0);
   for (int e = tid; e < n_tiles; e += blockDim.x) {
     int4 t = make_int4(-1, 0, 0, 0);
     if (e < s_tile[groups]) {
@@ -1157,17 +1221,22 @@ int launch_direct_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
   return MG_OK;
 }
 template <int RP, bool BACK>
-int launch_tiles_as(const Handle* h, const AdapterArgs& a, cudaStream_t st) {
+int launch_tiles_as(const Handle* h, AdapterArgs a, cudaStream_t st) {
   using C = TileCfg<RP>;
   static bool done[64];
   if (int rc = allow_smem(h, adapter_tile_kernel<RP, BACK>, C::SMEM, done)) return rc;
-  // As many blocks to a tile as run at once, were all tiles full.  K = N = 4096, 8 adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16
-  // 92, 50, 29, 18; 4096 rows 93, 52, 34, 36; 8192 rows rank 64 107, 65, 55, 68; 16384 rows rank 16 101, 83, 90, 98; 32768 rows 151,
-  // 161, 164, 179.
-  const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile;
-  int cs = 8;
-  while (cs > 1 && full * cs > C::BLOCKS * h->sm_count) cs /= 2;
-  MG_CUDA(launch_clusters(adapter_tile_kernel<RP, BACK>, full + a.n_adapters + 1, cs, kTileThreads, C::SMEM, st, a));
+  // As many blocks to a tile as run at once, were all rows in full tiles; how many tiles there are in earnest the device knows.  K = N = 4096, 8
+  // adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16 92, 50, 29, 18; 4096 rows 93, 52, 34, 36; 8192 rows rank 64 107, 65, 55, 68; 16384
+  // rows rank 16 101, 83, 90, 98; 32768 rows 151, 161, 164, 179.  Rows in not much more than a tile to an adapter, as those of expert-sorted
+  // buffers of few tokens, are in clusters of four at any number, since most of their tiles may be without an adapter: 20864 rows for 160
+  // adapters, 300 of them with one, 5120 to 5120, add 98 and grad x 64, without clusters 129 and 104.  Elsewhere clusters of four cost: they leave
+  // places of a GPC empty, and 296 full tiles take 124 where single blocks take 90.
+  const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile, places = C::BLOCKS * h->sm_count;
+  int P = 8;
+  while (P > 1 && full * P > places && !(P == 4 && 4 * full <= 5 * a.n_adapters)) P /= 2;
+  a.slots = static_cast<int>(places / P * P);
+  const int64_t all = a.n_tiles + full, most = a.n_tiles + full * P + (P > 1 ? a.slots : 0);      // blocks, P to a tile and one to those of adapters
+  MG_CUDA(launch_clusters(adapter_tile_kernel<RP, BACK>, (all * P < most ? all * P : most) / P + 2, P, kTileThreads, C::SMEM, st, a));
   return MG_OK;
 }
 template <bool BACK>
@@ -1215,7 +1284,7 @@ int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* coun
                         void* plan, cudaStream_t st) {
   const PlanLayout p = plan_layout(rows, adapters);
   int32_t* w = static_cast<int32_t*>(plan);
-  const int n_tiles = static_cast<int>(p.segs / 4), groups = adapters + 1;
+  const int n_tiles = static_cast<int>(p.segs / 4) - 1, groups = adapters + 1;
   static bool done[2][64];
   constexpr size_t most = (4 * (MG_ADAPTER_MAX + 1) + 1 + kPlanWarps * (MG_ADAPTER_MAX + 1)) * sizeof(int);
   const size_t smem = (4 * groups + 1 + (ids != nullptr ? kPlanWarps * groups : 0)) * sizeof(int);
@@ -1244,6 +1313,7 @@ static AdapterArgs adapter_args(const Handle* h, const mg_adapters* d, int64_t r
     const PlanLayout p = plan_layout(rows, d->n_adapters);
     const int32_t* w = static_cast<const int32_t*>(plan);
     a.tiles = reinterpret_cast<const int4*>(w);
+    a.n_tiles = static_cast<int>(p.segs / 4) - 1;
     a.order = w + p.order;
   } else {
     a.ids = ids;

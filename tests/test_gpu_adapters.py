@@ -146,6 +146,31 @@ def test_adapters_of_sorted_rows(layer, counts, K, N, r):
     assert not grads[0][none].any() and not any(grads[k][g].any() for g, n in enumerate(counts) if n == 0 for k in (1, 2))
 
 
+@pytest.mark.parametrize("counts,extra", [([1] * 100 + [0] * 60, 1), ([3] * 300, 1), ([5, 0, 2], 300), ([2] * 160, 100), ([0] * 20 + [130] * 5, 7),
+                                          ([1, 200] * 40, 0), ([9] * 75, 75)])
+def test_tiles_that_share_blocks_and_tiles_that_do_not(layer, counts, extra):
+    """More and fewer tiles than run at once, by rounds, by clusters, and by halves of clusters; rows without an adapter behind them."""
+    c, pad, rows = _segments(counts, extra)
+    ids = torch.full((rows,), -1, dtype=torch.int32, device=DEV)
+    for g, n in enumerate(counts):
+        ids[int(pad[g]):int(pad[g]) + n] = g
+    K, N, r = 328, 203, 16
+    x, y, go = _rows(rows, K, 1), _rows(rows, N, 2), _rows(rows, N, 3)
+    down, up, scale = _adapters(len(counts), r, K, N, 4)
+    refs = _reference(x, y, down, up, scale, ids, go)
+    plan = layer.adapter_plan_sorted(c, pad, rows)
+    none = ids < 0
+    out, s = layer.adapter_add(y, x, down, up, plan, scale, keep=True)
+    assert _near(out, refs[0]) and torch.equal(out[none], y[none]) and not s[none].any()
+    grads = layer.adapter_grad(go, x, down, up, plan, scale, s)
+    assert all(_near(g, ref) for g, ref in zip(grads, refs[1:]))
+    assert not grads[0][none].any() and not any(grads[k][g].any() for g, n in enumerate(counts) if n == 0 for k in (1, 2))
+    place = _rows(rows, N, 2)
+    assert torch.equal(layer.adapter_add(place, x, down, up, plan, scale, out=place), out)
+    part = layer.adapter_grad(go, x, down, up, plan, scale, s, False, True, True)
+    assert torch.equal(part[1], grads[1]) and torch.equal(part[2], grads[2])
+
+
 def test_plans_from_permute_plan(layer):
     idx = torch.randint(0, 8, (50, 2), generator=_gen(1), device=DEV, dtype=torch.int32)
     idx[:, 1] = (idx[:, 0] + 1) % 8
