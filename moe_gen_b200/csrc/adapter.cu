@@ -38,9 +38,9 @@ __device__ __forceinline__ void copy_row(uint32_t to, const uint16_t* row, int c
 __device__ __forceinline__ void copy_whole(uint32_t to, const uint16_t* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-// the same, or zeros
-__device__ __forceinline__ void copy_or_zeros(uint32_t to, const uint16_t* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+// the first `bytes` of them, zeros behind
+__device__ __forceinline__ void copy_part(uint32_t to, const uint16_t* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -439,7 +439,7 @@ struct TileCopies {
   __device__ __forceinline__ void step(uint32_t to, bool first, int c, int n, int rows) const {
     const int r0 = t >> 3, p = t & 7, first_row = t / 32 * 4;
     const uint32_t mine = r0 * 128 + ((p ^ (r0 & 7)) << 4);
-    const bool inside = c + 64 <= n, filled = a.rank == RP;
+    const bool inside = c + 64 <= n;
 #pragma unroll
     for (int j = 0; j < EACH; ++j)
       if (first_row + j * ROWS < rows) {
@@ -449,10 +449,13 @@ struct TileCopies {
     if (RP * 8 < WARPS * 32 && t >= RP * 8) return;
     if (first != BACK) {
       const int64_t ld = BACK ? a.ld2 : a.ld1;
-      if (inside && filled) {
-        const uint16_t* w = wide + r0 * ld + p * 8 + c;
+      if (inside) {
+        const uint16_t *first_row = wide + p * 8 + c, *w = first_row + r0 * ld;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j, w += ROWS * ld) copy_whole(to + C::ROWS + mine + j * ROWS * 128, w);
+        for (int j = 0; j < PIECES; ++j, w += ROWS * ld) {
+          const bool there = r0 + j * ROWS < a.rank;
+          copy_part(to + C::ROWS + mine + j * ROWS * 128, there ? w : first_row, there ? 16 : 0);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
@@ -464,10 +467,11 @@ struct TileCopies {
       const int64_t ld = BACK ? a.ld1 : a.ld2;
       const int nr = t / (RP / 8), np = t % (RP / 8);
       const uint32_t at = to + C::ROWS + (np >> 3) * 8192 + nr * 128 + (((np & 7) ^ (nr & 7)) << 4);
-      if (inside && filled) {
-        const uint16_t* w = narrow + (c + nr) * ld + np * 8;
+      if (inside) {
+        const int bytes = min(max(2 * (a.rank - np * 8), 0), 16);
+        const uint16_t* w = narrow + (c + nr) * ld + (bytes > 0 ? np * 8 : 0);
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j, w += NARROW_ROWS * ld) copy_whole(at + j * NARROW_ROWS * 128, w);
+        for (int j = 0; j < PIECES; ++j, w += NARROW_ROWS * ld) copy_part(at + j * NARROW_ROWS * 128, w, bytes);
       } else {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
@@ -936,16 +940,17 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
         for (int j = 0; j < 2; ++j) {
           const int64_t row = max(rows[j], 0);
           const bool there = rows[j] >= 0;
+          const int bytes = there ? 16 : 0;
           const uint16_t* w = wide + row * ldw;
           const uint16_t* n = narrow + row * C::NR + p * 8;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
-            if (f.c0 + 128 <= cols) copy_or_zeros(filling + mine + j * 4096 + b * 8192, w + c + b * 64, there);
+            if (f.c0 + 128 <= cols) copy_part(filling + mine + j * 4096 + b * 8192, w + c + b * 64, bytes);
             else copy_row<16>(filling + mine + j * 4096 + b * 8192, w, c + b * 64, there ? cols : 0);
           }
 #pragma unroll
           for (int b = 0; b < C::HALVES; ++b)
-            if (p < C::NR / 8) copy_or_zeros(filling + C::WIDE + mine + j * 4096 + b * 8192, n + b * 64, there);
+            if (p < C::NR / 8) copy_part(filling + C::WIDE + mine + j * 4096 + b * 8192, n + b * 64, bytes);
         }
         ++in;
         if (!ONE && in == f.steps) next_job();
