@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -25,6 +26,21 @@ def _whole(t: torch.Tensor) -> torch.Tensor:
     """t contiguous and on a 16-byte boundary, as the kernels read rows: a copy where it is a view that begins elsewhere."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+# Sizes are asked for once: a call of the library costs a microsecond, a tenth of an adapter call.
+@functools.lru_cache(maxsize=1024)
+def _plan_bytes(rows: int, n_adapters: int) -> int:
+    size = C.c_size_t()
+    L.check(L.load().mg_adapter_plan_bytes(rows, n_adapters, C.byref(size)))
+    return size.value
+
+
+@functools.lru_cache(maxsize=None)
+def _rank_stride(rank: int) -> int:
+    n = C.c_int32()
+    L.check(L.load().mg_adapter_rank_stride(rank, C.byref(n)))
+    return n.value
 
 
 class AdapterPlan:
@@ -659,9 +675,7 @@ class MoELayer:
 
     # ------------------------------------------------------------------ low-rank adapters
     def _plan_buffer(self, rows: int, n_adapters: int) -> torch.Tensor:
-        size = C.c_size_t()
-        L.check(self.lib.mg_adapter_plan_bytes(rows, n_adapters, C.byref(size)))
-        return torch.empty(size.value, dtype=torch.uint8, device=self.device)
+        return torch.empty_strided((_plan_bytes(rows, n_adapters),), (1,), dtype=torch.uint8, device=self.device)
 
     def adapter_plan(self, ids: torch.Tensor, n_adapters: int) -> AdapterPlan:
         """The rows of a batch sorted by adapter: ids [rows] int32, an id outside [0, n_adapters) for none."""
@@ -722,9 +736,8 @@ class MoELayer:
         return who if rows <= L.ADAPTER_DIRECT else self.adapter_plan(who, n_adapters)
 
     def _rank_rows(self, rows: int, rank: int) -> torch.Tensor:
-        n = C.c_int32()
-        L.check(self.lib.mg_adapter_rank_stride(rank, C.byref(n)))
-        return torch.empty(rows, n.value, dtype=torch.bfloat16, device=self.device)
+        n = _rank_stride(rank)
+        return torch.empty_strided((rows, n), (n, 1), dtype=torch.bfloat16, device=self.device)
 
     def adapter_add(self, y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, who, scale=1.0,
                     out: Optional[torch.Tensor] = None, keep: bool = False):
@@ -772,8 +785,8 @@ class MoELayer:
         if not (need_x or need_down or need_up):
             return None, None, None
         gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
-        gdown = torch.empty(down.shape, dtype=torch.bfloat16, device=self.device) if need_down else None
-        gup = torch.empty(up.shape, dtype=torch.bfloat16, device=self.device) if need_up else None
+        gdown = torch.empty_like(down, memory_format=torch.contiguous_format) if need_down else None
+        gup = torch.empty_like(up, memory_format=torch.contiguous_format) if need_up else None
         with self._on_device():
             L.check(self.lib.mg_adapter_grad(self._h, ad, grad_out.data_ptr(), ldg, x.data_ptr(), ldx, n, who.buf.data_ptr(),
                                              s.data_ptr(), gs.data_ptr(), _ptr(gx), ldgx, _ptr(gdown), _ptr(gup), self._stream()))

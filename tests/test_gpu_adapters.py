@@ -242,6 +242,19 @@ def test_scales_and_one_adapter_for_all(layer):
     assert _near(shared, _reference(x, y, down[:1], up[:1], torch.tensor([0.75]), first)[0])
 
 
+def test_adapters_whose_rows_lie_between_one_anothers(layer):
+    """down [rank, adapters, cols] and up [n_out, adapters, rank] seen as adapters: their gradients come as adapters one behind another."""
+    x, y, go = _rows(70, 64, 1), _rows(70, 96, 2), _rows(70, 96, 3)
+    down, up, scale = _adapters(3, 16, 64, 96, 4)
+    ids = _ids(70, 3, 5)
+    out, s = layer.adapter_add(y, x, down, up, ids, scale, keep=True)
+    want = layer.adapter_grad(go, x, down, up, ids, scale, s)
+    d2, u2 = down.transpose(0, 1).contiguous().transpose(0, 1), up.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(layer.adapter_add(y, x, d2, u2, ids, scale), out)
+    got = layer.adapter_grad(go, x, d2, u2, ids, scale, s)
+    assert all(torch.equal(a, b) and b.is_contiguous() for a, b in zip(want, got))
+
+
 def test_what_is_not_finite_stays_in_its_row(layer):
     n, K, N, r, G = 90, 160, 96, 12, 4
     x, y = _rows(n, K, 1), _rows(n, N, 2)
