@@ -280,12 +280,15 @@ class MoELayer:
         nr, rcols, ldr = self._rows_of(residual, torch.bfloat16, "residual")
         if (nr, rcols) != (n, cols):
             raise ValueError(f"residual {tuple(residual.shape)} for rows of {tuple(x.shape)}")
-        sum_out, lds = self._out_rows(sum_out, n, cols, "sum_out")
+        sum_out, lds = self._out_rows(sum_out, n, cols, "sum_out", x, ldx)
         return n, cols, ldx, ldr, sum_out, lds
 
-    def _out_rows(self, out: Optional[torch.Tensor], n: int, cols: int, what: str):
-        """out and the elements between its rows; a new one has its rows on 16-byte boundaries."""
+    def _out_rows(self, out: Optional[torch.Tensor], n: int, cols: int, what: str, like: torch.Tensor, ld_like: int):
+        """out and the elements between its rows; a new one has its rows on 16-byte boundaries (as those of `like`, bf16 rows of
+        n and cols ld_like apart, where these do: the cheaper allocation)."""
         if out is None:
+            if ld_like == cols and cols % 8 == 0:
+                return torch.empty_like(like), cols
             ld = (cols + 7) // 8 * 8
             return torch.empty_strided((n, cols), (ld, 1), dtype=torch.bfloat16, device=self.device), ld
         rows, o_cols, ld = self._rows_of(out, torch.bfloat16, what)
@@ -300,7 +303,7 @@ class MoELayer:
         adjacent columns (any cols, rows may lie further apart).  out and sum_out may each be x or the residual,
         not one another, and overlap nothing otherwise.  Any layer serves."""
         n, cols, ldx, ldr, h, lds = self._norm_args(x, residual, weight, sum_out)
-        y, ldo = self._out_rows(out, n, cols, "out")
+        y, ldo = self._out_rows(out, n, cols, "out", x, ldx)
         with self._on_device():
             L.check(self.lib.mg_add_rmsnorm(self._h, x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), eps, n, cols,
                                             None if residual is None else h.data_ptr(), lds, y.data_ptr(), ldo, self._stream()))
@@ -332,7 +335,7 @@ class MoELayer:
         nh, hcols, ldgh = (n, cols, 0) if grad_h is None else self._rows_of(grad_h, torch.bfloat16, "grad_h")
         if (ng, gcols) != (n, cols) or (nh, hcols) != (n, cols):
             raise ValueError(f"gradients of {(ng, gcols)} and {(nh, hcols)} for rows of {(n, cols)}")
-        gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
+        gx, ldgx = self._out_rows(None, n, cols, "grad_x", h, ldh) if need_x else (None, 0)
         if not (need_x or need_w):
             return None, None
         gw = torch.empty(cols, dtype=torch.float32, device=self.device) if need_w else None
@@ -756,7 +759,7 @@ class MoELayer:
             raise ValueError(f"y {tuple(y.shape)}, expected {(n, a_out)}")
         who = self._adapter_plan_of(who, n, n_adapters)
         ids, plan = (None, who.buf) if isinstance(who, AdapterPlan) else (who, None)
-        out, ldo = self._out_rows(out, n, n_out, "out")
+        out, ldo = self._out_rows(out, n, n_out, "out", y, ldy)
         s = self._rank_rows(n, rank) if keep else None
         with self._on_device():
             L.check(self.lib.mg_adapter_add(self._h, ad, x.data_ptr(), ldx, y.data_ptr(), ldy, n, _ptr(ids), _ptr(plan),
@@ -784,7 +787,7 @@ class MoELayer:
         self._check_rows(s, torch.bfloat16, n, gs.shape[1], "s")
         if not (need_x or need_down or need_up):
             return None, None, None
-        gx, ldgx = self._out_rows(None, n, cols, "grad_x") if need_x else (None, 0)
+        gx, ldgx = self._out_rows(None, n, cols, "grad_x", x, ldx) if need_x else (None, 0)
         gdown = torch.empty_like(down, memory_format=torch.contiguous_format) if need_down else None
         gup = torch.empty_like(up, memory_format=torch.contiguous_format) if need_up else None
         with self._on_device():
