@@ -147,7 +147,8 @@ struct AdapterArgs {
   float factor;
   int rank, n_adapters, n_rows;
   const int32_t* ids;         // a call without a plan
-  const int4* tiles;          // adapter (-1: none), first entry of order, rows with it, rows; behind them, the tiles of adapters and all
+  const int4* tiles;          // adapter (-1: none), first entry of order, rows with it, rows; behind them, the tiles of adapters, all, and the
+                              // adapters with rows
   int n_tiles, slots;         // tiles there is room for; blocks that run at once, a multiple of a cluster's
   const int32_t* order;
   int32_t* status;
@@ -821,8 +822,9 @@ struct AdapterGradArgs {
   uint16_t* out[2];             // [adapters][cols][rank], [adapters][rank][cols]
   const float* scale;
   float factor;
-  int rank, jobs;
+  int rank, n_adapters, jobs;
   const int4* segs;             // first entry of order, rows and number of every adapter, those of most rows first
+  const int4* total;            // .z of them have rows
   const int32_t* order;
   int32_t* status;
 };
@@ -871,7 +873,9 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
     j.steps = cr < all ? (all - cr + cs - 1) / cs : 0;
     return j;
   };
-  const int first = ONE ? static_cast<int>(blockIdx.x) / cs : static_cast<int>(blockIdx.x), last = ONE ? first + 1 : a.jobs;
+  const int with_rows = ONE ? 0 : a.total->z;
+  const int first = ONE ? static_cast<int>(blockIdx.x) / cs : static_cast<int>(blockIdx.x);
+  const int last = ONE ? first + 1 : with_rows * (a.blocks[0] + a.blocks[1]);
   // the jobs' lengths descend: turns go to and fro, the last block of one being the first of the next
   const int both = 2 * static_cast<int>(gridDim.x), hop0 = ONE ? 1 : both - 1 - 2 * first;
   if (tid == 0) {
@@ -921,14 +925,11 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
       }
     };
     auto next_job = [&]() {
-      do {
-        ahead += ahead_hop;
-        ahead_hop = both - ahead_hop;
-        if (ahead < last) f = job_of(ahead);
-      } while (ahead < last && f.steps == 0);
+      ahead += ahead_hop;
+      ahead_hop = both - ahead_hop;
+      if (ahead < last) f = job_of(ahead);
       in = 0;
     };
-    if (!ONE && f.steps == 0) next_job();
     look();
     auto fetch = [&]() {                               // what lies behind the last row or column arrives as zeros
       if (ONE ? in < f.steps : ahead < last) {
@@ -972,7 +973,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
         if (k > 0) done(k - 1);
         fetch();
       }
-      if (j.live == 0) {
+      if (ONE && j.live == 0) {
         // zeros, 16 bytes at a time where rows begin so: 128 columns of every one of the rank, or the rank of 128 columns in a piece
         const int have = min(cols - j.c0, 128);
         const int lines = j.which ? a.rank : 1, width = j.which ? have : have * a.rank;
@@ -1040,6 +1041,23 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
           else cluster_sum8<2>(at, 128 * 16, 0, v);
           store8(j.c0 + c, r, v);
         }
+      }
+    }
+    // the adapters without rows, whose gradients are zeros: 32 KB at a time
+#pragma unroll
+    for (int which = 0; !ONE && which < 2; ++which) {
+      const int64_t size = static_cast<int64_t>(a.rank) * a.cols[which];
+      const int chunks = static_cast<int>((size + 16383) / 16384);
+      const bool wide = reinterpret_cast<uintptr_t>(a.out[which]) % 16 == 0 && size % 8 == 0;
+      if (a.out[which] == nullptr) continue;
+      for (int64_t n = blockIdx.x; n < static_cast<int64_t>(a.n_adapters - with_rows) * chunks; n += gridDim.x) {
+        const int e = static_cast<int>(n / chunks), part = static_cast<int>(n - static_cast<int64_t>(e) * chunks);
+        uint16_t* to = a.out[which] + a.segs[with_rows + e].z * size + static_cast<int64_t>(part) * 16384;
+        const int have = static_cast<int>(min(size - static_cast<int64_t>(part) * 16384, static_cast<int64_t>(16384)));
+        if (wide)
+          for (int q = tid; q < have / 8; q += kAdapterThreads) reinterpret_cast<uint4*>(to)[q] = make_uint4(0u, 0u, 0u, 0u);
+        else
+          for (int q = tid; q < have; q += kAdapterThreads) to[q] = 0;
       }
     }
     copies_wait<0>();
@@ -1173,6 +1191,7 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
   }
   __syncthreads();
   static_assert(MG_ADAPTER_MAX <= kPlanWarps * 32, "a thread to an adapter");
+  int with_rows;
   {                                        // the adapters by their rows: 2^bits neighbouring threads compare one with all
     int bits = 5;
     while (bits > 0 && adapters << bits > kPlanWarps * 32) --bits;
@@ -1181,9 +1200,11 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
     if (e < adapters)
       for (int f = tid & ((1 << bits) - 1); f < adapters; f += 1 << bits) before += s_live[f] > n || (s_live[f] == n && f < e);
     for (int o = 1 << bits >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-    if (e < adapters && (tid & ((1 << bits) - 1)) == 0) segs[before] = make_int4(s_start[e], n, e, 0);
+    const bool one = e < adapters && (tid & ((1 << bits) - 1)) == 0;
+    if (one) segs[before] = make_int4(s_start[e], n, e, 0);
+    with_rows = __syncthreads_count(one && n > 0);
   }
-  if (tid == 0) tiles[n_tiles] = make_int4(min(s_tile[adapters], n_tiles), min(s_tile[groups], n_tiles), 0, 0);
+  if (tid == 0) tiles[n_tiles] = make_int4(min(s_tile[adapters], n_tiles), min(s_tile[groups], n_tiles), with_rows, 0);
   for (int e = tid; e < n_tiles; e += blockDim.x) {
     int4 t = make_int4(-1, 0, 0, 0);
     if (e < s_tile[groups]) {
@@ -1360,6 +1381,8 @@ int launch_adapter_grad(const Handle* h, const mg_adapters* d, const void* gout,
   b.factor = a.factor;
   b.rank = a.rank;
   b.order = a.order;
+  b.total = a.tiles + a.n_tiles;
+  b.n_adapters = d->n_adapters;
   b.segs = reinterpret_cast<const int4*>(static_cast<const int32_t*>(plan) + plan_layout(rows, d->n_adapters).segs);
   const int64_t jobs = static_cast<int64_t>(d->n_adapters) * (b.blocks[0] + b.blocks[1]);       // below 2^28
   b.jobs = static_cast<int>(jobs);

@@ -147,14 +147,14 @@ def test_adapters_of_sorted_rows(layer, counts, K, N, r):
 
 
 @pytest.mark.parametrize("counts,extra", [([1] * 100 + [0] * 60, 1), ([3] * 300, 1), ([5, 0, 2], 300), ([2] * 160, 100), ([0] * 20 + [130] * 5, 7),
-                                          ([1, 200] * 40, 0), ([9] * 75, 75)])
+                                          ([1, 200] * 40, 0), ([9] * 75, 75), ([0] * 300, 1), ([0] * 200 + [4], 2), ([0, 3, 0] * 100, 1)])
 def test_tiles_that_share_blocks_and_tiles_that_do_not(layer, counts, extra):
     """More and fewer tiles than run at once, by rounds, by clusters, and by halves of clusters; rows without an adapter behind them."""
     c, pad, rows = _segments(counts, extra)
     ids = torch.full((rows,), -1, dtype=torch.int32, device=DEV)
     for g, n in enumerate(counts):
         ids[int(pad[g]):int(pad[g]) + n] = g
-    K, N, r = 328, 203, 16
+    K, N, r = 328, 203, 16 if extra % 2 else 13
     x, y, go = _rows(rows, K, 1), _rows(rows, N, 2), _rows(rows, N, 3)
     down, up, scale = _adapters(len(counts), r, K, N, 4)
     refs = _reference(x, y, down, up, scale, ids, go)
