@@ -384,9 +384,10 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
 // the first product's, then finish s and the outputs, while four others copy the second product's; one has the products done, into tensor
 // memory.  s passes through shared memory in two parts of bf16.  A cluster of up to eight blocks shares a tile where there are few: each sums
 // s over its columns of x, then over the blocks for its share of the rows, and hands that to all.
-// 8192 rows of 4096 to 4096 columns, rank 64, 8 adapters: 54 us for 210 MB, 3.9 TB/s; 49152 rows of 2048 to 2048, rank 16, 64 adapters:
-// 145 us for 600 MB, 4.2 TB/s, the way back 111 us for 400 MB.  What bounds it is the chain within a block, fill, first product, s, second
-// product, drain: two blocks to an SM cover one another's gaps in part.  By MMAs of warps on tiles of 16 rows the first took 88 us.
+// 8192 rows of 4096 to 4096 columns, rank 64, 8 adapters: 54 us for 210 MB, 3.9 TB/s; 49152 rows of 64 adapters in a buffer of 57344, 2048 to
+// 2048, rank 16: 145 us for 670 MB, 4.6 TB/s, the way back 110 us for 440 MB.  Within a turn of all places it streams at what memory gives (296
+// tiles of 2048 to 2048: 90 us, 5.2 TB/s, 1184 tiles 5.7); what bounds it is the turn that is not full, and where clusters share tiles their
+// meeting, 9 of the 54 us, in which all blocks pause at once.  By MMAs of warps on tiles of 16 rows the first took 88 us.
 constexpr int kFinishWarps = 8, kCopyWarps = 4, kTileThreads = 32 * (kFinishWarps + kCopyWarps + 1);
 template <int RP>
 struct TileCfg {
