@@ -192,6 +192,19 @@ def test_gradients(layer, n, cols, with_h):
     assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
 
 
+@pytest.mark.parametrize("n,cols", [(37, 2048), (300, 4096), (601, 8192), (70, 77), (2500, 256), (40, 16384)])
+def test_a_gradient_in_the_place_of_another(layer, n, cols):
+    """From C: grad_x over grad_y, or over grad_h."""
+    gy, h, w, gh = _rows(n, cols, 1), _rows(n, cols, 2), _weight(cols, 3), _rows(n, cols, 4)
+    want, _ = layer.add_rmsnorm_grad(gy, h, w, 1e-6, gh, need_w=False)
+    for which in (0, 1):
+        a, b = gy.clone(), gh.clone()
+        to = (a, b)[which]
+        assert layer.lib.mg_add_rmsnorm_grad(layer._h, a.data_ptr(), cols, h.data_ptr(), cols, w.data_ptr(), 1e-6, n, cols, b.data_ptr(), cols,
+                                             to.data_ptr(), cols, None, None, 0, layer._stream()) == 0
+        assert torch.equal(to, want)
+
+
 @pytest.mark.parametrize("n", (64, 65))
 def test_scratch_of_the_gradient(layer, n):
     """None up to 64 rows, refused where it is missing or too small beyond."""
