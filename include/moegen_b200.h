@@ -581,8 +581,9 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
  *   d_plan: mg_adapter_plan_bytes bytes on a 16-byte boundary.  One plan serves all calls on these rows (with n_adapters
  *   adapters), and is only read by them.
  * mg_adapter_plan_sorted: the same for rows that lie sorted, by mg_permute_plan's counts[n_adapters] and
- *   pad_offsets[n_adapters + 1]: adapter g has the rows [pad_offsets[g], pad_offsets[g] + counts[g]).  Offsets that leave
- *   [0, n_rows] or descend are cut off.
+ *   pad_offsets[n_adapters + 1]: adapter g has the rows [pad_offsets[g], pad_offsets[g] + counts[g]), as far as
+ *   they lie in front of pad_offsets[g + 1]; all other rows, those in front of pad_offsets[0] and behind the last offset too, have none.  An
+ *   offset outside [0, n_rows] counts as its nearer end, one below an offset in front of it as that one.
  * mg_adapter_add: with d_ids and no plan (NULL) up to MG_ADAPTER_DIRECT rows in one launch; with a plan any number, and d_ids is not
  *   read.  d_out may be d_y with its stride, and overlaps nothing otherwise.  d_s, where not NULL, receives s for mg_adapter_grad:
  *   [n_rows] rows of mg_adapter_rank_stride(rank) elements, s rounded to bf16 in their first half and what that leaves in the

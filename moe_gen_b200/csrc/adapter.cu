@@ -1081,6 +1081,7 @@ constexpr int kPlanWarps = 32, kPlanAhead = 8;
 struct PlanLayout { int64_t tiles, segs, order, place, words; };          // offsets in words
 PlanLayout plan_layout(int64_t rows, int64_t adapters) {
   PlanLayout p;
+  // tiles: G groups of rows, some of none, are cut into (rows - G) / 128 + G at most, rounded down; G is adapters + 2 at most
   const int64_t n = (rows + kAdapterTile - 1) / kAdapterTile + adapters + 1;
   p.tiles = 0;
   p.segs = 4 * (n + 1);
@@ -1092,13 +1093,15 @@ PlanLayout plan_layout(int64_t rows, int64_t adapters) {
 
 // One block sorts the rows by adapter, rows without one last, every adapter's in ascending order, and cuts them into tiles.  Warps take
 // runs of rows and count them by adapter; with the counts of the warps before, every row has its place.
-// SORTED: the rows lie in segments already (pad_offsets, counts); the order is the rows' own, written by the other blocks.
+// SORTED: the rows lie in segments already (pad_offsets, counts); the order is the rows' own, written by the other blocks.  Each offset counts as
+// no less than those in front of it, so that whatever they hold every row is in one tile, those in front of the first segment and behind
+// the last among them.
 template <bool SORTED>
 __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int32_t* ids, const int32_t* counts, const int32_t* pad,
                                                                        int rows, int adapters, int n_tiles, int4* tiles, int4* segs,
                                                                        int32_t* order, int32_t* place) {
   extern __shared__ __align__(16) int s_mem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, groups = adapters + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, groups = adapters + (SORTED ? 2 : 1);
   if (SORTED && blockIdx.x > 0) {
     const int64_t at = static_cast<int64_t>(blockIdx.x - 1) * blockDim.x + tid;
     if (at < rows) order[at] = static_cast<int32_t>(at);
@@ -1156,11 +1159,34 @@ __global__ void __launch_bounds__(kPlanWarps * 32) adapter_plan_kernel(const int
       }
     }
   } else {
-    for (int e = tid; e < groups; e += blockDim.x) {
-      const int lo = min(max(pad[e], 0), rows), hi = e < adapters ? min(max(pad[e + 1], lo), rows) : rows;
-      s_start[e] = lo;
-      s_len[e] = hi - lo;
-      s_live[e] = e < adapters ? min(max(counts[e], 0), hi - lo) : 0;
+    for (int e = tid; e <= adapters; e += blockDim.x) s_start[e] = min(max(pad[e], 0), rows);
+    __syncthreads();
+    if (warp == 0) {                                   // the largest so far, in runs of a lane
+      const int run = (adapters + 32) / 32;
+      int most = 0;
+      for (int k = 0; k < run; ++k)
+        if (lane * run + k <= adapters) most = max(most, s_start[lane * run + k]);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, most, o);
+        if (lane >= o) most = max(most, u);
+      }
+      most = __shfl_up_sync(0xFFFFFFFFu, most, 1);
+      if (lane == 0) most = 0;
+      for (int k = 0; k < run; ++k)
+        if (lane * run + k <= adapters) s_start[lane * run + k] = most = max(most, s_start[lane * run + k]);
+    }
+    __syncthreads();
+    for (int e = tid; e < adapters; e += blockDim.x) {
+      const int len = s_start[e + 1] - s_start[e];
+      s_len[e] = len;
+      s_live[e] = min(max(counts[e], 0), len);
+    }
+    if (tid == 0) {                                    // the rows without an adapter: behind the last segment, in front of the first
+      s_len[adapters] = rows - s_start[adapters];
+      s_start[adapters + 1] = 0;
+      s_len[adapters + 1] = s_start[0];
+      s_live[adapters] = s_live[adapters + 1] = 0;
     }
   }
   __syncthreads();
@@ -1263,6 +1289,7 @@ int launch_tiles_as(const Handle* h, AdapterArgs a, cudaStream_t st) {
   while (P > 1 && full * P > places && !(P == 4 && 4 * full <= 5 * a.n_adapters)) P /= 2;
   a.slots = static_cast<int>(places / P * P);
   const int64_t all = a.n_tiles + full, most = a.n_tiles + full * P + (P > 1 ? a.slots : 0);      // blocks, P to a tile and one to those of adapters
+  // two clusters more: one for what is left of a round, one for rows without an adapter that begin a tile at both ends of the buffer
   MG_CUDA(launch_clusters(adapter_tile_kernel<RP, BACK>, (all * P < most ? all * P : most) / P + 2, P, kTileThreads, C::SMEM, st, a));
   return MG_OK;
 }
@@ -1311,7 +1338,7 @@ int launch_adapter_plan(const Handle* h, const int32_t* ids, const int32_t* coun
                         void* plan, cudaStream_t st) {
   const PlanLayout p = plan_layout(rows, adapters);
   int32_t* w = static_cast<int32_t*>(plan);
-  const int n_tiles = static_cast<int>(p.segs / 4) - 1, groups = adapters + 1;
+  const int n_tiles = static_cast<int>(p.segs / 4) - 1, groups = adapters + (ids != nullptr ? 1 : 2);
   static bool done[2][64];
   constexpr size_t most = (4 * (MG_ADAPTER_MAX + 1) + 1 + kPlanWarps * (MG_ADAPTER_MAX + 1)) * sizeof(int);
   const size_t smem = (4 * groups + 1 + (ids != nullptr ? kPlanWarps * groups : 0)) * sizeof(int);

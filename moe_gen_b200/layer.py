@@ -690,7 +690,8 @@ class MoELayer:
         return AdapterPlan(buf, rows, n_adapters)
 
     def adapter_plan_sorted(self, counts: torch.Tensor, pad_offsets: torch.Tensor, rows: int) -> AdapterPlan:
-        """The plan of expert-sorted rows (permute_plan's counts and pad_offsets, buffers of `rows` rows), an adapter to an expert."""
+        """The plan of expert-sorted rows (permute_plan's counts and pad_offsets, buffers of `rows` rows), an adapter to an expert.  Rows in
+        no expert's segment have none, those in front of the first offset among them."""
         self._check_in(counts, torch.int32, "counts")
         self._check_in(pad_offsets, torch.int32, "pad_offsets")
         n = counts.numel()
