@@ -590,8 +590,8 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
  *   second, zeros behind the rank and for rows without an adapter.
  * mg_adapter_grad: the gradients, with gs[t] = f[g] * grad_out[t] . up[g], taken to 16 bits like s:
  *     grad_x[t] = gs[t] . down[g],   grad_down[g] = sum_t gs[t]^T x[t],   grad_up[g] = f[g] * sum_t grad_out[t]^T s[t]
- *   grad_x is zero in rows without an adapter, grad_down [n_adapters][rank][cols] and grad_up [n_adapters][n_out][rank] (bf16, contiguous,
- *   rounded once) in adapters without rows.  Each may be NULL and is then not computed.  The gradient of y is grad_out itself.  d_gs:
+ *   grad_x is zero in rows without an adapter, grad_down [n_adapters][rank][cols] and grad_up [n_adapters][n_out][rank] (bf16, contiguous, on
+ *   16-byte boundaries, rounded once) in adapters without rows.  Each may be NULL and is then not computed.  The gradient of y is grad_out itself.  d_gs:
  *   scratch like d_s.  d_s is read for grad_up alone.  What is written overlaps nothing.  The same rows and plan give the same bits. */
 #define MG_ADAPTER_MAX     1024
 #define MG_ADAPTER_DIRECT   256

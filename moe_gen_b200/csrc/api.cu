@@ -1646,10 +1646,10 @@ int mg_adapter_grad(mg_handle hh, const mg_adapters* ad, const void* d_gout, int
   MG_REQUIRE(d_gout && d_plan && (d_x || !d_gdown) && (d_s || !d_gup) && (d_gs || (!d_gx && !d_gdown)), MG_ERR_NULL,
              "mg_adapter_grad: null pointer");
   MG_REQUIRE(aligned16(d_gout) && aligned16(d_x) && aligned16(d_s) && aligned16(d_gs) && aligned16(d_gx) && aligned16(d_plan) &&
-                 row_stride(ldg, ad->n_out) && (d_gdown == nullptr || row_stride(ldx, ad->cols)) &&
+                 aligned16(d_gdown) && aligned16(d_gup) && row_stride(ldg, ad->n_out) && (d_gdown == nullptr || row_stride(ldx, ad->cols)) &&
                  (d_gx == nullptr || row_stride(ldgx, ad->cols)),
-             MG_ERR_SHAPE, "mg_adapter_grad: rows must begin on 16-byte boundaries (strides %lld, %lld, %lld)", static_cast<long long>(ldg),
-             static_cast<long long>(ldx), static_cast<long long>(ldgx));
+             MG_ERR_SHAPE, "mg_adapter_grad: rows and the adapters' gradients must begin on 16-byte boundaries (strides %lld, %lld, %lld)",
+             static_cast<long long>(ldg), static_cast<long long>(ldx), static_cast<long long>(ldgx));
   MG_REQUIRE(d_gx == nullptr || (d_gx != d_gout && d_gx != d_x), MG_ERR_CONFIG, "mg_adapter_grad: grad_x needs a buffer of its own");
   return launch_adapter_grad(h, ad, d_gout, ldg, d_x, ldx, n_rows, d_plan, d_s, d_gs, d_gx, ldgx, d_gdown, d_gup, st);
 }
