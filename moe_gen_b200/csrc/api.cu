@@ -1078,6 +1078,21 @@ constexpr int64_t kUnchainedDownTokens = 64;
 
 // d_residual: nullptr, or [T,H] bf16 added to the block's bf16 output in the combine (may be d_y)
 // d_logits_in: nullptr, or caller-computed fp32 router logits [T,E] used in place of the router GEMM
+// what moe_forward_impl asks of its arguments for T > 0 tokens, for calls that write something before it as well
+static int check_forward(const Handle* h, const void* d_x, int64_t T, const void* d_gate_w, const float* d_logits_in, const float* d_bias,
+                         const void* d_packed, const void* d_ws, size_t ws_bytes, const void* d_residual, const void* d_y) {
+  MG_REQUIRE(d_x && (d_gate_w || d_logits_in) && d_packed && d_ws && d_y, MG_ERR_NULL, "mg_moe_forward: null pointer");
+  MG_REQUIRE(aligned16(d_x) && aligned16(d_y) && aligned16(d_residual), MG_ERR_SHAPE,
+             "mg_moe_forward: hidden states and output must begin on a 16-byte boundary");
+  MG_REQUIRE(h->d.ep_size == 1, MG_ERR_CONFIG, "mg_moe_forward is the single-GPU path (ep_size == 1)");
+  MG_REQUIRE(h->d.gating != MG_GATE_SIGMOID_NOAUX_TC || d_bias != nullptr, MG_ERR_NULL,
+             "noaux_tc gating needs e_score_correction_bias");
+  const size_t need = ws_layout(h, T, 0).total;
+  MG_REQUIRE(ws_bytes >= need, MG_ERR_WORKSPACE, "workspace %zu bytes < %zu needed for %lld tokens", ws_bytes, need,
+             static_cast<long long>(T));
+  return MG_OK;
+}
+
 static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void* d_gate_w, const float* d_bias,
                             const void* d_packed, void* d_ws, size_t ws_bytes, const void* d_residual, void* d_y,
                             void* stream, const float* d_logits_in = nullptr) {
@@ -1085,18 +1100,11 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   if (!h) return MG_ERR_STATE;
   MG_REQUIRE(T >= 0, MG_ERR_SHAPE, "negative token count");
   if (T == 0) { h->last_launches = 0; return MG_OK; }   // empty batch: nothing to read or write
-  MG_REQUIRE(d_x && (d_gate_w || d_logits_in) && d_packed && d_ws && d_y, MG_ERR_NULL, "mg_moe_forward: null pointer");
-  MG_REQUIRE(aligned16(d_x) && aligned16(d_y) && aligned16(d_residual), MG_ERR_SHAPE,
-             "mg_moe_forward: hidden states and output must begin on a 16-byte boundary");
-  MG_REQUIRE(h->d.ep_size == 1, MG_ERR_CONFIG, "mg_moe_forward is the single-GPU path (ep_size == 1)");
-  MG_REQUIRE(h->d.gating != MG_GATE_SIGMOID_NOAUX_TC || d_bias != nullptr, MG_ERR_NULL,
-             "noaux_tc gating needs e_score_correction_bias");
+  int rc = check_forward(h, d_x, T, d_gate_w, d_logits_in, d_bias, d_packed, d_ws, ws_bytes, d_residual, d_y);
+  if (rc != MG_OK) return rc;
   const mg_layer_desc& d = h->d;
   const WsLayout L = ws_layout(h, T, 0);
-  MG_REQUIRE(ws_bytes >= L.total, MG_ERR_WORKSPACE, "workspace %zu bytes < %zu needed for %lld tokens", ws_bytes,
-             L.total, static_cast<long long>(T));
   h->last_launches = 0;
-  if (T == 0) return MG_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(d_ws);
   float* logits = reinterpret_cast<float*>(ws + L.off[WS_LOGITS]);
@@ -1121,7 +1129,6 @@ static int moe_forward_impl(mg_handle hh, const void* d_x, int64_t T, const void
   // them or their times are asked for one by one; the int8 products are launched by ordinary dependence
   const bool chain = deq == nullptr && !h->stage_timing && d.weight_format != MG_WEIGHT_INT8_CHANNEL;
   if (h->stage_timing) MG_CUDA(cudaEventRecord(h->stage_ev[h->stage_calls % kStageSlots][0], st));
-  int rc;
   const bool deq_same = h->deq_scratch == deq && h->deq_packed == d_packed && h->deq_stream == st;
   if (deq != nullptr && fp8_predequant(h, T) && !(h->opt_keep_dequant && h->deq_valid && deq_same) &&
       !(h->deq_inflight && deq_same)) {
@@ -1445,8 +1452,14 @@ int mg_moe_block_forward_add(mg_handle hh, const void* d_hidden, const void* d_r
              MG_ERR_SHAPE, "mg_moe_block_forward_add: rows and weight must begin on a 16-byte boundary");
   const int64_t H = h->d.hidden;
   MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_moe_block_forward_add: negative eps");
-  int rc = launch_add_norm(d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, nullptr, true,
-                           static_cast<cudaStream_t>(stream));
+  MG_REQUIRE(T < (1ll << 31), MG_ERR_LIMIT, "mg_moe_block_forward_add: %lld tokens", static_cast<long long>(T));
+  // all that is refused, before the sum takes the place of one of its terms
+  MG_REQUIRE(aligned16(d_gate_w) && aligned16(d_packed) && aligned16(d_ws), MG_ERR_SHAPE,
+             "mg_moe_block_forward_add: weights and workspace must begin on a 16-byte boundary");
+  int rc = check_forward(h, d_xnorm, T, d_gate_w, nullptr, d_bias, d_packed, d_ws, ws_bytes, d_out, d_out);
+  if (rc != MG_OK) return rc;
+  rc = launch_add_norm(d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, nullptr, true,
+                       static_cast<cudaStream_t>(stream));
   if (rc != MG_OK) return rc;
   rc = moe_forward_impl(hh, d_xnorm, T, d_gate_w, d_bias, d_packed, d_ws, ws_bytes, d_out, d_out, stream);
   if (rc == MG_OK) h->last_launches += 1;

@@ -17,3 +17,13 @@ def test_gradients_of_adapters_off_a_boundary_are_refused(handle, kw, rank, cols
     ad = _adapters(rank=rank, cols=cols, n_out=n_out, down_stride=rank * 72, ld_down=72, up_stride=n_out * ld_up, ld_up=ld_up)
     assert L.load().mg_adapter_grad(handle[0], C.byref(ad), a["go"], a["ldg"], a["x"], a["ldx"], a["n"], a["plan"], a["s"], a["gs"], a["gx"],
                                     a["ldgx"], a["gdown"], a["gup"], None) == -2
+
+
+@pytest.mark.parametrize("kw,code", [(dict(gate=None), -1), (dict(packed=None), -1), (dict(ws=None), -1), (dict(n=1 << 31), -7), (dict(n=1 << 40), -7), (dict(), -3),
+                                     (dict(gate=5 * P + 8), -2), (dict(packed=6 * P + 2), -2), (dict(ws=8 * P + 4), -2)])
+def test_blocks_with_a_residual_are_refused_before_anything_is_launched(handle, kw, code):  # noqa: F811
+    """The stand-in belongs to no number of ranks, which the block refuses: were the sum launched first, it would be the launch that fails here."""
+    a = dict(n=4, gate=5 * P, packed=6 * P, ws=8 * P)
+    a.update(kw)
+    assert L.load().mg_moe_block_forward_add(handle[0], P, 2 * P, 3 * P, 1e-6, a["n"], a["gate"], None, a["packed"], 7 * P, a["ws"], 1 << 40, P,
+                                             None) == code
