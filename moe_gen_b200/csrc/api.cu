@@ -1456,6 +1456,7 @@ int mg_moe_block_forward_add(mg_handle hh, const void* d_hidden, const void* d_r
   // all that is refused, before the sum takes the place of one of its terms
   MG_REQUIRE(aligned16(d_gate_w) && aligned16(d_packed) && aligned16(d_ws), MG_ERR_SHAPE,
              "mg_moe_block_forward_add: weights and workspace must begin on a 16-byte boundary");
+  MG_REQUIRE(h->d.n_experts <= 256, MG_ERR_SHAPE, "mg_moe_block_forward_add: the router's product takes at most 256 experts");
   int rc = check_forward(h, d_xnorm, T, d_gate_w, nullptr, d_bias, d_packed, d_ws, ws_bytes, d_out, d_out);
   if (rc != MG_OK) return rc;
   rc = launch_add_norm(d_hidden, H, d_residual, H, d_norm_weight, eps, T, H, d_out, H, d_xnorm, H, nullptr, true,

@@ -29,3 +29,17 @@ def test_a_refused_block_leaves_the_residual_stream(built_lib, place):
     want = layer.block_forward(before[0], w, 1e-6, residual=before[1])
     assert call() == 0 and torch.equal(t[place], want) and torch.equal(t[1 - place], before[1 - place])
     layer.close()
+
+
+def test_more_experts_than_the_router_takes(built_lib):
+    from moe_gen_b200 import MoELayer
+    layer = MoELayer(hidden=256, inter=128, n_experts=260, top_k=2, device=DEV)
+    layer.set_router(torch.zeros(260, 256))
+    t = [torch.randn(3, 256, device=DEV).to(torch.bfloat16) for _ in range(2)]
+    before = [v.clone() for v in t]
+    for out in t:
+        with pytest.raises(RuntimeError, match="256 experts"):
+            layer.block_forward(t[0], torch.ones(256, dtype=torch.bfloat16, device=DEV), out=out, residual=t[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(t, before))
+    layer.close()
