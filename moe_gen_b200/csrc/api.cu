@@ -1539,8 +1539,8 @@ int mg_add_rmsnorm_grad(mg_handle hh, const void* d_gy, int64_t ldgy, const void
              "mg_add_rmsnorm_grad: rows of %lld, strides %lld, %lld, %lld and %lld", static_cast<long long>(cols),
              static_cast<long long>(ldgy), static_cast<long long>(ldh), static_cast<long long>(ldgh), static_cast<long long>(ldgx));
   MG_REQUIRE(eps >= 0.f, MG_ERR_CONFIG, "mg_add_rmsnorm_grad: negative eps");
-  MG_REQUIRE(d_gx || d_gw, MG_ERR_NULL, "mg_add_rmsnorm_grad: no gradient asked for");
   if (n_rows > 0) {
+    MG_REQUIRE(d_gx || d_gw, MG_ERR_NULL, "mg_add_rmsnorm_grad: no gradient asked for");
     const size_t need = norm_grad_ws_bytes(h, n_rows, cols);
     MG_REQUIRE(d_gy && d_h && d_weight && (d_gw == nullptr || d_ws || need == 0), MG_ERR_NULL, "mg_add_rmsnorm_grad: null pointer");
     MG_REQUIRE((d_gx != d_gy || ldgx == ldgy) && (d_gx != d_gh || d_gh == nullptr || ldgx == ldgh) && d_gx != d_h, MG_ERR_CONFIG,

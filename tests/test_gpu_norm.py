@@ -417,3 +417,21 @@ def test_the_patched_decoder_layer_adds_in_the_norms_launch(built_lib, shape):
         else:
             assert torch.equal(dl(x)[0], want), name
         assert torch.equal(x, before)
+
+
+@pytest.mark.parametrize("with_h", (True, False))
+def test_gradients_of_no_rows(layer, with_h):
+    """Of each of the two alone, and through autograd with a frozen weight."""
+    from moe_gen_b200 import add_norm
+    w = _weight(64, 1)
+    x = torch.zeros(0, 64, dtype=torch.bfloat16, device=DEV)
+    gh = x if with_h else None
+    gx, gw = layer.add_rmsnorm_grad(x, x, w, 1e-6, gh, need_w=False)
+    assert gx.shape == (0, 64) and gw is None
+    gx, gw = layer.add_rmsnorm_grad(x, x, w, 1e-6, gh, need_x=False)
+    assert gx is None and not gw.any()
+    for frozen in (True, False):
+        leaves = [x.clone().requires_grad_(True), x.clone().requires_grad_(True), w.clone().requires_grad_(not frozen)]
+        h, y = add_norm(layer, *leaves)
+        got = torch.autograd.grad((h, y) if with_h else y, leaves[:2 if frozen else 3], (x, x) if with_h else x)
+        assert got[0].shape == got[1].shape == (0, 64) and (frozen or not got[2].any())

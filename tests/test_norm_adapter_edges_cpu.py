@@ -27,3 +27,9 @@ def test_blocks_with_a_residual_are_refused_before_anything_is_launched(handle, 
     a.update(kw)
     assert L.load().mg_moe_block_forward_add(handle[0], P, 2 * P, 3 * P, 1e-6, a["n"], a["gate"], None, a["packed"], 7 * P, a["ws"], 1 << 40, P,
                                              None) == code
+
+
+@pytest.mark.parametrize("n,gx,gw,code", [(0, None, None, 0), (0, 5 * P, None, 0), (3, None, None, -1)])
+def test_norm_gradients_of_no_rows(handle, n, gx, gw, code):  # noqa: F811
+    """torch's address of an empty tensor is null: a batch without rows is one gradient without an address."""
+    assert L.load().mg_add_rmsnorm_grad(handle[0], P, 64, 2 * P, 64, 3 * P, 1e-6, n, 64, 4 * P, 64, gx, 64, gw, None, 0, None) == code
