@@ -19,6 +19,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
+from . import lib as L
 from .layer import AdapterPlan, MoELayer, _whole
 
 
@@ -143,7 +144,9 @@ def combine_rows(layer: MoELayer, out_rows: torch.Tensor, dst_row: torch.Tensor,
 def add_norm(layer: MoELayer, x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor,
              eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """MoELayer.add_rmsnorm -> (h, y), differentiable in x, residual and weight: h = x + residual goes on as the residual stream, y is its
-    norm.  Without a residual h is a copy of x."""
+    norm.  Without a residual h is a copy of x.  At most 16384 columns where a gradient is to be taken."""
+    if weight.numel() > L.NORM_GRAD_COLS and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+        raise ValueError(f"rows of {weight.numel()}: the norm's gradient takes at most {L.NORM_GRAD_COLS} columns")
     return _AddNorm.apply(x, residual, weight, layer, eps)
 
 

@@ -42,7 +42,7 @@ class LayerDesc(C.Structure):
 
 
 ADAPTER_MAX, ADAPTER_DIRECT = 1024, 256
-NORM_GRAD_FEW = 64
+NORM_GRAD_FEW, NORM_GRAD_COLS = 64, 16384
 
 
 class Adapters(C.Structure):

@@ -33,3 +33,9 @@ def test_blocks_with_a_residual_are_refused_before_anything_is_launched(handle, 
 def test_norm_gradients_of_no_rows(handle, n, gx, gw, code):  # noqa: F811
     """torch's address of an empty tensor is null: a batch without rows is one gradient without an address."""
     assert L.load().mg_add_rmsnorm_grad(handle[0], P, 64, 2 * P, 64, 3 * P, 1e-6, n, 64, 4 * P, 64, gx, 64, gw, None, 0, None) == code
+
+
+def test_the_longest_rows_of_the_norms_gradient(handle):  # noqa: F811
+    n = C.c_size_t()
+    assert L.load().mg_add_rmsnorm_grad_ws_bytes(handle[0], 0, L.NORM_GRAD_COLS, C.byref(n)) == 0
+    assert L.load().mg_add_rmsnorm_grad_ws_bytes(handle[0], 0, L.NORM_GRAD_COLS + 1, C.byref(n)) == -7
