@@ -153,6 +153,8 @@ def add_norm(layer: MoELayer, x: torch.Tensor, residual: Optional[torch.Tensor],
 def adapt_rows(layer: MoELayer, y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, plan: AdapterPlan,
                scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
     """MoELayer.adapter_add by a plan, differentiable in y, x, down and up (the scales are constants)."""
+    if not isinstance(plan, AdapterPlan):
+        raise ValueError("adapt_rows takes a plan (adapter_plan, adapter_plan_sorted): ids could change before the gradient is taken")
     if isinstance(scale, torch.Tensor) and scale.requires_grad:
         raise ValueError("adapt_rows has no gradient for its scales: detach them")
     return _AdaptRows.apply(y, x, down, up, layer, plan, scale)

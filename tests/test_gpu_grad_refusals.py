@@ -37,3 +37,21 @@ def test_rows_longer_than_the_norms_gradient_takes(layer, with_residual):
             else:
                 with pytest.raises(ValueError, match="16384"):
                     add_norm(layer, *leaves)
+
+
+def test_adapters_of_rows_without_a_plan(layer):
+    """Ids that change between the passes would give another batch's gradients: a plan is made once and only read."""
+    from moe_gen_b200 import adapt_rows
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, y, down, up = (torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16) for s in ((40, 64), (40, 32), (3, 16, 64), (3, 32, 16)))
+    ids = torch.randint(-1, 3, (40,), generator=g, device=DEV, dtype=torch.int32)
+    plan = layer.adapter_plan(ids, 3)
+    for frozen in (True, False):
+        leaf = x.clone().requires_grad_(not frozen)
+        with pytest.raises(ValueError, match="plan"):
+            adapt_rows(layer, y, leaf, down, up, ids, 0.5)
+    out, s = layer.adapter_add(y, x, down, up, plan, 0.5, keep=True)
+    want = layer.adapter_grad(y, x, down, up, plan, 0.5, s)
+    got = adapt_rows(layer, y, leaf, down, up, plan, 0.5)
+    ids.fill_(1)
+    assert torch.equal(got, out) and torch.equal(torch.autograd.grad(got, leaf, y)[0], want[0])
