@@ -961,7 +961,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
       copies_commit();
       filling = filling == ring + (S - 1) * C::STAGE ? ring : filling + C::STAGE;
     };
-    auto done = [&](int k) { mbar_wait(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 128); };
+    auto done = [&](int k) { wait_warp(smem_u32(&s_done[k % S]), (k / S) & 1, &s_abort, a.status, 128); };
 #pragma unroll 1
     for (int k = 0; k < S - 1; ++k) fetch();
     int k = 0;
