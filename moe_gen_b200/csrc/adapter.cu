@@ -275,13 +275,11 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
       }
       return v;
     };
-    if (cs > 1) {
-      for (int p = tid; p < QUADS; p += kAdapterThreads) reinterpret_cast<float4*>(red)[p] = block_sum(p);
-      cluster_sync_all();
-    }
+    for (int p = tid; p < QUADS; p += kAdapterThreads) reinterpret_cast<float4*>(red)[p] = block_sum(p);
+    cluster_sync_all();
     for (int p = tid; p < QUADS; p += kAdapterThreads) {
       const int row = 4 * p / RP, r = 4 * p % RP;
-      const float4 u = cs > 1 ? cluster_sum(smem_u32(parts + p), cs) : block_sum(p);
+      const float4 u = cluster_sum(smem_u32(parts + p), cs);
       float v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = row < live && r + e < a.rank ? v[e] : 0.f;
@@ -302,8 +300,7 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
         *reinterpret_cast<uint2*>(kept + RP) = low;
       }
     }
-    if (cs > 1) cluster_sync_all();                   // the ring is free again, here and in the blocks that have read it
-    else __syncthreads();
+    cluster_sync_all();                               // the ring is free again, here and in the blocks that have read it
   } else if (a.s != nullptr && cr == 0) {
     for (int p = tid; p < len * RP; p += kAdapterThreads)
       *reinterpret_cast<uint32_t*>(a.s + static_cast<int64_t>(s_rows[p / RP]) * (2 * RP) + 2 * (p % RP)) = 0u;

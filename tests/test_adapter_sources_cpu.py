@@ -20,3 +20,9 @@ def test_which_kernels_wait():
 def test_warps_wait_by_one_vote(name):
     body = KERNELS[name]
     assert "wait_warp(" in body and not re.search(r"\bmbar_(try_)?wait\(", body)
+
+
+def test_few_rows_are_always_a_clusters():
+    """The launch gives a row two to eight blocks, and the kernel has no other form."""
+    launch = re.search(r"int launch_direct_as\(.*?\n}", TEXT, re.S).group(0)
+    assert re.search(r"int cs = 8;\s*while \(cs > 2 &&", launch) and "cs > 1" not in KERNELS["adapter_direct_kernel"]
