@@ -704,7 +704,7 @@ class MoELayer:
         return AdapterPlan(buf, rows, n)
 
     def _adapters(self, down: torch.Tensor, up: torch.Tensor, scale):
-        """-> (mg_adapters as bytes, adapters, rank, cols, n_out)"""
+        """-> (mg_adapters as bytes, adapters, rank, cols, n_out, what the bytes point to)"""
         for t, what in ((down, "down"), (up, "up")):
             if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != self.device:
                 raise ValueError(f"{what}: expected [adapters, rows, cols] bfloat16 on {self.device}, got {tuple(t.shape)} {t.dtype} on "
@@ -725,8 +725,22 @@ class MoELayer:
         else:
             factor = float(scale)
         # torch leaves the strides of single rows open
-        return L.ADAPTERS.pack(L.ADAPTERS.size, n, rank, factor, cols, n_out, down.data_ptr(), sd, ld if rank > 1 else (cols + 7) // 8 * 8,
-                               up.data_ptr(), su, lu if n_out > 1 else (rank + 7) // 8 * 8, d_scale or 0), n, rank, cols, n_out
+        p_down, p_up = down.data_ptr(), up.data_ptr()
+        ld, lu = ld if rank > 1 else (cols + 7) // 8 * 8, lu if n_out > 1 else (rank + 7) // 8 * 8
+        if (p_down % 16 or ld % 8 or (n > 1 and sd % 8)) and down.is_contiguous():
+            down = self._rows_on_boundaries(down)
+            p_down, (sd, ld, _) = down.data_ptr(), down.stride()
+        if (p_up % 16 or lu % 8 or (n > 1 and su % 8)) and up.is_contiguous():
+            up = self._rows_on_boundaries(up)
+            p_up, (su, lu, _) = up.data_ptr(), up.stride()
+        return L.ADAPTERS.pack(L.ADAPTERS.size, n, rank, factor, cols, n_out, p_down, sd, ld, p_up, su, lu, d_scale or 0), n, rank, cols, n_out, \
+            (down, up)
+
+    def _rows_on_boundaries(self, t: torch.Tensor) -> torch.Tensor:
+        """A copy of [matrices, rows, cols] bf16 whose rows begin on 16-byte boundaries."""
+        n, rows, cols = t.shape
+        ld = (cols + 7) // 8 * 8
+        return torch.empty_strided((n, rows, cols), (rows * ld, ld, 1), dtype=torch.bfloat16, device=self.device).copy_(t.detach())
 
     def _adapter_plan_of(self, who, rows: int, n_adapters: int):
         """ids or a plan -> the two pointers of the call (what the ids lie in is the caller's)."""
@@ -747,12 +761,13 @@ class MoELayer:
                     out: Optional[torch.Tensor] = None, keep: bool = False):
         """out[t] = y[t] + scale[g] * (x[t] . down[g]^T) . up[g]^T, g being row t's adapter; out[t] = y[t] for a row without one.
         x [rows, cols] and y [rows, n_out], down [adapters, rank, cols] and up [adapters, n_out, rank], bf16 with rows on 16-byte
-        boundaries (views will do); rank at most 128, a lower one filled up with zeros.  who: int32 ids [rows], outside [0, adapters)
+        boundaries (views will do; contiguous adapters that lie otherwise are copied to such rows first, by every call); rank at most
+        128, a lower one filled up with zeros.  who: int32 ids [rows], outside [0, adapters)
         for none, or the plan made of them (adapter_plan, adapter_plan_sorted), once for all of a batch's projections.  scale: a number or
         fp32 [adapters].  out may be y, and overlaps nothing otherwise.  With keep also the rows between the two products, in two
         parts of bf16, for adapter_grad: (out, s).  Any layer serves."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
-        ad, n_adapters, rank, a_cols, a_out = self._adapters(down, up, scale)
+        ad, n_adapters, rank, a_cols, a_out, _held = self._adapters(down, up, scale)
         if cols != a_cols:
             raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
         ny, n_out, ldy = self._rows_of(y, torch.bfloat16, "y")
@@ -772,7 +787,7 @@ class MoELayer:
         """Gradients of adapter_add -> (grad_x, grad_down, grad_up), bf16, None for what is not needed; s is what adapter_add kept.
         grad_x is zero in rows without an adapter, the others in adapters without rows.  The gradient of y is grad_out itself."""
         n, cols, ldx = self._rows_of(x, torch.bfloat16, "x")
-        ad, n_adapters, rank, a_cols, a_out = self._adapters(down, up, scale)
+        ad, n_adapters, rank, a_cols, a_out, _held = self._adapters(down, up, scale)
         if cols != a_cols:
             raise ValueError(f"down {tuple(down.shape)} for rows of {cols}")
         ng, n_out, ldg = self._rows_of(grad_out, torch.bfloat16, "grad_out")
