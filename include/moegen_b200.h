@@ -572,7 +572,8 @@ int mg_add_rmsnorm_grad(mg_handle h, const void* d_grad_y, int64_t ldgy, const v
 /* For rows that belong to different requests, or to different experts, each with an adapter of its own beside the weights that
  * all share (mg_int8_linear, mg_expert_ffn, ...).  No counterpart in the reference.  For the rows t of adapter g:
  *   s[t] = x[t] . down[g]^T,   out[t] = y[t] + f[g] * s[t] . up[g]^T,   f[g] = factor * d_scale[g] (d_scale NULL: factor)
- * with fp32 sums, s taken to 16 bits, out rounded once; out[t] = y[t] for rows without an adapter.
+ * with fp32 sums, s taken to 16 bits (as two bf16 numbers: an infinite element of up, or of down on the way back, makes a NaN where its
+ * product with a finite s may be an infinity), out rounded once; out[t] = y[t] for rows without an adapter.
  * down is [n_adapters][rank][cols], up [n_adapters][n_out][rank], bf16, with the rows of either matrix ld_* and the matrices *_stride
  * elements apart.  All rows (x, y, out, gradients, down, up) begin on 16-byte boundaries: strides are multiples of 8.  Adapters of
  * a lower rank are filled up with zeros.  rank <= 128, n_adapters <= MG_ADAPTER_MAX, cols and n_out <= 2^24, rows < 2^28.

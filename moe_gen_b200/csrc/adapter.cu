@@ -1014,7 +1014,7 @@ __global__ void __launch_bounds__(kGradThreads, GradCfg<RP, DEEP>::BLOCKS) adapt
         tc_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + r, v);
         tc_ld8(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + RP + r, rest);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += rest[e];
+        for (int e = 0; e < 8; ++e) v[e] = isfinite(v[e]) ? v[e] + rest[e] : v[e];       // zeros of the second parts times an infinity are NaN
         if (j.steps == 0)
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = 0.f;
