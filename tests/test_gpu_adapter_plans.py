@@ -83,3 +83,24 @@ def test_the_experts_of_a_part_of_the_buffer(layer):
     idx = torch.randint(0, 8, (300, 1), device=DEV, dtype=torch.int32, generator=torch.Generator(device=DEV).manual_seed(1))
     counts, _, pad, _ = layer.permute_plan(torch.cat([idx, (idx + 1) % 8], dim=1))
     _calls(layer, counts[4:].tolist(), pad[4:].tolist(), layer.padded_rows(600), 64, 72, 16)
+
+
+@pytest.mark.parametrize("counts", [[50, 0, 128, 7], [300, 1, 0, 129, 64], [9] * 40])
+def test_either_plan_of_the_same_tiles_gives_the_same_bits(layer, counts):
+    """Segments on 128-row boundaries are cut where the ids' rows are: the tiles' rows, their number and so the blocks that share them are the
+    same, and the sums' order with them."""
+    G, K, N, r = len(counts), 136, 72, 16
+    c = torch.tensor(counts, dtype=torch.int32)
+    pad = torch.zeros(G + 1, dtype=torch.int32)
+    pad[1:] = torch.cumsum((c + 127) // 128 * 128, 0)
+    rows = int(pad[-1]) + 128
+    ids = _ids_of(counts, pad.tolist(), rows)
+    x, y, go = _rows(rows, K, 1), _rows(rows, N, 2), _rows(rows, N, 3)
+    down, up, scale = _adapters(G, r, K, N, 4)
+    got = []
+    for plan in (layer.adapter_plan_sorted(c.to(DEV), pad.to(DEV), rows), layer.adapter_plan(ids, G)):
+        out, s = layer.adapter_add(y, x, down, up, plan, scale, keep=True)
+        got.append((out, s) + layer.adapter_grad(go, x, down, up, plan, scale, s))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    refs = _reference(x, y, down, up, scale, ids, go)
+    assert _near(got[0][0], refs[0]) and all(_near(t, ref) for t, ref in zip(got[0][2:], refs[1:]))
