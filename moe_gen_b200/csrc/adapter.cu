@@ -381,10 +381,10 @@ __global__ void __launch_bounds__(kAdapterThreads, RP <= 32 ? 2 : 1) adapter_dir
 // the first product's, then finish s and the outputs, while four others copy the second product's; one has the products done, into tensor
 // memory.  s passes through shared memory in two parts of bf16.  A cluster of up to eight blocks shares a tile where there are few: each sums
 // s over its columns of x, then over the blocks for its share of the rows, and hands that to all.
-// 8192 rows of 4096 to 4096 columns, rank 64, 8 adapters: 54 us for 210 MB, 3.9 TB/s; 49152 rows of 64 adapters in a buffer of 57344, 2048 to
+// 8192 rows of 4096 to 4096 columns, rank 64, 8 adapters: 55 us for 210 MB, 3.8 TB/s; 49152 rows of 64 adapters in a buffer of 57344, 2048 to
 // 2048, rank 16: 145 us for 670 MB, 4.6 TB/s, the way back 110 us for 440 MB.  Within a turn of all places it streams at what memory gives (296
 // tiles of 2048 to 2048: 90 us, 5.2 TB/s, 1184 tiles 5.7); what bounds it is the turn that is not full, and where clusters share tiles their
-// meeting, 9 of the 54 us, in which all blocks pause at once.  By MMAs of warps on tiles of 16 rows the first took 88 us.
+// meeting, 9 of the 55 us, in which all blocks pause at once.  By MMAs of warps on tiles of 16 rows the first took 88 us.
 constexpr int kFinishWarps = 8, kCopyWarps = 4, kTileThreads = 32 * (kFinishWarps + kCopyWarps + 1);
 template <int RP>
 struct TileCfg {
@@ -1285,14 +1285,19 @@ int launch_tiles_as(const Handle* h, AdapterArgs a, cudaStream_t st) {
   static bool done[64];
   if (int rc = allow_smem(h, adapter_tile_kernel<RP, BACK>, C::SMEM, done)) return rc;
   // As many blocks to a tile as run at once, were all rows in full tiles; how many tiles there are in earnest the device knows.  K = N = 4096, 8
-  // adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16 92, 50, 29, 18; 4096 rows 93, 52, 34, 36; 8192 rows rank 64 107, 65, 55, 68; 16384
-  // rows rank 16 101, 83, 90, 98; 32768 rows 151, 161, 164, 179.  Rows in not much more than a tile to an adapter, as those of expert-sorted
-  // buffers of few tokens, are in clusters of four at any number, since most of their tiles may be without an adapter: 20864 rows for 160
-  // adapters, 300 of them with one, 5120 to 5120, add 98 and grad x 64, without clusters 129 and 104.  Elsewhere clusters of four cost: they leave
-  // places of a GPC empty, and 296 full tiles take 124 where single blocks take 90.
+  // adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16 90, 50, 28, 18; 4096 rows 92, 51, 39, 41; 8192 rows rank 64 107, 65, 55, 73; 16384
+  // rows rank 16 99, 83, 84, 91; 32768 rows 159, 160, 162, 171.  Elsewhere clusters of four cost: they leave places of a GPC empty, and 296 full
+  // tiles of 2048 to 2048 take 123 where single blocks take 90.
+  // Long rows in not much more than a tile to an adapter, as those of expert-sorted buffers of few tokens, are in clusters of four at any
+  // number all the same, since most of their tiles may be without an adapter.  add and grad x, us, in clusters and without (tiles, of
+  // which with an adapter; rank 16 where none is named): 5120 to 5120, 163, 120: 102, 76 and 145, 107; 200, 160: 143, 114 and 152, 112; 161, 40,
+  // rank 128: 112, 84 and 150, 119; 7168 to 7168, 257, 16: 201, 104 and 269, 160; 4096 to 4096, 102, 30, rank 64: 56, 44 and 75, 57; 116, 100: 67, 55
+  // and 67, 53.  Of shorter rows a tile is too little work to share: 2048 to 2048, 261, 64: 95, 60 and 72, 50; 296, 256: 89, 69 and 77, 54; 301, 40,
+  // rank 128: 119, 75 and 70, 57.
   const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile, places = C::BLOCKS * h->sm_count;
+  const bool sparse = 4 * full <= 5 * a.n_adapters && (a.K >= 4096 || a.N >= 4096);
   int P = 8;
-  while (P > 1 && full * P > places && !(P == 4 && 4 * full <= 5 * a.n_adapters)) P /= 2;
+  while (P > 1 && full * P > places && !(P == 4 && sparse)) P /= 2;
   a.slots = static_cast<int>(places / P * P);
   const int64_t all = a.n_tiles + full, most = a.n_tiles + full * P + (P > 1 ? a.slots : 0);      // blocks, P to a tile and one to those of adapters
   // two clusters more: one for what is left of a round, one for rows without an adapter that begin a tile at both ends of the buffer

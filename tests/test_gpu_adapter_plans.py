@@ -42,7 +42,7 @@ def _calls(layer, counts, pad, rows, K, N, r):
     down, up, scale = _adapters(G, r, K, N, 4)
     refs = _reference(x, y, down, up, scale, ids, go)
     plan = layer.adapter_plan_sorted(torch.tensor(counts, dtype=torch.int32, device=DEV), torch.tensor(pad, dtype=torch.int32, device=DEV), rows)
-    out, gx = (torch.full_like(t, float("nan")) for t in (y, x))
+    out, gx = (_rows(*t.shape, 9).fill_(float("nan")) for t in (y, x))
     n = C.c_int32()
     L.check(layer.lib.mg_adapter_rank_stride(r, C.byref(n)))
     s, gs = (torch.full((rows, n.value), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
@@ -104,3 +104,14 @@ def test_either_plan_of_the_same_tiles_gives_the_same_bits(layer, counts):
     assert all(torch.equal(a, b) for a, b in zip(*got))
     refs = _reference(x, y, down, up, scale, ids, go)
     assert _near(got[0][0], refs[0]) and all(_near(t, ref) for t, ref in zip(got[0][2:], refs[1:]))
+
+
+@pytest.mark.parametrize("counts,extra", [([1] * 100 + [0] * 60, 128), ([3] * 300, 128), ([2] * 160, 40 * 128), ([0] * 300, 128), ([0, 3, 0] * 100, 0), ([9] * 75, 5),
+                                          ([0] * 90 + [128] * 70, 128)])
+@pytest.mark.parametrize("K,N,r", [(64, 4104, 16), (4100, 72, 13), (72, 4096, 100)])
+def test_clusters_that_share_the_tiles_of_long_rows(layer, counts, extra, K, N, r):
+    """More tiles than run at once, most of them without an adapter or of few rows, by rows of 4096 columns and more in either direction."""
+    pad = [0]
+    for n in counts:
+        pad.append(pad[-1] + (max(n, 1) + 127) // 128 * 128)
+    _calls(layer, counts, pad, pad[-1] + extra, K, N, r)
