@@ -156,10 +156,12 @@ struct AdapterArgs {
 
 // ---- few rows, without a plan ------------------------------------------------------------------
 // Tiles of sixteen rows, which the kernel finds by itself: what counts is the latency and the adapters' bytes.  In us, here and by a plan
-// that is made already (making it takes 2 to 5 more), K = N = 4096, rank 16: 1 row 6.0 and 16.1, 32 rows with 64 adapters 7.8 and 19.4,
-// 128 rows 14.4 and 35.6, 256 rows 14.9 and 37.4, with 8 adapters 12.5 and 17.3; rank 64, 64 adapters 35.3 and 50.3; rank 128, 8 adapters
-// 27.9 and 22.0.  Beyond 256 rows there is no thread to a row for the search, and the plan's larger tiles read the adapters less often.
-// 201 rows of 64 adapters, 5120 to 1000 columns, rank 12: 11.5 us for 12 MB; bound by two chains of copy, wait and product with a meeting
+// that is made already (making it takes 4 to 5 more), K = N = 4096, rank 16: 1 row 5.8 and 15.7, 32 rows with 64 adapters 7.7 and 19.3,
+// 128 rows 15.1 and 29.7, 256 rows 13.9 and 31.2, with 8 adapters 12.5 and 16.6; rank 64, 64 adapters 37.8 and 40.0, 8 adapters 19.5 and 19.9;
+// rank 128, 64 adapters 52 and 104, 8 adapters 27.4 and 23.2, 128 rows 23.8 and 23.0, 2048 columns 20.0 and 17.6: level with a plan and its
+// making, ahead of them elsewhere.  Beyond 256 rows there is no thread to a row for the search, and the plan's larger tiles read the
+// adapters less often.
+// 201 rows of 64 adapters, 5120 to 1000 columns, rank 12: 11.4 us for 12 MB; bound by two chains of copy, wait and product with a meeting
 // of the cluster between them.
 // Operands go through a ring
 // that every thread fills for itself, in the layout of its MMA fragments: the inner index of a product may be permuted at will, so a
@@ -811,7 +813,8 @@ __global__ void __launch_bounds__(kTileThreads, TileCfg<RP>::BLOCKS) adapter_til
 // fixed order.  The inner index is the rows', so both operands are read as they lie.  The narrow rows' two parts are columns side by side,
 // whose sums are added at the end.
 // 49152 rows of 64 adapters, 2048 and 2048 columns, rank 16: 77 us for 410 MB, 5.3 TB/s; a job's end, its last product and its sums on their
-// way out, is what the SM's other blocks do not quite cover.  Rank 128: 139 us, the narrow rows, twice the wide ones' bytes, from L2.
+// way out, is what the SM's other blocks do not quite cover.  Rank 128: 139 us, the narrow rows, twice the wide ones' bytes, from L2.  A job is
+// one block's, or one cluster's by the mean number of rows: all 49152 rows on one of 64 adapters take 530 us, loads of 1 / n 148.
 struct AdapterGradArgs {
   const uint16_t* wide[2];
   int64_t ldw[2];
