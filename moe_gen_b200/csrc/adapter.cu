@@ -1291,16 +1291,17 @@ int launch_tiles_as(const Handle* h, AdapterArgs a, cudaStream_t st) {
   // adapters, us with 1, 2, 4, 8 blocks: 1024 rows rank 16 90, 50, 28, 18; 4096 rows 92, 51, 39, 41; 8192 rows rank 64 107, 65, 55, 73; 16384
   // rows rank 16 99, 83, 84, 91; 32768 rows 159, 160, 162, 171.  Elsewhere clusters of four cost: they leave places of a GPC empty, and 296 full
   // tiles of 2048 to 2048 take 123 where single blocks take 90.
-  // Long rows in not much more than a tile to an adapter, as those of expert-sorted buffers of few tokens, are in clusters of four at any
-  // number all the same, since most of their tiles may be without an adapter.  add and grad x, us, in clusters and without (tiles, of
-  // which with an adapter; rank 16 where none is named): 5120 to 5120, 163, 120: 102, 76 and 145, 107; 200, 160: 143, 114 and 152, 112; 161, 40,
-  // rank 128: 112, 84 and 150, 119; 7168 to 7168, 257, 16: 201, 104 and 269, 160; 4096 to 4096, 102, 30, rank 64: 56, 44 and 75, 57; 116, 100: 67, 55
-  // and 67, 53.  Of shorter rows a tile is too little work to share: 2048 to 2048, 261, 64: 95, 60 and 72, 50; 296, 256: 89, 69 and 77, 54; 301, 40,
-  // rank 128: 119, 75 and 70, 57.
+  // Rows in not much more than a tile to an adapter, as those of expert-sorted buffers of few tokens, are shared at any number of tiles, since
+  // most of them may be without an adapter: by four blocks, or by two where there are many tiles for the length of their rows.  add and
+  // grad x, us, by 1, 2 and 4 (tiles, of which with an adapter; K = N):
+  //   2048, rank 16:  81, 8: 45 36, 32 25, 32 18    161, 16: 64 43, 43 31, 60 34    258, 25: 74 50, 65 41, 94 58    296, 256: 76 54, 78 59, 89 69
+  //   2048, rank 128: 81, 8: 58 45, 39 30, 33 21    161, 16: 68 52, 45 35, 67 43    258, 25: 69 57, 69 47, 104 68
+  //   4096, rank 16:  101, 10: 89 72, 67 47, 52 34  165, 80: 120 83, 92 59, 79 63   185, 160: 124 91, 111 90, 114 91   258, 25: 154 95, 118 64, 125 77
+  //   7168, rank 16, by 2 and 4: 101, 10: 110 78, 90 55   161, 16: 149 94, 130 70   264, 128: 213 126, 219 138   347, 300: 330 233, 389 283
   const int64_t full = (static_cast<int64_t>(a.n_rows) + kAdapterTile - 1) / kAdapterTile, places = C::BLOCKS * h->sm_count;
-  const bool sparse = 4 * full <= 5 * a.n_adapters && (a.K >= 4096 || a.N >= 4096);
+  const int least = 4 * full > 5 * a.n_adapters ? 1 : 20 * full > (a.K > a.N ? a.K : a.N) ? 2 : 4;
   int P = 8;
-  while (P > 1 && full * P > places && !(P == 4 && sparse)) P /= 2;
+  while (P > least && full * P > places) P /= 2;
   a.slots = static_cast<int>(places / P * P);
   const int64_t all = a.n_tiles + full, most = a.n_tiles + full * P + (P > 1 ? a.slots : 0);      // blocks, P to a tile and one to those of adapters
   // two clusters more: one for what is left of a round, one for rows without an adapter that begin a tile at both ends of the buffer

@@ -107,10 +107,11 @@ def test_either_plan_of_the_same_tiles_gives_the_same_bits(layer, counts):
 
 
 @pytest.mark.parametrize("counts,extra", [([1] * 100 + [0] * 60, 128), ([3] * 300, 128), ([2] * 160, 40 * 128), ([0] * 300, 128), ([0, 3, 0] * 100, 0), ([9] * 75, 5),
-                                          ([0] * 90 + [128] * 70, 128)])
+                                          ([0] * 90 + [128] * 70, 128), ([1] * 200, 40 * 128)])
 @pytest.mark.parametrize("K,N,r", [(64, 4104, 16), (4100, 72, 13), (72, 4096, 100)])
 def test_clusters_that_share_the_tiles_of_long_rows(layer, counts, extra, K, N, r):
-    """More tiles than run at once, most of them without an adapter or of few rows, by rows of 4096 columns and more in either direction."""
+    """More tiles than run at once, most of them without an adapter or of few rows, by rows of 4096 columns and more in either direction: up to
+    204 tiles of 4096 columns are shared by four blocks, more by two."""
     pad = [0]
     for n in counts:
         pad.append(pad[-1] + (max(n, 1) + 127) // 128 * 128)
